@@ -44,6 +44,7 @@ extern "C" {
 #define MVR_F32 0
 #define MVR_F16 1
 #define MVR_F64 2
+#define MVR_BF16 3                       /* the head operators at the end only */
 
 #define MVR_ROI_BOX 0
 #define MVR_ROI_ROTATED 1
@@ -62,6 +63,12 @@ extern "C" {
 #define MVR_ERR_SCRATCH_LIMIT (-11)
 #define MVR_ERR_SCRATCH_ADDRESS (-12)
 #define MVR_ERR_UNSUPPORTED (-13)     /* the entry point has no kernel for this shape: use the general one */
+
+#define MVR_ERR_WORKSPACE (-14)       /* the workspace is missing or smaller than the call needs */
+#define MVR_ERR_HEADS (-15)
+#define MVR_ERR_HEAD_SIZE (-16)
+#define MVR_ERR_PROBABILITY (-17)
+#define MVR_ERR_TOP (-18)
 
 /* element types of label volumes (mvr_affine_label_*) */
 #define MVR_LABEL_U8 0
@@ -291,6 +298,78 @@ int mvr_apply_offset_3d(const void* img, const void* offset, void* out, int dtyp
 int mvr_elastic(const float* coarse, int ndim, int gd, int gh, int gw, int border, const void* image, int dtype,
                 void* image_out, int64_t C_image, const void* labels, int label_dtype, int32_t* label_out, int64_t C_label,
                 float* field, int64_t B, int64_t D, int64_t H, int64_t W, void* stream);
+
+/* ---- operators of a head behind the roi modules ---------------------------------------- */
+/* Element types MVR_F32, MVR_F16 and MVR_BF16; sums, statistics and weights in float, one rounding of
+ * each result.  They have no counterpart in the reference.  Nothing is allocated; a workspace, where a
+ * call needs one, is the caller's, and belongs to that call until its kernels have run: calls that may
+ * overlap (two streams, two captured graphs) need one each.  Results do not depend on the order in
+ * which CTAs run. */
+
+/* Attention of queries to an encoder's states of another length:
+ *   out[r, t, h] = sum_l softmax_l(scale * q[r, t, h] . k[n, l, h / G]) v[n, l, h / G],  G = Hq / Hk,
+ * over the states l < lengths[n] of image n = index[r] with mask[n, l] != 0.  A query whose image has no
+ * such state, or lies outside [0, N) (bit MVR_STATUS_BAD_BATCH_INDEX is OR-ed into *status by the
+ * forward), gives zeros and takes no part in any gradient.  States that are left out are not computed
+ * with: they may hold anything.  Head sizes up to 256. */
+#define MVR_INDEX_F32 0
+#define MVR_INDEX_F16 1
+#define MVR_INDEX_F64 2
+#define MVR_INDEX_BF16 3
+#define MVR_INDEX_I32 4
+#define MVR_INDEX_I64 5
+#define MVR_INDEX_I16 6
+#define MVR_INDEX_U8 7
+typedef struct mvr_attention {
+  int dtype;
+  int has_index;              /* 0: region r reads image r (R must be N) */
+  int64_t R, T, Hq, Hk, N, L, D;
+  const void *q, *k, *v;      /* (R, T, Hq, D), (N, L, Hk, D) twice; the last dimension is contiguous */
+  int64_t q_strides[3], k_strides[3], v_strides[3]; /* elements, of the first three dimensions */
+  const void* index;          /* (R) of index_type, index_stride elements apart; floating ones are cut towards 0 */
+  int index_type;
+  int lengths_64;             /* lengths are int64 (else int32) */
+  int64_t index_stride;
+  const void* lengths;        /* (N) or null: all L; values are limited to [0, L] */
+  const unsigned char* mask;  /* (N, L) contiguous, or null */
+  float scale;
+  void* out;                  /* (R, T, Hq, D) contiguous; read by the backward */
+  float* lse;                 /* (R, T, Hq): written by the forward (null: not wanted), read by the backward */
+  const void* grad_out;       /* backward only, from here on */
+  int64_t g_strides[3];
+  void *grad_q, *grad_k, *grad_v; /* contiguous, written whole */
+} mvr_attention;
+/* Bytes of workspace of a call of these sizes (pointers are not looked at). */
+int mvr_attention_workspace(const mvr_attention* a, int backward, int64_t* bytes);
+int mvr_attention_forward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream);
+int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, void* stream);
+
+/* out[e] = residual[e] + (kept(e) ? x[e] / (1 - p) : 0), residual may be null (0).  kept(e) depends on
+ * (seed, offset, e) alone: element e takes 16 bits, halves of 32-bit words in order and the low half
+ * first, of Philox 4x32-10 with key `seed` and counter (e / 8, offset), both 64-bit words low first, and
+ * is kept when they are at least round(65536 probability); p is that number / 65536.  The gradient of x
+ * is the same call on the gradient of out without a residual.  seed_at, if not null, is a device address
+ * of the seed.  out may be x or residual. */
+int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64_t n, double probability, uint64_t seed,
+                const uint64_t* seed_at, uint64_t offset, void* stream);
+
+/* Of class scores (batch, classes, space), the element (b, c, s) at b * batch_stride + c * class_stride + s,
+ * per position (b, s):
+ *   log_prob = x[label] - lse, 0 where the label is not in [0, classes);  lse = log sum_c exp x[c]
+ *   entropy = lse - sum_c p[c] x[c];  the `top` largest x[c] - lse with their classes, (batch, top, space),
+ *   ties to the lowest class, NaN before everything.
+ * All float32, labels of label_dtype contiguous (batch, space), lse may be null.  Scores of -inf are classes
+ * of probability 0; where all are, log_prob is -inf, entropy 0 and the gradient 0. */
+#define MVR_MAX_TOP 16
+int mvr_label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
+                                float* lse, float* top_log_prob, int32_t* top_label, int64_t batch, int64_t classes, int64_t space,
+                                int64_t batch_stride, int64_t class_stride, int top, void* stream);
+/* grad_logits = grad_log_prob * d log_prob + grad_entropy * d entropy (either may be null: 0), from the
+ * forward's lse and entropy; written whole. */
+int mvr_label_log_probs_backward(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
+                                 const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                                 int64_t batch, int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride,
+                                 int64_t grad_batch_stride, int64_t grad_class_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -9,7 +9,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmvr.so")
 
-MVR_F32, MVR_F16, MVR_F64 = 0, 1, 2
+MVR_F32, MVR_F16, MVR_F64, MVR_BF16 = 0, 1, 2, 3
 MVR_ROI_BOX, MVR_ROI_ROTATED = 0, 1
 MVR_ERR_ROI_WIDTH = -7
 MVR_ERR_UNSUPPORTED = -13
@@ -17,6 +17,19 @@ MVR_STATUS_BAD_BATCH_INDEX = 1
 MVR_STATUS_TMA_TIMEOUT = 2
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
+_u64, _f64 = ctypes.c_uint64, ctypes.c_double
+
+
+class Attention(ctypes.Structure):
+    """struct mvr_attention of include/mvr.h."""
+    _fields_ = [("dtype", _i32), ("has_index", _i32)] + [(n, _i64) for n in ("R", "T", "Hq", "Hk", "N", "L", "D")] + \
+        [("q", _vp), ("k", _vp), ("v", _vp), ("q_strides", _i64 * 3), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3),
+         ("index", _vp), ("index_type", _i32), ("lengths_64", _i32), ("index_stride", _i64), ("lengths", _vp), ("mask", _vp),
+         ("scale", _f32), ("out", _vp), ("lse", _vp), ("grad_out", _vp), ("g_strides", _i64 * 3), ("grad_q", _vp),
+         ("grad_k", _vp), ("grad_v", _vp)]
+
+
+_attention = ctypes.POINTER(Attention)
 
 # name -> argtypes, exactly the prototypes of include/mvr.h
 _GENERAL = [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
@@ -52,6 +65,13 @@ PROTOTYPES = {
                              _f32, _i32, _i32, _vp, _vp],
     "mvr_elastic": [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _i64, _i64,
                     _i64, _vp],
+    "mvr_attention_workspace": [_attention, _i32, ctypes.POINTER(_i64)],
+    "mvr_attention_forward": [_attention, _vp, _i64, _vp, _vp],
+    "mvr_attention_backward": [_attention, _vp, _i64, _vp],
+    "mvr_dropout": [_vp, _vp, _vp, _i32, _i64, _f64, _u64, _vp, _u64, _vp],
+    "mvr_label_log_probs_forward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
+    "mvr_label_log_probs_backward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                     _vp],
     "mvr_affine_2d": _ROT2D,
     "mvr_affine_3d": _ROT3D,
 }

@@ -11,14 +11,17 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmvr.so")
 NATIVE = os.path.join(HERE, "_native.so")
-SOURCES = ["mvr_api.cu"]
+SOURCES = ["mvr_api.cu", "mvr_heads.cu"]  # one object file each
 HEADERS = ["mvr_arith.cuh", "mvr_geom.cuh", "mvr_generic.cuh", "mvr_stream3d.cuh", "mvr_tma3d.cuh", "mvr_brick3d.cuh", "mvr_bwd3d.cuh", "mvr_offset.cuh", "mvr_cubic3d.cuh", "mvr_flat.cuh", "mvr_label.cuh", "mvr_plane2d.cuh", "mvr_elastic.cuh", "mvr_head.cuh",
            os.path.join("..", "..", "include", "mvr.h")]
-NATIVE_SOURCES = ["mvr_torch.cpp"]
-NATIVE_HEADERS = [os.path.join("..", "..", "include", "mvr.h")]
+HEAD_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_dropout.cuh", "mvr_logprob.cuh",
+                os.path.join("..", "..", "include", "mvr.h")]
+HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": HEAD_HEADERS}
+NATIVE_SOURCES = ["mvr_torch.cpp", "mvr_torch_heads.cpp"]
+NATIVE_HEADERS = ["mvr_torch.h", os.path.join("..", "..", "include", "mvr.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-shared"]
+              "-Xcompiler", "-fPIC"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-w"]
 
 
@@ -30,7 +33,7 @@ def _older(target, files):
 
 
 def needs_build():
-    return _older(LIB, SOURCES + HEADERS) or _older(NATIVE, NATIVE_SOURCES + NATIVE_HEADERS)
+    return _older(LIB, SOURCES + HEADERS + HEAD_HEADERS) or _older(NATIVE, NATIVE_SOURCES + NATIVE_HEADERS)
 
 
 def _build_native():
@@ -53,11 +56,19 @@ def _build_native():
 
 def build(force=False, verbose=False):
     """nvcc cross-compiles without a GPU; both .so stay beside the package."""
-    if force or _older(LIB, SOURCES + HEADERS):
+    if force or _older(LIB, SOURCES + HEADERS + HEAD_HEADERS):
         nvcc = os.environ.get("NVCC", "nvcc")
-        cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + \
-              ["-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES]
-        subprocess.check_call(cmd)
+        objects, running = [], []
+        for source in SOURCES:
+            objects.append(os.path.join(CSRC, os.path.splitext(source)[0] + ".o"))
+            if force or _older(objects[-1], [source] + HEADERS_OF[source]):
+                cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + \
+                      ["-c", "-o", objects[-1], os.path.join(CSRC, source)]
+                running.append((cmd, subprocess.Popen(cmd)))
+        for cmd, process in running:
+            if process.wait() != 0:
+                raise subprocess.CalledProcessError(process.returncode, cmd)
+        subprocess.check_call([nvcc] + NVCC_FLAGS + ["-shared", "-o", LIB] + objects)
     if force or _older(NATIVE, NATIVE_SOURCES + NATIVE_HEADERS):
         _build_native()
     return LIB

@@ -181,6 +181,11 @@ const char* mvr_strerror(int code) {
              "(4194304 elements): use mvr_roi_resample_bwd, or split the batch";
     case MVR_ERR_SCRATCH_ADDRESS: return "the device address of the built-in scratch could not be obtained";
     case MVR_ERR_UNSUPPORTED: return "this entry point has no kernel for the given shape";
+    case MVR_ERR_WORKSPACE: return "the workspace is missing or too small";
+    case MVR_ERR_HEADS: return "the number of query heads must be a multiple of the number of key heads";
+    case MVR_ERR_HEAD_SIZE: return "head sizes up to 256 are supported";
+    case MVR_ERR_PROBABILITY: return "the dropout probability must be between 0 and 1";
+    case MVR_ERR_TOP: return "the number of alternatives must be between 0 and 16, and at most the number of classes";
     default: return "unknown error";
   }
 }

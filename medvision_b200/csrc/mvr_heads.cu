@@ -1,0 +1,307 @@
+// C ABI of the operators behind the roi modules (declared in include/mvr.h): attention to an encoder's states, dropout,
+// log-probabilities of labels.  Argument checks, kernel selection and launches; no torch types, device pointers and sizes only.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mvr.h"
+#include "mvr_attn_fma.cuh"
+#include "mvr_dropout.cuh"
+#include "mvr_logprob.cuh"
+
+namespace {
+
+using namespace mvr;
+
+bool head_dtype(int t) { return t == MVR_F32 || t == MVR_F16 || t == MVR_BF16; }
+
+int launched() { return cudaGetLastError() == cudaSuccess ? MVR_OK : MVR_ERR_LAUNCH; }
+
+// ---- attention ----------------------------------------------------------------------------------------
+
+constexpr int kMultiprocessors = 148;
+constexpr size_t kPlanShared = 200 * 1024;
+
+// How a call is cut into CTAs, and what lies where in its workspace.
+struct AttnCut {
+  int tile, kv_tile;            // rows and states of a CTA's tile
+  long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
+  int splits, row_splits;
+  long long order, starts, tiles, delta, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+};
+
+int fma_tile(int D) { return D <= 128 ? 64 : 32; }
+
+long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+
+AttnCut cut_attention(const mvr_attention* a, bool backward) {
+  AttnCut c = {};
+  c.tile = c.kv_tile = fma_tile(a->D);
+  const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
+  c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
+  const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
+  // a call whose tiles do not fill the GPU twice is cut along the axis that its CTAs walk, in parts of two tiles at least
+  const auto parts = [](long long ctas, long long walk) {
+    const long long want = cdiv(2 * kMultiprocessors, std::max<long long>(1, ctas));
+    return (int)std::max<long long>(1, std::min<long long>({want, walk / 2, 64}));
+  };
+  c.splits = parts(c.row_tiles * a->Hk, kv_tiles);
+  const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
+  c.row_splits = backward ? parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile)) : 1;
+  long long at = 0;
+  const auto take = [&at](long long bytes) {
+    const long long here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  if (a->has_index) {
+    c.order = take(a->R * 4);
+    c.starts = take((a->N + 2) * 4);
+    c.tiles = take((a->N + 2) * 4);
+  }
+  if (backward) {
+    c.delta = take(rows * 4);
+    if (c.splits > 1) c.part_gq = take(c.splits * rows * a->D * 4);
+    if (c.row_splits > 1) {
+      c.part_gk = take(c.row_splits * a->N * a->L * a->Hk * a->D * 4);
+      c.part_gv = take(c.row_splits * a->N * a->L * a->Hk * a->D * 4);
+    }
+  } else if (c.splits > 1) {
+    c.part_o = take(c.splits * rows * a->D * 4);
+    c.part_ml = take(c.splits * rows * 8);
+  }
+  c.bytes = at;
+  return c;
+}
+
+int check_attention(const mvr_attention* a, bool backward, bool sizes_only) {
+  if (!a) return MVR_ERR_NULL;
+  if (!head_dtype(a->dtype)) return MVR_ERR_DTYPE;
+  if (a->R < 0 || a->T < 0 || a->Hq < 1 || a->Hk < 1 || a->N < 0 || a->L < 0 || a->D < 1) return MVR_ERR_SHAPE;
+  if (a->Hq % a->Hk != 0) return MVR_ERR_HEADS;
+  if (a->D > 256) return MVR_ERR_HEAD_SIZE;
+  if (!a->has_index && a->R != a->N) return MVR_ERR_SHAPE;
+  const long long most = INT32_MAX / 4;
+  if (a->R > most || a->T > most || a->Hq > 65535 || a->Hk > 65535 || a->N > most || a->L > most) return MVR_ERR_TOO_LARGE;
+  if (a->T > 0 && a->R > 0 && a->R * a->T > most / (a->Hq / a->Hk)) return MVR_ERR_TOO_LARGE;  // rows of a key head: 32 bits
+  if (a->has_index && (size_t)(a->N + 1) * 8 > kPlanShared) return MVR_ERR_TOO_LARGE;
+  if (cdiv(a->L, 32) * a->N > INT32_MAX) return MVR_ERR_TOO_LARGE;
+  if (sizes_only) return MVR_OK;
+  const bool any_rows = a->R > 0 && a->T > 0, any_states = a->N > 0 && a->L > 0;
+  if (a->has_index && (a->index_type < MVR_INDEX_F32 || a->index_type > MVR_INDEX_U8)) return MVR_ERR_DTYPE;
+  if (any_rows && (!a->q || (a->has_index && !a->index))) return MVR_ERR_NULL;
+  if (any_states && (!a->k || !a->v)) return MVR_ERR_NULL;
+  if (any_rows && (!a->out || (backward && (!a->grad_out || !a->grad_q || !a->lse)))) return MVR_ERR_NULL;
+  if (any_states && backward && (!a->grad_k || !a->grad_v)) return MVR_ERR_NULL;
+  return MVR_OK;
+}
+
+AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) {
+  AttnParams p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.g = a->grad_out; p.out = a->out; p.o = a->out;
+  p.gq = a->grad_q; p.gk = a->grad_k; p.gv = a->grad_v; p.lse = a->lse;
+  p.q_r = a->q_strides[0]; p.q_t = a->q_strides[1]; p.q_h = a->q_strides[2];
+  p.k_n = a->k_strides[0]; p.k_l = a->k_strides[1]; p.k_h = a->k_strides[2];
+  p.v_n = a->v_strides[0]; p.v_l = a->v_strides[1]; p.v_h = a->v_strides[2];
+  p.g_r = a->g_strides[0]; p.g_t = a->g_strides[1]; p.g_h = a->g_strides[2];
+  if (a->has_index) {
+    p.order = (const int*)(ws + c.order); p.starts = (const int*)(ws + c.starts); p.tiles = (const int*)(ws + c.tiles);
+  }
+  p.lengths = a->lengths; p.lengths64 = a->lengths_64; p.mask = a->mask;
+  p.R = (int)a->R; p.T = (int)a->T; p.Hq = (int)a->Hq; p.Hk = (int)a->Hk; p.G = (int)(a->Hq / a->Hk);
+  p.N = (int)a->N; p.L = (int)a->L; p.D = (int)a->D;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.splits = c.splits; p.row_splits = c.row_splits;
+  p.delta = (float*)(ws + c.delta);
+  p.part_o = (float*)(ws + c.part_o); p.part_ml = (float*)(ws + c.part_ml);
+  p.part_gq = (float*)(ws + c.part_gq); p.part_gk = (float*)(ws + c.part_gk); p.part_gv = (float*)(ws + c.part_gv);
+  return p;
+}
+
+int plan_attention(const mvr_attention* a, const AttnCut& c, char* ws, int* status, cudaStream_t st) {
+  if (!a->has_index) return MVR_OK;
+  const int groups = (int)a->N + 1;
+  const int warps = (int)std::max<long long>(1, std::min<long long>({32, cdiv(a->R, 32), (long long)(kPlanShared / 4 / groups)}));
+  const size_t smem = (size_t)warps * groups * 4;
+  // (always the same limit: calls of several threads do not undo one another's)
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(attn_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanShared) != cudaSuccess) {
+    cudaGetLastError();
+    return MVR_ERR_LAUNCH;
+  }
+  launch_dependent(attn_plan, dim3(1), dim3(kPlanThreads), smem, st, a->index, a->index_type, (long long)a->index_stride, (int)a->R,
+                   (int)a->N, (int)(a->T * (a->Hq / a->Hk)), c.tile, warps, (int*)(ws + c.order), (int*)(ws + c.starts),
+                   (int*)(ws + c.tiles), status);
+  return launched();
+}
+
+template <typename K>
+int launch_fma(K kernel, dim3 grid, size_t smem, cudaStream_t st, const AttnParams& p) {
+  if (grid.x == 0 || grid.y == 0) return MVR_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return MVR_ERR_LAUNCH;
+  }
+  launch_dependent(kernel, grid, dim3(kFmaThreads), smem, st, p);
+  return launched();
+}
+
+template <typename T, int DP>
+int fma_forward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
+  return launch_fma(attn_fma_fwd<T, DP>, dim3((unsigned)c.row_tiles, p.Hk, c.splits), FmaTile<DP>::bytes(3), st, p);
+}
+template <typename T, int DP>
+int fma_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
+  if (p.R > 0 && p.T > 0) {
+    const int rc = launch_fma(attn_fma_dq<T, DP>, dim3((unsigned)c.row_tiles, p.Hk, c.splits), FmaTile<DP>::bytes(4), st, p);
+    if (rc != MVR_OK) return rc;
+  }
+  return launch_fma(attn_fma_dkv<T, DP>, dim3((unsigned)(cdiv(p.L, c.kv_tile) * p.N), p.Hk, c.row_splits), FmaTile<DP>::bytes(4), st, p);
+}
+
+unsigned blocks_of(long long n, int per) { return (unsigned)std::min<long long>(cdiv(n, per), 1 << 20); }
+
+template <typename T>
+int sum_parts(const float* part, void* dst, long long n, int parts, float factor, cudaStream_t st) {
+  if (n == 0) return MVR_OK;
+  launch_dependent(attn_sum<T>, dim3(blocks_of(n, 256)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
+  return launched();
+}
+
+template <typename T>
+int attention_forward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
+  int rc = p.D <= 32 ? fma_forward<T, 32>(p, c, st) : p.D <= 64 ? fma_forward<T, 64>(p, c, st)
+           : p.D <= 128 ? fma_forward<T, 128>(p, c, st) : fma_forward<T, 256>(p, c, st);
+  if (rc != MVR_OK || c.splits == 1) return rc;
+  launch_dependent(attn_join<T>, dim3((unsigned)cdiv((long long)p.R * p.T * p.Hq, 8)), dim3(256), 0, st, p);
+  return launched();
+}
+
+template <typename T>
+int attention_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
+  const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
+  int rc = MVR_OK;
+  if (rows > 0) {
+    launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, p);
+    if ((rc = launched()) != MVR_OK) return rc;
+  }
+  rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
+       : p.D <= 128 ? fma_backward<T, 128>(p, c, st) : fma_backward<T, 256>(p, c, st);
+  if (rc == MVR_OK && c.splits > 1) rc = sum_parts<T>(p.part_gq, p.gq, rows * p.D, c.splits, p.scale, st);
+  if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gk, p.gk, states, c.row_splits, p.scale, st);
+  if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gv, p.gv, states, c.row_splits, 1.0f, st);
+  return rc;
+}
+
+int attention(const mvr_attention* a, bool backward, void* workspace, int64_t bytes, int* status, void* stream) {
+  int rc = check_attention(a, backward, false);
+  if (rc != MVR_OK) return rc;
+  const AttnCut c = cut_attention(a, backward);
+  if (bytes < c.bytes || (c.bytes > 0 && !workspace)) return MVR_ERR_WORKSPACE;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool any_rows = a->R > 0 && a->T > 0, any_states = a->N > 0 && a->L > 0;
+  if (!any_rows && (!backward || !any_states)) return MVR_OK;
+  if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
+  if ((rc = plan_attention(a, c, (char*)workspace, status, st)) != MVR_OK) return rc;
+  const AttnParams p = attention_params(a, c, (char*)workspace);
+  switch (a->dtype) {
+    case MVR_F32: return backward ? attention_backward<float>(p, c, st) : attention_forward<float>(p, c, st);
+    case MVR_F16: return backward ? attention_backward<__half>(p, c, st) : attention_forward<__half>(p, c, st);
+    default: return backward ? attention_backward<__nv_bfloat16>(p, c, st) : attention_forward<__nv_bfloat16>(p, c, st);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int mvr_attention_workspace(const mvr_attention* a, int backward, int64_t* bytes) {
+  if (!bytes) return MVR_ERR_NULL;
+  const int rc = check_attention(a, backward != 0, true);
+  if (rc != MVR_OK) return rc;
+  *bytes = cut_attention(a, backward != 0).bytes;
+  return MVR_OK;
+}
+
+int mvr_attention_forward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream) {
+  return attention(a, false, workspace, bytes, status, stream);
+}
+
+int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, void* stream) {
+  return attention(a, true, workspace, bytes, nullptr, stream);
+}
+
+int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64_t n, double probability, uint64_t seed,
+                const uint64_t* seed_at, uint64_t offset, void* stream) {
+  if (!head_dtype(dtype)) return MVR_ERR_DTYPE;
+  if (n < 0) return MVR_ERR_SHAPE;
+  if (!(probability >= 0.0 && probability <= 1.0)) return MVR_ERR_PROBABILITY;
+  if (n == 0) return MVR_OK;
+  if (!x || !out) return MVR_ERR_NULL;
+  DropoutParams p = {};
+  p.x = x; p.residual = residual; p.out = out; p.n = n;
+  p.cut = (unsigned)std::floor(probability * 65536.0 + 0.5);
+  p.scale = p.cut < 65536 ? (float)(65536.0 / (65536.0 - p.cut)) : 0.0f;
+  p.seed = seed; p.seed_at = (const unsigned long long*)seed_at; p.offset = offset;
+  const cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case MVR_F32: launch_dropout<float>(p, st); break;
+    case MVR_F16: launch_dropout<__half>(p, st); break;
+    default: launch_dropout<__nv_bfloat16>(p, st); break;
+  }
+  return launched();
+}
+
+static int label_log_probs(const LogProbParams& p, int dtype, bool fwd, void* stream) {
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rc = dtype == MVR_F32 ? launch_logprob<float>(p, fwd, st) : dtype == MVR_F16 ? launch_logprob<__half>(p, fwd, st)
+                                                                                         : launch_logprob<__nv_bfloat16>(p, fwd, st);
+  return rc ? MVR_ERR_TOO_LARGE : launched();
+}
+
+static int check_label_log_probs(int dtype, int label_dtype, int64_t batch, int64_t classes, int64_t space) {
+  if (!head_dtype(dtype)) return MVR_ERR_DTYPE;
+  if (label_dtype < MVR_LABEL_U8 || label_dtype > MVR_LABEL_I64) return MVR_ERR_DTYPE;
+  if (batch < 0 || classes < 1 || space < 0) return MVR_ERR_SHAPE;
+  if (classes > INT32_MAX - 64) return MVR_ERR_TOO_LARGE;
+  if (space > 0 && batch > INT64_MAX / 32 / space) return MVR_ERR_TOO_LARGE;
+  return MVR_OK;
+}
+
+int mvr_label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
+                                float* lse, float* top_log_prob, int32_t* top_label, int64_t batch, int64_t classes, int64_t space,
+                                int64_t batch_stride, int64_t class_stride, int top, void* stream) {
+  const int rc = check_label_log_probs(dtype, label_dtype, batch, classes, space);
+  if (rc != MVR_OK) return rc;
+  if (top < 0 || top > MVR_MAX_TOP || top > classes) return MVR_ERR_TOP;
+  if (batch == 0 || space == 0) return MVR_OK;
+  if (!logits || !labels || !log_prob || !entropy || (top > 0 && (!top_log_prob || !top_label))) return MVR_ERR_NULL;
+  LogProbParams p = {};
+  p.x = logits; p.labels = labels; p.label_type = label_dtype;
+  p.log_prob = log_prob; p.entropy = entropy; p.lse = lse; p.top_value = top_log_prob; p.top_label = top_label;
+  p.batch = batch; p.space = space; p.batch_stride = batch_stride; p.class_stride = class_stride;
+  p.classes = (int)classes; p.top = top;
+  return label_log_probs(p, dtype, true, stream);
+}
+
+int mvr_label_log_probs_backward(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
+                                 const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                                 int64_t batch, int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride,
+                                 int64_t grad_batch_stride, int64_t grad_class_stride, void* stream) {
+  const int rc = check_label_log_probs(dtype, label_dtype, batch, classes, space);
+  if (rc != MVR_OK) return rc;
+  if (batch == 0 || space == 0) return MVR_OK;
+  if (!logits || !labels || !lse || !entropy || !grad_logits) return MVR_ERR_NULL;
+  LogProbParams p = {};
+  p.x = logits; p.labels = labels; p.label_type = label_dtype;
+  p.entropy = const_cast<float*>(entropy); p.lse = const_cast<float*>(lse);
+  p.grad_log_prob = grad_log_prob; p.grad_entropy = grad_entropy; p.grad = grad_logits;
+  p.batch = batch; p.space = space; p.batch_stride = batch_stride; p.class_stride = class_stride;
+  p.grad_batch_stride = grad_batch_stride; p.grad_class_stride = grad_class_stride;
+  p.classes = (int)classes;
+  return label_log_probs(p, dtype, false, stream);
+}
+
+}  // extern "C"

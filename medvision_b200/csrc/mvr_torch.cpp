@@ -26,6 +26,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/mvr.h"
+#include "mvr_torch.h"
 
 namespace {
 
@@ -1167,4 +1168,18 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__native(void) { return PyModule_Create(&module); }
+namespace mvr_host {
+std::string type_name(at::ScalarType t) { return dtype_name(t); }
+int label_type(at::ScalarType t) { return label_code(t); }
+void check(int rc) { check_rc(rc); }
+int* status_of(int index) { return status_ptr(index); }
+}  // namespace mvr_host
+
+PyMODINIT_FUNC PyInit__native(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddFunctions(m, mvr_host::head_methods()) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
