@@ -342,7 +342,7 @@ typedef struct mvr_attention {
 /* Bytes of workspace of a call of these sizes (pointers are not looked at). */
 int mvr_attention_workspace(const mvr_attention* a, int backward, int64_t* bytes);
 int mvr_attention_forward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream);
-int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, void* stream);
+int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream);
 
 /* out[e] = residual[e] + (kept(e) ? x[e] / (1 - p) : 0), residual may be null (0).  kept(e) depends on
  * (seed, offset, e) alone: element e takes 16 bits, halves of 32-bit words in order and the low half

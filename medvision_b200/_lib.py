@@ -67,7 +67,7 @@ PROTOTYPES = {
                     _i64, _vp],
     "mvr_attention_workspace": [_attention, _i32, ctypes.POINTER(_i64)],
     "mvr_attention_forward": [_attention, _vp, _i64, _vp, _vp],
-    "mvr_attention_backward": [_attention, _vp, _i64, _vp],
+    "mvr_attention_backward": [_attention, _vp, _i64, _vp, _vp],
     "mvr_dropout": [_vp, _vp, _vp, _i32, _i64, _f64, _u64, _vp, _u64, _vp],
     "mvr_label_log_probs_forward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "mvr_label_log_probs_backward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,

@@ -1,0 +1,377 @@
+// Attention forward on the tensor cores (float16, bfloat16; head sizes that are multiples of 8, up to 128).
+//
+// A CTA holds TILES tiles of 128 rows of queries and walks the states of their image 128 at a time.  One warp brings tiles of keys
+// and values into a ring in shared memory by TMA, one thread issues the products, and a warpgroup per row tile, one row a thread,
+// keeps the running maximum and sum:
+//
+//   S = Q K^T (128 x 128, tensor memory)  ->  P = 2^(S scale - m), rounded to T, over S  ->  O += P V (tensor memory)
+//
+// The maximum that P is formed about is only moved when it grows by more than 2^8 (P stays far below what T holds, and the sum is
+// formed of the same P): then O, in tensor memory, is scaled first.  With two row tiles one's products run under the other's
+// exponentials.  Few rows: one tile a CTA, two CTAs an SM, and the states cut into parts (attn_join).
+//
+// States that are left out (lengths, mask) are compacted to a list of tiles with 128 bits each before the walk; tiles without a state
+// are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its
+// own before the product reads them.
+#pragma once
+#include "mvr_attn.cuh"
+#include "mvr_tc.cuh"
+
+namespace mvr {
+
+constexpr int kTcRows = 128, kTcStates = 128, kTcMaxTiles = 512;  // tiles of states that one CTA can list
+
+template <int DP, int TILES, bool MASK>
+struct TcForward {
+  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128;       // a tile of rows or states
+  static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 4);
+  static constexpr int kSoftmax = TILES * 128, kThreads = kSoftmax + (MASK ? 96 : 64);
+  static constexpr int kColumns = TILES == 2 ? 512 : 256, kScores = 0, kOut = TILES * 128;
+  struct Control {
+    unsigned long long full[kSlots], empty[kSlots], clean[kSlots];
+    unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES];
+    uint32_t tmem;
+    int lost, tiles;
+    unsigned short list[MASK ? kTcMaxTiles : 1];
+    uint4 bits[MASK ? kTcMaxTiles : 1];
+  };
+  static constexpr size_t kShared = (size_t)(TILES + kSlots) * kTileBytes + sizeof(Control) + 1024;
+};
+
+struct TcMaps {
+  CUtensorMap k, v;
+};
+
+// Bits of the states [first, first + 128) that may be read, of `end` and the mask; the same in all lanes.
+__device__ __forceinline__ uint4 state_bits(const AttnParams& p, int n, int first, int end, int lane) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = first + i * 32 + lane;
+    w[i] = __ballot_sync(~0u, j < end && (!p.mask || p.mask[(long long)n * p.L + j] != 0));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// List of the tiles of 128 states in [begin, end) that have one to read, with their bits.  All threads; the result after a barrier.
+__device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin, int end, unsigned short* list, uint4* bits, int* count) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, tiles = (end - begin + kTcStates - 1) / kTcStates;
+  for (int i = threadIdx.x >> 5; i < tiles; i += warps) {
+    const uint4 b = state_bits(p, n, begin + i * kTcStates, end, lane);
+    if (lane == 0) bits[i] = b;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int at = 0;
+    for (int base = 0; base < tiles; base += 32) {
+      const int i = base + lane;
+      uint4 b = make_uint4(0, 0, 0, 0);
+      if (i < tiles) b = bits[i];
+      const bool any = (b.x | b.y | b.z | b.w) != 0;
+      const uint32_t who = __ballot_sync(~0u, any);
+      __syncwarp();
+      if (any) {  // (at + rank <= i: what is overwritten has been read)
+        const int to = at + __popc(who & ((1u << lane) - 1));
+        list[to] = (unsigned short)i;
+        bits[to] = b;
+      }
+      at += __popc(who);
+      __syncwarp();
+    }
+    if (lane == 0) *count = at;
+  }
+}
+
+// A row of 2-byte elements into a K-major tile in the 128-byte swizzle; zeros behind D, and for no row at all.
+template <int DP>
+__device__ __forceinline__ void put_row(char* tile, int r, const void* src, int D) {
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    const uint4 v = src && c * 8 < D ? ((const uint4*)src)[c] : make_uint4(0, 0, 0, 0);
+    *(uint4*)(tile + (c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+  }
+}
+
+template <typename T, int DP, int TILES, bool MASK>
+__global__ void __launch_bounds__(TcForward<DP, TILES, MASK>::kThreads, TILES == 2 ? 1 : 2)
+attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
+  typedef TcForward<DP, TILES, MASK> F;
+  extern __shared__ char tc_smem[];
+  char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);
+  char* ring = base + TILES * F::kTileBytes;
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kTileBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLoader = F::kSoftmax / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kSlots; ++i) {
+      bar_init(smem_at(&c.full[i]), 1);
+      bar_init(smem_at(&c.empty[i]), 1);
+      bar_init(smem_at(&c.clean[i]), 1);
+    }
+    for (int t = 0; t < TILES; ++t) {
+      bar_init(smem_at(&c.queries[t]), 128);
+      bar_init(smem_at(&c.scores[t]), 1);
+      bar_init(smem_at(&c.weights[t]), 128);
+      bar_init(smem_at(&c.out[t]), 1);
+    }
+    c.lost = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // Tensor memory is taken only when the kernel before has ended, and the next kernel may come only when it has been taken: no CTA
+  // holds it while it waits for another that still needs some.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
+  RowTile o;
+  const bool some = row_tile(p, blockIdx.x, TILES * kTcRows, o);
+  const int hk = blockIdx.y, split = blockIdx.z;
+  const int all = (p.L + kTcStates - 1) / kTcStates, per = (all + p.splits - 1) / p.splits;
+  const int begin = split * per * kTcStates;
+  int end = 0;
+  if (some) end = min(states_of(p, o.n), (split + 1) * per * kTcStates);
+  if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + kTcStates - 1) / kTcStates;
+  const int used = !some ? 0 : TILES == 2 && o.first + kTcRows < o.rows ? 2 : 1;  // row tiles that have rows
+  const uint32_t tmem = c.tmem;
+  volatile int* lost = &c.lost;
+  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
+
+  if (warp == kLoader) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
+        const int slot = i % F::kSlots;
+        const uint32_t bar = smem_at(&c.full[slot]);
+        if (i >= F::kSlots && !bar_wait(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+        bar_expect(bar, F::kTileBytes);
+        const int j = first_of(i >> 1);
+        for (int b = 0; b < F::kBlocks; ++b)
+          tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * kTcRows * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
+      }
+      // given up: the copies under way end before the CTA does
+      if (*lost)
+        for (int k = max(0, i - F::kSlots); k < i; ++k) {
+          const unsigned long long t = nanoseconds();
+          while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
+        }
+    }
+  } else if (warp == kIssuer) {
+    if (lane == 0 && tiles > 0) {
+      const int depth = (p.D + 15) / 16;
+      const uint32_t s_shape = tc_shape<T>(kTcStates, false, p.scale < 0.0f), o_shape = tc_shape<T>(depth * 16, true);
+      const auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
+        const uint32_t a = smem_at(base + t * F::kTileBytes), b = smem_at(ring + slot * F::kTileBytes);
+        for (int k = 0; k < depth; ++k) {
+          const uint32_t off = (k >> 2) * (kTcRows * 128) + (k & 3) * 32;
+          mma_ss(tmem + F::kScores + t * 128, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+        }
+        mma_commit(smem_at(&c.scores[t]));
+      };
+      bool ok = true;
+      for (int t = 0; t < used && ok; ++t) ok = bar_wait(smem_at(&c.queries[t]), 0, lost);
+      ok = ok && bar_wait(smem_at(&c.full[0]), 0, lost);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < used; ++t) scores(t, 0);
+        mma_commit(smem_at(&c.empty[0]));
+      }
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int v = 2 * j + 1, k = v + 1, vs = v % F::kSlots, ks = k % F::kSlots;
+        ok = bar_wait(smem_at(&c.full[vs]), (v / F::kSlots) & 1, lost);
+        if (MASK && ok) ok = bar_wait(smem_at(&c.clean[vs]), (v / F::kSlots) & 1, lost);
+        for (int t = 0; t < used && ok; ++t) {
+          ok = bar_wait(smem_at(&c.weights[t]), j & 1, lost);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = smem_at(ring + vs * F::kTileBytes);
+          for (int i = 0; i < kTcStates / 16; ++i)  // O_t += P_t V
+            mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * 128 + i * 8, desc_mn_major(b + i * 2048, kTcRows * 128), o_shape,
+                   j > 0 || i > 0);
+          if (j + 1 < tiles) {
+            if (t == 0) ok = bar_wait(smem_at(&c.full[ks]), (k / F::kSlots) & 1, lost);
+            if (ok) {
+              tc_fence_after();
+              scores(t, ks);
+            }
+          }
+        }
+        mma_commit(smem_at(&c.empty[vs]));
+        if (j + 1 < tiles) mma_commit(smem_at(&c.empty[ks]));
+      }
+      for (int t = 0; t < TILES; ++t) mma_commit(smem_at(&c.out[t]));
+    }
+  } else if (MASK && warp == kCleaner) {
+    for (int j = 0; j < tiles; ++j) {
+      const int v = 2 * j + 1, slot = v % F::kSlots;
+      if (!bar_wait(smem_at(&c.full[slot]), (v / F::kSlots) & 1, lost)) break;
+      const uint4 b = c.bits[j];
+      if ((b.x & b.y & b.z & b.w) != ~0u) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t out = ~word_of(b, w);
+          while (out) {
+            const int r = w * 32 + __ffs(out) - 1;
+            out &= out - 1;
+            if (lane < 8 * F::kBlocks)
+              *(uint4*)(ring + slot * F::kTileBytes + (lane >> 3) * (kTcRows * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_proxy();
+        __syncwarp();
+      }
+      if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
+    }
+  } else if (warp < kLoader) {
+    const int t = warp >> 2, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + F::kScores + t * 128, o_at = tmem + lanes + F::kOut + t * DP;
+    if (t < used) {
+      Row w = {};
+      const bool mine = j0 < o.rows;
+      if (mine) w = row_of(p, o, j0, hk);
+      if (tiles > 0) {
+        put_row<DP>(base + t * F::kTileBytes, r, mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr, p.D);
+        fence_async_proxy();
+        bar_arrive(smem_at(&c.queries[t]));
+      }
+      const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
+      float m = -INFINITY, l = 0.0f;  // m: in the units of S
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        uint4 bits = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (MASK) bits = c.bits[j];
+        else if (j + 1 == tiles && (end & 127)) {
+          const int n = end & 127;
+          bits.x = n >= 32 ? ~0u : (1u << n) - 1;
+          bits.y = n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1 : 0;
+          bits.z = n >= 96 ? ~0u : n > 64 ? (1u << (n - 64)) - 1 : 0;
+          bits.w = n > 96 ? (1u << (n - 96)) - 1 : 0;
+        }
+        ok = bar_wait(smem_at(&c.scores[t]), j & 1, lost);
+        if (!__all_sync(~0u, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const auto fetch = [&](float (&s)[32], int q) {
+          uint32_t v[32];
+          tmem_load32(v, s_at + q * 32);
+          tmem_wait_load();
+          const uint32_t b = word_of(bits, q);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
+          if (b != ~0u) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = (b >> i) & 1 ? s[i] : -INFINITY;
+          }
+        };
+        float top = -INFINITY, s[32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          fetch(s, q);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+        }
+        // move the maximum?  (the first tile: there is no O yet)
+        const bool move = top > m && (m == -INFINITY || (top - m) * scale > 8.0f);
+        if (__any_sync(~0u, move)) {
+          const float shrink = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - top) * scale)) : 1.0f;
+          if (move) m = top;
+          l *= shrink;
+          if (j > 0) {
+#pragma unroll 1
+            for (int q = 0; q < DP / 32; ++q) {
+              uint32_t v[32];
+              tmem_load32(v, o_at + q * 32);
+              tmem_wait_load();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * shrink);
+              tmem_store32(o_at + q * 32, v);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m * scale;
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          fetch(s, q);
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = exp2_fast(fmaf(s[2 * i], scale, -ref)), b = exp2_fast(fmaf(s[2 * i + 1], scale, -ref));
+            sum += a + b;
+            v[i] = pack2<T>(a, b);
+          }
+          tmem_store16(s_at + q * 16, v);
+        }
+        l += sum;
+        tmem_wait_store();
+        tc_fence_before();
+        bar_arrive(smem_at(&c.weights[t]));
+      }
+      if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.out[t]), 0, lost);
+      if (__all_sync(~0u, ok)) {
+        tc_fence_after();
+        const long long row = row_number(p, w), rows = (long long)p.R * p.T * p.Hq;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (mine) {
+          if (p.splits > 1) {
+            p.part_ml[(split * rows + row) * 2] = m == -INFINITY ? m : m * scale;
+            p.part_ml[(split * rows + row) * 2 + 1] = l;
+          } else if (p.lse) {
+            p.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? 0.0f : m * scale) + log2f(l);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < DP / 32; ++q) {
+          if (q * 32 >= p.D) break;
+          uint32_t v[32];
+          if (tiles > 0) {
+            tmem_load32(v, o_at + q * 32);
+            tmem_wait_load();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0;
+          }
+          if (mine && p.splits > 1) {
+            float* to = p.part_o + (split * rows + row) * p.D + q * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (q * 32 + i < p.D) *(uint4*)(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          } else if (mine) {
+            T* to = (T*)p.out + row * p.D + q * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (q * 32 + i >= p.D) continue;
+              uint32_t u[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                u[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
+              *(uint4*)(to + i) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    if (*lost) {  // products may still be under way: they end before tensor memory is freed
+      if (lane == 0) {
+        if (status) atomicOr(status, 2);
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.out[0]), 0) && nanoseconds() - t < kWaitLimit) {}
+      }
+      __syncwarp();
+    }
+    tc_fence_after();
+    tmem_free(tmem, F::kColumns);
+  }
+}
+
+}  // namespace mvr

@@ -8,6 +8,7 @@
 
 #include "../../include/mvr.h"
 #include "mvr_attn_fma.cuh"
+#include "mvr_attn_tc.cuh"
 #include "mvr_dropout.cuh"
 #include "mvr_logprob.cuh"
 
@@ -26,30 +27,42 @@ constexpr size_t kPlanShared = 200 * 1024;
 
 // How a call is cut into CTAs, and what lies where in its workspace.
 struct AttnCut {
+  bool tc;                      // tensor cores (mvr_attn_tc.cuh)
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
   long long order, starts, tiles, delta, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
-int fma_tile(int D) { return D <= 128 ? 64 : 32; }
-
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
-AttnCut cut_attention(const mvr_attention* a, bool backward) {
+// Parts in which `ctas` CTAs, each walking `steps` tiles, run for the least time on `slots` places: whole rounds of CTAs, each a
+// part's steps and `fixed` steps' time for its beginning and end; a part more costs `join` steps' time.
+int best_parts(long long ctas, long long steps, long long slots, double fixed, double join) {
+  int best = 1;
+  double least = 0;
+  for (long long s = 1; s <= std::min<long long>(64, std::max<long long>(1, steps)); ++s) {
+    const long long per = cdiv(steps, s);
+    if (s > 1 && cdiv(steps, per) < s) continue;  // a part would have nothing
+    const double rounds = (double)cdiv(ctas * s, slots), time = rounds * (per + fixed) + (s > 1 ? join * s : 0);
+    if (s == 1 || time < 0.97 * least) best = (int)s, least = time;
+  }
+  return best;
+}
+
+AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   AttnCut c = {};
-  c.tile = c.kv_tile = fma_tile(a->D);
+  c.tc = tc;
   const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
+  const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
+  c.tile = tc ? (rows_of_image > kTcRows ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
+  c.kv_tile = tc ? kTcStates : c.tile;
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
-  // a call whose tiles do not fill the GPU twice is cut along the axis that its CTAs walk, in parts of two tiles at least
-  const auto parts = [](long long ctas, long long walk) {
-    const long long want = cdiv(2 * kMultiprocessors, std::max<long long>(1, ctas));
-    return (int)std::max<long long>(1, std::min<long long>({want, walk / 2, 64}));
-  };
-  c.splits = parts(c.row_tiles * a->Hk, kv_tiles);
-  const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
-  c.row_splits = backward ? parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile)) : 1;
+  const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
+  c.splits = best_parts(expected, kv_tiles, tc ? (c.tile > kTcRows ? 1 : 2) * kMultiprocessors : 2 * kMultiprocessors, 3, 0.5);
+  if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(kv_tiles, kTcMaxTiles));
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), 2 * kMultiprocessors, 2, 1) : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
     const long long here = at;
@@ -74,6 +87,18 @@ AttnCut cut_attention(const mvr_attention* a, bool backward) {
   }
   c.bytes = at;
   return c;
+}
+
+// Whether type and head size are the tensor cores'; the operands' alignment is a matter of the call.
+bool tc_sizes(const mvr_attention* a) {
+  return a->dtype != MVR_F32 && a->D % 8 == 0 && a->D <= 128 && a->L > 0 && a->N > 0 && cdiv(a->L, kTcStates) <= 64 * kTcMaxTiles;
+}
+bool rows_aligned(const void* base, const int64_t (&strides)[3], const mvr_attention* a) {
+  const int64_t sizes[3] = {a->R, a->T, a->Hq};
+  if ((uintptr_t)base % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1 && strides[i] % 8 != 0) return false;
+  return true;
 }
 
 int check_attention(const mvr_attention* a, bool backward, bool sizes_only) {
@@ -170,10 +195,43 @@ int sum_parts(const float* part, void* dst, long long n, int parts, float factor
   return launched();
 }
 
+template <typename T, int DP, int TILES, bool MASK>
+int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
+  typedef TcForward<DP, TILES, MASK> F;
+  const auto kernel = attn_tc_fwd<T, DP, TILES, MASK>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::kShared) != cudaSuccess) {
+    cudaGetLastError();
+    return MVR_ERR_LAUNCH;
+  }
+  launch_dependent(kernel, dim3((unsigned)c.row_tiles, p.Hk, c.splits), dim3(F::kThreads), F::kShared, st, p, maps, status);
+  return launched();
+}
+template <typename T, int DP>
+int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
+  const bool mask = p.mask || p.lengths;
+  if (c.tile > kTcRows) return mask ? tc_forward_as<T, DP, 2, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false>(p, c, maps, status, st);
+  return mask ? tc_forward_as<T, DP, 1, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, false>(p, c, maps, status, st);
+}
+
 template <typename T>
-int attention_forward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
-  int rc = p.D <= 32 ? fma_forward<T, 32>(p, c, st) : p.D <= 64 ? fma_forward<T, 64>(p, c, st)
-           : p.D <= 128 ? fma_forward<T, 128>(p, c, st) : fma_forward<T, 256>(p, c, st);
+bool state_maps(const mvr_attention* a, TcMaps& maps, int rows) {
+  const auto map = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
+    return tc_state_map<T>(m, base, (int)a->D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], rows);
+  };
+  return map(&maps.k, a->k, a->k_strides) && map(&maps.v, a->v, a->v_strides);
+}
+
+template <typename T>
+int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
+  int rc;
+  if constexpr (sizeof(T) == 2) {
+    rc = c.tc ? (p.D <= 64 ? tc_forward<T, 64>(p, c, maps, status, st) : tc_forward<T, 128>(p, c, maps, status, st)) : MVR_ERR_UNSUPPORTED;
+  } else {
+    rc = MVR_ERR_UNSUPPORTED;
+  }
+  if (!c.tc)
+    rc = p.D <= 32 ? fma_forward<T, 32>(p, c, st) : p.D <= 64 ? fma_forward<T, 64>(p, c, st)
+         : p.D <= 128 ? fma_forward<T, 128>(p, c, st) : fma_forward<T, 256>(p, c, st);
   if (rc != MVR_OK || c.splits == 1) return rc;
   launch_dependent(attn_join<T>, dim3((unsigned)cdiv((long long)p.R * p.T * p.Hq, 8)), dim3(256), 0, st, p);
   return launched();
@@ -195,21 +253,36 @@ int attention_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
   return rc;
 }
 
-int attention(const mvr_attention* a, bool backward, void* workspace, int64_t bytes, int* status, void* stream) {
-  int rc = check_attention(a, backward, false);
+template <typename T>
+int attention_as(const mvr_attention* a, bool backward, char* workspace, int* status, cudaStream_t st) {
+  TcMaps maps;
+  bool tc = !backward && tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
+  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps, kTcStates);
+  const AttnCut c = cut_attention(a, backward, tc);
+  if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
+  const int rc = plan_attention(a, c, workspace, status, st);
   if (rc != MVR_OK) return rc;
-  const AttnCut c = cut_attention(a, backward);
-  if (bytes < c.bytes || (c.bytes > 0 && !workspace)) return MVR_ERR_WORKSPACE;
-  const cudaStream_t st = (cudaStream_t)stream;
+  const AttnParams p = attention_params(a, c, workspace);
+  return backward ? attention_backward<T>(p, c, st) : attention_forward<T>(p, c, maps, status, st);
+}
+
+long long attention_bytes(const mvr_attention* a, bool backward) {
+  const long long fma = cut_attention(a, backward, false).bytes;
+  return tc_sizes(a) ? std::max(fma, cut_attention(a, backward, true).bytes) : fma;
+}
+
+int attention(const mvr_attention* a, bool backward, void* workspace, int64_t bytes, int* status, void* stream) {
+  const int rc = check_attention(a, backward, false);
+  if (rc != MVR_OK) return rc;
+  const long long need = attention_bytes(a, backward);
+  if (bytes < need || (need > 0 && !workspace)) return MVR_ERR_WORKSPACE;
   const bool any_rows = a->R > 0 && a->T > 0, any_states = a->N > 0 && a->L > 0;
   if (!any_rows && (!backward || !any_states)) return MVR_OK;
-  if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
-  if ((rc = plan_attention(a, c, (char*)workspace, status, st)) != MVR_OK) return rc;
-  const AttnParams p = attention_params(a, c, (char*)workspace);
+  const cudaStream_t st = (cudaStream_t)stream;
   switch (a->dtype) {
-    case MVR_F32: return backward ? attention_backward<float>(p, c, st) : attention_forward<float>(p, c, st);
-    case MVR_F16: return backward ? attention_backward<__half>(p, c, st) : attention_forward<__half>(p, c, st);
-    default: return backward ? attention_backward<__nv_bfloat16>(p, c, st) : attention_forward<__nv_bfloat16>(p, c, st);
+    case MVR_F32: return attention_as<float>(a, backward, (char*)workspace, status, st);
+    case MVR_F16: return attention_as<__half>(a, backward, (char*)workspace, status, st);
+    default: return attention_as<__nv_bfloat16>(a, backward, (char*)workspace, status, st);
   }
 }
 
@@ -221,7 +294,7 @@ int mvr_attention_workspace(const mvr_attention* a, int backward, int64_t* bytes
   if (!bytes) return MVR_ERR_NULL;
   const int rc = check_attention(a, backward != 0, true);
   if (rc != MVR_OK) return rc;
-  *bytes = cut_attention(a, backward != 0).bytes;
+  *bytes = attention_bytes(a, backward != 0);
   return MVR_OK;
 }
 
@@ -229,8 +302,8 @@ int mvr_attention_forward(const mvr_attention* a, void* workspace, int64_t bytes
   return attention(a, false, workspace, bytes, status, stream);
 }
 
-int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, void* stream) {
-  return attention(a, true, workspace, bytes, nullptr, stream);
+int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream) {
+  return attention(a, true, workspace, bytes, status, stream);
 }
 
 int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64_t n, double probability, uint64_t seed,

@@ -153,7 +153,8 @@ struct AttentionBackward : public torch::autograd::Node {
       a.grad_k = data_or_null(gk);
       a.grad_v = data_or_null(gv);
       const at::Tensor ws = workspace_of(a, true, gq);
-      check(mvr_attention_backward(&a, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, stream_of(gq)));
+      check(mvr_attention_backward(&a, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
+                                   mvr_host::status_of(gq.device().index()), stream_of(gq)));
       result = {gq, gk, gv};
     }
     once_differentiable("cross_attention", result, {grads[0], q0, k0, v0});

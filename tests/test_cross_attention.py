@@ -326,7 +326,7 @@ def test_c_entry_checks_before_any_cuda_call():
             rc = L.mvr_attention_workspace(ctypes.byref(a), int(backward), ctypes.byref(need))
             return rc, need.value
         if backward:
-            return L.mvr_attention_backward(ctypes.byref(a), 16, bytes, null)
+            return L.mvr_attention_backward(ctypes.byref(a), 16, bytes, null, null)
         return L.mvr_attention_forward(ctypes.byref(a), 16, bytes, null, null)
 
     assert call()[0] == 0
