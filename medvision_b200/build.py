@@ -14,7 +14,7 @@ NATIVE = os.path.join(HERE, "_native.so")
 SOURCES = ["mvr_api.cu", "mvr_heads.cu"]  # one object file each
 HEADERS = ["mvr_arith.cuh", "mvr_geom.cuh", "mvr_generic.cuh", "mvr_stream3d.cuh", "mvr_tma3d.cuh", "mvr_brick3d.cuh", "mvr_bwd3d.cuh", "mvr_offset.cuh", "mvr_cubic3d.cuh", "mvr_flat.cuh", "mvr_label.cuh", "mvr_plane2d.cuh", "mvr_elastic.cuh", "mvr_head.cuh",
            os.path.join("..", "..", "include", "mvr.h")]
-HEAD_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_tc.cuh", "mvr_dropout.cuh", "mvr_logprob.cuh",
+HEAD_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_tc.cuh", "mvr_dropout.cuh", "mvr_logprob.cuh",
                 os.path.join("..", "..", "include", "mvr.h")]
 HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": HEAD_HEADERS}
 NATIVE_SOURCES = ["mvr_torch.cpp", "mvr_torch_heads.cpp"]

@@ -1,0 +1,664 @@
+// Attention gradients on the tensor cores (float16, bfloat16; head sizes that are multiples of 8, up to 128).
+//
+// Two kernels, so that every sum has one place and one order.  One keeps 128 states and walks the rows that read them (dk, dv), the
+// other keeps 128 rows and walks the states (dq); both form the scores again from the forward's lse, P = 2^(S scale - lse):
+//
+//   states kept:  S^T = K Q^T    dP^T = V G^T    dV += P^T G    dK += dS^T Q           dS = P (dP - delta)
+//   rows kept:    S   = Q K^T    dP   = G V^T    dQ += dS K
+//
+// Scores, dP and the sums are in tensor memory; P and dS, rounded to T, go back over the scores and dP as left operands.  Two
+// warpgroups share a tile, one row a thread and half its columns each.  One thread issues the products in an order in which those of
+// one tile run under the exponentials of the next: dV(i), S(i+1), dK(i), dP(i+1), and S(i+1), dQ(i), dP(i+1).
+//
+// float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= 2 D max|g| max|v|
+// below 2^15 (max|g| from attn_delta, max|v| over the states kept, or over all that the first kernel saw).  Both are taken out of
+// the sums again, exactly.
+#pragma once
+#include "mvr_attn_tc.cuh"
+
+namespace mvr {
+
+constexpr int kGradThreads = 256;  // of the two warpgroups
+
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Power of two for dS, from bounds of |g| and |v| (float bits).
+template <typename T>
+__device__ __forceinline__ float slope_scale(int D, float g, float v) {
+  if constexpr (TcType<T>::code == 1) return 1.0f;
+  const float most = 2.0f * D * g * v;
+  if (!(most > 0.0f) || most > 3e38f) return 1.0f;
+  const int e = 14 - ilogbf(most);
+  return ldexpf(1.0f, e < -60 ? -60 : e > 60 ? 60 : e);
+}
+template <typename T>
+__device__ __forceinline__ float weight_shift() { return TcType<T>::code == 1 ? 0.0f : 10.0f; }
+
+// 32 sums of a row from tensor memory, times `factor`, to a row of floats or of T; columns behind D are left out.
+template <typename T>
+__device__ __forceinline__ void put_sums(uint32_t at, float factor, T* to, float* part, int col, int D, bool store, bool any) {
+  uint32_t v[32];
+  if (any) {
+    tmem_load32(v, at);
+    tmem_wait_load();
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0;
+  }
+  if (store) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      if (col + i >= D) continue;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[i + e]) * factor;
+      if (part) {
+        *(float4*)(part + col + i) = make_float4(f[0], f[1], f[2], f[3]);
+        *(float4*)(part + col + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+        *(uint4*)(to + col + i) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// ---- states kept: dk, dv ------------------------------------------------------------------------------
+template <int DP>
+struct TcStates {
+  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128;
+  static constexpr int kLoaders = 128, kThreads = kGradThreads + kLoaders + 32;
+  static constexpr int kScores = 0, kSlopes = 128, kValues = 256, kKeys = 256 + DP, kColumns = 512;
+  struct Control {
+    unsigned long long states, full[2], empty[2], scores, slopes, weights, grads, done;
+    uint32_t tmem;
+    int lost, peak;
+    alignas(16) float lse[2][128];
+    alignas(16) float delta[2][128];
+  };
+  static constexpr size_t kShared = 6 * (size_t)kTileBytes + sizeof(Control) + 1024;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(TcStates<DP>::kThreads, 1)
+attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
+  typedef TcStates<DP> F;
+  extern __shared__ char tc_smem[];
+  char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of two stages
+  typename F::Control& c = *(typename F::Control*)(base + 6 * F::kTileBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLoader = kGradThreads / 32, kIssuer = kLoader + F::kLoaders / 32;
+  if (threadIdx.x == 0) {
+    bar_init(smem_at(&c.states), 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(smem_at(&c.full[i]), F::kLoaders);
+      bar_init(smem_at(&c.empty[i]), 1);
+    }
+    bar_init(smem_at(&c.scores), 1);
+    bar_init(smem_at(&c.slopes), 1);
+    bar_init(smem_at(&c.weights), kGradThreads);
+    bar_init(smem_at(&c.grads), kGradThreads);
+    bar_init(smem_at(&c.done), 1);
+    c.lost = 0;
+    c.peak = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
+  const int state_tiles = (p.L + 127) / 128, n = blockIdx.x / state_tiles, j0 = (blockIdx.x - n * state_tiles) * 128;
+  const int hk = blockIdx.y, split = blockIdx.z;
+  // one row a thread: its state, and whether it is read
+  const int r = ((warp & 3) << 5) + lane, half = warp >> 2, j = j0 + r;
+  bool in = false;
+  if (warp < kLoader) in = j < states_of(p, n) && (!p.mask || p.mask[(long long)n * p.L + j] != 0);
+  const bool any = __syncthreads_or(in);
+  const RowTile o = image_rows(p, n);
+  const int row_tiles = (o.rows + 127) / 128, per = (row_tiles + p.row_splits - 1) / p.row_splits;
+  const int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0;
+  // what lies behind D in the rows' tiles stays 0
+  if (count > 0 && p.D < DP) {
+    for (int e = threadIdx.x; e < 4 * F::kTileBytes / 16; e += F::kThreads)
+      *(uint4*)(base + 2 * F::kTileBytes + e * 16) = make_uint4(0, 0, 0, 0);
+    fence_async_proxy();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = c.tmem;
+  volatile int* lost = &c.lost;
+  const float shift = weight_shift<T>();
+
+  if (warp == kIssuer) {
+    if (lane == 0 && count > 0) {
+      bar_expect(smem_at(&c.states), 2 * F::kTileBytes);
+      for (int b = 0; b < F::kBlocks; ++b) {
+        tma_load_4d(smem_at(base + b * 16384), &maps.k, smem_at(&c.states), b * 64, hk, j0, n);
+        tma_load_4d(smem_at(base + F::kTileBytes + b * 16384), &maps.v, smem_at(&c.states), b * 64, hk, j0, n);
+      }
+      const int depth = (p.D + 15) / 16;
+      const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
+      const auto scores = [&](int left, int right, int to) {  // 128 x 128 over D, both K-major
+        const uint32_t a = smem_at(base + left * F::kTileBytes), b = smem_at(base + right * F::kTileBytes);
+        for (int k = 0; k < depth; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          mma_ss(tmem + to, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+        }
+      };
+      const auto sums = [&](int from, int right, int to, bool add) {  // over the 128 rows
+        const uint32_t b = smem_at(base + right * F::kTileBytes);
+        for (int i = 0; i < 8; ++i)
+          mma_ts(tmem + to, tmem + from + (i >> 2) * 64 + (i & 3) * 8, desc_mn_major(b + i * 2048, 16384), d_shape, add || i > 0);
+      };
+      bool ok = bar_wait(smem_at(&c.states), 0, lost) && bar_wait(smem_at(&c.full[0]), 0, lost);
+      if (ok) {
+        tc_fence_after();
+        scores(0, 2, F::kScores);
+        mma_commit(smem_at(&c.scores));
+        scores(1, 3, F::kSlopes);
+        mma_commit(smem_at(&c.slopes));
+      }
+      for (int i = 0; i < count && ok; ++i) {
+        const int now = i & 1, next = now ^ 1;
+        if (!(ok = bar_wait(smem_at(&c.weights), i & 1, lost))) break;
+        tc_fence_after();
+        sums(F::kScores, 3 + 2 * now, F::kValues, i > 0);
+        if (i + 1 < count) {
+          if (!(ok = bar_wait(smem_at(&c.full[next]), ((i + 1) >> 1) & 1, lost))) break;
+          tc_fence_after();
+          scores(0, 2 + 2 * next, F::kScores);
+          mma_commit(smem_at(&c.scores));
+        }
+        if (!(ok = bar_wait(smem_at(&c.grads), i & 1, lost))) break;
+        tc_fence_after();
+        sums(F::kSlopes, 2 + 2 * now, F::kKeys, i > 0);
+        mma_commit(smem_at(&c.empty[now]));
+        if (i + 1 < count) {
+          scores(1, 3 + 2 * next, F::kSlopes);
+          mma_commit(smem_at(&c.slopes));
+        }
+      }
+      mma_commit(smem_at(&c.done));
+      if (*lost) {
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.states), 0) && nanoseconds() - t < kWaitLimit) {}
+      }
+    }
+  } else if (warp >= kLoader) {
+    // rows of Q and G, 16 bytes a copy: a warp's 32 rows, their places handed round by shuffles
+    const int w = warp - kLoader, mine = (w << 5) + lane;
+    const int chunks = p.D / 8;  // 16-byte pieces of a row
+    const auto arrived = [&](int stage) {
+      fence_async_proxy();
+      bar_arrive(smem_at(&c.full[stage]));
+    };
+    for (int i = 0; i < count; ++i) {
+      const int stage = i & 1;
+      if (i >= 2 && !__all_sync(~0u, bar_wait(smem_at(&c.empty[stage]), ((i >> 1) - 1) & 1, lost))) break;
+      const int at = (first + i) * 128 + mine;
+      const char *q = (const char*)p.q, *g = (const char*)p.g;
+      const bool row_in = at < o.rows;
+      float lse = INFINITY, delta = 0.0f;  // no row: P = 0
+      if (row_in) {
+        const Row row = row_of(p, o, at, hk);
+        q += (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
+        g += (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
+        const long long number = row_number(p, row);
+        lse = p.lse[number];
+        lse = lse == -INFINITY ? INFINITY : lse - shift;
+        delta = p.delta[number];
+      }
+      c.lse[stage][mine] = lse;
+      c.delta[stage][mine] = delta;
+      const uint32_t qs = smem_at(base + (2 + 2 * stage) * F::kTileBytes), gs = qs + F::kTileBytes;
+#pragma unroll 4
+      for (int e = 0; e < DP / 8; ++e) {
+        const int idx = e * 32 + lane, k = idx / (DP / 8), piece = idx % (DP / 8), row = (w << 5) + k;
+        const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q, k);
+        const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g, k);
+        const bool there = __shfl_sync(~0u, row_in, k);
+        if (piece < chunks) {
+          const uint32_t to = (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+          copy16(qs + to, there ? qk + piece * 16 : qk, there);
+          copy16(gs + to, there ? gk + piece * 16 : gk, there);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i == 0 && count > 1) continue;  // the first two stages are both under way before either is waited for
+      if (i == 1) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        arrived(0);
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      arrived(stage);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    float factor = 1.0f;  // of dS
+    bool ok = true;
+    if (count > 0 && TcType<T>::code == 0) {
+      ok = __all_sync(~0u, bar_wait(smem_at(&c.states), 0, lost));
+      // largest |v| of the states that are read
+      float most = 0.0f;
+      if (ok && in) {
+        const char* row = base + F::kTileBytes + r * 128;
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) {
+          const int piece = half * (DP / 16) + e;
+          const uint4 v = *(const uint4*)(row + (piece >> 3) * 16384 + (((piece ^ r) & 7) << 4));
+          const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(*(const __half2*)&words[k]);
+            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+      }
+      for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+      if (lane == 0) atomicMax(&c.peak, __float_as_int(most));
+      group_sync();
+      const float peak = __int_as_float(c.peak);
+      if (threadIdx.x == 0) atomicMax((int*)peaks + 1, c.peak);
+      factor = slope_scale<T>(p.D, peaks[0], peak);
+    }
+    const float slope = factor * exp2f(-shift);
+    for (int i = 0; i < count; ++i) {
+      const int stage = i & 1;
+      ok = ok && bar_wait(smem_at(&c.full[stage]), (i >> 1) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
+      if (!(ok = __all_sync(~0u, ok))) break;
+      tc_fence_after();
+      float w[64];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_load32(v, tmem + lanes + F::kScores + half * 64 + q * 32);
+        tmem_wait_load();
+        uint32_t u[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 lse = *(const float4*)&c.lse[stage][half * 64 + q * 32 + e];
+          const float x[4] = {lse.x, lse.y, lse.z, lse.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[q * 32 + e + k] = in ? exp2_fast(fmaf(__uint_as_float(v[e + k]), p.scale_log2, -x[k])) : 0.0f;
+          u[e / 2] = pack2<T>(w[q * 32 + e], w[q * 32 + e + 1]);
+          u[e / 2 + 1] = pack2<T>(w[q * 32 + e + 2], w[q * 32 + e + 3]);
+        }
+        // (over this warpgroup's own half of the scores)
+        tmem_store16(tmem + lanes + F::kScores + half * 64 + q * 16, u);
+      }
+      tmem_wait_store();
+      tc_fence_before();
+      bar_arrive(smem_at(&c.weights));
+      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_load32(v, tmem + lanes + F::kSlopes + half * 64 + q * 32);
+        tmem_wait_load();
+        uint32_t u[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 delta = *(const float4*)&c.delta[stage][half * 64 + q * 32 + e];
+          const float x[4] = {delta.x, delta.y, delta.z, delta.w};
+          float ds[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ds[k] = in ? w[q * 32 + e + k] * slope * (__uint_as_float(v[e + k]) - x[k]) : 0.0f;
+          u[e / 2] = pack2<T>(ds[0], ds[1]);
+          u[e / 2 + 1] = pack2<T>(ds[2], ds[3]);
+        }
+        tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
+      }
+      tmem_wait_store();
+      tc_fence_before();
+      bar_arrive(smem_at(&c.grads));
+    }
+    if (count > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
+    if (__all_sync(~0u, ok)) {
+      tc_fence_after();
+      // the first warpgroup stores dv, the second dk
+      const long long all = (long long)p.N * p.L * p.Hk * p.D, at = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
+      const bool parts = p.row_splits > 1;
+      const float f = in ? (half ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
+      T* to = (T*)(half ? p.gk : p.gv) + at;
+      float* part = parts ? (half ? p.part_gk : p.part_gv) + split * all + at : nullptr;
+#pragma unroll 1
+      for (int q = 0; q < DP / 32; ++q) {
+        if (q * 32 >= p.D) break;
+        // (a state that is not read: its sums may be NaN where rows hold NaN)
+        const uint32_t from = tmem + lanes + (half ? F::kKeys : F::kValues) + q * 32;
+        uint32_t v[32];
+        if (count > 0) {
+          tmem_load32(v, from);
+          tmem_wait_load();
+        }
+        if (j < p.L) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            if (q * 32 + i >= p.D) continue;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = in && count > 0 ? __uint_as_float(v[i + e]) * f : 0.0f;
+            if (part) {
+              *(float4*)(part + q * 32 + i) = make_float4(x[0], x[1], x[2], x[3]);
+              *(float4*)(part + q * 32 + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+              *(uint4*)(to + q * 32 + i) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    if (*lost) {
+      if (lane == 0) {
+        if (status) atomicOr(status, 2);
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.done), 0) && nanoseconds() - t < kWaitLimit) {}
+      }
+      __syncwarp();
+    }
+    tc_fence_after();
+    tmem_free(tmem, F::kColumns);
+  }
+}
+
+// ---- rows kept: dq ------------------------------------------------------------------------------------
+template <int DP, bool MASK>
+struct TcRows {
+  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kSlots = 4;
+  static constexpr int kThreads = kGradThreads + (MASK ? 96 : 64);
+  static constexpr int kScores = 0, kSlopes = 128, kSums = 256, kColumns = 512;
+  struct Control {
+    unsigned long long full[kSlots], empty[kSlots], clean[kSlots], rows, scores, taken, slopes, grads, done;
+    uint32_t tmem;
+    int lost, tiles;
+    unsigned short list[MASK ? kTcMaxTiles : 1];
+    uint4 bits[MASK ? kTcMaxTiles : 1];
+  };
+  static constexpr size_t kShared = (2 + kSlots) * (size_t)kTileBytes + sizeof(Control) + 1024;
+};
+
+template <typename T, int DP, bool MASK>
+__global__ void __launch_bounds__(TcRows<DP, MASK>::kThreads, 1)
+attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const float* peaks, int* status) {
+  typedef TcRows<DP, MASK> F;
+  extern __shared__ char tc_smem[];
+  char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // Q, G, then the ring
+  char* ring = base + 2 * F::kTileBytes;
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kTileBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLoader = kGradThreads / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kSlots; ++i) {
+      bar_init(smem_at(&c.full[i]), 1);
+      bar_init(smem_at(&c.empty[i]), 1);
+      bar_init(smem_at(&c.clean[i]), 1);
+    }
+    bar_init(smem_at(&c.rows), kGradThreads);
+    bar_init(smem_at(&c.scores), 1);
+    bar_init(smem_at(&c.taken), kGradThreads);
+    bar_init(smem_at(&c.slopes), 1);
+    bar_init(smem_at(&c.grads), kGradThreads);
+    bar_init(smem_at(&c.done), 1);
+    c.lost = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
+  RowTile o;
+  const bool some = row_tile(p, blockIdx.x, kTcRows, o);
+  const int hk = blockIdx.y, split = blockIdx.z;
+  const int all = (p.L + kTcStates - 1) / kTcStates, per = (all + p.splits - 1) / p.splits;
+  const int begin = split * per * kTcStates;
+  int end = 0;
+  if (some) end = min(states_of(p, o.n), (split + 1) * per * kTcStates);
+  if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + kTcStates - 1) / kTcStates;
+  const uint32_t tmem = c.tmem;
+  volatile int* lost = &c.lost;
+  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
+
+  if (warp == kLoader) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
+        const int slot = i % F::kSlots;
+        const uint32_t bar = smem_at(&c.full[slot]);
+        if (i >= F::kSlots && !bar_wait(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+        bar_expect(bar, F::kTileBytes);
+        const int j = first_of(i >> 1);
+        for (int b = 0; b < F::kBlocks; ++b)
+          tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * 16384), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
+      }
+      if (*lost)
+        for (int k = max(0, i - F::kSlots); k < i; ++k) {
+          const unsigned long long t = nanoseconds();
+          while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
+        }
+    }
+  } else if (warp == kIssuer) {
+    if (lane == 0 && tiles > 0) {
+      const int depth = (p.D + 15) / 16;
+      const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
+      const auto scores = [&](int left, int slot, int to) {
+        const uint32_t a = smem_at(base + left * F::kTileBytes), b = smem_at(ring + slot * F::kTileBytes);
+        for (int k = 0; k < depth; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          mma_ss(tmem + to, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+        }
+      };
+      const auto wait_full = [&](int i) { return bar_wait(smem_at(&c.full[i % F::kSlots]), (i / F::kSlots) & 1, lost); };
+      bool ok = bar_wait(smem_at(&c.rows), 0, lost) && wait_full(0);
+      if (ok) {
+        tc_fence_after();
+        scores(0, 0, F::kScores);
+        mma_commit(smem_at(&c.scores));
+        if ((ok = wait_full(1))) {
+          tc_fence_after();
+          scores(1, 1, F::kSlopes);
+          mma_commit(smem_at(&c.slopes));
+          mma_commit(smem_at(&c.empty[1]));
+        }
+      }
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int k = 2 * i, next = k + 2;
+        if (i + 1 < tiles) {
+          if (!(ok = bar_wait(smem_at(&c.taken), i & 1, lost) && wait_full(next))) break;
+          tc_fence_after();
+          scores(0, next % F::kSlots, F::kScores);
+          mma_commit(smem_at(&c.scores));
+        }
+        if (!(ok = bar_wait(smem_at(&c.grads), i & 1, lost))) break;
+        if (MASK && !(ok = bar_wait(smem_at(&c.clean[k % F::kSlots]), (k / F::kSlots) & 1, lost))) break;
+        tc_fence_after();
+        const uint32_t b = smem_at(ring + (k % F::kSlots) * F::kTileBytes);
+        for (int e = 0; e < 8; ++e)
+          mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 2) * 64 + (e & 3) * 8, desc_mn_major(b + e * 2048, 16384), d_shape, i > 0 || e > 0);
+        mma_commit(smem_at(&c.empty[k % F::kSlots]));
+        if (i + 1 < tiles) {
+          if (!(ok = wait_full(next + 1))) break;
+          tc_fence_after();
+          scores(1, (next + 1) % F::kSlots, F::kSlopes);
+          mma_commit(smem_at(&c.slopes));
+          mma_commit(smem_at(&c.empty[(next + 1) % F::kSlots]));
+        }
+      }
+      mma_commit(smem_at(&c.done));
+    }
+  } else if (MASK && warp == kCleaner) {
+    // rows of K that are left out may hold NaN: zero before they meet the zeros of dS
+    for (int i = 0; i < tiles; ++i) {
+      const int k = 2 * i, slot = k % F::kSlots;
+      if (!__all_sync(~0u, bar_wait(smem_at(&c.full[slot]), (k / F::kSlots) & 1, lost))) break;
+      const uint4 b = c.bits[i];
+      if ((b.x & b.y & b.z & b.w) != ~0u) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t out = ~word_of(b, w);
+          while (out) {
+            const int r = w * 32 + __ffs(out) - 1;
+            out &= out - 1;
+            if (lane < 8 * F::kBlocks)
+              *(uint4*)(ring + slot * F::kTileBytes + (lane >> 3) * 16384 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_proxy();
+        __syncwarp();
+      }
+      if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
+    }
+  } else if (warp < kLoader) {
+    const int r = threadIdx.x & 127, half = warp >> 2, j0 = o.first + r;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const bool mine = some && j0 < o.rows;
+    Row w = {};
+    long long number = 0;
+    float lse = INFINITY, delta = 0.0f;
+    if (mine) {
+      w = row_of(p, o, j0, hk);
+      number = row_number(p, w);
+      if (tiles > 0) {
+        lse = p.lse[number];
+        if (lse == -INFINITY) lse = INFINITY;
+        delta = p.delta[number];
+      }
+    }
+    if (tiles > 0) {
+      const long long at = half ? w.r * p.g_r + w.t * p.g_t + w.h * p.g_h : w.r * p.q_r + w.t * p.q_t + w.h * p.q_h;
+      put_row<DP>(base + half * F::kTileBytes, r, mine ? (const char*)(half ? p.g : p.q) + at * 2 : nullptr, p.D);
+      fence_async_proxy();
+      bar_arrive(smem_at(&c.rows));
+    }
+    const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
+    bool ok = true;
+    for (int i = 0; i < tiles; ++i) {
+      uint32_t bits[2] = {~0u, ~0u};
+      if (MASK) {
+        const uint4 b = c.bits[i];
+        bits[0] = half ? b.z : b.x;
+        bits[1] = half ? b.w : b.y;
+      } else if (i + 1 == tiles && (end & 127)) {
+        const int left = (end & 127) - half * 64;
+        bits[0] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
+        bits[1] = left >= 64 ? ~0u : left > 32 ? (1u << (left - 32)) - 1 : 0;
+      }
+      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.scores), i & 1, lost)))) break;
+      tc_fence_after();
+      float wgt[64];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_load32(v, tmem + lanes + F::kScores + half * 64 + q * 32);
+        tmem_wait_load();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) wgt[q * 32 + e] = __uint_as_float(v[e]);
+      }
+      tc_fence_before();
+      bar_arrive(smem_at(&c.taken));
+#pragma unroll
+      for (int e = 0; e < 64; ++e) wgt[e] = exp2_fast(fmaf(wgt[e], p.scale_log2, -lse)) * factor;
+      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_load32(v, tmem + lanes + F::kSlopes + half * 64 + q * 32);
+        tmem_wait_load();
+        float ds[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) ds[e] = wgt[q * 32 + e] * (__uint_as_float(v[e]) - delta);
+        if (bits[q] != ~0u) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ds[e] = (bits[q] >> e) & 1 ? ds[e] : 0.0f;
+        }
+        uint32_t u[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = pack2<T>(ds[2 * e], ds[2 * e + 1]);
+        tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
+      }
+      tmem_wait_store();
+      tc_fence_before();
+      bar_arrive(smem_at(&c.grads));
+    }
+    if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
+    if (__all_sync(~0u, ok)) {
+      tc_fence_after();
+      const long long rows = (long long)p.R * p.T * p.Hq;
+      float* part = p.splits > 1 ? p.part_gq + (split * rows + number) * p.D : nullptr;
+#pragma unroll 1
+      for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
+        if (q * 32 >= p.D) break;
+        put_sums<T>(tmem + lanes + F::kSums + q * 32, (part ? 1.0f : p.scale) / factor, (T*)p.gq + number * p.D, part, q * 32, p.D, mine,
+                    tiles > 0);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    if (*lost) {
+      if (lane == 0) {
+        if (status) atomicOr(status, 2);
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.done), 0) && nanoseconds() - t < kWaitLimit) {}
+      }
+      __syncwarp();
+    }
+    tc_fence_after();
+    tmem_free(tmem, F::kColumns);
+  }
+}
+
+// delta = g.o per row, and the largest finite |g| (float bits) into peaks[0].  One warp a row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p, float* peaks) {
+  grid_dependency();
+  __shared__ int peak;
+  if (threadIdx.x == 0) peak = 0;
+  __syncthreads();
+  const long long rows = (long long)p.R * p.T * p.Hq;
+  const int lane = threadIdx.x & 31, per = p.D / 8;  // a lane takes 8 elements of a row; 32 / width rows a warp
+  const int width = per <= 4 ? 4 : per <= 8 ? 8 : 16, sub = lane / width, piece = lane % width;
+  float most = 0.0f;
+  for (long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / width); first < rows; first += (long long)gridDim.x * 8 * (32 / width)) {
+    const long long row = first + sub;
+    float v = 0.0f;
+    if (row < rows && piece < per) {
+      const int h = (int)(row % p.Hq);
+      const long long rt = row / p.Hq, r = rt / p.T, t = rt - r * p.T;
+      const Vec<T, 8> g = *(const Vec<T, 8>*)((const T*)p.g + r * p.g_r + t * p.g_t + h * p.g_h + piece * 8);
+      const Vec<T, 8> o = *(const Vec<T, 8>*)((const T*)p.o + row * p.D + piece * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = to_float(g.v[e]);
+        v += a * to_float(o.v[e]);
+        if (fabsf(a) <= 3e38f) most = fmaxf(most, fabsf(a));
+      }
+    }
+    for (int d = width / 2; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+    if (row < rows && piece == 0) p.delta[row] = v;
+  }
+  if constexpr (TcType<T>::code == 0) {
+    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (lane == 0) atomicMax(&peak, __float_as_int(most));
+    __syncthreads();
+    if (threadIdx.x == 0) atomicMax((int*)peaks, peak);
+  }
+}
+
+}  // namespace mvr

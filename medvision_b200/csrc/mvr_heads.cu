@@ -9,6 +9,7 @@
 #include "../../include/mvr.h"
 #include "mvr_attn_fma.cuh"
 #include "mvr_attn_tc.cuh"
+#include "mvr_attn_tc_bwd.cuh"
 #include "mvr_dropout.cuh"
 #include "mvr_logprob.cuh"
 
@@ -31,7 +32,7 @@ struct AttnCut {
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
-  long long order, starts, tiles, delta, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+  long long order, starts, tiles, delta, peaks, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
@@ -55,14 +56,14 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   c.tc = tc;
   const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
   const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
-  c.tile = tc ? (rows_of_image > kTcRows ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
+  c.tile = tc ? (rows_of_image > kTcRows && !backward ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
   c.kv_tile = tc ? kTcStates : c.tile;
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
-  c.splits = best_parts(expected, kv_tiles, tc ? (c.tile > kTcRows ? 1 : 2) * kMultiprocessors : 2 * kMultiprocessors, 3, 0.5);
+  c.splits = best_parts(expected, kv_tiles, tc ? (c.tile > kTcRows || backward ? 1 : 2) * kMultiprocessors : 2 * kMultiprocessors, 3, 0.5);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(kv_tiles, kTcMaxTiles));
-  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), 2 * kMultiprocessors, 2, 1) : 1;
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), (tc ? 1 : 2) * kMultiprocessors, 2, 1) : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
     const long long here = at;
@@ -76,6 +77,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   }
   if (backward) {
     c.delta = take(rows * 4);
+    c.peaks = take(8);
     if (c.splits > 1) c.part_gq = take(c.splits * rows * a->D * 4);
     if (c.row_splits > 1) {
       c.part_gk = take(c.row_splits * a->N * a->L * a->Hk * a->D * 4);
@@ -237,16 +239,47 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
   return launched();
 }
 
+template <typename T, int DP>
+int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float* peaks, int* status, cudaStream_t st) {
+  const auto run = [&](auto kernel, dim3 grid, int threads, size_t smem, auto... args) {
+    if (grid.x == 0) return MVR_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+      cudaGetLastError();
+      return MVR_ERR_LAUNCH;
+    }
+    launch_dependent(kernel, grid, dim3(threads), smem, st, p, maps, args...);
+    return launched();
+  };
+  const int rc = run(attn_tc_dkv<T, DP>, dim3((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits), TcStates<DP>::kThreads,
+                     TcStates<DP>::kShared, peaks, status);
+  if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
+  const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
+  const float* bounds = peaks;
+  if (p.mask || p.lengths) return run(attn_tc_dq<T, DP, true>, grid, TcRows<DP, true>::kThreads, TcRows<DP, true>::kShared, bounds, status);
+  return run(attn_tc_dq<T, DP, false>, grid, TcRows<DP, false>::kThreads, TcRows<DP, false>::kShared, bounds, status);
+}
+
 template <typename T>
-int attention_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
+int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float* peaks, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
+  if (c.tc && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
+    cudaGetLastError();
+    return MVR_ERR_LAUNCH;
+  }
   if (rows > 0) {
-    launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, p);
+    if constexpr (sizeof(T) == 2) {
+      if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)std::min<long long>(cdiv(rows, 16), 8 * kMultiprocessors)), dim3(256), 0, st, p, peaks);
+    }
+    if (!c.tc) launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, p);
     if ((rc = launched()) != MVR_OK) return rc;
   }
-  rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
-       : p.D <= 128 ? fma_backward<T, 128>(p, c, st) : fma_backward<T, 256>(p, c, st);
+  if constexpr (sizeof(T) == 2) {
+    if (c.tc) rc = p.D <= 64 ? tc_backward<T, 64>(p, c, maps, peaks, status, st) : tc_backward<T, 128>(p, c, maps, peaks, status, st);
+  }
+  if (!c.tc)
+    rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
+         : p.D <= 128 ? fma_backward<T, 128>(p, c, st) : fma_backward<T, 256>(p, c, st);
   if (rc == MVR_OK && c.splits > 1) rc = sum_parts<T>(p.part_gq, p.gq, rows * p.D, c.splits, p.scale, st);
   if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gk, p.gk, states, c.row_splits, p.scale, st);
   if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gv, p.gv, states, c.row_splits, 1.0f, st);
@@ -256,14 +289,16 @@ int attention_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
 template <typename T>
 int attention_as(const mvr_attention* a, bool backward, char* workspace, int* status, cudaStream_t st) {
   TcMaps maps;
-  bool tc = !backward && tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
+  bool tc = tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
+  if (backward)
+    tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
   if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps, kTcStates);
   const AttnCut c = cut_attention(a, backward, tc);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
   const int rc = plan_attention(a, c, workspace, status, st);
   if (rc != MVR_OK) return rc;
   const AttnParams p = attention_params(a, c, workspace);
-  return backward ? attention_backward<T>(p, c, st) : attention_forward<T>(p, c, maps, status, st);
+  return backward ? attention_backward<T>(p, c, maps, (float*)(workspace + c.peaks), status, st) : attention_forward<T>(p, c, maps, status, st);
 }
 
 long long attention_bytes(const mvr_attention* a, bool backward) {
