@@ -11,6 +11,18 @@
 
 namespace mvr {
 
+struct PhiloxKeys {
+  unsigned x[10], y[10];  // of the rounds
+
+  __host__ __device__ __forceinline__ void from(unsigned long long seed) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      x[r] = (unsigned)seed + r * 0x9E3779B9u;
+      y[r] = (unsigned)(seed >> 32) + r * 0xBB67AE85u;
+    }
+  }
+};
+
 struct DropoutParams {
   const void* x;
   const void* residual;  // or null
@@ -18,84 +30,97 @@ struct DropoutParams {
   long long n;
   unsigned cut;          // an element stays when its 16 bits are >= cut; 65536: none stays
   float scale;
-  unsigned long long seed, offset;
+  PhiloxKeys keys;       // constants of the launch, so that a round is two products and two three-way exclusive ors
+  unsigned long long offset;
   const unsigned long long* seed_at;  // or null; else the seed lies there, on the device
 };
 
-__device__ __forceinline__ uint4 philox(uint2 key, uint4 c) {
+__device__ __forceinline__ uint4 philox(const PhiloxKeys& k, uint4 c) {
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)c.x * 0xD2511F53u, b = (unsigned long long)c.z * 0xCD9E8D57u;
-    c = make_uint4((unsigned)(b >> 32) ^ c.y ^ key.x, (unsigned)b, (unsigned)(a >> 32) ^ c.w ^ key.y, (unsigned)a);
-    key.x += 0x9E3779B9u;
-    key.y += 0xBB67AE85u;
+    c = make_uint4((unsigned)(b >> 32) ^ c.y ^ k.x[r], (unsigned)b, (unsigned)(a >> 32) ^ c.w ^ k.y[r], (unsigned)a);
   }
   return c;
 }
 
-constexpr int kDropThreads = 256;
+constexpr int kDropThreads = 256, kDropGroups = 2;
 
-// A thread takes groups of eight consecutive elements.  VECTOR: x, residual and out are 16-byte aligned.
-template <typename T, bool VECTOR, bool RESIDUAL>
+// A thread takes kDropGroups groups of eight consecutive elements, a CTA's width apart, all their loads under way together.
+// VECTOR: x, residual and out are 16-byte aligned.  DEVICE: the seed lies on the device.
+template <typename T, bool VECTOR, bool RESIDUAL, bool DEVICE>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const __grid_constant__ DropoutParams p) {
   grid_dependency();
-  const unsigned long long seed = p.seed_at ? *p.seed_at : p.seed;
-  const uint2 key = make_uint2((unsigned)seed, (unsigned)(seed >> 32));
+  PhiloxKeys own;
+  if (DEVICE) own.from(*p.seed_at);
   const T* x = (const T*)p.x;
   const T* res = (const T*)p.residual;
   T* out = (T*)p.out;
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2, kPart = 8 / kParts;
   typedef Vec<T, kPart> V;
-  const long long groups = (p.n + 7) >> 3;
-  for (long long g = (long long)blockIdx.x * kDropThreads + threadIdx.x; g < groups; g += (long long)gridDim.x * kDropThreads) {
-    const long long e = g << 3;
-    const bool whole = VECTOR && e + 8 <= p.n;
-    alignas(16) T xv[8];
-    alignas(16) T rv[8];
-    if (whole) {
+  const long long first = ((long long)blockIdx.x * kDropGroups * kDropThreads + threadIdx.x) << 3;
+  V xv[kDropGroups][kParts], rv[kDropGroups][kParts];
+  bool whole[kDropGroups];
+#pragma unroll
+  for (int i = 0; i < kDropGroups; ++i) {
+    const long long e = first + i * kDropThreads * 8;
+    whole[i] = VECTOR && e + 8 <= p.n;
+    if (whole[i]) {
 #pragma unroll
       for (int k = 0; k < kParts; ++k) {
-        *(V*)(xv + k * kPart) = *(const V*)(x + e + k * kPart);
-        if (RESIDUAL) *(V*)(rv + k * kPart) = *(const V*)(res + e + k * kPart);
+        xv[i][k] = *(const V*)(x + e + k * kPart);
+        if (RESIDUAL) rv[i][k] = *(const V*)(res + e + k * kPart);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const bool in = e + k < p.n;
-        xv[k] = in ? x[e + k] : from_float<T>(0.0f);
-        if (RESIDUAL) rv[k] = in ? res[e + k] : from_float<T>(0.0f);
+        xv[i][k / kPart].v[k % kPart] = in ? x[e + k] : from_float<T>(0.0f);
+        if (RESIDUAL) rv[i][k / kPart].v[k % kPart] = in ? res[e + k] : from_float<T>(0.0f);
       }
     }
-    const uint4 r = philox(key, make_uint4((unsigned)g, (unsigned)(g >> 32), (unsigned)p.offset, (unsigned)(p.offset >> 32)));
+  }
+#pragma unroll
+  for (int i = 0; i < kDropGroups; ++i) {
+    const long long e = first + i * kDropThreads * 8, g = e >> 3;
+    const uint4 r = philox(DEVICE ? own : p.keys, make_uint4((unsigned)g, (unsigned)(g >> 32), (unsigned)p.offset, (unsigned)(p.offset >> 32)));
     const unsigned word[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const unsigned bits = (k & 1) ? word[k >> 1] >> 16 : word[k >> 1] & 0xffffu;
+      // the high half is compared in place: its word is >= cut * 2^16 when the half is >= cut
+      const bool stays = (k & 1) ? word[k >> 1] >= (p.cut << 16) && p.cut < 65536 : (word[k >> 1] & 0xffffu) >= p.cut;
       // a dropped element gives 0 whatever it held, NaN and infinities included
-      float v = bits >= p.cut ? to_float(xv[k]) * p.scale : 0.0f;
-      if (RESIDUAL) v += to_float(rv[k]);
-      xv[k] = from_float<T>(v);
+      float v = stays ? to_float(xv[i][k / kPart].v[k % kPart]) * p.scale : 0.0f;
+      if (RESIDUAL) v += to_float(rv[i][k / kPart].v[k % kPart]);
+      xv[i][k / kPart].v[k % kPart] = from_float<T>(v);
     }
-    if (whole) {
+    if (whole[i]) {
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) *(V*)(out + e + k * kPart) = *(const V*)(xv + k * kPart);
+      for (int k = 0; k < kParts; ++k) *(V*)(out + e + k * kPart) = xv[i][k];
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (e + k < p.n) out[e + k] = xv[k];
+        if (e + k < p.n) out[e + k] = xv[i][k / kPart].v[k % kPart];
     }
   }
 }
 
+// 0, or 1: more CTAs than a grid has.
 template <typename T>
-cudaError_t launch_dropout(const DropoutParams& p, cudaStream_t st) {
-  const long long groups = (p.n + 7) >> 3, want = (groups + kDropThreads - 1) / kDropThreads;
-  const dim3 grid((unsigned)(want < (1LL << 30) ? want : (1LL << 30)));
+int launch_dropout(const DropoutParams& p, cudaStream_t st) {
+  const long long per = 8LL * kDropGroups * kDropThreads, ctas = (p.n + per - 1) / per;
+  if (ctas > 0x7fffffffLL) return 1;
+  const dim3 grid((unsigned)ctas);
   const bool vec = (((uintptr_t)p.x | (uintptr_t)p.out | (uintptr_t)p.residual) & 15) == 0;
-  if (vec) return p.residual ? launch_dependent(dropout_kernel<T, true, true>, grid, kDropThreads, 0, st, p)
-                             : launch_dependent(dropout_kernel<T, true, false>, grid, kDropThreads, 0, st, p);
-  return p.residual ? launch_dependent(dropout_kernel<T, false, true>, grid, kDropThreads, 0, st, p)
-                    : launch_dependent(dropout_kernel<T, false, false>, grid, kDropThreads, 0, st, p);
+  const auto go = [&](auto kernel) { launch_dependent(kernel, grid, kDropThreads, 0, st, p); };
+  if (p.seed_at) {
+    if (vec) p.residual ? go(dropout_kernel<T, true, true, true>) : go(dropout_kernel<T, true, false, true>);
+    else p.residual ? go(dropout_kernel<T, false, true, true>) : go(dropout_kernel<T, false, false, true>);
+  } else {
+    if (vec) p.residual ? go(dropout_kernel<T, true, true, false>) : go(dropout_kernel<T, true, false, false>);
+    else p.residual ? go(dropout_kernel<T, false, true, false>) : go(dropout_kernel<T, false, false, false>);
+  }
+  return 0;
 }
 
 }  // namespace mvr

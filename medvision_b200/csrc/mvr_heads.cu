@@ -352,14 +352,13 @@ int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64
   p.x = x; p.residual = residual; p.out = out; p.n = n;
   p.cut = (unsigned)std::floor(probability * 65536.0 + 0.5);
   p.scale = p.cut < 65536 ? (float)(65536.0 / (65536.0 - p.cut)) : 0.0f;
-  p.seed = seed; p.seed_at = (const unsigned long long*)seed_at; p.offset = offset;
+  p.keys.from(seed);
+  p.seed_at = (const unsigned long long*)seed_at;
+  p.offset = offset;
   const cudaStream_t st = (cudaStream_t)stream;
-  switch (dtype) {
-    case MVR_F32: launch_dropout<float>(p, st); break;
-    case MVR_F16: launch_dropout<__half>(p, st); break;
-    default: launch_dropout<__nv_bfloat16>(p, st); break;
-  }
-  return launched();
+  const int rc = dtype == MVR_F32 ? launch_dropout<float>(p, st) : dtype == MVR_F16 ? launch_dropout<__half>(p, st)
+                                                                                    : launch_dropout<__nv_bfloat16>(p, st);
+  return rc ? MVR_ERR_TOO_LARGE : launched();
 }
 
 static int label_log_probs(const LogProbParams& p, int dtype, bool fwd, void* stream) {

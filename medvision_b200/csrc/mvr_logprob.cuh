@@ -5,12 +5,15 @@
 //   top: the largest x_c - lse, ties to the lowest class, NaN before everything
 //   dx_c = a (1[c == y] - p_c) - b p_c (log p_c + H)           a, b: gradients of log_prob (0 where no label is given) and of H
 //
-// One pass keeps, per position, the running maximum m, l = sum exp(x - m) and u = sum (x - m) exp(x - m), all in float: with them
-// lse = m + log l and H = log l - u / l, a difference that stays small whatever the scores' offset.  When the maximum moves by d,
-// l and u + d l are scaled by exp(d).  A position whose scores are all -inf has log_prob -inf, entropy 0 and gradient 0.
+// With the maximum m, l = sum exp(x - m) and u = sum (x - m) exp(x - m), all in float: lse = m + log l, and H = log l - u / l, a
+// difference that stays small whatever the scores' offset.  Where the scores do not fit the registers they are walked once with a
+// running maximum: when it moves by d, l and u + d l are scaled by exp(d).  A position whose scores are all -inf has log_prob -inf,
+// entropy 0 and gradient 0.
 //
 // Two layouts: classes apart (NC[D]HW maps; a thread walks the classes of neighbouring positions, so that a warp reads
-// consecutive ones) and classes together (rows; a warp or a CTA shares a row).
+// consecutive ones) and classes together (rows; a warp or a CTA shares a row).  Up to 16 classes apart, 1024 classes of a warp's row
+// and 65536 half (32768 float) classes of a CTA's row are read once, all loads under way together, and stay in registers.  The scores
+// are read once by each direction, the gradient written once: bound by memory.
 #pragma once
 #include "mvr_types.cuh"
 
@@ -44,6 +47,13 @@ __device__ __forceinline__ int label_at(const LogProbParams& p, long long i) {
   return v >= 0 && v < p.classes ? (int)v : -1;
 }
 
+// 2^x to some 2^-22, relatively; 0 below 2^-126.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Running (m, l, u) of one position.
 struct Online {
   float m = -INFINITY, l = 0.0f, u = 0.0f;
@@ -60,9 +70,10 @@ struct Online {
     m = to;
   }
   __device__ __forceinline__ void add(float x) {  // x <= m
-    const float d = x - m, e = exp2f(d * kLog2e);
+    // (a score of -inf adds 0 to both: its distance is kept finite)
+    const float d = x - m, e = exp2_approx(d * kLog2e);
     l += e;
-    u += e == 0.0f ? 0.0f : d * e;
+    u = fmaf(fmaxf(d, -1e30f), e, u);
   }
   __device__ __forceinline__ void join(const Online& o) {
     // NaN wins over everything: fmaxf would drop it
@@ -78,7 +89,8 @@ struct Online {
   __device__ __forceinline__ float entropy() const { return m == -INFINITY ? 0.0f : log2f(l) * kLn2 - u / l; }
 };
 
-__device__ __forceinline__ float log_prob_of(float x, const Online& o) { return x == -INFINITY ? x : (x - o.m) - log2f(o.l) * kLn2; }
+__device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2f(l) * kLn2; }
+__device__ __forceinline__ float log_prob_of(float x, const Online& o) { return log_prob_of(x, o.m, o.l); }
 
 // Order of the alternatives: NaN first, then the larger score; equal ones by class.
 __device__ __forceinline__ bool above(float a, float b) { return a > b || (a != a && b == b); }
@@ -86,33 +98,57 @@ __device__ __forceinline__ bool before(float a, int ia, float b, int ib) {
   return above(a, b) || (!above(b, a) && ia < ib);
 }
 
-// Sorted list of the best TOP (value, class) pairs offered so far, classes in rising order.
-template <int TOP>
-struct Best {
-  float v[TOP > 0 ? TOP : 1];
-  int c[TOP > 0 ? TOP : 1];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int k = 0; k < TOP; ++k) v[k] = -INFINITY, c[k] = 0x7fffffff;
-  }
-  __device__ __forceinline__ void offer(float x, int cls) {
-    if (TOP == 0 || !before(x, cls, v[TOP > 0 ? TOP - 1 : 0], c[TOP > 0 ? TOP - 1 : 0])) return;
-#pragma unroll
-    for (int k = TOP - 1; k >= 0; --k) {
-      const bool here = before(x, cls, v[k], c[k]);
-      if (here && k + 1 < TOP) v[k + 1] = v[k], c[k + 1] = c[k];
-      const bool next = k > 0 && before(x, cls, v[k > 0 ? k - 1 : 0], c[k > 0 ? k - 1 : 0]);
-      if (here && !next) v[k] = x, c[k] = cls;
+// The alternatives of a position whose scores are NaN, infinite or too few for the fast way, one by one.
+template <typename T>
+__device__ __noinline__ void pick_apart(const T* x, long long stride, int classes, int top, long long space, float* value, int* label,
+                                        float m, float l) {
+  float last_v = 0.0f;
+  int last_c = -1;
+  for (int t = 0; t < top; ++t) {
+    float v = -INFINITY;
+    int c = 0x7fffffff;
+    for (int k = 0; k < classes; ++k) {
+      const float f = to_float(x[k * stride]);
+      if ((t == 0 || before(last_v, last_c, f, k)) && before(f, k, v, c)) v = f, c = k;
     }
+    value[t * space] = log_prob_of(v, m, l);
+    label[t * space] = c;
+    last_v = v, last_c = c;
   }
-};
+}
 
 // ---- classes apart: positions consecutive ------------------------------------------------------------
 constexpr int kApartThreads = 128;
 
-// A thread takes V consecutive positions of one batch item and walks their classes eight at a time: the maximum of eight moves
-// the sums once.
-template <typename T, int V, int TOP>
+// Sorted list of the best TOP scores, offered by rising class: an equal score comes behind.  (NaN is left to pick_slowly.)
+template <int TOP>
+struct Best {
+  float v[TOP];
+  int c[TOP];
+  __device__ __forceinline__ Best() {
+#pragma unroll
+    for (int k = 0; k < TOP; ++k) v[k] = -INFINITY, c[k] = -1;
+  }
+  __device__ __forceinline__ void offer(float x, int cls) {
+    if (TOP > 2 && !(x > v[TOP - 1])) return;
+#pragma unroll
+    for (int k = TOP - 1; k > 0; --k) {
+      const bool above_k = x > v[k], above_next = x > v[k - 1];
+      v[k] = above_next ? v[k - 1] : above_k ? x : v[k];
+      c[k] = above_next ? c[k - 1] : above_k ? cls : c[k];
+    }
+    c[0] = x > v[0] ? cls : c[0];
+    v[0] = fmaxf(v[0], x);
+  }
+};
+template <>
+struct Best<0> {
+  __device__ __forceinline__ void offer(float, int) {}
+};
+
+// A thread takes V consecutive positions of one batch item.  CACHE: number of classes that stay in registers (0: eight at a time,
+// the maximum of eight moves the sums once).
+template <typename T, int V, int TOP, int CACHE>
 __global__ void __launch_bounds__(kApartThreads) logprob_apart_fwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const long long per_item = (p.space + V - 1) / V, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
@@ -121,51 +157,55 @@ __global__ void __launch_bounds__(kApartThreads) logprob_apart_fwd(const __grid_
   const T* x = (const T*)p.x + b * p.batch_stride + s;
   const int n = (int)(p.space - s < V ? p.space - s : V);
   const long long at = b * p.space + s;
+  constexpr int kStep = CACHE > 0 ? CACHE : 8;
   Online o[V];
   Best<TOP> best[V];
   float given[V];
   int label[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    best[k].clear();
     given[k] = 0.0f;
     label[k] = k < n ? label_at(p, at + k) : -1;
   }
-  constexpr int kStep = V >= 4 ? 4 : 8;
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
-    float f[kStep][V];
+    Vec<T, V> w[kStep];
 #pragma unroll
     for (int j = 0; j < kStep; ++j) {
       if (c0 + j < p.classes) {
         const T* q = x + (long long)(c0 + j) * p.class_stride;
         if (n == V) {
-          const Vec<T, V> w = *(const Vec<T, V>*)q;
-#pragma unroll
-          for (int k = 0; k < V; ++k) f[j][k] = to_float(w.v[k]);
+          w[j] = *(const Vec<T, V>*)q;
         } else {
 #pragma unroll
-          for (int k = 0; k < V; ++k) f[j][k] = k < n ? to_float(q[k]) : 0.0f;
+          for (int k = 0; k < V; ++k) w[j].v[k] = k < n ? q[k] : from_float<T>(0.0f);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) f[j][k] = -INFINITY;
+        for (int k = 0; k < V; ++k) w[j].v[k] = from_float<T>(-INFINITY);
       }
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float m = o[k].m;
 #pragma unroll
-      for (int j = 0; j < kStep; ++j) m = m != m || f[j][k] <= m ? m : f[j][k];  // NaN stays
-      o[k].raise(m);
-      if (m != -INFINITY) {
+      for (int j = 0; j < kStep; ++j) m = fmaxf(m, to_float(w[j].v[k]));
+      if (m == -INFINITY) {  // nothing yet; NaN is not seen by the maximum
 #pragma unroll
-        for (int j = 0; j < kStep; ++j) o[k].add(f[j][k]);
+        for (int j = 0; j < kStep; ++j) m = to_float(w[j].v[k]) != to_float(w[j].v[k]) ? NAN : m;
+      }
+      if (m != -INFINITY) {
+        o[k].raise(m);
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+          if (CACHE == 0 || j < p.classes) o[k].add(to_float(w[j].v[k]));
+        }
       }
 #pragma unroll
       for (int j = 0; j < kStep; ++j) {
-        if (c0 + j < p.classes) {
-          if (TOP > 0) best[k].offer(f[j][k], c0 + j);
-          if (label[k] == c0 + j) given[k] = f[j][k];
+        if (CACHE == 0 || j < p.classes) {
+          const float f = to_float(w[j].v[k]);
+          if (c0 + j < p.classes) best[k].offer(f, c0 + j);
+          given[k] = label[k] == c0 + j ? f : given[k];
         }
       }
     }
@@ -176,34 +216,43 @@ __global__ void __launch_bounds__(kApartThreads) logprob_apart_fwd(const __grid_
     p.log_prob[at + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
     p.entropy[at + k] = o[k].entropy();
     if (p.lse) p.lse[at + k] = o[k].lse();
+    if constexpr (TOP > 0) {
+      float* value = p.top_value + b * p.top * p.space + s + k;
+      int* best_label = p.top_label + b * p.top * p.space + s + k;
+      bool all = o[k].l == o[k].l;
 #pragma unroll
-    for (int t = 0; t < TOP; ++t) {
-      if (t < p.top) {
-        p.top_value[(b * p.top + t) * p.space + s + k] = log_prob_of(best[k].v[t], o[k]);
-        p.top_label[(b * p.top + t) * p.space + s + k] = best[k].c[t];
+      for (int t = 0; t < TOP; ++t) all = all && (t >= p.top || best[k].c[t] >= 0);
+      if (all) {
+#pragma unroll
+        for (int t = 0; t < TOP; ++t)
+          if (t < p.top) value[t * p.space] = log_prob_of(best[k].v[t], o[k]), best_label[t * p.space] = best[k].c[t];
+      } else {
+        pick_apart(x + k, p.class_stride, p.classes, p.top, p.space, value, best_label, o[k].m, o[k].l);
       }
     }
   }
 }
 
-// What the gradient of one position needs beside its scores.
+// What the gradient of one position needs beside its scores: g_c = -e (k + b lp), lp = x - lse, e = exp lp, k = a + b H; a more at
+// the label.
 struct Slope {
-  float lse, h, a, b;
+  float lse, a, b, k;
   int label;
-  __device__ __forceinline__ float at(float x, int c) const {
-    const float lp = x - lse, e = exp2f(lp * kLog2e);
-    const float w = e == 0.0f ? 0.0f : e * (a + b * (lp + h));  // probability 0: lp may be -inf
-    const float g = (c == label ? a : 0.0f) - w;
-    return lse == -INFINITY ? 0.0f : g;
+  __device__ __forceinline__ float at(float x) const {
+    // (a class of probability 0 has lp = -inf: kept finite, so that e = 0 gives 0; NaN is in lse and k as well)
+    const float lp = fmaxf(x - lse, -1e30f);
+    return -exp2_approx(lp * kLog2e) * fmaf(b, lp, k);
   }
+  __device__ __forceinline__ bool empty() const { return lse == -INFINITY; }
 };
 __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
   Slope s;
   s.label = label_at(p, i);
   s.lse = p.lse[i];
-  s.h = p.entropy[i];
   s.a = s.label >= 0 && p.grad_log_prob ? p.grad_log_prob[i] : 0.0f;
   s.b = p.grad_entropy ? p.grad_entropy[i] : 0.0f;
+  s.k = fmaf(s.b, p.entropy[i], s.a);
+  if (s.lse != s.lse) s.k = NAN;
   return s;
 }
 
@@ -219,249 +268,437 @@ __global__ void __launch_bounds__(kApartThreads) logprob_apart_bwd(const __grid_
   Slope q[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) q[k] = slope_at(p, b * p.space + s + (k < n ? k : 0));
-#pragma unroll 4
-  for (int c = 0; c < p.classes; ++c) {
-    const T* xc = x + (long long)c * p.class_stride;
-    T* gc = g + (long long)c * p.grad_class_stride;
-    if (n == V) {
-      const Vec<T, V> w = *(const Vec<T, V>*)xc;
-      Vec<T, V> r;
+  for (int c0 = 0; c0 < p.classes; c0 += 8) {
+    Vec<T, V> w[8];
 #pragma unroll
-      for (int k = 0; k < V; ++k) r.v[k] = from_float<T>(q[k].at(to_float(w.v[k]), c));
-      *(Vec<T, V>*)gc = r;
-    } else {
+    for (int j = 0; j < 8; ++j) {
+      if (c0 + j < p.classes) {
+        const T* xc = x + (long long)(c0 + j) * p.class_stride;
+        if (n == V) {
+          w[j] = *(const Vec<T, V>*)xc;
+        } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (k < n) gc[k] = from_float<T>(q[k].at(to_float(xc[k]), c));
+          for (int k = 0; k < V; ++k) w[j].v[k] = xc[k < n ? k : 0];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (c0 + j < p.classes) {
+        T* gc = g + (long long)(c0 + j) * p.grad_class_stride;
+        Vec<T, V> r;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float v = q[k].at(to_float(w[j].v[k])) + (c0 + j == q[k].label ? q[k].a : 0.0f);
+          r.v[k] = from_float<T>(q[k].empty() ? 0.0f : v);
+        }
+        if (n == V) {
+          *(Vec<T, V>*)gc = r;
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (k < n) gc[k] = r.v[k];
+        }
+      }
     }
   }
 }
 
 // ---- classes together: rows -------------------------------------------------------------------------
-// LANES threads (a warp, or a CTA of 512) share a row.  The alternatives need a second look at the row: split into 32 parts, the
-// top-th largest of the parts' maxima is a bound that at least `top` classes reach, and few more do (some 20 of a random row for
-// top = 8); what reaches it is collected and ranked.  Where more reach it than there is room for (many equal scores), the
-// alternatives are picked one by one instead.
-constexpr int kWide = 512, kRoom = 256;
-
-template <int LANES>
-struct RowShared {
-  static constexpr int kWarps = LANES / 32;
-  float m[kWarps], l[kWarps], u[kWarps];
-  float peak[32];
-  float cand[kRoom];
-  int cand_class[kRoom];
-  int count;
-  float pick_v;
-  float wv[kWarps];
-  int wc[kWarps];
-};
-
-template <int LANES>
-__device__ __forceinline__ void row_sync() {
-  if (LANES == 32) __syncwarp();
-  else __syncthreads();
-}
-
-// Visits a row: f(value, class) on this thread's classes, 16-byte vectors in between for the wide form.
-template <typename T, int LANES, typename F>
-__device__ __forceinline__ void walk_row(const T* x, int n, int lane, F&& f) {
-  if (LANES == 32) {
-    for (int c = lane; c < n; c += 32) f(to_float(x[c]), c);
-  } else {
-    constexpr int V = 16 / (int)sizeof(T);
-    const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), vecs = (n - head) / V;
-    if (lane < head) f(to_float(x[lane]), lane);
-    const Vec<T, V>* v = (const Vec<T, V>*)(x + head);
-#pragma unroll 4
-    for (int i = lane; i < vecs; i += LANES) {
-      const Vec<T, V> w = v[i];
-#pragma unroll
-      for (int k = 0; k < V; ++k) f(to_float(w.v[k]), head + i * V + k);
-    }
-    for (int c = head + vecs * V + lane; c < n; c += LANES) f(to_float(x[c]), c);
-  }
-}
-
-template <int LANES>
-__device__ __forceinline__ void best_of_row(float& v, int& c, RowShared<LANES>& sh, int lane) {
+// A warp's row: lane i holds the classes i, i + 32, ...; the alternatives are picked one by one, each a round of the lanes' best.
+__device__ __forceinline__ void best_of_warp(float& v, int& c) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     const float ov = __shfl_xor_sync(~0u, v, d);
     const int oc = __shfl_xor_sync(~0u, c, d);
     if (before(ov, oc, v, c)) v = ov, c = oc;
   }
-  if (LANES > 32) {
-    if ((lane & 31) == 0) sh.wv[lane >> 5] = v, sh.wc[lane >> 5] = c;
-    __syncthreads();
-    v = sh.wv[0], c = sh.wc[0];
-    for (int w = 1; w < LANES / 32; ++w)
-      if (before(sh.wv[w], sh.wc[w], v, c)) v = sh.wv[w], c = sh.wc[w];
-    __syncthreads();
+}
+
+template <typename T, int CAP>
+__global__ void __launch_bounds__(128) logprob_warp_fwd(const __grid_constant__ LogProbParams p) {
+  grid_dependency();
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= p.batch) return;
+  const T* x = (const T*)p.x + row * p.batch_stride;
+  const int n = p.classes, y = label_at(p, row);
+  float f[CAP];
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) f[j] = lane + 32 * j < n ? to_float(x[lane + 32 * j]) : -INFINITY;
+  const float given = y < 0 ? 0.0f : to_float(x[y]);
+  Online o;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) {
+    o.m = fmaxf(o.m, f[j]);
+    nan |= f[j] != f[j];
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) o.m = fmaxf(o.m, __shfl_xor_sync(~0u, o.m, d));
+  if (__any_sync(~0u, nan)) o.m = NAN;
+  if (o.m != -INFINITY) {
+#pragma unroll
+    for (int j = 0; j < CAP; ++j)
+      if (32 * j < n) o.add(f[j]);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    o.l += __shfl_xor_sync(~0u, o.l, d);
+    o.u += __shfl_xor_sync(~0u, o.u, d);
+  }
+  if (lane == 0) {
+    p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
+    p.entropy[row] = o.entropy();
+    if (p.lse) p.lse[row] = o.lse();
+  }
+  float last_v = 0.0f;
+  int last_c = -1;
+  for (int t = 0; t < p.top; ++t) {
+    float v = -INFINITY;
+    int c = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) {
+      const int k = lane + 32 * j;
+      if (k < n && (t == 0 || before(last_v, last_c, f[j], k)) && before(f[j], k, v, c)) v = f[j], c = k;
+    }
+    best_of_warp(v, c);
+    if (lane == t) {
+      p.top_value[row * p.top + t] = log_prob_of(v, o);
+      p.top_label[row * p.top + t] = c;
+    }
+    last_v = v, last_c = c;
   }
 }
 
-template <typename T, int LANES>
-__global__ void __launch_bounds__(LANES == 32 ? 128 : LANES) logprob_rows_fwd(const __grid_constant__ LogProbParams p) {
-  constexpr int kRows = LANES == 32 ? 4 : 1;
-  __shared__ RowShared<LANES> shared[kRows];
+template <typename T>
+__global__ void __launch_bounds__(128) logprob_warp_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const int lane = LANES == 32 ? threadIdx.x & 31 : threadIdx.x, mine = LANES == 32 ? threadIdx.x >> 5 : 0;
-  RowShared<LANES>& sh = shared[mine];
-  const long long row = (long long)blockIdx.x * kRows + mine;
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= p.batch) return;
   const T* x = (const T*)p.x + row * p.batch_stride;
-  const int n = p.classes;
+  T* g = (T*)p.grad + row * p.grad_batch_stride;
+  const Slope q = slope_at(p, row);
+#pragma unroll 4
+  for (int c = lane; c < p.classes; c += 32) {
+    const float v = q.at(to_float(x[c])) + (c == q.label ? q.a : 0.0f);
+    g[c] = from_float<T>(q.empty() ? 0.0f : v);
+  }
+}
+
+// A CTA's row.  The alternatives need a second look at the scores: split into 32 parts, the top-th largest of the parts' maxima is a
+// bound that at least `top` classes reach, and few more do (some 20 of a random row for top = 8); what reaches it is collected and
+// ranked.  Where more reach it than there is room for (many equal scores), or there is a NaN, they are picked one by one.
+constexpr int kWide = 512, kRoom = 256;
+
+struct RowShared {
+  float m[kWide / 32], l[kWide / 32], u[kWide / 32];
+  float peak[32], cand[kRoom];
+  int cand_class[kRoom];
+  int count, wc[kWide / 32];
+  float bound, wv[kWide / 32];
+};
+
+template <typename T>
+__device__ __noinline__ void pick_row(const T* x, int classes, int top, float* value, int* label, float m, float l, RowShared& sh) {
+  const int lane = threadIdx.x, w = lane >> 5;
+  float last_v = 0.0f;
+  int last_c = -1;
+  for (int t = 0; t < top; ++t) {
+    float v = -INFINITY;
+    int c = 0x7fffffff;
+    for (int k = lane; k < classes; k += kWide) {
+      const float f = to_float(x[k]);
+      if ((t == 0 || before(last_v, last_c, f, k)) && before(f, k, v, c)) v = f, c = k;
+    }
+    best_of_warp(v, c);
+    if ((lane & 31) == 0) sh.wv[w] = v, sh.wc[w] = c;
+    __syncthreads();
+    v = sh.wv[0], c = sh.wc[0];
+    for (int i = 1; i < kWide / 32; ++i)
+      if (before(sh.wv[i], sh.wc[i], v, c)) v = sh.wv[i], c = sh.wc[i];
+    __syncthreads();
+    if (lane == 0) value[t] = log_prob_of(v, m, l), label[t] = c;
+    last_v = v, last_c = c;
+  }
+}
+
+// A row as a few classes in front, vectors of 16 bytes, a few classes behind.
+template <typename T>
+struct RowShape {
+  static constexpr int V = 16 / (int)sizeof(T);
+  const T* x;
+  int n, head, vecs, behind;  // behind: first class after the vectors
+  __device__ __forceinline__ RowShape(const T* row, int classes) : x(row), n(classes) {
+    head = min(n, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+    vecs = (n - head) / V;
+    behind = head + vecs * V;
+  }
+  __device__ __forceinline__ const Vec<T, V>* vectors() const { return (const Vec<T, V>*)(x + head); }
+};
+
+// NV > 0: that many vectors a thread stay in registers; 0: the row is read again.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const __grid_constant__ LogProbParams p) {
+  __shared__ RowShared sh;
+  grid_dependency();
+  const int lane = threadIdx.x, w = lane >> 5;
+  const long long row = blockIdx.x;
+  const RowShape<T> r((const T*)p.x + row * p.batch_stride, p.classes);
+  constexpr int V = RowShape<T>::V;
+  const int y = label_at(p, row);
+  if (lane == 0) sh.count = 0;
+  // the odd ones: in front of the vectors (threads 0..) and behind them (threads 32..)
+  int odd_class = lane < r.head ? lane : lane >= 32 && r.behind + lane - 32 < r.n ? r.behind + lane - 32 : -1;
+  const float odd = odd_class >= 0 ? to_float(r.x[odd_class]) : -INFINITY;
+  const float given = y < 0 || lane ? 0.0f : to_float(r.x[y]);
   Online o;
-  float peak = -INFINITY;  // this thread's maximum, NaN above all
-  walk_row<T, LANES>(x, n, lane, [&](float v, int) {
-    if (!(v <= o.m)) o.raise(v != v || o.m == o.m ? v : o.m);
-    if (o.m != -INFINITY) o.add(v);
-    peak = above(v, peak) ? v : peak;
-  });
+  Vec<T, V> f[NV > 0 ? NV : 1];
+  if (NV > 0) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    Online b;
-    b.m = __shfl_xor_sync(~0u, o.m, d);
-    b.l = __shfl_xor_sync(~0u, o.l, d);
-    b.u = __shfl_xor_sync(~0u, o.u, d);
-    // the same two operands in the same order on both lanes, so that all lanes hold the same sums
-    if (lane & d) {
-      b.join(o);
-      o = b;
-    } else {
-      o.join(b);
+    for (int j = 0; j < NV; ++j) {
+      if (lane + j * kWide < r.vecs) {
+        f[j] = r.vectors()[lane + j * kWide];
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[j].v[k] = from_float<T>(-INFINITY);
+      }
+    }
+    o.m = odd;  // (fmaxf: NaN is not seen by the maximum, but by the sum)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) o.m = fmaxf(o.m, to_float(f[j].v[k]));
+  } else {
+    o.m = odd;
+    if (odd != -INFINITY) o.add(odd);
+#pragma unroll 4
+    for (int i = lane; i < r.vecs; i += kWide) {
+      const Vec<T, V> v = r.vectors()[i];
+      float m = to_float(v.v[0]);
+#pragma unroll
+      for (int k = 1; k < V; ++k) m = fmaxf(m, to_float(v.v[k]));
+      if (m > o.m) o.raise(m);
+      if (o.m != -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.add(to_float(v.v[k]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.m = to_float(v.v[k]) != to_float(v.v[k]) ? NAN : o.m;
+      }
     }
   }
-  if (LANES > 32) {
-    if ((lane & 31) == 0) sh.m[lane >> 5] = o.m, sh.l[lane >> 5] = o.l, sh.u[lane >> 5] = o.u;
+  float peak = o.m;
+  if (NV > 0) {
+    // maximum of the row, then the sums about it
+    float m = o.m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    if ((lane & 31) == 0) sh.m[w] = m;
     __syncthreads();
-    o.m = sh.m[0], o.l = sh.l[0], o.u = sh.u[0];
-    for (int w = 1; w < LANES / 32; ++w) {
+    m = sh.m[lane & 15];
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    o.m = m;
+    const float at = m == -INFINITY ? 0.0f : m;  // all -inf: the sums are 0, or NaN where there is one
+    o.m = at;
+    if (odd_class >= 0) o.add(odd);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * kWide < r.vecs) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.add(to_float(f[j].v[k]));
+      }
+    }
+    o.m = m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      o.l += __shfl_xor_sync(~0u, o.l, d);
+      o.u += __shfl_xor_sync(~0u, o.u, d);
+    }
+  } else {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
       Online b;
-      b.m = sh.m[w], b.l = sh.l[w], b.u = sh.u[w];
+      b.m = __shfl_xor_sync(~0u, o.m, d);
+      b.l = __shfl_xor_sync(~0u, o.l, d);
+      b.u = __shfl_xor_sync(~0u, o.u, d);
+      // the same two operands in the same order on both lanes, so that all lanes hold the same sums
+      if (lane & d) {
+        b.join(o);
+        o = b;
+      } else {
+        o.join(b);
+      }
+    }
+  }
+  // the parts' maxima: 16 neighbouring threads each
+#pragma unroll
+  for (int d = 8; d; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(~0u, peak, d));
+  if ((lane & 15) == 0) sh.peak[lane >> 4] = peak;
+  if ((lane & 31) == 0) {
+    if (NV == 0) sh.m[w] = o.m;
+    sh.l[w] = o.l, sh.u[w] = o.u;
+  }
+  __syncthreads();
+  if (NV > 0) {
+    o.l = o.u = 0.0f;
+    for (int i = 0; i < kWide / 32; ++i) o.l += sh.l[i], o.u += sh.u[i];
+    if (o.m == -INFINITY && o.l != o.l) o.m = NAN;
+  } else {
+    o.m = sh.m[0], o.l = sh.l[0], o.u = sh.u[0];
+    for (int i = 1; i < kWide / 32; ++i) {
+      Online b;
+      b.m = sh.m[i], b.l = sh.l[i], b.u = sh.u[i];
       o.join(b);
     }
   }
   if (lane == 0) {
-    const int y = label_at(p, row);
-    p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(to_float(x[y]), o);
+    p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
     p.entropy[row] = o.entropy();
     if (p.lse) p.lse[row] = o.lse();
-    sh.count = 0;
   }
   if (p.top == 0) return;
-  // the parts' maxima, and of them the one of rank top - 1 (equal ones by part); a part without classes counts as -inf
-#pragma unroll
-  for (int d = LANES / 64; d; d >>= 1) {
-    const float other = __shfl_xor_sync(~0u, peak, d);
-    peak = above(other, peak) ? other : peak;
-  }
-  if (lane % (LANES / 32) == 0) sh.peak[lane / (LANES / 32)] = peak;
-  row_sync<LANES>();
-  if (lane < 32) {
-    peak = sh.peak[lane];
-    int rank = 0;
-    for (int i = 0; i < 32; ++i) rank += before(sh.peak[i], i, peak, lane);
-    if (rank == p.top - 1) sh.pick_v = peak;
-  }
-  row_sync<LANES>();
-  const float bound = sh.pick_v;
-  walk_row<T, LANES>(x, n, lane, [&](float v, int c) {
-    if (!above(bound, v)) {
-      const int k = atomicAdd(&sh.count, 1);
-      if (k < kRoom) sh.cand[k] = v, sh.cand_class[k] = c;
-    }
-  });
-  row_sync<LANES>();
-  const int count = sh.count;
-  if (count <= kRoom) {
-    for (int i = lane; i < count; i += LANES) {
-      const float v = sh.cand[i];
-      const int c = sh.cand_class[i];
+  const auto put = [&](int t, float v, int c) {
+    p.top_value[row * p.top + t] = log_prob_of(v, o);
+    p.top_label[row * p.top + t] = c;
+  };
+  if (o.l == o.l) {
+    if (w == 0) {
+      // of the parts' maxima the one of rank top - 1 (equal ones by part); a part without classes counts as -inf
+      peak = sh.peak[lane];
       int rank = 0;
-      for (int j = 0; j < count; ++j) rank += before(sh.cand[j], sh.cand_class[j], v, c);
-      if (rank < p.top) {
-        p.top_value[row * p.top + rank] = log_prob_of(v, o);
-        p.top_label[row * p.top + rank] = c;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float other = __shfl_sync(~0u, peak, i);
+        rank += other > peak || (other == peak && i < lane);
       }
+      if (rank == p.top - 1) sh.bound = peak;
     }
-  } else {
-    float last_v = 0.0f;
-    int last_c = -1;
-    for (int t = 0; t < p.top; ++t) {
-      float v = -INFINITY;
-      int c = 0x7fffffff;
-      walk_row<T, LANES>(x, n, lane, [&](float w, int k) {
-        if ((t == 0 || before(last_v, last_c, w, k)) && before(w, k, v, c)) v = w, c = k;
-      });
-      best_of_row<LANES>(v, c, sh, lane);
-      if (lane == 0) {
-        p.top_value[row * p.top + t] = log_prob_of(v, o);
-        p.top_label[row * p.top + t] = c;
+    __syncthreads();
+    const float bound = sh.bound;
+    const auto offer = [&](float v, int c) {
+      if (v >= bound) {
+        const int k = atomicAdd(&sh.count, 1);
+        if (k < kRoom) sh.cand[k] = v, sh.cand_class[k] = c;
       }
-      last_v = v, last_c = c;
+    };
+    const auto offer_vector = [&](const Vec<T, V>& v, int first) {
+      float m = to_float(v.v[0]);
+#pragma unroll
+      for (int k = 1; k < V; ++k) m = fmaxf(m, to_float(v.v[k]));
+      if (m >= bound) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) offer(to_float(v.v[k]), first + k);
+      }
+    };
+    if (odd_class >= 0) offer(odd, odd_class);
+    if (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (lane + j * kWide < r.vecs) offer_vector(f[j], r.head + (lane + j * kWide) * V);
+    } else {
+#pragma unroll 4
+      for (int i = lane; i < r.vecs; i += kWide) offer_vector(r.vectors()[i], r.head + i * V);
+    }
+    __syncthreads();
+    const int count = sh.count;
+    if (count <= kRoom) {
+      for (int i = lane; i < count; i += kWide) {
+        const float v = sh.cand[i];
+        const int c = sh.cand_class[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += sh.cand[j] > v || (sh.cand[j] == v && sh.cand_class[j] < c);
+        if (rank < p.top) put(rank, v, c);
+      }
+      return;
     }
   }
+  pick_row(r.x, r.n, p.top, p.top_value + row * p.top, p.top_label + row * p.top, o.m, o.l, sh);
 }
 
-template <typename T, int LANES>
-__global__ void __launch_bounds__(LANES == 32 ? 128 : LANES) logprob_rows_bwd(const __grid_constant__ LogProbParams p) {
-  constexpr int kRows = LANES == 32 ? 4 : 1;
+template <typename T>
+__global__ void __launch_bounds__(kWide) logprob_row_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const int lane = LANES == 32 ? threadIdx.x & 31 : threadIdx.x, mine = LANES == 32 ? threadIdx.x >> 5 : 0;
-  const long long row = (long long)blockIdx.x * kRows + mine;
-  if (row >= p.batch) return;
-  const T* x = (const T*)p.x + row * p.batch_stride;
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;
+  const RowShape<T> r((const T*)p.x + row * p.batch_stride, p.classes);
   T* g = (T*)p.grad + row * p.grad_batch_stride;
-  const int n = p.classes;
   const Slope q = slope_at(p, row);
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = RowShape<T>::V;
+  const auto one = [&](int c) {
+    const float v = q.at(to_float(r.x[c])) + (c == q.label ? q.a : 0.0f);
+    g[c] = from_float<T>(q.empty() ? 0.0f : v);
+  };
   // vectors where scores and gradient have the same alignment
-  if (LANES > 32 && (((uintptr_t)x ^ (uintptr_t)g) & 15) == 0) {
-    const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), vecs = (n - head) / V;
-    if (lane < head) g[lane] = from_float<T>(q.at(to_float(x[lane]), lane));
+  if ((((uintptr_t)r.x ^ (uintptr_t)g) & 15) != 0) {
 #pragma unroll 4
-    for (int i = lane; i < vecs; i += LANES) {
-      const Vec<T, V> w = ((const Vec<T, V>*)(x + head))[i];
-      Vec<T, V> r;
-#pragma unroll
-      for (int k = 0; k < V; ++k) r.v[k] = from_float<T>(q.at(to_float(w.v[k]), head + i * V + k));
-      ((Vec<T, V>*)(g + head))[i] = r;
-    }
-    for (int c = head + vecs * V + lane; c < n; c += LANES) g[c] = from_float<T>(q.at(to_float(x[c]), c));
+    for (int c = lane; c < r.n; c += kWide) one(c);
     return;
   }
-  for (int c = lane; c < n; c += LANES) g[c] = from_float<T>(q.at(to_float(x[c]), c));
+  if (lane < r.head) one(lane);
+  if (r.behind + lane < r.n) one(r.behind + lane);
+  const int vector_of_label = q.label < r.head || q.label >= r.behind ? -1 : (q.label - r.head) / V;
+#pragma unroll 4
+  for (int i = lane; i < r.vecs; i += kWide) {
+    const Vec<T, V> v = r.vectors()[i];
+    Vec<T, V> to;
+    float f[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = q.at(to_float(v.v[k]));
+    if (i == vector_of_label) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] += r.head + i * V + k == q.label ? q.a : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) to.v[k] = from_float<T>(q.empty() ? 0.0f : f[k]);
+    ((Vec<T, V>*)(g + r.head))[i] = to;
+  }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------
 // 0, or 1: more CTAs than a grid has.
+template <typename T, int V, int TOP>
+void launch_apart_fwd(const LogProbParams& p, cudaStream_t st) {
+  const dim3 grid((unsigned)(((p.space + V - 1) / V * p.batch + kApartThreads - 1) / kApartThreads));
+  if (p.classes <= 4) launch_dependent(logprob_apart_fwd<T, V, TOP, 4>, grid, kApartThreads, 0, st, p);
+  else if (p.classes <= 16) launch_dependent(logprob_apart_fwd<T, V, TOP, 16>, grid, kApartThreads, 0, st, p);
+  else launch_dependent(logprob_apart_fwd<T, V, TOP, 0>, grid, kApartThreads, 0, st, p);
+}
 template <typename T, int V>
-int launch_logprob_apart(const LogProbParams& p, bool fwd, cudaStream_t st) {
-  const long long items = (p.space + V - 1) / V * p.batch, ctas = (items + kApartThreads - 1) / kApartThreads;
-  if (ctas > 0x7fffffffLL) return 1;
-  const dim3 grid((unsigned)ctas);
-  if (!fwd) launch_dependent(logprob_apart_bwd<T, V>, grid, kApartThreads, 0, st, p);
-  else if (p.top == 0) launch_dependent(logprob_apart_fwd<T, V, 0>, grid, kApartThreads, 0, st, p);
-  else if (p.top <= 2) launch_dependent(logprob_apart_fwd<T, V, 2>, grid, kApartThreads, 0, st, p);
-  else if (p.top <= 5) launch_dependent(logprob_apart_fwd<T, 1, 5>, dim3((unsigned)((p.space * p.batch + kApartThreads - 1) / kApartThreads)), kApartThreads, 0, st, p);
-  else launch_dependent(logprob_apart_fwd<T, 1, 16>, dim3((unsigned)((p.space * p.batch + kApartThreads - 1) / kApartThreads)), kApartThreads, 0, st, p);
-  return 0;
+void launch_logprob_apart(const LogProbParams& p, bool fwd, cudaStream_t st) {
+  if (!fwd)
+    launch_dependent(logprob_apart_bwd<T, V>, dim3((unsigned)(((p.space + V - 1) / V * p.batch + kApartThreads - 1) / kApartThreads)),
+                     kApartThreads, 0, st, p);
+  else if (p.top == 0) launch_apart_fwd<T, V, 0>(p, st);
+  else if (p.top <= 2) launch_apart_fwd<T, V, 2>(p, st);
+  else if (p.top <= 5) launch_apart_fwd<T, 1, 5>(p, st);
+  else launch_apart_fwd<T, 1, 16>(p, st);
 }
 
 template <typename T>
 int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
   if (p.class_stride == 1 && p.space == 1) {
+    const long long ctas = p.classes <= 1024 ? (p.batch + 3) / 4 : p.batch;
+    if (ctas > 0x7fffffffLL) return 1;
+    const dim3 grid((unsigned)ctas);
+    // vectors of a thread, if the row is to stay in registers (one more where it starts between two)
+    const long long vecs = (p.classes / RowShape<T>::V + kWide - 1) / kWide;
     if (p.classes <= 1024) {
-      const long long ctas = (p.batch + 3) / 4;
-      if (ctas > 0x7fffffffLL) return 1;
-      if (fwd) launch_dependent(logprob_rows_fwd<T, 32>, dim3((unsigned)ctas), 128, 0, st, p);
-      else launch_dependent(logprob_rows_bwd<T, 32>, dim3((unsigned)ctas), 128, 0, st, p);
+      if (!fwd) launch_dependent(logprob_warp_bwd<T>, grid, 128, 0, st, p);
+      else if (p.classes <= 128) launch_dependent(logprob_warp_fwd<T, 4>, grid, 128, 0, st, p);
+      else launch_dependent(logprob_warp_fwd<T, 32>, grid, 128, 0, st, p);
+    } else if (!fwd) {
+      launch_dependent(logprob_row_bwd<T>, grid, kWide, 0, st, p);
+    } else if (vecs <= 2) {
+      launch_dependent(logprob_row_fwd<T, 2>, grid, kWide, 0, st, p);
+    } else if (vecs <= 8) {
+      launch_dependent(logprob_row_fwd<T, 8>, grid, kWide, 0, st, p);
+    } else if (vecs <= 16) {
+      launch_dependent(logprob_row_fwd<T, 16>, grid, kWide, 0, st, p);
     } else {
-      if (p.batch > 0x7fffffffLL) return 1;
-      if (fwd) launch_dependent(logprob_rows_fwd<T, kWide>, dim3((unsigned)p.batch), kWide, 0, st, p);
-      else launch_dependent(logprob_rows_bwd<T, kWide>, dim3((unsigned)p.batch), kWide, 0, st, p);
+      launch_dependent(logprob_row_fwd<T, 0>, grid, kWide, 0, st, p);
     }
     return 0;
   }
@@ -469,8 +706,9 @@ int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
   constexpr int V = 8 / (int)sizeof(T);
   const long long strides = p.batch_stride | p.class_stride | (fwd ? 0 : p.grad_batch_stride | p.grad_class_stride);
   const uintptr_t at = (uintptr_t)p.x | (fwd ? 0 : (uintptr_t)p.grad);
-  if (strides % V == 0 && at % 8 == 0) return launch_logprob_apart<T, V>(p, fwd, st);
-  return launch_logprob_apart<T, 1>(p, fwd, st);
+  if (strides % V == 0 && at % 8 == 0) launch_logprob_apart<T, V>(p, fwd, st);
+  else launch_logprob_apart<T, 1>(p, fwd, st);
+  return 0;
 }
 
 }  // namespace mvr
