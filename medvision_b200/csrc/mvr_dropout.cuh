@@ -28,7 +28,7 @@ struct DropoutParams {
   const void* residual;  // or null
   void* out;
   long long n;
-  unsigned cut;          // an element stays when its 16 bits are >= cut; 65536: none stays
+  unsigned floor;        // an element stays when its 16 bits, as the upper half of a word, are >= this
   float scale;
   PhiloxKeys keys;       // constants of the launch, so that a round is two products and two three-way exclusive ors
   unsigned long long offset;
@@ -87,8 +87,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const __grid_cons
     const unsigned word[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      // the high half is compared in place: its word is >= cut * 2^16 when the half is >= cut
-      const bool stays = (k & 1) ? word[k >> 1] >= (p.cut << 16) && p.cut < 65536 : (word[k >> 1] & 0xffffu) >= p.cut;
+      const bool stays = ((k & 1) ? word[k >> 1] : word[k >> 1] << 16) >= p.floor;
       // a dropped element gives 0 whatever it held, NaN and infinities included
       float v = stays ? to_float(xv[i][k / kPart].v[k % kPart]) * p.scale : 0.0f;
       if (RESIDUAL) v += to_float(rv[i][k / kPart].v[k % kPart]);

@@ -350,12 +350,19 @@ int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64
   if (!x || !out) return MVR_ERR_NULL;
   DropoutParams p = {};
   p.x = x; p.residual = residual; p.out = out; p.n = n;
-  p.cut = (unsigned)std::floor(probability * 65536.0 + 0.5);
-  p.scale = p.cut < 65536 ? (float)(65536.0 / (65536.0 - p.cut)) : 0.0f;
+  const int cut = (int)std::floor(probability * 65536.0 + 0.5);  // an element stays when its 16 bits are >= cut
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (cut == 65536) {  // none does
+    const size_t bytes = (size_t)n * (dtype == MVR_F32 ? 4 : 2);
+    const cudaError_t e = residual ? cudaMemcpyAsync(out, residual, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(out, 0, bytes, st);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e == cudaSuccess ? MVR_OK : MVR_ERR_LAUNCH;
+  }
+  p.floor = (unsigned)cut << 16;
+  p.scale = (float)(65536.0 / (65536.0 - cut));
   p.keys.from(seed);
   p.seed_at = (const unsigned long long*)seed_at;
   p.offset = offset;
-  const cudaStream_t st = (cudaStream_t)stream;
   const int rc = dtype == MVR_F32 ? launch_dropout<float>(p, st) : dtype == MVR_F16 ? launch_dropout<__half>(p, st)
                                                                                     : launch_dropout<__nv_bfloat16>(p, st);
   return rc ? MVR_ERR_TOO_LARGE : launched();

@@ -92,6 +92,18 @@ struct Online {
 __device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2f(l) * kLn2; }
 __device__ __forceinline__ float log_prob_of(float x, const Online& o) { return log_prob_of(x, o.m, o.l); }
 
+// (l, u) of pairs of scores about fixed maxima.
+struct Sums2 {
+  float2 l = make_float2(0.0f, 0.0f), u = make_float2(0.0f, 0.0f);
+  __device__ __forceinline__ void add(float2 x, float2 minus_m) {
+    // (a score of -inf adds 0 to both: its distance is kept finite)
+    const float2 d = add2(x, minus_m), t = mul2(d, make_float2(kLog2e, kLog2e));
+    const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+    l = add2(l, e);
+    u = fma2(make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), e, u);
+  }
+};
+
 // Order of the alternatives: NaN first, then the larger score; equal ones by class.
 __device__ __forceinline__ bool above(float a, float b) { return a > b || (a != a && b == b); }
 __device__ __forceinline__ bool before(float a, int ia, float b, int ib) {
@@ -146,76 +158,65 @@ struct Best<0> {
   __device__ __forceinline__ void offer(float, int) {}
 };
 
-// A thread takes V consecutive positions of one batch item.  CACHE: number of classes that stay in registers (0: eight at a time,
-// the maximum of eight moves the sums once).
-template <typename T, int V, int TOP, int CACHE>
-__global__ void __launch_bounds__(kApartThreads) logprob_apart_fwd(const __grid_constant__ LogProbParams p) {
+// A thread takes two consecutive positions of one batch item (PAIR: they are loaded and stored together).  CACHE: number of classes
+// that stay in registers (0: eight at a time, the maximum of eight moves the sums once).
+template <typename T, bool PAIR, int TOP, int CACHE>
+__global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 : 4) logprob_apart_fwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const long long per_item = (p.space + V - 1) / V, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
+  const long long per_item = (p.space + 1) / 2, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
   if (item >= per_item * p.batch) return;
-  const long long b = item / per_item, s = (item - b * per_item) * V;
+  const long long b = item / per_item, s = (item - b * per_item) * 2;
   const T* x = (const T*)p.x + b * p.batch_stride + s;
-  const int n = (int)(p.space - s < V ? p.space - s : V);
+  const bool second = s + 1 < p.space;
   const long long at = b * p.space + s;
   constexpr int kStep = CACHE > 0 ? CACHE : 8;
-  Online o[V];
-  Best<TOP> best[V];
-  float given[V];
-  int label[V];
+  const int label[2] = {label_at(p, at), second ? label_at(p, at + 1) : -1};
+  float given[2];
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    given[k] = 0.0f;
-    label[k] = k < n ? label_at(p, at + k) : -1;
-  }
+  for (int k = 0; k < 2; ++k) given[k] = label[k] >= 0 ? to_float(x[(long long)label[k] * p.class_stride + k]) : 0.0f;
+  Online o[2];
+  Best<TOP> best[2];
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
-    Vec<T, V> w[kStep];
+    Two<T> w[kStep];
 #pragma unroll
     for (int j = 0; j < kStep; ++j) {
+      w[j] = both<T>(-INFINITY);  // classes that are not there
       if (c0 + j < p.classes) {
         const T* q = x + (long long)(c0 + j) * p.class_stride;
-        if (n == V) {
-          w[j] = *(const Vec<T, V>*)q;
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) w[j].v[k] = k < n ? q[k] : from_float<T>(0.0f);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) w[j].v[k] = from_float<T>(-INFINITY);
+        if (PAIR) w[j] = *(const Two<T>*)q;
+        else w[j] = rounded<T>(make_float2(to_float(q[0]), second ? to_float(q[1]) : 0.0f));
       }
     }
+    Two<T> most = w[0];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      float m = o[k].m;
+    for (int j = 1; j < kStep; ++j) most = larger(most, w[j]);
+    const float2 m2 = floats(most);
+    float m[2] = {fmaxf(m2.x, o[0].m), fmaxf(m2.y, o[1].m)};
 #pragma unroll
-      for (int j = 0; j < kStep; ++j) m = fmaxf(m, to_float(w[j].v[k]));
-      if (m == -INFINITY) {  // nothing yet; NaN is not seen by the maximum
+    for (int k = 0; k < 2; ++k) {
+      if (CACHE == 0 && m[k] != o[k].m) o[k].raise(m[k]);
+      o[k].m = m[k];
+    }
+    // (nothing but -inf so far: about 0, which leaves the sums 0, or makes them NaN where there is one)
+    const float2 minus = make_float2(m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]);
+    Sums2 sum;
 #pragma unroll
-        for (int j = 0; j < kStep; ++j) m = to_float(w[j].v[k]) != to_float(w[j].v[k]) ? NAN : m;
-      }
-      if (m != -INFINITY) {
-        o[k].raise(m);
-#pragma unroll
-        for (int j = 0; j < kStep; ++j) {
-          if (CACHE == 0 || j < p.classes) o[k].add(to_float(w[j].v[k]));
-        }
-      }
+    for (int j = 0; j < kStep; ++j) sum.add(floats(w[j]), minus);
+    o[0].l += sum.l.x, o[1].l += sum.l.y;
+    o[0].u += sum.u.x, o[1].u += sum.u.y;
+    if constexpr (TOP > 0) {
 #pragma unroll
       for (int j = 0; j < kStep; ++j) {
-        if (CACHE == 0 || j < p.classes) {
-          const float f = to_float(w[j].v[k]);
-          if (c0 + j < p.classes) best[k].offer(f, c0 + j);
-          given[k] = label[k] == c0 + j ? f : given[k];
-        }
+        const float2 f = floats(w[j]);
+        best[0].offer(f.x, c0 + j);
+        best[1].offer(f.y, c0 + j);
       }
     }
   }
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    if (k >= n) break;
-    p.log_prob[at + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
-    p.entropy[at + k] = o[k].entropy();
-    if (p.lse) p.lse[at + k] = o[k].lse();
+  for (int k = 0; k < 2; ++k) {
+    if (o[k].l != o[k].l) o[k].m = NAN;
+    if (k == 1 && !second) break;
     if constexpr (TOP > 0) {
       float* value = p.top_value + b * p.top * p.space + s + k;
       int* best_label = p.top_label + b * p.top * p.space + s + k;
@@ -230,6 +231,9 @@ __global__ void __launch_bounds__(kApartThreads) logprob_apart_fwd(const __grid_
         pick_apart(x + k, p.class_stride, p.classes, p.top, p.space, value, best_label, o[k].m, o[k].l);
       }
     }
+    p.log_prob[at + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
+    p.entropy[at + k] = o[k].entropy();
+    if (p.lse) p.lse[at + k] = o[k].lse();
   }
 }
 
@@ -256,48 +260,43 @@ __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
   return s;
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kApartThreads) logprob_apart_bwd(const __grid_constant__ LogProbParams p) {
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const long long per_item = (p.space + V - 1) / V, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
+  const long long per_item = (p.space + 1) / 2, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
   if (item >= per_item * p.batch) return;
-  const long long b = item / per_item, s = (item - b * per_item) * V;
+  const long long b = item / per_item, s = (item - b * per_item) * 2;
   const T* x = (const T*)p.x + b * p.batch_stride + s;
   T* g = (T*)p.grad + b * p.grad_batch_stride + s;
-  const int n = (int)(p.space - s < V ? p.space - s : V);
-  Slope q[V];
+  const bool second = s + 1 < p.space;
+  const Slope q[2] = {slope_at(p, b * p.space + s), slope_at(p, b * p.space + s + (second ? 1 : 0))};
+  constexpr int kStep = 8;
+  for (int c0 = 0; c0 < p.classes; c0 += kStep) {
+    Two<T> w[kStep];
 #pragma unroll
-  for (int k = 0; k < V; ++k) q[k] = slope_at(p, b * p.space + s + (k < n ? k : 0));
-  for (int c0 = 0; c0 < p.classes; c0 += 8) {
-    Vec<T, V> w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kStep; ++j) {
       if (c0 + j < p.classes) {
         const T* xc = x + (long long)(c0 + j) * p.class_stride;
-        if (n == V) {
-          w[j] = *(const Vec<T, V>*)xc;
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) w[j].v[k] = xc[k < n ? k : 0];
-        }
+        if (PAIR) w[j] = *(const Two<T>*)xc;
+        else w[j] = rounded<T>(make_float2(to_float(xc[0]), to_float(xc[second ? 1 : 0])));
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kStep; ++j) {
       if (c0 + j < p.classes) {
         T* gc = g + (long long)(c0 + j) * p.grad_class_stride;
-        Vec<T, V> r;
+        const float2 f = floats(w[j]);
+        float r[2] = {q[0].at(f.x), q[1].at(f.y)};
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float v = q[k].at(to_float(w[j].v[k])) + (c0 + j == q[k].label ? q[k].a : 0.0f);
-          r.v[k] = from_float<T>(q[k].empty() ? 0.0f : v);
+        for (int k = 0; k < 2; ++k) {
+          if (c0 + j == q[k].label) r[k] += q[k].a;
+          if (q[k].empty()) r[k] = 0.0f;
         }
-        if (n == V) {
-          *(Vec<T, V>*)gc = r;
+        if (PAIR) {
+          *(Two<T>*)gc = rounded<T>(make_float2(r[0], r[1]));
         } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (k < n) gc[k] = r.v[k];
+          gc[0] = from_float<T>(r[0]);
+          if (second) gc[1] = from_float<T>(r[1]);
         }
       }
     }
@@ -438,6 +437,19 @@ struct RowShape {
   __device__ __forceinline__ const Vec<T, V>* vectors() const { return (const Vec<T, V>*)(x + head); }
 };
 
+// The vectors' elements as pairs.
+template <typename T>
+struct alignas(16) Pairs {
+  static constexpr int N = 8 / (int)sizeof(T);
+  Two<T> v[N];
+  __device__ __forceinline__ Two<T> most() const {
+    Two<T> m = v[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = larger(m, v[k]);
+    return m;
+  }
+};
+
 // NV > 0: that many vectors a thread stay in registers; 0: the row is read again.
 template <typename T, int NV>
 __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const __grid_constant__ LogProbParams p) {
@@ -447,47 +459,48 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
   const long long row = blockIdx.x;
   const RowShape<T> r((const T*)p.x + row * p.batch_stride, p.classes);
   constexpr int V = RowShape<T>::V;
+  typedef Pairs<T> P;
+  const P* vectors = (const P*)r.vectors();
   const int y = label_at(p, row);
   if (lane == 0) sh.count = 0;
   // the odd ones: in front of the vectors (threads 0..) and behind them (threads 32..)
-  int odd_class = lane < r.head ? lane : lane >= 32 && r.behind + lane - 32 < r.n ? r.behind + lane - 32 : -1;
+  const int odd_class = lane < r.head ? lane : lane >= 32 && r.behind + lane - 32 < r.n ? r.behind + lane - 32 : -1;
   const float odd = odd_class >= 0 ? to_float(r.x[odd_class]) : -INFINITY;
   const float given = y < 0 || lane ? 0.0f : to_float(r.x[y]);
   Online o;
-  Vec<T, V> f[NV > 0 ? NV : 1];
+  P f[NV > 0 ? NV : 1];
   if (NV > 0) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (lane + j * kWide < r.vecs) {
-        f[j] = r.vectors()[lane + j * kWide];
+        f[j] = vectors[lane + j * kWide];
       } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) f[j].v[k] = from_float<T>(-INFINITY);
+        for (int k = 0; k < P::N; ++k) f[j].v[k] = both<T>(-INFINITY);
       }
     }
-    o.m = odd;  // (fmaxf: NaN is not seen by the maximum, but by the sum)
+    Two<T> most = f[0].most();
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < V; ++k) o.m = fmaxf(o.m, to_float(f[j].v[k]));
+    for (int j = 1; j < NV; ++j) most = larger(most, f[j].most());
+    const float2 m = floats(most);
+    o.m = fmaxf(odd, fmaxf(m.x, m.y));  // (NaN is not seen by the maximum, but by the sum)
   } else {
     o.m = odd;
     if (odd != -INFINITY) o.add(odd);
 #pragma unroll 4
     for (int i = lane; i < r.vecs; i += kWide) {
-      const Vec<T, V> v = r.vectors()[i];
-      float m = to_float(v.v[0]);
-#pragma unroll
-      for (int k = 1; k < V; ++k) m = fmaxf(m, to_float(v.v[k]));
+      const P v = vectors[i];
+      const float2 m2 = floats(v.most());
+      const float m = fmaxf(m2.x, m2.y);
       if (m > o.m) o.raise(m);
-      if (o.m != -INFINITY) {
+      const float minus = o.m == -INFINITY ? 0.0f : -o.m;
+      Sums2 sum;
 #pragma unroll
-        for (int k = 0; k < V; ++k) o.add(to_float(v.v[k]));
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) o.m = to_float(v.v[k]) != to_float(v.v[k]) ? NAN : o.m;
-      }
+      for (int k = 0; k < P::N; ++k) sum.add(floats(v.v[k]), make_float2(minus, minus));
+      o.l += sum.l.x + sum.l.y;
+      o.u += sum.u.x + sum.u.y;
     }
+    if (o.l != o.l) o.m = NAN;
   }
   float peak = o.m;
   if (NV > 0) {
@@ -500,18 +513,19 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
     m = sh.m[lane & 15];
 #pragma unroll
     for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-    o.m = m;
-    const float at = m == -INFINITY ? 0.0f : m;  // all -inf: the sums are 0, or NaN where there is one
-    o.m = at;
-    if (odd_class >= 0) o.add(odd);
+    const float minus = m == -INFINITY ? 0.0f : -m;  // all -inf: the sums are 0, or NaN where there is one
+    Sums2 sum;
+    if (odd_class >= 0) sum.add(make_float2(odd, -INFINITY), make_float2(minus, minus));
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j * kWide < r.vecs) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) o.add(to_float(f[j].v[k]));
+        for (int k = 0; k < P::N; ++k) sum.add(floats(f[j].v[k]), make_float2(minus, minus));
       }
     }
     o.m = m;
+    o.l = sum.l.x + sum.l.y;
+    o.u = sum.u.x + sum.u.y;
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
       o.l += __shfl_xor_sync(~0u, o.l, d);
@@ -545,7 +559,7 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
   if (NV > 0) {
     o.l = o.u = 0.0f;
     for (int i = 0; i < kWide / 32; ++i) o.l += sh.l[i], o.u += sh.u[i];
-    if (o.m == -INFINITY && o.l != o.l) o.m = NAN;
+    if (o.l != o.l) o.m = NAN;
   } else {
     o.m = sh.m[0], o.l = sh.l[0], o.u = sh.u[0];
     for (int i = 1; i < kWide / 32; ++i) {
@@ -584,13 +598,15 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
         if (k < kRoom) sh.cand[k] = v, sh.cand_class[k] = c;
       }
     };
-    const auto offer_vector = [&](const Vec<T, V>& v, int first) {
-      float m = to_float(v.v[0]);
+    const auto offer_vector = [&](const P& v, int first) {
+      const float2 m = floats(v.most());
+      if (fmaxf(m.x, m.y) >= bound) {
 #pragma unroll
-      for (int k = 1; k < V; ++k) m = fmaxf(m, to_float(v.v[k]));
-      if (m >= bound) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) offer(to_float(v.v[k]), first + k);
+        for (int k = 0; k < P::N; ++k) {
+          const float2 e = floats(v.v[k]);
+          offer(e.x, first + 2 * k);
+          offer(e.y, first + 2 * k + 1);
+        }
       }
     };
     if (odd_class >= 0) offer(odd, odd_class);
@@ -600,7 +616,7 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
         if (lane + j * kWide < r.vecs) offer_vector(f[j], r.head + (lane + j * kWide) * V);
     } else {
 #pragma unroll 4
-      for (int i = lane; i < r.vecs; i += kWide) offer_vector(r.vectors()[i], r.head + i * V);
+      for (int i = lane; i < r.vecs; i += kWide) offer_vector(vectors[i], r.head + i * V);
     }
     __syncthreads();
     const int count = sh.count;
@@ -622,7 +638,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWide) logprob_row_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const int lane = threadIdx.x;
-  const long long row = blockIdx.x;
+  const long long row = gridDim.x - 1 - blockIdx.x;  // backwards: the rows that the forward read last are still in L2
   const RowShape<T> r((const T*)p.x + row * p.batch_stride, p.classes);
   T* g = (T*)p.grad + row * p.grad_batch_stride;
   const Slope q = slope_at(p, row);
@@ -659,22 +675,20 @@ __global__ void __launch_bounds__(kWide) logprob_row_bwd(const __grid_constant__
 
 // ---- launches ----------------------------------------------------------------------------------------
 // 0, or 1: more CTAs than a grid has.
-template <typename T, int V, int TOP>
-void launch_apart_fwd(const LogProbParams& p, cudaStream_t st) {
-  const dim3 grid((unsigned)(((p.space + V - 1) / V * p.batch + kApartThreads - 1) / kApartThreads));
-  if (p.classes <= 4) launch_dependent(logprob_apart_fwd<T, V, TOP, 4>, grid, kApartThreads, 0, st, p);
-  else if (p.classes <= 16) launch_dependent(logprob_apart_fwd<T, V, TOP, 16>, grid, kApartThreads, 0, st, p);
-  else launch_dependent(logprob_apart_fwd<T, V, TOP, 0>, grid, kApartThreads, 0, st, p);
+template <typename T, bool PAIR, int TOP>
+void launch_apart_fwd(const LogProbParams& p, dim3 grid, cudaStream_t st) {
+  // (with more than two alternatives the registers hold those)
+  if (TOP <= 2 && p.classes <= 8) launch_dependent(logprob_apart_fwd<T, PAIR, TOP, TOP <= 2 ? 8 : 0>, grid, kApartThreads, 0, st, p);
+  else if (TOP <= 2 && p.classes <= 16) launch_dependent(logprob_apart_fwd<T, PAIR, TOP, TOP <= 2 ? 16 : 0>, grid, kApartThreads, 0, st, p);
+  else launch_dependent(logprob_apart_fwd<T, PAIR, TOP, 0>, grid, kApartThreads, 0, st, p);
 }
-template <typename T, int V>
-void launch_logprob_apart(const LogProbParams& p, bool fwd, cudaStream_t st) {
-  if (!fwd)
-    launch_dependent(logprob_apart_bwd<T, V>, dim3((unsigned)(((p.space + V - 1) / V * p.batch + kApartThreads - 1) / kApartThreads)),
-                     kApartThreads, 0, st, p);
-  else if (p.top == 0) launch_apart_fwd<T, V, 0>(p, st);
-  else if (p.top <= 2) launch_apart_fwd<T, V, 2>(p, st);
-  else if (p.top <= 5) launch_apart_fwd<T, 1, 5>(p, st);
-  else launch_apart_fwd<T, 1, 16>(p, st);
+template <typename T, bool PAIR>
+void launch_logprob_apart(const LogProbParams& p, bool fwd, dim3 grid, cudaStream_t st) {
+  if (!fwd) launch_dependent(logprob_apart_bwd<T, PAIR>, grid, kApartThreads, 0, st, p);
+  else if (p.top == 0) launch_apart_fwd<T, PAIR, 0>(p, grid, st);
+  else if (p.top <= 2) launch_apart_fwd<T, PAIR, 2>(p, grid, st);
+  else if (p.top <= 5) launch_apart_fwd<T, PAIR, 5>(p, grid, st);
+  else launch_apart_fwd<T, PAIR, 16>(p, grid, st);
 }
 
 template <typename T>
@@ -702,12 +716,12 @@ int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
     }
     return 0;
   }
-  if (p.space * p.batch > 0x7fffffffLL * kApartThreads) return 1;
-  constexpr int V = 8 / (int)sizeof(T);
-  const long long strides = p.batch_stride | p.class_stride | (fwd ? 0 : p.grad_batch_stride | p.grad_class_stride);
+  const long long ctas = ((p.space + 1) / 2 * p.batch + kApartThreads - 1) / kApartThreads;
+  if (ctas > 0x7fffffffLL) return 1;
+  const long long strides = p.space | p.batch_stride | p.class_stride | (fwd ? 0 : p.grad_batch_stride | p.grad_class_stride);
   const uintptr_t at = (uintptr_t)p.x | (fwd ? 0 : (uintptr_t)p.grad);
-  if (strides % V == 0 && at % 8 == 0) launch_logprob_apart<T, V>(p, fwd, st);
-  else launch_logprob_apart<T, 1>(p, fwd, st);
+  if (strides % 2 == 0 && at % (2 * sizeof(T)) == 0) launch_logprob_apart<T, true>(p, fwd, dim3((unsigned)ctas), st);
+  else launch_logprob_apart<T, false>(p, fwd, dim3((unsigned)ctas), st);
   return 0;
 }
 
