@@ -201,37 +201,51 @@ attn_plan(const void* index, int type, long long stride, int R, int N, int rows_
 }
 
 // ---- joining of parts ---------------------------------------------------------------------------------
-// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s of the parts' maxima, sums and unscaled outputs.  One warp a row.
-template <typename T>
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s of the parts' maxima, sums and unscaled outputs.  A thread takes W columns of
+// a row.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) attn_join(const __grid_constant__ AttnParams p) {
   grid_dependency();
-  const long long rows = (long long)p.R * p.T * p.Hq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)p.R * p.T * p.Hq, at = (long long)blockIdx.x * 256 + threadIdx.x, row = at / (p.D / W);
+  const int d = (int)(at - row * (p.D / W)) * W;
   if (row >= rows) return;
-  float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[(s * rows + row) * 2]);
+  const float2* ml = (const float2*)p.part_ml + row;
+  float m = -INFINITY, l = 0.0f, o[W] = {};
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows].x);
   const float ref = m == -INFINITY ? 0.0f : m;
-  for (int s = 0; s < p.splits; ++s) l += exp2f(p.part_ml[(s * rows + row) * 2] - ref) * p.part_ml[(s * rows + row) * 2 + 1];
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int d = lane; d < p.D; d += 32) {
-    float o = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float w = exp2f(p.part_ml[(s * rows + row) * 2] - ref);
-      if (w != 0.0f) o += w * p.part_o[(s * rows + row) * p.D + d];
-    }
-    ((T*)p.out)[row * p.D + d] = from_float<T>(o * inv);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 v = ml[s * rows];
+    const float w = exp2f(v.x - ref);
+    const Vec<float, W> part = *(const Vec<float, W>*)(p.part_o + (s * rows + row) * p.D + d);
+    l += w * v.y;
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] += w * part.v[i];
   }
-  if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : ref + log2f(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  Vec<T, W> out;
+#pragma unroll
+  for (int i = 0; i < W; ++i) out.v[i] = from_float<T>(o[i] * inv);
+  *(Vec<T, W>*)((T*)p.out + row * p.D + d) = out;
+  if (p.lse && d == 0) p.lse[row] = l == 0.0f ? -INFINITY : ref + log2f(l);
 }
 
-// dst[i] = factor * sum over the parts, in order.
-template <typename T>
+// dst[i] = factor * sum over the parts, in order.  A thread takes W elements at a time.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) attn_sum(const float* part, T* dst, long long n, int parts, float factor) {
   grid_dependency();
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int s = 0; s < parts; ++s) v += part[s * n + i];
-    dst[i] = from_float<T>(v * factor);
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * W; i < n; i += (long long)gridDim.x * 256 * W) {
+    float v[W] = {};
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+      const Vec<float, W> x = *(const Vec<float, W>*)(part + s * n + i);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] += x.v[k];
+    }
+    Vec<T, W> out;
+#pragma unroll
+    for (int k = 0; k < W; ++k) out.v[k] = from_float<T>(v[k] * factor);
+    *(Vec<T, W>*)(dst + i) = out;
   }
 }
 

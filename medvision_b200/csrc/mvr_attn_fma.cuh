@@ -81,9 +81,21 @@ __device__ __forceinline__ void fma_put(float* w, const float (&v)[FmaTile<DP>::
 template <typename T, int DP>
 __device__ __forceinline__ void fma_load_states(float* dst, const T* src, long long stride, int first, const float* allowed, int D) {
   typedef FmaTile<DP> F;
-  for (int e = threadIdx.x; e < F::BT * DP; e += kFmaThreads) {
-    const int j = e / DP, d = e % DP;
-    dst[j * F::LD + d] = allowed[j] != 0.0f && d < D ? to_float(src[(long long)(first + j) * stride + d]) : 0.0f;
+  constexpr int U = 8;  // loads under way together; those of elements left out go to the first one
+  for (int e0 = threadIdx.x; e0 < F::BT * DP; e0 += U * kFmaThreads) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kFmaThreads, j = e / DP, d = e % DP;
+      const bool in = allowed[j] != 0.0f && d < D;
+      const float x = to_float(src[in ? (long long)(first + j) * stride + d : 0]);
+      v[u] = in ? x : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kFmaThreads;
+      dst[e / DP * F::LD + e % DP] = v[u];
+    }
   }
 }
 // Where the rows of a tile lie: offsets into queries and gradient, and row numbers (-1: no row).
@@ -106,9 +118,21 @@ struct FmaRows {
 template <typename T, int DP>
 __device__ __forceinline__ void fma_load_rows(float* dst, const T* src, const long long* at, const long long* number, int D) {
   typedef FmaTile<DP> F;
-  for (int e = threadIdx.x; e < F::BT * DP; e += kFmaThreads) {
-    const int j = e / DP, d = e % DP;
-    dst[j * F::LD + d] = number[j] >= 0 && d < D ? to_float(src[at[j] + d]) : 0.0f;
+  constexpr int U = 8;
+  for (int e0 = threadIdx.x; e0 < F::BT * DP; e0 += U * kFmaThreads) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kFmaThreads, j = e / DP, d = e % DP;
+      const bool in = number[j] >= 0 && d < D;
+      const float x = to_float(src[in ? at[j] + d : 0]);
+      v[u] = in ? x : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kFmaThreads;
+      dst[e / DP * F::LD + e % DP] = v[u];
+    }
   }
 }
 

@@ -37,15 +37,15 @@ struct AttnCut {
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
-// Parts in which `ctas` CTAs, each walking `steps` tiles, run for the least time on `slots` places: whole rounds of CTAs, each a
-// part's steps and `fixed` steps' time for its beginning and end; a part more costs `join` steps' time.
-int best_parts(long long ctas, long long steps, long long slots, double fixed, double join) {
+// Parts in which `ctas` CTAs, each walking `steps` tiles of `step` us, run for the least time on `slots` places: whole rounds of
+// CTAs, each a part's steps and 3 us for its beginning and end; joining takes 3 us and `join` us a part.
+int best_parts(long long ctas, long long steps, long long slots, double step, double join) {
   int best = 1;
   double least = 0;
   for (long long s = 1; s <= std::min<long long>(64, std::max<long long>(1, steps)); ++s) {
     const long long per = cdiv(steps, s);
     if (s > 1 && cdiv(steps, per) < s) continue;  // a part would have nothing
-    const double rounds = (double)cdiv(ctas * s, slots), time = rounds * (per + fixed) + (s > 1 ? join * s : 0);
+    const double time = (double)cdiv(ctas * s, slots) * (per * step + 3) + (s > 1 ? 3 + join * s : 0);
     if (s == 1 || time < 0.97 * least) best = (int)s, least = time;
   }
   return best;
@@ -61,9 +61,13 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
-  c.splits = best_parts(expected, kv_tiles, tc ? (c.tile > kTcRows || backward ? 1 : 2) * kMultiprocessors : 2 * kMultiprocessors, 3, 0.5);
+  // us of one tile of states against one of rows, measured; a part's sums are written and read at 4 MB/us
+  const bool wide = a->D > 64;
+  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.1) : c.tile > kTcRows ? (wide ? 1.2 : 0.9) : (wide ? 1.6 : 1.1);
+  c.splits = best_parts(expected, kv_tiles, (!tc || (c.tile == kTcRows && !backward) ? 2 : 1) * kMultiprocessors, step, rows * a->D * 8 / 4e6);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(kv_tiles, kTcMaxTiles));
-  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), (tc ? 1 : 2) * kMultiprocessors, 2, 1) : 1;
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), (tc ? 1 : 2) * kMultiprocessors,
+                                       !tc ? 10.0 : wide ? 2.0 : 1.3, (double)a->N * a->L * a->Hk * a->D * 16 / 4e6) : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
     const long long here = at;
@@ -113,6 +117,7 @@ int check_attention(const mvr_attention* a, bool backward, bool sizes_only) {
   const long long most = INT32_MAX / 4;
   if (a->R > most || a->T > most || a->Hq > 65535 || a->Hk > 65535 || a->N > most || a->L > most) return MVR_ERR_TOO_LARGE;
   if (a->T > 0 && a->R > 0 && a->R * a->T > most / (a->Hq / a->Hk)) return MVR_ERR_TOO_LARGE;  // rows of a key head: 32 bits
+  if (a->R * a->T * a->Hq * a->D / 256 > INT32_MAX - 1) return MVR_ERR_TOO_LARGE;  // CTAs of the small kernels
   if (a->has_index && (size_t)(a->N + 1) * 8 > kPlanShared) return MVR_ERR_TOO_LARGE;
   if (cdiv(a->L, 32) * a->N > INT32_MAX) return MVR_ERR_TOO_LARGE;
   if (sizes_only) return MVR_OK;
@@ -193,7 +198,10 @@ unsigned blocks_of(long long n, int per) { return (unsigned)std::min<long long>(
 template <typename T>
 int sum_parts(const float* part, void* dst, long long n, int parts, float factor, cudaStream_t st) {
   if (n == 0) return MVR_OK;
-  launch_dependent(attn_sum<T>, dim3(blocks_of(n, 256)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
+  if (n % 4 == 0 && (uintptr_t)dst % (4 * sizeof(T)) == 0)
+    launch_dependent(attn_sum<T, 4>, dim3(blocks_of(n, 1024)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
+  else
+    launch_dependent(attn_sum<T, 1>, dim3(blocks_of(n, 256)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
   return launched();
 }
 
@@ -235,7 +243,11 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
     rc = p.D <= 32 ? fma_forward<T, 32>(p, c, st) : p.D <= 64 ? fma_forward<T, 64>(p, c, st)
          : p.D <= 128 ? fma_forward<T, 128>(p, c, st) : fma_forward<T, 256>(p, c, st);
   if (rc != MVR_OK || c.splits == 1) return rc;
-  launch_dependent(attn_join<T>, dim3((unsigned)cdiv((long long)p.R * p.T * p.Hq, 8)), dim3(256), 0, st, p);
+  const long long outputs = (long long)p.R * p.T * p.Hq * p.D;
+  if (p.D % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(T)) == 0)
+    launch_dependent(attn_join<T, 4>, dim3((unsigned)cdiv(outputs, 1024)), dim3(256), 0, st, p);
+  else
+    launch_dependent(attn_join<T, 1>, dim3((unsigned)cdiv(outputs, 256)), dim3(256), 0, st, p);
   return launched();
 }
 
