@@ -19,6 +19,8 @@
 
 namespace mvr {
 
+constexpr int kPolynomials = 2;  // of eight pairs of exponentials, how many are polynomials
+
 constexpr int kTcRows = 128, kTcStates = 128, kTcMaxTiles = 512;  // tiles of states that one CTA can list
 
 template <int DP, int TILES, bool MASK>
@@ -256,27 +258,48 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           break;
         }
         tc_fence_after();
-        const auto fetch = [&](float (&s)[32], int q) {
-          uint32_t v[32];
-          tmem_load32(v, s_at + q * 32);
-          tmem_wait_load();
+        // scores of 32 states, those that are left out as -inf
+        const auto settle = [&](uint32_t (&v)[32], int q) {
           const uint32_t b = word_of(bits, q);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
           if (b != ~0u) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = (b >> i) & 1 ? s[i] : -INFINITY;
+            for (int i = 0; i < 32; ++i) v[i] = (b >> i) & 1 ? v[i] : __float_as_uint(-INFINITY);
           }
         };
-        float top = -INFINITY, s[32];
+        const auto most = [&](const uint32_t (&v)[32], float a) {  // of 32 scores and a; two chains
+          float c = __uint_as_float(v[0]);
+#pragma unroll
+          for (int i = 1; i < 31; i += 4) {
+            a = max3(a, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            c = max3(c, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3 < 32 ? i + 3 : 31]));
+          }
+          return max3(max3(a, c, __uint_as_float(v[31])), __uint_as_float(v[30]), __uint_as_float(v[30]));
+        };
+        // one warpgroup a CTA has the registers to keep all scores; two CTAs an SM fetch them twice
+        constexpr bool kKeep = TILES == 2;
+        uint32_t s[kKeep ? 4 : 1][32];
+        float tops[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          fetch(s, q);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+          tmem_load32(s[kKeep ? q : 0], s_at + q * 32);
+          if (!kKeep) {
+            tmem_wait_load();
+            settle(s[0], q);
+            tops[q] = most(s[0], -INFINITY);
+          }
         }
+        if (kKeep) {
+          tmem_wait_load();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            settle(s[kKeep ? q : 0], q);
+            tops[q] = most(s[kKeep ? q : 0], -INFINITY);
+          }
+        }
+        float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+        if (top == INFINITY) top = NAN;  // (as inf - inf is; the sums are NaN from here on)
         // move the maximum?  (the first tile: there is no O yet)
-        const bool move = top > m && (m == -INFINITY || (top - m) * scale > 8.0f);
+        const bool move = !(top <= m) && (m == -INFINITY || !((top - m) * scale <= 8.0f));  // (NaN moves it)
         if (__any_sync(~0u, move)) {
           const float shrink = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - top) * scale)) : 1.0f;
           if (move) m = top;
@@ -294,20 +317,28 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m * scale;
-        float sum = 0.0f;
+        const float2 scale2 = make_float2(scale, scale), minus = make_float2(-ref, -ref);
+        float2 sums[2] = {};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          fetch(s, q);
+          uint32_t (&x)[32] = s[kKeep ? q : 0];
+          if (!kKeep) {
+            tmem_load32(x, s_at + q * 32);
+            tmem_wait_load();
+            settle(x, q);
+          }
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = exp2_fast(fmaf(s[2 * i], scale, -ref)), b = exp2_fast(fmaf(s[2 * i + 1], scale, -ref));
-            sum += a + b;
-            v[i] = pack2<T>(a, b);
+            const float2 a = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, minus);
+            const float2 e = kPolynomials && i % 8 < kPolynomials ? exp2_polynomial(a) : make_float2(exp2_fast(a.x), exp2_fast(a.y));
+            sums[i & 1] = add2(sums[i & 1], e);
+            v[i] = pack2<T>(e.x, e.y);
           }
           tmem_store16(s_at + q * 16, v);
         }
-        l += sum;
+        const float2 sum = add2(sums[0], sums[1]);
+        l += sum.x + sum.y;
         tmem_wait_store();
         tc_fence_before();
         bar_arrive(smem_at(&c.weights[t]));
@@ -316,6 +347,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (__all_sync(~0u, ok)) {
         tc_fence_after();
         const long long row = row_number(p, w), rows = (long long)p.R * p.T * p.Hq;
+        if (m == -INFINITY) l = 0.0f;  // no state, or only scores of -inf
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (mine) {
           if (p.splits > 1) {

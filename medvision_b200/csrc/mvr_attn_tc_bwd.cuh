@@ -73,8 +73,8 @@ struct TcStates {
     unsigned long long states, full[2], empty[2], scores, slopes, weights, grads, done;
     uint32_t tmem;
     int lost, peak;
-    alignas(16) float lse[2][128];
-    alignas(16) float delta[2][128];
+    alignas(16) float lse[2][128];    // negative
+    alignas(16) float delta[2][128];  // negative
   };
   static constexpr size_t kShared = 6 * (size_t)kTileBytes + sizeof(Control) + 1024;
 };
@@ -212,8 +212,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         lse = lse == -INFINITY ? INFINITY : lse - shift;
         delta = p.delta[number];
       }
-      c.lse[stage][mine] = lse;
-      c.delta[stage][mine] = delta;
+      c.lse[stage][mine] = -lse;
+      c.delta[stage][mine] = -delta;
       const uint32_t qs = smem_at(base + (2 + 2 * stage) * F::kTileBytes), gs = qs + F::kTileBytes;
 #pragma unroll 4
       for (int e = 0; e < DP / 8; ++e) {
@@ -266,28 +266,32 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (threadIdx.x == 0) atomicMax((int*)peaks + 1, c.peak);
       factor = slope_scale<T>(p.D, peaks[0], peak);
     }
-    const float slope = factor * exp2f(-shift);
+    const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
+    const uint32_t keep = in ? ~0u : 0u;  // a state that is not read: zeros, whatever its scores are
     for (int i = 0; i < count; ++i) {
       const int stage = i & 1;
       ok = ok && bar_wait(smem_at(&c.full[stage]), (i >> 1) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
       if (!(ok = __all_sync(~0u, ok))) break;
       tc_fence_after();
-      float w[64];
+      float2 w[32];
+      uint32_t v[2][32];
+      tmem_load32(v[0], tmem + lanes + F::kScores + half * 64);
+      tmem_load32(v[1], tmem + lanes + F::kScores + half * 64 + 32);
+      tmem_wait_load();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_load32(v, tmem + lanes + F::kScores + half * 64 + q * 32);
-        tmem_wait_load();
         uint32_t u[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 lse = *(const float4*)&c.lse[stage][half * 64 + q * 32 + e];
-          const float x[4] = {lse.x, lse.y, lse.z, lse.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[q * 32 + e + k] = in ? exp2_fast(fmaf(__uint_as_float(v[e + k]), p.scale_log2, -x[k])) : 0.0f;
-          u[e / 2] = pack2<T>(w[q * 32 + e], w[q * 32 + e + 1]);
-          u[e / 2 + 1] = pack2<T>(w[q * 32 + e + 2], w[q * 32 + e + 3]);
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = fma2(make_float2(__uint_as_float(v[q][e + 2 * k]), __uint_as_float(v[q][e + 2 * k + 1])), scale2,
+                                  k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
+            const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            w[q * 16 + e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
+            u[e / 2 + k] = pack2<T>(y.x, y.y) & keep;
+          }
         }
         // (over this warpgroup's own half of the scores)
         tmem_store16(tmem + lanes + F::kScores + half * 64 + q * 16, u);
@@ -297,21 +301,22 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       bar_arrive(smem_at(&c.weights));
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
       tc_fence_after();
+      tmem_load32(v[0], tmem + lanes + F::kSlopes + half * 64);
+      tmem_load32(v[1], tmem + lanes + F::kSlopes + half * 64 + 32);
+      tmem_wait_load();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_load32(v, tmem + lanes + F::kSlopes + half * 64 + q * 32);
-        tmem_wait_load();
         uint32_t u[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 delta = *(const float4*)&c.delta[stage][half * 64 + q * 32 + e];
-          const float x[4] = {delta.x, delta.y, delta.z, delta.w};
-          float ds[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ds[k] = in ? w[q * 32 + e + k] * slope * (__uint_as_float(v[e + k]) - x[k]) : 0.0f;
-          u[e / 2] = pack2<T>(ds[0], ds[1]);
-          u[e / 2 + 1] = pack2<T>(ds[2], ds[3]);
+          for (int k = 0; k < 2; ++k) {
+            const float2 ds = mul2(w[q * 16 + e / 2 + k],
+                                   add2(make_float2(__uint_as_float(v[q][e + 2 * k]), __uint_as_float(v[q][e + 2 * k + 1])),
+                                        k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
+            u[e / 2 + k] = pack2<T>(ds.x, ds.y) & keep;
+          }
         }
         tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
       }
@@ -545,6 +550,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       bar_arrive(smem_at(&c.rows));
     }
     const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
     bool ok = true;
     for (int i = 0; i < tiles; ++i) {
       uint32_t bits[2] = {~0u, ~0u};
@@ -559,36 +565,33 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       }
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.scores), i & 1, lost)))) break;
       tc_fence_after();
-      float wgt[64];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_load32(v, tmem + lanes + F::kScores + half * 64 + q * 32);
-        tmem_wait_load();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) wgt[q * 32 + e] = __uint_as_float(v[e]);
-      }
+      uint32_t v[2][32];
+      tmem_load32(v[0], tmem + lanes + F::kScores + half * 64);
+      tmem_load32(v[1], tmem + lanes + F::kScores + half * 64 + 32);
+      tmem_wait_load();
       tc_fence_before();
       bar_arrive(smem_at(&c.taken));
+      float2 wgt[32];
 #pragma unroll
-      for (int e = 0; e < 64; ++e) wgt[e] = exp2_fast(fmaf(wgt[e], p.scale_log2, -lse)) * factor;
+      for (int e = 0; e < 32; ++e) {
+        const float2 x = fma2(make_float2(__uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1])), scale2, minus);
+        const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+        wgt[e] = TcType<T>::code == 0 ? mul2(y, make_float2(factor, factor)) : y;
+      }
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
       tc_fence_after();
+      tmem_load32(v[0], tmem + lanes + F::kSlopes + half * 64);
+      tmem_load32(v[1], tmem + lanes + F::kSlopes + half * 64 + 32);
+      tmem_wait_load();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_load32(v, tmem + lanes + F::kSlopes + half * 64 + q * 32);
-        tmem_wait_load();
-        float ds[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) ds[e] = wgt[q * 32 + e] * (__uint_as_float(v[e]) - delta);
-        if (bits[q] != ~0u) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) ds[e] = (bits[q] >> e) & 1 ? ds[e] : 0.0f;
-        }
         uint32_t u[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) u[e] = pack2<T>(ds[2 * e], ds[2 * e + 1]);
+        for (int e = 0; e < 16; ++e) {
+          float2 ds = mul2(wgt[q * 16 + e], add2(make_float2(__uint_as_float(v[q][2 * e]), __uint_as_float(v[q][2 * e + 1])), less));
+          if (bits[q] != ~0u) ds = make_float2((bits[q] >> (2 * e)) & 1 ? ds.x : 0.0f, (bits[q] >> (2 * e + 1)) & 1 ? ds.y : 0.0f);
+          u[e] = pack2<T>(ds.x, ds.y);
+        }
         tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
       }
       tmem_wait_store();
