@@ -1,8 +1,8 @@
 // Attention forward on the tensor cores (float16, bfloat16; head sizes that are multiples of 8, up to 128).
 //
 // A CTA holds TILES tiles of 128 rows of queries and walks the states of their image 128 at a time.  One warp brings tiles of keys
-// and values into a ring in shared memory by TMA, one thread issues the products, and a warpgroup per row tile, one row a thread,
-// keeps the running maximum and sum:
+// and values into a ring in shared memory by TMA, one thread issues the products, and two warpgroups per row tile, half a row a
+// thread, keep the running maximum and sum:
 //
 //   S = Q K^T (128 x 128, tensor memory)  ->  P = 2^(S scale - m), rounded to T, over S  ->  O += P V (tensor memory)
 //
@@ -27,13 +27,14 @@ template <int DP, int TILES, bool MASK>
 struct TcForward {
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128;       // a tile of rows or states
   static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 4);
-  static constexpr int kSoftmax = TILES * 128, kThreads = kSoftmax + (MASK ? 96 : 64);
+  static constexpr int kSoftmax = TILES * 256, kThreads = kSoftmax + 96;
   static constexpr int kColumns = TILES == 2 ? 512 : 256, kScores = 0, kOut = TILES * 128;
   struct Control {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots];
-    unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES];
+    unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES], halves[TILES];
     uint32_t tmem;
     int lost, tiles;
+    float top[2][TILES][2][128];  // what the two halves of a row tell each other
     unsigned short list[MASK ? kTcMaxTiles : 1];
     uint4 bits[MASK ? kTcMaxTiles : 1];
   };
@@ -87,9 +88,9 @@ __device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin
 
 // A row of 2-byte elements into a K-major tile in the 128-byte swizzle; zeros behind D, and for no row at all.
 template <int DP>
-__device__ __forceinline__ void put_row(char* tile, int r, const void* src, int D) {
+__device__ __forceinline__ void put_row(char* tile, int r, const void* src, int D, int first = 0, int last = DP / 8) {
 #pragma unroll
-  for (int c = 0; c < DP / 8; ++c) {
+  for (int c = first; c < last; ++c) {
     const uint4 v = src && c * 8 < D ? ((const uint4*)src)[c] : make_uint4(0, 0, 0, 0);
     *(uint4*)(tile + (c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
   }
@@ -112,9 +113,10 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       bar_init(smem_at(&c.clean[i]), 1);
     }
     for (int t = 0; t < TILES; ++t) {
-      bar_init(smem_at(&c.queries[t]), 128);
+      bar_init(smem_at(&c.queries[t]), 8);
       bar_init(smem_at(&c.scores[t]), 1);
-      bar_init(smem_at(&c.weights[t]), 128);
+      bar_init(smem_at(&c.weights[t]), 8);
+      bar_init(smem_at(&c.halves[t]), 8);
       bar_init(smem_at(&c.out[t]), 1);
     }
     c.lost = 0;
@@ -143,68 +145,84 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
 
   if (warp == kLoader) {
-    if (lane == 0) {
-      int i = 0;
-      for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
-        const int slot = i % F::kSlots;
-        const uint32_t bar = smem_at(&c.full[slot]);
-        if (i >= F::kSlots && !bar_wait(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+    int i = 0;
+    for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
+      const int slot = i % F::kSlots;
+      const uint32_t bar = smem_at(&c.full[slot]);
+      if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+      const int j = first_of(i >> 1);
+      if (elect_one()) {
         bar_expect(bar, F::kTileBytes);
-        const int j = first_of(i >> 1);
+#pragma unroll
         for (int b = 0; b < F::kBlocks; ++b)
           tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * kTcRows * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
       }
-      // given up: the copies under way end before the CTA does
-      if (*lost)
-        for (int k = max(0, i - F::kSlots); k < i; ++k) {
-          const unsigned long long t = nanoseconds();
-          while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
-        }
+      __syncwarp();
     }
+    // given up: the copies under way end before the CTA does
+    if (*lost)
+      for (int k = max(0, i - F::kSlots); k < i; ++k) {
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
+      }
   } else if (warp == kIssuer) {
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0) {
       const int depth = (p.D + 15) / 16;
       const uint32_t s_shape = tc_shape<T>(kTcStates, false, p.scale < 0.0f), o_shape = tc_shape<T>(depth * 16, true);
+      const uint64_t queries = desc_k_major(smem_at(base)), keys = desc_k_major(smem_at(ring)), values = desc_mn_major(smem_at(ring), kTcRows * 128);
       const auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
-        const uint32_t a = smem_at(base + t * F::kTileBytes), b = smem_at(ring + slot * F::kTileBytes);
-        for (int k = 0; k < depth; ++k) {
-          const uint32_t off = (k >> 2) * (kTcRows * 128) + (k & 3) * 32;
-          mma_ss(tmem + F::kScores + t * 128, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = (k >> 2) * (kTcRows * 128) + (k & 3) * 32;
+            if (k < depth)
+              mma_ss(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes + off) >> 4), keys + ((slot * F::kTileBytes + off) >> 4), s_shape, k > 0);
+          }
+          mma_commit(smem_at(&c.scores[t]));
         }
-        mma_commit(smem_at(&c.scores[t]));
+        __syncwarp();
+      };
+      const auto commit = [&](unsigned long long* bar) {
+        if (elect_one()) mma_commit(smem_at(bar));
+        __syncwarp();
       };
       bool ok = true;
-      for (int t = 0; t < used && ok; ++t) ok = bar_wait(smem_at(&c.queries[t]), 0, lost);
-      ok = ok && bar_wait(smem_at(&c.full[0]), 0, lost);
+      for (int t = 0; t < used && ok; ++t) ok = bar_wait_warp(smem_at(&c.queries[t]), 0, lost);
+      ok = ok && bar_wait_warp(smem_at(&c.full[0]), 0, lost);
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < used; ++t) scores(t, 0);
-        mma_commit(smem_at(&c.empty[0]));
+        commit(&c.empty[0]);
       }
       for (int j = 0; j < tiles && ok; ++j) {
         const int v = 2 * j + 1, k = v + 1, vs = v % F::kSlots, ks = k % F::kSlots;
-        ok = bar_wait(smem_at(&c.full[vs]), (v / F::kSlots) & 1, lost);
-        if (MASK && ok) ok = bar_wait(smem_at(&c.clean[vs]), (v / F::kSlots) & 1, lost);
-        for (int t = 0; t < used && ok; ++t) {
-          ok = bar_wait(smem_at(&c.weights[t]), j & 1, lost);
+        ok = bar_wait_warp(smem_at(&c.full[vs]), (v / F::kSlots) & 1, lost);
+        if (MASK && ok) ok = bar_wait_warp(smem_at(&c.clean[vs]), (v / F::kSlots) & 1, lost);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          if (t >= used || !ok) break;
+          ok = bar_wait_warp(smem_at(&c.weights[t]), j & 1, lost);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = smem_at(ring + vs * F::kTileBytes);
-          for (int i = 0; i < kTcStates / 16; ++i)  // O_t += P_t V
-            mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * 128 + i * 8, desc_mn_major(b + i * 2048, kTcRows * 128), o_shape,
-                   j > 0 || i > 0);
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kTcStates / 16; ++i)  // O_t += P_t V
+              mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * 128 + (i >> 2) * 64 + (i & 3) * 8,
+                     values + ((vs * F::kTileBytes + i * 2048) >> 4), o_shape, j > 0 || i > 0);
+          }
+          __syncwarp();
           if (j + 1 < tiles) {
-            if (t == 0) ok = bar_wait(smem_at(&c.full[ks]), (k / F::kSlots) & 1, lost);
+            if (t == 0) ok = bar_wait_warp(smem_at(&c.full[ks]), (k / F::kSlots) & 1, lost);
             if (ok) {
               tc_fence_after();
               scores(t, ks);
             }
           }
         }
-        mma_commit(smem_at(&c.empty[vs]));
-        if (j + 1 < tiles) mma_commit(smem_at(&c.empty[ks]));
+        commit(&c.empty[vs]);
+        if (j + 1 < tiles) commit(&c.empty[ks]);
       }
-      for (int t = 0; t < TILES; ++t) mma_commit(smem_at(&c.out[t]));
+      for (int t = 0; t < TILES; ++t) commit(&c.out[t]);
     }
   } else if (MASK && warp == kCleaner) {
     for (int j = 0; j < tiles; ++j) {
@@ -228,29 +246,32 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
-    const int t = warp >> 2, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + F::kScores + t * 128, o_at = tmem + lanes + F::kOut + t * DP;
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + F::kScores + t * 128 + half * 64, o_at = tmem + lanes + F::kOut + t * DP;
     if (t < used) {
       Row w = {};
       const bool mine = j0 < o.rows;
       if (mine) w = row_of(p, o, j0, hk);
       if (tiles > 0) {
-        put_row<DP>(base + t * F::kTileBytes, r, mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr, p.D);
+        const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
+        if (half) put_row<DP>(base + t * F::kTileBytes, r, q, p.D, DP / 16, DP / 8);
+        else put_row<DP>(base + t * F::kTileBytes, r, q, p.D, 0, DP / 16);
         fence_async_proxy();
-        bar_arrive(smem_at(&c.queries[t]));
+        bar_arrive_warp(smem_at(&c.queries[t]));
       }
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
-      float m = -INFINITY, l = 0.0f;  // m: in the units of S
+      float m = -INFINITY, l = 0.0f;  // m: in the units of S, the same in both halves; l: of this half
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
-        uint4 bits = make_uint4(~0u, ~0u, ~0u, ~0u);
-        if (MASK) bits = c.bits[j];
-        else if (j + 1 == tiles && (end & 127)) {
-          const int n = end & 127;
-          bits.x = n >= 32 ? ~0u : (1u << n) - 1;
-          bits.y = n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1 : 0;
-          bits.z = n >= 96 ? ~0u : n > 64 ? (1u << (n - 64)) - 1 : 0;
-          bits.w = n > 96 ? (1u << (n - 96)) - 1 : 0;
+        uint32_t bits[2] = {~0u, ~0u};
+        if (MASK) {
+          const uint4 b = c.bits[j];
+          bits[0] = half ? b.z : b.x;
+          bits[1] = half ? b.w : b.y;
+        } else if (j + 1 == tiles && (end & 127)) {
+          const int left = (end & 127) - half * 64;
+          bits[0] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
+          bits[1] = left >= 64 ? ~0u : left > 32 ? (1u << (left - 32)) - 1 : 0;
         }
         ok = bar_wait(smem_at(&c.scores[t]), j & 1, lost);
         if (!__all_sync(~0u, ok)) {
@@ -260,43 +281,40 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         tc_fence_after();
         // scores of 32 states, those that are left out as -inf
         const auto settle = [&](uint32_t (&v)[32], int q) {
-          const uint32_t b = word_of(bits, q);
-          if (b != ~0u) {
+          if (bits[q] != ~0u) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = (b >> i) & 1 ? v[i] : __float_as_uint(-INFINITY);
+            for (int i = 0; i < 32; ++i) v[i] = (bits[q] >> i) & 1 ? v[i] : __float_as_uint(-INFINITY);
           }
         };
-        const auto most = [&](const uint32_t (&v)[32], float a) {  // of 32 scores and a; two chains
-          float c = __uint_as_float(v[0]);
+        const auto most = [&](const uint32_t (&v)[32]) {  // of 32 scores; two chains
+          float a = -INFINITY, c = __uint_as_float(v[0]);
 #pragma unroll
-          for (int i = 1; i < 31; i += 4) {
+          for (int i = 1; i < 29; i += 4) {
             a = max3(a, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            c = max3(c, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3 < 32 ? i + 3 : 31]));
+            c = max3(c, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
           }
-          return max3(max3(a, c, __uint_as_float(v[31])), __uint_as_float(v[30]), __uint_as_float(v[30]));
+          a = max3(a, __uint_as_float(v[29]), __uint_as_float(v[30]));
+          return max3(a, c, __uint_as_float(v[31]));
         };
-        // one warpgroup a CTA has the registers to keep all scores; two CTAs an SM fetch them twice
-        constexpr bool kKeep = TILES == 2;
-        uint32_t s[kKeep ? 4 : 1][32];
-        float tops[4];
+        // (fetched twice: keeping them costs more registers than a thread has)
+        uint32_t x[32];
+        float top = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tmem_load32(s[kKeep ? q : 0], s_at + q * 32);
-          if (!kKeep) {
-            tmem_wait_load();
-            settle(s[0], q);
-            tops[q] = most(s[0], -INFINITY);
-          }
-        }
-        if (kKeep) {
+        for (int q = 0; q < 2; ++q) {
+          tmem_load32(x, s_at + q * 32);
           tmem_wait_load();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            settle(s[kKeep ? q : 0], q);
-            tops[q] = most(s[kKeep ? q : 0], -INFINITY);
-          }
+          settle(x, q);
+          top = max3(top, most(x), top);
         }
-        float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+        // the row's maximum, of both halves
+        c.top[j & 1][t][half][r] = top;
+        bar_arrive_warp(smem_at(&c.halves[t]));
+        ok = bar_wait(smem_at(&c.halves[t]), j & 1, lost);
+        if (!__all_sync(~0u, ok)) {
+          ok = false;
+          break;
+        }
+        top = max3(top, c.top[j & 1][t][half ^ 1][r], top);
         if (top == INFINITY) top = NAN;  // (as inf - inf is; the sums are NaN from here on)
         // move the maximum?  (the first tile: there is no O yet)
         const bool move = !(top <= m) && (m == -INFINITY || !((top - m) * scale <= 8.0f));  // (NaN moves it)
@@ -306,7 +324,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           l *= shrink;
           if (j > 0) {
 #pragma unroll 1
-            for (int q = 0; q < DP / 32; ++q) {
+            for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
               uint32_t v[32];
               tmem_load32(v, o_at + q * 32);
               tmem_wait_load();
@@ -320,13 +338,10 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         const float2 scale2 = make_float2(scale, scale), minus = make_float2(-ref, -ref);
         float2 sums[2] = {};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t (&x)[32] = s[kKeep ? q : 0];
-          if (!kKeep) {
-            tmem_load32(x, s_at + q * 32);
-            tmem_wait_load();
-            settle(x, q);
-          }
+        for (int q = 0; q < 2; ++q) {
+          tmem_load32(x, s_at + q * 32);
+          tmem_wait_load();
+          settle(x, q);
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -335,21 +350,26 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             sums[i & 1] = add2(sums[i & 1], e);
             v[i] = pack2<T>(e.x, e.y);
           }
-          tmem_store16(s_at + q * 16, v);
+          tmem_store16(s_at + q * 16, v);  // (over this half's own scores)
         }
         const float2 sum = add2(sums[0], sums[1]);
         l += sum.x + sum.y;
         tmem_wait_store();
         tc_fence_before();
-        bar_arrive(smem_at(&c.weights[t]));
+        bar_arrive_warp(smem_at(&c.weights[t]));
       }
+      // the halves' sums together (a + b is b + a: the same in both)
+      c.top[tiles & 1][t][half][r] = l;
+      bar_arrive_warp(smem_at(&c.halves[t]));
+      ok = ok && bar_wait(smem_at(&c.halves[t]), tiles & 1, lost);
+      l += c.top[tiles & 1][t][half ^ 1][r];
       if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.out[t]), 0, lost);
       if (__all_sync(~0u, ok)) {
         tc_fence_after();
         const long long row = row_number(p, w), rows = (long long)p.R * p.T * p.Hq;
         if (m == -INFINITY) l = 0.0f;  // no state, or only scores of -inf
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (mine) {
+        if (mine && !half) {
           if (p.splits > 1) {
             p.part_ml[(split * rows + row) * 2] = m == -INFINITY ? m : m * scale;
             p.part_ml[(split * rows + row) * 2 + 1] = l;
@@ -357,8 +377,8 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             p.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? 0.0f : m * scale) + log2f(l);
           }
         }
-#pragma unroll
-        for (int q = 0; q < DP / 32; ++q) {
+#pragma unroll 1
+        for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
           if (q * 32 >= p.D) break;
           uint32_t v[32];
           if (tiles > 0) {

@@ -6,8 +6,8 @@
 //   states kept:  S^T = K Q^T    dP^T = V G^T    dV += P^T G    dK += dS^T Q           dS = P (dP - delta)
 //   rows kept:    S   = Q K^T    dP   = G V^T    dQ += dS K
 //
-// Scores, dP and the sums are in tensor memory; P and dS, rounded to T, go back over the scores and dP as left operands.  Two
-// warpgroups share a tile, one row a thread and half its columns each.  One thread issues the products in an order in which those of
+// Scores, dP and the sums are in tensor memory; P and dS, rounded to T, go back over the scores and dP as left operands.  Four
+// warpgroups share a tile, a quarter of a row a thread: with two, a warp's own latencies set the pace.  One thread issues the products in an order in which those of
 // one tile run under the exponentials of the next: dV(i), S(i+1), dK(i), dP(i+1), and S(i+1), dQ(i), dP(i+1).
 //
 // float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= 2 D max|g| max|v|
@@ -18,9 +18,9 @@
 
 namespace mvr {
 
-constexpr int kGradThreads = 256;  // of the two warpgroups
+constexpr int kGradThreads = 512;  // of the four warpgroups
 
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
 // Power of two for dS, from bounds of |g| and |v| (float bits).
 template <typename T>
@@ -67,7 +67,7 @@ __device__ __forceinline__ void put_sums(uint32_t at, float factor, T* to, float
 template <int DP>
 struct TcStates {
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128;
-  static constexpr int kLoaders = 128, kThreads = kGradThreads + kLoaders + 32;
+  static constexpr int kLoaders = 64, kThreads = kGradThreads + kLoaders + 32;
   static constexpr int kScores = 0, kSlopes = 128, kValues = 256, kKeys = 256 + DP, kColumns = 512;
   struct Control {
     unsigned long long states, full[2], empty[2], scores, slopes, weights, grads, done;
@@ -95,13 +95,13 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   if (threadIdx.x == 0) {
     bar_init(smem_at(&c.states), 1);
     for (int i = 0; i < 2; ++i) {
-      bar_init(smem_at(&c.full[i]), F::kLoaders);
+      bar_init(smem_at(&c.full[i]), F::kLoaders / 32);
       bar_init(smem_at(&c.empty[i]), 1);
     }
     bar_init(smem_at(&c.scores), 1);
     bar_init(smem_at(&c.slopes), 1);
-    bar_init(smem_at(&c.weights), kGradThreads);
-    bar_init(smem_at(&c.grads), kGradThreads);
+    bar_init(smem_at(&c.weights), kGradThreads / 32);
+    bar_init(smem_at(&c.grads), kGradThreads / 32);
     bar_init(smem_at(&c.done), 1);
     c.lost = 0;
     c.peak = 0;
@@ -112,7 +112,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const int state_tiles = (p.L + 127) / 128, n = blockIdx.x / state_tiles, j0 = (blockIdx.x - n * state_tiles) * 128;
   const int hk = blockIdx.y, split = blockIdx.z;
   // one row a thread: its state, and whether it is read
-  const int r = ((warp & 3) << 5) + lane, half = warp >> 2, j = j0 + r;
+  const int r = ((warp & 3) << 5) + lane, part_of = warp >> 2, j = j0 + r;
   bool in = false;
   if (warp < kLoader) in = j < states_of(p, n) && (!p.mask || p.mask[(long long)n * p.L + j] != 0);
   const bool any = __syncthreads_or(in);
@@ -134,97 +134,110 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const float shift = weight_shift<T>();
 
   if (warp == kIssuer) {
-    if (lane == 0 && count > 0) {
-      bar_expect(smem_at(&c.states), 2 * F::kTileBytes);
-      for (int b = 0; b < F::kBlocks; ++b) {
-        tma_load_4d(smem_at(base + b * 16384), &maps.k, smem_at(&c.states), b * 64, hk, j0, n);
-        tma_load_4d(smem_at(base + F::kTileBytes + b * 16384), &maps.v, smem_at(&c.states), b * 64, hk, j0, n);
+    if (count > 0) {
+      if (elect_one()) {
+        bar_expect(smem_at(&c.states), 2 * F::kTileBytes);
+#pragma unroll
+        for (int b = 0; b < F::kBlocks; ++b) {
+          tma_load_4d(smem_at(base + b * 16384), &maps.k, smem_at(&c.states), b * 64, hk, j0, n);
+          tma_load_4d(smem_at(base + F::kTileBytes + b * 16384), &maps.v, smem_at(&c.states), b * 64, hk, j0, n);
+        }
       }
+      __syncwarp();
       const int depth = (p.D + 15) / 16;
       const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
-      const auto scores = [&](int left, int right, int to) {  // 128 x 128 over D, both K-major
-        const uint32_t a = smem_at(base + left * F::kTileBytes), b = smem_at(base + right * F::kTileBytes);
-        for (int k = 0; k < depth; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          mma_ss(tmem + to, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+      const uint64_t tiles_k = desc_k_major(smem_at(base)), tiles_mn = desc_mn_major(smem_at(base), 16384);
+      const auto scores = [&](int left, int right, int to, unsigned long long* bar) {  // 128 x 128 over D, both K-major
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+            if (k < depth)
+              mma_ss(tmem + to, tiles_k + ((left * F::kTileBytes + off) >> 4), tiles_k + ((right * F::kTileBytes + off) >> 4), s_shape, k > 0);
+          }
+          mma_commit(smem_at(bar));
         }
+        __syncwarp();
       };
       const auto sums = [&](int from, int right, int to, bool add) {  // over the 128 rows
-        const uint32_t b = smem_at(base + right * F::kTileBytes);
-        for (int i = 0; i < 8; ++i)
-          mma_ts(tmem + to, tmem + from + (i >> 2) * 64 + (i & 3) * 8, desc_mn_major(b + i * 2048, 16384), d_shape, add || i > 0);
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + (i & 1) * 8, tiles_mn + ((right * F::kTileBytes + i * 2048) >> 4), d_shape, add || i > 0);
+        }
+        __syncwarp();
       };
-      bool ok = bar_wait(smem_at(&c.states), 0, lost) && bar_wait(smem_at(&c.full[0]), 0, lost);
+      const auto commit = [&](unsigned long long* bar) {
+        if (elect_one()) mma_commit(smem_at(bar));
+        __syncwarp();
+      };
+      bool ok = bar_wait_warp(smem_at(&c.states), 0, lost) && bar_wait_warp(smem_at(&c.full[0]), 0, lost);
       if (ok) {
         tc_fence_after();
-        scores(0, 2, F::kScores);
-        mma_commit(smem_at(&c.scores));
-        scores(1, 3, F::kSlopes);
-        mma_commit(smem_at(&c.slopes));
+        scores(0, 2, F::kScores, &c.scores);
+        scores(1, 3, F::kSlopes, &c.slopes);
       }
       for (int i = 0; i < count && ok; ++i) {
         const int now = i & 1, next = now ^ 1;
-        if (!(ok = bar_wait(smem_at(&c.weights), i & 1, lost))) break;
+        if (!(ok = bar_wait_warp(smem_at(&c.weights), i & 1, lost))) break;
         tc_fence_after();
         sums(F::kScores, 3 + 2 * now, F::kValues, i > 0);
         if (i + 1 < count) {
-          if (!(ok = bar_wait(smem_at(&c.full[next]), ((i + 1) >> 1) & 1, lost))) break;
+          if (!(ok = bar_wait_warp(smem_at(&c.full[next]), ((i + 1) >> 1) & 1, lost))) break;
           tc_fence_after();
-          scores(0, 2 + 2 * next, F::kScores);
-          mma_commit(smem_at(&c.scores));
+          scores(0, 2 + 2 * next, F::kScores, &c.scores);
         }
-        if (!(ok = bar_wait(smem_at(&c.grads), i & 1, lost))) break;
+        if (!(ok = bar_wait_warp(smem_at(&c.grads), i & 1, lost))) break;
         tc_fence_after();
         sums(F::kSlopes, 2 + 2 * now, F::kKeys, i > 0);
-        mma_commit(smem_at(&c.empty[now]));
-        if (i + 1 < count) {
-          scores(1, 3 + 2 * next, F::kSlopes);
-          mma_commit(smem_at(&c.slopes));
-        }
+        commit(&c.empty[now]);
+        if (i + 1 < count) scores(1, 3 + 2 * next, F::kSlopes, &c.slopes);
       }
-      mma_commit(smem_at(&c.done));
+      commit(&c.done);
       if (*lost) {
         const unsigned long long t = nanoseconds();
         while (!bar_try(smem_at(&c.states), 0) && nanoseconds() - t < kWaitLimit) {}
       }
     }
   } else if (warp >= kLoader) {
-    // rows of Q and G, 16 bytes a copy: a warp's 32 rows, their places handed round by shuffles
-    const int w = warp - kLoader, mine = (w << 5) + lane;
+    // rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places handed round by shuffles
     const int chunks = p.D / 8;  // 16-byte pieces of a row
     const auto arrived = [&](int stage) {
       fence_async_proxy();
-      bar_arrive(smem_at(&c.full[stage]));
+      bar_arrive_warp(smem_at(&c.full[stage]));
     };
     for (int i = 0; i < count; ++i) {
       const int stage = i & 1;
       if (i >= 2 && !__all_sync(~0u, bar_wait(smem_at(&c.empty[stage]), ((i >> 1) - 1) & 1, lost))) break;
-      const int at = (first + i) * 128 + mine;
-      const char *q = (const char*)p.q, *g = (const char*)p.g;
-      const bool row_in = at < o.rows;
-      float lse = INFINITY, delta = 0.0f;  // no row: P = 0
-      if (row_in) {
-        const Row row = row_of(p, o, at, hk);
-        q += (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
-        g += (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
-        const long long number = row_number(p, row);
-        lse = p.lse[number];
-        lse = lse == -INFINITY ? INFINITY : lse - shift;
-        delta = p.delta[number];
-      }
-      c.lse[stage][mine] = -lse;
-      c.delta[stage][mine] = -delta;
       const uint32_t qs = smem_at(base + (2 + 2 * stage) * F::kTileBytes), gs = qs + F::kTileBytes;
+#pragma unroll 1
+      for (int w = warp - kLoader; w < 4; w += F::kLoaders / 32) {
+        const int mine = (w << 5) + lane, at = (first + i) * 128 + mine;
+        const char *q = (const char*)p.q, *g = (const char*)p.g;
+        const bool row_in = at < o.rows;
+        float lse = INFINITY, delta = 0.0f;  // no row: P = 0
+        if (row_in) {
+          const Row row = row_of(p, o, at, hk);
+          q += (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
+          g += (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
+          const long long number = row_number(p, row);
+          lse = p.lse[number];
+          lse = lse == -INFINITY ? INFINITY : lse - shift;
+          delta = p.delta[number];
+        }
+        c.lse[stage][mine] = -lse;
+        c.delta[stage][mine] = -delta;
 #pragma unroll 4
-      for (int e = 0; e < DP / 8; ++e) {
-        const int idx = e * 32 + lane, k = idx / (DP / 8), piece = idx % (DP / 8), row = (w << 5) + k;
-        const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q, k);
-        const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g, k);
-        const bool there = __shfl_sync(~0u, row_in, k);
-        if (piece < chunks) {
-          const uint32_t to = (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-          copy16(qs + to, there ? qk + piece * 16 : qk, there);
-          copy16(gs + to, there ? gk + piece * 16 : gk, there);
+        for (int e = 0; e < DP / 8; ++e) {
+          const int idx = e * 32 + lane, k = idx / (DP / 8), piece = idx % (DP / 8), row = (w << 5) + k;
+          const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q, k);
+          const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g, k);
+          const bool there = __shfl_sync(~0u, row_in, k);
+          if (piece < chunks) {
+            const uint32_t to = (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            copy16(qs + to, there ? qk + piece * 16 : qk, there);
+            copy16(gs + to, there ? gk + piece * 16 : gk, there);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -248,8 +261,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (ok && in) {
         const char* row = base + F::kTileBytes + r * 128;
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) {
-          const int piece = half * (DP / 16) + e;
+        for (int e = 0; e < DP / 32; ++e) {
+          const int piece = part_of * (DP / 32) + e;
           const uint4 v = *(const uint4*)(row + (piece >> 3) * 16384 + (((piece ^ r) & 7) << 4));
           const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -273,71 +286,61 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       ok = ok && bar_wait(smem_at(&c.full[stage]), (i >> 1) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
       if (!(ok = __all_sync(~0u, ok))) break;
       tc_fence_after();
-      float2 w[32];
-      uint32_t v[2][32];
-      tmem_load32(v[0], tmem + lanes + F::kScores + half * 64);
-      tmem_load32(v[1], tmem + lanes + F::kScores + half * 64 + 32);
+      const int col = part_of * 32;
+      float2 w[16];
+      uint32_t v[32], u[16];
+      tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t u[16];
+      for (int e = 0; e < 32; e += 4) {
+        const float4 lse = *(const float4*)&c.lse[stage][col + e];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 lse = *(const float4*)&c.lse[stage][half * 64 + q * 32 + e];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 x = fma2(make_float2(__uint_as_float(v[q][e + 2 * k]), __uint_as_float(v[q][e + 2 * k + 1])), scale2,
-                                  k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
-            const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-            w[q * 16 + e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
-            u[e / 2 + k] = pack2<T>(y.x, y.y) & keep;
-          }
+        for (int k = 0; k < 2; ++k) {
+          const float2 x = fma2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])), scale2,
+                                k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
+          const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+          w[e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
+          u[e / 2 + k] = pack2<T>(y.x, y.y) & keep;
         }
-        // (over this warpgroup's own half of the scores)
-        tmem_store16(tmem + lanes + F::kScores + half * 64 + q * 16, u);
       }
+      tmem_store16(tmem + lanes + F::kScores + col, u);  // (over this warpgroup's own scores)
       tmem_wait_store();
       tc_fence_before();
-      bar_arrive(smem_at(&c.weights));
+      bar_arrive_warp(smem_at(&c.weights));
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
       tc_fence_after();
-      tmem_load32(v[0], tmem + lanes + F::kSlopes + half * 64);
-      tmem_load32(v[1], tmem + lanes + F::kSlopes + half * 64 + 32);
+      tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t u[16];
+      for (int e = 0; e < 32; e += 4) {
+        const float4 delta = *(const float4*)&c.delta[stage][col + e];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 delta = *(const float4*)&c.delta[stage][half * 64 + q * 32 + e];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 ds = mul2(w[q * 16 + e / 2 + k],
-                                   add2(make_float2(__uint_as_float(v[q][e + 2 * k]), __uint_as_float(v[q][e + 2 * k + 1])),
-                                        k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
-            u[e / 2 + k] = pack2<T>(ds.x, ds.y) & keep;
-          }
+        for (int k = 0; k < 2; ++k) {
+          const float2 ds = mul2(w[e / 2 + k], add2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])),
+                                                    k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
+          u[e / 2 + k] = pack2<T>(ds.x, ds.y) & keep;
         }
-        tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
       }
+      tmem_store16(tmem + lanes + F::kSlopes + col, u);
       tmem_wait_store();
       tc_fence_before();
-      bar_arrive(smem_at(&c.grads));
+      bar_arrive_warp(smem_at(&c.grads));
     }
     if (count > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
     if (__all_sync(~0u, ok)) {
       tc_fence_after();
-      // the first warpgroup stores dv, the second dk
+      // the first two warpgroups store dv, the others dk, half the columns each
+      const bool keys = part_of >= 2;
       const long long all = (long long)p.N * p.L * p.Hk * p.D, at = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
       const bool parts = p.row_splits > 1;
-      const float f = in ? (half ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
-      T* to = (T*)(half ? p.gk : p.gv) + at;
-      float* part = parts ? (half ? p.part_gk : p.part_gv) + split * all + at : nullptr;
+      const float f = in ? (keys ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
+      T* to = (T*)(keys ? p.gk : p.gv) + at;
+      float* part = parts ? (keys ? p.part_gk : p.part_gv) + split * all + at : nullptr;
 #pragma unroll 1
-      for (int q = 0; q < DP / 32; ++q) {
+      for (int q = (part_of & 1) * (DP / 64); q < ((part_of & 1) + 1) * (DP / 64); ++q) {
         if (q * 32 >= p.D) break;
         // (a state that is not read: its sums may be NaN where rows hold NaN)
-        const uint32_t from = tmem + lanes + (half ? F::kKeys : F::kValues) + q * 32;
+        const uint32_t from = tmem + lanes + (keys ? F::kKeys : F::kValues) + q * 32;
         uint32_t v[32];
         if (count > 0) {
           tmem_load32(v, from);
@@ -410,11 +413,11 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       bar_init(smem_at(&c.empty[i]), 1);
       bar_init(smem_at(&c.clean[i]), 1);
     }
-    bar_init(smem_at(&c.rows), kGradThreads);
+    bar_init(smem_at(&c.rows), kGradThreads / 32);
     bar_init(smem_at(&c.scores), 1);
-    bar_init(smem_at(&c.taken), kGradThreads);
+    bar_init(smem_at(&c.taken), kGradThreads / 32);
     bar_init(smem_at(&c.slopes), 1);
-    bar_init(smem_at(&c.grads), kGradThreads);
+    bar_init(smem_at(&c.grads), kGradThreads / 32);
     bar_init(smem_at(&c.done), 1);
     c.lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -439,71 +442,83 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
 
   if (warp == kLoader) {
-    if (lane == 0) {
-      int i = 0;
-      for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
-        const int slot = i % F::kSlots;
-        const uint32_t bar = smem_at(&c.full[slot]);
-        if (i >= F::kSlots && !bar_wait(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+    int i = 0;
+    for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
+      const int slot = i % F::kSlots;
+      const uint32_t bar = smem_at(&c.full[slot]);
+      if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
+      const int j = first_of(i >> 1);
+      if (elect_one()) {
         bar_expect(bar, F::kTileBytes);
-        const int j = first_of(i >> 1);
+#pragma unroll
         for (int b = 0; b < F::kBlocks; ++b)
           tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * 16384), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
       }
-      if (*lost)
-        for (int k = max(0, i - F::kSlots); k < i; ++k) {
-          const unsigned long long t = nanoseconds();
-          while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
-        }
+      __syncwarp();
     }
+    if (*lost)
+      for (int k = max(0, i - F::kSlots); k < i; ++k) {
+        const unsigned long long t = nanoseconds();
+        while (!bar_try(smem_at(&c.full[k % F::kSlots]), (k / F::kSlots) & 1) && nanoseconds() - t < kWaitLimit) {}
+      }
   } else if (warp == kIssuer) {
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0) {
       const int depth = (p.D + 15) / 16;
       const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
-      const auto scores = [&](int left, int slot, int to) {
-        const uint32_t a = smem_at(base + left * F::kTileBytes), b = smem_at(ring + slot * F::kTileBytes);
-        for (int k = 0; k < depth; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          mma_ss(tmem + to, desc_k_major(a + off), desc_k_major(b + off), s_shape, k > 0);
+      const uint64_t rows_k = desc_k_major(smem_at(base)), ring_k = desc_k_major(smem_at(ring)), ring_mn = desc_mn_major(smem_at(ring), 16384);
+      const auto scores = [&](int left, int slot, int to, unsigned long long* bar) {
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+            if (k < depth)
+              mma_ss(tmem + to, rows_k + ((left * F::kTileBytes + off) >> 4), ring_k + ((slot * F::kTileBytes + off) >> 4), s_shape, k > 0);
+          }
+          mma_commit(smem_at(bar));
         }
+        __syncwarp();
       };
-      const auto wait_full = [&](int i) { return bar_wait(smem_at(&c.full[i % F::kSlots]), (i / F::kSlots) & 1, lost); };
-      bool ok = bar_wait(smem_at(&c.rows), 0, lost) && wait_full(0);
+      const auto commit = [&](unsigned long long* bar) {
+        if (elect_one()) mma_commit(smem_at(bar));
+        __syncwarp();
+      };
+      const auto wait_full = [&](int i) { return bar_wait_warp(smem_at(&c.full[i % F::kSlots]), (i / F::kSlots) & 1, lost); };
+      bool ok = bar_wait_warp(smem_at(&c.rows), 0, lost) && wait_full(0);
       if (ok) {
         tc_fence_after();
-        scores(0, 0, F::kScores);
-        mma_commit(smem_at(&c.scores));
+        scores(0, 0, F::kScores, &c.scores);
         if ((ok = wait_full(1))) {
           tc_fence_after();
-          scores(1, 1, F::kSlopes);
-          mma_commit(smem_at(&c.slopes));
-          mma_commit(smem_at(&c.empty[1]));
+          scores(1, 1, F::kSlopes, &c.slopes);
+          commit(&c.empty[1]);
         }
       }
       for (int i = 0; i < tiles && ok; ++i) {
         const int k = 2 * i, next = k + 2;
         if (i + 1 < tiles) {
-          if (!(ok = bar_wait(smem_at(&c.taken), i & 1, lost) && wait_full(next))) break;
+          if (!(ok = bar_wait_warp(smem_at(&c.taken), i & 1, lost) && wait_full(next))) break;
           tc_fence_after();
-          scores(0, next % F::kSlots, F::kScores);
-          mma_commit(smem_at(&c.scores));
+          scores(0, next % F::kSlots, F::kScores, &c.scores);
         }
-        if (!(ok = bar_wait(smem_at(&c.grads), i & 1, lost))) break;
-        if (MASK && !(ok = bar_wait(smem_at(&c.clean[k % F::kSlots]), (k / F::kSlots) & 1, lost))) break;
+        if (!(ok = bar_wait_warp(smem_at(&c.grads), i & 1, lost))) break;
+        if (MASK && !(ok = bar_wait_warp(smem_at(&c.clean[k % F::kSlots]), (k / F::kSlots) & 1, lost))) break;
         tc_fence_after();
-        const uint32_t b = smem_at(ring + (k % F::kSlots) * F::kTileBytes);
-        for (int e = 0; e < 8; ++e)
-          mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 2) * 64 + (e & 3) * 8, desc_mn_major(b + e * 2048, 16384), d_shape, i > 0 || e > 0);
-        mma_commit(smem_at(&c.empty[k % F::kSlots]));
+        if (elect_one()) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 1) * 32 + (e & 1) * 8, ring_mn + (((k % F::kSlots) * F::kTileBytes + e * 2048) >> 4),
+                   d_shape, i > 0 || e > 0);
+          mma_commit(smem_at(&c.empty[k % F::kSlots]));
+        }
+        __syncwarp();
         if (i + 1 < tiles) {
           if (!(ok = wait_full(next + 1))) break;
           tc_fence_after();
-          scores(1, (next + 1) % F::kSlots, F::kSlopes);
-          mma_commit(smem_at(&c.slopes));
-          mma_commit(smem_at(&c.empty[(next + 1) % F::kSlots]));
+          scores(1, (next + 1) % F::kSlots, F::kSlopes, &c.slopes);
+          commit(&c.empty[(next + 1) % F::kSlots]);
         }
       }
-      mma_commit(smem_at(&c.done));
+      commit(&c.done);
     }
   } else if (MASK && warp == kCleaner) {
     // rows of K that are left out may hold NaN: zero before they meet the zeros of dS
@@ -528,7 +543,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
-    const int r = threadIdx.x & 127, half = warp >> 2, j0 = o.first + r;
+    const int r = threadIdx.x & 127, part_of = warp >> 2, j0 = o.first + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const bool mine = some && j0 < o.rows;
     Row w = {};
@@ -544,59 +559,54 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       }
     }
     if (tiles > 0) {
-      const long long at = half ? w.r * p.g_r + w.t * p.g_t + w.h * p.g_h : w.r * p.q_r + w.t * p.q_t + w.h * p.q_h;
-      put_row<DP>(base + half * F::kTileBytes, r, mine ? (const char*)(half ? p.g : p.q) + at * 2 : nullptr, p.D);
+      const bool g = part_of & 1;
+      const long long at = g ? w.r * p.g_r + w.t * p.g_t + w.h * p.g_h : w.r * p.q_r + w.t * p.q_t + w.h * p.q_h;
+      const char* row = mine ? (const char*)(g ? p.g : p.q) + at * 2 : nullptr;
+      if (part_of & 2) put_row<DP>(base + g * F::kTileBytes, r, row, p.D, DP / 16, DP / 8);
+      else put_row<DP>(base + g * F::kTileBytes, r, row, p.D, 0, DP / 16);
       fence_async_proxy();
-      bar_arrive(smem_at(&c.rows));
+      bar_arrive_warp(smem_at(&c.rows));
     }
     const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
     bool ok = true;
     for (int i = 0; i < tiles; ++i) {
-      uint32_t bits[2] = {~0u, ~0u};
+      uint32_t bits = ~0u;
       if (MASK) {
-        const uint4 b = c.bits[i];
-        bits[0] = half ? b.z : b.x;
-        bits[1] = half ? b.w : b.y;
+        bits = word_of(c.bits[i], part_of);
       } else if (i + 1 == tiles && (end & 127)) {
-        const int left = (end & 127) - half * 64;
-        bits[0] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
-        bits[1] = left >= 64 ? ~0u : left > 32 ? (1u << (left - 32)) - 1 : 0;
+        const int left = (end & 127) - part_of * 32;
+        bits = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
       }
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.scores), i & 1, lost)))) break;
       tc_fence_after();
-      uint32_t v[2][32];
-      tmem_load32(v[0], tmem + lanes + F::kScores + half * 64);
-      tmem_load32(v[1], tmem + lanes + F::kScores + half * 64 + 32);
+      const int col = part_of * 32;
+      uint32_t v[32], u[16];
+      tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
       tc_fence_before();
-      bar_arrive(smem_at(&c.taken));
-      float2 wgt[32];
+      bar_arrive_warp(smem_at(&c.taken));
+      float2 wgt[16];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float2 x = fma2(make_float2(__uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1])), scale2, minus);
+      for (int e = 0; e < 16; ++e) {
+        const float2 x = fma2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, minus);
         const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
         wgt[e] = TcType<T>::code == 0 ? mul2(y, make_float2(factor, factor)) : y;
       }
       if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
       tc_fence_after();
-      tmem_load32(v[0], tmem + lanes + F::kSlopes + half * 64);
-      tmem_load32(v[1], tmem + lanes + F::kSlopes + half * 64 + 32);
+      tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t u[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 ds = mul2(wgt[q * 16 + e], add2(make_float2(__uint_as_float(v[q][2 * e]), __uint_as_float(v[q][2 * e + 1])), less));
-          if (bits[q] != ~0u) ds = make_float2((bits[q] >> (2 * e)) & 1 ? ds.x : 0.0f, (bits[q] >> (2 * e + 1)) & 1 ? ds.y : 0.0f);
-          u[e] = pack2<T>(ds.x, ds.y);
-        }
-        tmem_store16(tmem + lanes + F::kSlopes + half * 64 + q * 16, u);
+      for (int e = 0; e < 16; ++e) {
+        float2 ds = mul2(wgt[e], add2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), less));
+        if (bits != ~0u) ds = make_float2((bits >> (2 * e)) & 1 ? ds.x : 0.0f, (bits >> (2 * e + 1)) & 1 ? ds.y : 0.0f);
+        u[e] = pack2<T>(ds.x, ds.y);
       }
+      tmem_store16(tmem + lanes + F::kSlopes + col, u);
       tmem_wait_store();
       tc_fence_before();
-      bar_arrive(smem_at(&c.grads));
+      bar_arrive_warp(smem_at(&c.grads));
     }
     if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
     if (__all_sync(~0u, ok)) {
@@ -604,7 +614,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       const long long rows = (long long)p.R * p.T * p.Hq;
       float* part = p.splits > 1 ? p.part_gq + (split * rows + number) * p.D : nullptr;
 #pragma unroll 1
-      for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
+      for (int q = part_of; q < DP / 32; q += 4) {
         if (q * 32 >= p.D) break;
         put_sums<T>(tmem + lanes + F::kSums + q * 32, (part ? 1.0f : p.scale) / factor, (T*)p.gq + number * p.D, part, q * 32, p.D, mine,
                     tiles > 0);

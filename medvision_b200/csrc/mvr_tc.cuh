@@ -18,6 +18,11 @@ __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// One arrival of a warp, behind what all its lanes did before (an arrival of every lane is 32 accesses, one after another).
+__device__ __forceinline__ void bar_arrive_warp(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(bar);
+}
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -59,6 +64,28 @@ __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volati
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* lost) {
   if (bar_try(bar, parity) || bar_try(bar, parity)) return true;
   return bar_wait_slow(bar, parity, lost);
+}
+
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* lost) {
+  return __all_sync(~0u, bar_wait(bar, parity, lost));
+}
+// One lane of a converged warp.  (The products and copies below take their operands from registers that a warp shares: in a branch
+// that elect.sync guards the compiler knows that one thread runs; behind a comparison of the lane it would issue them in a loop over
+// the lanes.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t lane = 0, is = 0;
+  asm volatile(
+      "{\n"
+      "  .reg .b32 r;\n"
+      "  .reg .pred p;\n"
+      "  elect.sync r|p, %2;\n"
+      "  @p mov.s32 %1, 1;\n"
+      "  mov.s32 %0, r;\n"
+      "}\n"
+      : "+r"(lane), "+r"(is)
+      : "r"(0xffffffffu));
+  return is != 0;
 }
 
 // Writes of this thread to shared memory become visible to TMA and the tensor cores.
