@@ -67,16 +67,16 @@ __device__ __forceinline__ void put_sums(uint32_t at, float factor, T* to, float
 template <int DP>
 struct TcStates {
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128;
-  static constexpr int kLoaders = 64, kThreads = kGradThreads + kLoaders + 32;
+  static constexpr int kLoaders = 64, kThreads = kGradThreads + kLoaders + 32, kStages = DP == 64 ? 4 : 2;
   static constexpr int kScores = 0, kSlopes = 128, kValues = 256, kKeys = 256 + DP, kColumns = 512;
   struct Control {
-    unsigned long long states, full[2], empty[2], scores, slopes, weights, grads, done;
+    unsigned long long states, full[kStages], empty[kStages], scores, slopes, weights, grads, done;
     uint32_t tmem;
     int lost, peak;
-    alignas(16) float lse[2][128];    // negative
-    alignas(16) float delta[2][128];  // negative
+    alignas(16) float lse[kStages][128];    // negative
+    alignas(16) float delta[kStages][128];  // negative
   };
-  static constexpr size_t kShared = 6 * (size_t)kTileBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = (2 + 2 * kStages) * (size_t)kTileBytes + sizeof(Control) + 1024;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
@@ -88,13 +88,13 @@ __global__ void __launch_bounds__(TcStates<DP>::kThreads, 1)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
   typedef TcStates<DP> F;
   extern __shared__ char tc_smem[];
-  char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of two stages
-  typename F::Control& c = *(typename F::Control*)(base + 6 * F::kTileBytes);
+  char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of the stages
+  typename F::Control& c = *(typename F::Control*)(base + (2 + 2 * F::kStages) * F::kTileBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoader = kGradThreads / 32, kIssuer = kLoader + F::kLoaders / 32;
   if (threadIdx.x == 0) {
     bar_init(smem_at(&c.states), 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < F::kStages; ++i) {
       bar_init(smem_at(&c.full[i]), F::kLoaders / 32);
       bar_init(smem_at(&c.empty[i]), 1);
     }
@@ -121,7 +121,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0;
   // what lies behind D in the rows' tiles stays 0
   if (count > 0 && p.D < DP) {
-    for (int e = threadIdx.x; e < 4 * F::kTileBytes / 16; e += F::kThreads)
+    for (int e = threadIdx.x; e < 2 * F::kStages * F::kTileBytes / 16; e += F::kThreads)
       *(uint4*)(base + 2 * F::kTileBytes + e * 16) = make_uint4(0, 0, 0, 0);
     fence_async_proxy();
   }
@@ -178,12 +178,12 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         scores(1, 3, F::kSlopes, &c.slopes);
       }
       for (int i = 0; i < count && ok; ++i) {
-        const int now = i & 1, next = now ^ 1;
+        const int now = i % F::kStages, next = (i + 1) % F::kStages;
         if (!(ok = bar_wait_warp(smem_at(&c.weights), i & 1, lost))) break;
         tc_fence_after();
         sums(F::kScores, 3 + 2 * now, F::kValues, i > 0);
         if (i + 1 < count) {
-          if (!(ok = bar_wait_warp(smem_at(&c.full[next]), ((i + 1) >> 1) & 1, lost))) break;
+          if (!(ok = bar_wait_warp(smem_at(&c.full[next]), ((i + 1) / F::kStages) & 1, lost))) break;
           tc_fence_after();
           scores(0, 2 + 2 * next, F::kScores, &c.scores);
         }
@@ -200,54 +200,68 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
     }
   } else if (warp >= kLoader) {
-    // rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places handed round by shuffles
+    // Rows of Q and G, 16 bytes a copy: two times 32 rows of a warp, their places handed round by shuffles.  Where the rows of the
+    // next tile lie is looked up while the copies of this one are under way.
+    constexpr int kGroups = 128 / F::kLoaders;
     const int chunks = p.D / 8;  // 16-byte pieces of a row
+    const char *q[kGroups], *g[kGroups];
+    float lse[kGroups], delta[kGroups];
+    const auto look_up = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int at = (first + i) * 128 + (warp - kLoader) * 32 + k * F::kLoaders + lane;
+        q[k] = g[k] = nullptr;
+        lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
+        if (i < count && at < o.rows) {
+          const Row row = row_of(p, o, at, hk);
+          q[k] = (const char*)p.q + (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
+          g[k] = (const char*)p.g + (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
+          const long long number = row_number(p, row);
+          lse[k] = p.lse[number];
+          delta[k] = p.delta[number];
+        }
+      }
+    };
     const auto arrived = [&](int stage) {
       fence_async_proxy();
       bar_arrive_warp(smem_at(&c.full[stage]));
     };
+    look_up(0);
+    bool pending = false;
     for (int i = 0; i < count; ++i) {
-      const int stage = i & 1;
-      if (i >= 2 && !__all_sync(~0u, bar_wait(smem_at(&c.empty[stage]), ((i >> 1) - 1) & 1, lost))) break;
+      const int stage = i % F::kStages;
+      if (i >= F::kStages && !bar_wait_warp(smem_at(&c.empty[stage]), (i / F::kStages - 1) & 1, lost)) break;
       const uint32_t qs = smem_at(base + (2 + 2 * stage) * F::kTileBytes), gs = qs + F::kTileBytes;
-#pragma unroll 1
-      for (int w = warp - kLoader; w < 4; w += F::kLoaders / 32) {
-        const int mine = (w << 5) + lane, at = (first + i) * 128 + mine;
-        const char *q = (const char*)p.q, *g = (const char*)p.g;
-        const bool row_in = at < o.rows;
-        float lse = INFINITY, delta = 0.0f;  // no row: P = 0
-        if (row_in) {
-          const Row row = row_of(p, o, at, hk);
-          q += (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
-          g += (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
-          const long long number = row_number(p, row);
-          lse = p.lse[number];
-          lse = lse == -INFINITY ? INFINITY : lse - shift;
-          delta = p.delta[number];
-        }
-        c.lse[stage][mine] = -lse;
-        c.delta[stage][mine] = -delta;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int mine = (warp - kLoader) * 32 + k * F::kLoaders;
+        c.lse[stage][mine + lane] = lse[k] == -INFINITY ? -INFINITY : shift - lse[k];
+        c.delta[stage][mine + lane] = -delta[k];
 #pragma unroll 4
         for (int e = 0; e < DP / 8; ++e) {
-          const int idx = e * 32 + lane, k = idx / (DP / 8), piece = idx % (DP / 8), row = (w << 5) + k;
-          const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q, k);
-          const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g, k);
-          const bool there = __shfl_sync(~0u, row_in, k);
+          const int idx = e * 32 + lane, from = idx / (DP / 8), piece = idx % (DP / 8), row = mine + from;
+          const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q[k], from);
+          const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g[k], from);
+          const bool there = qk != nullptr;
           if (piece < chunks) {
             const uint32_t to = (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-            copy16(qs + to, there ? qk + piece * 16 : qk, there);
-            copy16(gs + to, there ? gk + piece * 16 : gk, there);
+            copy16(qs + to, there ? qk + piece * 16 : (const char*)p.q, there);
+            copy16(gs + to, there ? gk + piece * 16 : (const char*)p.g, there);
           }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      if (i == 0 && count > 1) continue;  // the first two stages are both under way before either is waited for
-      if (i == 1) {
+      look_up(i + 1);
+      // the first stages are told of behind the copies of the next; from the last on, a stage is waited for at once
+      if (pending) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
-        arrived(0);
+        arrived((i - 1) % F::kStages);
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      arrived(stage);
+      pending = i + 1 < count && i + 1 < F::kStages;
+      if (!pending) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        arrived(stage);
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
@@ -282,8 +296,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
     const uint32_t keep = in ? ~0u : 0u;  // a state that is not read: zeros, whatever its scores are
     for (int i = 0; i < count; ++i) {
-      const int stage = i & 1;
-      ok = ok && bar_wait(smem_at(&c.full[stage]), (i >> 1) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
+      const int stage = i % F::kStages;
+      ok = ok && bar_wait(smem_at(&c.full[stage]), (i / F::kStages) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
       if (!(ok = __all_sync(~0u, ok))) break;
       tc_fence_after();
       const int col = part_of * 32;
