@@ -23,6 +23,30 @@ constexpr int kPolynomials = 2;  // of eight pairs of exponentials, how many are
 
 constexpr int kTcRows = 128, kTcStates = 128, kTcMaxTiles = 512;  // tiles of states that one CTA can list
 
+// Which of STEP states may be read.
+template <int STEP>
+struct StateBits {
+  uint32_t w[STEP / 32];
+  __device__ __forceinline__ uint32_t word(int i) const {
+    uint32_t r = w[0];
+#pragma unroll
+    for (int k = 1; k < STEP / 32; ++k) r = i == k ? w[k] : r;
+    return r;
+  }
+  __device__ __forceinline__ bool any() const {
+    uint32_t r = 0;
+#pragma unroll
+    for (int k = 0; k < STEP / 32; ++k) r |= w[k];
+    return r != 0;
+  }
+  __device__ __forceinline__ bool all() const {
+    uint32_t r = ~0u;
+#pragma unroll
+    for (int k = 0; k < STEP / 32; ++k) r &= w[k];
+    return r == ~0u;
+  }
+};
+
 template <int DP, int TILES, bool MASK>
 struct TcForward {
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128;       // a tile of rows or states
@@ -36,7 +60,7 @@ struct TcForward {
     int lost, tiles;
     float top[2][TILES][2][128];  // what the two halves of a row tell each other
     unsigned short list[MASK ? kTcMaxTiles : 1];
-    uint4 bits[MASK ? kTcMaxTiles : 1];
+    StateBits<kTcStates> bits[MASK ? kTcMaxTiles : 1];
   };
   static constexpr size_t kShared = (size_t)(TILES + kSlots) * kTileBytes + sizeof(Control) + 1024;
 };
@@ -45,23 +69,18 @@ struct TcMaps {
   CUtensorMap k, v;
 };
 
-// Bits of the states [first, first + 128) that may be read, of `end` and the mask; the same in all lanes.
-__device__ __forceinline__ uint4 state_bits(const AttnParams& p, int n, int first, int end, int lane) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = first + i * 32 + lane;
-    w[i] = __ballot_sync(~0u, j < end && (!p.mask || p.mask[(long long)n * p.L + j] != 0));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// List of the tiles of 128 states in [begin, end) that have one to read, with their bits.  All threads; the result after a barrier.
-__device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin, int end, unsigned short* list, uint4* bits, int* count) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, tiles = (end - begin + kTcStates - 1) / kTcStates;
+// List of the tiles of STEP states in [begin, end) that have one to read, with their bits.  All threads; the result after a barrier.
+template <int STEP>
+__device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin, int end, unsigned short* list, StateBits<STEP>* bits,
+                                           int* count) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, tiles = (end - begin + STEP - 1) / STEP;
   for (int i = threadIdx.x >> 5; i < tiles; i += warps) {
-    const uint4 b = state_bits(p, n, begin + i * kTcStates, end, lane);
+    StateBits<STEP> b;
+#pragma unroll
+    for (int k = 0; k < STEP / 32; ++k) {
+      const int j = begin + i * STEP + k * 32 + lane;
+      b.w[k] = __ballot_sync(~0u, j < end && (!p.mask || p.mask[(long long)n * p.L + j] != 0));
+    }
     if (lane == 0) bits[i] = b;
   }
   __syncthreads();
@@ -69,9 +88,9 @@ __device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin
     int at = 0;
     for (int base = 0; base < tiles; base += 32) {
       const int i = base + lane;
-      uint4 b = make_uint4(0, 0, 0, 0);
+      StateBits<STEP> b = {};
       if (i < tiles) b = bits[i];
-      const bool any = (b.x | b.y | b.z | b.w) != 0;
+      const bool any = b.any();
       const uint32_t who = __ballot_sync(~0u, any);
       __syncwarp();
       if (any) {  // (at + rank <= i: what is overwritten has been read)
@@ -84,6 +103,23 @@ __device__ __forceinline__ void list_tiles(const AttnParams& p, int n, int begin
     }
     if (lane == 0) *count = at;
   }
+}
+
+// Rows of states that are left out become 0 in a tile of STEP rows in shared memory.  One warp.
+template <int STEP, int BLOCKS>
+__device__ __forceinline__ void clear_rows(char* tile, const StateBits<STEP>& b, int lane) {
+  if (b.all()) return;
+#pragma unroll
+  for (int w = 0; w < STEP / 32; ++w) {
+    uint32_t out = ~b.w[w];
+    while (out) {
+      const int r = w * 32 + __ffs(out) - 1;
+      out &= out - 1;
+      if (lane < 8 * BLOCKS) *(uint4*)(tile + (lane >> 3) * (STEP * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_async_proxy();
+  __syncwarp();
 }
 
 // A row of 2-byte elements into a K-major tile in the 128-byte swizzle; zeros behind D, and for no row at all.
@@ -172,12 +208,8 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       const uint64_t queries = desc_k_major(smem_at(base)), keys = desc_k_major(smem_at(ring)), values = desc_mn_major(smem_at(ring), kTcRows * 128);
       const auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t off = (k >> 2) * (kTcRows * 128) + (k & 3) * 32;
-            if (k < depth)
-              mma_ss(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes + off) >> 4), keys + ((slot * F::kTileBytes + off) >> 4), s_shape, k > 0);
-          }
+          mma_rows<DP / 16>(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes) >> 4), keys + ((slot * F::kTileBytes) >> 4), s_shape, depth,
+                            kTcRows * 128, kTcRows * 128);
           mma_commit(smem_at(&c.scores[t]));
         }
         __syncwarp();
@@ -186,41 +218,38 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         if (elect_one()) mma_commit(smem_at(bar));
         __syncwarp();
       };
-      bool ok = true;
-      for (int t = 0; t < used && ok; ++t) ok = bar_wait_warp(smem_at(&c.queries[t]), 0, lost);
-      ok = ok && bar_wait_warp(smem_at(&c.full[0]), 0, lost);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < used; ++t) scores(t, 0);
-        commit(&c.empty[0]);
-      }
-      for (int j = 0; j < tiles && ok; ++j) {
+      for (int t = 0; t < used; ++t) bar_pass(smem_at(&c.queries[t]), 0, lost);
+      bar_pass(smem_at(&c.full[0]), 0, lost);
+      tc_fence_after();
+      for (int t = 0; t < used; ++t) scores(t, 0);
+      commit(&c.empty[0]);
+      for (int j = 0; j < tiles; ++j) {
         const int v = 2 * j + 1, k = v + 1, vs = v % F::kSlots, ks = k % F::kSlots;
-        ok = bar_wait_warp(smem_at(&c.full[vs]), (v / F::kSlots) & 1, lost);
-        if (MASK && ok) ok = bar_wait_warp(smem_at(&c.clean[vs]), (v / F::kSlots) & 1, lost);
+        bar_pass(smem_at(&c.full[vs]), (v / F::kSlots) & 1, lost);
+        if (MASK) bar_pass(smem_at(&c.clean[vs]), (v / F::kSlots) & 1, lost);
+        if (j + 1 < tiles) bar_pass(smem_at(&c.full[ks]), (k / F::kSlots) & 1, lost);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-          if (t >= used || !ok) break;
-          ok = bar_wait_warp(smem_at(&c.weights[t]), j & 1, lost);
-          if (!ok) break;
+          if (t >= used) break;
+          bar_pass(smem_at(&c.weights[t]), j & 1, lost);
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < kTcStates / 16; ++i)  // O_t += P_t V
               mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * 128 + (i >> 2) * 64 + (i & 3) * 8,
                      values + ((vs * F::kTileBytes + i * 2048) >> 4), o_shape, j > 0 || i > 0);
-          }
-          __syncwarp();
-          if (j + 1 < tiles) {
-            if (t == 0) ok = bar_wait_warp(smem_at(&c.full[ks]), (k / F::kSlots) & 1, lost);
-            if (ok) {
-              tc_fence_after();
-              scores(t, ks);
+            if (j + 1 < tiles) {
+              mma_rows<DP / 16>(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes) >> 4), keys + ((ks * F::kTileBytes) >> 4), s_shape, depth,
+                                kTcRows * 128, kTcRows * 128);
+              mma_commit(smem_at(&c.scores[t]));
+            }
+            if (t + 1 == used) {
+              mma_commit(smem_at(&c.empty[vs]));
+              if (j + 1 < tiles) mma_commit(smem_at(&c.empty[ks]));
             }
           }
+          __syncwarp();
         }
-        commit(&c.empty[vs]);
-        if (j + 1 < tiles) commit(&c.empty[ks]);
       }
       for (int t = 0; t < TILES; ++t) commit(&c.out[t]);
     }
@@ -228,21 +257,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     for (int j = 0; j < tiles; ++j) {
       const int v = 2 * j + 1, slot = v % F::kSlots;
       if (!bar_wait(smem_at(&c.full[slot]), (v / F::kSlots) & 1, lost)) break;
-      const uint4 b = c.bits[j];
-      if ((b.x & b.y & b.z & b.w) != ~0u) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t out = ~word_of(b, w);
-          while (out) {
-            const int r = w * 32 + __ffs(out) - 1;
-            out &= out - 1;
-            if (lane < 8 * F::kBlocks)
-              *(uint4*)(ring + slot * F::kTileBytes + (lane >> 3) * (kTcRows * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_async_proxy();
-        __syncwarp();
-      }
+      clear_rows<kTcStates, F::kBlocks>(ring + slot * F::kTileBytes, c.bits[j], lane);
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
@@ -261,23 +276,17 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
       float m = -INFINITY, l = 0.0f;  // m: in the units of S, the same in both halves; l: of this half
-      bool ok = true;
       for (int j = 0; j < tiles; ++j) {
         uint32_t bits[2] = {~0u, ~0u};
         if (MASK) {
-          const uint4 b = c.bits[j];
-          bits[0] = half ? b.z : b.x;
-          bits[1] = half ? b.w : b.y;
+          bits[0] = c.bits[j].w[half * 2];
+          bits[1] = c.bits[j].w[half * 2 + 1];
         } else if (j + 1 == tiles && (end & 127)) {
           const int left = (end & 127) - half * 64;
           bits[0] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
           bits[1] = left >= 64 ? ~0u : left > 32 ? (1u << (left - 32)) - 1 : 0;
         }
-        ok = bar_wait(smem_at(&c.scores[t]), j & 1, lost);
-        if (!__all_sync(~0u, ok)) {
-          ok = false;
-          break;
-        }
+        bar_pass(smem_at(&c.scores[t]), j & 1, lost);
         tc_fence_after();
         // scores of 32 states, those that are left out as -inf
         const auto settle = [&](uint32_t (&v)[32], int q) {
@@ -309,11 +318,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         // the row's maximum, of both halves
         c.top[j & 1][t][half][r] = top;
         bar_arrive_warp(smem_at(&c.halves[t]));
-        ok = bar_wait(smem_at(&c.halves[t]), j & 1, lost);
-        if (!__all_sync(~0u, ok)) {
-          ok = false;
-          break;
-        }
+        bar_pass(smem_at(&c.halves[t]), j & 1, lost);
         top = max3(top, c.top[j & 1][t][half ^ 1][r], top);
         if (top == INFINITY) top = NAN;  // (as inf - inf is; the sums are NaN from here on)
         // move the maximum?  (the first tile: there is no O yet)
@@ -361,10 +366,10 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       // the halves' sums together (a + b is b + a: the same in both)
       c.top[tiles & 1][t][half][r] = l;
       bar_arrive_warp(smem_at(&c.halves[t]));
-      ok = ok && bar_wait(smem_at(&c.halves[t]), tiles & 1, lost);
+      bar_pass(smem_at(&c.halves[t]), tiles & 1, lost);
       l += c.top[tiles & 1][t][half ^ 1][r];
-      if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.out[t]), 0, lost);
-      if (__all_sync(~0u, ok)) {
+      if (tiles > 0) bar_pass(smem_at(&c.out[t]), 0, lost);
+      if (__all_sync(~0u, *lost == 0)) {
         tc_fence_after();
         const long long row = row_number(p, w), rows = (long long)p.R * p.T * p.Hq;
         if (m == -INFINITY) l = 0.0f;  // no state, or only scores of -inf

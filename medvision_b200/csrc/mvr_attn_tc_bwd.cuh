@@ -6,8 +6,10 @@
 //   states kept:  S^T = K Q^T    dP^T = V G^T    dV += P^T G    dK += dS^T Q           dS = P (dP - delta)
 //   rows kept:    S   = Q K^T    dP   = G V^T    dQ += dS K
 //
-// Scores, dP and the sums are in tensor memory; P and dS, rounded to T, go back over the scores and dP as left operands.  Four
-// warpgroups share a tile, a quarter of a row a thread: with two, a warp's own latencies set the pace.  One thread issues the products in an order in which those of
+// Scores, dP and the sums are in tensor memory; P and dS, rounded to T, go back over the scores and dP as left operands.  A
+// warpgroup takes 32 columns of a tile, one row a thread.  A tile's chain (scores, exponentials, dP, dS, products) leaves every unit
+// idle for a part of it, so up to 64 columns of a head two CTAs share an SM, each 128 x 64 at a time; beyond, tensor memory holds the
+// sums of one CTA only, which takes 128 x 128.  One thread issues the products in an order in which those of
 // one tile run under the exponentials of the next: dV(i), S(i+1), dK(i), dP(i+1), and S(i+1), dQ(i), dP(i+1).
 //
 // float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= 2 D max|g| max|v|
@@ -18,9 +20,10 @@
 
 namespace mvr {
 
-constexpr int kGradThreads = 512;  // of the four warpgroups
+template <int DP>
+constexpr int kGradStep = DP == 64 ? 64 : 128;  // columns of a tile
 
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
 // Power of two for dS, from bounds of |g| and |v| (float bits).
 template <typename T>
@@ -66,17 +69,18 @@ __device__ __forceinline__ void put_sums(uint32_t at, float factor, T* to, float
 // ---- states kept: dk, dv ------------------------------------------------------------------------------
 template <int DP>
 struct TcStates {
-  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128;
-  static constexpr int kLoaders = 64, kThreads = kGradThreads + kLoaders + 32, kStages = DP == 64 ? 4 : 2;
-  static constexpr int kScores = 0, kSlopes = 128, kValues = 256, kKeys = 256 + DP, kColumns = 512;
+  static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128;
+  static constexpr int kGroups = kStep * 4, kLoaders = 64, kThreads = kGroups + kLoaders + 32, kStages = DP == 64 ? 3 : 2;
+  static constexpr int kScores = 0, kSlopes = kStep, kValues = 2 * kStep, kKeys = 2 * kStep + DP, kColumns = 2 * kStep + 2 * DP;
+  static constexpr int kResident = DP == 64 ? 2 : 1;
   struct Control {
     unsigned long long states, full[kStages], empty[kStages], scores, slopes, weights, grads, done;
     uint32_t tmem;
     int lost, peak;
-    alignas(16) float lse[kStages][128];    // negative
-    alignas(16) float delta[kStages][128];  // negative
+    alignas(16) float lse[kStages][kStep];    // negative
+    alignas(16) float delta[kStages][kStep];  // negative
   };
-  static constexpr size_t kShared = (2 + 2 * kStages) * (size_t)kTileBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = 2 * (size_t)kTileBytes + 2 * kStages * (size_t)kStepBytes + sizeof(Control) + 1024;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
@@ -84,14 +88,14 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(TcStates<DP>::kThreads, 1)
+__global__ void __launch_bounds__(TcStates<DP>::kThreads, TcStates<DP>::kResident)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
   typedef TcStates<DP> F;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of the stages
-  typename F::Control& c = *(typename F::Control*)(base + (2 + 2 * F::kStages) * F::kTileBytes);
+  typename F::Control& c = *(typename F::Control*)(base + 2 * F::kTileBytes + 2 * F::kStages * F::kStepBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kLoader = kGradThreads / 32, kIssuer = kLoader + F::kLoaders / 32;
+  constexpr int kLoader = F::kGroups / 32, kIssuer = kLoader + F::kLoaders / 32;
   if (threadIdx.x == 0) {
     bar_init(smem_at(&c.states), 1);
     for (int i = 0; i < F::kStages; ++i) {
@@ -100,8 +104,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     }
     bar_init(smem_at(&c.scores), 1);
     bar_init(smem_at(&c.slopes), 1);
-    bar_init(smem_at(&c.weights), kGradThreads / 32);
-    bar_init(smem_at(&c.grads), kGradThreads / 32);
+    bar_init(smem_at(&c.weights), F::kGroups / 32);
+    bar_init(smem_at(&c.grads), F::kGroups / 32);
     bar_init(smem_at(&c.done), 1);
     c.lost = 0;
     c.peak = 0;
@@ -117,11 +121,11 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   if (warp < kLoader) in = j < states_of(p, n) && (!p.mask || p.mask[(long long)n * p.L + j] != 0);
   const bool any = __syncthreads_or(in);
   const RowTile o = image_rows(p, n);
-  const int row_tiles = (o.rows + 127) / 128, per = (row_tiles + p.row_splits - 1) / p.row_splits;
+  const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   const int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0;
   // what lies behind D in the rows' tiles stays 0
   if (count > 0 && p.D < DP) {
-    for (int e = threadIdx.x; e < 2 * F::kStages * F::kTileBytes / 16; e += F::kThreads)
+    for (int e = threadIdx.x; e < 2 * F::kStages * F::kStepBytes / 16; e += F::kThreads)
       *(uint4*)(base + 2 * F::kTileBytes + e * 16) = make_uint4(0, 0, 0, 0);
     fence_async_proxy();
   }
@@ -139,31 +143,31 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         bar_expect(smem_at(&c.states), 2 * F::kTileBytes);
 #pragma unroll
         for (int b = 0; b < F::kBlocks; ++b) {
-          tma_load_4d(smem_at(base + b * 16384), &maps.k, smem_at(&c.states), b * 64, hk, j0, n);
-          tma_load_4d(smem_at(base + F::kTileBytes + b * 16384), &maps.v, smem_at(&c.states), b * 64, hk, j0, n);
+#pragma unroll
+          for (int r = 0; r < 128; r += F::kStep) {  // (boxes of as many states as the other kernel takes)
+            tma_load_4d(smem_at(base + b * 16384 + r * 128), &maps.k, smem_at(&c.states), b * 64, hk, j0 + r, n);
+            tma_load_4d(smem_at(base + F::kTileBytes + b * 16384 + r * 128), &maps.v, smem_at(&c.states), b * 64, hk, j0 + r, n);
+          }
         }
       }
       __syncwarp();
       const int depth = (p.D + 15) / 16;
-      const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
-      const uint64_t tiles_k = desc_k_major(smem_at(base)), tiles_mn = desc_mn_major(smem_at(base), 16384);
-      const auto scores = [&](int left, int right, int to, unsigned long long* bar) {  // 128 x 128 over D, both K-major
+      const uint32_t s_shape = tc_shape<T>(F::kStep, false), d_shape = tc_shape<T>(depth * 16, true);
+      const char* steps = base + 2 * F::kTileBytes;
+      const uint64_t tiles_k = desc_k_major(smem_at(base)), steps_k = desc_k_major(smem_at(steps)), steps_mn = desc_mn_major(smem_at(steps), F::kStep * 128);
+      const auto scores = [&](int left, int right, int to, unsigned long long* bar) {  // 128 x kStep over D, both K-major
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            if (k < depth)
-              mma_ss(tmem + to, tiles_k + ((left * F::kTileBytes + off) >> 4), tiles_k + ((right * F::kTileBytes + off) >> 4), s_shape, k > 0);
-          }
+          mma_rows<DP / 16>(tmem + to, tiles_k + ((left * F::kTileBytes) >> 4), steps_k + ((right * F::kStepBytes) >> 4), s_shape, depth, 16384,
+                            F::kStep * 128);
           mma_commit(smem_at(bar));
         }
         __syncwarp();
       };
-      const auto sums = [&](int from, int right, int to, bool add) {  // over the 128 rows
+      const auto sums = [&](int from, int right, int to, bool add) {  // over the rows
         if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + (i & 1) * 8, tiles_mn + ((right * F::kTileBytes + i * 2048) >> 4), d_shape, add || i > 0);
+          for (int i = 0; i < F::kStep / 16; ++i)
+            mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + (i & 1) * 8, steps_mn + ((right * F::kStepBytes + i * 2048) >> 4), d_shape, add || i > 0);
         }
         __syncwarp();
       };
@@ -171,27 +175,26 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         if (elect_one()) mma_commit(smem_at(bar));
         __syncwarp();
       };
-      bool ok = bar_wait_warp(smem_at(&c.states), 0, lost) && bar_wait_warp(smem_at(&c.full[0]), 0, lost);
-      if (ok) {
-        tc_fence_after();
-        scores(0, 2, F::kScores, &c.scores);
-        scores(1, 3, F::kSlopes, &c.slopes);
-      }
-      for (int i = 0; i < count && ok; ++i) {
+      bar_pass(smem_at(&c.states), 0, lost);
+      bar_pass(smem_at(&c.full[0]), 0, lost);
+      tc_fence_after();
+      scores(0, 0, F::kScores, &c.scores);
+      scores(1, 1, F::kSlopes, &c.slopes);
+      for (int i = 0; i < count; ++i) {
         const int now = i % F::kStages, next = (i + 1) % F::kStages;
-        if (!(ok = bar_wait_warp(smem_at(&c.weights), i & 1, lost))) break;
+        bar_pass(smem_at(&c.weights), i & 1, lost);
         tc_fence_after();
-        sums(F::kScores, 3 + 2 * now, F::kValues, i > 0);
+        sums(F::kScores, 1 + 2 * now, F::kValues, i > 0);
         if (i + 1 < count) {
-          if (!(ok = bar_wait_warp(smem_at(&c.full[next]), ((i + 1) / F::kStages) & 1, lost))) break;
+          bar_pass(smem_at(&c.full[next]), ((i + 1) / F::kStages) & 1, lost);
           tc_fence_after();
-          scores(0, 2 + 2 * next, F::kScores, &c.scores);
+          scores(0, 2 * next, F::kScores, &c.scores);
         }
-        if (!(ok = bar_wait_warp(smem_at(&c.grads), i & 1, lost))) break;
+        bar_pass(smem_at(&c.grads), i & 1, lost);
         tc_fence_after();
-        sums(F::kSlopes, 2 + 2 * now, F::kKeys, i > 0);
+        sums(F::kSlopes, 2 * now, F::kKeys, i > 0);
         commit(&c.empty[now]);
-        if (i + 1 < count) scores(1, 3 + 2 * next, F::kSlopes, &c.slopes);
+        if (i + 1 < count) scores(1, 1 + 2 * next, F::kSlopes, &c.slopes);
       }
       commit(&c.done);
       if (*lost) {
@@ -200,16 +203,16 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
     }
   } else if (warp >= kLoader) {
-    // Rows of Q and G, 16 bytes a copy: two times 32 rows of a warp, their places handed round by shuffles.  Where the rows of the
+    // Rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places handed round by shuffles.  Where the rows of the
     // next tile lie is looked up while the copies of this one are under way.
-    constexpr int kGroups = 128 / F::kLoaders;
+    constexpr int kGroups = F::kStep / F::kLoaders;
     const int chunks = p.D / 8;  // 16-byte pieces of a row
     const char *q[kGroups], *g[kGroups];
     float lse[kGroups], delta[kGroups];
     const auto look_up = [&](int i) {
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
-        const int at = (first + i) * 128 + (warp - kLoader) * 32 + k * F::kLoaders + lane;
+        const int at = (first + i) * F::kStep + (warp - kLoader) * 32 + k * F::kLoaders + lane;
         q[k] = g[k] = nullptr;
         lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
         if (i < count && at < o.rows) {
@@ -231,7 +234,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     for (int i = 0; i < count; ++i) {
       const int stage = i % F::kStages;
       if (i >= F::kStages && !bar_wait_warp(smem_at(&c.empty[stage]), (i / F::kStages - 1) & 1, lost)) break;
-      const uint32_t qs = smem_at(base + (2 + 2 * stage) * F::kTileBytes), gs = qs + F::kTileBytes;
+      const uint32_t qs = smem_at(base + 2 * F::kTileBytes + 2 * stage * F::kStepBytes), gs = qs + F::kStepBytes;
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
         const int mine = (warp - kLoader) * 32 + k * F::kLoaders;
@@ -244,7 +247,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g[k], from);
           const bool there = qk != nullptr;
           if (piece < chunks) {
-            const uint32_t to = (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            const uint32_t to = (piece >> 3) * (F::kStep * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
             copy16(qs + to, there ? qk + piece * 16 : (const char*)p.q, there);
             copy16(gs + to, there ? gk + piece * 16 : (const char*)p.g, there);
           }
@@ -267,16 +270,15 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   } else {
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float factor = 1.0f;  // of dS
-    bool ok = true;
     if (count > 0 && TcType<T>::code == 0) {
-      ok = __all_sync(~0u, bar_wait(smem_at(&c.states), 0, lost));
+      bar_pass(smem_at(&c.states), 0, lost);
       // largest |v| of the states that are read
       float most = 0.0f;
-      if (ok && in) {
+      if (in) {
         const char* row = base + F::kTileBytes + r * 128;
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) {
-          const int piece = part_of * (DP / 32) + e;
+        for (int e = 0; e < DP * 16 / F::kGroups; ++e) {
+          const int piece = part_of * (DP * 16 / F::kGroups) + e;
           const uint4 v = *(const uint4*)(row + (piece >> 3) * 16384 + (((piece ^ r) & 7) << 4));
           const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -288,17 +290,17 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
       if (lane == 0) atomicMax(&c.peak, __float_as_int(most));
-      group_sync();
+      group_sync(F::kGroups);
       const float peak = __int_as_float(c.peak);
       if (threadIdx.x == 0) atomicMax((int*)peaks + 1, c.peak);
       factor = slope_scale<T>(p.D, peaks[0], peak);
     }
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
-    const uint32_t keep = in ? ~0u : 0u;  // a state that is not read: zeros, whatever its scores are
+    // (A state that is not read is a row of its own in both products: whatever comes of it reaches no other, and is not stored.)
     for (int i = 0; i < count; ++i) {
       const int stage = i % F::kStages;
-      ok = ok && bar_wait(smem_at(&c.full[stage]), (i / F::kStages) & 1, lost) && bar_wait(smem_at(&c.scores), i & 1, lost);
-      if (!(ok = __all_sync(~0u, ok))) break;
+      bar_pass(smem_at(&c.full[stage]), (i / F::kStages) & 1, lost);
+      bar_pass(smem_at(&c.scores), i & 1, lost);
       tc_fence_after();
       const int col = part_of * 32;
       float2 w[16];
@@ -314,14 +316,14 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
                                 k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
           const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
           w[e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
-          u[e / 2 + k] = pack2<T>(y.x, y.y) & keep;
+          u[e / 2 + k] = pack2<T>(y.x, y.y);
         }
       }
       tmem_store16(tmem + lanes + F::kScores + col, u);  // (over this warpgroup's own scores)
       tmem_wait_store();
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.weights));
-      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
+      bar_pass(smem_at(&c.slopes), i & 1, lost);
       tc_fence_after();
       tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
@@ -332,7 +334,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         for (int k = 0; k < 2; ++k) {
           const float2 ds = mul2(w[e / 2 + k], add2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])),
                                                     k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
-          u[e / 2 + k] = pack2<T>(ds.x, ds.y) & keep;
+          u[e / 2 + k] = pack2<T>(ds.x, ds.y);
         }
       }
       tmem_store16(tmem + lanes + F::kSlopes + col, u);
@@ -340,18 +342,19 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.grads));
     }
-    if (count > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
-    if (__all_sync(~0u, ok)) {
+    if (count > 0) bar_pass(smem_at(&c.done), 0, lost);
+    if (__all_sync(~0u, *lost == 0)) {
       tc_fence_after();
-      // the first two warpgroups store dv, the others dk, half the columns each
-      const bool keys = part_of >= 2;
+      // the first half of the warpgroups stores dv, the other dk
+      constexpr int kHalf = F::kGroups / 256;
+      const bool keys = part_of >= kHalf;
       const long long all = (long long)p.N * p.L * p.Hk * p.D, at = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
       const bool parts = p.row_splits > 1;
       const float f = in ? (keys ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
       T* to = (T*)(keys ? p.gk : p.gv) + at;
       float* part = parts ? (keys ? p.part_gk : p.part_gv) + split * all + at : nullptr;
 #pragma unroll 1
-      for (int q = (part_of & 1) * (DP / 64); q < ((part_of & 1) + 1) * (DP / 64); ++q) {
+      for (int q = part_of % kHalf; q < DP / 32; q += kHalf) {
         if (q * 32 >= p.D) break;
         // (a state that is not read: its sums may be NaN where rows hold NaN)
         const uint32_t from = tmem + lanes + (keys ? F::kKeys : F::kValues) + q * 32;
@@ -398,40 +401,41 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
 // ---- rows kept: dq ------------------------------------------------------------------------------------
 template <int DP, bool MASK>
 struct TcRows {
-  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kSlots = 4;
-  static constexpr int kThreads = kGradThreads + (MASK ? 96 : 64);
-  static constexpr int kScores = 0, kSlopes = 128, kSums = 256, kColumns = 512;
+  static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128, kSlots = 4;
+  static constexpr int kGroups = kStep * 4, kThreads = kGroups + 96, kMaxTiles = kTcMaxTiles * kTcStates / kStep;
+  static constexpr int kScores = 0, kSlopes = kStep, kSums = 2 * kStep, kColumns = DP == 64 ? 256 : 512;
+  static constexpr int kResident = DP == 64 ? 2 : 1;
   struct Control {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots], rows, scores, taken, slopes, grads, done;
     uint32_t tmem;
     int lost, tiles;
-    unsigned short list[MASK ? kTcMaxTiles : 1];
-    uint4 bits[MASK ? kTcMaxTiles : 1];
+    unsigned short list[MASK ? kMaxTiles : 1];
+    StateBits<kStep> bits[MASK ? kMaxTiles : 1];
   };
-  static constexpr size_t kShared = (2 + kSlots) * (size_t)kTileBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = 2 * (size_t)kTileBytes + kSlots * (size_t)kStepBytes + sizeof(Control) + 1024;
 };
 
 template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(TcRows<DP, MASK>::kThreads, 1)
+__global__ void __launch_bounds__(TcRows<DP, MASK>::kThreads, TcRows<DP, MASK>::kResident)
 attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const float* peaks, int* status) {
   typedef TcRows<DP, MASK> F;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // Q, G, then the ring
   char* ring = base + 2 * F::kTileBytes;
-  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kTileBytes);
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kStepBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kLoader = kGradThreads / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
+  constexpr int kLoader = F::kGroups / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::kSlots; ++i) {
       bar_init(smem_at(&c.full[i]), 1);
       bar_init(smem_at(&c.empty[i]), 1);
       bar_init(smem_at(&c.clean[i]), 1);
     }
-    bar_init(smem_at(&c.rows), kGradThreads / 32);
+    bar_init(smem_at(&c.rows), F::kGroups / 32);
     bar_init(smem_at(&c.scores), 1);
-    bar_init(smem_at(&c.taken), kGradThreads / 32);
+    bar_init(smem_at(&c.taken), F::kGroups / 32);
     bar_init(smem_at(&c.slopes), 1);
-    bar_init(smem_at(&c.grads), kGradThreads / 32);
+    bar_init(smem_at(&c.grads), F::kGroups / 32);
     bar_init(smem_at(&c.done), 1);
     c.lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -441,19 +445,19 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   RowTile o;
   const bool some = row_tile(p, blockIdx.x, kTcRows, o);
   const int hk = blockIdx.y, split = blockIdx.z;
-  const int all = (p.L + kTcStates - 1) / kTcStates, per = (all + p.splits - 1) / p.splits;
-  const int begin = split * per * kTcStates;
+  const int all = (p.L + F::kStep - 1) / F::kStep, per = (all + p.splits - 1) / p.splits;
+  const int begin = split * per * F::kStep;
   int end = 0;
-  if (some) end = min(states_of(p, o.n), (split + 1) * per * kTcStates);
+  if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
   if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + kTcStates - 1) / kTcStates;
+  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
   const uint32_t tmem = c.tmem;
   volatile int* lost = &c.lost;
-  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
+  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * F::kStep; };
 
   if (warp == kLoader) {
     int i = 0;
@@ -463,10 +467,10 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
       const int j = first_of(i >> 1);
       if (elect_one()) {
-        bar_expect(bar, F::kTileBytes);
+        bar_expect(bar, F::kStepBytes);
 #pragma unroll
         for (int b = 0; b < F::kBlocks; ++b)
-          tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * 16384), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
+          tma_load_4d(smem_at(ring + slot * F::kStepBytes + b * F::kStep * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
       }
       __syncwarp();
     }
@@ -478,16 +482,12 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   } else if (warp == kIssuer) {
     if (tiles > 0) {
       const int depth = (p.D + 15) / 16;
-      const uint32_t s_shape = tc_shape<T>(128, false), d_shape = tc_shape<T>(depth * 16, true);
-      const uint64_t rows_k = desc_k_major(smem_at(base)), ring_k = desc_k_major(smem_at(ring)), ring_mn = desc_mn_major(smem_at(ring), 16384);
+      const uint32_t s_shape = tc_shape<T>(F::kStep, false), d_shape = tc_shape<T>(depth * 16, true);
+      const uint64_t rows_k = desc_k_major(smem_at(base)), ring_k = desc_k_major(smem_at(ring)), ring_mn = desc_mn_major(smem_at(ring), F::kStep * 128);
       const auto scores = [&](int left, int slot, int to, unsigned long long* bar) {
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            if (k < depth)
-              mma_ss(tmem + to, rows_k + ((left * F::kTileBytes + off) >> 4), ring_k + ((slot * F::kTileBytes + off) >> 4), s_shape, k > 0);
-          }
+          mma_rows<DP / 16>(tmem + to, rows_k + ((left * F::kTileBytes) >> 4), ring_k + ((slot * F::kStepBytes) >> 4), s_shape, depth, 16384,
+                            F::kStep * 128);
           mma_commit(smem_at(bar));
         }
         __syncwarp();
@@ -496,38 +496,35 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         if (elect_one()) mma_commit(smem_at(bar));
         __syncwarp();
       };
-      const auto wait_full = [&](int i) { return bar_wait_warp(smem_at(&c.full[i % F::kSlots]), (i / F::kSlots) & 1, lost); };
-      bool ok = bar_wait_warp(smem_at(&c.rows), 0, lost) && wait_full(0);
-      if (ok) {
-        tc_fence_after();
-        scores(0, 0, F::kScores, &c.scores);
-        if ((ok = wait_full(1))) {
-          tc_fence_after();
-          scores(1, 1, F::kSlopes, &c.slopes);
-          commit(&c.empty[1]);
-        }
-      }
-      for (int i = 0; i < tiles && ok; ++i) {
+      const auto wait_full = [&](int i) { bar_pass(smem_at(&c.full[i % F::kSlots]), (i / F::kSlots) & 1, lost); };
+      bar_pass(smem_at(&c.rows), 0, lost);
+      wait_full(0);
+      wait_full(1);
+      tc_fence_after();
+      scores(0, 0, F::kScores, &c.scores);
+      scores(1, 1, F::kSlopes, &c.slopes);
+      commit(&c.empty[1]);
+      for (int i = 0; i < tiles; ++i) {
         const int k = 2 * i, next = k + 2;
         if (i + 1 < tiles) {
-          if (!(ok = bar_wait_warp(smem_at(&c.taken), i & 1, lost) && wait_full(next))) break;
+          wait_full(next);
+          bar_pass(smem_at(&c.taken), i & 1, lost);
           tc_fence_after();
           scores(0, next % F::kSlots, F::kScores, &c.scores);
+          wait_full(next + 1);
         }
-        if (!(ok = bar_wait_warp(smem_at(&c.grads), i & 1, lost))) break;
-        if (MASK && !(ok = bar_wait_warp(smem_at(&c.clean[k % F::kSlots]), (k / F::kSlots) & 1, lost))) break;
+        if (MASK) bar_pass(smem_at(&c.clean[k % F::kSlots]), (k / F::kSlots) & 1, lost);
+        bar_pass(smem_at(&c.grads), i & 1, lost);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 1) * 32 + (e & 1) * 8, ring_mn + (((k % F::kSlots) * F::kTileBytes + e * 2048) >> 4),
+          for (int e = 0; e < F::kStep / 16; ++e)
+            mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 1) * 32 + (e & 1) * 8, ring_mn + (((k % F::kSlots) * F::kStepBytes + e * 2048) >> 4),
                    d_shape, i > 0 || e > 0);
           mma_commit(smem_at(&c.empty[k % F::kSlots]));
         }
         __syncwarp();
         if (i + 1 < tiles) {
-          if (!(ok = wait_full(next + 1))) break;
-          tc_fence_after();
           scores(1, (next + 1) % F::kSlots, F::kSlopes, &c.slopes);
           commit(&c.empty[(next + 1) % F::kSlots]);
         }
@@ -539,21 +536,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     for (int i = 0; i < tiles; ++i) {
       const int k = 2 * i, slot = k % F::kSlots;
       if (!__all_sync(~0u, bar_wait(smem_at(&c.full[slot]), (k / F::kSlots) & 1, lost))) break;
-      const uint4 b = c.bits[i];
-      if ((b.x & b.y & b.z & b.w) != ~0u) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t out = ~word_of(b, w);
-          while (out) {
-            const int r = w * 32 + __ffs(out) - 1;
-            out &= out - 1;
-            if (lane < 8 * F::kBlocks)
-              *(uint4*)(ring + slot * F::kTileBytes + (lane >> 3) * 16384 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_async_proxy();
-        __syncwarp();
-      }
+      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kStepBytes, c.bits[i], lane);
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
@@ -573,26 +556,28 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       }
     }
     if (tiles > 0) {
-      const bool g = part_of & 1;
+      // the first half of the warpgroups brings the rows of Q, the other those of G
+      constexpr int kHalf = F::kGroups / 256;
+      const bool g = part_of >= kHalf;
       const long long at = g ? w.r * p.g_r + w.t * p.g_t + w.h * p.g_h : w.r * p.q_r + w.t * p.q_t + w.h * p.q_h;
       const char* row = mine ? (const char*)(g ? p.g : p.q) + at * 2 : nullptr;
-      if (part_of & 2) put_row<DP>(base + g * F::kTileBytes, r, row, p.D, DP / 16, DP / 8);
+      if (kHalf == 1) put_row<DP>(base + g * F::kTileBytes, r, row, p.D);
+      else if (part_of & 1) put_row<DP>(base + g * F::kTileBytes, r, row, p.D, DP / 16, DP / 8);
       else put_row<DP>(base + g * F::kTileBytes, r, row, p.D, 0, DP / 16);
       fence_async_proxy();
       bar_arrive_warp(smem_at(&c.rows));
     }
     const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
-    bool ok = true;
     for (int i = 0; i < tiles; ++i) {
       uint32_t bits = ~0u;
       if (MASK) {
-        bits = word_of(c.bits[i], part_of);
-      } else if (i + 1 == tiles && (end & 127)) {
-        const int left = (end & 127) - part_of * 32;
+        bits = c.bits[i].w[part_of];
+      } else if (i + 1 == tiles && end % F::kStep) {
+        const int left = end % F::kStep - part_of * 32;
         bits = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
       }
-      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.scores), i & 1, lost)))) break;
+      bar_pass(smem_at(&c.scores), i & 1, lost);
       tc_fence_after();
       const int col = part_of * 32;
       uint32_t v[32], u[16];
@@ -607,7 +592,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
         wgt[e] = TcType<T>::code == 0 ? mul2(y, make_float2(factor, factor)) : y;
       }
-      if (!(ok = __all_sync(~0u, bar_wait(smem_at(&c.slopes), i & 1, lost)))) break;
+      bar_pass(smem_at(&c.slopes), i & 1, lost);
       tc_fence_after();
       tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
@@ -622,13 +607,13 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.grads));
     }
-    if (tiles > 0 && ok) ok = bar_wait(smem_at(&c.done), 0, lost);
-    if (__all_sync(~0u, ok)) {
+    if (tiles > 0) bar_pass(smem_at(&c.done), 0, lost);
+    if (__all_sync(~0u, *lost == 0)) {
       tc_fence_after();
       const long long rows = (long long)p.R * p.T * p.Hq;
       float* part = p.splits > 1 ? p.part_gq + (split * rows + number) * p.D : nullptr;
 #pragma unroll 1
-      for (int q = part_of; q < DP / 32; q += 4) {
+      for (int q = part_of; q < DP / 32; q += F::kGroups / 128) {
         if (q * 32 >= p.D) break;
         put_sums<T>(tmem + lanes + F::kSums + q * 32, (part ? 1.0f : p.scale) / factor, (T*)p.gq + number * p.D, part, q * 32, p.D, mine,
                     tiles > 0);

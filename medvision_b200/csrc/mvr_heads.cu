@@ -57,17 +57,18 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
   const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
   c.tile = tc ? (rows_of_image > kTcRows && !backward ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
-  c.kv_tile = tc ? kTcStates : c.tile;
+  c.kv_tile = tc ? kTcStates : c.tile;  // (the tensor cores' dq takes half tiles up to 64 columns: splits are whole tiles)
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
   // us of one tile of states against one of rows, measured; a part's sums are written and read at 4 MB/us
-  const bool wide = a->D > 64;
-  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.1) : c.tile > kTcRows ? (wide ? 1.2 : 0.9) : (wide ? 1.6 : 1.1);
-  c.splits = best_parts(expected, kv_tiles, (!tc || (c.tile == kTcRows && !backward) ? 2 : 1) * kMultiprocessors, step, rows * a->D * 8 / 4e6);
+  const bool wide = a->D > 64, pairs = !tc || (backward ? !wide : c.tile == kTcRows);  // pairs: two CTAs an SM
+  const int places = (pairs ? 2 : 1) * kMultiprocessors;
+  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.5) : pairs ? (wide ? 1.6 : 1.1) : (wide ? 1.1 : 0.8);
+  c.splits = best_parts(expected, kv_tiles, places, step, rows * a->D * 8 / 4e6);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(kv_tiles, kTcMaxTiles));
-  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), (tc ? 1 : 2) * kMultiprocessors,
-                                       !tc ? 10.0 : wide ? 2.0 : 1.3, (double)a->N * a->L * a->Hk * a->D * 16 / 4e6) : 1;
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), places, !tc ? 10.0 : wide ? 2.0 : 1.8,
+                                       (double)a->N * a->L * a->Hk * a->D * 16 / 4e6) : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
     const long long here = at;
@@ -304,7 +305,7 @@ int attention_as(const mvr_attention* a, bool backward, char* workspace, int* st
   bool tc = tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
   if (backward)
     tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
-  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps, kTcStates);
+  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps, backward && a->D <= 64 ? kGradStep<64> : kTcStates);
   const AttnCut c = cut_attention(a, backward, tc);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
   const int rc = plan_attention(a, c, workspace, status, st);

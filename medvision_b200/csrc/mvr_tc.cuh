@@ -48,28 +48,31 @@ __device__ __forceinline__ unsigned long long nanoseconds() {
 constexpr unsigned long long kWaitLimit = 2000000000ull;  // 2 s: far above any wait of a call that makes progress
 
 // Waits until the phase of the given parity has completed; false when it has not within the limit, or another thread of the CTA
-// has given up (`lost`, in shared memory).  A thread that gets false goes to the end of the kernel.
+// has given up (`lost`, in shared memory).
 __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* lost) {
   const unsigned long long begin = nanoseconds();
   for (;;) {
+    if (*lost) return false;
     for (int i = 0; i < 32; ++i)
       if (bar_try(bar, parity)) return true;
-    if (*lost) return false;
-    if (nanoseconds() - begin > kWaitLimit) {
-      *lost = 1;
-      return false;
-    }
+    if (nanoseconds() - begin > kWaitLimit) *lost = 1;
   }
 }
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* lost) {
-  if (bar_try(bar, parity) || bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, lost);
+  return bar_try(bar, parity) || bar_wait_slow(bar, parity, lost);
 }
 
 // The same by a whole warp, with one answer.
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* lost) {
   return __all_sync(~0u, bar_wait(bar, parity, lost));
 }
+// A wait whose outcome is not looked at: once given up, every later wait ends at once, and the kernel runs to its end on whatever lies
+// in its buffers, always within them, and stores nothing.  (A vote about each outcome took a tenth of the kernels' time.)
+__device__ __forceinline__ void bar_pass(uint32_t bar, uint32_t parity, volatile int* lost) {
+  if (!bar_try(bar, parity)) bar_wait_slow(bar, parity, lost);
+  __syncwarp();
+}
+
 // One lane of a converged warp.  (The products and copies below take their operands from registers that a warp shares: in a branch
 // that elect.sync guards the compiler knows that one thread runs; behind a comparison of the lane it would issue them in a loop over
 // the lanes.)
@@ -174,6 +177,8 @@ __device__ __forceinline__ uint32_t tc_shape(int n, bool b_mn_major, bool negate
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+template <int N> struct Number { static constexpr int value = N; };
+
 // d (+)= a b, 16 deep; a in shared memory (SS) or tensor memory (TS).  One thread.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
   asm volatile(
@@ -193,6 +198,24 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "}\n" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"(add ? 1u : 0u)
       : "memory");
 }
+// d (+)= a b over `depth` sixteens of K-major tiles in blocks of 64 elements a row, `block_a` and `block_b` bytes each.
+template <int MOST>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, int depth, uint32_t block_a, uint32_t block_b) {
+  const auto step = [&](int k) {
+    mma_ss(d, a + (((k >> 2) * block_a + (k & 3) * 32) >> 4), b + (((k >> 2) * block_b + (k & 3) * 32) >> 4), shape, k > 0);
+  };
+  const auto steps = [&](auto n) {  // (a number the compiler knows: a loop issues at half the rate)
+#pragma unroll
+    for (int k = 0; k < decltype(n)::value; ++k) step(k);
+  };
+  if (depth == MOST) {
+    steps(Number<MOST>());
+  } else if (depth == MOST / 2) {
+    steps(Number<MOST / 2>());
+  } else {
+    for (int k = 0; k < depth; ++k) step(k);
+  }
+}
 // Arrives at the barrier once when all products issued before by this thread are complete.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -204,19 +227,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^x of two numbers up to 64 on the arithmetic pipes, where the units for functions are the limit: x = n + f with f within a half,
 // a polynomial of degree 4 for 2^f (least-squares fit of the relative error over the interval: off by at most 2.7e-6, a hundredth
-// of a half step of float16), n added to its exponent.  -inf, and whatever lies below, gives about 2^-126; NaN is not kept.
+// of a half step of float16), times 2^n.  -inf, and whatever lies below, gives about 2^-126; NaN stays.
 __device__ __forceinline__ float2 exp2_polynomial(float2 x) {
   const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: its sum with x ends in n
-  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
   const float2 n = add2(x, magic), f = fma2(add2(n, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f), x);
   float2 p = fma2(f, make_float2(0.009570100344717503f, 0.009570100344717503f), make_float2(0.05591785907745361f, 0.05591785907745361f));
   p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
   p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
   p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(n.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(n.y) << 23)));
+  return mul2(p, make_float2(__int_as_float((__float_as_int(n.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
 }
 
 // The largest of three; NaN if one is.
