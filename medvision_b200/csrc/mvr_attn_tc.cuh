@@ -1,14 +1,16 @@
 // Attention forward on the tensor cores (float16, bfloat16; head sizes that are multiples of 8, up to 128).
 //
-// A CTA holds TILES tiles of 128 rows of queries and walks the states of their image 128 at a time.  One warp brings tiles of keys
-// and values into a ring in shared memory by TMA, one thread issues the products, and two warpgroups per row tile, half a row a
-// thread, keep the running maximum and sum:
+// A CTA holds TILES tiles of 128 rows of queries and walks the states of their image 64 or 128 at a time.  One warp brings tiles of
+// keys and values into a ring in shared memory by TMA, one thread issues the products, and a warpgroup for every 64 columns of a
+// tile, one row a thread, keeps the running maximum and sum:
 //
-//   S = Q K^T (128 x 128, tensor memory)  ->  P = 2^(S scale - m), rounded to T, over S  ->  O += P V (tensor memory)
+//   S = Q K^T (128 x 64 or 128, tensor memory)  ->  P = 2^(S scale - m), rounded to T, over S  ->  O += P V (tensor memory)
 //
 // The maximum that P is formed about is only moved when it grows by more than 2^8 (P stays far below what T holds, and the sum is
-// formed of the same P): then O, in tensor memory, is scaled first.  With two row tiles one's products run under the other's
-// exponentials.  Few rows: one tile a CTA, two CTAs an SM, and the states cut into parts (attn_join).
+// formed of the same P): then O, in tensor memory, is scaled first.  One CTA's chain of products, exponentials and products leaves
+// every unit idle for a part of it.  Up to 64 columns of a head four CTAs share an SM, each with a tile of rows and 64 states at a
+// time.  Beyond, two row tiles of one CTA alternate, which read every tile of states once for both, or, where rows are few, two CTAs
+// with a tile each.  Few rows: the states are cut into parts as well (attn_join).
 //
 // States that are left out (lengths, mask) are compacted to a list of tiles with 128 bits each before the walk; tiles without a state
 // are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its
@@ -21,7 +23,8 @@ namespace mvr {
 
 constexpr int kPolynomials = 2;  // of eight pairs of exponentials, how many are polynomials
 
-constexpr int kTcRows = 128, kTcStates = 128, kTcMaxTiles = 512;  // tiles of states that one CTA can list
+constexpr int kTcRows = 128, kTcBox = 64;   // rows of a tile; states of a TMA box
+constexpr int kTcMaxStates = 32768;         // states that one CTA can list
 
 // Which of STEP states may be read.
 template <int STEP>
@@ -49,20 +52,22 @@ struct StateBits {
 
 template <int DP, int TILES, bool MASK>
 struct TcForward {
-  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128;       // a tile of rows or states
-  static constexpr int kSlots = TILES == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 4);
-  static constexpr int kSoftmax = TILES * 256, kThreads = kSoftmax + 96;
-  static constexpr int kColumns = TILES == 2 ? 512 : 256, kScores = 0, kOut = TILES * 128;
+  static constexpr int kStep = TILES == 2 ? 128 : 64, kHalves = kStep / 64, kMaxTiles = kTcMaxStates / kStep;
+  static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128, kStepBytes = kBlocks * kStep * 128;
+  static constexpr int kSlots = 4;
+  static constexpr int kSoftmax = TILES * kHalves * 128, kThreads = kSoftmax + 96;
+  static constexpr int kScores = 0, kOut = TILES * kStep, kColumns = TILES == 2 ? 512 : DP == 64 ? 128 : 256;
+  static constexpr int kResident = TILES == 2 ? 1 : DP == 64 ? 4 : 2;
   struct Control {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots];
     unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES], halves[TILES];
     uint32_t tmem;
     int lost, tiles;
-    float top[2][TILES][2][128];  // what the two halves of a row tell each other
-    unsigned short list[MASK ? kTcMaxTiles : 1];
-    StateBits<kTcStates> bits[MASK ? kTcMaxTiles : 1];
+    float top[kHalves == 2 ? 2 : 1][TILES][2][128];  // what the two halves of a row tell each other
+    unsigned short list[MASK ? kMaxTiles : 1];
+    StateBits<kStep> bits[MASK ? kMaxTiles : 1];
   };
-  static constexpr size_t kShared = (size_t)(TILES + kSlots) * kTileBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = TILES * (size_t)kTileBytes + kSlots * (size_t)kStepBytes + sizeof(Control) + 1024;
 };
 
 struct TcMaps {
@@ -133,13 +138,13 @@ __device__ __forceinline__ void put_row(char* tile, int r, const void* src, int 
 }
 
 template <typename T, int DP, int TILES, bool MASK>
-__global__ void __launch_bounds__(TcForward<DP, TILES, MASK>::kThreads, TILES == 2 ? 1 : 2)
+__global__ void __launch_bounds__(TcForward<DP, TILES, MASK>::kThreads, TcForward<DP, TILES, MASK>::kResident)
 attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcForward<DP, TILES, MASK> F;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);
   char* ring = base + TILES * F::kTileBytes;
-  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kTileBytes);
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kStepBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoader = F::kSoftmax / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
   if (threadIdx.x == 0) {
@@ -149,9 +154,9 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       bar_init(smem_at(&c.clean[i]), 1);
     }
     for (int t = 0; t < TILES; ++t) {
-      bar_init(smem_at(&c.queries[t]), 8);
+      bar_init(smem_at(&c.queries[t]), 4 * F::kHalves);
       bar_init(smem_at(&c.scores[t]), 1);
-      bar_init(smem_at(&c.weights[t]), 8);
+      bar_init(smem_at(&c.weights[t]), 4 * F::kHalves);
       bar_init(smem_at(&c.halves[t]), 8);
       bar_init(smem_at(&c.out[t]), 1);
     }
@@ -165,20 +170,20 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   RowTile o;
   const bool some = row_tile(p, blockIdx.x, TILES * kTcRows, o);
   const int hk = blockIdx.y, split = blockIdx.z;
-  const int all = (p.L + kTcStates - 1) / kTcStates, per = (all + p.splits - 1) / p.splits;
-  const int begin = split * per * kTcStates;
+  const int all = (p.L + F::kStep - 1) / F::kStep, per = (all + p.splits - 1) / p.splits;
+  const int begin = split * per * F::kStep;
   int end = 0;
-  if (some) end = min(states_of(p, o.n), (split + 1) * per * kTcStates);
+  if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
   if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + kTcStates - 1) / kTcStates;
+  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
   const int used = !some ? 0 : TILES == 2 && o.first + kTcRows < o.rows ? 2 : 1;  // row tiles that have rows
   const uint32_t tmem = c.tmem;
   volatile int* lost = &c.lost;
-  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * kTcStates; };
+  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * F::kStep; };
 
   if (warp == kLoader) {
     int i = 0;
@@ -188,10 +193,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
       const int j = first_of(i >> 1);
       if (elect_one()) {
-        bar_expect(bar, F::kTileBytes);
+        bar_expect(bar, F::kStepBytes);
 #pragma unroll
         for (int b = 0; b < F::kBlocks; ++b)
-          tma_load_4d(smem_at(ring + slot * F::kTileBytes + b * kTcRows * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
+#pragma unroll
+          for (int r = 0; r < F::kStep; r += kTcBox)
+            tma_load_4d(smem_at(ring + slot * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j + r, o.n);
       }
       __syncwarp();
     }
@@ -204,12 +211,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   } else if (warp == kIssuer) {
     if (tiles > 0) {
       const int depth = (p.D + 15) / 16;
-      const uint32_t s_shape = tc_shape<T>(kTcStates, false, p.scale < 0.0f), o_shape = tc_shape<T>(depth * 16, true);
-      const uint64_t queries = desc_k_major(smem_at(base)), keys = desc_k_major(smem_at(ring)), values = desc_mn_major(smem_at(ring), kTcRows * 128);
+      const uint32_t s_shape = tc_shape<T>(F::kStep, false, p.scale < 0.0f), o_shape = tc_shape<T>(depth * 16, true);
+      const uint64_t queries = desc_k_major(smem_at(base)), keys = desc_k_major(smem_at(ring)), values = desc_mn_major(smem_at(ring), F::kStep * 128);
       const auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
         if (elect_one()) {
-          mma_rows<DP / 16>(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes) >> 4), keys + ((slot * F::kTileBytes) >> 4), s_shape, depth,
-                            kTcRows * 128, kTcRows * 128);
+          mma_rows<DP / 16>(tmem + F::kScores + t * F::kStep, queries + ((t * F::kTileBytes) >> 4), keys + ((slot * F::kStepBytes) >> 4), s_shape,
+                            depth, kTcRows * 128, F::kStep * 128);
           mma_commit(smem_at(&c.scores[t]));
         }
         __syncwarp();
@@ -235,12 +242,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < kTcStates / 16; ++i)  // O_t += P_t V
-              mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * 128 + (i >> 2) * 64 + (i & 3) * 8,
-                     values + ((vs * F::kTileBytes + i * 2048) >> 4), o_shape, j > 0 || i > 0);
+            for (int i = 0; i < F::kStep / 16; ++i)  // O_t += P_t V
+              mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * F::kStep + (i >> 2) * 64 + (i & 3) * 8,
+                     values + ((vs * F::kStepBytes + i * 2048) >> 4), o_shape, j > 0 || i > 0);
             if (j + 1 < tiles) {
-              mma_rows<DP / 16>(tmem + F::kScores + t * 128, queries + ((t * F::kTileBytes) >> 4), keys + ((ks * F::kTileBytes) >> 4), s_shape, depth,
-                                kTcRows * 128, kTcRows * 128);
+              mma_rows<DP / 16>(tmem + F::kScores + t * F::kStep, queries + ((t * F::kTileBytes) >> 4), keys + ((ks * F::kStepBytes) >> 4), s_shape,
+                                depth, kTcRows * 128, F::kStep * 128);
               mma_commit(smem_at(&c.scores[t]));
             }
             if (t + 1 == used) {
@@ -257,19 +264,20 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     for (int j = 0; j < tiles; ++j) {
       const int v = 2 * j + 1, slot = v % F::kSlots;
       if (!bar_wait(smem_at(&c.full[slot]), (v / F::kSlots) & 1, lost)) break;
-      clear_rows<kTcStates, F::kBlocks>(ring + slot * F::kTileBytes, c.bits[j], lane);
+      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kStepBytes, c.bits[j], lane);
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
-    const int t = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + F::kScores + t * 128 + half * 64, o_at = tmem + lanes + F::kOut + t * DP;
+    const int t = warp / (4 * F::kHalves), half = F::kHalves == 2 ? (warp >> 2) & 1 : 0, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + lanes + F::kScores + t * F::kStep + half * 64, o_at = tmem + lanes + F::kOut + t * DP;
     if (t < used) {
       Row w = {};
       const bool mine = j0 < o.rows;
       if (mine) w = row_of(p, o, j0, hk);
       if (tiles > 0) {
         const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
-        if (half) put_row<DP>(base + t * F::kTileBytes, r, q, p.D, DP / 16, DP / 8);
+        if (F::kHalves == 1) put_row<DP>(base + t * F::kTileBytes, r, q, p.D);
+        else if (half) put_row<DP>(base + t * F::kTileBytes, r, q, p.D, DP / 16, DP / 8);
         else put_row<DP>(base + t * F::kTileBytes, r, q, p.D, 0, DP / 16);
         fence_async_proxy();
         bar_arrive_warp(smem_at(&c.queries[t]));
@@ -281,8 +289,8 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         if (MASK) {
           bits[0] = c.bits[j].w[half * 2];
           bits[1] = c.bits[j].w[half * 2 + 1];
-        } else if (j + 1 == tiles && (end & 127)) {
-          const int left = (end & 127) - half * 64;
+        } else if (j + 1 == tiles && end % F::kStep) {
+          const int left = end % F::kStep - half * 64;
           bits[0] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
           bits[1] = left >= 64 ? ~0u : left > 32 ? (1u << (left - 32)) - 1 : 0;
         }
@@ -316,10 +324,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           top = max3(top, most(x), top);
         }
         // the row's maximum, of both halves
-        c.top[j & 1][t][half][r] = top;
-        bar_arrive_warp(smem_at(&c.halves[t]));
-        bar_pass(smem_at(&c.halves[t]), j & 1, lost);
-        top = max3(top, c.top[j & 1][t][half ^ 1][r], top);
+        if constexpr (F::kHalves == 2) {
+          c.top[j & 1][t][half][r] = top;
+          bar_arrive_warp(smem_at(&c.halves[t]));
+          bar_pass(smem_at(&c.halves[t]), j & 1, lost);
+          top = max3(top, c.top[j & 1][t][half ^ 1][r], top);
+        }
         if (top == INFINITY) top = NAN;  // (as inf - inf is; the sums are NaN from here on)
         // move the maximum?  (the first tile: there is no O yet)
         const bool move = !(top <= m) && (m == -INFINITY || !((top - m) * scale <= 8.0f));  // (NaN moves it)
@@ -329,7 +339,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           l *= shrink;
           if (j > 0) {
 #pragma unroll 1
-            for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
+            for (int q = half; q < DP / 32; q += F::kHalves) {
               uint32_t v[32];
               tmem_load32(v, o_at + q * 32);
               tmem_wait_load();
@@ -364,10 +374,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         bar_arrive_warp(smem_at(&c.weights[t]));
       }
       // the halves' sums together (a + b is b + a: the same in both)
-      c.top[tiles & 1][t][half][r] = l;
-      bar_arrive_warp(smem_at(&c.halves[t]));
-      bar_pass(smem_at(&c.halves[t]), tiles & 1, lost);
-      l += c.top[tiles & 1][t][half ^ 1][r];
+      if constexpr (F::kHalves == 2) {
+        c.top[tiles & 1][t][half][r] = l;
+        bar_arrive_warp(smem_at(&c.halves[t]));
+        bar_pass(smem_at(&c.halves[t]), tiles & 1, lost);
+        l += c.top[tiles & 1][t][half ^ 1][r];
+      }
       if (tiles > 0) bar_pass(smem_at(&c.out[t]), 0, lost);
       if (__all_sync(~0u, *lost == 0)) {
         tc_fence_after();
@@ -383,7 +395,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           }
         }
 #pragma unroll 1
-        for (int q = half * (DP / 64); q < (half + 1) * (DP / 64); ++q) {
+        for (int q = half; q < DP / 32; q += F::kHalves) {
           if (q * 32 >= p.D) break;
           uint32_t v[32];
           if (tiles > 0) {

@@ -144,7 +144,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
 #pragma unroll
         for (int b = 0; b < F::kBlocks; ++b) {
 #pragma unroll
-          for (int r = 0; r < 128; r += F::kStep) {  // (boxes of as many states as the other kernel takes)
+          for (int r = 0; r < 128; r += kTcBox) {
             tma_load_4d(smem_at(base + b * 16384 + r * 128), &maps.k, smem_at(&c.states), b * 64, hk, j0 + r, n);
             tma_load_4d(smem_at(base + F::kTileBytes + b * 16384 + r * 128), &maps.v, smem_at(&c.states), b * 64, hk, j0 + r, n);
           }
@@ -402,7 +402,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
 template <int DP, bool MASK>
 struct TcRows {
   static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128, kSlots = 4;
-  static constexpr int kGroups = kStep * 4, kThreads = kGroups + 96, kMaxTiles = kTcMaxTiles * kTcStates / kStep;
+  static constexpr int kGroups = kStep * 4, kThreads = kGroups + 96, kMaxTiles = kTcMaxStates / kStep;
   static constexpr int kScores = 0, kSlopes = kStep, kSums = 2 * kStep, kColumns = DP == 64 ? 256 : 512;
   static constexpr int kResident = DP == 64 ? 2 : 1;
   struct Control {
@@ -470,7 +470,9 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         bar_expect(bar, F::kStepBytes);
 #pragma unroll
         for (int b = 0; b < F::kBlocks; ++b)
-          tma_load_4d(smem_at(ring + slot * F::kStepBytes + b * F::kStep * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j, o.n);
+#pragma unroll
+          for (int r = 0; r < F::kStep; r += kTcBox)
+            tma_load_4d(smem_at(ring + slot * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j + r, o.n);
       }
       __syncwarp();
     }

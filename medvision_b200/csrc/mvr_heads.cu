@@ -56,17 +56,17 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   c.tc = tc;
   const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
   const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
-  c.tile = tc ? (rows_of_image > kTcRows && !backward ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
-  c.kv_tile = tc ? kTcStates : c.tile;  // (the tensor cores' dq takes half tiles up to 64 columns: splits are whole tiles)
+  c.tile = tc ? (rows_of_image > kTcRows && !backward && a->D > 64 ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
+  c.kv_tile = tc ? 128 : c.tile;  // (some kernels walk half of that at a time)
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
-  // us of one tile of states against one of rows, measured; a part's sums are written and read at 4 MB/us
-  const bool wide = a->D > 64, pairs = !tc || (backward ? !wide : c.tile == kTcRows);  // pairs: two CTAs an SM
-  const int places = (pairs ? 2 : 1) * kMultiprocessors;
-  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.5) : pairs ? (wide ? 1.6 : 1.1) : (wide ? 1.1 : 0.8);
+  // us of one tile of 128 states against one of rows on a full GPU, measured; a part's sums are written and read at 4 MB/us
+  const bool wide = a->D > 64;
+  const int resident = !tc ? 2 : backward ? (wide ? 1 : 2) : c.tile > kTcRows ? 1 : wide ? 2 : 4, places = resident * kMultiprocessors;
+  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.5) : c.tile > kTcRows ? 1.1 : wide ? 1.6 : 1.8;
   c.splits = best_parts(expected, kv_tiles, places, step, rows * a->D * 8 / 4e6);
-  if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(kv_tiles, kTcMaxTiles));
+  if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(a->L, kTcMaxStates));
   c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), places, !tc ? 10.0 : wide ? 2.0 : 1.8,
                                        (double)a->N * a->L * a->Hk * a->D * 16 / 4e6) : 1;
   long long at = 0;
@@ -98,7 +98,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
 
 // Whether type and head size are the tensor cores'; the operands' alignment is a matter of the call.
 bool tc_sizes(const mvr_attention* a) {
-  return a->dtype != MVR_F32 && a->D % 8 == 0 && a->D <= 128 && a->L > 0 && a->N > 0 && cdiv(a->L, kTcStates) <= 64 * kTcMaxTiles;
+  return a->dtype != MVR_F32 && a->D % 8 == 0 && a->D <= 128 && a->L > 0 && a->N > 0 && a->L <= 64LL * kTcMaxStates;
 }
 bool rows_aligned(const void* base, const int64_t (&strides)[3], const mvr_attention* a) {
   const int64_t sizes[3] = {a->R, a->T, a->Hq};
@@ -220,14 +220,16 @@ int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int
 template <typename T, int DP>
 int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   const bool mask = p.mask || p.lengths;
-  if (c.tile > kTcRows) return mask ? tc_forward_as<T, DP, 2, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false>(p, c, maps, status, st);
+  if constexpr (DP == 128) {
+    if (c.tile > kTcRows) return mask ? tc_forward_as<T, DP, 2, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false>(p, c, maps, status, st);
+  }
   return mask ? tc_forward_as<T, DP, 1, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, false>(p, c, maps, status, st);
 }
 
 template <typename T>
-bool state_maps(const mvr_attention* a, TcMaps& maps, int rows) {
+bool state_maps(const mvr_attention* a, TcMaps& maps) {
   const auto map = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-    return tc_state_map<T>(m, base, (int)a->D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], rows);
+    return tc_state_map<T>(m, base, (int)a->D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], kTcBox);
   };
   return map(&maps.k, a->k, a->k_strides) && map(&maps.v, a->v, a->v_strides);
 }
@@ -305,7 +307,7 @@ int attention_as(const mvr_attention* a, bool backward, char* workspace, int* st
   bool tc = tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
   if (backward)
     tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
-  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps, backward && a->D <= 64 ? kGradStep<64> : kTcStates);
+  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps);
   const AttnCut c = cut_attention(a, backward, tc);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
   const int rc = plan_attention(a, c, workspace, status, st);
