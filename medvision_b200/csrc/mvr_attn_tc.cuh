@@ -284,6 +284,14 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
       float m = -INFINITY, l = 0.0f;  // m: in the units of S, the same in both halves; l: of this half
+      // A warp without a row only keeps step: what lies in its rows of P reaches no other row of O.  (A single token leaves three
+      // warps of four idle.)
+      if (F::kHalves == 1 && !__any_sync(~0u, mine)) {
+        for (int j = 0; j < tiles; ++j) {
+          bar_pass(smem_at(&c.scores[t]), j & 1, lost);
+          bar_arrive_warp(smem_at(&c.weights[t]));
+        }
+      } else {
       for (int j = 0; j < tiles; ++j) {
         uint32_t bits[2] = {~0u, ~0u};
         if (MASK) {
@@ -372,6 +380,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         tmem_wait_store();
         tc_fence_before();
         bar_arrive_warp(smem_at(&c.weights[t]));
+      }
       }
       // the halves' sums together (a + b is b + a: the same in both)
       if constexpr (F::kHalves == 2) {

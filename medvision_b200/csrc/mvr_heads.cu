@@ -37,16 +37,25 @@ struct AttnCut {
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
-// Parts in which `ctas` CTAs, each walking `steps` tiles of `step` us, run for the least time on `slots` places: whole rounds of
-// CTAs, each a part's steps and 3 us for its beginning and end; joining takes 3 us and `join` us a part.
-int best_parts(long long ctas, long long steps, long long slots, double step, double join) {
+// What a kernel takes for one of its steps (a tile of rows against a tile of states), in us, measured: `full` of an SM with all the
+// CTAs that it holds (`resident`), `alone` of a CTA by itself.
+struct StepTime {
+  int resident;
+  double full, alone;
+};
+
+// Parts into which to cut the `steps` steps of `ctas` CTAs so that they end soonest: the SMs' CTAs one after another at the full rate,
+// or, where an SM has few, one CTA's own chain; 1 us a CTA for its beginning and end.  Where CTAs differ in length (`uneven`: lengths
+// or a mask), half a part is lost at the end.  Joining takes 3 us and `join` us a part.
+int best_parts(long long ctas, long long steps, const StepTime& t, double join, bool uneven) {
   int best = 1;
   double least = 0;
   for (long long s = 1; s <= std::min<long long>(64, std::max<long long>(1, steps)); ++s) {
-    const long long per = cdiv(steps, s);
+    const long long per = cdiv(steps, s), on_sm = cdiv(ctas * s, kMultiprocessors), rounds = cdiv(on_sm, t.resident);
     if (s > 1 && cdiv(steps, per) < s) continue;  // a part would have nothing
-    const double time = (double)cdiv(ctas * s, slots) * (per * step + 3) + (s > 1 ? 3 + join * s : 0);
-    if (s == 1 || time < 0.97 * least) best = (int)s, least = time;
+    const double time = std::max(on_sm * (per * t.full + 1.0 / t.resident), rounds * (per * t.alone + 1.0)) + (uneven ? per * t.alone / 2 : 0) +
+                        (s > 1 ? 3 + join * s : 0);
+    if (s == 1 || time < 0.92 * least) best = (int)s, least = time;
   }
   return best;
 }
@@ -61,14 +70,15 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
-  // us of one tile of 128 states against one of rows on a full GPU, measured; a part's sums are written and read at 4 MB/us
-  const bool wide = a->D > 64;
-  const int resident = !tc ? 2 : backward ? (wide ? 1 : 2) : c.tile > kTcRows ? 1 : wide ? 2 : 4, places = resident * kMultiprocessors;
-  const double step = !tc ? 6.0 : backward ? (wide ? 1.6 : 1.5) : c.tile > kTcRows ? 1.1 : wide ? 1.6 : 1.8;
-  c.splits = best_parts(expected, kv_tiles, places, step, rows * a->D * 8 / 4e6);
+  const bool wide = a->D > 64, uneven = a->lengths || a->mask;
+  const StepTime walk = !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
+                        : c.tile > kTcRows ? StepTime{1, 2.1, 2.1} : wide ? StepTime{2, 1.5, 1.8} : StepTime{4, 0.85, 1.5};
+  // (a part's sums are written and read at 4 MB/us)
+  c.splits = best_parts(expected, kv_tiles, walk, rows * a->D * 8 / 4e6, uneven);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(a->L, kTcMaxStates));
-  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), places, !tc ? 10.0 : wide ? 2.0 : 1.8,
-                                       (double)a->N * a->L * a->Hk * a->D * 16 / 4e6) : 1;
+  const StepTime walk_rows = !tc ? StepTime{2, 5.0, 7.0} : wide ? StepTime{1, 2.6, 2.6} : StepTime{2, 1.7, 2.3};
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), walk_rows, (double)a->N * a->L * a->Hk * a->D * 16 / 4e6, false)
+                          : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
     const long long here = at;
