@@ -16,6 +16,18 @@
 
 namespace mvr {
 
+// Division of numbers below 2^31 by a constant of the launch: a product and a shift.
+struct Divisor {
+  unsigned d, factor, shift;
+  void set(unsigned divisor) {
+    d = divisor;
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    factor = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)((__umulhi((unsigned)n, factor) + (unsigned)n) >> shift); }
+};
+
 struct AttnParams {
   const void *q, *k, *v, *g;                     // g: gradient of the output (backward)
   void *out, *gq, *gk, *gv;                      // out, gq: (R, T, Hq, D); gk, gv: (N, L, Hk, D); all contiguous
@@ -28,6 +40,7 @@ struct AttnParams {
   int lengths64;
   const unsigned char* mask;                     // (N, L) or null
   int R, T, Hq, Hk, G, N, L, D;
+  Divisor by_T, by_G;
   float scale, scale_log2;
   int splits;                                    // parts of the states (forward, dq) or of the rows (dk, dv)
   float *part_o, *part_ml;                       // splits > 1: (split, row, D) and (split, row, 2)
@@ -81,10 +94,10 @@ struct Row {
   int r, t, h;
 };
 __device__ __forceinline__ Row row_of(const AttnParams& p, const RowTile& o, int j, int hk) {
-  const int token = j / p.G;
+  const int token = p.by_G.quotient(j);
   Row w;
   w.h = hk * p.G + (j - token * p.G);
-  const int slot = token / p.T;
+  const int slot = p.by_T.quotient(token);
   w.t = token - slot * p.T;
   w.r = o.order ? o.order[slot] : o.n;
   return w;

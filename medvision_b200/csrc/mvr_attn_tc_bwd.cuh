@@ -203,22 +203,23 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
     }
   } else if (warp >= kLoader) {
-    // Rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places handed round by shuffles.  Where the rows of the
-    // next tile lie is looked up while the copies of this one are under way.
-    constexpr int kGroups = F::kStep / F::kLoaders;
-    const int chunks = p.D / 8;  // 16-byte pieces of a row
-    const char *q[kGroups], *g[kGroups];
-    float lse[kGroups], delta[kGroups];
+    // Rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places (in 16 bytes from the tensors' beginnings) handed
+    // round by shuffles.  Where the rows of the next tile lie is looked up while the copies of this one are under way.
+    constexpr int kParts = F::kStep / F::kLoaders, kPieces = DP / 8, kAtOnce = 32 / kPieces;  // rows of one round of copies
+    const int piece = lane % kPieces;
+    const bool there = piece * 8 < p.D;
+    unsigned q[kParts], g[kParts];  // ~0: no row
+    float lse[kParts], delta[kParts];
     const auto look_up = [&](int i) {
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
+      for (int k = 0; k < kParts; ++k) {
         const int at = (first + i) * F::kStep + (warp - kLoader) * 32 + k * F::kLoaders + lane;
-        q[k] = g[k] = nullptr;
+        q[k] = g[k] = ~0u;
         lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
         if (i < count && at < o.rows) {
           const Row row = row_of(p, o, at, hk);
-          q[k] = (const char*)p.q + (row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) * 2;
-          g[k] = (const char*)p.g + (row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) * 2;
+          q[k] = (unsigned)((row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) >> 3);
+          g[k] = (unsigned)((row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) >> 3);
           const long long number = row_number(p, row);
           lse[k] = p.lse[number];
           delta[k] = p.delta[number];
@@ -229,27 +230,26 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       fence_async_proxy();
       bar_arrive_warp(smem_at(&c.full[stage]));
     };
+    const char *q_piece = (const char*)p.q + (there ? piece * 16 : 0), *g_piece = (const char*)p.g + (there ? piece * 16 : 0);
+    const uint32_t to_block = smem_at(base + 2 * F::kTileBytes) + (piece >> 3) * (F::kStep * 128);
     look_up(0);
     bool pending = false;
     for (int i = 0; i < count; ++i) {
       const int stage = i % F::kStages;
       if (i >= F::kStages && !bar_wait_warp(smem_at(&c.empty[stage]), (i / F::kStages - 1) & 1, lost)) break;
-      const uint32_t qs = smem_at(base + 2 * F::kTileBytes + 2 * stage * F::kStepBytes), gs = qs + F::kStepBytes;
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
+      for (int k = 0; k < kParts; ++k) {
         const int mine = (warp - kLoader) * 32 + k * F::kLoaders;
         c.lse[stage][mine + lane] = lse[k] == -INFINITY ? -INFINITY : shift - lse[k];
         c.delta[stage][mine + lane] = -delta[k];
-#pragma unroll 4
-        for (int e = 0; e < DP / 8; ++e) {
-          const int idx = e * 32 + lane, from = idx / (DP / 8), piece = idx % (DP / 8), row = mine + from;
-          const char* qk = (const char*)__shfl_sync(~0u, (unsigned long long)q[k], from);
-          const char* gk = (const char*)__shfl_sync(~0u, (unsigned long long)g[k], from);
-          const bool there = qk != nullptr;
-          if (piece < chunks) {
-            const uint32_t to = (piece >> 3) * (F::kStep * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-            copy16(qs + to, there ? qk + piece * 16 : (const char*)p.q, there);
-            copy16(gs + to, there ? gk + piece * 16 : (const char*)p.g, there);
+#pragma unroll
+        for (int e = 0; e < 32 / kAtOnce; ++e) {
+          const int from = e * kAtOnce + lane / kPieces, row = mine + from;
+          const unsigned qk = __shfl_sync(~0u, q[k], from), gk = __shfl_sync(~0u, g[k], from);
+          const uint32_t to = to_block + 2 * stage * F::kStepBytes + row * 128 + (((piece ^ row) & 7) << 4);
+          if (there) {
+            copy16(to, q_piece + (qk == ~0u ? 0 : (long long)qk * 16), qk != ~0u);
+            copy16(to + F::kStepBytes, g_piece + (gk == ~0u ? 0 : (long long)gk * 16), gk != ~0u);
           }
         }
       }

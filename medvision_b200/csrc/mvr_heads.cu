@@ -113,9 +113,13 @@ bool tc_sizes(const mvr_attention* a) {
 bool rows_aligned(const void* base, const int64_t (&strides)[3], const mvr_attention* a) {
   const int64_t sizes[3] = {a->R, a->T, a->Hq};
   if ((uintptr_t)base % 16 != 0) return false;
-  for (int i = 0; i < 3; ++i)
-    if (sizes[i] > 1 && strides[i] % 8 != 0) return false;
-  return true;
+  int64_t last = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (sizes[i] <= 1) continue;
+    if (strides[i] % 8 != 0 || strides[i] < 0 || strides[i] > INT64_MAX / 4 / sizes[i]) return false;
+    last += (sizes[i] - 1) * strides[i];
+  }
+  return last / 8 < 0xffffffffLL;  // (rows are found by 32-bit numbers of 16 bytes)
 }
 
 int check_attention(const mvr_attention* a, bool backward, bool sizes_only) {
@@ -155,6 +159,8 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   p.lengths = a->lengths; p.lengths64 = a->lengths_64; p.mask = a->mask;
   p.R = (int)a->R; p.T = (int)a->T; p.Hq = (int)a->Hq; p.Hk = (int)a->Hk; p.G = (int)(a->Hq / a->Hk);
   p.N = (int)a->N; p.L = (int)a->L; p.D = (int)a->D;
+  p.by_T.set((unsigned)std::max(1, p.T));
+  p.by_G.set((unsigned)p.G);
   p.scale = a->scale;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.splits = c.splits; p.row_splits = c.row_splits;
