@@ -71,7 +71,8 @@ struct TcForward {
 };
 
 struct TcMaps {
-  CUtensorMap k, v;
+  CUtensorMap k, v;  // (D, heads, states, images)
+  CUtensorMap q, g;  // (D, heads, tokens, regions): set where tiles of rows are boxes of the queries and their gradient
 };
 
 // List of the tiles of STEP states in [begin, end) that have one to read, with their bits.  All threads; the result after a barrier.

@@ -87,7 +87,8 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-template <typename T, int DP>
+// BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
+template <typename T, int DP, bool BOXES>
 __global__ void __launch_bounds__(TcStates<DP>::kThreads, TcStates<DP>::kResident)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
   typedef TcStates<DP> F;
@@ -203,8 +204,10 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
     }
   } else if (warp >= kLoader) {
-    // Rows of Q and G, 16 bytes a copy: 32 rows of a warp at a time, their places (in 16 bytes from the tensors' beginnings) handed
-    // round by shuffles.  Where the rows of the next tile lie is looked up while the copies of this one are under way.
+    // Rows of Q and G.  Without an index a tile of rows is a box of the tensors: tokens, and the heads that share the key head.  Else
+    // 16 bytes a copy, 32 rows of a warp at a time, their places (in 16 bytes from the tensors' beginnings) handed round by shuffles.
+    // (TMA's gathering of four rows a copy took half as long again.)  What belongs to the rows of the next tile is looked up while the
+    // copies of this one are under way.
     constexpr int kParts = F::kStep / F::kLoaders, kPieces = DP / 8, kAtOnce = 32 / kPieces;  // rows of one round of copies
     const int piece = lane % kPieces;
     const bool there = piece * 8 < p.D;
@@ -218,8 +221,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
         if (i < count && at < o.rows) {
           const Row row = row_of(p, o, at, hk);
-          q[k] = (unsigned)((row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) >> 3);
-          g[k] = (unsigned)((row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) >> 3);
+          if (!BOXES) q[k] = (unsigned)((row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) >> 3);
+          if (!BOXES) g[k] = (unsigned)((row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) >> 3);
           const long long number = row_number(p, row);
           lse[k] = p.lse[number];
           delta[k] = p.delta[number];
@@ -242,6 +245,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         const int mine = (warp - kLoader) * 32 + k * F::kLoaders;
         c.lse[stage][mine + lane] = lse[k] == -INFINITY ? -INFINITY : shift - lse[k];
         c.delta[stage][mine + lane] = -delta[k];
+        if (BOXES) continue;
 #pragma unroll
         for (int e = 0; e < 32 / kAtOnce; ++e) {
           const int from = e * kAtOnce + lane / kPieces, row = mine + from;
@@ -252,6 +256,24 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             copy16(to + F::kStepBytes, g_piece + (gk == ~0u ? 0 : (long long)gk * 16), gk != ~0u);
           }
         }
+      }
+      if (BOXES) {
+        const uint32_t bar = smem_at(&c.full[stage]), to = smem_at(base + 2 * F::kTileBytes) + 2 * stage * F::kStepBytes;
+        __syncwarp();
+        if (warp != kLoader) {
+          bar_arrive_warp(bar);
+        } else if (elect_one()) {
+          bar_expect(bar, 2 * F::kStepBytes);
+          const int token = p.by_G.quotient((first + i) * F::kStep);
+#pragma unroll
+          for (int b = 0; b < F::kBlocks; ++b) {
+            tma_load_4d(to + b * F::kStep * 128, &maps.q, bar, b * 64, hk * p.G, token, n);
+            tma_load_4d(to + F::kStepBytes + b * F::kStep * 128, &maps.g, bar, b * 64, hk * p.G, token, n);
+          }
+        }
+        __syncwarp();
+        look_up(i + 1);
+        continue;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       look_up(i + 1);
@@ -267,6 +289,11 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (BOXES && *lost && warp == kLoader) {  // given up: the copies under way end, or the limit passes, before the CTA does
+      const unsigned long long t = nanoseconds();
+      for (int k = 0; k < F::kStages; ++k)
+        while (!bar_try(smem_at(&c.full[k]), 0) && !bar_try(smem_at(&c.full[k]), 1) && nanoseconds() - t < kWaitLimit) {}
+    }
   } else {
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float factor = 1.0f;  // of dS

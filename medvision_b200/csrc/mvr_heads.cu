@@ -243,11 +243,20 @@ int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* s
 }
 
 template <typename T>
-bool state_maps(const mvr_attention* a, TcMaps& maps) {
-  const auto map = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-    return tc_state_map<T>(m, base, (int)a->D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], kTcBox);
+bool tensor_maps(const mvr_attention* a, bool backward, TcMaps& maps, bool& boxes) {
+  const int D = (int)a->D, G = (int)(a->Hq / a->Hk);
+  const auto states = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
+    return tc_map<T>(m, base, D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], 1, kTcBox);
   };
-  return map(&maps.k, a->k, a->k_strides) && map(&maps.v, a->v, a->v_strides);
+  if (!states(&maps.k, a->k, a->k_strides) || !states(&maps.v, a->v, a->v_strides)) return false;
+  const int step = D <= 64 ? kGradStep<64> : kGradStep<128>;
+  if (backward && !a->has_index && a->R > 0 && a->T > 0 && step % G == 0) {
+    const auto rows = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
+      return tc_map<T>(m, base, D, (int)a->Hq, (int)a->T, (int)a->R, s[2], s[1], s[0], G, step / G);
+    };
+    boxes = rows(&maps.q, a->q, a->q_strides) && rows(&maps.g, a->grad_out, a->g_strides);
+  }
+  return true;
 }
 
 template <typename T>
@@ -271,7 +280,7 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
 }
 
 template <typename T, int DP>
-int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float* peaks, int* status, cudaStream_t st) {
+int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
   const auto run = [&](auto kernel, dim3 grid, int threads, size_t smem, auto... args) {
     if (grid.x == 0) return MVR_OK;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
@@ -281,8 +290,9 @@ int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float
     launch_dependent(kernel, grid, dim3(threads), smem, st, p, maps, args...);
     return launched();
   };
-  const int rc = run(attn_tc_dkv<T, DP>, dim3((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits), TcStates<DP>::kThreads,
-                     TcStates<DP>::kShared, peaks, status);
+  const dim3 states((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits);
+  const int rc = boxes ? run(attn_tc_dkv<T, DP, true>, states, TcStates<DP>::kThreads, TcStates<DP>::kShared, peaks, status)
+                       : run(attn_tc_dkv<T, DP, false>, states, TcStates<DP>::kThreads, TcStates<DP>::kShared, peaks, status);
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
   const float* bounds = peaks;
@@ -291,7 +301,7 @@ int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float
 }
 
 template <typename T>
-int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, float* peaks, int* status, cudaStream_t st) {
+int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
   if (c.tc && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
@@ -306,7 +316,7 @@ int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps
     if ((rc = launched()) != MVR_OK) return rc;
   }
   if constexpr (sizeof(T) == 2) {
-    if (c.tc) rc = p.D <= 64 ? tc_backward<T, 64>(p, c, maps, peaks, status, st) : tc_backward<T, 128>(p, c, maps, peaks, status, st);
+    if (c.tc) rc = p.D <= 64 ? tc_backward<T, 64>(p, c, maps, boxes, peaks, status, st) : tc_backward<T, 128>(p, c, maps, boxes, peaks, status, st);
   }
   if (!c.tc)
     rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
@@ -319,17 +329,18 @@ int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps
 
 template <typename T>
 int attention_as(const mvr_attention* a, bool backward, char* workspace, int* status, cudaStream_t st) {
-  TcMaps maps;
+  TcMaps maps = {};
+  bool boxes = false;
   bool tc = tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
   if (backward)
     tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
-  if constexpr (sizeof(T) == 2) tc = tc && state_maps<T>(a, maps);
+  if constexpr (sizeof(T) == 2) tc = tc && tensor_maps<T>(a, backward, maps, boxes);
   const AttnCut c = cut_attention(a, backward, tc);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
   const int rc = plan_attention(a, c, workspace, status, st);
   if (rc != MVR_OK) return rc;
   const AttnParams p = attention_params(a, c, workspace);
-  return backward ? attention_backward<T>(p, c, maps, (float*)(workspace + c.peaks), status, st) : attention_forward<T>(p, c, maps, status, st);
+  return backward ? attention_backward<T>(p, c, maps, boxes, (float*)(workspace + c.peaks), status, st) : attention_forward<T>(p, c, maps, status, st);
 }
 
 long long attention_bytes(const mvr_attention* a, bool backward) {

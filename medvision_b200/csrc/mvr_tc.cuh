@@ -282,22 +282,22 @@ inline TcEncodeTiled tc_encoder() {
   return fn;
 }
 
-// Map over (D, heads, states, images), rows of D contiguous elements of 2 bytes, boxes of 64 elements x `rows` states; false where
+// Map over (D, heads, rows, images), D contiguous elements of 2 bytes, boxes of 64 elements x `box_heads` x `box_rows`; false where
 // TMA cannot describe the tensor.
 template <typename T>
-bool tc_state_map(CUtensorMap* map, const void* base, int D, int heads, int states, int images, long long s_head, long long s_state,
-                  long long s_image, int rows) {
+bool tc_map(CUtensorMap* map, const void* base, int D, int heads, int rows, int images, long long s_head, long long s_row,
+            long long s_image, int box_heads, int box_rows) {
   TcEncodeTiled encode = tc_encoder();
   if (!encode || (uintptr_t)base % 16 != 0) return false;
   // a dimension of one element may have any stride
   if (heads == 1) s_head = D;
-  if (states == 1) s_state = D;
+  if (rows == 1) s_row = D;
   if (images == 1) s_image = D;
-  for (long long s : {s_head, s_state, s_image})
+  for (long long s : {s_head, s_row, s_image})
     if (s <= 0 || s % 8 != 0 || s * 2 >= (1LL << 40)) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)states, (cuuint64_t)images};
-  const cuuint64_t strides[3] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_state * 2, (cuuint64_t)s_image * 2};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)images};
+  const cuuint64_t strides[3] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_row * 2, (cuuint64_t)s_image * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1}, step[4] = {1, 1, 1, 1};
   return encode(map, TcType<T>::tma, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
