@@ -101,6 +101,10 @@ SHAPES = [  # R, T, H, Hk, D, N, L
     (2, 1, 8, 2, 128, 2, 1500),
     (1, 700, 1, 1, 32, 1, 5),
     (4, 1, 32, 4, 40, 4, 517),
+    (2, 150, 4, 2, 33, 2, 1000),  # large enough that odd head sizes are padded
+    (1, 260, 2, 2, 100, 1, 2100),
+    (3, 70, 6, 1, 64, 3, 140),    # six heads share a key head: 64 rows are no whole tokens
+    (2, 300, 2, 2, 128, 2, 260),
 ]
 
 
