@@ -35,7 +35,10 @@ struct DropoutParams {
   const unsigned long long* seed_at;  // or null; else the seed lies there, on the device
 };
 
-__device__ __forceinline__ uint4 philox(const PhiloxKeys& k, uint4 c) {
+// `low`, `high`: the counter's first two words; `offset` (and `high`, which is the CTA's) are the same in all threads, and with them
+// the second product of the first round and the first of the second.
+__device__ __forceinline__ uint4 philox(const PhiloxKeys& k, unsigned low, unsigned high, unsigned long long offset) {
+  uint4 c = make_uint4(low, high, (unsigned)offset, (unsigned)(offset >> 32));
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)c.x * 0xD2511F53u, b = (unsigned long long)c.z * 0xCD9E8D57u;
@@ -44,7 +47,7 @@ __device__ __forceinline__ uint4 philox(const PhiloxKeys& k, uint4 c) {
   return c;
 }
 
-constexpr int kDropThreads = 256, kDropGroups = 2;
+constexpr int kDropThreads = 256, kDropGroups = 4;
 
 // A thread takes kDropGroups groups of eight consecutive elements, a CTA's width apart, all their loads under way together.
 // VECTOR: x, residual and out are 16-byte aligned.  DEVICE: the seed lies on the device.
@@ -53,28 +56,34 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const __grid_cons
   grid_dependency();
   PhiloxKeys own;
   if (DEVICE) own.from(*p.seed_at);
-  const T* x = (const T*)p.x;
-  const T* res = (const T*)p.residual;
-  T* out = (T*)p.out;
+  // A CTA's elements: a place of 64 bits that is the CTA's, and one of 32 that is the thread's.
+  constexpr int kGroups = kDropGroups * kDropThreads;
+  const long long group0 = (long long)blockIdx.x * kGroups, e0 = group0 * 8;
+  const int left = (int)(p.n - e0 < 8 * kGroups ? p.n - e0 : 8 * kGroups);  // elements from there on
+  const T* x = (const T*)p.x + e0;
+  const T* res = (const T*)p.residual + e0;
+  T* out = (T*)p.out + e0;
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2, kPart = 8 / kParts;
   typedef Vec<T, kPart> V;
-  const long long first = ((long long)blockIdx.x * kDropGroups * kDropThreads + threadIdx.x) << 3;
   V xv[kDropGroups][kParts], rv[kDropGroups][kParts];
-  bool whole[kDropGroups];
+  const bool full = VECTOR && left == 8 * kGroups;  // (the same in all threads)
+  if (full) {
 #pragma unroll
-  for (int i = 0; i < kDropGroups; ++i) {
-    const long long e = first + i * kDropThreads * 8;
-    whole[i] = VECTOR && e + 8 <= p.n;
-    if (whole[i]) {
+    for (int i = 0; i < kDropGroups; ++i) {
+      const int e = (threadIdx.x + i * kDropThreads) * 8;
 #pragma unroll
       for (int k = 0; k < kParts; ++k) {
         xv[i][k] = *(const V*)(x + e + k * kPart);
         if (RESIDUAL) rv[i][k] = *(const V*)(res + e + k * kPart);
       }
-    } else {
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kDropGroups; ++i) {
+      const int e = (threadIdx.x + i * kDropThreads) * 8;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const bool in = e + k < p.n;
+        const bool in = e + k < left;
         xv[i][k / kPart].v[k % kPart] = in ? x[e + k] : from_float<T>(0.0f);
         if (RESIDUAL) rv[i][k / kPart].v[k % kPart] = in ? res[e + k] : from_float<T>(0.0f);
       }
@@ -82,8 +91,9 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const __grid_cons
   }
 #pragma unroll
   for (int i = 0; i < kDropGroups; ++i) {
-    const long long e = first + i * kDropThreads * 8, g = e >> 3;
-    const uint4 r = philox(DEVICE ? own : p.keys, make_uint4((unsigned)g, (unsigned)(g >> 32), (unsigned)p.offset, (unsigned)(p.offset >> 32)));
+    const int e = (threadIdx.x + i * kDropThreads) * 8;
+    // (a CTA's groups begin at a multiple of their number: no carry)
+    const uint4 r = philox(DEVICE ? own : p.keys, (unsigned)group0 + threadIdx.x + i * kDropThreads, (unsigned)(group0 >> 32), p.offset);
     const unsigned word[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -93,13 +103,13 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const __grid_cons
       if (RESIDUAL) v += to_float(rv[i][k / kPart].v[k % kPart]);
       xv[i][k / kPart].v[k % kPart] = from_float<T>(v);
     }
-    if (whole[i]) {
+    if (full) {
 #pragma unroll
       for (int k = 0; k < kParts; ++k) *(V*)(out + e + k * kPart) = xv[i][k];
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (e + k < p.n) out[e + k] = xv[i][k / kPart].v[k % kPart];
+        if (e + k < left) out[e + k] = xv[i][k / kPart].v[k % kPart];
     }
   }
 }

@@ -30,6 +30,8 @@ struct LogProbParams {
   // backward
   const float *grad_log_prob, *grad_entropy;           // or null
   void* grad;
+  long long first;                                     // classes apart: first position of the launch, and how many
+  int positions;
   long long grad_batch_stride, grad_class_stride;
 };
 
@@ -51,6 +53,13 @@ __device__ __forceinline__ int label_at(const LogProbParams& p, long long i) {
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// log2 of a sum that is at least 1: off by at most 2^-22 absolutely below 2, relatively above.
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -85,11 +94,11 @@ struct Online {
     l += b.l;
     u += b.u;
   }
-  __device__ __forceinline__ float lse() const { return m == -INFINITY ? m : m + log2f(l) * kLn2; }
-  __device__ __forceinline__ float entropy() const { return m == -INFINITY ? 0.0f : log2f(l) * kLn2 - u / l; }
+  __device__ __forceinline__ float lse() const { return m == -INFINITY ? m : m + log2_approx(l) * kLn2; }
+  __device__ __forceinline__ float entropy() const { return m == -INFINITY ? 0.0f : log2_approx(l) * kLn2 - __fdividef(u, l); }
 };
 
-__device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2f(l) * kLn2; }
+__device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2_approx(l) * kLn2; }
 __device__ __forceinline__ float log_prob_of(float x, const Online& o) { return log_prob_of(x, o.m, o.l); }
 
 // (l, u) of pairs of scores about fixed maxima.
@@ -130,7 +139,7 @@ __device__ __noinline__ void pick_apart(const T* x, long long stride, int classe
 }
 
 // ---- classes apart: positions consecutive ------------------------------------------------------------
-constexpr int kApartThreads = 128;
+constexpr int kApartThreads = 128, kApartItems = 32768;  // batch items of a grid's second dimension
 
 // Sorted list of the best TOP scores, offered by rising class: an equal score comes behind.  (NaN is left to pick_slowly.)
 template <int TOP>
@@ -158,22 +167,24 @@ struct Best<0> {
   __device__ __forceinline__ void offer(float, int) {}
 };
 
-// A thread takes two consecutive positions of one batch item (PAIR: they are loaded and stored together).  CACHE: number of classes
-// that stay in registers (0: eight at a time, the maximum of eight moves the sums once).
+// A thread takes two consecutive positions of one batch item (PAIR: they are loaded and stored together).  Batch item and class are
+// the CTA's, the position is the thread's and has 32 bits, so that an access costs no arithmetic on addresses: with 64 bits of each
+// they were two thirds of the instructions.  CACHE: number of classes that stay in registers (0: eight at a time, the maximum of eight
+// moves the sums once).
 template <typename T, bool PAIR, int TOP, int CACHE>
 __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 : 4) logprob_apart_fwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const long long per_item = (p.space + 1) / 2, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
-  if (item >= per_item * p.batch) return;
-  const long long b = item / per_item, s = (item - b * per_item) * 2;
-  const T* x = (const T*)p.x + b * p.batch_stride + s;
-  const bool second = s + 1 < p.space;
-  const long long at = b * p.space + s;
+  const unsigned s = (blockIdx.x * kApartThreads + threadIdx.x) * 2;
+  const long long b = blockIdx.y + (long long)blockIdx.z * kApartItems;
+  if (s >= (unsigned)p.positions || b >= p.batch) return;
+  const T* items = (const T*)p.x + b * p.batch_stride + p.first;
+  const bool second = s + 1 < (unsigned)p.positions;
+  const long long at = b * p.space + p.first;
   constexpr int kStep = CACHE > 0 ? CACHE : 8;
-  const int label[2] = {label_at(p, at), second ? label_at(p, at + 1) : -1};
+  const int label[2] = {label_at(p, at + s), second ? label_at(p, at + s + 1) : -1};
   float given[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) given[k] = label[k] >= 0 ? to_float(x[(long long)label[k] * p.class_stride + k]) : 0.0f;
+  for (int k = 0; k < 2; ++k) given[k] = label[k] >= 0 ? to_float(items[(long long)label[k] * p.class_stride + s + k]) : 0.0f;
   Online o[2];
   Best<TOP> best[2];
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
@@ -182,9 +193,9 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
     for (int j = 0; j < kStep; ++j) {
       w[j] = both<T>(-INFINITY);  // classes that are not there
       if (c0 + j < p.classes) {
-        const T* q = x + (long long)(c0 + j) * p.class_stride;
-        if (PAIR) w[j] = *(const Two<T>*)q;
-        else w[j] = rounded<T>(make_float2(to_float(q[0]), second ? to_float(q[1]) : 0.0f));
+        const T* q = items + (long long)(c0 + j) * p.class_stride;
+        if (PAIR) w[j] = *(const Two<T>*)(q + s);
+        else w[j] = rounded<T>(make_float2(to_float(q[s]), second ? to_float(q[s + 1]) : 0.0f));
       }
     }
     Two<T> most = w[0];
@@ -218,22 +229,22 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
     if (o[k].l != o[k].l) o[k].m = NAN;
     if (k == 1 && !second) break;
     if constexpr (TOP > 0) {
-      float* value = p.top_value + b * p.top * p.space + s + k;
-      int* best_label = p.top_label + b * p.top * p.space + s + k;
+      float* value = p.top_value + b * p.top * p.space + p.first;
+      int* best_label = p.top_label + b * p.top * p.space + p.first;
       bool all = o[k].l == o[k].l;
 #pragma unroll
       for (int t = 0; t < TOP; ++t) all = all && (t >= p.top || best[k].c[t] >= 0);
       if (all) {
 #pragma unroll
         for (int t = 0; t < TOP; ++t)
-          if (t < p.top) value[t * p.space] = log_prob_of(best[k].v[t], o[k]), best_label[t * p.space] = best[k].c[t];
+          if (t < p.top) (value + t * p.space)[s + k] = log_prob_of(best[k].v[t], o[k]), (best_label + t * p.space)[s + k] = best[k].c[t];
       } else {
-        pick_apart(x + k, p.class_stride, p.classes, p.top, p.space, value, best_label, o[k].m, o[k].l);
+        pick_apart(items + s + k, p.class_stride, p.classes, p.top, p.space, value + s + k, best_label + s + k, o[k].m, o[k].l);
       }
     }
-    p.log_prob[at + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
-    p.entropy[at + k] = o[k].entropy();
-    if (p.lse) p.lse[at + k] = o[k].lse();
+    (p.log_prob + at)[s + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
+    (p.entropy + at)[s + k] = o[k].entropy();
+    if (p.lse) (p.lse + at)[s + k] = o[k].lse();
   }
 }
 
@@ -263,13 +274,14 @@ __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
-  const long long per_item = (p.space + 1) / 2, item = (long long)blockIdx.x * kApartThreads + threadIdx.x;
-  if (item >= per_item * p.batch) return;
-  const long long b = item / per_item, s = (item - b * per_item) * 2;
-  const T* x = (const T*)p.x + b * p.batch_stride + s;
-  T* g = (T*)p.grad + b * p.grad_batch_stride + s;
-  const bool second = s + 1 < p.space;
-  const Slope q[2] = {slope_at(p, b * p.space + s), slope_at(p, b * p.space + s + (second ? 1 : 0))};
+  const unsigned s = (blockIdx.x * kApartThreads + threadIdx.x) * 2;
+  const long long b = blockIdx.y + (long long)blockIdx.z * kApartItems;
+  if (s >= (unsigned)p.positions || b >= p.batch) return;
+  const T* x = (const T*)p.x + b * p.batch_stride + p.first;
+  T* g = (T*)p.grad + b * p.grad_batch_stride + p.first;
+  const bool second = s + 1 < (unsigned)p.positions;
+  const long long at = b * p.space + p.first;
+  const Slope q[2] = {slope_at(p, at + s), slope_at(p, at + s + (second ? 1 : 0))};
   constexpr int kStep = 8;
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
     Two<T> w[kStep];
@@ -277,8 +289,8 @@ __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __gr
     for (int j = 0; j < kStep; ++j) {
       if (c0 + j < p.classes) {
         const T* xc = x + (long long)(c0 + j) * p.class_stride;
-        if (PAIR) w[j] = *(const Two<T>*)xc;
-        else w[j] = rounded<T>(make_float2(to_float(xc[0]), to_float(xc[second ? 1 : 0])));
+        if (PAIR) w[j] = *(const Two<T>*)(xc + s);
+        else w[j] = rounded<T>(make_float2(to_float(xc[s]), to_float(xc[s + (second ? 1 : 0)])));
       }
     }
 #pragma unroll
@@ -293,10 +305,10 @@ __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __gr
           if (q[k].empty()) r[k] = 0.0f;
         }
         if (PAIR) {
-          *(Two<T>*)gc = rounded<T>(make_float2(r[0], r[1]));
+          *(Two<T>*)(gc + s) = rounded<T>(make_float2(r[0], r[1]));
         } else {
-          gc[0] = from_float<T>(r[0]);
-          if (second) gc[1] = from_float<T>(r[1]);
+          gc[s] = from_float<T>(r[0]);
+          if (second) gc[s + 1] = from_float<T>(r[1]);
         }
       }
     }
@@ -579,16 +591,14 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
     p.top_label[row * p.top + t] = c;
   };
   if (o.l == o.l) {
-    if (w == 0) {
-      // of the parts' maxima the one of rank top - 1 (equal ones by part); a part without classes counts as -inf
-      peak = sh.peak[lane];
-      int rank = 0;
+    // of the parts' maxima the one of rank top - 1 (equal ones by part); a part without classes counts as -inf
+    peak = sh.peak[lane & 31];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float other = __shfl_sync(~0u, peak, i);
-        rank += other > peak || (other == peak && i < lane);
-      }
-      if (rank == p.top - 1) sh.bound = peak;
+    for (int k = 0; k < 2; ++k) {
+      const int part = w * 2 + k;
+      const float mine = sh.peak[part];
+      const int rank = __popc(__ballot_sync(~0u, peak > mine || (peak == mine && (lane & 31) < part)));
+      if (rank == p.top - 1) sh.bound = mine;
     }
     __syncthreads();
     const float bound = sh.bound;
@@ -635,7 +645,7 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kWide) logprob_row_bwd(const __grid_constant__ LogProbParams p) {
+__global__ void __launch_bounds__(kWide, 3) logprob_row_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const int lane = threadIdx.x;
   const long long row = gridDim.x - 1 - blockIdx.x;  // backwards: the rows that the forward read last are still in L2
@@ -656,20 +666,27 @@ __global__ void __launch_bounds__(kWide) logprob_row_bwd(const __grid_constant__
   if (lane < r.head) one(lane);
   if (r.behind + lane < r.n) one(r.behind + lane);
   const int vector_of_label = q.label < r.head || q.label >= r.behind ? -1 : (q.label - r.head) / V;
-#pragma unroll 4
-  for (int i = lane; i < r.vecs; i += kWide) {
-    const Vec<T, V> v = r.vectors()[i];
-    Vec<T, V> to;
-    float f[V];
+  for (int i0 = lane; i0 < r.vecs; i0 += 4 * kWide) {
+    Vec<T, V> v[4];  // all under way together
 #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = q.at(to_float(v.v[k]));
-    if (i == vector_of_label) {
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * kWide < r.vecs) v[j] = r.vectors()[i0 + j * kWide];
 #pragma unroll
-      for (int k = 0; k < V; ++k) f[k] += r.head + i * V + k == q.label ? q.a : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * kWide;
+      if (i >= r.vecs) break;
+      Vec<T, V> to;
+      float f[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = q.at(to_float(v[j].v[k]));
+      if (i == vector_of_label) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] += r.head + i * V + k == q.label ? q.a : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) to.v[k] = from_float<T>(q.empty() ? 0.0f : f[k]);
+      ((Vec<T, V>*)(g + r.head))[i] = to;
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) to.v[k] = from_float<T>(q.empty() ? 0.0f : f[k]);
-    ((Vec<T, V>*)(g + r.head))[i] = to;
   }
 }
 
@@ -716,12 +733,19 @@ int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
     }
     return 0;
   }
-  const long long ctas = ((p.space + 1) / 2 * p.batch + kApartThreads - 1) / kApartThreads;
-  if (ctas > 0x7fffffffLL) return 1;
+  if (p.batch > 60000LL * kApartItems) return 1;
   const long long strides = p.space | p.batch_stride | p.class_stride | (fwd ? 0 : p.grad_batch_stride | p.grad_class_stride);
   const uintptr_t at = (uintptr_t)p.x | (fwd ? 0 : (uintptr_t)p.grad);
-  if (strides % 2 == 0 && at % (2 * sizeof(T)) == 0) launch_logprob_apart<T, true>(p, fwd, dim3((unsigned)ctas), st);
-  else launch_logprob_apart<T, false>(p, fwd, dim3((unsigned)ctas), st);
+  const bool pair = strides % 2 == 0 && at % (2 * sizeof(T)) == 0;
+  LogProbParams q = p;
+  constexpr long long kMost = 1LL << 30;  // positions of a launch
+  for (q.first = 0; q.first < p.space; q.first += kMost) {
+    q.positions = (int)(p.space - q.first < kMost ? p.space - q.first : kMost);
+    const dim3 grid((unsigned)(((q.positions + 1) / 2 + kApartThreads - 1) / kApartThreads), (unsigned)(p.batch < kApartItems ? p.batch : kApartItems),
+                    (unsigned)((p.batch + kApartItems - 1) / kApartItems));
+    if (pair) launch_logprob_apart<T, true>(q, fwd, grid, st);
+    else launch_logprob_apart<T, false>(q, fwd, grid, st);
+  }
   return 0;
 }
 
