@@ -186,7 +186,7 @@ def test_strides_and_broadcast_states(dtype):
 @pytest.mark.gpu
 def test_gradients_agree_with_differences():
     q, k, v, g = (t.cuda() for t in make(2, 3, 2, 1, 8, 2, 11, torch.float32, seed=4))
-    f = lambda *t: float((cross_attention(*t).double() * g.double()).sum())  # noqa: E731
+    f = lambda *t: float((cross_attention(*t).detach().double() * g.double()).sum())  # noqa: E731
     grads = run(q, k, v, g)[1:]
     gen = torch.Generator().manual_seed(5)
     for i in range(3):
@@ -262,6 +262,33 @@ def test_many_regions_of_many_images_are_grouped_right():
         want[(index < 0) | (index >= N)] = 0
         # sums of 3 and 8 terms of size about 1
         assert float((out[:, 0, 0] - want).abs().max()) <= 64 * E * 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_states_beyond_32_bits(dtype):
+    """More than 2^32 elements of keys: the last states of a long cache, read alone."""
+    L, Hk, D = 2 ** 20 + 40, 64, 64
+    q, k5, v5, _ = make(1, 2, Hk, Hk, D, 1, 5, dtype, seed=11)
+    k = torch.full((1, L, Hk, D), float("nan"), dtype=dtype, device="cuda")
+    v = torch.full((1, L, Hk, D), float("nan"), dtype=dtype, device="cuda")
+    k[:, -5:], v[:, -5:] = k5.cuda(), v5.cuda()
+    assert k.numel() > 2 ** 32
+    mask = torch.zeros(1, L, dtype=torch.bool, device="cuda")
+    mask[:, -5:] = True
+    res, bound = reference(q, k5, v5, torch.zeros_like(q), [0], torch.ones(1, 5, dtype=torch.bool), D ** -0.5, dtype)
+    check(cross_attention(q.cuda(), k, v, mask=mask), res[0], bound[0], "out")
+
+
+@pytest.mark.gpu
+def test_the_status_word_is_clean_after_all_kinds_of_calls():
+    """No wait of the kernels ran out."""
+    from medvision_b200 import _C
+    _C.last_status()
+    for dtype in HALF:
+        for shape in [(2, 300, 4, 2, 64, 2, 1000), (1, 300, 2, 2, 128, 1, 700), (8, 1, 8, 2, 128, 8, 3000)]:
+            run(*make(*shape, dtype))
+    assert _C.last_status() == 0
 
 
 @pytest.mark.gpu

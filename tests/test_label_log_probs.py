@@ -79,7 +79,7 @@ def scores(shape, dtype, seed=0, scale=3.0):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("rows,K,top", [(1, 1, 1), (5, 2, 0), (3, 31, 16), (9, 81, 5), (2, 1024, 16), (7, 1025, 8), (3, 4099, 1), (2, 33000, 16), (130, 17, 3)])
+@pytest.mark.parametrize("rows,K,top", [(1, 1, 1), (5, 2, 0), (3, 31, 16), (9, 81, 5), (2, 1024, 16), (7, 1025, 8), (3, 4099, 1), (2, 33000, 16), (130, 17, 3), (1, 140001, 4)])
 def test_rows(dtype, rows, K, top):
     y = torch.randint(-1, K + 1, (rows,), generator=torch.Generator().manual_seed(1))
     compare(scores((rows, K), dtype).cuda(), y.int().cuda(), top)
@@ -226,6 +226,28 @@ def test_empty_and_graphs():
     fresh = label_log_probs(x, y, 3)
     assert all(torch.equal(a, b) for a, b in zip(r, fresh))
     assert torch.equal(g, torch.autograd.grad(fresh.log_prob.sum() + fresh.entropy.sum(), x)[0])
+
+
+@pytest.mark.gpu
+def test_many_items_and_positions_beyond_one_launch():
+    x = scores((40000, 3, 2), torch.float16, 12)
+    y = torch.randint(-1, 3, (40000, 2), generator=torch.Generator().manual_seed(13))
+    compare(x.cuda(), y.cuda(), 1)
+    n = 2 ** 30 + 6                                # a launch takes 2^30 positions; outputs pass 2^32 bytes
+    x = torch.zeros(1, 2, n, dtype=torch.float16, device="cuda")
+    x[0, 1, -8:] = torch.arange(8).half().cuda()
+    y = torch.zeros(1, n, dtype=torch.uint8, device="cuda")
+    y[0, -3:] = 1
+    leaf = x.requires_grad_()
+    got = label_log_probs(leaf, y, 1)
+    lp, h, tv, tc, _ = reference(x[..., -8:].detach().cpu().double(), y[:, -8:].cpu().long(), 1)
+    check(got.log_prob[:, -8:], lp, 64 * E, "log_prob")
+    check(got.entropy[:, -8:], h, 64 * E, "entropy")
+    assert torch.equal(got.top_label[..., -8:].cpu().long(), tc)
+    g, = torch.autograd.grad(got.log_prob, leaf, torch.ones_like(got.log_prob))
+    want = torch.nn.functional.one_hot(y[0, -8:].cpu().long(), 2).t() - torch.softmax(x[0, :, -8:].detach().cpu().double(), 0)
+    check(g[0, :, -8:], want, 2.0 ** -11, "gradient")
+    assert bool((g[0, 0, :4] == 0.5).all())
 
 
 def test_refusals():
