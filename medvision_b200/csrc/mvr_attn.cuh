@@ -40,6 +40,8 @@ struct AttnParams {
   int lengths64;
   const unsigned char* mask;                     // (N, L) or null
   int R, T, Hq, Hk, G, N, L, D;
+  int W;                                         // columns of the operands in memory: D, or with pieces D rounded up to 8
+  long long q_piece, g_piece;                    // elements from one piece of the queries (gradient) to the next
   Divisor by_T, by_G;
   float scale, scale_log2;
   int splits;                                    // parts of the states (forward, dq) or of the rows (dk, dv)

@@ -50,14 +50,18 @@ struct StateBits {
   }
 };
 
-template <int DP, int TILES, bool MASK>
+template <int DP, int TILES, bool MASK, int PIECES>
 struct TcForward {
+  static_assert(PIECES == 1 || (DP == 64 && TILES == 1), "");
   static constexpr int kStep = TILES == 2 ? 128 : 64, kHalves = kStep / 64, kMaxTiles = kTcMaxStates / kStep;
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128, kStepBytes = kBlocks * kStep * 128;
-  static constexpr int kSlots = 4;
-  static constexpr int kSoftmax = TILES * kHalves * 128, kThreads = kSoftmax + 96;
-  static constexpr int kScores = 0, kOut = TILES * kStep, kColumns = TILES == 2 ? 512 : DP == 64 ? 128 : 256;
-  static constexpr int kResident = TILES == 2 ? 1 : DP == 64 ? 4 : 2;
+  static constexpr int kRowsBytes = PIECES * kTileBytes, kSlotBytes = PIECES * kStepBytes;  // of a row tile and of a place of the ring
+  static constexpr int kSlots = PIECES == 1 ? 4 : 2;
+  static constexpr int kSoftmax = TILES * kHalves * 128, kThreads = kSoftmax + (PIECES == 1 ? 96 : 64);
+  // tensor memory: scores (P over them), third pieces of P, O
+  static constexpr int kScores = 0, kThird = TILES * kStep, kOut = kThird + (PIECES == 1 ? 0 : 32);
+  static constexpr int kColumns = TILES == 2 ? 512 : DP == 64 && PIECES == 1 ? 128 : 256;
+  static constexpr int kResident = TILES == 2 ? 1 : DP == 64 && PIECES == 1 ? 4 : 2;
   struct Control {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots];
     unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES], halves[TILES];
@@ -67,11 +71,11 @@ struct TcForward {
     unsigned short list[MASK ? kMaxTiles : 1];
     StateBits<kStep> bits[MASK ? kMaxTiles : 1];
   };
-  static constexpr size_t kShared = TILES * (size_t)kTileBytes + kSlots * (size_t)kStepBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = TILES * (size_t)kRowsBytes + kSlots * (size_t)kSlotBytes + sizeof(Control) + 1024;
 };
 
 struct TcMaps {
-  CUtensorMap k, v;  // (D, heads, states, images)
+  CUtensorMap k, v;  // (D, heads, states, images; pieces one behind another)
   CUtensorMap q, g;  // (D, heads, tokens, regions): set where tiles of rows are boxes of the queries and their gradient
 };
 
@@ -138,14 +142,36 @@ __device__ __forceinline__ void put_row(char* tile, int r, const void* src, int 
   }
 }
 
-template <typename T, int DP, int TILES, bool MASK>
-__global__ void __launch_bounds__(TcForward<DP, TILES, MASK>::kThreads, TcForward<DP, TILES, MASK>::kResident)
+// `left` floats of 32 to a row; sixteen bytes at a time where every row starts at a multiple of them.
+template <int PIECES>
+__device__ __forceinline__ void put_floats(float* to, const uint32_t (&v)[32], int left) {
+  if (PIECES == 1 || ((uintptr_t)to & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      if (i + 4 <= left) {
+        *(uint4*)(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < left) to[i + e] = __uint_as_float(v[i + e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < left) to[i] = __uint_as_float(v[i]);
+  }
+}
+
+// PIECES 3: float tensors, whose operands lie in pieces (T is bfloat16).
+template <typename T, int DP, int TILES, bool MASK, int PIECES>
+__global__ void __launch_bounds__(TcForward<DP, TILES, MASK, PIECES>::kThreads, TcForward<DP, TILES, MASK, PIECES>::kResident)
 attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
-  typedef TcForward<DP, TILES, MASK> F;
+  typedef TcForward<DP, TILES, MASK, PIECES> F;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);
-  char* ring = base + TILES * F::kTileBytes;
-  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kStepBytes);
+  char* ring = base + TILES * F::kRowsBytes;
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kSlotBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoader = F::kSoftmax / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
   if (threadIdx.x == 0) {
@@ -186,6 +212,12 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   volatile int* lost = &c.lost;
   const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * F::kStep; };
 
+  const auto clean = [&](int tile, int slot) {
+    for (int piece = 0; piece < PIECES; ++piece)
+      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, c.bits[MASK ? tile : 0], lane);
+    if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
+  };
+
   if (warp == kLoader) {
     int i = 0;
     for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
@@ -194,14 +226,22 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
       const int j = first_of(i >> 1);
       if (elect_one()) {
-        bar_expect(bar, F::kStepBytes);
+        bar_expect(bar, F::kSlotBytes);
 #pragma unroll
-        for (int b = 0; b < F::kBlocks; ++b)
+        for (int piece = 0; piece < PIECES; ++piece)
 #pragma unroll
-          for (int r = 0; r < F::kStep; r += kTcBox)
-            tma_load_4d(smem_at(ring + slot * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j + r, o.n);
+          for (int b = 0; b < F::kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < F::kStep; r += kTcBox)
+              tma_load_4d(smem_at(ring + slot * F::kSlotBytes + piece * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar,
+                          b * 64, hk, j + r, o.n + piece * p.N);
       }
       __syncwarp();
+      // (with pieces, registers are for two CTAs of six warps: this one clears rows of V as well)
+      if (MASK && PIECES == 3 && (i & 1)) {
+        bar_pass(bar, (i / F::kSlots) & 1, lost);
+        clean(i >> 1, slot);
+      }
     }
     // given up: the copies under way end before the CTA does
     if (*lost)
@@ -214,10 +254,15 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       const int depth = (p.D + 15) / 16;
       const uint32_t s_shape = tc_shape<T>(F::kStep, false, p.scale < 0.0f), o_shape = tc_shape<T>(depth * 16, true);
       const uint64_t queries = desc_k_major(smem_at(base)), keys = desc_k_major(smem_at(ring)), values = desc_mn_major(smem_at(ring), F::kStep * 128);
+      const auto multiply = [&](int t, int slot) {
+        for_pairs<PIECES>([&](int a, int b, bool first) {
+          mma_rows<DP / 16>(tmem + F::kScores + t * F::kStep, queries + ((t * F::kRowsBytes + a * F::kTileBytes) >> 4),
+                            keys + ((slot * F::kSlotBytes + b * F::kStepBytes) >> 4), s_shape, depth, kTcRows * 128, F::kStep * 128, !first);
+        });
+      };
       const auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
         if (elect_one()) {
-          mma_rows<DP / 16>(tmem + F::kScores + t * F::kStep, queries + ((t * F::kTileBytes) >> 4), keys + ((slot * F::kStepBytes) >> 4), s_shape,
-                            depth, kTcRows * 128, F::kStep * 128);
+          multiply(t, slot);
           mma_commit(smem_at(&c.scores[t]));
         }
         __syncwarp();
@@ -242,13 +287,17 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           bar_pass(smem_at(&c.weights[t]), j & 1, lost);
           tc_fence_after();
           if (elect_one()) {
+            for_pairs<PIECES>([&](int a, int b, bool first) {
 #pragma unroll
-            for (int i = 0; i < F::kStep / 16; ++i)  // O_t += P_t V
-              mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * F::kStep + (i >> 2) * 64 + (i & 3) * 8,
-                     values + ((vs * F::kStepBytes + i * 2048) >> 4), o_shape, j > 0 || i > 0);
+              for (int i = 0; i < F::kStep / 16; ++i) {  // O_t += P_t V
+                const int at = PIECES == 1 ? t * F::kStep + (i >> 2) * 64 + (i & 3) * 8
+                                           : a == 2 ? F::kThird + i * 8 : (i >> 1) * 32 + a * 16 + (i & 1) * 8;
+                mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + at, values + ((vs * F::kSlotBytes + b * F::kStepBytes + i * 2048) >> 4), o_shape,
+                       (PIECES == 1 && j > 0) || i > 0 || !first);
+              }
+            });
             if (j + 1 < tiles) {
-              mma_rows<DP / 16>(tmem + F::kScores + t * F::kStep, queries + ((t * F::kTileBytes) >> 4), keys + ((ks * F::kStepBytes) >> 4), s_shape,
-                                depth, kTcRows * 128, F::kStep * 128);
+              multiply(t, ks);
               mma_commit(smem_at(&c.scores[t]));
             }
             if (t + 1 == used) {
@@ -261,12 +310,11 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       for (int t = 0; t < TILES; ++t) commit(&c.out[t]);
     }
-  } else if (MASK && warp == kCleaner) {
+  } else if (MASK && PIECES == 1 && warp == kCleaner) {
     for (int j = 0; j < tiles; ++j) {
       const int v = 2 * j + 1, slot = v % F::kSlots;
       if (!bar_wait(smem_at(&c.full[slot]), (v / F::kSlots) & 1, lost)) break;
-      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kStepBytes, c.bits[j], lane);
-      if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
+      clean(j, slot);
     }
   } else if (warp < kLoader) {
     const int t = warp / (4 * F::kHalves), half = F::kHalves == 2 ? (warp >> 2) & 1 : 0, r = threadIdx.x & 127, j0 = o.first + t * kTcRows + r;
@@ -277,7 +325,8 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (mine) w = row_of(p, o, j0, hk);
       if (tiles > 0) {
         const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
-        if (F::kHalves == 1) put_row<DP>(base + t * F::kTileBytes, r, q, p.D);
+        if (F::kHalves == 1)
+          for (int piece = 0; piece < PIECES; ++piece) put_row<DP>(base + piece * F::kTileBytes, r, q ? q + piece * p.q_piece * 2 : q, p.W);
         else if (half) put_row<DP>(base + t * F::kTileBytes, r, q, p.D, DP / 16, DP / 8);
         else put_row<DP>(base + t * F::kTileBytes, r, q, p.D, 0, DP / 16);
         fence_async_proxy();
@@ -285,6 +334,19 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
       float m = -INFINITY, l = 0.0f;  // m: in the units of S, the same in both halves; l: of this half
+      // With pieces, O of each tile is added up in registers: the tensor cores' additions cut off what they do not hold, which over a
+      // hundred tiles comes to some 4e-6, five times the error of float sums.
+      float acc[PIECES == 1 ? 1 : 64] = {};
+      const auto collect = [&]() {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t v[32];
+          tmem_load32(v, o_at + q * 32);
+          tmem_wait_load();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[PIECES == 1 ? 0 : q * 32 + i] += __uint_as_float(v[i]);
+        }
+      };
       // A warp without a row only keeps step: what lies in its rows of P reaches no other row of O.  (A single token leaves three
       // warps of four idle.)
       if (F::kHalves == 1 && !__any_sync(~0u, mine)) {
@@ -305,6 +367,9 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         }
         bar_pass(smem_at(&c.scores[t]), j & 1, lost);
         tc_fence_after();
+        if constexpr (PIECES == 3) {
+          if (j > 0) collect();  // (of the tile before: its product ended before these scores)
+        }
         // scores of 32 states, those that are left out as -inf
         const auto settle = [&](uint32_t (&v)[32], int q) {
           if (bits[q] != ~0u) {
@@ -346,7 +411,10 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           const float shrink = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - top) * scale)) : 1.0f;
           if (move) m = top;
           l *= shrink;
-          if (j > 0) {
+          if constexpr (PIECES == 3) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] *= shrink;
+          } else if (j > 0) {
 #pragma unroll 1
             for (int q = half; q < DP / 32; q += F::kHalves) {
               uint32_t v[32];
@@ -366,15 +434,23 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           tmem_load32(x, s_at + q * 32);
           tmem_wait_load();
           settle(x, q);
-          uint32_t v[16];
+          uint32_t v[16], v1[PIECES == 1 ? 1 : 16], v2[PIECES == 1 ? 1 : 16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 a = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, minus);
-            const float2 e = kPolynomials && i % 8 < kPolynomials ? exp2_polynomial(a) : make_float2(exp2_fast(a.x), exp2_fast(a.y));
+            const float2 e = PIECES == 1 && i % 8 < kPolynomials ? exp2_polynomial(a) : make_float2(exp2_fast(a.x), exp2_fast(a.y));
             sums[i & 1] = add2(sums[i & 1], e);
-            v[i] = pack2<T>(e.x, e.y);
+            if constexpr (PIECES == 1) v[i] = pack2<T>(e.x, e.y);
+            else pieces_of(e, v[i], v1[i], v2[i]);
           }
-          tmem_store16(s_at + q * 16, v);  // (over this half's own scores)
+          // (over this half's own scores; with pieces, over the 32 that have just been read)
+          if constexpr (PIECES == 1) {
+            tmem_store16(s_at + q * 16, v);
+          } else {
+            tmem_store16(s_at + q * 32, v);
+            tmem_store16(s_at + q * 32 + 16, v1);
+            tmem_store16(tmem + lanes + F::kThird + q * 16, v2);
+          }
         }
         const float2 sum = add2(sums[0], sums[1]);
         l += sum.x + sum.y;
@@ -393,6 +469,9 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (tiles > 0) bar_pass(smem_at(&c.out[t]), 0, lost);
       if (__all_sync(~0u, *lost == 0)) {
         tc_fence_after();
+        if constexpr (PIECES == 3) {
+          if (tiles > 0) collect();
+        }
         const long long row = row_number(p, w), rows = (long long)p.R * p.T * p.Hq;
         if (m == -INFINITY) l = 0.0f;  // no state, or only scores of -inf
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -404,22 +483,13 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             p.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? 0.0f : m * scale) + log2f(l);
           }
         }
-#pragma unroll 1
-        for (int q = half; q < DP / 32; q += F::kHalves) {
-          if (q * 32 >= p.D) break;
-          uint32_t v[32];
-          if (tiles > 0) {
-            tmem_load32(v, o_at + q * 32);
-            tmem_wait_load();
-          } else {
+        const auto put = [&](int q, uint32_t (&v)[32]) {
+          if (mine && (p.splits > 1 || PIECES == 3)) {
+            float* to = (p.splits > 1 ? p.part_o + (split * rows + row) * p.D : (float*)p.out + row * p.D) + q * 32;
+            const float f = p.splits > 1 ? 1.0f : inv;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0;
-          }
-          if (mine && p.splits > 1) {
-            float* to = p.part_o + (split * rows + row) * p.D + q * 32;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (q * 32 + i < p.D) *(uint4*)(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+            put_floats<PIECES>(to, v, p.D - q * 32);
           } else if (mine) {
             T* to = (T*)p.out + row * p.D + q * 32;
 #pragma unroll
@@ -432,7 +502,27 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
               *(uint4*)(to + i) = make_uint4(u[0], u[1], u[2], u[3]);
             }
           }
-          __syncwarp();
+        };
+        if constexpr (PIECES == 3) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[q * 32 + i]);
+            if (q * 32 < p.D) put(q, v);
+          }
+        } else {
+#pragma unroll 1
+          for (int q = half; q < DP / 32; q += F::kHalves) {
+            if (q * 32 >= p.D) break;
+            uint32_t v[32] = {};
+            if (tiles > 0) {
+              tmem_load32(v, o_at + q * 32);
+              tmem_wait_load();
+            }
+            put(q, v);
+            __syncwarp();
+          }
         }
       }
     }

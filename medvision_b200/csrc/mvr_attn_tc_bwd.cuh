@@ -16,6 +16,8 @@
 // below 2^15 (max|g| from attn_delta, max|v| over the states kept, or over all that the first kernel saw).  Both are taken out of
 // the sums again, exactly.
 #pragma once
+#include <type_traits>
+
 #include "mvr_attn_tc.cuh"
 
 namespace mvr {
@@ -37,42 +39,36 @@ __device__ __forceinline__ float slope_scale(int D, float g, float v) {
 template <typename T>
 __device__ __forceinline__ float weight_shift() { return TcType<T>::code == 1 ? 0.0f : 10.0f; }
 
-// 32 sums of a row from tensor memory, times `factor`, to a row of floats or of T; columns behind D are left out.
-template <typename T>
-__device__ __forceinline__ void put_sums(uint32_t at, float factor, T* to, float* part, int col, int D, bool store, bool any) {
-  uint32_t v[32];
-  if (any) {
-    tmem_load32(v, at);
-    tmem_wait_load();
+// 32 sums of a row to a row of floats, if there is one, or of Out; `left` of them are there.
+template <typename Out, int PIECES>
+__device__ __forceinline__ void put_part(Out* to, float* part, const uint32_t (&v)[32], int left) {
+  if (part) {
+    put_floats<PIECES>(part, v, left);
+  } else if constexpr (PIECES == 3) {
+    put_floats<PIECES>((float*)to, v, left);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = 0;
-  }
-  if (store) {
-#pragma unroll
     for (int i = 0; i < 32; i += 8) {
-      if (col + i >= D) continue;
-      float f[8];
+      if (i >= left) continue;
+      uint32_t u[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[i + e]) * factor;
-      if (part) {
-        *(float4*)(part + col + i) = make_float4(f[0], f[1], f[2], f[3]);
-        *(float4*)(part + col + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
-      } else {
-        *(uint4*)(to + col + i) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-      }
+      for (int e = 0; e < 4; ++e) u[e] = pack2<Out>(__uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
+      *(uint4*)(to + i) = make_uint4(u[0], u[1], u[2], u[3]);
     }
   }
-  __syncwarp();
 }
 
 // ---- states kept: dk, dv ------------------------------------------------------------------------------
-template <int DP>
+template <int DP, int PIECES>
 struct TcStates {
+  static_assert(PIECES == 1 || DP == 64, "");
   static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128;
-  static constexpr int kGroups = kStep * 4, kLoaders = 64, kThreads = kGroups + kLoaders + 32, kStages = DP == 64 ? 3 : 2;
-  static constexpr int kScores = 0, kSlopes = kStep, kValues = 2 * kStep, kKeys = 2 * kStep + DP, kColumns = 2 * kStep + 2 * DP;
-  static constexpr int kResident = DP == 64 ? 2 : 1;
+  static constexpr int kStageBytes = PIECES * kStepBytes;  // Q (G) of a stage
+  static constexpr int kGroups = kStep * 4, kLoaders = 64, kThreads = kGroups + kLoaders + 32, kStages = DP == 64 && PIECES == 1 ? 3 : 2;
+  // tensor memory: scores (P over them), dP (dS over it), third pieces of both, dV, dK
+  static constexpr int kScores = 0, kSlopes = kStep, kThird = 2 * kStep, kValues = kThird + (PIECES == 1 ? 0 : kStep), kKeys = kValues + DP;
+  static constexpr int kColumns = PIECES == 1 ? 2 * kStep + 2 * DP : 512;
+  static constexpr int kResident = DP == 64 && PIECES == 1 ? 2 : 1;
   struct Control {
     unsigned long long states, full[kStages], empty[kStages], scores, slopes, weights, grads, done;
     uint32_t tmem;
@@ -80,7 +76,7 @@ struct TcStates {
     alignas(16) float lse[kStages][kStep];    // negative
     alignas(16) float delta[kStages][kStep];  // negative
   };
-  static constexpr size_t kShared = 2 * (size_t)kTileBytes + 2 * kStages * (size_t)kStepBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = 2 * PIECES * (size_t)kTileBytes + 2 * kStages * (size_t)kStageBytes + sizeof(Control) + 1024;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
@@ -88,13 +84,14 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 }
 
 // BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
-template <typename T, int DP, bool BOXES>
-__global__ void __launch_bounds__(TcStates<DP>::kThreads, TcStates<DP>::kResident)
+template <typename T, int DP, bool BOXES, int PIECES>
+__global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, PIECES>::kResident)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
-  typedef TcStates<DP> F;
+  typedef TcStates<DP, PIECES> F;
+  typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of the stages
-  typename F::Control& c = *(typename F::Control*)(base + 2 * F::kTileBytes + 2 * F::kStages * F::kStepBytes);
+  typename F::Control& c = *(typename F::Control*)(base + 2 * PIECES * F::kTileBytes + 2 * F::kStages * F::kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoader = F::kGroups / 32, kIssuer = kLoader + F::kLoaders / 32;
   if (threadIdx.x == 0) {
@@ -125,9 +122,9 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   const int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0;
   // what lies behind D in the rows' tiles stays 0
-  if (count > 0 && p.D < DP) {
-    for (int e = threadIdx.x; e < 2 * F::kStages * F::kStepBytes / 16; e += F::kThreads)
-      *(uint4*)(base + 2 * F::kTileBytes + e * 16) = make_uint4(0, 0, 0, 0);
+  if (count > 0 && p.W < DP) {
+    for (int e = threadIdx.x; e < 2 * F::kStages * F::kStageBytes / 16; e += F::kThreads)
+      *(uint4*)(base + 2 * PIECES * F::kTileBytes + e * 16) = make_uint4(0, 0, 0, 0);
     fence_async_proxy();
   }
   tc_fence_before();
@@ -141,34 +138,42 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   if (warp == kIssuer) {
     if (count > 0) {
       if (elect_one()) {
-        bar_expect(smem_at(&c.states), 2 * F::kTileBytes);
+        bar_expect(smem_at(&c.states), 2 * PIECES * F::kTileBytes);
 #pragma unroll
-        for (int b = 0; b < F::kBlocks; ++b) {
+        for (int piece = 0; piece < PIECES; ++piece)
 #pragma unroll
-          for (int r = 0; r < 128; r += kTcBox) {
-            tma_load_4d(smem_at(base + b * 16384 + r * 128), &maps.k, smem_at(&c.states), b * 64, hk, j0 + r, n);
-            tma_load_4d(smem_at(base + F::kTileBytes + b * 16384 + r * 128), &maps.v, smem_at(&c.states), b * 64, hk, j0 + r, n);
-          }
-        }
+          for (int b = 0; b < F::kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < 128; r += kTcBox) {
+              const uint32_t to = smem_at(base + piece * F::kTileBytes + b * 16384 + r * 128);
+              tma_load_4d(to, &maps.k, smem_at(&c.states), b * 64, hk, j0 + r, n + piece * p.N);
+              tma_load_4d(to + PIECES * F::kTileBytes, &maps.v, smem_at(&c.states), b * 64, hk, j0 + r, n + piece * p.N);
+            }
       }
       __syncwarp();
       const int depth = (p.D + 15) / 16;
       const uint32_t s_shape = tc_shape<T>(F::kStep, false), d_shape = tc_shape<T>(depth * 16, true);
-      const char* steps = base + 2 * F::kTileBytes;
+      const char* steps = base + 2 * PIECES * F::kTileBytes;
       const uint64_t tiles_k = desc_k_major(smem_at(base)), steps_k = desc_k_major(smem_at(steps)), steps_mn = desc_mn_major(smem_at(steps), F::kStep * 128);
       const auto scores = [&](int left, int right, int to, unsigned long long* bar) {  // 128 x kStep over D, both K-major
         if (elect_one()) {
-          mma_rows<DP / 16>(tmem + to, tiles_k + ((left * F::kTileBytes) >> 4), steps_k + ((right * F::kStepBytes) >> 4), s_shape, depth, 16384,
-                            F::kStep * 128);
+          for_pairs<PIECES>([&](int a, int b, bool first) {
+            mma_rows<DP / 16>(tmem + to, tiles_k + (((left * PIECES + a) * F::kTileBytes) >> 4), steps_k + ((right * F::kStageBytes + b * F::kStepBytes) >> 4),
+                              s_shape, depth, 16384, F::kStep * 128, !first);
+          });
           mma_commit(smem_at(bar));
         }
         __syncwarp();
       };
       const auto sums = [&](int from, int right, int to, bool add) {  // over the rows
         if (elect_one()) {
+          for_pairs<PIECES>([&](int a, int b, bool first) {
 #pragma unroll
-          for (int i = 0; i < F::kStep / 16; ++i)
-            mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + (i & 1) * 8, steps_mn + ((right * F::kStepBytes + i * 2048) >> 4), d_shape, add || i > 0);
+            for (int i = 0; i < F::kStep / 16; ++i) {
+              const int at = a == 2 ? F::kThird + (from == F::kSlopes ? F::kStep / 2 : 0) + i * 8 : from + (i >> 1) * 32 + a * 16 + (i & 1) * 8;
+              mma_ts(tmem + to, tmem + at, steps_mn + ((right * F::kStageBytes + b * F::kStepBytes + i * 2048) >> 4), d_shape, (PIECES == 1 && add) || i > 0 || !first);
+            }
+          });
         }
         __syncwarp();
       };
@@ -210,7 +215,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     // copies of this one are under way.
     constexpr int kParts = F::kStep / F::kLoaders, kPieces = DP / 8, kAtOnce = 32 / kPieces;  // rows of one round of copies
     const int piece = lane % kPieces;
-    const bool there = piece * 8 < p.D;
+    const bool there = piece * 8 < p.W;
     unsigned q[kParts], g[kParts];  // ~0: no row
     float lse[kParts], delta[kParts];
     const auto look_up = [&](int i) {
@@ -234,7 +239,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       bar_arrive_warp(smem_at(&c.full[stage]));
     };
     const char *q_piece = (const char*)p.q + (there ? piece * 16 : 0), *g_piece = (const char*)p.g + (there ? piece * 16 : 0);
-    const uint32_t to_block = smem_at(base + 2 * F::kTileBytes) + (piece >> 3) * (F::kStep * 128);
+    const uint32_t to_block = smem_at(base + 2 * PIECES * F::kTileBytes) + (piece >> 3) * (F::kStep * 128);
     look_up(0);
     bool pending = false;
     for (int i = 0; i < count; ++i) {
@@ -250,26 +255,32 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         for (int e = 0; e < 32 / kAtOnce; ++e) {
           const int from = e * kAtOnce + lane / kPieces, row = mine + from;
           const unsigned qk = __shfl_sync(~0u, q[k], from), gk = __shfl_sync(~0u, g[k], from);
-          const uint32_t to = to_block + 2 * stage * F::kStepBytes + row * 128 + (((piece ^ row) & 7) << 4);
+          const uint32_t to = to_block + 2 * stage * F::kStageBytes + row * 128 + (((piece ^ row) & 7) << 4);
           if (there) {
-            copy16(to, q_piece + (qk == ~0u ? 0 : (long long)qk * 16), qk != ~0u);
-            copy16(to + F::kStepBytes, g_piece + (gk == ~0u ? 0 : (long long)gk * 16), gk != ~0u);
+#pragma unroll
+            for (int part = 0; part < PIECES; ++part) {
+              copy16(to + part * F::kStepBytes, q_piece + (qk == ~0u ? 0 : ((long long)qk * 8 + part * p.q_piece) * 2), qk != ~0u);
+              copy16(to + F::kStageBytes + part * F::kStepBytes, g_piece + (gk == ~0u ? 0 : ((long long)gk * 8 + part * p.g_piece) * 2), gk != ~0u);
+            }
           }
         }
       }
       if (BOXES) {
-        const uint32_t bar = smem_at(&c.full[stage]), to = smem_at(base + 2 * F::kTileBytes) + 2 * stage * F::kStepBytes;
+        const uint32_t bar = smem_at(&c.full[stage]), to = smem_at(base + 2 * PIECES * F::kTileBytes) + 2 * stage * F::kStageBytes;
         __syncwarp();
         if (warp != kLoader) {
           bar_arrive_warp(bar);
         } else if (elect_one()) {
-          bar_expect(bar, 2 * F::kStepBytes);
+          bar_expect(bar, 2 * F::kStageBytes);
           const int token = p.by_G.quotient((first + i) * F::kStep);
 #pragma unroll
-          for (int b = 0; b < F::kBlocks; ++b) {
-            tma_load_4d(to + b * F::kStep * 128, &maps.q, bar, b * 64, hk * p.G, token, n);
-            tma_load_4d(to + F::kStepBytes + b * F::kStep * 128, &maps.g, bar, b * 64, hk * p.G, token, n);
-          }
+          for (int part = 0; part < PIECES; ++part)
+#pragma unroll
+            for (int b = 0; b < F::kBlocks; ++b) {
+              const uint32_t at = to + part * F::kStepBytes + b * F::kStep * 128;
+              tma_load_4d(at, &maps.q, bar, b * 64, hk * p.G, token, n + part * p.R);
+              tma_load_4d(at + F::kStageBytes, &maps.g, bar, b * 64, hk * p.G, token, n + part * p.R);
+            }
         }
         __syncwarp();
         look_up(i + 1);
@@ -323,15 +334,30 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       factor = slope_scale<T>(p.D, peaks[0], peak);
     }
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
+    // With pieces, each tile's sums are added up in registers (dv in the first warpgroup, dk in the second): see the forward.
+    float acc[PIECES == 1 ? 1 : 64] = {};
+    const auto collect = [&](int from) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_load32(v, tmem + lanes + from + q * 32);
+        tmem_wait_load();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) acc[PIECES == 1 ? 0 : q * 32 + e] += __uint_as_float(v[e]);
+      }
+    };
     // (A state that is not read is a row of its own in both products: whatever comes of it reaches no other, and is not stored.)
     for (int i = 0; i < count; ++i) {
       const int stage = i % F::kStages;
       bar_pass(smem_at(&c.full[stage]), (i / F::kStages) & 1, lost);
       bar_pass(smem_at(&c.scores), i & 1, lost);
       tc_fence_after();
+      if constexpr (PIECES == 3) {
+        if (i > 0 && part_of == 0) collect(F::kValues);  // (of the tile before: its product ended before these scores)
+      }
       const int col = part_of * 32;
       float2 w[16];
-      uint32_t v[32], u[16];
+      uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
 #pragma unroll
@@ -343,15 +369,23 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
                                 k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
           const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
           w[e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
-          u[e / 2 + k] = pack2<T>(y.x, y.y);
+          if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(y.x, y.y);
+          else pieces_of(y, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
         }
       }
       tmem_store16(tmem + lanes + F::kScores + col, u);  // (over this warpgroup's own scores)
+      if constexpr (PIECES == 3) {
+        tmem_store16(tmem + lanes + F::kScores + col + 16, u1);
+        tmem_store16(tmem + lanes + F::kThird + col / 2, u2);
+      }
       tmem_wait_store();
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.weights));
       bar_pass(smem_at(&c.slopes), i & 1, lost);
       tc_fence_after();
+      if constexpr (PIECES == 3) {
+        if (i > 0 && part_of == 1) collect(F::kKeys);
+      }
       tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
 #pragma unroll
@@ -361,10 +395,15 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         for (int k = 0; k < 2; ++k) {
           const float2 ds = mul2(w[e / 2 + k], add2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])),
                                                     k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
-          u[e / 2 + k] = pack2<T>(ds.x, ds.y);
+          if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(ds.x, ds.y);
+          else pieces_of(ds, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
         }
       }
       tmem_store16(tmem + lanes + F::kSlopes + col, u);
+      if constexpr (PIECES == 3) {
+        tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
+        tmem_store16(tmem + lanes + F::kThird + F::kStep / 2 + col / 2, u2);
+      }
       tmem_wait_store();
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.grads));
@@ -378,34 +417,37 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       const long long all = (long long)p.N * p.L * p.Hk * p.D, at = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
       const bool parts = p.row_splits > 1;
       const float f = in ? (keys ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
-      T* to = (T*)(keys ? p.gk : p.gv) + at;
+      Out* to = (Out*)(keys ? p.gk : p.gv) + at;
       float* part = parts ? (keys ? p.part_gk : p.part_gv) + split * all + at : nullptr;
-#pragma unroll 1
-      for (int q = part_of % kHalf; q < DP / 32; q += kHalf) {
-        if (q * 32 >= p.D) break;
+      const auto put = [&](int q, uint32_t (&v)[32]) {
         // (a state that is not read: its sums may be NaN where rows hold NaN)
-        const uint32_t from = tmem + lanes + (keys ? F::kKeys : F::kValues) + q * 32;
-        uint32_t v[32];
-        if (count > 0) {
-          tmem_load32(v, from);
-          tmem_wait_load();
-        }
         if (j < p.L) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            if (q * 32 + i >= p.D) continue;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = in && count > 0 ? __uint_as_float(v[i + e]) * f : 0.0f;
-            if (part) {
-              *(float4*)(part + q * 32 + i) = make_float4(x[0], x[1], x[2], x[3]);
-              *(float4*)(part + q * 32 + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
-              *(uint4*)(to + q * 32 + i) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-            }
-          }
+          for (int i = 0; i < 32; ++i) v[i] = in && count > 0 ? __float_as_uint(__uint_as_float(v[i]) * f) : 0;
+          put_part<Out, PIECES>(to + q * 32, part ? part + q * 32 : nullptr, v, p.D - q * 32);
         }
-        __syncwarp();
+      };
+      if constexpr (PIECES == 3) {
+        if (count > 0) collect(keys ? F::kKeys : F::kValues);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[q * 32 + i]);
+          if (q * 32 < p.D) put(q, v);
+        }
+      } else {
+#pragma unroll 1
+        for (int q = part_of % kHalf; q < DP / 32; q += kHalf) {
+          if (q * 32 >= p.D) break;
+          uint32_t v[32] = {};
+          if (count > 0) {
+            tmem_load32(v, tmem + lanes + (keys ? F::kKeys : F::kValues) + q * 32);
+            tmem_wait_load();
+          }
+          put(q, v);
+          __syncwarp();
+        }
       }
     }
   }
@@ -426,12 +468,14 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
 }
 
 // ---- rows kept: dq ------------------------------------------------------------------------------------
-template <int DP, bool MASK>
+template <int DP, bool MASK, int PIECES>
 struct TcRows {
   static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128, kSlots = 4;
+  static constexpr int kRowsBytes = PIECES * kTileBytes, kSlotBytes = PIECES * kStepBytes;
   static constexpr int kGroups = kStep * 4, kThreads = kGroups + 96, kMaxTiles = kTcMaxStates / kStep;
-  static constexpr int kScores = 0, kSlopes = kStep, kSums = 2 * kStep, kColumns = DP == 64 ? 256 : 512;
-  static constexpr int kResident = DP == 64 ? 2 : 1;
+  // tensor memory: scores, dP (dS over it), third pieces of dS, dQ
+  static constexpr int kScores = 0, kSlopes = kStep, kThird = 2 * kStep, kSums = kThird + (PIECES == 1 ? 0 : kStep / 2), kColumns = DP == 64 ? 256 : 512;
+  static constexpr int kResident = DP == 64 && PIECES == 1 ? 2 : 1;
   struct Control {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots], rows, scores, taken, slopes, grads, done;
     uint32_t tmem;
@@ -439,17 +483,18 @@ struct TcRows {
     unsigned short list[MASK ? kMaxTiles : 1];
     StateBits<kStep> bits[MASK ? kMaxTiles : 1];
   };
-  static constexpr size_t kShared = 2 * (size_t)kTileBytes + kSlots * (size_t)kStepBytes + sizeof(Control) + 1024;
+  static constexpr size_t kShared = 2 * (size_t)kRowsBytes + kSlots * (size_t)kSlotBytes + sizeof(Control) + 1024;
 };
 
-template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(TcRows<DP, MASK>::kThreads, TcRows<DP, MASK>::kResident)
+template <typename T, int DP, bool MASK, int PIECES>
+__global__ void __launch_bounds__(TcRows<DP, MASK, PIECES>::kThreads, TcRows<DP, MASK, PIECES>::kResident)
 attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const float* peaks, int* status) {
-  typedef TcRows<DP, MASK> F;
+  typedef TcRows<DP, MASK, PIECES> F;
+  typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // Q, G, then the ring
-  char* ring = base + 2 * F::kTileBytes;
-  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kStepBytes);
+  char* ring = base + 2 * F::kRowsBytes;
+  typename F::Control& c = *(typename F::Control*)(ring + F::kSlots * F::kSlotBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoader = F::kGroups / 32, kIssuer = kLoader + 1, kCleaner = kLoader + 2;
   if (threadIdx.x == 0) {
@@ -494,12 +539,15 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       if (i >= F::kSlots && !bar_wait_warp(smem_at(&c.empty[slot]), (i / F::kSlots - 1) & 1, lost)) break;
       const int j = first_of(i >> 1);
       if (elect_one()) {
-        bar_expect(bar, F::kStepBytes);
+        bar_expect(bar, F::kSlotBytes);
 #pragma unroll
-        for (int b = 0; b < F::kBlocks; ++b)
+        for (int piece = 0; piece < PIECES; ++piece)
 #pragma unroll
-          for (int r = 0; r < F::kStep; r += kTcBox)
-            tma_load_4d(smem_at(ring + slot * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar, b * 64, hk, j + r, o.n);
+          for (int b = 0; b < F::kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < F::kStep; r += kTcBox)
+              tma_load_4d(smem_at(ring + slot * F::kSlotBytes + piece * F::kStepBytes + (b * F::kStep + r) * 128), i & 1 ? &maps.v : &maps.k, bar,
+                          b * 64, hk, j + r, o.n + piece * p.N);
       }
       __syncwarp();
     }
@@ -515,8 +563,10 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       const uint64_t rows_k = desc_k_major(smem_at(base)), ring_k = desc_k_major(smem_at(ring)), ring_mn = desc_mn_major(smem_at(ring), F::kStep * 128);
       const auto scores = [&](int left, int slot, int to, unsigned long long* bar) {
         if (elect_one()) {
-          mma_rows<DP / 16>(tmem + to, rows_k + ((left * F::kTileBytes) >> 4), ring_k + ((slot * F::kStepBytes) >> 4), s_shape, depth, 16384,
-                            F::kStep * 128);
+          for_pairs<PIECES>([&](int a, int b, bool first) {
+            mma_rows<DP / 16>(tmem + to, rows_k + ((left * F::kRowsBytes + a * F::kTileBytes) >> 4), ring_k + ((slot * F::kSlotBytes + b * F::kStepBytes) >> 4),
+                              s_shape, depth, 16384, F::kStep * 128, !first);
+          });
           mma_commit(smem_at(bar));
         }
         __syncwarp();
@@ -546,10 +596,14 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         bar_pass(smem_at(&c.grads), i & 1, lost);
         tc_fence_after();
         if (elect_one()) {
+          for_pairs<PIECES>([&](int a, int b, bool first) {
 #pragma unroll
-          for (int e = 0; e < F::kStep / 16; ++e)
-            mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 1) * 32 + (e & 1) * 8, ring_mn + (((k % F::kSlots) * F::kStepBytes + e * 2048) >> 4),
-                   d_shape, i > 0 || e > 0);
+            for (int e = 0; e < F::kStep / 16; ++e) {
+              const int at = a == 2 ? F::kThird + e * 8 : F::kSlopes + (e >> 1) * 32 + a * 16 + (e & 1) * 8;
+              mma_ts(tmem + F::kSums, tmem + at, ring_mn + (((k % F::kSlots) * F::kSlotBytes + b * F::kStepBytes + e * 2048) >> 4), d_shape,
+                     (PIECES == 1 && i > 0) || e > 0 || !first);
+            }
+          });
           mma_commit(smem_at(&c.empty[k % F::kSlots]));
         }
         __syncwarp();
@@ -565,7 +619,8 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     for (int i = 0; i < tiles; ++i) {
       const int k = 2 * i, slot = k % F::kSlots;
       if (!__all_sync(~0u, bar_wait(smem_at(&c.full[slot]), (k / F::kSlots) & 1, lost))) break;
-      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kStepBytes, c.bits[i], lane);
+      for (int piece = 0; piece < PIECES; ++piece)
+        clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, c.bits[i], lane);
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
@@ -590,7 +645,9 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       const bool g = part_of >= kHalf;
       const long long at = g ? w.r * p.g_r + w.t * p.g_t + w.h * p.g_h : w.r * p.q_r + w.t * p.q_t + w.h * p.q_h;
       const char* row = mine ? (const char*)(g ? p.g : p.q) + at * 2 : nullptr;
-      if (kHalf == 1) put_row<DP>(base + g * F::kTileBytes, r, row, p.D);
+      if (kHalf == 1)
+        for (int piece = 0; piece < PIECES; ++piece)
+          put_row<DP>(base + g * F::kRowsBytes + piece * F::kTileBytes, r, row ? row + piece * (g ? p.g_piece : p.q_piece) * 2 : row, p.W);
       else if (part_of & 1) put_row<DP>(base + g * F::kTileBytes, r, row, p.D, DP / 16, DP / 8);
       else put_row<DP>(base + g * F::kTileBytes, r, row, p.D, 0, DP / 16);
       fence_async_proxy();
@@ -598,6 +655,15 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     }
     const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
+    // With pieces, each tile's sums are added up in registers (half the columns a warpgroup): see the forward.
+    float acc[PIECES == 1 ? 1 : 32] = {};
+    const auto collect = [&]() {
+      uint32_t v[32];
+      tmem_load32(v, tmem + lanes + F::kSums + part_of * 32);
+      tmem_wait_load();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) acc[PIECES == 1 ? 0 : e] += __uint_as_float(v[e]);
+    };
     for (int i = 0; i < tiles; ++i) {
       uint32_t bits = ~0u;
       if (MASK) {
@@ -609,7 +675,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       bar_pass(smem_at(&c.scores), i & 1, lost);
       tc_fence_after();
       const int col = part_of * 32;
-      uint32_t v[32], u[16];
+      uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
       tc_fence_before();
@@ -623,15 +689,23 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       }
       bar_pass(smem_at(&c.slopes), i & 1, lost);
       tc_fence_after();
+      if constexpr (PIECES == 3) {
+        if (i > 0) collect();  // (of the tile before: its product ended before this dP)
+      }
       tmem_load32(v, tmem + lanes + F::kSlopes + col);
       tmem_wait_load();
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float2 ds = mul2(wgt[e], add2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), less));
         if (bits != ~0u) ds = make_float2((bits >> (2 * e)) & 1 ? ds.x : 0.0f, (bits >> (2 * e + 1)) & 1 ? ds.y : 0.0f);
-        u[e] = pack2<T>(ds.x, ds.y);
+        if constexpr (PIECES == 1) u[e] = pack2<T>(ds.x, ds.y);
+        else pieces_of(ds, u[e], u1[e], u2[e]);
       }
       tmem_store16(tmem + lanes + F::kSlopes + col, u);
+      if constexpr (PIECES == 3) {
+        tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
+        tmem_store16(tmem + lanes + F::kThird + col / 2, u2);
+      }
       tmem_wait_store();
       tc_fence_before();
       bar_arrive_warp(smem_at(&c.grads));
@@ -641,11 +715,30 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       tc_fence_after();
       const long long rows = (long long)p.R * p.T * p.Hq;
       float* part = p.splits > 1 ? p.part_gq + (split * rows + number) * p.D : nullptr;
+      const float f = (part ? 1.0f : p.scale) / factor;
+      const auto put = [&](int q, uint32_t (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+        if (mine) put_part<Out, PIECES>((Out*)p.gq + number * p.D + q * 32, part ? part + q * 32 : nullptr, v, p.D - q * 32);
+      };
+      if constexpr (PIECES == 3) {
+        if (tiles > 0) collect();
+        uint32_t v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[i]);
+        if (part_of * 32 < p.D) put(part_of, v);
+      } else {
 #pragma unroll 1
-      for (int q = part_of; q < DP / 32; q += F::kGroups / 128) {
-        if (q * 32 >= p.D) break;
-        put_sums<T>(tmem + lanes + F::kSums + q * 32, (part ? 1.0f : p.scale) / factor, (T*)p.gq + number * p.D, part, q * 32, p.D, mine,
-                    tiles > 0);
+        for (int q = part_of; q < DP / 32; q += F::kGroups / 128) {
+          if (q * 32 >= p.D) break;
+          uint32_t v[32] = {};
+          if (tiles > 0) {
+            tmem_load32(v, tmem + lanes + F::kSums + q * 32);
+            tmem_wait_load();
+          }
+          put(q, v);
+          __syncwarp();
+        }
       }
     }
   }

@@ -28,11 +28,12 @@ constexpr size_t kPlanShared = 200 * 1024;
 
 // How a call is cut into CTAs, and what lies where in its workspace.
 struct AttnCut {
-  bool tc;                      // tensor cores (mvr_attn_tc.cuh)
+  bool tc;                      // tensor cores (mvr_attn_tc.cuh); float operands in pieces
+  int W;                        // columns of the operands in memory
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
-  long long order, starts, tiles, delta, peaks, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+  long long order, starts, tiles, delta, peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
@@ -63,6 +64,8 @@ int best_parts(long long ctas, long long steps, const StepTime& t, double join, 
 AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   AttnCut c = {};
   c.tc = tc;
+  const bool pieces = tc && a->dtype == MVR_F32;
+  c.W = (int)(pieces ? cdiv(a->D, 8) * 8 : a->D);
   const long long per = a->T * (a->Hq / a->Hk), rows = a->R * a->T * a->Hq;
   const long long rows_of_image = a->has_index ? cdiv(a->R * per, std::max<int64_t>(1, a->N)) : per;
   c.tile = tc ? (rows_of_image > kTcRows && !backward && a->D > 64 ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
@@ -71,12 +74,12 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
   const bool wide = a->D > 64, uneven = a->lengths || a->mask;
-  const StepTime walk = !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
+  const StepTime walk = pieces ? (backward ? StepTime{1, 4.0, 4.0} : StepTime{2, 2.5, 4.0}) : !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
                         : c.tile > kTcRows ? StepTime{1, 2.1, 2.1} : wide ? StepTime{2, 1.5, 1.8} : StepTime{4, 0.85, 1.5};
   // (a part's sums are written and read at 4 MB/us)
   c.splits = best_parts(expected, kv_tiles, walk, rows * a->D * 8 / 4e6, uneven);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(a->L, kTcMaxStates));
-  const StepTime walk_rows = !tc ? StepTime{2, 5.0, 7.0} : wide ? StepTime{1, 2.6, 2.6} : StepTime{2, 1.7, 2.3};
+  const StepTime walk_rows = pieces ? StepTime{1, 5.0, 5.0} : !tc ? StepTime{2, 5.0, 7.0} : wide ? StepTime{1, 2.6, 2.6} : StepTime{2, 1.7, 2.3};
   c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), walk_rows, (double)a->N * a->L * a->Hk * a->D * 16 / 4e6, false)
                           : 1;
   long long at = 0;
@@ -89,6 +92,12 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
     c.order = take(a->R * 4);
     c.starts = take((a->N + 2) * 4);
     c.tiles = take((a->N + 2) * 4);
+  }
+  if (pieces) {
+    c.q = take(rows * c.W * 6);
+    c.k = take(a->N * a->L * a->Hk * c.W * 6);
+    c.v = take(a->N * a->L * a->Hk * c.W * 6);
+    if (backward) c.g = take(rows * c.W * 6);
   }
   if (backward) {
     c.delta = take(rows * 4);
@@ -106,9 +115,14 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   return c;
 }
 
-// Whether type and head size are the tensor cores'; the operands' alignment is a matter of the call.
+// Scores (rows times states) from which float operands in pieces are worth the launches that make them.
+constexpr double kPieceScores = 1 << 18;
+
+// Whether type and sizes are the tensor cores'; the operands' alignment is a matter of the call.
 bool tc_sizes(const mvr_attention* a) {
-  return a->dtype != MVR_F32 && a->D % 8 == 0 && a->D <= 128 && a->L > 0 && a->N > 0 && a->L <= 64LL * kTcMaxStates;
+  const double rows = (double)a->R * a->T * a->Hq;
+  if (a->L == 0 || a->N == 0 || a->L > 64LL * kTcMaxStates || a->N > INT32_MAX / 4 || rows > 2e9) return false;
+  return a->dtype == MVR_F32 ? a->D <= 64 && rows * a->L >= kPieceScores : a->D % 8 == 0 && a->D <= 128;
 }
 bool rows_aligned(const void* base, const int64_t (&strides)[3], const mvr_attention* a) {
   const int64_t sizes[3] = {a->R, a->T, a->Hq};
@@ -159,6 +173,7 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   p.lengths = a->lengths; p.lengths64 = a->lengths_64; p.mask = a->mask;
   p.R = (int)a->R; p.T = (int)a->T; p.Hq = (int)a->Hq; p.Hk = (int)a->Hk; p.G = (int)(a->Hq / a->Hk);
   p.N = (int)a->N; p.L = (int)a->L; p.D = (int)a->D;
+  p.W = c.W;
   p.by_T.set((unsigned)std::max(1, p.T));
   p.by_G.set((unsigned)p.G);
   p.scale = a->scale;
@@ -222,10 +237,10 @@ int sum_parts(const float* part, void* dst, long long n, int parts, float factor
   return launched();
 }
 
-template <typename T, int DP, int TILES, bool MASK>
+template <typename T, int DP, int TILES, bool MASK, int PIECES>
 int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
-  typedef TcForward<DP, TILES, MASK> F;
-  const auto kernel = attn_tc_fwd<T, DP, TILES, MASK>;
+  typedef TcForward<DP, TILES, MASK, PIECES> F;
+  const auto kernel = attn_tc_fwd<T, DP, TILES, MASK, PIECES>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::kShared) != cudaSuccess) {
     cudaGetLastError();
     return MVR_ERR_LAUNCH;
@@ -233,26 +248,27 @@ int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int
   launch_dependent(kernel, dim3((unsigned)c.row_tiles, p.Hk, c.splits), dim3(F::kThreads), F::kShared, st, p, maps, status);
   return launched();
 }
-template <typename T, int DP>
+template <typename T, int DP, int PIECES>
 int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   const bool mask = p.mask || p.lengths;
   if constexpr (DP == 128) {
-    if (c.tile > kTcRows) return mask ? tc_forward_as<T, DP, 2, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false>(p, c, maps, status, st);
+    if (c.tile > kTcRows)
+      return mask ? tc_forward_as<T, DP, 2, true, 1>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false, 1>(p, c, maps, status, st);
   }
-  return mask ? tc_forward_as<T, DP, 1, true>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, false>(p, c, maps, status, st);
+  return mask ? tc_forward_as<T, DP, 1, true, PIECES>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, false, PIECES>(p, c, maps, status, st);
 }
 
 template <typename T>
-bool tensor_maps(const mvr_attention* a, bool backward, TcMaps& maps, bool& boxes) {
+bool tensor_maps(const mvr_attention* a, bool backward, int pieces, TcMaps& maps, bool& boxes) {
   const int D = (int)a->D, G = (int)(a->Hq / a->Hk);
   const auto states = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-    return tc_map<T>(m, base, D, (int)a->Hk, (int)a->L, (int)a->N, s[2], s[1], s[0], 1, kTcBox);
+    return tc_map<T>(m, base, D, (int)a->Hk, (int)a->L, (int)a->N * pieces, s[2], s[1], s[0], 1, kTcBox);
   };
   if (!states(&maps.k, a->k, a->k_strides) || !states(&maps.v, a->v, a->v_strides)) return false;
   const int step = D <= 64 ? kGradStep<64> : kGradStep<128>;
   if (backward && !a->has_index && a->R > 0 && a->T > 0 && step % G == 0) {
     const auto rows = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-      return tc_map<T>(m, base, D, (int)a->Hq, (int)a->T, (int)a->R, s[2], s[1], s[0], G, step / G);
+      return tc_map<T>(m, base, D, (int)a->Hq, (int)a->T, (int)a->R * pieces, s[2], s[1], s[0], G, step / G);
     };
     boxes = rows(&maps.q, a->q, a->q_strides) && rows(&maps.g, a->grad_out, a->g_strides);
   }
@@ -262,14 +278,13 @@ bool tensor_maps(const mvr_attention* a, bool backward, TcMaps& maps, bool& boxe
 template <typename T>
 int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   int rc;
-  if constexpr (sizeof(T) == 2) {
-    rc = c.tc ? (p.D <= 64 ? tc_forward<T, 64>(p, c, maps, status, st) : tc_forward<T, 128>(p, c, maps, status, st)) : MVR_ERR_UNSUPPORTED;
+  if (c.tc) {
+    if constexpr (sizeof(T) == 2) rc = p.D <= 64 ? tc_forward<T, 64, 1>(p, c, maps, status, st) : tc_forward<T, 128, 1>(p, c, maps, status, st);
+    else rc = tc_forward<__nv_bfloat16, 64, 3>(p, c, maps, status, st);
   } else {
-    rc = MVR_ERR_UNSUPPORTED;
-  }
-  if (!c.tc)
     rc = p.D <= 32 ? fma_forward<T, 32>(p, c, st) : p.D <= 64 ? fma_forward<T, 64>(p, c, st)
          : p.D <= 128 ? fma_forward<T, 128>(p, c, st) : fma_forward<T, 256>(p, c, st);
+  }
   if (rc != MVR_OK || c.splits == 1) return rc;
   const long long outputs = (long long)p.R * p.T * p.Hq * p.D;
   if (p.D % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(T)) == 0)
@@ -279,7 +294,7 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
   return launched();
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int PIECES>
 int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
   const auto run = [&](auto kernel, dim3 grid, int threads, size_t smem, auto... args) {
     if (grid.x == 0) return MVR_OK;
@@ -291,17 +306,23 @@ int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool 
     return launched();
   };
   const dim3 states((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits);
-  const int rc = boxes ? run(attn_tc_dkv<T, DP, true>, states, TcStates<DP>::kThreads, TcStates<DP>::kShared, peaks, status)
-                       : run(attn_tc_dkv<T, DP, false>, states, TcStates<DP>::kThreads, TcStates<DP>::kShared, peaks, status);
+  typedef TcStates<DP, PIECES> S;
+  const int rc = boxes ? run(attn_tc_dkv<T, DP, true, PIECES>, states, S::kThreads, S::kShared, peaks, status)
+                       : run(attn_tc_dkv<T, DP, false, PIECES>, states, S::kThreads, S::kShared, peaks, status);
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
   const float* bounds = peaks;
-  if (p.mask || p.lengths) return run(attn_tc_dq<T, DP, true>, grid, TcRows<DP, true>::kThreads, TcRows<DP, true>::kShared, bounds, status);
-  return run(attn_tc_dq<T, DP, false>, grid, TcRows<DP, false>::kThreads, TcRows<DP, false>::kShared, bounds, status);
+  if (p.mask || p.lengths) {
+    typedef TcRows<DP, true, PIECES> F;
+    return run(attn_tc_dq<T, DP, true, PIECES>, grid, F::kThreads, F::kShared, bounds, status);
+  }
+  typedef TcRows<DP, false, PIECES> F;
+  return run(attn_tc_dq<T, DP, false, PIECES>, grid, F::kThreads, F::kShared, bounds, status);
 }
 
+// plain: the call's own tensors, where the operands are in pieces.
 template <typename T>
-int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
+int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
   if (c.tc && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
@@ -309,14 +330,19 @@ int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps
     return MVR_ERR_LAUNCH;
   }
   if (rows > 0) {
+    bool done = false;
     if constexpr (sizeof(T) == 2) {
+      done = c.tc;
       if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)std::min<long long>(cdiv(rows, 16), 8 * kMultiprocessors)), dim3(256), 0, st, p, peaks);
     }
-    if (!c.tc) launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, p);
+    if (!done) launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, plain);
     if ((rc = launched()) != MVR_OK) return rc;
   }
-  if constexpr (sizeof(T) == 2) {
-    if (c.tc) rc = p.D <= 64 ? tc_backward<T, 64>(p, c, maps, boxes, peaks, status, st) : tc_backward<T, 128>(p, c, maps, boxes, peaks, status, st);
+  if (c.tc) {
+    if constexpr (sizeof(T) == 2)
+      rc = p.D <= 64 ? tc_backward<T, 64, 1>(p, c, maps, boxes, peaks, status, st) : tc_backward<T, 128, 1>(p, c, maps, boxes, peaks, status, st);
+    else
+      rc = tc_backward<__nv_bfloat16, 64, 3>(p, c, maps, boxes, peaks, status, st);
   }
   if (!c.tc)
     rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
@@ -327,20 +353,61 @@ int attention_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps
   return rc;
 }
 
+// Float operands of a call in pieces, in its workspace; `b` is the call on them.
+int split_operands(const mvr_attention* a, bool backward, const AttnCut& c, char* ws, mvr_attention& b, AttnParams& p, cudaStream_t st) {
+  const auto split = [&](const void* from, const int64_t (&s)[3], long long n0, long long n1, long long n2, long long to) {
+    const long long rows = n0 * n1 * n2;
+    if (rows > 0)
+      launch_dependent(split_floats, dim3((unsigned)cdiv(rows * (c.W / 8), 256)), dim3(256), 0, st, (const float*)from, (long long)s[0], (long long)s[1],
+                       (long long)s[2], (int)n1, (int)n2, rows, (int)a->D, c.W, (__nv_bfloat16*)(ws + to));
+    return launched();
+  };
+  int rc = split(a->q, a->q_strides, a->R, a->T, a->Hq, c.q);
+  if (rc == MVR_OK) rc = split(a->k, a->k_strides, a->N, a->L, a->Hk, c.k);
+  if (rc == MVR_OK) rc = split(a->v, a->v_strides, a->N, a->L, a->Hk, c.v);
+  if (rc == MVR_OK && backward) rc = split(a->grad_out, a->g_strides, a->R, a->T, a->Hq, c.g);
+  if (rc != MVR_OK) return rc;
+  b = *a;
+  b.D = c.W;
+  b.q = ws + c.q; b.k = ws + c.k; b.v = ws + c.v; b.grad_out = ws + c.g;
+  const int64_t W = c.W;
+  for (int64_t(*s)[3] : {&b.q_strides, &b.g_strides}) (*s)[0] = a->T * a->Hq * W, (*s)[1] = a->Hq * W, (*s)[2] = W;
+  for (int64_t(*s)[3] : {&b.k_strides, &b.v_strides}) (*s)[0] = a->L * a->Hk * W, (*s)[1] = a->Hk * W, (*s)[2] = W;
+  p.q = b.q; p.k = b.k; p.v = b.v; p.g = b.grad_out;
+  p.q_r = p.g_r = b.q_strides[0]; p.q_t = p.g_t = b.q_strides[1]; p.q_h = p.g_h = W;
+  p.k_n = p.v_n = b.k_strides[0]; p.k_l = p.v_l = b.k_strides[1]; p.k_h = p.v_h = W;
+  p.q_piece = p.g_piece = a->R * a->T * a->Hq * W;
+  return MVR_OK;
+}
+
 template <typename T>
 int attention_as(const mvr_attention* a, bool backward, char* workspace, int* status, cudaStream_t st) {
   TcMaps maps = {};
   bool boxes = false;
-  bool tc = tc_sizes(a) && rows_aligned(a->q, a->q_strides, a) && (uintptr_t)a->out % 16 == 0;
-  if (backward)
-    tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
-  if constexpr (sizeof(T) == 2) tc = tc && tensor_maps<T>(a, backward, maps, boxes);
+  bool tc = tc_sizes(a);
+  if constexpr (sizeof(T) == 2) {
+    tc = tc && (uintptr_t)a->out % 16 == 0 && rows_aligned(a->q, a->q_strides, a);
+    if (backward)
+      tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
+    tc = tc && tensor_maps<T>(a, backward, 1, maps, boxes);
+  }
   const AttnCut c = cut_attention(a, backward, tc);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
-  const int rc = plan_attention(a, c, workspace, status, st);
+  int rc = plan_attention(a, c, workspace, status, st);
   if (rc != MVR_OK) return rc;
-  const AttnParams p = attention_params(a, c, workspace);
-  return backward ? attention_backward<T>(p, c, maps, boxes, (float*)(workspace + c.peaks), status, st) : attention_forward<T>(p, c, maps, status, st);
+  AttnParams p = attention_params(a, c, workspace);
+  if constexpr (sizeof(T) == 4) {
+    if (tc) {
+      const AttnParams plain = p;
+      mvr_attention b;
+      if ((rc = split_operands(a, backward, c, workspace, b, p, st)) != MVR_OK) return rc;
+      if (!tensor_maps<__nv_bfloat16>(&b, backward, 3, maps, boxes)) return MVR_ERR_LAUNCH;
+      return backward ? attention_backward<T>(p, plain, c, maps, boxes, (float*)(workspace + c.peaks), status, st)
+                      : attention_forward<T>(p, c, maps, status, st);
+    }
+  }
+  return backward ? attention_backward<T>(p, p, c, maps, boxes, (float*)(workspace + c.peaks), status, st)
+                  : attention_forward<T>(p, c, maps, status, st);
 }
 
 long long attention_bytes(const mvr_attention* a, bool backward) {

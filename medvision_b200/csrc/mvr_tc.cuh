@@ -200,9 +200,10 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 // d (+)= a b over `depth` sixteens of K-major tiles in blocks of 64 elements a row, `block_a` and `block_b` bytes each.
 template <int MOST>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, int depth, uint32_t block_a, uint32_t block_b) {
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, int depth, uint32_t block_a, uint32_t block_b,
+                                         bool add = false) {
   const auto step = [&](int k) {
-    mma_ss(d, a + (((k >> 2) * block_a + (k & 3) * 32) >> 4), b + (((k >> 2) * block_b + (k & 3) * 32) >> 4), shape, k > 0);
+    mma_ss(d, a + (((k >> 2) * block_a + (k & 3) * 32) >> 4), b + (((k >> 2) * block_b + (k & 3) * 32) >> 4), shape, add || k > 0);
   };
   const auto steps = [&](auto n) {  // (a number the compiler knows: a loop issues at half the rate)
 #pragma unroll
@@ -263,6 +264,61 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// ---- float operands in pieces --------------------------------------------------------------------------
+// A float is the exact sum of three bfloat16 numbers, its 24 bits eight at a time (cut off, so that no piece overflows).  A product of
+// two floats is that of their pieces; of the nine, the three whose size is 2^-24 of the product or less are left out: six products of
+// bfloat16 operands, summed in float, for one of float operands.
+template <int PIECES, typename F>
+__device__ __forceinline__ void for_pairs(F&& f) {  // f(piece of a, piece of b, is it the first): small products first
+  if constexpr (PIECES == 1) {
+    f(0, 0, true);
+  } else {
+    f(1, 1, true);
+    f(0, 2, false);
+    f(2, 0, false);
+    f(0, 1, false);
+    f(1, 0, false);
+    f(0, 0, false);
+  }
+}
+// Two floats as the three words of their pieces.
+__device__ __forceinline__ void pieces_of(float2 f, uint32_t& a, uint32_t& b, uint32_t& c) {
+  const float2 neg = make_float2(-1.0f, -1.0f);
+  a = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+  f = fma2(make_float2(__uint_as_float(__float_as_uint(f.x) & 0xffff0000u), __uint_as_float(__float_as_uint(f.y) & 0xffff0000u)), neg, f);
+  b = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+  f = fma2(make_float2(__uint_as_float(__float_as_uint(f.x) & 0xffff0000u), __uint_as_float(__float_as_uint(f.y) & 0xffff0000u)), neg, f);
+  c = pack2<__nv_bfloat16>(f.x, f.y);
+}
+
+// Rows of D floats (three outer dimensions with strides) as pieces: to[piece][row][W], W: D rounded up to 8, zeros behind D.  A thread
+// takes eight columns.  An infinity is its first piece, the others 0.
+__global__ void __launch_bounds__(256) split_floats(const float* from, long long s0, long long s1, long long s2, int n1, int n2, long long rows,
+                                                    int D, int W, __nv_bfloat16* to) {
+  grid_dependency();
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (W / 8);
+  if (row >= rows) return;
+  const int col = (int)(id - row * (W / 8)) * 8;
+  const long long i01 = row / n2, i0 = i01 / n1;
+  const float* src = from + i0 * s0 + (i01 - i0 * n1) * s1 + (row - i01 * n2) * s2 + col;
+  float f[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = col + k < D ? src[k] : 0.0f;
+  uint32_t w[3][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    pieces_of(make_float2(f[2 * k], f[2 * k + 1]), w[0][k], w[1][k], w[2][k]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (!(fabsf(f[2 * k + h]) < INFINITY)) {  // (infinity less itself is no number)
+        w[1][k] &= h ? 0xffffu : 0xffff0000u;
+        w[2][k] &= h ? 0xffffu : 0xffff0000u;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *(uint4*)(to + (k * rows + row) * W + col) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
