@@ -74,7 +74,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
   const bool wide = a->D > 64, uneven = a->lengths || a->mask;
-  const StepTime walk = pieces ? (backward ? StepTime{1, 4.0, 4.0} : StepTime{2, 2.5, 4.0}) : !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
+  const StepTime walk = pieces ? (backward ? StepTime{1, 4.5, 4.5} : StepTime{2, 2.6, 4.0}) : !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
                         : c.tile > kTcRows ? StepTime{1, 2.1, 2.1} : wide ? StepTime{2, 1.5, 1.8} : StepTime{4, 0.85, 1.5};
   // (a part's sums are written and read at 4 MB/us)
   c.splits = best_parts(expected, kv_tiles, walk, rows * a->D * 8 / 4e6, uneven);
