@@ -57,7 +57,7 @@ struct TcForward {
   static constexpr int kBlocks = DP / 64, kTileBytes = kBlocks * kTcRows * 128, kStepBytes = kBlocks * kStep * 128;
   static constexpr int kRowsBytes = PIECES * kTileBytes, kSlotBytes = PIECES * kStepBytes;  // of a row tile and of a place of the ring
   static constexpr int kSlots = PIECES == 1 ? 4 : 2;
-  static constexpr int kSoftmax = TILES * kHalves * 128, kThreads = kSoftmax + (PIECES == 1 ? 96 : 64);
+  static constexpr int kSoftmax = TILES * kHalves * 128, kThreads = kSoftmax + (TILES == 2 ? 96 : 64);
   // tensor memory: scores (P over them), third pieces of P, O
   static constexpr int kScores = 0, kThird = TILES * kStep, kOut = kThird + (PIECES == 1 ? 0 : 32);
   static constexpr int kColumns = TILES == 2 ? 512 : DP == 64 && PIECES == 1 ? 128 : 256;
@@ -220,6 +220,11 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   };
 
   if (warp == kLoader) {
+    constexpr int kBehind = F::kSlots == 4 ? 2 : 0;
+    const auto clean_values = [&](int item) {
+      bar_pass(smem_at(&c.full[item % F::kSlots]), (item / F::kSlots) & 1, lost);
+      clean(item >> 1, item % F::kSlots);
+    };
     int i = 0;
     for (; i < 2 * tiles; ++i) {  // K0 V0 K1 V1 ...
       const int slot = i % F::kSlots;
@@ -238,12 +243,11 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
                           b * 64, hk, j + r, o.n + piece * p.N);
       }
       __syncwarp();
-      // (with pieces, registers are for two CTAs of six warps: this one clears rows of V as well)
-      if (MASK && PIECES == 3 && (i & 1)) {
-        bar_pass(bar, (i / F::kSlots) & 1, lost);
-        clean(i >> 1, slot);
-      }
+      // One row tile: registers go further with six warps a CTA, so this one clears rows of V as well, a tile behind where the ring
+      // holds two.
+      if (MASK && TILES == 1 && (i & 1) && i >= kBehind) clean_values(i - kBehind);
     }
+    if (MASK && TILES == 1 && kBehind > 0 && i == 2 * tiles && tiles > 0) clean_values(i - 1);
     // given up: the copies under way end before the CTA does
     if (*lost)
       for (int k = max(0, i - F::kSlots); k < i; ++k) {
@@ -311,7 +315,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       for (int t = 0; t < TILES; ++t) commit(&c.out[t]);
     }
-  } else if (MASK && PIECES == 1 && warp == kCleaner) {
+  } else if (MASK && TILES == 2 && warp == kCleaner) {
     for (int j = 0; j < tiles; ++j) {
       const int v = 2 * j + 1, slot = v % F::kSlots;
       if (!bar_wait(smem_at(&c.full[slot]), (v / F::kSlots) & 1, lost)) break;
