@@ -36,6 +36,9 @@ struct AttnParams {
   long long q_r, q_t, q_h, g_r, g_t, g_h;        // strides in elements; the last dimension is contiguous
   long long k_n, k_l, k_h, v_n, v_l, v_h;
   const int *order, *starts, *tiles;             // grouping by image, or null: region r reads image r
+  const void* index;                             // set: no grouping; tile t is all rows of image t, found from the index (forward)
+  int index_type;
+  long long index_stride;
   const void* lengths;                           // (N) int32 or int64, or null
   int lengths64;
   const unsigned char* mask;                     // (N, L) or null

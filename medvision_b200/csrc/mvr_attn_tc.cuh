@@ -66,7 +66,8 @@ struct TcForward {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots];
     unsigned long long queries[TILES], scores[TILES], weights[TILES], out[TILES], halves[TILES];
     uint32_t tmem;
-    int lost, tiles;
+    int lost, tiles, regions;
+    int order[TILES == 1 ? kTcRows : 1];          // regions of the image, where the index is not grouped
     float top[kHalves == 2 ? 2 : 1][TILES][2][128];  // what the two halves of a row tell each other
     unsigned short list[MASK ? kMaxTiles : 1];
     StateBits<kStep> bits[MASK ? kMaxTiles : 1];
@@ -196,8 +197,30 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
   RowTile o;
-  const bool some = row_tile(p, blockIdx.x, TILES * kTcRows, o);
   const int hk = blockIdx.y, split = blockIdx.z;
+  bool some;
+  if (TILES == 1 && p.index) {
+    // few regions: the CTA looks for those of its image itself, which is faster than a kernel that groups them
+    const int n = blockIdx.x;
+    if (warp == 0) {
+      int at = 0;
+      for (int r0 = 0; r0 < p.R; r0 += 32) {
+        const bool mine = r0 + lane < p.R && image_index(p.index, p.index_type, p.index_stride, r0 + lane, p.N) == n;
+        const uint32_t who = __ballot_sync(~0u, mine);
+        if (mine) c.order[at + __popc(who & ((1u << lane) - 1))] = r0 + lane;
+        at += __popc(who);
+      }
+      if (lane == 0) {
+        c.regions = at;
+        if (n == p.N && at > 0 && hk == 0 && split == 0 && status) atomicOr(status, 1);
+      }
+    }
+    __syncthreads();
+    o = {n, 0, c.regions * p.T * p.G, c.order};
+    some = o.rows > 0;
+  } else {
+    some = row_tile(p, blockIdx.x, TILES * kTcRows, o);
+  }
   const int all = (p.L + F::kStep - 1) / F::kStep, per = (all + p.splits - 1) / p.splits;
   const int begin = split * per * F::kStep;
   int end = 0;

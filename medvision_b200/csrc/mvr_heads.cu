@@ -29,6 +29,7 @@ constexpr size_t kPlanShared = 200 * 1024;
 // How a call is cut into CTAs, and what lies where in its workspace.
 struct AttnCut {
   bool tc;                      // tensor cores (mvr_attn_tc.cuh); float operands in pieces
+  bool direct;                  // few regions: the kernel finds those of an image itself
   int W;                        // columns of the operands in memory
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
@@ -71,6 +72,8 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   c.tile = tc ? (rows_of_image > kTcRows && !backward && a->D > 64 ? 2 * kTcRows : kTcRows) : a->D <= 128 ? 64 : 32;
   c.kv_tile = tc ? 128 : c.tile;  // (some kernels walk half of that at a time)
   c.row_tiles = a->has_index ? cdiv(a->R * per, c.tile) + std::min(a->N + 1, a->R) : a->R * cdiv(per, c.tile);
+  c.direct = tc && !backward && a->has_index && a->R * per <= kTcRows && a->N <= 256;
+  if (c.direct) c.row_tiles = a->N + 1;
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
   const bool wide = a->D > 64, uneven = a->lengths || a->mask;
@@ -88,7 +91,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  if (a->has_index) {
+  if (a->has_index && !c.direct) {
     c.order = take(a->R * 4);
     c.starts = take((a->N + 2) * 4);
     c.tiles = take((a->N + 2) * 4);
@@ -168,7 +171,9 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   p.k_n = a->k_strides[0]; p.k_l = a->k_strides[1]; p.k_h = a->k_strides[2];
   p.v_n = a->v_strides[0]; p.v_l = a->v_strides[1]; p.v_h = a->v_strides[2];
   p.g_r = a->g_strides[0]; p.g_t = a->g_strides[1]; p.g_h = a->g_strides[2];
-  if (a->has_index) {
+  if (c.direct) {
+    p.index = a->index; p.index_type = a->index_type; p.index_stride = a->index_stride;
+  } else if (a->has_index) {
     p.order = (const int*)(ws + c.order); p.starts = (const int*)(ws + c.starts); p.tiles = (const int*)(ws + c.tiles);
   }
   p.lengths = a->lengths; p.lengths64 = a->lengths_64; p.mask = a->mask;
@@ -187,7 +192,7 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
 }
 
 int plan_attention(const mvr_attention* a, const AttnCut& c, char* ws, int* status, cudaStream_t st) {
-  if (!a->has_index) return MVR_OK;
+  if (!a->has_index || c.direct) return MVR_OK;
   const int groups = (int)a->N + 1;
   const int warps = (int)std::max<long long>(1, std::min<long long>({32, cdiv(a->R, 32), (long long)(kPlanShared / 4 / groups)}));
   const size_t smem = (size_t)warps * groups * 4;

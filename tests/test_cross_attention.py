@@ -122,7 +122,7 @@ def test_against_the_formula(shape, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("kind", ["lengths", "mask", "both"])
-@pytest.mark.parametrize("tokens,dim", [(1, 32), (49, 64), (3, 20)])
+@pytest.mark.parametrize("tokens,dim", [(1, 32), (49, 64), (3, 20), (2, 128)])
 def test_regions_of_images_with_states_left_out(dtype, kind, tokens, dim):
     """Regions in no order, images without regions, without states, indices outside; the states left out hold NaN and infinities."""
     R, N, L, H, Hk = 23, 6, 211, 4, 2
