@@ -4,7 +4,9 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/mvr.h"
 #include "mvr_attn_fma.cuh"
@@ -191,44 +193,54 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   return p;
 }
 
+// Lets a kernel have `smem` bytes of dynamic shared memory, once per device.  (The same limit in every call of a kernel: calls of
+// several threads do not undo one another's.)
+template <auto KERNEL>
+bool shared_memory(size_t smem) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
+template <auto KERNEL, typename... A>
+int launch_shared(dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  if (grid.x == 0 || grid.y == 0) return MVR_OK;
+  if (!shared_memory<KERNEL>(smem)) return MVR_ERR_LAUNCH;
+  launch_dependent(KERNEL, grid, dim3(threads), smem, st, args...);
+  return launched();
+}
+
 int plan_attention(const mvr_attention* a, const AttnCut& c, char* ws, int* status, cudaStream_t st) {
   if (!a->has_index || c.direct) return MVR_OK;
   const int groups = (int)a->N + 1;
   const int warps = (int)std::max<long long>(1, std::min<long long>({32, cdiv(a->R, 32), (long long)(kPlanShared / 4 / groups)}));
   const size_t smem = (size_t)warps * groups * 4;
-  // (always the same limit: calls of several threads do not undo one another's)
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(attn_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanShared) != cudaSuccess) {
-    cudaGetLastError();
-    return MVR_ERR_LAUNCH;
-  }
+  if (!shared_memory<attn_plan>(kPlanShared)) return MVR_ERR_LAUNCH;
   launch_dependent(attn_plan, dim3(1), dim3(kPlanThreads), smem, st, a->index, a->index_type, (long long)a->index_stride, (int)a->R,
                    (int)a->N, (int)(a->T * (a->Hq / a->Hk)), c.tile, warps, (int*)(ws + c.order), (int*)(ws + c.starts),
                    (int*)(ws + c.tiles), status);
   return launched();
 }
 
-template <typename K>
-int launch_fma(K kernel, dim3 grid, size_t smem, cudaStream_t st, const AttnParams& p) {
-  if (grid.x == 0 || grid.y == 0) return MVR_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return MVR_ERR_LAUNCH;
-  }
-  launch_dependent(kernel, grid, dim3(kFmaThreads), smem, st, p);
-  return launched();
-}
-
 template <typename T, int DP>
 int fma_forward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
-  return launch_fma(attn_fma_fwd<T, DP>, dim3((unsigned)c.row_tiles, p.Hk, c.splits), FmaTile<DP>::bytes(3), st, p);
+  return launch_shared<attn_fma_fwd<T, DP>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), kFmaThreads, FmaTile<DP>::bytes(3), st, p);
 }
 template <typename T, int DP>
 int fma_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
   if (p.R > 0 && p.T > 0) {
-    const int rc = launch_fma(attn_fma_dq<T, DP>, dim3((unsigned)c.row_tiles, p.Hk, c.splits), FmaTile<DP>::bytes(4), st, p);
+    const int rc = launch_shared<attn_fma_dq<T, DP>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), kFmaThreads, FmaTile<DP>::bytes(4), st, p);
     if (rc != MVR_OK) return rc;
   }
-  return launch_fma(attn_fma_dkv<T, DP>, dim3((unsigned)(cdiv(p.L, c.kv_tile) * p.N), p.Hk, c.row_splits), FmaTile<DP>::bytes(4), st, p);
+  return launch_shared<attn_fma_dkv<T, DP>>(dim3((unsigned)(cdiv(p.L, c.kv_tile) * p.N), p.Hk, c.row_splits), kFmaThreads, FmaTile<DP>::bytes(4), st, p);
 }
 
 unsigned blocks_of(long long n, int per) { return (unsigned)std::min<long long>(cdiv(n, per), 1 << 20); }
@@ -246,13 +258,7 @@ int sum_parts(const float* part, void* dst, long long n, int parts, float factor
 template <typename T, int DP, int TILES, bool MASK, int PIECES>
 int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   typedef TcForward<DP, TILES, MASK, PIECES> F;
-  const auto kernel = attn_tc_fwd<T, DP, TILES, MASK, PIECES>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::kShared) != cudaSuccess) {
-    cudaGetLastError();
-    return MVR_ERR_LAUNCH;
-  }
-  launch_dependent(kernel, dim3((unsigned)c.row_tiles, p.Hk, c.splits), dim3(F::kThreads), F::kShared, st, p, maps, status);
-  return launched();
+  return launch_shared<attn_tc_fwd<T, DP, TILES, MASK, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);
 }
 template <typename T, int DP, int PIECES>
 int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
@@ -302,28 +308,18 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
 
 template <typename T, int DP, int PIECES>
 int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
-  const auto run = [&](auto kernel, dim3 grid, int threads, size_t smem, auto... args) {
-    if (grid.x == 0) return MVR_OK;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-      cudaGetLastError();
-      return MVR_ERR_LAUNCH;
-    }
-    launch_dependent(kernel, grid, dim3(threads), smem, st, p, maps, args...);
-    return launched();
-  };
   const dim3 states((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits);
   typedef TcStates<DP, PIECES> S;
-  const int rc = boxes ? run(attn_tc_dkv<T, DP, true, PIECES>, states, S::kThreads, S::kShared, peaks, status)
-                       : run(attn_tc_dkv<T, DP, false, PIECES>, states, S::kThreads, S::kShared, peaks, status);
+  const int rc = boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, peaks, status)
+                       : launch_shared<attn_tc_dkv<T, DP, false, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, peaks, status);
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
-  const float* bounds = peaks;
   if (p.mask || p.lengths) {
     typedef TcRows<DP, true, PIECES> F;
-    return run(attn_tc_dq<T, DP, true, PIECES>, grid, F::kThreads, F::kShared, bounds, status);
+    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const float*)peaks, status);
   }
   typedef TcRows<DP, false, PIECES> F;
-  return run(attn_tc_dq<T, DP, false, PIECES>, grid, F::kThreads, F::kShared, bounds, status);
+  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const float*)peaks, status);
 }
 
 // plain: the call's own tensors, where the operands are in pieces.
@@ -331,7 +327,7 @@ template <typename T>
 int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
-  if (c.tc && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
+  if (c.tc && std::is_same<T, __half>::value && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
     cudaGetLastError();
     return MVR_ERR_LAUNCH;
   }
