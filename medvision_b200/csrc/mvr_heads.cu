@@ -272,6 +272,7 @@ int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* s
 
 template <typename T>
 bool tensor_maps(const mvr_attention* a, bool backward, int pieces, TcMaps& maps, bool& boxes) {
+  tc_need_context();
   const int D = (int)a->D, G = (int)(a->Hq / a->Hk);
   const auto states = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
     return tc_map<T>(m, base, D, (int)a->Hk, (int)a->L, (int)a->N * pieces, s[2], s[1], s[0], 1, kTcBox);

@@ -325,17 +325,28 @@ __global__ void __launch_bounds__(256) split_floats(const float* from, long long
 typedef CUresult (*TcEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline void* tc_driver_function(const char* name) {
+  void* ptr = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint(name, &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  return ptr;
+}
 inline TcEncodeTiled tc_encoder() {
-  static TcEncodeTiled fn = []() -> TcEncodeTiled {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      return nullptr;
-    }
-    return (TcEncodeTiled)ptr;
-  }();
+  static TcEncodeTiled fn = (TcEncodeTiled)tc_driver_function("cuTensorMapEncodeTiled");
   return fn;
+}
+// Makes the runtime's context current in a thread that has not called CUDA yet (autograd's threads, a data loader's): a tensor map
+// cannot be made without one.
+inline void tc_need_context() {
+  static CUresult (*const current)(CUcontext*) = (CUresult(*)(CUcontext*))tc_driver_function("cuCtxGetCurrent");
+  CUcontext context = nullptr;
+  int device = 0;
+  if (current && current(&context) == CUDA_SUCCESS && context) return;
+  if (cudaGetDevice(&device) == cudaSuccess) cudaSetDevice(device);
+  cudaGetLastError();
 }
 
 // Map over (D, heads, rows, images), D contiguous elements of 2 bytes, boxes of 64 elements x `box_heads` x `box_rows`; false where

@@ -250,6 +250,31 @@ def test_the_same_call_gives_the_same_bits_on_any_stream_and_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_a_thread_that_has_not_called_cuda_gets_the_same_kernels():
+    """Tensor maps need a context: without one the call would take the kernels of float arithmetic, whose last bits differ."""
+    import subprocess
+    import sys
+    import threading
+    q, k, v, g = make(2, 70, 4, 2, 64, 2, 600, torch.float16, seed=12)
+    want = run(q, k, v, g)
+    got, cuda = [], [t.cuda() for t in (q, k, v)]
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: got.append(cross_attention(*cuda)))
+    thread.start()
+    thread.join()
+    assert torch.equal(got[0], want[0])
+    # the first gradient of a process, in autograd's new thread, equals the second
+    code = ("import torch; from medvision_b200.ops import cross_attention as f\n"
+            "t = [torch.randn(2, 300, 4, 64, device='cuda', dtype=torch.float16, requires_grad=True) for _ in range(3)]\n"
+            "a, b = (torch.autograd.grad(f(*t).sum(), t) for _ in range(2))\n"
+            "assert all(torch.equal(x, y) for x, y in zip(a, b))\n")
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_many_regions_of_many_images_are_grouped_right():
     R, N, L, D = 5000, 700, 3, 8
     q, k, v, _ = make(R, 1, 1, 1, D, N, L, torch.float32, seed=9)
