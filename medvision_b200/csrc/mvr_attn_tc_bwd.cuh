@@ -12,6 +12,11 @@
 // sums of one CTA only, which takes 128 x 128.  One thread issues the products in an order in which those of
 // one tile run under the exponentials of the next: dV(i), S(i+1), dK(i), dP(i+1), and S(i+1), dQ(i), dP(i+1).
 //
+// Measured (tensor pipe, function units, issue slots busy): 2 x 2048 rows of 16 heads of 64 (4 key heads) over 8191 and 6144 states,
+// bfloat16: states kept 0.33 ms (36, 36, 36 %), rows kept 0.30 ms (29, 39, 41 %).  Bound by a step's chain, as the forward is: two CTAs
+// an SM instead of one of twice the columns took it from 0.53 and 0.41 ms.  One exponential per score in each kernel is the price of
+// sums without atomics.
+//
 // float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= 2 D max|g| max|v|
 // below 2^15 (max|g| from attn_delta, max|v| over the states kept, or over all that the first kernel saw).  Both are taken out of
 // the sums again, exactly.

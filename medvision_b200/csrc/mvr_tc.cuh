@@ -269,7 +269,9 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
 // ---- float operands in pieces --------------------------------------------------------------------------
 // A float is the exact sum of three bfloat16 numbers, its 24 bits eight at a time (cut off, so that no piece overflows).  A product of
 // two floats is that of their pieces; of the nine, the three whose size is 2^-24 of the product or less are left out: six products of
-// bfloat16 operands, summed in float, for one of float operands.
+// bfloat16 operands, summed in float, for one of float operands.  (200 regions' queries, 4 heads of 64, over three images of 13 635
+// states, forward and backward: 0.30 ms, of which the cutting into pieces, bound by memory, is a quarter; in float arithmetic 0.51 ms.
+// Errors against float64 2.9e-7 to 5.3e-7; the plain float form has 2.5e-7 to 7.7e-7.)
 template <int PIECES, typename F>
 __device__ __forceinline__ void for_pairs(F&& f) {  // f(piece of a, piece of b, is it the first): small products first
   if constexpr (PIECES == 1) {
