@@ -3,10 +3,11 @@
 //
 // A CTA of 16 x 16 threads holds a stationary tile of BT rows and streams tiles of BT others through shared memory, padded by four
 // floats so that 16-byte reads of neighbouring rows fall on different banks.  Per tile a thread forms an (BT/16)^2 patch of
-// products from two 16-byte reads for 16 multiply-adds, stores its weights, and adds them into its rows' sums.  Bound by shared
-// memory's and the multiply-adds' pipes together: about a quarter of the peak (200 regions over three images of 13 635 states, 4 heads
-// of 64, forward 0.12 ms, backward 0.45 ms).  What is left to it: small float calls, where it is the faster form, float head sizes
-// above 64, half ones above 128, and operands that TMA cannot read.
+// products from two 16-byte reads for 16 multiply-adds, stores its weights, and adds them into its rows' sums.  Bound by the
+// issue of the multiply-adds and of the reads that feed them: issue slots 58 to 62 % busy in the gradients of 128 x 49 rows of 8 heads
+// of 32 over 2 x 4096 states.  (200 regions over three images of 13 635 states, 4 heads of 64, forward 0.12 ms, backward 0.45 to 0.53.)
+// What is left to it: small float calls, where it is the faster form, float head sizes above 64, half ones above 128, and
+// operands that TMA cannot read.
 #pragma once
 #include "mvr_attn.cuh"
 

@@ -12,12 +12,12 @@
 // time.  Beyond, two row tiles of one CTA alternate, which read every tile of states once for both, or, where rows are few, two CTAs
 // with a tile each.  Few rows: the states are cut into parts as well (attn_join).
 //
-// Measured (tensor pipe, function units, issue slots busy): 2 x 4096 rows of 16 heads of 128 over 8192 states, bfloat16: 0.53 ms, 1.04
-// PFLOP/s (49, 37, 41 %); 2 x 2048 rows of 16 heads of 64 (4 key heads) over 8191 and 6144: 0.22 ms, 0.55 PFLOP/s (26, 39, 45 %);
-// one token of 32 heads of 128 (8 key heads) in each of 32 caches of 8448 to 16384: 0.27 ms, 6.0 TB/s.  None of the units is the
-// limit: a step's chain (wait, fetch, maximum, exponentials, store, products) takes some 2200 cycles, and tensor memory holds no more
-// chains.  Keeping the scores in registers between maximum and exponentials spilled; a vote on each wait cost a tenth; of eight pairs
-// of exponentials two as polynomials were best (0: 3 % slower, 4: 6 %).
+// Measured (tensor pipe, function units, issue slots busy): 2 x 4096 rows of 16 heads of 128 over 8192 states, bfloat16: 0.53 ms in a
+// short run, 1.04 PFLOP/s (counters, in 0.56 ms: 49, 37, 41 %); 2 x 2048 rows of 16 heads of 64 (4 key heads) over 8191 and 6144:
+// 0.23 ms, 0.53 PFLOP/s (26, 39, 45 %); one token of 32 heads of 128 (8 key heads) in each of 32 caches of 8448 to 16384 states:
+// 0.27 ms, 6.0 TB/s.  None of the units is the limit of the first two: a step's chain (wait, fetch, maximum, exponentials, store) takes
+// 2100 to 2500 cycles of a CTA, and tensor memory holds no more CTAs.  Of eight pairs of exponentials two as polynomials were best
+// (none: 3 % slower, four: 6 %).
 //
 // States that are left out (lengths, mask) are compacted to a list of tiles with 128 bits each before the walk; tiles without a state
 // are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its

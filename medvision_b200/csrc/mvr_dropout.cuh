@@ -8,7 +8,7 @@
 // most 2^-17), and the scale is the inverse of the probability that results, so that the expectation is exact.
 //
 // Measured: 27.9 M bfloat16 elements with a residual 30 us (5.5 TB/s), their gradient 23 us (4.8 TB/s); 33.6 M float16 elements 26 us
-// (5.1 TB/s): 78 % of a plain copy's rate.  Half of the issue slots are busy with the generator's products beside the loads.
+// (5.1 TB/s): 85, 73 and 78 % of a plain copy's rate.  Half of the issue slots are busy with the generator's products beside the loads.
 #pragma once
 #include "mvr_types.cuh"
 

@@ -17,7 +17,7 @@
 //
 // Measured: 2 x 14 x 96^3 half scores with two alternatives 47 us, gradient 34 us (issue slots 54 and 55 % busy: the alternatives, the
 // exponentials and the conversions of 24.8 M scores beside the memory's 15 us); 2000 rows of 32 001 bfloat16 scores with eight
-// alternatives 57 us (issue 42 %, waits between the row's phases), gradient 49 us (4.5 TB/s); 16 rows of 81 float scores 6 us.
+// alternatives 57 us (issue 42 %, waits between the row's phases), gradient 49 us (5.2 TB/s); 16 rows of 81 float scores 6 us.
 #pragma once
 #include "mvr_types.cuh"
 

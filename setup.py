@@ -48,9 +48,9 @@ class BuildWithLibrary(build_py):
 setup(
     name="medvision-b200",
     version="0.2.0",
-    description="RoI Align / RoI Align Rotated / affine resampling of MedVision for NVIDIA B200 (sm_100a only)",
+    description="RoI Align / RoI Align Rotated / affine resampling of MedVision, attention, dropout and label log-probabilities behind them, for NVIDIA B200 (sm_100a only)",
     packages=find_packages(include=["medvision_b200", "medvision_b200.*"]),
-    package_data={"medvision_b200": ["libmvr.so", "_native.so", "include/mvr.h", "csrc/*.cu", "csrc/*.cuh", "csrc/*.cpp"]},
+    package_data={"medvision_b200": ["libmvr.so", "_native.so", "include/mvr.h", "csrc/*.cu", "csrc/*.cuh", "csrc/*.h", "csrc/*.cpp"]},
     python_requires=">=3.9",
     install_requires=["torch", "numpy"],
     cmdclass={"build_py": BuildWithLibrary},
