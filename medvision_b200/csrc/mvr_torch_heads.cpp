@@ -220,7 +220,7 @@ at::Tensor cross_attention(const at::Tensor& query, const at::Tensor& key, const
     TORCH_CHECK(s.mask.scalar_type() == at::kBool, what, ": mask must be bool (true: the state is read)");
   }
   if (default_scale) s.scale = 1.0 / std::sqrt((double)query.size(3));
-  TORCH_CHECK(std::isfinite(s.scale), what, ": scale must be finite");
+  TORCH_CHECK(std::isfinite((float)(s.scale * 1.4426950408889634)), what, ": scale must be finite (in float32, in powers of two)");
   TORCH_CHECK(query.size(3) <= 256, mvr_strerror(MVR_ERR_HEAD_SIZE));
   TORCH_CHECK(query.size(2) % key.size(2) == 0, mvr_strerror(MVR_ERR_HEADS));
   check_cuda(what, query);

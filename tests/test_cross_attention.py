@@ -317,6 +317,54 @@ def test_the_status_word_is_clean_after_all_kinds_of_calls():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape", [(2, 5, 4, 2, 33, 2, 40), (2, 140, 4, 2, 64, 2, 700), (2, 140, 4, 2, 128, 2, 700)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales_that_are_not_positive(shape, dtype, scale):
+    R, T, H, Hk, D, N, L = shape
+    q, k, v, g = make(*shape, dtype, seed=11)
+    allowed = torch.rand(N, L, generator=torch.Generator().manual_seed(12)) < 0.6
+    res, bound = reference(q, k, v, g, list(range(R)), allowed, scale, dtype)
+    for name, a, b, c in zip(NAMES, run(q, k, v, g, mask=allowed.cuda(), scale=scale), res, bound):
+        check(a, b, c, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("R,T,N", [(128, 1, 256), (129, 1, 256), (128, 1, 257), (64, 2, 3), (43, 3, 3), (1, 1, 1)])
+def test_edges_of_the_ways_regions_are_found(dtype, R, T, N):
+    """128 rows and 256 images are the most that a kernel looks through itself; many regions in one image, and some in none."""
+    from medvision_b200 import _C, _lib
+    L = 70 if dtype == torch.float16 else 2 ** 13  # (float: enough scores for the tensor cores)
+    if dtype == torch.float32 and N > 3:
+        L = 2 ** 12
+    q, k, v, g = make(R, T, 1, 1, 16, 1, L, dtype, seed=13)
+    k, v = k.expand(N, L, 1, 16), v.expand(N, L, 1, 16)
+    index = torch.randint(-1, N + 1, (R,), generator=torch.Generator().manual_seed(14))
+    index[: R // 2] = N - 1
+    _C.last_status()
+    with torch.no_grad():
+        got = cross_attention(q.cuda(), k.cuda(), v.cuda(), batch_index=index.cuda())
+    one, bound = reference(q, k[:1], v[:1], g, [0 if 0 <= i < N else -1 for i in index.tolist()], torch.ones(1, L, dtype=torch.bool), 0.25, dtype)
+    check(got, one[0], bound[0], "out")
+    outside = bool(((index < 0) | (index >= N)).any())
+    assert _C.last_status() == (_lib.MVR_STATUS_BAD_BATCH_INDEX if outside else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_states_that_no_region_reads_get_zero_gradients(dtype, dim):
+    q, k, v, g = make(150, 20, 2, 1, dim, 3, 300, dtype, seed=15)
+    index = torch.ones(150)
+    out, dq, dk, dv = run(q, k, v, g, batch_index=index.cuda())
+    for t in (dk, dv):
+        assert not bool(t[[0, 2]].any()) and bool(t[1].any())
+    none = run(q[:0], k, v, g[:0], batch_index=index[:0].cuda())
+    assert none[0].shape == q[:0].shape and not bool(none[2].any()) and not bool(none[3].any())
+
+
+@pytest.mark.gpu
 def test_empty_calls():
     for shape in [(0, 2, 2, 2, 16, 0, 5), (2, 0, 2, 2, 16, 2, 5), (2, 2, 2, 2, 16, 2, 0)]:
         q, k, v, g = make(*shape, torch.float16)
@@ -365,6 +413,8 @@ def test_refusals():
         cross_attention(q, k, v, mask=torch.ones(2, 5))
     with pytest.raises(RuntimeError, match="scale must be finite"):
         cross_attention(q, k, v, scale=math.inf)
+    with pytest.raises(RuntimeError, match="scale must be finite"):  # (in float32)
+        cross_attention(q, k, v, scale=1e300)
     with pytest.raises(TypeError, match="query must be a Tensor"):
         cross_attention(None, k, v)
 
