@@ -18,9 +18,10 @@
 // rest.  One exponential per score in each kernel is the price of
 // sums without atomics.
 //
-// float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= 2 D max|g| max|v|
-// below 2^15 (max|g| from attn_delta, max|v| over the states kept, or over all that the first kernel saw).  Both are taken out of
-// the sums again, exactly.
+// float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= |g.v| + |delta| below
+// 2^15.  Where states are kept that is D max|g| max|v| + max|delta|, max|v| over those states: delta averages the values of all
+// states, so that it has to be counted by itself (attn_tc_delta finds it).  Where rows are kept, 2 D max|g| max|v| with max|v| over all
+// that the first kernel saw.  Both powers are taken out of the sums again, exactly.
 #pragma once
 #include <type_traits>
 
@@ -33,11 +34,15 @@ constexpr int kGradStep = DP == 64 ? 64 : 128;  // columns of a tile
 
 __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
-// Power of two for dS, from bounds of |g| and |v| (float bits).
+// What a call's largest |g|, |v| and |delta| are kept in (float bits).
+struct Peaks {
+  float g, v, delta;
+};
+
+// Power of two for dS, from a bound of |dS|.
 template <typename T>
-__device__ __forceinline__ float slope_scale(int D, float g, float v) {
+__device__ __forceinline__ float slope_scale(float most) {
   if constexpr (TcType<T>::code == 1) return 1.0f;
-  const float most = 2.0f * D * g * v;
   if (!(most > 0.0f) || most > 3e38f) return 1.0f;
   const int e = 14 - ilogbf(most);
   return ldexpf(1.0f, e < -60 ? -60 : e > 60 ? 60 : e);
@@ -92,7 +97,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 // BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
 template <typename T, int DP, bool BOXES, int PIECES>
 __global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, PIECES>::kResident)
-attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, float* peaks, int* status) {
+attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, Peaks* peaks, int* status) {
   typedef TcStates<DP, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
@@ -336,8 +341,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (lane == 0) atomicMax(&c.peak, __float_as_int(most));
       group_sync(F::kGroups);
       const float peak = __int_as_float(c.peak);
-      if (threadIdx.x == 0) atomicMax((int*)peaks + 1, c.peak);
-      factor = slope_scale<T>(p.D, peaks[0], peak);
+      if (threadIdx.x == 0) atomicMax((int*)&peaks->v, c.peak);
+      factor = slope_scale<T>(p.D * peaks->g * peak + peaks->delta);
     }
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
     // With pieces, each tile's sums are added up in registers (dv in the first warpgroup, dk in the second): see the forward.
@@ -494,7 +499,7 @@ struct TcRows {
 
 template <typename T, int DP, bool MASK, int PIECES>
 __global__ void __launch_bounds__(TcRows<DP, MASK, PIECES>::kThreads, TcRows<DP, MASK, PIECES>::kResident)
-attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const float* peaks, int* status) {
+attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const Peaks* peaks, int* status) {
   typedef TcRows<DP, MASK, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
@@ -659,7 +664,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       fence_async_proxy();
       bar_arrive_warp(smem_at(&c.rows));
     }
-    const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(p.D, peaks[0], peaks[1]) : 1.0f;
+    const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(2.0f * p.D * peaks->g * peaks->v) : 1.0f;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
     // With pieces, each tile's sums are added up in registers (half the columns a warpgroup): see the forward.
     float acc[PIECES == 1 ? 1 : 32] = {};
@@ -764,17 +769,17 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   }
 }
 
-// delta = g.o per row, and the largest finite |g| (float bits) into peaks[0].  One warp a row.
+// delta = g.o per row, and the largest finite |g| and |delta|.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p, float* peaks) {
+__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p, Peaks* peaks) {
   grid_dependency();
-  __shared__ int peak;
-  if (threadIdx.x == 0) peak = 0;
+  __shared__ int peak[2];
+  if (threadIdx.x < 2) peak[threadIdx.x] = 0;
   __syncthreads();
   const long long rows = (long long)p.R * p.T * p.Hq;
   const int lane = threadIdx.x & 31, per = p.D / 8;  // a lane takes 8 elements of a row; 32 / width rows a warp
   const int width = per <= 4 ? 4 : per <= 8 ? 8 : 16, sub = lane / width, piece = lane % width;
-  float most = 0.0f;
+  float most = 0.0f, most_delta = 0.0f;
   for (long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / width); first < rows; first += (long long)gridDim.x * 8 * (32 / width)) {
     const long long row = first + sub;
     float v = 0.0f;
@@ -791,13 +796,23 @@ __global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ Att
       }
     }
     for (int d = width / 2; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+    if (fabsf(v) <= 3e38f) most_delta = fmaxf(most_delta, fabsf(v));
     if (row < rows && piece == 0) p.delta[row] = v;
   }
   if constexpr (TcType<T>::code == 0) {
-    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-    if (lane == 0) atomicMax(&peak, __float_as_int(most));
+    for (int d = 16; d; d >>= 1) {
+      most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+      most_delta = fmaxf(most_delta, __shfl_xor_sync(~0u, most_delta, d));
+    }
+    if (lane == 0) {
+      atomicMax(&peak[0], __float_as_int(most));
+      atomicMax(&peak[1], __float_as_int(most_delta));
+    }
     __syncthreads();
-    if (threadIdx.x == 0) atomicMax((int*)peaks, peak);
+    if (threadIdx.x == 0) {
+      atomicMax((int*)&peaks->g, peak[0]);
+      atomicMax((int*)&peaks->delta, peak[1]);
+    }
   }
 }
 

@@ -106,7 +106,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   }
   if (backward) {
     c.delta = take(rows * 4);
-    c.peaks = take(8);
+    c.peaks = take(sizeof(Peaks));
     if (c.splits > 1) c.part_gq = take(c.splits * rows * a->D * 4);
     if (c.row_splits > 1) {
       c.part_gk = take(c.row_splits * a->N * a->L * a->Hk * a->D * 4);
@@ -308,7 +308,7 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
 }
 
 template <typename T, int DP, int PIECES>
-int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
+int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, Peaks* peaks, int* status, cudaStream_t st) {
   const dim3 states((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits);
   typedef TcStates<DP, PIECES> S;
   const int rc = boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, peaks, status)
@@ -317,18 +317,18 @@ int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool 
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
   if (p.mask || p.lengths) {
     typedef TcRows<DP, true, PIECES> F;
-    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const float*)peaks, status);
+    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const Peaks*)peaks, status);
   }
   typedef TcRows<DP, false, PIECES> F;
-  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const float*)peaks, status);
+  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const Peaks*)peaks, status);
 }
 
 // plain: the call's own tensors, where the operands are in pieces.
 template <typename T>
-int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, float* peaks, int* status, cudaStream_t st) {
+int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, Peaks* peaks, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
-  if (c.tc && std::is_same<T, __half>::value && cudaMemsetAsync(peaks, 0, 8, st) != cudaSuccess) {
+  if (c.tc && std::is_same<T, __half>::value && cudaMemsetAsync(peaks, 0, sizeof(Peaks), st) != cudaSuccess) {
     cudaGetLastError();
     return MVR_ERR_LAUNCH;
   }
@@ -405,11 +405,11 @@ int attention_as(const mvr_attention* a, bool backward, char* workspace, int* st
       mvr_attention b;
       if ((rc = split_operands(a, backward, c, workspace, b, p, st)) != MVR_OK) return rc;
       if (!tensor_maps<__nv_bfloat16>(&b, backward, 3, maps, boxes)) return MVR_ERR_LAUNCH;
-      return backward ? attention_backward<T>(p, plain, c, maps, boxes, (float*)(workspace + c.peaks), status, st)
+      return backward ? attention_backward<T>(p, plain, c, maps, boxes, (Peaks*)(workspace + c.peaks), status, st)
                       : attention_forward<T>(p, c, maps, status, st);
     }
   }
-  return backward ? attention_backward<T>(p, p, c, maps, boxes, (float*)(workspace + c.peaks), status, st)
+  return backward ? attention_backward<T>(p, p, c, maps, boxes, (Peaks*)(workspace + c.peaks), status, st)
                   : attention_forward<T>(p, c, maps, status, st);
 }
 
