@@ -364,12 +364,23 @@ int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64
 int mvr_label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
                                 float* lse, float* top_log_prob, int32_t* top_label, int64_t batch, int64_t classes, int64_t space,
                                 int64_t batch_stride, int64_t class_stride, int top, void* stream);
+/* The same, and lse_rest: lse + lse_rest is log sum exp to the accuracy of log_prob, which far from 0 one
+ * float is not.  Both are wanted. */
+int mvr_label_log_probs_forward_rest(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob,
+                                     float* entropy, float* lse, float* lse_rest, float* top_log_prob, int32_t* top_label, int64_t batch,
+                                     int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride, int top,
+                                     void* stream);
 /* grad_logits = grad_log_prob * d log_prob + grad_entropy * d entropy (either may be null: 0), from the
- * forward's lse and entropy; written whole. */
+ * forward's lse and entropy; written whole.  Without the forward's lse_rest the scores are walked once more. */
 int mvr_label_log_probs_backward(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
                                  const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
                                  int64_t batch, int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride,
                                  int64_t grad_batch_stride, int64_t grad_class_stride, void* stream);
+int mvr_label_log_probs_backward_rest(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
+                                      const float* lse_rest, const float* entropy, const float* grad_log_prob,
+                                      const float* grad_entropy, void* grad_logits, int64_t batch, int64_t classes, int64_t space,
+                                      int64_t batch_stride, int64_t class_stride, int64_t grad_batch_stride,
+                                      int64_t grad_class_stride, void* stream);
 
 #ifdef __cplusplus
 }

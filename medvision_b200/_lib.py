@@ -72,6 +72,9 @@ PROTOTYPES = {
     "mvr_label_log_probs_forward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "mvr_label_log_probs_backward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                      _vp],
+    "mvr_label_log_probs_forward_rest": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
+    "mvr_label_log_probs_backward_rest": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                          _vp],
     "mvr_affine_2d": _ROT2D,
     "mvr_affine_3d": _ROT3D,
 }

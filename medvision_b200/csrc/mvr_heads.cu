@@ -496,38 +496,72 @@ static int check_label_log_probs(int dtype, int label_dtype, int64_t batch, int6
   return MVR_OK;
 }
 
-int mvr_label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
-                                float* lse, float* top_log_prob, int32_t* top_label, int64_t batch, int64_t classes, int64_t space,
-                                int64_t batch_stride, int64_t class_stride, int top, void* stream) {
+// rest: the entries that keep what the rounding of lse left; both are wanted then.
+static int label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
+                                   float* lse, bool rest, float* lse_rest, float* top_log_prob, int32_t* top_label, int64_t batch,
+                                   int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride, int top, void* stream) {
   const int rc = check_label_log_probs(dtype, label_dtype, batch, classes, space);
   if (rc != MVR_OK) return rc;
   if (top < 0 || top > MVR_MAX_TOP || top > classes) return MVR_ERR_TOP;
   if (batch == 0 || space == 0) return MVR_OK;
   if (!logits || !labels || !log_prob || !entropy || (top > 0 && (!top_log_prob || !top_label))) return MVR_ERR_NULL;
+  if (rest && (!lse || !lse_rest)) return MVR_ERR_NULL;
   LogProbParams p = {};
   p.x = logits; p.labels = labels; p.label_type = label_dtype;
-  p.log_prob = log_prob; p.entropy = entropy; p.lse = lse; p.top_value = top_log_prob; p.top_label = top_label;
+  p.log_prob = log_prob; p.entropy = entropy; p.lse = lse; p.lse_rest = lse_rest; p.top_value = top_log_prob; p.top_label = top_label;
   p.batch = batch; p.space = space; p.batch_stride = batch_stride; p.class_stride = class_stride;
   p.classes = (int)classes; p.top = top;
   return label_log_probs(p, dtype, true, stream);
+}
+
+static int label_log_probs_backward(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse, bool rest,
+                                    const float* lse_rest, const float* entropy, const float* grad_log_prob, const float* grad_entropy,
+                                    void* grad_logits, int64_t batch, int64_t classes, int64_t space, int64_t batch_stride,
+                                    int64_t class_stride, int64_t grad_batch_stride, int64_t grad_class_stride, void* stream) {
+  const int rc = check_label_log_probs(dtype, label_dtype, batch, classes, space);
+  if (rc != MVR_OK) return rc;
+  if (batch == 0 || space == 0) return MVR_OK;
+  if (!logits || !labels || !lse || (rest && !lse_rest) || !entropy || !grad_logits) return MVR_ERR_NULL;
+  LogProbParams p = {};
+  p.x = logits; p.labels = labels; p.label_type = label_dtype;
+  p.entropy = const_cast<float*>(entropy); p.lse = const_cast<float*>(lse); p.lse_rest = const_cast<float*>(lse_rest);
+  p.grad_log_prob = grad_log_prob; p.grad_entropy = grad_entropy; p.grad = grad_logits;
+  p.batch = batch; p.space = space; p.batch_stride = batch_stride; p.class_stride = class_stride;
+  p.grad_batch_stride = grad_batch_stride; p.grad_class_stride = grad_class_stride;
+  p.classes = (int)classes;
+  return label_log_probs(p, dtype, false, stream);
+}
+
+int mvr_label_log_probs_forward(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob, float* entropy,
+                                float* lse, float* top_log_prob, int32_t* top_label, int64_t batch, int64_t classes, int64_t space,
+                                int64_t batch_stride, int64_t class_stride, int top, void* stream) {
+  return label_log_probs_forward(logits, dtype, labels, label_dtype, log_prob, entropy, lse, false, nullptr, top_log_prob, top_label, batch,
+                                 classes, space, batch_stride, class_stride, top, stream);
+}
+
+int mvr_label_log_probs_forward_rest(const void* logits, int dtype, const void* labels, int label_dtype, float* log_prob,
+                                     float* entropy, float* lse, float* lse_rest, float* top_log_prob, int32_t* top_label, int64_t batch,
+                                     int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride, int top,
+                                     void* stream) {
+  return label_log_probs_forward(logits, dtype, labels, label_dtype, log_prob, entropy, lse, true, lse_rest, top_log_prob, top_label, batch,
+                                 classes, space, batch_stride, class_stride, top, stream);
 }
 
 int mvr_label_log_probs_backward(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
                                  const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
                                  int64_t batch, int64_t classes, int64_t space, int64_t batch_stride, int64_t class_stride,
                                  int64_t grad_batch_stride, int64_t grad_class_stride, void* stream) {
-  const int rc = check_label_log_probs(dtype, label_dtype, batch, classes, space);
-  if (rc != MVR_OK) return rc;
-  if (batch == 0 || space == 0) return MVR_OK;
-  if (!logits || !labels || !lse || !entropy || !grad_logits) return MVR_ERR_NULL;
-  LogProbParams p = {};
-  p.x = logits; p.labels = labels; p.label_type = label_dtype;
-  p.entropy = const_cast<float*>(entropy); p.lse = const_cast<float*>(lse);
-  p.grad_log_prob = grad_log_prob; p.grad_entropy = grad_entropy; p.grad = grad_logits;
-  p.batch = batch; p.space = space; p.batch_stride = batch_stride; p.class_stride = class_stride;
-  p.grad_batch_stride = grad_batch_stride; p.grad_class_stride = grad_class_stride;
-  p.classes = (int)classes;
-  return label_log_probs(p, dtype, false, stream);
+  return label_log_probs_backward(logits, dtype, labels, label_dtype, lse, false, nullptr, entropy, grad_log_prob, grad_entropy, grad_logits,
+                                  batch, classes, space, batch_stride, class_stride, grad_batch_stride, grad_class_stride, stream);
+}
+
+int mvr_label_log_probs_backward_rest(const void* logits, int dtype, const void* labels, int label_dtype, const float* lse,
+                                      const float* lse_rest, const float* entropy, const float* grad_log_prob,
+                                      const float* grad_entropy, void* grad_logits, int64_t batch, int64_t classes, int64_t space,
+                                      int64_t batch_stride, int64_t class_stride, int64_t grad_batch_stride,
+                                      int64_t grad_class_stride, void* stream) {
+  return label_log_probs_backward(logits, dtype, labels, label_dtype, lse, true, lse_rest, entropy, grad_log_prob, grad_entropy, grad_logits,
+                                  batch, classes, space, batch_stride, class_stride, grad_batch_stride, grad_class_stride, stream);
 }
 
 }  // extern "C"

@@ -10,6 +10,10 @@
 // running maximum: when it moves by d, l and u + d l are scaled by exp(d).  A position whose scores are all -inf has log_prob -inf,
 // entropy 0 and gradient 0.
 //
+// The gradient forms log p_c = (x_c - lse) - rest, where rest is what the rounding of lse to a float left: half a step of lse, which far
+// from 0 is no small change of a probability (0.02 % at 8192, 3 % at 10^6).  The forward writes both; where the caller has kept lse alone,
+// the rest is log sum exp(x - lse), one more walk over the scores.
+//
 // Two layouts: classes apart (NC[D]HW maps; a thread walks the classes of neighbouring positions, so that a warp reads
 // consecutive ones) and classes together (rows; a warp or a CTA shares a row).  Up to 16 classes apart, 1024 classes of a warp's row
 // and 65536 half (32768 float) classes of a CTA's row are read once, all loads under way together, and stay in registers.  The scores
@@ -27,7 +31,7 @@ struct LogProbParams {
   const void* x;
   const void* labels;
   int label_type;        // 0 uint8, 1 int16, 2 int32, 3 int64
-  float *log_prob, *entropy, *lse, *top_value;
+  float *log_prob, *entropy, *lse, *lse_rest, *top_value;  // lse + lse_rest: log sum exp; either may be null
   int* top_label;
   long long batch, space, batch_stride, class_stride;  // elements; positions of one batch item are consecutive
   int classes, top;
@@ -98,9 +102,20 @@ struct Online {
     l += b.l;
     u += b.u;
   }
-  __device__ __forceinline__ float lse() const { return m == -INFINITY ? m : m + log2_approx(l) * kLn2; }
+  // m + log l as its float and what that leaves of it
+  __device__ __forceinline__ float2 lse() const {
+    if (m == -INFINITY) return make_float2(m, 0.0f);
+    const float g = log2_approx(l) * kLn2, sum = m + g, of_g = sum - m;
+    return make_float2(sum, (m - (sum - of_g)) + (g - of_g));
+  }
   __device__ __forceinline__ float entropy() const { return m == -INFINITY ? 0.0f : log2_approx(l) * kLn2 - __fdividef(u, l); }
 };
+
+__device__ __forceinline__ void put_lse(const LogProbParams& p, long long i, const Online& o) {
+  const float2 lse = o.lse();
+  if (p.lse) p.lse[i] = lse.x;
+  if (p.lse_rest) p.lse_rest[i] = lse.y;
+}
 
 __device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2_approx(l) * kLn2; }
 __device__ __forceinline__ float log_prob_of(float x, const Online& o) { return log_prob_of(x, o.m, o.l); }
@@ -248,26 +263,28 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
     }
     (p.log_prob + at)[s + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
     (p.entropy + at)[s + k] = o[k].entropy();
-    if (p.lse) (p.lse + at)[s + k] = o[k].lse();
+    put_lse(p, at + s + k, o[k]);
   }
 }
 
-// What the gradient of one position needs beside its scores: g_c = -e (k + b lp), lp = x - lse, e = exp lp, k = a + b H; a more at
-// the label.
+// What the gradient of one position needs beside its scores: g_c = -e (k + b lp), lp = x - lse - rest, e = exp lp, k = a + b H; a more
+// at the label.
 struct Slope {
-  float lse, a, b, k;
+  float lse, rest, a, b, k;
   int label;
   __device__ __forceinline__ float at(float x) const {
     // (a class of probability 0 has lp = -inf: kept finite, so that e = 0 gives 0; NaN is in lse and k as well)
-    const float lp = fmaxf(x - lse, -1e30f);
+    const float lp = fmaxf((x - lse) - rest, -1e30f);
     return -exp2_approx(lp * kLog2e) * fmaf(b, lp, k);
   }
   __device__ __forceinline__ bool empty() const { return lse == -INFINITY; }
 };
+template <bool REST>
 __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
   Slope s;
   s.label = label_at(p, i);
   s.lse = p.lse[i];
+  s.rest = REST ? p.lse_rest[i] : 0.0f;
   s.a = s.label >= 0 && p.grad_log_prob ? p.grad_log_prob[i] : 0.0f;
   s.b = p.grad_entropy ? p.grad_entropy[i] : 0.0f;
   s.k = fmaf(s.b, p.entropy[i], s.a);
@@ -275,7 +292,18 @@ __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
   return s;
 }
 
-template <typename T, bool PAIR>
+// A thread's part of the sum of exp(x - lse): classes first, first + step, ... (0 where lse is -inf).
+template <typename T>
+__device__ __noinline__ float rest_part(const T* x, long long stride, int first, int step, int classes, float lse) {
+  float l = 0.0f;
+  if (lse != -INFINITY)
+    for (int c = first; c < classes; c += step) l += exp2_approx((to_float(x[c * stride]) - lse) * kLog2e);
+  return l;
+}
+__device__ __forceinline__ float rest_of(float l, float lse) { return lse == -INFINITY ? 0.0f : log2_approx(l) * kLn2; }
+
+// REST: the forward's lse_rest is there.
+template <typename T, bool PAIR, bool REST>
 __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const unsigned s = (blockIdx.x * kApartThreads + threadIdx.x) * 2;
@@ -285,7 +313,11 @@ __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __gr
   T* g = (T*)p.grad + b * p.grad_batch_stride + p.first;
   const bool second = s + 1 < (unsigned)p.positions;
   const long long at = b * p.space + p.first;
-  const Slope q[2] = {slope_at(p, at + s), slope_at(p, at + s + (second ? 1 : 0))};
+  Slope q[2] = {slope_at<REST>(p, at + s), slope_at<REST>(p, at + s + (second ? 1 : 0))};
+  if (!REST) {
+    for (int k = 0; k < 2; ++k)
+      q[k].rest = rest_of(rest_part(x + s + (second ? k : 0), p.class_stride, 0, 1, p.classes, q[k].lse), q[k].lse);
+  }
   constexpr int kStep = 8;
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
     Two<T> w[kStep];
@@ -365,7 +397,7 @@ __global__ void __launch_bounds__(128) logprob_warp_fwd(const __grid_constant__ 
   if (lane == 0) {
     p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
     p.entropy[row] = o.entropy();
-    if (p.lse) p.lse[row] = o.lse();
+    put_lse(p, row, o);
   }
   float last_v = 0.0f;
   int last_c = -1;
@@ -386,7 +418,7 @@ __global__ void __launch_bounds__(128) logprob_warp_fwd(const __grid_constant__ 
   }
 }
 
-template <typename T>
+template <typename T, bool REST>
 __global__ void __launch_bounds__(128) logprob_warp_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const int lane = threadIdx.x & 31;
@@ -394,7 +426,13 @@ __global__ void __launch_bounds__(128) logprob_warp_bwd(const __grid_constant__ 
   if (row >= p.batch) return;
   const T* x = (const T*)p.x + row * p.batch_stride;
   T* g = (T*)p.grad + row * p.grad_batch_stride;
-  const Slope q = slope_at(p, row);
+  Slope q = slope_at<REST>(p, row);
+  if (!REST) {
+    float l = rest_part(x, 1, lane, 32, p.classes, q.lse);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+    q.rest = rest_of(l, q.lse);
+  }
 #pragma unroll 4
   for (int c = lane; c < p.classes; c += 32) {
     const float v = q.at(to_float(x[c])) + (c == q.label ? q.a : 0.0f);
@@ -587,7 +625,7 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
   if (lane == 0) {
     p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
     p.entropy[row] = o.entropy();
-    if (p.lse) p.lse[row] = o.lse();
+    put_lse(p, row, o);
   }
   if (p.top == 0) return;
   const auto put = [&](int t, float v, int c) {
@@ -648,14 +686,25 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
   pick_row(r.x, r.n, p.top, p.top_value + row * p.top, p.top_label + row * p.top, o.m, o.l, sh);
 }
 
-template <typename T>
+template <typename T, bool REST>
 __global__ void __launch_bounds__(kWide, 3) logprob_row_bwd(const __grid_constant__ LogProbParams p) {
   grid_dependency();
   const int lane = threadIdx.x;
   const long long row = gridDim.x - 1 - blockIdx.x;  // backwards: the rows that the forward read last are still in L2
   const RowShape<T> r((const T*)p.x + row * p.batch_stride, p.classes);
   T* g = (T*)p.grad + row * p.grad_batch_stride;
-  const Slope q = slope_at(p, row);
+  Slope q = slope_at<REST>(p, row);
+  if (!REST) {
+    __shared__ float parts[kWide / 32];
+    float l = rest_part(r.x, 1, lane, kWide, r.n, q.lse);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+    if ((lane & 31) == 0) parts[lane >> 5] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int i = 0; i < kWide / 32; ++i) l += parts[i];
+    q.rest = rest_of(l, q.lse);
+  }
   constexpr int V = RowShape<T>::V;
   const auto one = [&](int c) {
     const float v = q.at(to_float(r.x[c])) + (c == q.label ? q.a : 0.0f);
@@ -705,7 +754,7 @@ void launch_apart_fwd(const LogProbParams& p, dim3 grid, cudaStream_t st) {
 }
 template <typename T, bool PAIR>
 void launch_logprob_apart(const LogProbParams& p, bool fwd, dim3 grid, cudaStream_t st) {
-  if (!fwd) launch_dependent(logprob_apart_bwd<T, PAIR>, grid, kApartThreads, 0, st, p);
+  if (!fwd) launch_dependent(p.lse_rest ? logprob_apart_bwd<T, PAIR, true> : logprob_apart_bwd<T, PAIR, false>, grid, kApartThreads, 0, st, p);
   else if (p.top == 0) launch_apart_fwd<T, PAIR, 0>(p, grid, st);
   else if (p.top <= 2) launch_apart_fwd<T, PAIR, 2>(p, grid, st);
   else if (p.top <= 5) launch_apart_fwd<T, PAIR, 5>(p, grid, st);
@@ -721,11 +770,11 @@ int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
     // vectors of a thread, if the row is to stay in registers (one more where it starts between two)
     const long long vecs = (p.classes / RowShape<T>::V + kWide - 1) / kWide;
     if (p.classes <= 1024) {
-      if (!fwd) launch_dependent(logprob_warp_bwd<T>, grid, 128, 0, st, p);
+      if (!fwd) launch_dependent(p.lse_rest ? logprob_warp_bwd<T, true> : logprob_warp_bwd<T, false>, grid, 128, 0, st, p);
       else if (p.classes <= 128) launch_dependent(logprob_warp_fwd<T, 4>, grid, 128, 0, st, p);
       else launch_dependent(logprob_warp_fwd<T, 32>, grid, 128, 0, st, p);
     } else if (!fwd) {
-      launch_dependent(logprob_row_bwd<T>, grid, kWide, 0, st, p);
+      launch_dependent(p.lse_rest ? logprob_row_bwd<T, true> : logprob_row_bwd<T, false>, grid, kWide, 0, st, p);
     } else if (vecs <= 2) {
       launch_dependent(logprob_row_fwd<T, 2>, grid, kWide, 0, st, p);
     } else if (vecs <= 8) {

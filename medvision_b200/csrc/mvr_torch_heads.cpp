@@ -394,7 +394,7 @@ at::Tensor scores_like(const at::Tensor& x, int64_t K, const ScoreLayout& layout
 }
 
 struct LabelLogProbsBackward : public torch::autograd::Node {
-  SavedVariable logits, labels, lse, entropy;
+  SavedVariable logits, labels, lse, entropy;  // lse: (2, ...), its float and what that leaves of it
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -420,11 +420,12 @@ struct LabelLogProbsBackward : public torch::autograd::Node {
       const int64_t K = x.size(1);
       at::Tensor gx = scores_like(x, K, in, x.scalar_type());
       const int64_t positions = in.rows ? K : gx.stride(0), classes = in.rows ? 1 : in.space;
-      check(mvr_label_log_probs_backward(data_or_null(x), head_code(x.scalar_type()), data_or_null(y),
-                                         mvr_host::label_type(y.scalar_type()), (const float*)data_or_null(l),
-                                         (const float*)data_or_null(h), (const float*)data_or_null(g[0]),
-                                         (const float*)data_or_null(g[1]), data_or_null(gx), in.batch, K, in.space, in.batch_stride,
-                                         in.class_stride, positions, classes, stream_of(x)));
+      const float* lse0 = (const float*)data_or_null(l);
+      check(mvr_label_log_probs_backward_rest(data_or_null(x), head_code(x.scalar_type()), data_or_null(y),
+                                              mvr_host::label_type(y.scalar_type()), lse0, lse0 ? lse0 + y.numel() : nullptr,
+                                              (const float*)data_or_null(h), (const float*)data_or_null(g[0]),
+                                              (const float*)data_or_null(g[1]), data_or_null(gx), in.batch, K, in.space,
+                                              in.batch_stride, in.class_stride, positions, classes, stream_of(x)));
       result[0] = gx;
     }
     once_differentiable("label_log_probs", result, {grads[0], grads[1], x0});
@@ -475,15 +476,22 @@ LabelLogProbs label_log_probs(const at::Tensor& logits, const at::Tensor& labels
     const at::TensorOptions f = logits.options().dtype(at::kFloat).requires_grad(false);
     r.log_prob = at::empty(labels.sizes(), f);
     r.entropy = at::empty(labels.sizes(), f);
-    if (graph) lse = at::empty(labels.sizes(), f);
+    if (graph) lse = at::empty({2, labels.numel()}, f);
     if (top > 0) {
       r.top_value = scores_like(x, top, in, at::kFloat);
       r.top_label = scores_like(x, top, in, at::kInt);
     }
-    check(mvr_label_log_probs_forward(data_or_null(x), head_code(x.scalar_type()), data_or_null(y), mvr_host::label_type(y.scalar_type()),
-                                      (float*)data_or_null(r.log_prob), (float*)data_or_null(r.entropy), (float*)data_or_null(lse),
-                                      (float*)data_or_null(r.top_value), (int32_t*)data_or_null(r.top_label), in.batch, K, in.space,
-                                      in.batch_stride, in.class_stride, (int)top, stream_of(x)));
+    const void *scores = data_or_null(x), *given = data_or_null(y);
+    const int type = head_code(x.scalar_type()), label_type = mvr_host::label_type(y.scalar_type());
+    float *log_prob = (float*)data_or_null(r.log_prob), *entropy = (float*)data_or_null(r.entropy),
+          *top_value = (float*)data_or_null(r.top_value);
+    int32_t* top_label = (int32_t*)data_or_null(r.top_label);
+    float* lse0 = (float*)data_or_null(lse);
+    check(graph ? mvr_label_log_probs_forward_rest(scores, type, given, label_type, log_prob, entropy, lse0,
+                                                   lse0 ? lse0 + labels.numel() : nullptr, top_value, top_label, in.batch, K, in.space,
+                                                   in.batch_stride, in.class_stride, (int)top, stream_of(x))
+                : mvr_label_log_probs_forward(scores, type, given, label_type, log_prob, entropy, nullptr, top_value, top_label, in.batch, K,
+                                              in.space, in.batch_stride, in.class_stride, (int)top, stream_of(x)));
   }
   if (graph) {
     auto node = std::shared_ptr<LabelLogProbsBackward>(new LabelLogProbsBackward(), torch::autograd::deleteNode);
