@@ -6,9 +6,10 @@
 //   dx_c = a (1[c == y] - p_c) - b p_c (log p_c + H)           a, b: gradients of log_prob (0 where no label is given) and of H
 //
 // With the maximum m, l = sum exp(x - m) and u = sum (x - m) exp(x - m), all in float: lse = m + log l, and H = log l - u / l, a
-// difference that stays small whatever the scores' offset.  Where the scores do not fit the registers they are walked once with a
-// running maximum: when it moves by d, l and u + d l are scaled by exp(d).  A position whose scores are all -inf has log_prob -inf,
-// entropy 0 and gradient 0.
+// difference that stays small whatever the scores' offset.  The logarithm is the accurate one, once a position: near certainty l = 1 + r,
+// and a loss of r is off by half a step of 1 (2^-24) and no more, where the fast one would add 1.7e-7.  Where the scores do not fit the
+// registers they are walked once with a running maximum: when it moves by d, l and u + d l are scaled by exp(d).  A position whose
+// scores are all -inf has log_prob -inf, entropy 0 and gradient 0.
 //
 // The gradient forms log p_c = (x_c - lse) - rest, where rest is what the rounding of lse to a float left: half a step of lse, which far
 // from 0 is no small change of a probability (0.02 % at 8192, 3 % at 10^6).  The forward writes both; where the caller has kept lse alone,
@@ -43,7 +44,7 @@ struct LogProbParams {
   long long grad_batch_stride, grad_class_stride;
 };
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // The label at a position; -1 where none is given (it is not one of the classes).
 __device__ __forceinline__ int label_at(const LogProbParams& p, long long i) {
@@ -61,13 +62,6 @@ __device__ __forceinline__ int label_at(const LogProbParams& p, long long i) {
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// log2 of a sum that is at least 1: off by at most 2^-22 absolutely below 2, relatively above.
-__device__ __forceinline__ float log2_approx(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -102,23 +96,22 @@ struct Online {
     l += b.l;
     u += b.u;
   }
-  // m + log l as its float and what that leaves of it
-  __device__ __forceinline__ float2 lse() const {
-    if (m == -INFINITY) return make_float2(m, 0.0f);
-    const float g = log2_approx(l) * kLn2, sum = m + g, of_g = sum - m;
-    return make_float2(sum, (m - (sum - of_g)) + (g - of_g));
-  }
-  __device__ __forceinline__ float entropy() const { return m == -INFINITY ? 0.0f : log2_approx(l) * kLn2 - __fdividef(u, l); }
 };
 
-__device__ __forceinline__ void put_lse(const LogProbParams& p, long long i, const Online& o) {
-  const float2 lse = o.lse();
-  if (p.lse) p.lse[i] = lse.x;
-  if (p.lse_rest) p.lse_rest[i] = lse.y;
-}
-
-__device__ __forceinline__ float log_prob_of(float x, float m, float l) { return m == -INFINITY ? m : (x - m) - log2_approx(l) * kLn2; }
-__device__ __forceinline__ float log_prob_of(float x, const Online& o) { return log_prob_of(x, o.m, o.l); }
+// What the sums of one position come to: its maximum and log l.
+struct Position {
+  float m, g;
+  __device__ __forceinline__ explicit Position(const Online& o) : m(o.m), g(logf(o.l)) {}
+  __device__ __forceinline__ float log_prob(float x) const { return m == -INFINITY ? m : (x - m) - g; }
+  // log_prob of the label's score, entropy, and lse = m + g as its float and what that leaves of it
+  __device__ __forceinline__ void put(const LogProbParams& p, long long i, const Online& o, int label, float given) const {
+    p.log_prob[i] = label < 0 ? 0.0f : log_prob(given);
+    p.entropy[i] = m == -INFINITY ? 0.0f : g - o.u / o.l;
+    const float sum = m + g, of_g = sum - m;
+    if (p.lse) p.lse[i] = m == -INFINITY ? m : sum;
+    if (p.lse_rest) p.lse_rest[i] = m == -INFINITY ? 0.0f : (m - (sum - of_g)) + (g - of_g);
+  }
+};
 
 // (l, u) of pairs of scores about fixed maxima.
 struct Sums2 {
@@ -141,7 +134,7 @@ __device__ __forceinline__ bool before(float a, int ia, float b, int ib) {
 // The alternatives of a position whose scores are NaN, infinite or too few for the fast way, one by one.
 template <typename T>
 __device__ __noinline__ void pick_apart(const T* x, long long stride, int classes, int top, long long space, float* value, int* label,
-                                        float m, float l) {
+                                        Position q) {
   float last_v = 0.0f;
   int last_c = -1;
   for (int t = 0; t < top; ++t) {
@@ -151,7 +144,7 @@ __device__ __noinline__ void pick_apart(const T* x, long long stride, int classe
       const float f = to_float(x[k * stride]);
       if ((t == 0 || before(last_v, last_c, f, k)) && before(f, k, v, c)) v = f, c = k;
     }
-    value[t * space] = log_prob_of(v, m, l);
+    value[t * space] = q.log_prob(v);
     label[t * space] = c;
     last_v = v, last_c = c;
   }
@@ -247,6 +240,7 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
   for (int k = 0; k < 2; ++k) {
     if (o[k].l != o[k].l) o[k].m = NAN;
     if (k == 1 && !second) break;
+    const Position q(o[k]);
     if constexpr (TOP > 0) {
       float* value = p.top_value + b * p.top * p.space + p.first;
       int* best_label = p.top_label + b * p.top * p.space + p.first;
@@ -256,14 +250,12 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
       if (all) {
 #pragma unroll
         for (int t = 0; t < TOP; ++t)
-          if (t < p.top) (value + t * p.space)[s + k] = log_prob_of(best[k].v[t], o[k]), (best_label + t * p.space)[s + k] = best[k].c[t];
+          if (t < p.top) (value + t * p.space)[s + k] = q.log_prob(best[k].v[t]), (best_label + t * p.space)[s + k] = best[k].c[t];
       } else {
-        pick_apart(items + s + k, p.class_stride, p.classes, p.top, p.space, value + s + k, best_label + s + k, o[k].m, o[k].l);
+        pick_apart(items + s + k, p.class_stride, p.classes, p.top, p.space, value + s + k, best_label + s + k, q);
       }
     }
-    (p.log_prob + at)[s + k] = label[k] < 0 ? 0.0f : log_prob_of(given[k], o[k]);
-    (p.entropy + at)[s + k] = o[k].entropy();
-    put_lse(p, at + s + k, o[k]);
+    q.put(p, at + s + k, o[k], label[k], given[k]);
   }
 }
 
@@ -300,7 +292,7 @@ __device__ __noinline__ float rest_part(const T* x, long long stride, int first,
     for (int c = first; c < classes; c += step) l += exp2_approx((to_float(x[c * stride]) - lse) * kLog2e);
   return l;
 }
-__device__ __forceinline__ float rest_of(float l, float lse) { return lse == -INFINITY ? 0.0f : log2_approx(l) * kLn2; }
+__device__ __forceinline__ float rest_of(float l, float lse) { return lse == -INFINITY ? 0.0f : logf(l); }
 
 // REST: the forward's lse_rest is there.
 template <typename T, bool PAIR, bool REST>
@@ -394,11 +386,8 @@ __global__ void __launch_bounds__(128) logprob_warp_fwd(const __grid_constant__ 
     o.l += __shfl_xor_sync(~0u, o.l, d);
     o.u += __shfl_xor_sync(~0u, o.u, d);
   }
-  if (lane == 0) {
-    p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
-    p.entropy[row] = o.entropy();
-    put_lse(p, row, o);
-  }
+  const Position q(o);
+  if (lane == 0) q.put(p, row, o, y, given);
   float last_v = 0.0f;
   int last_c = -1;
   for (int t = 0; t < p.top; ++t) {
@@ -411,7 +400,7 @@ __global__ void __launch_bounds__(128) logprob_warp_fwd(const __grid_constant__ 
     }
     best_of_warp(v, c);
     if (lane == t) {
-      p.top_value[row * p.top + t] = log_prob_of(v, o);
+      p.top_value[row * p.top + t] = q.log_prob(v);
       p.top_label[row * p.top + t] = c;
     }
     last_v = v, last_c = c;
@@ -454,7 +443,7 @@ struct RowShared {
 };
 
 template <typename T>
-__device__ __noinline__ void pick_row(const T* x, int classes, int top, float* value, int* label, float m, float l, RowShared& sh) {
+__device__ __noinline__ void pick_row(const T* x, int classes, int top, float* value, int* label, Position q, RowShared& sh) {
   const int lane = threadIdx.x, w = lane >> 5;
   float last_v = 0.0f;
   int last_c = -1;
@@ -472,7 +461,7 @@ __device__ __noinline__ void pick_row(const T* x, int classes, int top, float* v
     for (int i = 1; i < kWide / 32; ++i)
       if (before(sh.wv[i], sh.wc[i], v, c)) v = sh.wv[i], c = sh.wc[i];
     __syncthreads();
-    if (lane == 0) value[t] = log_prob_of(v, m, l), label[t] = c;
+    if (lane == 0) value[t] = q.log_prob(v), label[t] = c;
     last_v = v, last_c = c;
   }
 }
@@ -622,14 +611,11 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
       o.join(b);
     }
   }
-  if (lane == 0) {
-    p.log_prob[row] = y < 0 ? 0.0f : log_prob_of(given, o);
-    p.entropy[row] = o.entropy();
-    put_lse(p, row, o);
-  }
+  const Position q(o);
+  if (lane == 0) q.put(p, row, o, y, given);
   if (p.top == 0) return;
   const auto put = [&](int t, float v, int c) {
-    p.top_value[row * p.top + t] = log_prob_of(v, o);
+    p.top_value[row * p.top + t] = q.log_prob(v);
     p.top_label[row * p.top + t] = c;
   };
   if (o.l == o.l) {
@@ -683,7 +669,7 @@ __global__ void __launch_bounds__(kWide, NV >= 16 ? 1 : 2) logprob_row_fwd(const
       return;
     }
   }
-  pick_row(r.x, r.n, p.top, p.top_value + row * p.top, p.top_label + row * p.top, o.m, o.l, sh);
+  pick_row(r.x, r.n, p.top, p.top_value + row * p.top, p.top_label + row * p.top, q, sh);
 }
 
 template <typename T, bool REST>

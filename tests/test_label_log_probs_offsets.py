@@ -1,4 +1,4 @@
-"""ops.label_log_probs on scores far from 0, whose differences alone count.
+"""ops.label_log_probs on scores far from 0, whose differences alone count, and near certainty.
 
 Tolerances.  e = 2^-24, s_c the distance of a score from the largest.  A difference of float scores is off by half a step of itself, and a
 sum of K exponentials by 8 sqrt(K) e (six standard deviations, the functions' ulps):
@@ -103,6 +103,26 @@ def test_equal_scores_far_from_0_have_equal_probabilities(K, rows):
         # (a probability is off by 8 sqrt(K) e and its exponential, relatively; the label's by a rounding of 1)
         assert float((g[row] - want).abs().max()) <= (8 * math.sqrt(K) + 16) * E / classes + 2 * E, row
     assert not bool(g[3].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4096, 2), (1, 2, 4096), (4096, 20)])
+def test_a_loss_near_certainty(shape):
+    """log_prob = -log(1 + r), r between 2^-24 and 2^-9: the sum in float is off by half a step of 1, its logarithm by no more."""
+    rest = torch.linspace(-24, -9, 4096) * math.log(2)
+    x = torch.full(shape, -200.0)
+    if len(shape) == 2:
+        x[:, 0], x[:, 1] = 0, rest
+        y = torch.zeros(4096, dtype=torch.int64)
+    else:
+        x[0, 0], x[0, 1] = 0, rest
+        y = torch.zeros(1, 4096, dtype=torch.int64)
+    got = label_log_probs(x.cuda(), y.cuda(), 1)
+    want = torch.log_softmax(x.double(), 1)[:, 0]
+    # l = 1 + r: rounded once (2^-24); r itself off by 8 e r; the logarithm's own rounding
+    bound = 2.0 ** -24 + 16 * E * want.abs()
+    check(got.log_prob, want, bound, "log_prob")
+    check(got.top_log_prob[:, 0], want, bound, "top")
 
 
 @pytest.mark.gpu
