@@ -6,8 +6,11 @@
 //
 //   S = Q K^T (128 x 64 or 128, tensor memory)  ->  P = 2^(S scale - m), rounded to T, over S  ->  O += P V (tensor memory)
 //
-// The maximum that P is formed about is only moved when it grows by more than 2^8 (P stays far below what T holds, and the sum is
-// formed of the same P): then O, in tensor memory, is scaled first.  One CTA's chain of products, exponentials and products leaves
+// The maximum that P is formed about is only moved when it grows by more than 2^8, in float16 2^4: then O, in tensor memory, is scaled
+// first.  float16 has few small numbers, so there P is 2^11 times as large: up to 2^15, and a weight is off by at most 2^-36 of the
+// largest beside its relative rounding, which 2^21 states, the most of a call, bring to 2^-15.  (About 1 itself a weight below 2^-25
+// would be 0, and 2^18 of them a percent of the result.)  The sum is formed of P before it is rounded; the factor is in both and
+// goes out with the normaliser.  One CTA's chain of products, exponentials and products leaves
 // every unit idle for a part of it.  Up to 64 columns of a head four CTAs share an SM, each with a tile of rows and 64 states at a
 // time.  Beyond, two row tiles of one CTA alternate, which read every tile of states once for both, or, where rows are few, two CTAs
 // with a tile each.  Few rows: the states are cut into parts as well (attn_join).
@@ -29,6 +32,10 @@
 namespace mvr {
 
 constexpr int kPolynomials = 2;  // of eight pairs of exponentials, how many are polynomials (halves: their error is below the rounding)
+
+// P of the largest score (as a power of two), and how much further one may rise before the maximum is moved.
+template <typename T> constexpr float kWeightShift = TcType<T>::code == 0 ? 11.0f : 0.0f;
+template <typename T> constexpr float kLazy = TcType<T>::code == 0 ? 4.0f : 8.0f;
 
 constexpr int kTcRows = 128, kTcBox = 64;   // rows of a tile; states of a TMA box
 constexpr int kTcMaxStates = 32768;         // states that one CTA can list
@@ -369,6 +376,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // (not 0: a score that is left out is -inf)
       float m = -INFINITY, l = 0.0f;  // m: in the units of S, the same in both halves; l: of this half
+      const auto reference = [&](float m) { return m == -INFINITY ? 0.0f : fmaf(m, scale, -kWeightShift<T>); };  // P = 2^(S scale - this)
       // With pieces, O of each tile is added up in registers: the tensor cores' additions cut off what they do not hold, which over a
       // hundred tiles comes to some 4e-6, five times the error of float sums.
       float acc[PIECES == 1 ? 1 : 64] = {};
@@ -441,7 +449,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         }
         if (top == INFINITY) top = NAN;  // (as inf - inf is; the sums are NaN from here on)
         // move the maximum?  (the first tile: there is no O yet)
-        const bool move = !(top <= m) && (m == -INFINITY || !((top - m) * scale <= 8.0f));  // (NaN moves it)
+        const bool move = !(top <= m) && (m == -INFINITY || !((top - m) * scale <= kLazy<T>));  // (NaN moves it)
         if (__any_sync(~0u, move)) {
           const float shrink = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - top) * scale)) : 1.0f;
           if (move) m = top;
@@ -461,7 +469,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.0f : m * scale;
+        const float ref = reference(m);
         const float2 scale2 = make_float2(scale, scale), minus = make_float2(-ref, -ref);
         float2 sums[2] = {};
 #pragma unroll
@@ -512,10 +520,10 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (mine && !half) {
           if (p.splits > 1) {
-            p.part_ml[(split * rows + row) * 2] = m == -INFINITY ? m : m * scale;
+            p.part_ml[(split * rows + row) * 2] = m == -INFINITY ? m : reference(m);
             p.part_ml[(split * rows + row) * 2 + 1] = l;
           } else if (p.lse) {
-            p.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? 0.0f : m * scale) + log2f(l);
+            p.lse[row] = l == 0.0f ? -INFINITY : reference(m) + log2f(l);
           }
         }
         const auto put = [&](int q, uint32_t (&v)[32]) {
