@@ -33,6 +33,8 @@ struct AttnParams {
   void *out, *gq, *gk, *gv;                      // out, gq: (R, T, Hq, D); gk, gv: (N, L, Hk, D); all contiguous
   const void* o;                                 // the forward's output (backward)
   float *lse, *delta;                            // (R, T, Hq); lse in powers of two: log2 of the sum of 2^(s log2 e)
+  float* norm;                                   // (R, T, Hq): |g| (float16 gradients)
+  int* peaks;                                    // (N, Hk): largest |v| of the states that are read, float bits (float16 gradients)
   long long q_r, q_t, q_h, g_r, g_t, g_h;        // strides in elements; the last dimension is contiguous
   long long k_n, k_l, k_h, v_n, v_l, v_h;
   const int *order, *starts, *tiles;             // grouping by image, or null: region r reads image r

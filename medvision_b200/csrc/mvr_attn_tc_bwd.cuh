@@ -18,10 +18,11 @@
 // rest.  One exponential per score in each kernel is the price of
 // sums without atomics.
 //
-// float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that keeps |dS| <= |g.v| + |delta| below
-// 2^15.  Where states are kept that is D max|g| max|v| + max|delta|, max|v| over those states: delta averages the values of all
-// states, so that it has to be counted by itself (attn_tc_delta finds it).  Where rows are kept, 2 D max|g| max|v| with max|v| over all
-// that the first kernel saw.  Both powers are taken out of the sums again, exactly.
+// float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that brings a bound of |dS| <= |g.v| +
+// |delta| to 2^14.  Where rows are kept every row has its own, from |g| of the row (2-norms, by attn_tc_delta) and the largest |v| of the
+// states of its image and key head (by the first kernel).  Where states are kept it is one power a CTA, from the largest |v| of its 128 states
+// and the largest |g| and |delta| of the rows that it walks: delta averages the values of all states and has to be counted by itself.  So
+// no gradient depends, in its bits or its range, on rows that have nothing to do with it.  Both are taken out of the sums again, exactly.
 #pragma once
 #include <type_traits>
 
@@ -34,16 +35,13 @@ constexpr int kGradStep = DP == 64 ? 64 : 128;  // columns of a tile
 
 __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
-// What a call's largest |g|, |v| and |delta| are kept in (float bits).
-struct Peaks {
-  float g, v, delta;
-};
+__device__ __forceinline__ float finite_or_0(float x) { return x <= 3e38f ? x : 0.0f; }  // x >= 0, or NaN
 
-// Power of two for dS, from a bound of |dS|.
+// Power of two for dS, from a bound of |dS| (1 where that is 0 or not finite).
 template <typename T>
 __device__ __forceinline__ float slope_scale(float most) {
   if constexpr (TcType<T>::code == 1) return 1.0f;
-  if (!(most > 0.0f) || most > 3e38f) return 1.0f;
+  if (!(most > 0.0f && most <= 3e38f)) return 1.0f;
   const int e = 14 - ilogbf(most);
   return ldexpf(1.0f, e < -60 ? -60 : e > 60 ? 60 : e);
 }
@@ -83,7 +81,7 @@ struct TcStates {
   struct Control {
     unsigned long long states, full[kStages], empty[kStages], scores, slopes, weights, grads, done;
     uint32_t tmem;
-    int lost, peak;
+    int lost, peak[3];  // peak: largest |v|, |g|, |delta| (float bits)
     alignas(16) float lse[kStages][kStep];    // negative
     alignas(16) float delta[kStages][kStep];  // negative
   };
@@ -97,7 +95,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 // BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
 template <typename T, int DP, bool BOXES, int PIECES>
 __global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, PIECES>::kResident)
-attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, Peaks* peaks, int* status) {
+attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcStates<DP, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
@@ -117,7 +115,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     bar_init(smem_at(&c.grads), F::kGroups / 32);
     bar_init(smem_at(&c.done), 1);
     c.lost = 0;
-    c.peak = 0;
+    c.peak[0] = c.peak[1] = c.peak[2] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -320,29 +318,37 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float factor = 1.0f;  // of dS
     if (count > 0 && TcType<T>::code == 0) {
+      float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of some of the rows (what is not finite bounds nothing)
+      const int last = min(o.rows, (first + count) * F::kStep);
+#pragma unroll 4
+      for (int at = first * F::kStep + threadIdx.x; at < last; at += F::kGroups) {
+        const long long number = row_number(p, row_of(p, o, at, hk));
+        most[1] = fmaxf(most[1], finite_or_0(p.norm[number]));
+        most[2] = fmaxf(most[2], finite_or_0(fabsf(p.delta[number])));
+      }
       bar_pass(smem_at(&c.states), 0, lost);
-      // largest |v| of the states that are read
-      float most = 0.0f;
-      if (in) {
+      if (in && part_of == 0) {
         const char* row = base + F::kTileBytes + r * 128;
 #pragma unroll
-        for (int e = 0; e < DP * 16 / F::kGroups; ++e) {
-          const int piece = part_of * (DP * 16 / F::kGroups) + e;
+        for (int piece = 0; piece < DP / 8; ++piece) {
           const uint4 v = *(const uint4*)(row + (piece >> 3) * 16384 + (((piece ^ r) & 7) << 4));
           const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 f = __half22float2(*(const __half2*)&words[k]);
-            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+            most[0] = fmaf(f.x, f.x, fmaf(f.y, f.y, most[0]));
           }
         }
+        most[0] = finite_or_0(sqrtf(most[0]));
       }
-      for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-      if (lane == 0) atomicMax(&c.peak, __float_as_int(most));
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        for (int d = 16; d; d >>= 1) most[k] = fmaxf(most[k], __shfl_xor_sync(~0u, most[k], d));
+        if (lane == 0) atomicMax(&c.peak[k], __float_as_int(most[k]));
+      }
       group_sync(F::kGroups);
-      const float peak = __int_as_float(c.peak);
-      if (threadIdx.x == 0) atomicMax((int*)&peaks->v, c.peak);
-      factor = slope_scale<T>(p.D * peaks->g * peak + peaks->delta);
+      if (threadIdx.x == 0) atomicMax(p.peaks + (long long)n * p.Hk + hk, c.peak[0]);
+      factor = slope_scale<T>(__int_as_float(c.peak[1]) * __int_as_float(c.peak[0]) + __int_as_float(c.peak[2]));
     }
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
     // With pieces, each tile's sums are added up in registers (dv in the first warpgroup, dk in the second): see the forward.
@@ -499,7 +505,7 @@ struct TcRows {
 
 template <typename T, int DP, bool MASK, int PIECES>
 __global__ void __launch_bounds__(TcRows<DP, MASK, PIECES>::kThreads, TcRows<DP, MASK, PIECES>::kResident)
-attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, const Peaks* peaks, int* status) {
+attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcRows<DP, MASK, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
@@ -640,7 +646,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     const bool mine = some && j0 < o.rows;
     Row w = {};
     long long number = 0;
-    float lse = INFINITY, delta = 0.0f;
+    float lse = INFINITY, delta = 0.0f, factor = 1.0f;  // factor: of dS
     if (mine) {
       w = row_of(p, o, j0, hk);
       number = row_number(p, w);
@@ -648,6 +654,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         lse = p.lse[number];
         if (lse == -INFINITY) lse = INFINITY;
         delta = p.delta[number];
+        if (TcType<T>::code == 0) factor = slope_scale<T>(p.norm[number] * __int_as_float(p.peaks[(long long)o.n * p.Hk + hk]) + fabsf(delta));
       }
     }
     if (tiles > 0) {
@@ -664,7 +671,6 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       fence_async_proxy();
       bar_arrive_warp(smem_at(&c.rows));
     }
-    const float factor = tiles > 0 && TcType<T>::code == 0 ? slope_scale<T>(2.0f * p.D * peaks->g * peaks->v) : 1.0f;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-lse, -lse), less = make_float2(-delta, -delta);
     // With pieces, each tile's sums are added up in registers (half the columns a warpgroup): see the forward.
     float acc[PIECES == 1 ? 1 : 32] = {};
@@ -769,20 +775,16 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   }
 }
 
-// delta = g.o per row, and the largest finite |g| and |delta|.
+// delta = g.o per row, and for float16 |g| (2-norm).  16 lanes a row at most.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p, Peaks* peaks) {
+__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p) {
   grid_dependency();
-  __shared__ int peak[2];
-  if (threadIdx.x < 2) peak[threadIdx.x] = 0;
-  __syncthreads();
   const long long rows = (long long)p.R * p.T * p.Hq;
   const int lane = threadIdx.x & 31, per = p.D / 8;  // a lane takes 8 elements of a row; 32 / width rows a warp
   const int width = per <= 4 ? 4 : per <= 8 ? 8 : 16, sub = lane / width, piece = lane % width;
-  float most = 0.0f, most_delta = 0.0f;
   for (long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / width); first < rows; first += (long long)gridDim.x * 8 * (32 / width)) {
     const long long row = first + sub;
-    float v = 0.0f;
+    float v = 0.0f, square = 0.0f;
     if (row < rows && piece < per) {
       const int h = (int)(row % p.Hq);
       const long long rt = row / p.Hq, r = rt / p.T, t = rt - r * p.T;
@@ -792,26 +794,16 @@ __global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ Att
       for (int e = 0; e < 8; ++e) {
         const float a = to_float(g.v[e]);
         v += a * to_float(o.v[e]);
-        if (fabsf(a) <= 3e38f) most = fmaxf(most, fabsf(a));
+        if (TcType<T>::code == 0) square += a * a;
       }
     }
-    for (int d = width / 2; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-    if (fabsf(v) <= 3e38f) most_delta = fmaxf(most_delta, fabsf(v));
-    if (row < rows && piece == 0) p.delta[row] = v;
-  }
-  if constexpr (TcType<T>::code == 0) {
-    for (int d = 16; d; d >>= 1) {
-      most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-      most_delta = fmaxf(most_delta, __shfl_xor_sync(~0u, most_delta, d));
+    for (int d = width / 2; d; d >>= 1) {
+      v += __shfl_xor_sync(~0u, v, d);
+      if (TcType<T>::code == 0) square += __shfl_xor_sync(~0u, square, d);
     }
-    if (lane == 0) {
-      atomicMax(&peak[0], __float_as_int(most));
-      atomicMax(&peak[1], __float_as_int(most_delta));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      atomicMax((int*)&peaks->g, peak[0]);
-      atomicMax((int*)&peaks->delta, peak[1]);
+    if (row < rows && piece == 0) {
+      p.delta[row] = v;
+      if (TcType<T>::code == 0) p.norm[row] = sqrtf(square);
     }
   }
 }

@@ -36,7 +36,7 @@ struct AttnCut {
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
-  long long order, starts, tiles, delta, peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+  long long order, starts, tiles, delta, norm, peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
@@ -106,7 +106,10 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   }
   if (backward) {
     c.delta = take(rows * 4);
-    c.peaks = take(sizeof(Peaks));
+    if (tc && a->dtype == MVR_F16) {
+      c.norm = take(rows * 4);
+      c.peaks = take(a->N * a->Hk * 4);
+    }
     if (c.splits > 1) c.part_gq = take(c.splits * rows * a->D * 4);
     if (c.row_splits > 1) {
       c.part_gk = take(c.row_splits * a->N * a->L * a->Hk * a->D * 4);
@@ -187,7 +190,7 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   p.scale = a->scale;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.splits = c.splits; p.row_splits = c.row_splits;
-  p.delta = (float*)(ws + c.delta);
+  p.delta = (float*)(ws + c.delta); p.norm = (float*)(ws + c.norm); p.peaks = (int*)(ws + c.peaks);
   p.part_o = (float*)(ws + c.part_o); p.part_ml = (float*)(ws + c.part_ml);
   p.part_gq = (float*)(ws + c.part_gq); p.part_gk = (float*)(ws + c.part_gk); p.part_gv = (float*)(ws + c.part_gv);
   return p;
@@ -308,27 +311,27 @@ int attention_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps,
 }
 
 template <typename T, int DP, int PIECES>
-int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, Peaks* peaks, int* status, cudaStream_t st) {
+int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool boxes, int* status, cudaStream_t st) {
   const dim3 states((unsigned)(cdiv(p.L, 128) * p.N), p.Hk, c.row_splits);
   typedef TcStates<DP, PIECES> S;
-  const int rc = boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, peaks, status)
-                       : launch_shared<attn_tc_dkv<T, DP, false, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, peaks, status);
+  const int rc = boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, status)
+                       : launch_shared<attn_tc_dkv<T, DP, false, PIECES>>(states, S::kThreads, S::kShared, st, p, maps, status);
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
   if (p.mask || p.lengths) {
     typedef TcRows<DP, true, PIECES> F;
-    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const Peaks*)peaks, status);
+    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
   }
   typedef TcRows<DP, false, PIECES> F;
-  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, (const Peaks*)peaks, status);
+  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
 }
 
 // plain: the call's own tensors, where the operands are in pieces.
 template <typename T>
-int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, Peaks* peaks, int* status, cudaStream_t st) {
+int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnCut& c, const TcMaps& maps, bool boxes, int* status, cudaStream_t st) {
   const long long rows = (long long)p.R * p.T * p.Hq, states = (long long)p.N * p.L * p.Hk * p.D;
   int rc = MVR_OK;
-  if (c.tc && std::is_same<T, __half>::value && cudaMemsetAsync(peaks, 0, sizeof(Peaks), st) != cudaSuccess) {
+  if (c.tc && std::is_same<T, __half>::value && cudaMemsetAsync(p.peaks, 0, (size_t)p.N * p.Hk * 4, st) != cudaSuccess) {
     cudaGetLastError();
     return MVR_ERR_LAUNCH;
   }
@@ -336,16 +339,16 @@ int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnC
     bool done = false;
     if constexpr (sizeof(T) == 2) {
       done = c.tc;
-      if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)std::min<long long>(cdiv(rows, 16), 8 * kMultiprocessors)), dim3(256), 0, st, p, peaks);
+      if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)std::min<long long>(cdiv(rows, 16), 8 * kMultiprocessors)), dim3(256), 0, st, p);
     }
     if (!done) launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, plain);
     if ((rc = launched()) != MVR_OK) return rc;
   }
   if (c.tc) {
     if constexpr (sizeof(T) == 2)
-      rc = p.D <= 64 ? tc_backward<T, 64, 1>(p, c, maps, boxes, peaks, status, st) : tc_backward<T, 128, 1>(p, c, maps, boxes, peaks, status, st);
+      rc = p.D <= 64 ? tc_backward<T, 64, 1>(p, c, maps, boxes, status, st) : tc_backward<T, 128, 1>(p, c, maps, boxes, status, st);
     else
-      rc = tc_backward<__nv_bfloat16, 64, 3>(p, c, maps, boxes, peaks, status, st);
+      rc = tc_backward<__nv_bfloat16, 64, 3>(p, c, maps, boxes, status, st);
   }
   if (!c.tc)
     rc = p.D <= 32 ? fma_backward<T, 32>(p, c, st) : p.D <= 64 ? fma_backward<T, 64>(p, c, st)
@@ -405,11 +408,11 @@ int attention_as(const mvr_attention* a, bool backward, char* workspace, int* st
       mvr_attention b;
       if ((rc = split_operands(a, backward, c, workspace, b, p, st)) != MVR_OK) return rc;
       if (!tensor_maps<__nv_bfloat16>(&b, backward, 3, maps, boxes)) return MVR_ERR_LAUNCH;
-      return backward ? attention_backward<T>(p, plain, c, maps, boxes, (Peaks*)(workspace + c.peaks), status, st)
+      return backward ? attention_backward<T>(p, plain, c, maps, boxes, status, st)
                       : attention_forward<T>(p, c, maps, status, st);
     }
   }
-  return backward ? attention_backward<T>(p, p, c, maps, boxes, (Peaks*)(workspace + c.peaks), status, st)
+  return backward ? attention_backward<T>(p, p, c, maps, boxes, status, st)
                   : attention_forward<T>(p, c, maps, status, st);
 }
 

@@ -2,7 +2,8 @@
 
 Tolerances are those of test_cross_attention, and for what float16 rounds on its way into a product:
   slopes   dS is rounded after a power of two that brings a bound B of |dS| to at least 2^14; a half's smallest step there is 2^-24, so
-           an element is off by at most 2^-25 2^-14 B = 2^-39 B beside its relative rounding.  B: 2 D max|g| max|v|.
+           an element is off by at most 2^-25 2^-14 B = 2^-39 B beside its relative rounding.  B: |g| times the largest |v| (2-norms) plus
+           |delta|, of the row (dq) or the largest of the rows that read the state (dk).
   weights  the largest is at least 2^11 before it is rounded: an element is off by at most 2^-25 2^-11 = 2^-36 of the largest, and 2^21
            states, the most that a call takes, by at most 2^-15 of it together, whatever their number.
 """
@@ -17,15 +18,23 @@ from test_cross_attention import E, HALF, NAMES, check, make, reference, run
 
 
 def slopes(q, k, v, g, image, allowed, scale):
-    """What 2^-39 B per element of dS comes to in dq and dk, with B of the whole call."""
+    """What 2^-39 B per element of dS comes to in dq (B of the row) and dk (B of all rows of the state's image and key head)."""
     q, k, v, g = (t.double() for t in (q, k, v, g))
-    H, Hk, D = q.shape[2], k.shape[2], q.shape[3]
+    H, Hk = q.shape[2], k.shape[2]
     dq, dk = torch.zeros_like(q), torch.zeros_like(k)
-    most = 2 * D * float(g.abs().max()) * float(v[allowed].abs().max())
+    largest = torch.zeros(2, k.shape[0], Hk, dtype=torch.float64)  # of |g||v| and of |delta|
+    rows = []
     for r, n in enumerate(image):
-        for h in range(H if 0 <= n < k.shape[0] else 0):
-            dq[r, :, h] = abs(scale) * 2.0 ** -39 * most * k[n, allowed[n], h * Hk // H].abs().sum(0)
-            dk[n, allowed[n], h * Hk // H] += abs(scale) * 2.0 ** -39 * most * q[r, :, h].abs().sum(0)
+        for h in range(H if 0 <= n < k.shape[0] and bool(allowed[n].any()) else 0):
+            kh = h * Hk // H
+            a, b = k[n, allowed[n], kh], v[n, allowed[n], kh]
+            delta = (g[r, :, h] * (torch.softmax(scale * q[r, :, h] @ a.T, 1) @ b)).sum(1).abs()
+            gv = g[r, :, h].norm(dim=1) * b.norm(dim=1).max()
+            dq[r, :, h] = abs(scale) * 2.0 ** -39 * (gv + delta)[:, None] * a.abs().sum(0)
+            largest[:, n, kh] = torch.maximum(largest[:, n, kh], torch.stack([gv.max(), delta.max()]))
+            rows.append((r, n, h, kh))
+    for r, n, h, kh in rows:
+        dk[n, allowed[n], kh] += abs(scale) * 2.0 ** -39 * largest[:, n, kh].sum() * q[r, :, h].abs().sum(0)
     return dq, dk
 
 
@@ -53,6 +62,34 @@ def test_half_gradients_where_values_of_some_states_are_small_or_zero(dim, index
     for name, a, b, c in zip(NAMES, run(q, k, v, g, **kw), res, bound):
         check(a, b, c, name)
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_half_gradients_of_quiet_rows_beside_loud_ones(dim, tokens):
+    """Gradients that differ by 2^17 between regions: those of the quiet ones keep their bits, and do not depend on the others."""
+    R, H, Hk, N, L = 6, 4, 2, 3, 500
+    q, k, v, g = make(R, tokens, H, Hk, dim, N, L, torch.float32, seed=22)
+    image = [0, 1, 1, -1, 2, 2]
+    size = torch.tensor([2.0 ** 11, 2.0 ** -6, 2.0 ** -6, 2.0 ** 13, 2.0 ** 11, 2.0 ** -6])
+    g = g * size.view(R, 1, 1, 1)
+    q, k, v, g = (t.half() for t in (q, k, v, g))
+    allowed = torch.ones(N, L, dtype=torch.bool)
+    index = torch.tensor(image).cuda()
+    res, bound = reference(q, k, v, g, image, allowed, dim ** -0.5, torch.float16)
+    more = slopes(q, k, v, g, image, allowed, dim ** -0.5)
+    bound[1] += more[0]
+    bound[2] += more[1]
+    got = run(q, k, v, g, batch_index=index)
+    for name, a, b, c in zip(NAMES, got, res, bound):
+        check(a, b, c, name)
+    quiet = g.clone()
+    quiet[size > 1] = 0
+    alone = run(q, k, v, quiet, batch_index=index)
+    assert torch.equal(got[1][size < 1], alone[1][size < 1])            # dq of the quiet regions
+    assert torch.equal(got[2][1], alone[2][1]) and torch.equal(got[3][1], alone[3][1])  # dk, dv of an image that only they read
+    assert not bool(got[1][3].any())
 
 
 @pytest.mark.gpu
