@@ -296,7 +296,9 @@ __device__ __forceinline__ void pieces_of(float2 f, uint32_t& a, uint32_t& b, ui
 }
 
 // Rows of D floats (three outer dimensions with strides) as pieces: to[piece][row][W], W: D rounded up to 8, zeros behind D.  A thread
-// takes eight columns.  An infinity is its first piece, the others 0.
+// takes eight columns.  An infinity is the largest bfloat16 of its sign, 0 and the infinity: the third piece meets nothing but the other
+// operand's first, so that no 0 among that one's smaller pieces makes a NaN of an infinite product, and the first piece gives infinity
+// times infinity.  NaN is the third piece alone.
 __global__ void __launch_bounds__(256) split_floats(const float* from, long long s0, long long s1, long long s2, int n1, int n2, long long rows,
                                                     int D, int W, __nv_bfloat16* to) {
   grid_dependency();
@@ -315,8 +317,11 @@ __global__ void __launch_bounds__(256) split_floats(const float* from, long long
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       if (!(fabsf(f[2 * k + h]) < INFINITY)) {  // (infinity less itself is no number)
-        w[1][k] &= h ? 0xffffu : 0xffff0000u;
-        w[2][k] &= h ? 0xffffu : 0xffff0000u;
+        const uint32_t sign = (__float_as_uint(f[2 * k + h]) >> 16) & 0x8000, keep = h ? 0xffffu : 0xffff0000u;
+        const bool nan = f[2 * k + h] != f[2 * k + h];
+        w[0][k] = (w[0][k] & keep) | ((nan ? 0u : sign | 0x7f7f) << (16 * h));
+        w[1][k] &= keep;
+        w[2][k] = (w[2][k] & keep) | ((nan ? 0x7fffu : sign | 0x7f80) << (16 * h));
       }
   }
 #pragma unroll

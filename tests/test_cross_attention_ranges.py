@@ -1,4 +1,5 @@
-"""ops.cross_attention where operands of one call differ in size by many powers of two: float16 has few bits for small numbers.
+"""ops.cross_attention where operands of one call differ in size by many powers of two, where float16 has few bits for small
+numbers, and where float32 operands are infinite, which the tensor cores take in pieces.
 
 Tolerances are those of test_cross_attention, and for what float16 rounds on its way into a product:
   slopes   dS is rounded after a power of two that brings a bound B of |dS| to at least 2^14; a half's smallest step there is 2^-24, so
@@ -124,3 +125,54 @@ def test_half_weights_of_many_states_far_below_the_largest(dim, states, masked):
     bound = (2 * w + HALF[torch.float16]) * want + 2.0 ** -15 + 2.0 ** -25
     assert float(want.min()) > 3 * 2.0 ** -15  # (0 in its place would not pass)
     check(out, want, bound, "out")
+
+
+def _float_bits(pattern):
+    return torch.tensor([pattern], dtype=torch.int32).view(torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,states", [(3, 40), (70, 8192)])  # float arithmetic, and pieces on the tensor cores
+@pytest.mark.parametrize("dim", [20, 64])
+def test_infinite_float_operands(tokens, states, dim):
+    """An infinite value makes its column infinite; a key whose product with the query is -inf has no weight; NaN stays."""
+    H, inf = 2, float("inf")
+    q, k, v, g = make(1, tokens, H, H, dim, 1, states, torch.float32, seed=24)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    allowed = torch.ones(1, states, dtype=torch.bool)
+    res, bound = reference(q, k, v, g, [0], allowed, dim ** -0.5, torch.float32)
+    dirty = v.clone()
+    dirty[0, 5, 0, 3], dirty[0, 9, 1, 4], dirty[0, 7, 1, 6], dirty[0, 11, 1, 6] = inf, -inf, inf, -inf
+    dirty[0, 12, 0, 8] = _float_bits(0x7f800001)                            # NaN whose upper half alone reads as infinity
+    with torch.no_grad():
+        out = cross_attention(q.cuda(), k.cuda(), dirty.cuda()).cpu()
+    assert bool((out[..., 0, 3] == inf).all()) and bool((out[..., 1, 4] == -inf).all())
+    assert bool(out[..., 1, 6].isnan().all()) and bool(out[..., 0, 8].isnan().all())
+    special = torch.zeros(H, dim, dtype=torch.bool)
+    for place in ((0, 3), (1, 4), (1, 6), (0, 8)):
+        special[place] = True
+    check(torch.where(special, res[0].float(), out), res[0], bound[0], "out")
+    # keys that are infinitely far: as if they were left out
+    dirty, gone = k.clone(), torch.zeros(1, states, dtype=torch.bool)
+    gone[0, [0, 17, 33]] = True
+    dirty[0, [0, 17, 33], :, 0] = -inf
+    with torch.no_grad():
+        out = cross_attention(q.cuda(), dirty.cuda(), v.cuda())
+    res, bound = reference(q, k, v, g, [0], ~gone, dim ** -0.5, torch.float32)
+    check(out, res[0], bound[0], "out")
+    # an infinite query has no softmax; the other rows do not see it
+    dirty = q.clone()
+    dirty[0, 1, 0, 2] = inf
+    with torch.no_grad():
+        out = cross_attention(dirty.cuda(), k.cuda(), v.cuda()).cpu()
+    res, bound = reference(q, k, v, g, [0], allowed, dim ** -0.5, torch.float32)
+    assert bool(out[0, 1, 0].isnan().all())
+    out[0, 1, 0] = res[0][0, 1, 0].float()
+    check(out, res[0], bound[0], "out")
+    # an infinite gradient reaches the values' gradients as it is
+    dirty = g.clone()
+    dirty[0, 2, 1, 7] = -inf
+    dv = run(q, k, v, dirty)[3].cpu()
+    assert bool((dv[0, :, 1, 7] == -inf).all())
+    dv[0, :, 1, 7] = res[3][0, :, 1, 7].float()
+    check(dv, res[3], bound[3], "dv")
