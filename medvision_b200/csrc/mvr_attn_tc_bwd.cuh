@@ -251,7 +251,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const uint32_t to_block = smem_at(base + 2 * PIECES * F::kTileBytes) + (piece >> 3) * (F::kStep * 128);
     look_up(0);
     bool pending = false;
-    for (int i = 0; i < count; ++i) {
+    int i = 0;
+    for (; i < count; ++i) {
       const int stage = i % F::kStages;
       if (i >= F::kStages && !bar_wait_warp(smem_at(&c.empty[stage]), (i / F::kStages - 1) & 1, lost)) break;
 #pragma unroll
@@ -311,8 +312,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (BOXES && *lost && warp == kLoader) {  // given up: the copies under way end, or the limit passes, before the CTA does
       const unsigned long long t = nanoseconds();
-      for (int k = 0; k < F::kStages; ++k)
-        while (!bar_try(smem_at(&c.full[k]), 0) && !bar_try(smem_at(&c.full[k]), 1) && nanoseconds() - t < kWaitLimit) {}
+      for (int k = max(0, i - F::kStages); k < i; ++k)
+        while (!bar_try(smem_at(&c.full[k % F::kStages]), (k / F::kStages) & 1) && nanoseconds() - t < kWaitLimit) {}
     }
   } else {
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
