@@ -468,6 +468,7 @@ int mvr_dropout(const void* x, const void* residual, void* out, int dtype, int64
   const int cut = (int)std::floor(probability * 65536.0 + 0.5);  // an element stays when its 16 bits are >= cut
   const cudaStream_t st = (cudaStream_t)stream;
   if (cut == 65536) {  // none does
+    if (residual == out) return MVR_OK;
     const size_t bytes = (size_t)n * (dtype == MVR_F32 ? 4 : 2);
     const cudaError_t e = residual ? cudaMemcpyAsync(out, residual, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(out, 0, bytes, st);
     if (e != cudaSuccess) cudaGetLastError();
