@@ -20,12 +20,22 @@ def dropout(x, p=0.5, seed=None, offset=0, residual=None, training=True):
             captured graph a replay repeats the mask drawn while it was captured)
         offset (int): 64 bits; calls that share a seed (the layers of a step) take different ones
         residual (Tensor): added to the result in the same pass; of x's shape and type
-        training (bool): False gives x, or x + residual
+        training (bool): False gives x, or x + residual, of the same shapes and types (on the CPU as well)
 
     Differentiable in x and residual.  A dropped element gives 0 whatever it holds.
     """
     if not training:
-        return x if residual is None else x + residual
+        if residual is None:
+            return x
+        if not isinstance(residual, torch.Tensor):
+            raise TypeError(f"residual must be a Tensor, not {type(residual).__name__}")
+        if residual.device != x.device:
+            raise RuntimeError("expected all tensors to be on the same CUDA device")
+        if residual.dtype != x.dtype:
+            raise RuntimeError(f"expected scalar type {x.dtype} but found {residual.dtype}")
+        if residual.shape != x.shape:
+            raise RuntimeError("dropout: x and residual must have the same shape")
+        return x + residual
     if seed is None:
         seed = int(torch.randint(2 ** 63 - 1, ()))
     return _C._native.dropout(x, p, seed, offset, residual)

@@ -1,11 +1,28 @@
-"""ops.dropout: results that lie over x or over the residual."""
+"""ops.dropout: evaluation takes the residuals that training takes; results that lie over x or over the residual."""
 import ctypes
 
 import pytest
 import torch
 
 from medvision_b200 import _lib
-from medvision_b200.ops import dropout
+from medvision_b200.ops import Dropout, dropout
+
+
+def test_evaluation_refuses_the_residuals_that_training_refuses():
+    x = torch.zeros(4, 3)
+    layer = Dropout(0.5).eval()
+    for residual, words in ((torch.zeros(3), "same shape"), (torch.zeros(4, 1), "same shape"), (torch.zeros(2, 4, 3), "same shape"),
+                            (torch.zeros(4, 3).half(), "expected scalar type torch.float32 but found torch.float16"),
+                            (torch.zeros(4, 3).double(), "expected scalar type torch.float32 but found torch.float64"),
+                            (torch.zeros(4, 3, device="meta"), "same CUDA device")):
+        for call in (lambda: dropout(x, 0.5, 1, residual=residual), lambda: dropout(x, 0.5, training=False, residual=residual),
+                     lambda: layer(x, residual)):
+            with pytest.raises(RuntimeError, match=words):
+                call()
+    for training in (True, False):
+        with pytest.raises(TypeError, match="residual must be a Tensor, not float"):
+            dropout(x, 0.5, 1, residual=1.0, training=training)
+    assert layer(x) is x and torch.equal(layer(x, x + 1), x + 1)
 
 
 def test_nothing_is_copied_where_the_result_is_the_residual():
