@@ -37,7 +37,7 @@ def dropout(x, p=0.5, seed=None, offset=0, residual=None, training=True):
             raise RuntimeError("dropout: x and residual must have the same shape")
         return x + residual
     if seed is None:
-        seed = int(torch.randint(2 ** 63 - 1, ()))
+        seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
     return _C._native.dropout(x, p, seed, offset, residual)
 
 

@@ -1,4 +1,4 @@
-"""ops.dropout: evaluation takes the residuals that training takes; results that lie over x or over the residual."""
+"""ops.dropout: evaluation takes the residuals that training takes; a seed that is not given; results that lie over x or over the residual."""
 import ctypes
 
 import pytest
@@ -23,6 +23,32 @@ def test_evaluation_refuses_the_residuals_that_training_refuses():
         with pytest.raises(TypeError, match="residual must be a Tensor, not float"):
             dropout(x, 0.5, 1, residual=1.0, training=training)
     assert layer(x) is x and torch.equal(layer(x, x + 1), x + 1)
+
+
+def test_a_seed_that_is_not_given_is_drawn_on_the_cpu():
+    """Also where tensors are made on another device by default: its generator could not be asked while a graph is captured."""
+    x = torch.zeros(4)
+    torch.manual_seed(3)
+    torch.randint(2 ** 63 - 1, ())
+    after = torch.rand(())
+    torch.manual_seed(3)
+    with torch.device("meta"), pytest.raises(RuntimeError, match="dropout is not implemented on CPU"):
+        dropout(x, 0.5)
+    assert torch.equal(torch.rand(()), after)
+
+
+@pytest.mark.gpu
+def test_a_default_device_changes_no_mask_and_no_capture():
+    x = torch.randn(1000, device="cuda")
+    torch.manual_seed(4)
+    want = dropout(x, 0.5)
+    torch.manual_seed(4)
+    with torch.device("cuda"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = dropout(x, 0.5)
+    graph.replay()
+    assert torch.equal(out, want)
 
 
 def test_nothing_is_copied_where_the_result_is_the_residual():
