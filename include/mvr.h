@@ -309,8 +309,8 @@ int mvr_elastic(const float* coarse, int ndim, int gd, int gh, int gw, int borde
 /* Attention of queries to an encoder's states of another length:
  *   out[r, t, h] = sum_l softmax_l(scale * q[r, t, h] . k[n, l, h / G]) v[n, l, h / G],  G = Hq / Hk,
  * over the states l < lengths[n] of image n = index[r] with mask[n, l] != 0.  A query whose image has no
- * such state, or lies outside [0, N) (bit MVR_STATUS_BAD_BATCH_INDEX is OR-ed into *status by the
- * forward), gives zeros and takes no part in any gradient.  States that are left out are not computed
+ * such state, or lies outside [0, N) (bit MVR_STATUS_BAD_BATCH_INDEX is OR-ed into *status, by the
+ * backward as well), gives zeros and takes no part in any gradient.  States that are left out are not computed
  * with: they may hold anything.  Head sizes up to 256. */
 #define MVR_INDEX_F32 0
 #define MVR_INDEX_F16 1

@@ -22,7 +22,7 @@
 // 2100 to 2500 cycles of a CTA, and tensor memory holds no more CTAs.  Of eight pairs of exponentials two as polynomials were best
 // (none: 3 % slower, four: 6 %).
 //
-// States that are left out (lengths, mask) are compacted to a list of tiles with 128 bits each before the walk; tiles without a state
+// States that are left out (lengths, mask) are compacted to a list of tiles, with a bit a state, before the walk; tiles without a state
 // are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its
 // own before the product reads them.
 #pragma once
@@ -44,12 +44,6 @@ constexpr int kTcMaxStates = 32768;         // states that one CTA can list
 template <int STEP>
 struct StateBits {
   uint32_t w[STEP / 32];
-  __device__ __forceinline__ uint32_t word(int i) const {
-    uint32_t r = w[0];
-#pragma unroll
-    for (int k = 1; k < STEP / 32; ++k) r = i == k ? w[k] : r;
-    return r;
-  }
   __device__ __forceinline__ bool any() const {
     uint32_t r = 0;
 #pragma unroll

@@ -17,8 +17,9 @@
 //
 // Two layouts: classes apart (NC[D]HW maps; a thread walks the classes of neighbouring positions, so that a warp reads
 // consecutive ones) and classes together (rows; a warp or a CTA shares a row).  Up to 16 classes apart, 1024 classes of a warp's row
-// and 65536 half (32768 float) classes of a CTA's row are read once, all loads under way together, and stay in registers.  The scores
-// are read once by each direction, the gradient written once.
+// and 65536 half (32768 float) classes of a CTA's row are read once, all loads under way together, and kept: in registers, but
+// that half scores apart have 64 of them a thread, so that eight CTAs fit an SM, and 9 to 16 classes 13 to 38 words more.  The scores are
+// read once by each direction, the gradient written once.
 //
 // Measured: 2 x 14 x 96^3 half scores with two alternatives 47 us, gradient 34 us (issue slots 54 and 55 % busy: the alternatives, the
 // exponentials and the conversions of 24.8 M scores beside the memory's 15 us); 2000 rows of 32 001 bfloat16 scores with eight
@@ -153,7 +154,7 @@ __device__ __noinline__ void pick_apart(const T* x, long long stride, int classe
 // ---- classes apart: positions consecutive ------------------------------------------------------------
 constexpr int kApartThreads = 128, kApartItems = 32768;  // batch items of a grid's second dimension
 
-// Sorted list of the best TOP scores, offered by rising class: an equal score comes behind.  (NaN is left to pick_slowly.)
+// Sorted list of the best TOP scores, offered by rising class: an equal score comes behind.  (NaN is left to pick_apart.)
 template <int TOP>
 struct Best {
   float v[TOP];
@@ -430,8 +431,9 @@ __global__ void __launch_bounds__(128) logprob_warp_bwd(const __grid_constant__ 
 }
 
 // A CTA's row.  The alternatives need a second look at the scores: split into 32 parts, the top-th largest of the parts' maxima is a
-// bound that at least `top` classes reach, and few more do (some 20 of a random row for top = 8); what reaches it is collected and
-// ranked.  Where more reach it than there is room for (many equal scores), or there is a NaN, they are picked one by one.
+// bound that at least `top` classes reach, and of long rows few more do (some 20 of a random row for top = 8); what reaches it is collected
+// and ranked.  Where more reach it than there is room for, or there is a NaN, they are picked one by one: many equal scores, and rows so
+// short that fewer than `top` parts hold a class (half types with up to 128 (top - 1) of them), whose bound is -inf.
 constexpr int kWide = 512, kRoom = 256;
 
 struct RowShared {
@@ -753,7 +755,7 @@ int launch_logprob(const LogProbParams& p, bool fwd, cudaStream_t st) {
     const long long ctas = p.classes <= 1024 ? (p.batch + 3) / 4 : p.batch;
     if (ctas > 0x7fffffffLL) return 1;
     const dim3 grid((unsigned)ctas);
-    // vectors of a thread, if the row is to stay in registers (one more where it starts between two)
+    // vectors of a thread, if the row is to stay in registers
     const long long vecs = (p.classes / RowShape<T>::V + kWide - 1) / kWide;
     if (p.classes <= 1024) {
       if (!fwd) launch_dependent(p.lse_rest ? logprob_warp_bwd<T, true> : logprob_warp_bwd<T, false>, grid, 128, 0, st, p);
