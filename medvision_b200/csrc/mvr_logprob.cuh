@@ -266,8 +266,8 @@ struct Slope {
   float lse, rest, a, b, k;
   int label;
   __device__ __forceinline__ float at(float x) const {
-    // (a class of probability 0 has lp = -inf: kept finite, so that e = 0 gives 0; NaN is in lse and k as well)
-    const float lp = fmaxf((x - lse) - rest, -1e30f);
+    // (a class of probability 0 has lp = -inf: kept where e is 0 and b lp finite, whatever b; NaN is in lse and k as well)
+    const float lp = fmaxf((x - lse) - rest, -1e4f);
     return -exp2_approx(lp * kLog2e) * fmaf(b, lp, k);
   }
   __device__ __forceinline__ bool empty() const { return lse == -INFINITY; }

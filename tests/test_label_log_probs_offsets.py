@@ -126,6 +126,25 @@ def test_a_loss_near_certainty(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K,space", [(14, 6), (14, 7), (50, 1), (700, 1), (1500, 1)])
+def test_large_gradients_and_classes_without_probability(K, space):
+    """Gradients scaled by 2^40: a class of probability 0 gets 0 from them, the others their multiples."""
+    x = torch.randn(3, K, space, generator=torch.Generator().manual_seed(6))
+    x[:, K // 2] = -float("inf")
+    x[:, K // 3] = -1e30
+    y = torch.randint(-1, K // 3, (3, space), generator=torch.Generator().manual_seed(7))
+    leaf = (x if space > 1 else x.squeeze(2)).cuda().requires_grad_()
+    got = label_log_probs(leaf, (y if space > 1 else y.squeeze(1)).cuda())
+    a, b = (torch.randn(3, space, generator=torch.Generator().manual_seed(8 + i)) * 2.0 ** 40 for i in range(2))
+    g, = torch.autograd.grad((got.log_prob, got.entropy), leaf, (a.cuda().view(got.entropy.shape), b.cuda().view(got.entropy.shape)))
+    xd = x.double()
+    _, h, _, _, grad = reference(xd, y.long(), 0, a.double(), b.double())
+    near = xd.where(xd > -1e3, torch.tensor(-60.0, dtype=torch.float64))
+    check(g.view(3, K, space), grad, gradient_bound(near, grad, a, b, h, 8 * math.sqrt(K) + 4, torch.float32), "gradient")
+    assert not bool(g.view(3, K, space)[:, [K // 2, K // 3]].any())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("K,space", [(14, 6), (14, 7), (50, 1), (700, 1), (1500, 1), (5001, 1)])
 @pytest.mark.parametrize("rest", [True, False])
 def test_the_c_entries_with_the_rest_of_lse_and_without(K, space, rest):
