@@ -11,7 +11,7 @@
 // registers they are walked once with a running maximum: when it moves by d, l and u + d l are scaled by exp(d).  A position whose
 // scores are all -inf has log_prob -inf, entropy 0 and gradient 0.
 //
-// The gradient forms log p_c = (x_c - lse) - rest, where rest is what the rounding of lse to a float left: half a step of lse, which far
+// The gradient forms log p_c = x_c - lse - rest, where rest is what the rounding of lse to a float left: half a step of lse, which far
 // from 0 is no small change of a probability (0.02 % at 8192, 3 % at 10^6).  The forward writes both; where the caller has kept lse alone,
 // the rest is log sum exp(x - lse), one more walk over the scores.
 //
@@ -260,27 +260,28 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
   }
 }
 
-// What the gradient of one position needs beside its scores: g_c = -e (k + b lp), lp = x - lse - rest, e = exp lp, k = a + b H; a more
-// at the label.
+// What the gradient of one position needs beside its scores: g_c = -e (a + b (lp + H)), lp = x - lse - rest, e = exp lp; a more at the
+// label.  With d = x - lse the rest goes into two constants: e = 2^(d log2 e + shift), and k + b d with k = a + b (H - rest).
 struct Slope {
-  float lse, rest, a, b, k;
+  float lse, shift, a, b, k;
   int label;
   __device__ __forceinline__ float at(float x) const {
-    // (a class of probability 0 has lp = -inf: kept where e is 0 and b lp finite, whatever b; NaN is in lse and k as well)
-    const float lp = fmaxf((x - lse) - rest, -1e4f);
-    return -exp2_approx(lp * kLog2e) * fmaf(b, lp, k);
+    // (a class of probability 0 has d = -inf: kept where e is 0 and b d finite, whatever b; NaN is in lse and k as well)
+    const float d = fmaxf(x - lse, -1e4f);
+    return -exp2_approx(fmaf(d, kLog2e, shift)) * fmaf(b, d, k);
   }
   __device__ __forceinline__ bool empty() const { return lse == -INFINITY; }
+  __device__ __forceinline__ void less(float rest) { shift = -rest * kLog2e, k = fmaf(-b, rest, k); }
 };
 template <bool REST>
 __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
   Slope s;
   s.label = label_at(p, i);
   s.lse = p.lse[i];
-  s.rest = REST ? p.lse_rest[i] : 0.0f;
   s.a = s.label >= 0 && p.grad_log_prob ? p.grad_log_prob[i] : 0.0f;
   s.b = p.grad_entropy ? p.grad_entropy[i] : 0.0f;
   s.k = fmaf(s.b, p.entropy[i], s.a);
+  if (REST) s.less(p.lse_rest[i]);
   if (s.lse != s.lse) s.k = NAN;
   return s;
 }
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kApartThreads, 8) logprob_apart_bwd(const __gr
   Slope q[2] = {slope_at<REST>(p, at + s), slope_at<REST>(p, at + s + (second ? 1 : 0))};
   if (!REST) {
     for (int k = 0; k < 2; ++k)
-      q[k].rest = rest_of(rest_part(x + s + (second ? k : 0), p.class_stride, 0, 1, p.classes, q[k].lse), q[k].lse);
+      q[k].less(rest_of(rest_part(x + s + (second ? k : 0), p.class_stride, 0, 1, p.classes, q[k].lse), q[k].lse));
   }
   constexpr int kStep = 8;
   for (int c0 = 0; c0 < p.classes; c0 += kStep) {
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(128) logprob_warp_bwd(const __grid_constant__ 
     float l = rest_part(x, 1, lane, 32, p.classes, q.lse);
 #pragma unroll
     for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
-    q.rest = rest_of(l, q.lse);
+    q.less(rest_of(l, q.lse));
   }
 #pragma unroll 4
   for (int c = lane; c < p.classes; c += 32) {
@@ -691,7 +692,7 @@ __global__ void __launch_bounds__(kWide, 3) logprob_row_bwd(const __grid_constan
     __syncthreads();
     l = 0.0f;
     for (int i = 0; i < kWide / 32; ++i) l += parts[i];
-    q.rest = rest_of(l, q.lse);
+    q.less(rest_of(l, q.lse));
   }
   constexpr int V = RowShape<T>::V;
   const auto one = [&](int c) {
