@@ -35,6 +35,7 @@ struct AttnParams {
   float *lse, *delta;                            // (R, T, Hq); lse in powers of two: log2 of the sum of 2^(s log2 e)
   float* norm;                                   // (R, T, Hq): |g| (float16 gradients)
   int* peaks;                                    // (N, Hk): largest |v| of the states that are read, float bits (float16 gradients)
+  float2* row_peaks;                             // (tile of 128 rows, Hk): largest |g| and |delta| (float16 gradients)
   long long q_r, q_t, q_h, g_r, g_t, g_h;        // strides in elements; the last dimension is contiguous
   long long k_n, k_l, k_h, v_n, v_l, v_h;
   const int *order, *starts, *tiles;             // grouping by image, or null: region r reads image r

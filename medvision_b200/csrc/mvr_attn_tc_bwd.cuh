@@ -319,13 +319,12 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float factor = 1.0f;  // of dS
     if (count > 0 && TcType<T>::code == 0) {
-      float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of some of the rows (what is not finite bounds nothing)
-      const int last = min(o.rows, (first + count) * F::kStep);
-#pragma unroll 4
-      for (int at = first * F::kStep + threadIdx.x; at < last; at += F::kGroups) {
-        const long long number = row_number(p, row_of(p, o, at, hk));
-        most[1] = fmaxf(most[1], finite_or_0(p.norm[number]));
-        most[2] = fmaxf(most[2], finite_or_0(fabsf(p.delta[number])));
+      float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of a tile of rows
+      const int before = o.order ? p.tiles[n] : n * ((o.rows + kTcRows - 1) / kTcRows);
+      for (int t = first * F::kStep / kTcRows + threadIdx.x; t * kTcRows < min(o.rows, (first + count) * F::kStep); t += F::kGroups) {
+        const float2 peak = p.row_peaks[(long long)(before + t) * p.Hk + hk];
+        most[1] = fmaxf(most[1], peak.x);
+        most[2] = fmaxf(most[2], peak.y);
       }
       bar_pass(smem_at(&c.states), 0, lost);
       if (in && part_of == 0) {
@@ -776,25 +775,34 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   }
 }
 
-// delta = g.o per row, and for float16 |g| (2-norm).  16 lanes a row at most.
+// delta = g.o per row; for float16 |g| (2-norm) too, and the largest of both of a tile of rows (what is not finite bounds nothing), so that
+// where states are kept a CTA looks at as many bounds as it has tiles of rows: looking at the rows themselves cost it 9 us of 150 in
+// 128 x 49 rows of two images.  A CTA takes a tile, a row 4, 8 or 16 lanes.
+constexpr int kDeltaThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kDeltaThreads) attn_tc_delta(const __grid_constant__ AttnParams p) {
   grid_dependency();
-  const long long rows = (long long)p.R * p.T * p.Hq;
-  const int lane = threadIdx.x & 31, per = p.D / 8;  // a lane takes 8 elements of a row; 32 / width rows a warp
-  const int width = per <= 4 ? 4 : per <= 8 ? 8 : 16, sub = lane / width, piece = lane % width;
-  for (long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / width); first < rows; first += (long long)gridDim.x * 8 * (32 / width)) {
-    const long long row = first + sub;
+  RowTile o;
+  if (!row_tile(p, blockIdx.x, kTcRows, o) || o.n >= p.N) return;
+  __shared__ int peak[2];
+  if (threadIdx.x < 2) peak[threadIdx.x] = 0;
+  __syncthreads();
+  const int hk = blockIdx.y, lane = threadIdx.x & 31, per = p.D / 8;  // a lane takes 8 elements of a row
+  const int width = per <= 4 ? 4 : per <= 8 ? 8 : 16, piece = lane % width;
+  float most = 0.0f, most_delta = 0.0f;
+  for (int j = threadIdx.x / width; j < kTcRows && o.first + (j & ~(32 / width - 1)) < o.rows; j += kDeltaThreads / width) {
+    const bool mine = o.first + j < o.rows;
+    Row w = {};
+    if (mine) w = row_of(p, o, o.first + j, hk);
+    const long long row = row_number(p, w);
     float v = 0.0f, square = 0.0f;
-    if (row < rows && piece < per) {
-      const int h = (int)(row % p.Hq);
-      const long long rt = row / p.Hq, r = rt / p.T, t = rt - r * p.T;
-      const Vec<T, 8> g = *(const Vec<T, 8>*)((const T*)p.g + r * p.g_r + t * p.g_t + h * p.g_h + piece * 8);
-      const Vec<T, 8> o = *(const Vec<T, 8>*)((const T*)p.o + row * p.D + piece * 8);
+    if (mine && piece < per) {
+      const Vec<T, 8> g = *(const Vec<T, 8>*)((const T*)p.g + w.r * p.g_r + w.t * p.g_t + w.h * p.g_h + piece * 8);
+      const Vec<T, 8> out = *(const Vec<T, 8>*)((const T*)p.o + row * p.D + piece * 8);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = to_float(g.v[e]);
-        v += a * to_float(o.v[e]);
+        v += a * to_float(out.v[e]);
         if (TcType<T>::code == 0) square += a * a;
       }
     }
@@ -802,10 +810,22 @@ __global__ void __launch_bounds__(256) attn_tc_delta(const __grid_constant__ Att
       v += __shfl_xor_sync(~0u, v, d);
       if (TcType<T>::code == 0) square += __shfl_xor_sync(~0u, square, d);
     }
-    if (row < rows && piece == 0) {
+    if (mine && piece == 0) {
       p.delta[row] = v;
-      if (TcType<T>::code == 0) p.norm[row] = sqrtf(square);
+      if (TcType<T>::code == 0) {
+        p.norm[row] = sqrtf(square);
+        most = fmaxf(most, finite_or_0(sqrtf(square)));
+        most_delta = fmaxf(most_delta, finite_or_0(fabsf(v)));
+      }
     }
+  }
+  if constexpr (TcType<T>::code == 0) {
+    if (piece == 0) {
+      atomicMax(&peak[0], __float_as_int(most));
+      atomicMax(&peak[1], __float_as_int(most_delta));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.row_peaks[(long long)blockIdx.x * p.Hk + hk] = make_float2(__int_as_float(peak[0]), __int_as_float(peak[1]));
   }
 }
 

@@ -36,7 +36,7 @@ struct AttnCut {
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
-  long long order, starts, tiles, delta, norm, peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+  long long order, starts, tiles, delta, norm, peaks, row_peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
@@ -109,6 +109,7 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
     if (tc && a->dtype == MVR_F16) {
       c.norm = take(rows * 4);
       c.peaks = take(a->N * a->Hk * 4);
+      c.row_peaks = take(c.row_tiles * a->Hk * 8);
     }
     if (c.splits > 1) c.part_gq = take(c.splits * rows * a->D * 4);
     if (c.row_splits > 1) {
@@ -190,7 +191,7 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   p.scale = a->scale;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.splits = c.splits; p.row_splits = c.row_splits;
-  p.delta = (float*)(ws + c.delta); p.norm = (float*)(ws + c.norm); p.peaks = (int*)(ws + c.peaks);
+  p.delta = (float*)(ws + c.delta); p.norm = (float*)(ws + c.norm); p.peaks = (int*)(ws + c.peaks); p.row_peaks = (float2*)(ws + c.row_peaks);
   p.part_o = (float*)(ws + c.part_o); p.part_ml = (float*)(ws + c.part_ml);
   p.part_gq = (float*)(ws + c.part_gq); p.part_gk = (float*)(ws + c.part_gk); p.part_gv = (float*)(ws + c.part_gv);
   return p;
@@ -339,7 +340,7 @@ int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnC
     bool done = false;
     if constexpr (sizeof(T) == 2) {
       done = c.tc;
-      if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)std::min<long long>(cdiv(rows, 16), 8 * kMultiprocessors)), dim3(256), 0, st, p);
+      if (c.tc) launch_dependent(attn_tc_delta<T>, dim3((unsigned)c.row_tiles, p.Hk), dim3(kDeltaThreads), 0, st, p);
     }
     if (!done) launch_dependent(attn_delta<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, plain);
     if ((rc = launched()) != MVR_OK) return rc;
