@@ -134,7 +134,7 @@ __device__ __forceinline__ bool before(float a, int ia, float b, int ib) {
 
 // The alternatives of a position whose scores are NaN, infinite or too few for the fast way, one by one.
 template <typename T>
-__device__ __noinline__ void pick_apart(const T* x, long long stride, int classes, int top, long long space, float* value, int* label,
+__device__ __forceinline__ void pick_apart(const T* x, long long stride, int classes, int top, long long space, float* value, int* label,
                                         Position q) {
   float last_v = 0.0f;
   int last_c = -1;
@@ -238,25 +238,35 @@ __global__ void __launch_bounds__(kApartThreads, TOP <= 2 && sizeof(T) == 2 ? 8 
     }
   }
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < 2; ++k)
     if (o[k].l != o[k].l) o[k].m = NAN;
+  const Position q[2] = {Position(o[0]), Position(o[1])};
+  float* value = TOP > 0 ? p.top_value + b * p.top * p.space + p.first + s : nullptr;
+  int* best_label = TOP > 0 ? p.top_label + b * p.top * p.space + p.first + s : nullptr;
+  unsigned apart = 0;  // a bit for each position whose alternatives are left to pick_apart
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
     if (k == 1 && !second) break;
-    const Position q(o[k]);
     if constexpr (TOP > 0) {
-      float* value = p.top_value + b * p.top * p.space + p.first;
-      int* best_label = p.top_label + b * p.top * p.space + p.first;
       bool all = o[k].l == o[k].l;
 #pragma unroll
       for (int t = 0; t < TOP; ++t) all = all && (t >= p.top || best[k].c[t] >= 0);
       if (all) {
 #pragma unroll
         for (int t = 0; t < TOP; ++t)
-          if (t < p.top) (value + t * p.space)[s + k] = q.log_prob(best[k].v[t]), (best_label + t * p.space)[s + k] = best[k].c[t];
+          if (t < p.top) (value + t * p.space)[k] = q[k].log_prob(best[k].v[t]), (best_label + t * p.space)[k] = best[k].c[t];
       } else {
-        pick_apart(items + s + k, p.class_stride, p.classes, p.top, p.space, value + s + k, best_label + s + k, q);
+        apart |= 1u << k;
       }
     }
-    q.put(p, at + s + k, o[k], label[k], given[k]);
+    q[k].put(p, at + s + k, o[k], label[k], given[k]);
+  }
+  if constexpr (TOP > 0) {
+    // (At the end and in place, once for both.  As a function that was called between the two, it cost the kernels spills, and those
+    // of more than two alternatives ended in accesses outside of memory that no line of it makes.)
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k)
+      if ((apart >> k) & 1) pick_apart(items + s + k, p.class_stride, p.classes, p.top, p.space, value + k, best_label + k, k ? q[1] : q[0]);
   }
 }
 
@@ -288,7 +298,7 @@ __device__ __forceinline__ Slope slope_at(const LogProbParams& p, long long i) {
 
 // A thread's part of the sum of exp(x - lse): classes first, first + step, ... (0 where lse is -inf).
 template <typename T>
-__device__ __noinline__ float rest_part(const T* x, long long stride, int first, int step, int classes, float lse) {
+__device__ __forceinline__ float rest_part(const T* x, long long stride, int first, int step, int classes, float lse) {
   float l = 0.0f;
   if (lse != -INFINITY)
     for (int c = first; c < classes; c += step) l += exp2_approx((to_float(x[c * stride]) - lse) * kLog2e);
@@ -446,7 +456,7 @@ struct RowShared {
 };
 
 template <typename T>
-__device__ __noinline__ void pick_row(const T* x, int classes, int top, float* value, int* label, Position q, RowShared& sh) {
+__device__ __forceinline__ void pick_row(const T* x, int classes, int top, float* value, int* label, Position q, RowShared& sh) {
   const int lane = threadIdx.x, w = lane >> 5;
   float last_v = 0.0f;
   int last_c = -1;
