@@ -18,12 +18,12 @@
 // Two layouts: classes apart (NC[D]HW maps; a thread walks the classes of neighbouring positions, so that a warp reads
 // consecutive ones) and classes together (rows; a warp or a CTA shares a row).  Up to 16 classes apart, 1024 classes of a warp's row
 // and 65536 half (32768 float) classes of a CTA's row are read once, all loads under way together, and kept: in registers, but
-// that half scores apart have 64 of them a thread, so that eight CTAs fit an SM, and 9 to 16 classes 13 to 38 words more.  The scores are
+// that half scores apart have 64 of them a thread, so that eight CTAs fit an SM, and 9 to 16 classes up to 17 words more.  The scores are
 // read once by each direction, the gradient written once.
 //
-// Measured: 2 x 14 x 96^3 half scores with two alternatives 47 us, gradient 34 us (issue slots 54 and 55 % busy: the alternatives, the
-// exponentials and the conversions of 24.8 M scores beside the memory's 15 us); 2000 rows of 32 001 bfloat16 scores with eight
-// alternatives 57 us (issue 42 %, waits between the row's phases), gradient 49 us (5.2 TB/s); 16 rows of 81 float scores 6 us.
+// Measured: 2 x 14 x 96^3 half scores with two alternatives 41 us, gradient 36 us (issue slots 61 and 53 % busy: the alternatives, the
+// exponentials and the conversions of 24.8 M scores beside the memory's 16 us); 2000 rows of 32 001 bfloat16 scores with eight
+// alternatives 58 us (issue 43 %, waits between the row's phases), gradient 50 us (5.1 TB/s); 16 rows of 81 float scores 6 us.
 #pragma once
 #include "mvr_types.cuh"
 

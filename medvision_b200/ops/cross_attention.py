@@ -22,6 +22,7 @@ def cross_attention(query, key, value, batch_index=None, lengths=None, mask=None
 
     A query for which no state is left gives zeros, and no gradients.  States that are not read may hold anything.
     Returns a contiguous tensor of the query's shape and type.  Sums, weights and statistics are held in float32 and the
-    result is rounded once; for float16 and bfloat16 the weights are rounded to that type before they meet the values.
+    result is rounded once; for float16 and bfloat16 the weights are rounded to that type before they meet the values, and the
+    gradients are formed with the rounded result.
     """
     return _C._native.cross_attention(query, key, value, batch_index, lengths, mask, scale)
