@@ -69,6 +69,10 @@ extern "C" {
 #define MVR_ERR_HEAD_SIZE (-16)
 #define MVR_ERR_PROBABILITY (-17)
 #define MVR_ERR_TOP (-18)
+#define MVR_ERR_WINDOW (-19)          /* a window's reach or number of first states is negative */
+#define MVR_ERR_GROUPS (-20)          /* channels that the groups do not divide */
+#define MVR_ERR_ACTIVATION (-21)
+#define MVR_ERR_AXES (-22)            /* axes, sections or base of rotary positions */
 
 /* element types of label volumes (mvr_affine_label_*) */
 #define MVR_LABEL_U8 0
@@ -306,6 +310,49 @@ int mvr_elastic(const float* coarse, int ndim, int gd, int gh, int gw, int borde
  * overlap (two streams, two captured graphs) need one each.  Results do not depend on the order in
  * which CTAs run. */
 
+/* Group norm with its activation over channels-last values (N, S, C), contiguous, groups of C / groups
+ * consecutive channels:
+ *   z = (x - mean) rstd weight[c] + bias[c],  out = act(z),  rstd = 1 / sqrt(variance + eps)
+ * with mean and variance of an image's group.  weight, bias and their gradients are of parameter_dtype
+ * (MVR_F32 or dtype); null weight and bias: 1 and 0; null gradients: not wanted. */
+#define MVR_ACT_NONE 0
+#define MVR_ACT_RELU 1
+#define MVR_ACT_SILU 2
+#define MVR_ACT_GELU 3                   /* z Phi(z) */
+typedef struct mvr_group_norm {
+  int dtype, parameter_dtype, activation;
+  float eps;
+  int64_t N, S, C, groups;
+  const void *x, *weight, *bias;
+  void* out;
+  float *mean, *rstd;                    /* (N, groups): written by the forward, read by the backward */
+  const void* grad_out;                  /* backward only, from here on */
+  void *grad_x, *grad_weight, *grad_bias;
+} mvr_group_norm;
+int mvr_group_norm_workspace(const mvr_group_norm* a, int backward, int64_t* bytes);
+int mvr_group_norm_forward(const mvr_group_norm* a, void* workspace, int64_t bytes, void* stream);
+int mvr_group_norm_backward(const mvr_group_norm* a, void* workspace, int64_t bytes, void* stream);
+
+/* Rotary positions of several axes.  sections[a] pairs of columns belong to axis a, P in all; pair i of an axis
+ * with n pairs is turned by positions[n, l, axis] * base^(-i / n):
+ *   (u, v) -> (u cos - v sin, u sin + v cos)        (inverse: the other way round, which is the gradient)
+ * Pairs are columns (2i, 2i + 1) (interleaved) or (i, i + P), counted over all axes; the columns from 2P on are
+ * copied.  x[1] (heads[1] > 0) is a second tensor of the same tokens.  out may not overlap x. */
+#define MVR_MAX_AXES 4
+typedef struct mvr_rotary {
+  int dtype, interleaved, inverse, axes;
+  int64_t N, L, D, heads[2];
+  int64_t sections[MVR_MAX_AXES];
+  double base;
+  const void* x[2];                      /* (N, L, heads, D); the last dimension is contiguous */
+  int64_t strides[2][3];                 /* elements, of the first three dimensions */
+  void* out[2];                          /* contiguous */
+  const void* positions;                 /* (N, L, axes) of position_dtype (MVR_INDEX_F32, _I32 or _I64) */
+  int position_dtype;
+  int64_t position_strides[3];
+} mvr_rotary;
+int mvr_rotary_positions(const mvr_rotary* a, void* stream);
+
 /* Attention of queries to an encoder's states of another length:
  *   out[r, t, h] = sum_l softmax_l(scale * q[r, t, h] . k[n, l, h / G]) v[n, l, h / G],  G = Hq / Hk,
  * over the states l < lengths[n] of image n = index[r] with mask[n, l] != 0.  A query whose image has no
@@ -343,6 +390,20 @@ typedef struct mvr_attention {
 int mvr_attention_workspace(const mvr_attention* a, int backward, int64_t* bytes);
 int mvr_attention_forward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream);
 int mvr_attention_backward(const mvr_attention* a, void* workspace, int64_t bytes, int* status, void* stream);
+
+/* The same over a sliding window: token t of sequence n stands at place p = offset + t (offsets[n] + t, if given)
+ * and reads the states j < lengths[n] with j <= p + after and (j >= p - before or j < sinks).  `a` describes the
+ * operands, without an index and a mask (R = N).  A token that reads no state gives zeros and takes no part in
+ * any gradient; states that no token of their sequence reads may hold anything. */
+typedef struct mvr_window {
+  int64_t before, after, sinks; /* not negative */
+  int64_t offset;
+  const void* offsets;          /* (N) or null: offset for all */
+  int offsets_64;               /* offsets are int64 (else int32) */
+} mvr_window;
+int mvr_window_attention_workspace(const mvr_attention* a, const mvr_window* w, int backward, int64_t* bytes);
+int mvr_window_attention_forward(const mvr_attention* a, const mvr_window* w, void* workspace, int64_t bytes, int* status, void* stream);
+int mvr_window_attention_backward(const mvr_attention* a, const mvr_window* w, void* workspace, int64_t bytes, int* status, void* stream);
 
 /* out[e] = residual[e] + (kept(e) ? x[e] / (1 - p) : 0), residual may be null (0).  kept(e) depends on
  * (seed, offset, e) alone: element e takes 16 bits, halves of 32-bit words in order and the low half

@@ -29,7 +29,25 @@ class Attention(ctypes.Structure):
          ("grad_k", _vp), ("grad_v", _vp)]
 
 
-_attention = ctypes.POINTER(Attention)
+class Window(ctypes.Structure):
+    """struct mvr_window of include/mvr.h."""
+    _fields_ = [("before", _i64), ("after", _i64), ("sinks", _i64), ("offset", _i64), ("offsets", _vp), ("offsets_64", _i32)]
+
+
+class GroupNorm(ctypes.Structure):
+    """struct mvr_group_norm of include/mvr.h."""
+    _fields_ = [("dtype", _i32), ("parameter_dtype", _i32), ("activation", _i32), ("eps", _f32)] + [(n, _i64) for n in ("N", "S", "C", "groups")] + \
+        [(n, _vp) for n in ("x", "weight", "bias", "out", "mean", "rstd", "grad_out", "grad_x", "grad_weight", "grad_bias")]
+
+
+class Rotary(ctypes.Structure):
+    """struct mvr_rotary of include/mvr.h."""
+    _fields_ = [("dtype", _i32), ("interleaved", _i32), ("inverse", _i32), ("axes", _i32), ("N", _i64), ("L", _i64), ("D", _i64), ("heads", _i64 * 2),
+                ("sections", _i64 * 4), ("base", _f64), ("x", _vp * 2), ("strides", (_i64 * 3) * 2), ("out", _vp * 2), ("positions", _vp),
+                ("position_dtype", _i32), ("position_strides", _i64 * 3)]
+
+
+_attention, _window, _norm = ctypes.POINTER(Attention), ctypes.POINTER(Window), ctypes.POINTER(GroupNorm)
 
 # name -> argtypes, exactly the prototypes of include/mvr.h
 _GENERAL = [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
@@ -68,6 +86,13 @@ PROTOTYPES = {
     "mvr_attention_workspace": [_attention, _i32, ctypes.POINTER(_i64)],
     "mvr_attention_forward": [_attention, _vp, _i64, _vp, _vp],
     "mvr_attention_backward": [_attention, _vp, _i64, _vp, _vp],
+    "mvr_window_attention_workspace": [_attention, _window, _i32, ctypes.POINTER(_i64)],
+    "mvr_window_attention_forward": [_attention, _window, _vp, _i64, _vp, _vp],
+    "mvr_window_attention_backward": [_attention, _window, _vp, _i64, _vp, _vp],
+    "mvr_group_norm_workspace": [_norm, _i32, ctypes.POINTER(_i64)],
+    "mvr_group_norm_forward": [_norm, _vp, _i64, _vp],
+    "mvr_group_norm_backward": [_norm, _vp, _i64, _vp],
+    "mvr_rotary_positions": [ctypes.POINTER(Rotary), _vp],
     "mvr_dropout": [_vp, _vp, _vp, _i32, _i64, _f64, _u64, _vp, _u64, _vp],
     "mvr_label_log_probs_forward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "mvr_label_log_probs_backward": [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,

@@ -11,14 +11,16 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmvr.so")
 NATIVE = os.path.join(HERE, "_native.so")
-SOURCES = ["mvr_api.cu", "mvr_heads.cu"]  # one object file each
+SOURCES = ["mvr_api.cu", "mvr_heads.cu", "mvr_window.cu", "mvr_encoder.cu"]  # one object file each
 HEADERS = ["mvr_arith.cuh", "mvr_geom.cuh", "mvr_generic.cuh", "mvr_stream3d.cuh", "mvr_tma3d.cuh", "mvr_brick3d.cuh", "mvr_bwd3d.cuh", "mvr_offset.cuh", "mvr_cubic3d.cuh", "mvr_flat.cuh", "mvr_label.cuh", "mvr_plane2d.cuh", "mvr_elastic.cuh", "mvr_head.cuh",
            os.path.join("..", "..", "include", "mvr.h")]
-HEAD_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_tc.cuh", "mvr_dropout.cuh", "mvr_logprob.cuh",
-                os.path.join("..", "..", "include", "mvr.h")]
-HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": HEAD_HEADERS}
-NATIVE_SOURCES = ["mvr_torch.cpp", "mvr_torch_heads.cpp"]
-NATIVE_HEADERS = ["mvr_torch.h", os.path.join("..", "..", "include", "mvr.h")]
+ATTENTION_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_attn_host.cuh", "mvr_tc.cuh",
+                     os.path.join("..", "..", "include", "mvr.h")]
+HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": ATTENTION_HEADERS + ["mvr_dropout.cuh", "mvr_logprob.cuh"], "mvr_window.cu": ATTENTION_HEADERS,
+              "mvr_encoder.cu": ["mvr_types.cuh", "mvr_norm.cuh", "mvr_rotary.cuh", os.path.join("..", "..", "include", "mvr.h")]}
+LIB_FILES = sorted(set(SOURCES).union(*HEADERS_OF.values()))
+NATIVE_SOURCES = ["mvr_torch.cpp", "mvr_torch_heads.cpp", "mvr_torch_encoder.cpp"]
+NATIVE_HEADERS = ["mvr_torch.h", "mvr_torch_operators.h", os.path.join("..", "..", "include", "mvr.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -33,7 +35,7 @@ def _older(target, files):
 
 
 def needs_build():
-    return _older(LIB, SOURCES + HEADERS + HEAD_HEADERS) or _older(NATIVE, NATIVE_SOURCES + NATIVE_HEADERS)
+    return _older(LIB, LIB_FILES) or _older(NATIVE, NATIVE_SOURCES + NATIVE_HEADERS)
 
 
 def _build_native():
@@ -56,7 +58,7 @@ def _build_native():
 
 def build(force=False, verbose=False):
     """nvcc cross-compiles without a GPU; both .so stay beside the package."""
-    if force or _older(LIB, SOURCES + HEADERS + HEAD_HEADERS):
+    if force or _older(LIB, LIB_FILES):
         nvcc = os.environ.get("NVCC", "nvcc")
         objects, running = [], []
         for source in SOURCES:

@@ -185,6 +185,10 @@ const char* mvr_strerror(int code) {
     case MVR_ERR_HEADS: return "the number of query heads must be a multiple of the number of key heads";
     case MVR_ERR_HEAD_SIZE: return "head sizes up to 256 are supported";
     case MVR_ERR_PROBABILITY: return "the dropout probability must be between 0 and 1";
+    case MVR_ERR_WINDOW: return "a window's reach and number of first states must not be negative";
+    case MVR_ERR_GROUPS: return "the number of groups must divide the number of channels";
+    case MVR_ERR_ACTIVATION: return "unknown activation";
+    case MVR_ERR_AXES: return "rotary positions take 1 to 4 axes, sections of no more pairs than the head size has, and a positive base";
     case MVR_ERR_TOP: return "the number of alternatives must be between 0 and 16, and at most the number of classes";
     default: return "unknown error";
   }

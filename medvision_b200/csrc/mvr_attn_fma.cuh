@@ -150,7 +150,36 @@ __device__ __forceinline__ bool fma_allowed(float* allowed, const AttnParams& p,
   return __syncthreads_or(any);
 }
 
-template <typename T, int DP>
+// The same for the states of a span.
+__device__ __forceinline__ bool in_span(const Span& s, int j) { return (j >= s.lo && j < s.hi) || j < s.sink; }
+__device__ __forceinline__ bool fma_allowed(float* allowed, const Span& s, int first, int size) {
+  bool any = false;
+  if ((int)threadIdx.x < size) {
+    any = in_span(s, first + threadIdx.x);
+    allowed[threadIdx.x] = any ? 1.0f : 0.0f;
+  }
+  return __syncthreads_or(any);
+}
+// A window's part of a row tile's walk, and the spans of a thread's rows.
+template <int DP>
+struct FmaWindow {
+  typedef FmaTile<DP> F;
+  Span span, own[F::MT];
+  int first, last;  // tiles of the span
+  __device__ __forceinline__ FmaWindow(const AttnParams& p, const RowTile& o, int split, int ty) {
+    const long long place0 = first_place(p, o.n);
+    const int end = states_of(p, o.n);
+    const auto place = [&](int row) { return place0 + p.by_G.quotient(min(row, o.rows - 1)); };
+    span = span_of(p, place(o.first), place(o.first + F::BT - 1), end);
+#pragma unroll
+    for (int i = 0; i < F::MT; ++i) own[i] = span_of(p, place(o.first + ty * F::MT + i), place(o.first + ty * F::MT + i), end);
+    first = split * p.tiles_per;
+    last = min(first + p.tiles_per, SpanTiles<F::BT>(span).count);
+  }
+};
+
+// WINDOW: a sliding window's states instead of all.
+template <typename T, int DP, bool WINDOW = false>
 __global__ void __launch_bounds__(kFmaThreads) attn_fma_fwd(const __grid_constant__ AttnParams p) {
   typedef FmaTile<DP> F;
   extern __shared__ __align__(16) float fma_smem[];
@@ -170,9 +199,11 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_fwd(const __grid_constan
   float acc[F::MT][F::CW] = {}, m[F::MT], l[F::MT] = {};
 #pragma unroll
   for (int i = 0; i < F::MT; ++i) m[i] = -INFINITY;
-  for (int j0 = begin; j0 < end; j0 += F::BT) {
+  const FmaWindow<WINDOW ? DP : 16> window(p, o, split, ty);
+  for (int step = WINDOW ? window.first : begin; step < (WINDOW ? window.last : end); step += WINDOW ? 1 : F::BT) {
+    const int j0 = WINDOW ? SpanTiles<F::BT>(window.span).first(step) : step;
     // (the barrier inside also ends the last tile's reads)
-    if (!fma_allowed(allowed, p, o.n, j0, end, F::BT)) continue;
+    if (!(WINDOW ? fma_allowed(allowed, window.span, j0, F::BT) : fma_allowed(allowed, p, o.n, j0, end, F::BT))) continue;
     fma_load_states<T, DP>(ks, k, p.k_l, j0, allowed, p.D);
     fma_load_states<T, DP>(vs, v, p.v_l, j0, allowed, p.D);
     __syncthreads();
@@ -183,7 +214,7 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_fwd(const __grid_constan
       float top = m[i];
 #pragma unroll
       for (int j = 0; j < F::MT; ++j) {
-        s[i][j] = allowed[tx + 16 * j] != 0.0f ? s[i][j] * p.scale_log2 : -INFINITY;
+        s[i][j] = (WINDOW ? in_span(window.own[i], j0 + tx + 16 * j) : allowed[tx + 16 * j] != 0.0f) ? s[i][j] * p.scale_log2 : -INFINITY;
         top = fmaxf(top, s[i][j]);
       }
 #pragma unroll
@@ -232,7 +263,7 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_fwd(const __grid_constan
 }
 
 // Gradient of the queries: a tile of rows against the states of its image.
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW = false>
 __global__ void __launch_bounds__(kFmaThreads) attn_fma_dq(const __grid_constant__ AttnParams p) {
   typedef FmaTile<DP> F;
   extern __shared__ __align__(16) float fma_smem[];
@@ -258,8 +289,10 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dq(const __grid_constant
     lse[i] = row < 0 ? -INFINITY : p.lse[row];
     delta[i] = row < 0 ? 0.0f : p.delta[row];
   }
-  for (int j0 = begin; j0 < end; j0 += F::BT) {
-    if (!fma_allowed(allowed, p, o.n, j0, end, F::BT)) continue;
+  const FmaWindow<WINDOW ? DP : 16> window(p, o, split, ty);
+  for (int step = WINDOW ? window.first : begin; step < (WINDOW ? window.last : end); step += WINDOW ? 1 : F::BT) {
+    const int j0 = WINDOW ? SpanTiles<F::BT>(window.span).first(step) : step;
+    if (!(WINDOW ? fma_allowed(allowed, window.span, j0, F::BT) : fma_allowed(allowed, p, o.n, j0, end, F::BT))) continue;
     fma_load_states<T, DP>(ks, k, p.k_l, j0, allowed, p.D);
     fma_load_states<T, DP>(vs, v, p.v_l, j0, allowed, p.D);
     __syncthreads();
@@ -270,7 +303,7 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dq(const __grid_constant
     for (int i = 0; i < F::MT; ++i)
 #pragma unroll
       for (int j = 0; j < F::MT; ++j) {
-        const bool in = allowed[tx + 16 * j] != 0.0f && lse[i] != -INFINITY;
+        const bool in = (WINDOW ? in_span(window.own[i], j0 + tx + 16 * j) : allowed[tx + 16 * j] != 0.0f) && lse[i] != -INFINITY;
         s[i][j] = in ? exp2f(s[i][j] * p.scale_log2 - lse[i]) * (dp[i][j] - delta[i]) : 0.0f;
       }
     fma_put<DP>(ws, s, tx, ty);
@@ -294,20 +327,30 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dq(const __grid_constant
 }
 
 // Gradients of keys and values: a tile of states against the rows that read its image.
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW = false>
 __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constant__ AttnParams p) {
   typedef FmaTile<DP> F;
   extern __shared__ __align__(16) float fma_smem[];
   float *ks = fma_smem, *vs = ks + F::BT * F::LD, *qs = vs + F::BT * F::LD, *gs = qs + F::BT * F::LD, *ws = gs + F::BT * F::LD,
         *allowed = ws + F::BT * F::LP, *lse = allowed + F::BT, *delta = lse + F::BT;
   grid_dependency();
-  const int tiles = (p.L + F::BT - 1) / F::BT, n = blockIdx.x / tiles, j0 = (blockIdx.x - n * tiles) * F::BT;
-  const int hk = blockIdx.y, split = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int tiles = (p.L + F::BT - 1) / F::BT, hk = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const StateTile st = WINDOW ? state_tile(p, tiles) : StateTile{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles, (int)blockIdx.z, false};
+  const int n = st.n, j0 = st.tile * F::BT, split = st.part;
   __shared__ FmaRows<F::BT> at;
   const RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::BT - 1) / F::BT, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   const bool any = fma_allowed(allowed, p, n, j0, states_of(p, n), F::BT);
-  const int first = any ? split * per * F::BT : 0, last = any ? min(o.rows, (split + 1) * per * F::BT) : 0;
+  int first = any ? split * per * F::BT : 0, last = any ? min(o.rows, (split + 1) * per * F::BT) : 0;
+  const long long place0 = WINDOW ? first_place(p, n) : 0;
+  if (WINDOW) {
+    const TileRows r = rows_of_states(p, st, place0, j0, F::BT, F::BT);
+    first = any ? r.first * F::BT : 0;
+    last = any ? min(o.rows, (r.first + r.count) * F::BT) : 0;
+  }
+  int row_lo[F::MT], row_hi[F::MT];
+#pragma unroll
+  for (int i = 0; i < F::MT; ++i) rows_of_state(p, place0, j0 + ty * F::MT + i, row_lo[i], row_hi[i]);
   float dk[F::MT][F::CW] = {}, dv[F::MT][F::CW] = {};
   if (first < last) {
     fma_load_states<T, DP>(ks, (const T*)p.k + (long long)n * p.k_n + (long long)hk * p.k_h, p.k_l, j0, allowed, p.D);
@@ -332,7 +375,8 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
 #pragma unroll
       for (int j = 0; j < F::MT; ++j) {
         const float a = lse[tx + 16 * j];
-        const bool in = allowed[ty * F::MT + i] != 0.0f && a != -INFINITY;
+        const int row = r0 + tx + 16 * j;
+        const bool in = allowed[ty * F::MT + i] != 0.0f && a != -INFINITY && (!WINDOW || (row >= row_lo[i] && row < row_hi[i]));
         s[i][j] = in ? exp2f(s[i][j] * p.scale_log2 - a) : 0.0f;
         dp[i][j] = in ? s[i][j] * (dp[i][j] - delta[tx + 16 * j]) : 0.0f;
       }
@@ -351,15 +395,16 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
     const int j = j0 + ty * F::MT + i;
     if (j >= p.L) continue;
     const long long to = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
+    const PartPlace part = part_place(p, st, j, hk, F::BT);
     const bool in = allowed[ty * F::MT + i] != 0.0f;  // others: 0, also where rows hold NaN
 #pragma unroll
     for (int c = 0; c < F::CW; ++c) {
       const int d = fma_col<DP>(c, tx);
       if (d >= p.D) continue;
       const float a = in ? dk[i][c] : 0.0f, b = in ? dv[i][c] : 0.0f;
-      if (p.row_splits > 1) {
-        p.part_gk[split * all + to + d] = a;
-        p.part_gv[split * all + to + d] = b;
+      if (WINDOW ? part.parts : p.row_splits > 1) {
+        p.part_gk[WINDOW ? part.at + d : split * all + to + d] = a;
+        p.part_gv[WINDOW ? part.at + d : split * all + to + d] = b;
       } else {
         ((T*)p.gk)[to + d] = from_float<T>(a * p.scale);
         ((T*)p.gv)[to + d] = from_float<T>(b);

@@ -58,7 +58,10 @@ struct StateBits {
   }
 };
 
-template <int DP, int TILES, bool MASK, int PIECES>
+// Which states a row reads: all of its image, those on a list (lengths, mask), or those of a sliding window.
+enum { kAll = 0, kListed = 1, kWindow = 2 };
+
+template <int DP, int TILES, int MODE, int PIECES>
 struct TcForward {
   static_assert(PIECES == 1 || (DP == 64 && TILES == 1), "");
   static constexpr int kStep = TILES == 2 ? 128 : 64, kHalves = kStep / 64, kMaxTiles = kTcMaxStates / kStep;
@@ -77,11 +80,19 @@ struct TcForward {
     int lost, tiles, regions;
     int order[TILES == 1 ? kTcRows : 1];          // regions of the image, where the index is not grouped
     float top[kHalves == 2 ? 2 : 1][TILES][2][128];  // what the two halves of a row tell each other
-    unsigned short list[MASK ? kMaxTiles : 1];
-    StateBits<kStep> bits[MASK ? kMaxTiles : 1];
+    unsigned short list[MODE == kListed ? kMaxTiles : 1];
+    StateBits<kStep> bits[MODE == kListed ? kMaxTiles : 1];
   };
   static constexpr size_t kShared = TILES * (size_t)kRowsBytes + kSlots * (size_t)kSlotBytes + sizeof(Control) + 1024;
 };
+
+template <int STEP>
+__device__ __forceinline__ StateBits<STEP> bits_of_span(const Span& s, int first) {
+  StateBits<STEP> b;
+#pragma unroll
+  for (int k = 0; k < STEP / 32; ++k) b.w[k] = span_bits(s, first + k * 32);
+  return b;
+}
 
 struct TcMaps {
   CUtensorMap k, v;  // (D, heads, states, images; pieces one behind another)
@@ -174,10 +185,11 @@ __device__ __forceinline__ void put_floats(float* to, const uint32_t (&v)[32], i
 }
 
 // PIECES 3: float tensors, whose operands lie in pieces (T is bfloat16).
-template <typename T, int DP, int TILES, bool MASK, int PIECES>
-__global__ void __launch_bounds__(TcForward<DP, TILES, MASK, PIECES>::kThreads, TcForward<DP, TILES, MASK, PIECES>::kResident)
+template <typename T, int DP, int TILES, int MODE, int PIECES>
+__global__ void __launch_bounds__(TcForward<DP, TILES, MODE, PIECES>::kThreads, TcForward<DP, TILES, MODE, PIECES>::kResident)
 attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
-  typedef TcForward<DP, TILES, MASK, PIECES> F;
+  typedef TcForward<DP, TILES, MODE, PIECES> F;
+  constexpr bool MASK = MODE != kAll;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);
   char* ring = base + TILES * F::kRowsBytes;
@@ -207,7 +219,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   RowTile o;
   const int hk = blockIdx.y, split = blockIdx.z;
   bool some;
-  if (TILES == 1 && p.index) {
+  if (MODE != kWindow && TILES == 1 && p.index) {
     // few regions: the CTA looks for those of its image itself, which is faster than a kernel that groups them
     const int n = blockIdx.x;
     if (warp == 0) {
@@ -233,20 +245,34 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const int begin = split * per * F::kStep;
   int end = 0;
   if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
-  if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  if (MODE == kListed && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  // a window: the states that any of the tile's rows reads, and this part's tiles of them
+  const long long place0 = MODE == kWindow && some ? first_place(p, o.n) : 0;
+  const int states = MODE == kWindow && some ? states_of(p, o.n) : 0;
+  Span span = {};
+  if (MODE == kWindow && some)
+    span = span_of(p, place0 + p.by_G.quotient(o.first), place0 + p.by_G.quotient(min(o.first + TILES * kTcRows, o.rows) - 1), states);
+  const SpanTiles<F::kStep> window(span);
+  const int window_first = split * p.tiles_per;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
+  const int tiles = MODE == kWindow ? max(0, min(p.tiles_per, window.count - window_first))
+                    : !some || begin >= end ? 0 : MODE == kListed ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
   const int used = !some ? 0 : TILES == 2 && o.first + kTcRows < o.rows ? 2 : 1;  // row tiles that have rows
   const uint32_t tmem = c.tmem;
   volatile int* lost = &c.lost;
-  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * F::kStep; };
+  const auto first_of = [&](int i) {
+    return MODE == kWindow ? window.first(window_first + i) : begin + (MODE == kListed ? (int)c.list[i] : i) * F::kStep;
+  };
 
   const auto clean = [&](int tile, int slot) {
+    StateBits<F::kStep> bits;
+    if constexpr (MODE == kWindow) bits = bits_of_span<F::kStep>(span, first_of(tile));
+    else bits = c.bits[MASK ? tile : 0];
     for (int piece = 0; piece < PIECES; ++piece)
-      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, c.bits[MASK ? tile : 0], lane);
+      clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, bits, lane);
     if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
   };
 
@@ -359,6 +385,8 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       Row w = {};
       const bool mine = j0 < o.rows;
       if (mine) w = row_of(p, o, j0, hk);
+      Span own = {};  // of this row
+      if (MODE == kWindow && mine) own = span_of(p, place0 + w.t, place0 + w.t, states);
       if (tiles > 0) {
         const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
         if (F::kHalves == 1)
@@ -394,7 +422,13 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       } else {
       for (int j = 0; j < tiles; ++j) {
         uint32_t bits[2] = {~0u, ~0u};
-        if (MASK) {
+        if (MODE == kWindow) {
+          const int at = first_of(j) + half * 64;
+          if (at < own.lo || at + 64 > own.hi) {
+            bits[0] = span_bits(own, at);
+            bits[1] = span_bits(own, at + 32);
+          }
+        } else if (MODE == kListed) {
           bits[0] = c.bits[j].w[half * 2];
           bits[1] = c.bits[j].w[half * 2 + 1];
         } else if (j + 1 == tiles && end % F::kStep) {

@@ -93,7 +93,8 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 }
 
 // BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
-template <typename T, int DP, bool BOXES, int PIECES>
+// WINDOW: a tile of states meets the rows whose windows reach it; the first tiles, which all tokens may read, are cut into more parts.
+template <typename T, int DP, bool BOXES, int PIECES, bool WINDOW = false>
 __global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, PIECES>::kResident)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcStates<DP, PIECES> F;
@@ -120,8 +121,9 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
-  const int state_tiles = (p.L + 127) / 128, n = blockIdx.x / state_tiles, j0 = (blockIdx.x - n * state_tiles) * 128;
-  const int hk = blockIdx.y, split = blockIdx.z;
+  const int state_tiles = (p.L + 127) / 128, hk = blockIdx.y;
+  const StateTile st = WINDOW ? state_tile(p, state_tiles) : StateTile{(int)blockIdx.x / state_tiles, (int)blockIdx.x % state_tiles, (int)blockIdx.z, false};
+  const int n = st.n, j0 = st.tile * 128, split = st.part;
   // one row a thread: its state, and whether it is read
   const int r = ((warp & 3) << 5) + lane, part_of = warp >> 2, j = j0 + r;
   bool in = false;
@@ -129,7 +131,14 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const bool any = __syncthreads_or(in);
   const RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
-  const int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0;
+  int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0, row_lo = 0, row_hi = 0;
+  if (WINDOW) {
+    const long long place0 = first_place(p, n);
+    rows_of_state(p, place0, j, row_lo, row_hi);  // (one state a thread)
+    const TileRows r = rows_of_states(p, st, place0, j0, 128, F::kStep);
+    first = r.first;
+    count = any ? r.count : 0;
+  }
   // what lies behind D in the rows' tiles stays 0
   if (count > 0 && p.W < DP) {
     for (int e = threadIdx.x; e < 2 * F::kStages * F::kStageBytes / 16; e += F::kThreads)
@@ -347,7 +356,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         if (lane == 0) atomicMax(&c.peak[k], __float_as_int(most[k]));
       }
       group_sync(F::kGroups);
-      if (threadIdx.x == 0) atomicMax(p.peaks + (long long)n * p.Hk + hk, c.peak[0]);
+      if (threadIdx.x == 0) atomicMax(p.peaks + (WINDOW ? (long long)n * state_tiles + st.tile : (long long)n) * p.Hk + hk, c.peak[0]);
       factor = slope_scale<T>(__int_as_float(c.peak[1]) * __int_as_float(c.peak[0]) + __int_as_float(c.peak[2]));
     }
     const float2 slope2 = make_float2(factor * exp2f(-shift), factor * exp2f(-shift)), scale2 = make_float2(p.scale_log2, p.scale_log2);
@@ -373,6 +382,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         if (i > 0 && part_of == 0) collect(F::kValues);  // (of the tile before: its product ended before these scores)
       }
       const int col = part_of * 32;
+      // rows that do not read this state
+      const uint32_t bits = WINDOW ? bits_below(row_hi - (first + i) * F::kStep - col) & ~bits_below(row_lo - (first + i) * F::kStep - col) : ~0u;
       float2 w[16];
       uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
@@ -384,7 +395,8 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         for (int k = 0; k < 2; ++k) {
           const float2 x = fma2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])), scale2,
                                 k ? make_float2(lse.z, lse.w) : make_float2(lse.x, lse.y));
-          const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+          float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+          if (WINDOW && bits != ~0u) y = make_float2((bits >> (e + 2 * k)) & 1 ? y.x : 0.0f, (bits >> (e + 2 * k + 1)) & 1 ? y.y : 0.0f);
           w[e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
           if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(y.x, y.y);
           else pieces_of(y, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
@@ -410,8 +422,9 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         const float4 delta = *(const float4*)&c.delta[stage][col + e];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float2 ds = mul2(w[e / 2 + k], add2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])),
-                                                    k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
+          float2 ds = mul2(w[e / 2 + k], add2(make_float2(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])),
+                                              k ? make_float2(delta.z, delta.w) : make_float2(delta.x, delta.y)));
+          if (WINDOW && bits != ~0u) ds = make_float2((bits >> (e + 2 * k)) & 1 ? ds.x : 0.0f, (bits >> (e + 2 * k + 1)) & 1 ? ds.y : 0.0f);
           if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(ds.x, ds.y);
           else pieces_of(ds, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
         }
@@ -432,10 +445,11 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       constexpr int kHalf = F::kGroups / 256;
       const bool keys = part_of >= kHalf;
       const long long all = (long long)p.N * p.L * p.Hk * p.D, at = (((long long)n * p.L + j) * p.Hk + hk) * p.D;
-      const bool parts = p.row_splits > 1;
+      const PartPlace place = WINDOW ? part_place(p, st, j, hk, 128) : PartPlace{p.row_splits > 1, split * all + at};
+      const bool parts = place.parts;
       const float f = in ? (keys ? (parts ? 1.0f : p.scale) / factor : exp2f(-shift)) : 0.0f;
       Out* to = (Out*)(keys ? p.gk : p.gv) + at;
-      float* part = parts ? (keys ? p.part_gk : p.part_gv) + split * all + at : nullptr;
+      float* part = parts ? (keys ? p.part_gk : p.part_gv) + place.at : nullptr;
       const auto put = [&](int q, uint32_t (&v)[32]) {
         // (a state that is not read: its sums may be NaN where rows hold NaN)
         if (j < p.L) {
@@ -485,7 +499,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
 }
 
 // ---- rows kept: dq ------------------------------------------------------------------------------------
-template <int DP, bool MASK, int PIECES>
+template <int DP, int MODE, int PIECES>
 struct TcRows {
   static constexpr int kStep = kGradStep<DP>, kBlocks = DP / 64, kTileBytes = kBlocks * 128 * 128, kStepBytes = kBlocks * kStep * 128, kSlots = 4;
   static constexpr int kRowsBytes = PIECES * kTileBytes, kSlotBytes = PIECES * kStepBytes;
@@ -497,16 +511,17 @@ struct TcRows {
     unsigned long long full[kSlots], empty[kSlots], clean[kSlots], rows, scores, taken, slopes, grads, done;
     uint32_t tmem;
     int lost, tiles;
-    unsigned short list[MASK ? kMaxTiles : 1];
-    StateBits<kStep> bits[MASK ? kMaxTiles : 1];
+    unsigned short list[MODE == kListed ? kMaxTiles : 1];
+    StateBits<kStep> bits[MODE == kListed ? kMaxTiles : 1];
   };
   static constexpr size_t kShared = 2 * (size_t)kRowsBytes + kSlots * (size_t)kSlotBytes + sizeof(Control) + 1024;
 };
 
-template <typename T, int DP, bool MASK, int PIECES>
-__global__ void __launch_bounds__(TcRows<DP, MASK, PIECES>::kThreads, TcRows<DP, MASK, PIECES>::kResident)
+template <typename T, int DP, int MODE, int PIECES>
+__global__ void __launch_bounds__(TcRows<DP, MODE, PIECES>::kThreads, TcRows<DP, MODE, PIECES>::kResident)
 attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
-  typedef TcRows<DP, MASK, PIECES> F;
+  typedef TcRows<DP, MODE, PIECES> F;
+  constexpr bool MASK = MODE != kAll;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // Q, G, then the ring
@@ -538,15 +553,25 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   const int begin = split * per * F::kStep;
   int end = 0;
   if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
-  if (MASK && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  if (MODE == kListed && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
+  const long long place0 = MODE == kWindow && some ? first_place(p, o.n) : 0;
+  const int states = MODE == kWindow && some ? states_of(p, o.n) : 0;
+  Span span = {};
+  if (MODE == kWindow && some)
+    span = span_of(p, place0 + p.by_G.quotient(o.first), place0 + p.by_G.quotient(min(o.first + kTcRows, o.rows) - 1), states);
+  const SpanTiles<F::kStep> window(span);
+  const int window_first = split * p.tiles_per;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tiles = !some || begin >= end ? 0 : MASK ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
+  const int tiles = MODE == kWindow ? max(0, min(p.tiles_per, window.count - window_first))
+                    : !some || begin >= end ? 0 : MODE == kListed ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
   const uint32_t tmem = c.tmem;
   volatile int* lost = &c.lost;
-  const auto first_of = [&](int i) { return begin + (MASK ? (int)c.list[i] : i) * F::kStep; };
+  const auto first_of = [&](int i) {
+    return MODE == kWindow ? window.first(window_first + i) : begin + (MODE == kListed ? (int)c.list[i] : i) * F::kStep;
+  };
 
   if (warp == kLoader) {
     int i = 0;
@@ -636,8 +661,11 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     for (int i = 0; i < tiles; ++i) {
       const int k = 2 * i, slot = k % F::kSlots;
       if (!__all_sync(~0u, bar_wait(smem_at(&c.full[slot]), (k / F::kSlots) & 1, lost))) break;
+      StateBits<F::kStep> bits;
+      if constexpr (MODE == kWindow) bits = bits_of_span<F::kStep>(span, first_of(i));
+      else bits = c.bits[i];
       for (int piece = 0; piece < PIECES; ++piece)
-        clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, c.bits[i], lane);
+        clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, bits, lane);
       if (lane == 0) bar_arrive(smem_at(&c.clean[slot]));
     }
   } else if (warp < kLoader) {
@@ -647,14 +675,27 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     Row w = {};
     long long number = 0;
     float lse = INFINITY, delta = 0.0f, factor = 1.0f;  // factor: of dS
+    Span own = {};
+    // (float16, a window: the largest |v| of the tiles of states that this part walks)
+    int peak = 0;
+    if (MODE == kWindow && TcType<T>::code == 0 && tiles > 0) {
+      const int state_tiles = (p.L + 127) / 128;
+      for (int i = lane; i < tiles; i += 32)
+        peak = max(peak, p.peaks[((long long)o.n * state_tiles + first_of(i) / 128) * p.Hk + hk]);
+      peak = __reduce_max_sync(~0u, peak);
+    }
     if (mine) {
       w = row_of(p, o, j0, hk);
+      if (MODE == kWindow) own = span_of(p, place0 + w.t, place0 + w.t, states);
       number = row_number(p, w);
       if (tiles > 0) {
         lse = p.lse[number];
         if (lse == -INFINITY) lse = INFINITY;
         delta = p.delta[number];
-        if (TcType<T>::code == 0) factor = slope_scale<T>(p.norm[number] * __int_as_float(p.peaks[(long long)o.n * p.Hk + hk]) + fabsf(delta));
+        if (TcType<T>::code == 0) {
+          if (MODE != kWindow) peak = p.peaks[(long long)o.n * p.Hk + hk];
+          factor = slope_scale<T>(p.norm[number] * __int_as_float(peak) + fabsf(delta));
+        }
       }
     }
     if (tiles > 0) {
@@ -683,7 +724,10 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     };
     for (int i = 0; i < tiles; ++i) {
       uint32_t bits = ~0u;
-      if (MASK) {
+      if (MODE == kWindow) {
+        const int at = first_of(i) + part_of * 32;
+        if (at < own.lo || at + 32 > own.hi) bits = span_bits(own, at);
+      } else if (MODE == kListed) {
         bits = c.bits[i].w[part_of];
       } else if (i + 1 == tiles && end % F::kStep) {
         const int left = end % F::kStep - part_of * 32;

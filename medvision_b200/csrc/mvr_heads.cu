@@ -9,9 +9,7 @@
 #include <type_traits>
 
 #include "../../include/mvr.h"
-#include "mvr_attn_fma.cuh"
-#include "mvr_attn_tc.cuh"
-#include "mvr_attn_tc_bwd.cuh"
+#include "mvr_attn_host.cuh"
 #include "mvr_dropout.cuh"
 #include "mvr_logprob.cuh"
 
@@ -19,50 +17,19 @@ namespace {
 
 using namespace mvr;
 
-bool head_dtype(int t) { return t == MVR_F32 || t == MVR_F16 || t == MVR_BF16; }
-
-int launched() { return cudaGetLastError() == cudaSuccess ? MVR_OK : MVR_ERR_LAUNCH; }
-
 // ---- attention ----------------------------------------------------------------------------------------
 
-constexpr int kMultiprocessors = 148;
 constexpr size_t kPlanShared = 200 * 1024;
 
 // How a call is cut into CTAs, and what lies where in its workspace.
-struct AttnCut {
+struct AttnCut : OperandPieces {
   bool tc;                      // tensor cores (mvr_attn_tc.cuh); float operands in pieces
   bool direct;                  // few regions: the kernel finds those of an image itself
-  int W;                        // columns of the operands in memory
   int tile, kv_tile;            // rows and states of a CTA's tile
   long long row_tiles;          // tiles of rows per key head: exact without an index, else no call has more
   int splits, row_splits;
-  long long order, starts, tiles, delta, norm, peaks, row_peaks, q, k, v, g, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
+  long long order, starts, tiles, delta, norm, peaks, row_peaks, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
-
-long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
-
-// What a kernel takes for one of its steps (a tile of rows against a tile of states), in us, measured: `full` of an SM with all the
-// CTAs that it holds (`resident`), `alone` of a CTA by itself.
-struct StepTime {
-  int resident;
-  double full, alone;
-};
-
-// Parts into which to cut the `steps` steps of `ctas` CTAs so that they end soonest: the SMs' CTAs one after another at the full rate,
-// or, where an SM has few, one CTA's own chain; 1 us a CTA for its beginning and end.  Where CTAs differ in length (`uneven`: lengths
-// or a mask), half a part is lost at the end.  Joining takes 3 us and `join` us a part.
-int best_parts(long long ctas, long long steps, const StepTime& t, double join, bool uneven) {
-  int best = 1;
-  double least = 0;
-  for (long long s = 1; s <= std::min<long long>(64, std::max<long long>(1, steps)); ++s) {
-    const long long per = cdiv(steps, s), on_sm = cdiv(ctas * s, kMultiprocessors), rounds = cdiv(on_sm, t.resident);
-    if (s > 1 && cdiv(steps, per) < s) continue;  // a part would have nothing
-    const double time = std::max(on_sm * (per * t.full + 1.0 / t.resident), rounds * (per * t.alone + 1.0)) + (uneven ? per * t.alone / 2 : 0) +
-                        (s > 1 ? 3 + join * s : 0);
-    if (s == 1 || time < 0.92 * least) best = (int)s, least = time;
-  }
-  return best;
-}
 
 AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   AttnCut c = {};
@@ -79,13 +46,10 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   const long long kv_tiles = std::max<long long>(1, cdiv(a->L, c.kv_tile));
   const long long expected = std::max<long long>(1, a->has_index ? cdiv(rows_of_image, c.tile) * a->N : c.row_tiles) * a->Hk;
   const bool wide = a->D > 64, uneven = a->lengths || a->mask;
-  const StepTime walk = pieces ? (backward ? StepTime{1, 4.5, 4.5} : StepTime{2, 2.6, 4.0}) : !tc ? StepTime{2, 3.0, 4.0} : backward ? (wide ? StepTime{1, 2.0, 2.0} : StepTime{2, 1.25, 1.8})
-                        : c.tile > kTcRows ? StepTime{1, 2.1, 2.1} : wide ? StepTime{2, 1.5, 1.8} : StepTime{4, 0.85, 1.5};
   // (a part's sums are written and read at 4 MB/us)
-  c.splits = best_parts(expected, kv_tiles, walk, rows * a->D * 8 / 4e6, uneven);
+  c.splits = best_parts(expected, kv_tiles, states_step(tc, pieces, backward, wide, c.tile > kTcRows), rows * a->D * 8 / 4e6, uneven);
   if (tc) c.splits = (int)std::max<long long>(c.splits, cdiv(a->L, kTcMaxStates));
-  const StepTime walk_rows = pieces ? StepTime{1, 5.0, 5.0} : !tc ? StepTime{2, 5.0, 7.0} : wide ? StepTime{1, 2.6, 2.6} : StepTime{2, 1.7, 2.3};
-  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), walk_rows, (double)a->N * a->L * a->Hk * a->D * 16 / 4e6, false)
+  c.row_splits = backward ? best_parts(a->N * a->Hk * kv_tiles, cdiv(rows_of_image, c.tile), rows_step(tc, pieces, wide), (double)a->N * a->L * a->Hk * a->D * 16 / 4e6, false)
                           : 1;
   long long at = 0;
   const auto take = [&at](long long bytes) {
@@ -124,28 +88,12 @@ AttnCut cut_attention(const mvr_attention* a, bool backward, bool tc) {
   return c;
 }
 
-// Scores (rows times states) from which float operands in pieces are worth the launches that make them.  (Forward and backward, 4 x 16
-// rows over 1024 states, 4 heads of 32: 139 us, in float arithmetic 95; over 2048 states, 8 heads of 64: 146 and 239.)
-constexpr double kPieceScores = 1 << 19;
-
 // Whether type and sizes are the tensor cores'; the operands' alignment is a matter of the call.
 bool tc_sizes(const mvr_attention* a) {
   const double rows = (double)a->R * a->T * a->Hq;
   if (a->L == 0 || a->N == 0 || a->L > 64LL * kTcMaxStates || a->N > INT32_MAX / 4 || rows > 2e9) return false;
   return a->dtype == MVR_F32 ? a->D <= 64 && rows * a->L >= kPieceScores : a->D % 8 == 0 && a->D <= 128;
 }
-bool rows_aligned(const void* base, const int64_t (&strides)[3], const mvr_attention* a) {
-  const int64_t sizes[3] = {a->R, a->T, a->Hq};
-  if ((uintptr_t)base % 16 != 0) return false;
-  int64_t last = 0;
-  for (int i = 0; i < 3; ++i) {
-    if (sizes[i] <= 1) continue;
-    if (strides[i] % 8 != 0 || strides[i] < 0 || strides[i] > INT64_MAX / 4 / sizes[i]) return false;
-    last += (sizes[i] - 1) * strides[i];
-  }
-  return last / 8 < 0xffffffffLL;  // (rows are found by 32-bit numbers of 16 bytes)
-}
-
 int check_attention(const mvr_attention* a, bool backward, bool sizes_only) {
   if (!a) return MVR_ERR_NULL;
   if (!head_dtype(a->dtype)) return MVR_ERR_DTYPE;
@@ -197,31 +145,6 @@ AttnParams attention_params(const mvr_attention* a, const AttnCut& c, char* ws) 
   return p;
 }
 
-// Lets a kernel have `smem` bytes of dynamic shared memory, once per device.  (The same limit in every call of a kernel: calls of
-// several threads do not undo one another's.)
-template <auto KERNEL>
-bool shared_memory(size_t smem) {
-  static std::atomic<uint64_t> done{0};  // a bit per device
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (device & 63);
-  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
-  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  if (device < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-
-template <auto KERNEL, typename... A>
-int launch_shared(dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  if (grid.x == 0 || grid.y == 0) return MVR_OK;
-  if (!shared_memory<KERNEL>(smem)) return MVR_ERR_LAUNCH;
-  launch_dependent(KERNEL, grid, dim3(threads), smem, st, args...);
-  return launched();
-}
-
 int plan_attention(const mvr_attention* a, const AttnCut& c, char* ws, int* status, cudaStream_t st) {
   if (!a->has_index || c.direct) return MVR_OK;
   const int groups = (int)a->N + 1;
@@ -247,49 +170,19 @@ int fma_backward(const AttnParams& p, const AttnCut& c, cudaStream_t st) {
   return launch_shared<attn_fma_dkv<T, DP>>(dim3((unsigned)(cdiv(p.L, c.kv_tile) * p.N), p.Hk, c.row_splits), kFmaThreads, FmaTile<DP>::bytes(4), st, p);
 }
 
-unsigned blocks_of(long long n, int per) { return (unsigned)std::min<long long>(cdiv(n, per), 1 << 20); }
-
-template <typename T>
-int sum_parts(const float* part, void* dst, long long n, int parts, float factor, cudaStream_t st) {
-  if (n == 0) return MVR_OK;
-  if (n % 4 == 0 && (uintptr_t)dst % (4 * sizeof(T)) == 0)
-    launch_dependent(attn_sum<T, 4>, dim3(blocks_of(n, 1024)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
-  else
-    launch_dependent(attn_sum<T, 1>, dim3(blocks_of(n, 256)), dim3(256), 0, st, part, (T*)dst, n, parts, factor);
-  return launched();
-}
-
-template <typename T, int DP, int TILES, bool MASK, int PIECES>
+template <typename T, int DP, int TILES, int MODE, int PIECES>
 int tc_forward_as(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
-  typedef TcForward<DP, TILES, MASK, PIECES> F;
-  return launch_shared<attn_tc_fwd<T, DP, TILES, MASK, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);
+  typedef TcForward<DP, TILES, MODE, PIECES> F;
+  return launch_shared<attn_tc_fwd<T, DP, TILES, MODE, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);
 }
 template <typename T, int DP, int PIECES>
 int tc_forward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   const bool mask = p.mask || p.lengths;
   if constexpr (DP == 128) {
     if (c.tile > kTcRows)
-      return mask ? tc_forward_as<T, DP, 2, true, 1>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, false, 1>(p, c, maps, status, st);
+      return mask ? tc_forward_as<T, DP, 2, kListed, 1>(p, c, maps, status, st) : tc_forward_as<T, DP, 2, kAll, 1>(p, c, maps, status, st);
   }
-  return mask ? tc_forward_as<T, DP, 1, true, PIECES>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, false, PIECES>(p, c, maps, status, st);
-}
-
-template <typename T>
-bool tensor_maps(const mvr_attention* a, bool backward, int pieces, TcMaps& maps, bool& boxes) {
-  tc_need_context();
-  const int D = (int)a->D, G = (int)(a->Hq / a->Hk);
-  const auto states = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-    return tc_map<T>(m, base, D, (int)a->Hk, (int)a->L, (int)a->N * pieces, s[2], s[1], s[0], 1, kTcBox);
-  };
-  if (!states(&maps.k, a->k, a->k_strides) || !states(&maps.v, a->v, a->v_strides)) return false;
-  const int step = D <= 64 ? kGradStep<64> : kGradStep<128>;
-  if (backward && !a->has_index && a->R > 0 && a->T > 0 && step % G == 0) {
-    const auto rows = [&](CUtensorMap* m, const void* base, const int64_t (&s)[3]) {
-      return tc_map<T>(m, base, D, (int)a->Hq, (int)a->T, (int)a->R * pieces, s[2], s[1], s[0], G, step / G);
-    };
-    boxes = rows(&maps.q, a->q, a->q_strides) && rows(&maps.g, a->grad_out, a->g_strides);
-  }
-  return true;
+  return mask ? tc_forward_as<T, DP, 1, kListed, PIECES>(p, c, maps, status, st) : tc_forward_as<T, DP, 1, kAll, PIECES>(p, c, maps, status, st);
 }
 
 template <typename T>
@@ -320,11 +213,11 @@ int tc_backward(const AttnParams& p, const AttnCut& c, const TcMaps& maps, bool 
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   const dim3 grid((unsigned)c.row_tiles, p.Hk, c.splits);
   if (p.mask || p.lengths) {
-    typedef TcRows<DP, true, PIECES> F;
-    return launch_shared<attn_tc_dq<T, DP, true, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
+    typedef TcRows<DP, kListed, PIECES> F;
+    return launch_shared<attn_tc_dq<T, DP, kListed, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
   }
-  typedef TcRows<DP, false, PIECES> F;
-  return launch_shared<attn_tc_dq<T, DP, false, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
+  typedef TcRows<DP, kAll, PIECES> F;
+  return launch_shared<attn_tc_dq<T, DP, kAll, PIECES>>(grid, F::kThreads, F::kShared, st, p, maps, status);
 }
 
 // plain: the call's own tensors, where the operands are in pieces.
@@ -358,33 +251,6 @@ int attention_backward(const AttnParams& p, const AttnParams& plain, const AttnC
   if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gk, p.gk, states, c.row_splits, p.scale, st);
   if (rc == MVR_OK && c.row_splits > 1) rc = sum_parts<T>(p.part_gv, p.gv, states, c.row_splits, 1.0f, st);
   return rc;
-}
-
-// Float operands of a call in pieces, in its workspace; `b` is the call on them.
-int split_operands(const mvr_attention* a, bool backward, const AttnCut& c, char* ws, mvr_attention& b, AttnParams& p, cudaStream_t st) {
-  const auto split = [&](const void* from, const int64_t (&s)[3], long long n0, long long n1, long long n2, long long to) {
-    const long long rows = n0 * n1 * n2;
-    if (rows > 0)
-      launch_dependent(split_floats, dim3((unsigned)cdiv(rows * (c.W / 8), 256)), dim3(256), 0, st, (const float*)from, (long long)s[0], (long long)s[1],
-                       (long long)s[2], (int)n1, (int)n2, rows, (int)a->D, c.W, (__nv_bfloat16*)(ws + to));
-    return launched();
-  };
-  int rc = split(a->q, a->q_strides, a->R, a->T, a->Hq, c.q);
-  if (rc == MVR_OK) rc = split(a->k, a->k_strides, a->N, a->L, a->Hk, c.k);
-  if (rc == MVR_OK) rc = split(a->v, a->v_strides, a->N, a->L, a->Hk, c.v);
-  if (rc == MVR_OK && backward) rc = split(a->grad_out, a->g_strides, a->R, a->T, a->Hq, c.g);
-  if (rc != MVR_OK) return rc;
-  b = *a;
-  b.D = c.W;
-  b.q = ws + c.q; b.k = ws + c.k; b.v = ws + c.v; b.grad_out = ws + c.g;
-  const int64_t W = c.W;
-  for (int64_t(*s)[3] : {&b.q_strides, &b.g_strides}) (*s)[0] = a->T * a->Hq * W, (*s)[1] = a->Hq * W, (*s)[2] = W;
-  for (int64_t(*s)[3] : {&b.k_strides, &b.v_strides}) (*s)[0] = a->L * a->Hk * W, (*s)[1] = a->Hk * W, (*s)[2] = W;
-  p.q = b.q; p.k = b.k; p.v = b.v; p.g = b.grad_out;
-  p.q_r = p.g_r = b.q_strides[0]; p.q_t = p.g_t = b.q_strides[1]; p.q_h = p.g_h = W;
-  p.k_n = p.v_n = b.k_strides[0]; p.k_l = p.v_l = b.k_strides[1]; p.k_h = p.v_h = W;
-  p.q_piece = p.g_piece = a->R * a->T * a->Hq * W;
-  return MVR_OK;
 }
 
 template <typename T>

@@ -49,7 +49,7 @@ constexpr unsigned long long kWaitLimit = 2000000000ull;  // 2 s: far above any 
 
 // Waits until the phase of the given parity has completed; false when it has not within the limit, or another thread of the CTA
 // has given up (`lost`, in shared memory).
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* lost) {
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* lost) {
   const unsigned long long begin = nanoseconds();
   for (;;) {
     if (*lost) return false;
@@ -299,7 +299,7 @@ __device__ __forceinline__ void pieces_of(float2 f, uint32_t& a, uint32_t& b, ui
 // takes eight columns.  An infinity is the largest bfloat16 of its sign, 0 and the infinity: the third piece meets nothing but the other
 // operand's first, so that no 0 among that one's smaller pieces makes a NaN of an infinite product, and the first piece gives infinity
 // times infinity.  NaN is the third piece alone.
-__global__ void __launch_bounds__(256) split_floats(const float* from, long long s0, long long s1, long long s2, int n1, int n2, long long rows,
+static __global__ void __launch_bounds__(256) split_floats(const float* from, long long s0, long long s1, long long s2, int n1, int n2, long long rows,
                                                     int D, int W, __nv_bfloat16* to) {
   grid_dependency();
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (W / 8);

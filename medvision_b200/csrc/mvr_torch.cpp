@@ -1177,7 +1177,7 @@ int* status_of(int index) { return status_ptr(index); }
 
 PyMODINIT_FUNC PyInit__native(void) {
   PyObject* m = PyModule_Create(&module);
-  if (m && PyModule_AddFunctions(m, mvr_host::head_methods()) < 0) {
+  if (m && (PyModule_AddFunctions(m, mvr_host::head_methods()) < 0 || PyModule_AddFunctions(m, mvr_host::encoder_methods()) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }

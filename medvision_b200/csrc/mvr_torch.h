@@ -14,5 +14,6 @@ void check(int rc);                       // throws what the library's code mean
 int* status_of(int device);               // the device's status word
 
 PyMethodDef* head_methods();              // functions of mvr_torch_heads.cpp
+PyMethodDef* encoder_methods();           // functions of mvr_torch_encoder.cpp
 
 }  // namespace mvr_host

@@ -1,89 +1,18 @@
-// Host path of the operators behind the roi modules (attention to an encoder's states, dropout, log-probabilities of labels):
+// Host path of the operators behind the roi modules (attention to an encoder's states or in a window, dropout, log-probabilities of labels):
 // argument checks, results, workspaces, autograd nodes and launches, in one native call per operation.
-#include <Python.h>
-
-#include <cmath>
-#include <memory>
-#include <mutex>
-#include <string>
-#include <vector>
-
-#include <ATen/ATen.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include "../../include/mvr.h"
-#include "mvr_torch.h"
+#include "mvr_torch_operators.h"
 
 namespace {
-
-using mvr_host::check;
-using mvr_host::type_name;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-int head_code(at::ScalarType t) {
-  return t == at::kFloat ? MVR_F32 : t == at::kHalf ? MVR_F16 : t == at::kBFloat16 ? MVR_BF16 : -1;
-}
-int index_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return MVR_INDEX_F32;
-    case at::kHalf: return MVR_INDEX_F16;
-    case at::kDouble: return MVR_INDEX_F64;
-    case at::kBFloat16: return MVR_INDEX_BF16;
-    case at::kInt: return MVR_INDEX_I32;
-    case at::kLong: return MVR_INDEX_I64;
-    case at::kShort: return MVR_INDEX_I16;
-    case at::kByte: return MVR_INDEX_U8;
-    default: return -1;
-  }
-}
-
-// Types and shapes are looked at before the device, so that a wrong call fails alike on every machine.
-void check_cuda(const char* what, const at::Tensor& t) { TORCH_CHECK(t.is_cuda(), what, " is not implemented on CPU"); }
-void check_type(const char* what, const at::Tensor& t) {
-  TORCH_CHECK(head_code(t.scalar_type()) >= 0, "\"", what, "\" not implemented for '", type_name(t.scalar_type()), "'");
-}
-void check_like(const at::Tensor& t, const at::Tensor& like) {
-  TORCH_CHECK(t.device() == like.device(), "expected all tensors to be on the same CUDA device");
-  TORCH_CHECK(t.scalar_type() == like.scalar_type(), "expected scalar type torch.", type_name(like.scalar_type()), " but found torch.",
-              type_name(t.scalar_type()));
-}
-void check_tangent(const char* what, const at::Tensor& t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !torch::autograd::impl::get_autograd_meta(t) || !t._fw_grad(/*level=*/0).defined(), what,
-                              " has no forward-mode derivative");
-}
-
-void* stream_of(const at::Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-void* data_or_null(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
-
-// The gradients were computed without a graph of their own: asking for one (create_graph) ends in an error, not in a silent 0.
-void once_differentiable(const char* what, variable_list& results, const variable_list& from) {
-  if (!at::GradMode::is_enabled()) return;
-  bool any = false;
-  for (const at::Tensor& t : from) any |= t.defined() && t.requires_grad();
-  if (!any) return;
-  for (at::Tensor& r : results) {
-    if (!r.defined()) continue;
-    r = r.detach();
-    auto node = std::make_shared<torch::autograd::Error>(std::string("the gradients of ") + what + " cannot be differentiated again",
-                                                         torch::autograd::collect_next_edges(from));
-    torch::autograd::set_history(r, node);
-  }
-}
 
 // ---- attention ------------------------------------------------------------------------------------------
 
 struct Attention {
   at::Tensor index, lengths, mask;  // or undefined
   double scale;
+  bool in_window = false;           // ops.window_attention: a window instead of index and mask
+  mvr_window window = {};           // without the address of `offsets`
+  at::Tensor offsets;               // or undefined
+  const char* name() const { return in_window ? "window_attention" : "cross_attention"; }
 };
 
 // A tensor of rows of D consecutive elements: the tensor itself, or a copy where its rows are apart in themselves or start where the
@@ -101,10 +30,12 @@ at::Tensor rows_of(const at::Tensor& t, bool states) {
 // Half types with a head size that is no multiple of 8, which TMA cannot read: in calls of some size the operands are copied with zeros
 // behind, which changes no product.  (Forward and backward, 33 columns, 4 heads: 16 x 49 rows over 4096 states 458 us, in the kernels
 // of float arithmetic 883 us; 2 x 16 rows over 256 states, where the copies' launches count, 429 and 88 us.)
-int64_t padded_size(const at::Tensor& q, const at::Tensor& k) {
+int64_t padded_size(const Attention& s, const at::Tensor& q, const at::Tensor& k) {
   const int64_t D = q.size(3), padded = (D + 7) / 8 * 8;
   if (q.scalar_type() == at::kFloat || D == padded || padded > 128) return D;
-  const double scores = (double)q.size(0) * q.size(1) * q.size(2) * k.size(1);
+  double states = (double)k.size(1);
+  if (s.in_window) states = std::min(states, (double)s.window.before + (double)s.window.after + 1 + (double)s.window.sinks);
+  const double scores = (double)q.size(0) * q.size(1) * q.size(2) * states;
   return scores >= 1 << 22 ? padded : D;
 }
 at::Tensor padded(const at::Tensor& t, int64_t D) { return t.size(3) == D ? t : at::constant_pad_nd(t, {0, D - t.size(3)}); }
@@ -138,15 +69,24 @@ mvr_attention describe(const Attention& s, const at::Tensor& q, const at::Tensor
   return a;
 }
 
-at::Tensor workspace_of(const mvr_attention& a, bool backward, const at::Tensor& like) {
+mvr_window window_of(const Attention& s) {
+  mvr_window w = s.window;
+  if (s.offsets.defined()) {
+    w.offsets = data_or_null(s.offsets);
+    w.offsets_64 = s.offsets.scalar_type() == at::kLong;
+  }
+  return w;
+}
+
+at::Tensor workspace_of(const Attention& s, const mvr_attention& a, bool backward, const at::Tensor& like) {
   int64_t bytes = 0;
-  check(mvr_attention_workspace(&a, backward, &bytes));
+  check(s.in_window ? mvr_window_attention_workspace(&a, &s.window, backward, &bytes) : mvr_attention_workspace(&a, backward, &bytes));
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
 }
 
 struct AttentionBackward : public torch::autograd::Node {
   Attention s;
-  SavedVariable q, k, v, out, lse, index, lengths, mask;
+  SavedVariable q, k, v, out, lse, index, lengths, mask, offsets;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -156,11 +96,12 @@ struct AttentionBackward : public torch::autograd::Node {
     args.index = index.unpack();
     args.lengths = lengths.unpack();
     args.mask = mask.unpack();
+    args.offsets = offsets.unpack();
     if (!grads[0].defined()) return result;
     {
       at::NoGradGuard no_grad;
       c10::cuda::CUDAGuard guard(q0.device());
-      const int64_t D = q0.size(3), wide = padded_size(q0, k0);
+      const int64_t D = q0.size(3), wide = padded_size(args, q0, k0);
       const at::Tensor qc = rows_of(padded(q0, wide), false), kc = rows_of(padded(k0, wide), true), vc = rows_of(padded(v0, wide), true),
                        oc = padded(o, wide);
       check_like(grads[0], q0);
@@ -175,29 +116,34 @@ struct AttentionBackward : public torch::autograd::Node {
       a.grad_q = data_or_null(gq);
       a.grad_k = data_or_null(gk);
       a.grad_v = data_or_null(gv);
-      const at::Tensor ws = workspace_of(a, true, gq);
-      check(mvr_attention_backward(&a, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
-                                   mvr_host::status_of(gq.device().index()), stream_of(gq)));
+      const at::Tensor ws = workspace_of(args, a, true, gq);
+      void* workspace = ws.defined() ? ws.data_ptr() : nullptr;
+      const int64_t bytes = ws.defined() ? ws.numel() : 0;
+      int* status = mvr_host::status_of(gq.device().index());
+      const mvr_window w = window_of(args);
+      check(args.in_window ? mvr_window_attention_backward(&a, &w, workspace, bytes, status, stream_of(gq))
+                           : mvr_attention_backward(&a, workspace, bytes, status, stream_of(gq)));
       result = {narrowed(gq, D), narrowed(gk, D), narrowed(gv, D)};
     }
-    once_differentiable("cross_attention", result, {grads[0], q0, k0, v0});
+    once_differentiable(s.name(), result, {grads[0], q0, k0, v0});
     for (int i = 0; i < 3; ++i)
       if (!task_should_compute_output(i)) result[i] = at::Tensor();
     return result;
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* t : {&q, &k, &v, &out, &lse, &index, &lengths, &mask}) t->reset_data();
+    for (SavedVariable* t : {&q, &k, &v, &out, &lse, &index, &lengths, &mask, &offsets}) t->reset_data();
   }
-  std::string name() const override { return "CrossAttentionBackward"; }
+  std::string name() const override { return s.in_window ? "WindowAttentionBackward" : "CrossAttentionBackward"; }
 };
 
-at::Tensor cross_attention(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, Attention s, bool default_scale) {
-  const char* what = "cross_attention";
+at::Tensor attention(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, Attention s, bool default_scale) {
+  const char* what = s.name();
   check_type(what, query);
   check_like(key, query);
   check_like(value, query);
-  TORCH_CHECK(query.dim() == 4 && key.dim() == 4, what, ": expected query (regions, tokens, heads, dim) and key (images, states, heads, dim)");
+  const char *regions = s.in_window ? "sequence" : "region", *images = s.in_window ? "sequence" : "image";
+  TORCH_CHECK(query.dim() == 4 && key.dim() == 4, what, ": expected query (", regions, "s, tokens, heads, dim) and key (", images, "s, states, heads, dim)");
   TORCH_CHECK(value.sizes() == key.sizes(), what, ": key and value must have the same shape");
   TORCH_CHECK(key.size(3) == query.size(3), what, ": query and key must have the same head size");
   TORCH_CHECK(query.size(3) >= 1 && query.size(2) >= 1 && key.size(2) >= 1, what, ": heads and head size must not be 0");
@@ -207,13 +153,20 @@ at::Tensor cross_attention(const at::Tensor& query, const at::Tensor& key, const
     TORCH_CHECK(s.index.dim() == 1 && s.index.size(0) == R, what, ": batch_index must have one element per region");
     TORCH_CHECK(index_code(s.index.scalar_type()) >= 0, what, ": batch_index cannot be of type ", type_name(s.index.scalar_type()));
   } else {
+    TORCH_CHECK(!s.in_window || R == N, what, ": query and key must be of the same sequences, but there are ", R, " and ", N);
     TORCH_CHECK(R == N, what, ": without batch_index there must be one region per image, but there are ", R, " and ", N);
   }
   if (s.lengths.defined()) {
     TORCH_CHECK(s.lengths.device() == query.device(), "expected all tensors to be on the same CUDA device");
-    TORCH_CHECK(s.lengths.dim() == 1 && s.lengths.size(0) == N, what, ": lengths must have one element per image");
+    TORCH_CHECK(s.lengths.dim() == 1 && s.lengths.size(0) == N, what, ": lengths must have one element per ", images);
     TORCH_CHECK(s.lengths.scalar_type() == at::kInt || s.lengths.scalar_type() == at::kLong, what, ": lengths must be int32 or int64");
   }
+  if (s.offsets.defined()) {
+    TORCH_CHECK(s.offsets.device() == query.device(), "expected all tensors to be on the same CUDA device");
+    TORCH_CHECK(s.offsets.dim() == 1 && s.offsets.size(0) == N, what, ": offsets must have one element per sequence");
+    TORCH_CHECK(s.offsets.scalar_type() == at::kInt || s.offsets.scalar_type() == at::kLong, what, ": offsets must be int32 or int64");
+  }
+  TORCH_CHECK(s.window.before >= 0 && s.window.after >= 0 && s.window.sinks >= 0, what, ": before, after and sinks must not be negative");
   if (s.mask.defined()) {
     TORCH_CHECK(s.mask.device() == query.device(), "expected all tensors to be on the same CUDA device");
     TORCH_CHECK(s.mask.dim() == 2 && s.mask.size(0) == N && s.mask.size(1) == L, what, ": mask must be (images, states)");
@@ -232,22 +185,30 @@ at::Tensor cross_attention(const at::Tensor& query, const at::Tensor& key, const
     c10::cuda::CUDAGuard guard(query.device());
     if (s.lengths.defined()) s.lengths = s.lengths.contiguous();
     if (s.mask.defined()) s.mask = s.mask.contiguous();
-    const int64_t D = query.size(3), wide = padded_size(query, key);
+    if (s.offsets.defined()) s.offsets = s.offsets.contiguous();
+    const int64_t D = query.size(3), wide = padded_size(s, query, key);
     const at::Tensor q = rows_of(padded(query, wide), false), k = rows_of(padded(key, wide), true), v = rows_of(padded(value, wide), true);
     mvr_attention a = describe(s, q, k, v);
-    const at::Tensor ws = workspace_of(a, false, q);
+    const at::Tensor ws = workspace_of(s, a, false, q);
     out = at::empty(q.sizes(), query.options().requires_grad(false));
     if (graph) lse = at::empty({R, query.size(1), query.size(2)}, out.options().dtype(at::kFloat));
     a.out = data_or_null(out);
     a.lse = (float*)data_or_null(lse);
-    check(mvr_attention_forward(&a, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
-                                mvr_host::status_of(query.device().index()), stream_of(query)));
+    void* workspace = ws.defined() ? ws.data_ptr() : nullptr;
+    const int64_t bytes = ws.defined() ? ws.numel() : 0;
+    int* status = mvr_host::status_of(query.device().index());
+    const mvr_window w = window_of(s);
+    check(s.in_window ? mvr_window_attention_forward(&a, &w, workspace, bytes, status, stream_of(query))
+                      : mvr_attention_forward(&a, workspace, bytes, status, stream_of(query)));
     out = narrowed(out, D);
   }
   if (graph) {
     auto node = std::shared_ptr<AttentionBackward>(new AttentionBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(query, key, value));
     node->s.scale = s.scale;
+    node->s.in_window = s.in_window;
+    node->s.window = s.window;
+    node->offsets = SavedVariable(s.offsets, false);
     node->q = SavedVariable(query, false);
     node->k = SavedVariable(key, false);
     node->v = SavedVariable(value, false);
@@ -507,20 +468,6 @@ LabelLogProbs label_log_probs(const at::Tensor& logits, const at::Tensor& labels
 
 // ---- Python ---------------------------------------------------------------------------------------------
 
-const at::Tensor& tensor_arg(PyObject* o, const char* name) {
-  if (!THPVariable_Check(o)) {
-    PyErr_Format(PyExc_TypeError, "%s must be a Tensor, not %s", name, Py_TYPE(o)->tp_name);
-    throw python_error();
-  }
-  return THPVariable_Unpack(o);
-}
-at::Tensor optional_tensor(PyObject* o, const char* name) { return o == Py_None ? at::Tensor() : tensor_arg(o, name); }
-
-double number_arg(PyObject* o) {
-  const double v = PyFloat_AsDouble(o);
-  if (v == -1.0 && PyErr_Occurred()) throw python_error();
-  return v;
-}
 // A whole number of 64 bits; negative ones stand for their two's complement.
 uint64_t word_arg(PyObject* o, const char* name) {
   PyObject* index = PyNumber_Index(o);
@@ -542,13 +489,6 @@ uint64_t word_arg(PyObject* o, const char* name) {
   return word;
 }
 
-void expect(Py_ssize_t n, Py_ssize_t want) {
-  if (n != want) {
-    PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", want, n);
-    throw python_error();
-  }
-}
-
 // cross_attention(query, key, value, batch_index, lengths, mask, scale)
 PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -562,7 +502,30 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor out;
   {
     pybind11::gil_scoped_release nogil;
-    out = cross_attention(q, k, v, s, a[6] == Py_None);
+    out = attention(q, k, v, s, a[6] == Py_None);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// window_attention(query, key, value, before, after, sinks, offsets, lengths, scale)
+PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 9);
+  const at::Tensor &q = tensor_arg(a[0], "query"), &k = tensor_arg(a[1], "key"), &v = tensor_arg(a[2], "value");
+  Attention s;
+  s.in_window = true;
+  s.window.before = whole_arg(a[3], "before");
+  s.window.after = whole_arg(a[4], "after");
+  s.window.sinks = whole_arg(a[5], "sinks");
+  if (THPVariable_Check(a[6])) s.offsets = THPVariable_Unpack(a[6]);
+  else if (a[6] != Py_None) s.window.offset = whole_arg(a[6], "offsets");
+  s.lengths = optional_tensor(a[7], "lengths");
+  s.scale = a[8] == Py_None ? 0.0 : number_arg(a[8]);
+  at::Tensor out;
+  {
+    pybind11::gil_scoped_release nogil;
+    out = attention(q, k, v, s, a[8] == Py_None);
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -615,8 +578,8 @@ PyObject* py_label_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-#define FAST(f) (PyCFunction)(void (*)(void)) f, METH_FASTCALL
 PyMethodDef methods[] = {{"cross_attention", FAST(py_cross_attention), nullptr},
+                         {"window_attention", FAST(py_window_attention), nullptr},
                          {"dropout", FAST(py_dropout), nullptr},
                          {"label_log_probs", FAST(py_label_log_probs), nullptr},
                          {nullptr, nullptr, 0, nullptr}};
