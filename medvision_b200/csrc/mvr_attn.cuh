@@ -16,18 +16,6 @@
 
 namespace mvr {
 
-// Division of numbers below 2^31 by a constant of the launch: a product and a shift.
-struct Divisor {
-  unsigned d, factor, shift;
-  void set(unsigned divisor) {
-    d = divisor;
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    factor = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ int quotient(int n) const { return (int)((__umulhi((unsigned)n, factor) + (unsigned)n) >> shift); }
-};
-
 struct AttnParams {
   const void *q, *k, *v, *g;                     // g: gradient of the output (backward)
   void *out, *gq, *gk, *gv;                      // out, gq: (R, T, Hq, D); gk, gv: (N, L, Hk, D); all contiguous

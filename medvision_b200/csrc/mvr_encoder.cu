@@ -26,11 +26,11 @@ constexpr int kMultiprocessors = 148;
 
 // How a call is cut: by clusters of `chunks` CTAs, each with its rows in shared memory, or in passes over chunks of rows.
 struct NormCut {
-  bool clusters;
-  int V, columns, lanes, depth, blocks, chunks;
+  bool clusters, whole;  // whole: every vector lies in one group
+  int V, block_groups, blocks, columns, lanes, depth, chunks;
   long long rows;
   size_t shared;
-  long long part, means, bytes;
+  long long sums, slopes, bytes;
 };
 
 int vector_of(const mvr_group_norm* a, bool backward) {
@@ -47,33 +47,36 @@ constexpr size_t kNormShared = 200 * 1024;
 NormCut cut_norm(const mvr_group_norm* a, bool backward, int V) {
   NormCut c = {};
   c.V = V;
-  c.columns = (int)(a->C / V);
-  const int width = (int)(a->C / a->groups), elements = backward ? 2 : 1, entry = (int)(backward ? sizeof(float2) : sizeof(Moments));
-  const double bytes = (double)a->N * a->S * a->C * size_of(a->dtype);
-  // Passes: 3 launches, and memory at some 5 MB/us; the second read finds what fits L2.
-  double least = 7 + bytes * (backward ? 3 : 2) / 5e6 + bytes * elements / (bytes * elements < 80e6 ? 10e6 : 5e6);
+  const int width = (int)(a->C / a->groups), element = size_of(a->dtype), operands = backward ? 2 : 1;
+  c.whole = width % V == 0;
+  const int told = backward ? V * (int)sizeof(float2) : (c.whole ? 1 : V) * (int)sizeof(Moments);  // bytes of a thread's sums
+  const double bytes = (double)a->N * a->S * a->C * element;
+  // Times in us, measured from 0.5 to 268 MB of x.  Passes: 8.5 + 0.43 a MB (0.54 beyond L2), backward 9 + 1.0 (float: 0.65).  Clusters: 2 (4),
+  // 1.3 more where CTAs tell each other their sums, and for each wave 2.2 (3) and 0.06 a KB that an SM brings into shared memory (pieces of
+  // a row below 32 bytes: 0.1).  A wave: two CTAs an SM, of clusters of 4 and 8 as many as 128 and 96 SMs hold.  (2 x 4096 rows of 128 halves:
+  // clusters 7.2, passes 10.3; 2 x 32768 of 64: 13.2, 11.4; 8 x 1000 of 512: 8.0, 12.0.)
+  double least = backward ? 9 + bytes * (element == 2 ? 1.0e-6 : 0.65e-6) : 8.5 + bytes * (bytes < 60e6 ? 0.43e-6 : 0.54e-6);
   for (int groups = 1; groups <= a->groups; ++groups) {
     const long long channels = (long long)groups * width;
-    if (a->groups % groups != 0 || channels % V != 0 || channels / V > kNormThreads) continue;
+    if (channels / V > kNormThreads) break;
+    if (a->groups % groups != 0 || channels % V != 0) continue;
     for (int size = 1; size <= 8; size *= 2) {
-      const int lanes = (int)(channels / V), depth = (int)std::min<long long>(kNormThreads / lanes, std::max<long long>(1, cdiv(a->S, size)));
-      const long long rows = cdiv(a->S, size), data = cdiv(rows, depth) * depth * lanes * V * size_of(a->dtype) * elements;
-      const size_t shared = (size_t)(((depth + 1) * channels * entry + groups * 8 + 15) / 16 * 16 + data);
-      if (shared > kNormShared || (size > 1 && rows < 2 * depth)) continue;
-      const long long ctas = a->N * (a->groups / groups) * size;
-      if (ctas > INT32_MAX) continue;
-      // An SM's CTAs together take a wave; each waits some 3 us for its loads and its group's sums, 1.5 more in a cluster.  Row pieces below
-      // 64 bytes use the memory badly.
-      const int resident = (int)std::min<long long>(8, 220 * 1024 / (long long)(shared + 1024));
-      const double waves = std::max(1.0, (double)ctas / (kMultiprocessors * resident)), piece = (double)channels * size_of(a->dtype);
-      const double time = 2 + std::ceil(waves) * (3 + (size > 1 ? 1.5 : 0)) +
-                          std::max(bytes * (elements + 1) / 5e6, waves * resident * (double)data * (elements + 1) / elements / 40e3) * (piece < 32 ? 2 : piece < 64 ? 1.3 : 1);
+      const long long rows = cdiv(a->S, size);
+      const int lanes = (int)(channels / V), depth = (int)std::min<long long>(kNormThreads / lanes, rows);
+      const long long data = cdiv(rows, depth) * depth * channels * element * operands, ctas = a->N * (a->groups / groups) * size;
+      if (data > (long long)kNormShared || ctas > INT32_MAX) continue;
+      const size_t shared = (size_t)(NormShared::bytes(depth * lanes * told, groups) + data);
+      if (shared > kNormShared || (size > 1 && (size - 1) * rows >= a->S)) continue;
+      const int multiprocessors = size == 8 ? 96 : size == 4 ? 128 : kMultiprocessors;
+      const long long on_sm = cdiv(ctas, multiprocessors), resident = std::min<long long>(2, 220 * 1024 / (long long)(shared + 1024));
+      const double time = (backward ? 4 : 2) + (size > 1 ? 1.3 : 0) + (double)cdiv(on_sm, resident) * (backward ? 3 : 2.2) +
+                          (double)on_sm * data * (channels * element < 32 ? 0.1e-3 : 0.06e-3);
       if (time < least) {
         least = time;
         c.clusters = true;
-        c.lanes = lanes;
+        c.block_groups = groups;
+        c.lanes = c.columns = lanes;
         c.depth = depth;
-        c.blocks = (int)(a->groups / groups);
         c.chunks = size;
         c.rows = rows;
         c.shared = shared;
@@ -81,24 +84,31 @@ NormCut cut_norm(const mvr_group_norm* a, bool backward, int V) {
     }
   }
   if (!c.clusters) {
+    // blocks of up to 512 bytes of a row, if groups are not wider, and 64 groups
+    for (int groups = 1; groups <= a->groups; ++groups) {
+      if (a->groups % groups != 0 || (long long)groups * width % V != 0) continue;
+      if (c.block_groups > 0 && (groups > 64 || (long long)groups * width * element > 512)) break;
+      c.block_groups = groups;
+    }
+    c.columns = (int)((long long)c.block_groups * width / V);
     c.lanes = std::min(c.columns, kNormThreads);
     c.depth = kNormThreads / c.lanes;
-    c.blocks = (int)cdiv(c.columns, c.lanes);
-    // some six CTAs an SM, each with four rows a thread at least
-    const long long most = std::max<long long>(1, cdiv(a->S, 4 * c.depth)), want = cdiv(6 * kMultiprocessors, std::max<long long>(1, a->N * c.blocks));
-    c.chunks = (int)std::min<long long>({most, std::max<long long>(1, want), 1 << 16});
+    // all CTAs at once, two an SM, each with two rows a thread at least; and no more sums than a CTA of the second pass can look at
+    const long long blocks = a->groups / c.block_groups, all = std::max<long long>(1, 2 * kMultiprocessors / std::max<long long>(1, a->N * blocks));
+    c.chunks = (int)std::max<long long>(1, std::min({all, cdiv(a->S, 2 * c.depth), 8192LL / c.block_groups}));
     c.rows = cdiv(std::max<long long>(1, a->S), c.chunks);
     c.chunks = (int)std::max<long long>(1, cdiv(a->S, c.rows));
-    c.shared = (size_t)c.depth * c.lanes * V * entry;
+    c.shared = (size_t)c.depth * c.lanes * told;
   }
+  c.blocks = (int)(a->groups / c.block_groups);
   long long at = 0;
   const auto take = [&at](long long n) {
     const long long here = at;
     at += (n + 255) / 256 * 256;
     return here;
   };
-  if (!c.clusters || backward) c.part = take(a->N * (c.clusters ? 1 : c.chunks) * a->C * entry);
-  if (!c.clusters && backward) c.means = take(a->N * a->groups * 8);
+  if (!c.clusters) c.sums = take(a->N * c.chunks * a->groups * (backward ? 8 : 16));
+  if (backward) c.slopes = take(a->N * (c.clusters ? 1 : c.chunks) * a->C * 8);
   c.bytes = at;
   return c;
 }
@@ -123,18 +133,19 @@ NormParams norm_params(const mvr_group_norm* a, const NormCut& c, char* ws) {
   p.x = a->x; p.dy = a->grad_out; p.weight = a->weight; p.bias = a->bias;
   p.out = a->out; p.dx = a->grad_x; p.dweight = a->grad_weight; p.dbias = a->grad_bias;
   p.mean = a->mean; p.rstd = a->rstd;
-  p.moments = (Moments*)(ws + c.part); p.part = (float2*)(ws + c.part); p.means = (float2*)(ws + c.means);
+  p.moments = (Moments*)(ws + c.sums); p.sums = (float2*)(ws + c.sums); p.slopes = (float2*)(ws + c.slopes);
   p.S = a->S; p.rows = c.rows;
   p.N = (int)a->N; p.C = (int)a->C; p.groups = (int)a->groups; p.width = (int)(a->C / a->groups);
   p.parameters = a->parameter_dtype;
-  p.chunks = c.chunks; p.columns = c.columns; p.lanes = c.lanes; p.depth = c.depth; p.blocks = c.blocks;
+  p.by_width.set((unsigned)p.width);
+  p.chunks = c.chunks; p.blocks = c.blocks; p.block_groups = c.block_groups; p.columns = c.columns; p.lanes = c.lanes; p.depth = c.depth;
   p.eps = a->eps;
   return p;
 }
 
-// A kernel of clusters, with as much shared memory as it asks for (the limit is raised once per device).
+// Lets a kernel have as much shared memory as any call of it asks for, once per device, and launches it, in clusters of `size` CTAs.
 template <auto KERNEL>
-int launch_cluster(const NormParams& p, const NormCut& c, cudaStream_t st) {
+int launch_norm(const NormParams& p, long long ctas, size_t shared, int size, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return MVR_ERR_LAUNCH;
@@ -147,48 +158,53 @@ int launch_cluster(const NormParams& p, const NormCut& c, cudaStream_t st) {
     if (device < 64) done.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)p.N * c.blocks * c.chunks));
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kNormThreads);
-  cfg.dynamicSmemBytes = c.shared;
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = c.chunks;
+  attr[1].val.clusterDim.x = size;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = size > 1 ? 2 : 1;
   cudaLaunchKernelEx(&cfg, KERNEL, p);
   return launched();
 }
 
-template <typename T, int V, int ACT>
-int norm_as(const NormParams& p, const NormCut& c, bool backward, cudaStream_t st) {
-  const dim3 grid((unsigned)((long long)p.N * c.chunks * c.blocks)), threads(kNormThreads);
-  const int group_ctas = p.N * p.groups, channel_ctas = p.dweight || p.dbias ? (int)cdiv(p.C, 32) : 0;
+template <typename T, int V, bool WHOLE, int ACT>
+int norm_as(NormParams& p, const NormCut& c, bool backward, cudaStream_t st) {
+  const long long ctas = (long long)p.N * c.chunks * c.blocks;
+  const int channel_ctas = p.dweight || p.dbias ? (int)cdiv(p.C, 32) : 0;
+  // (the second passes: two numbers a group, and what the threads have joined)
+  const size_t joined = std::max<size_t>(kNormThreads, c.block_groups), groups = (size_t)c.block_groups * 8 + 16;
+  int rc;
   if (!backward) {
-    if (c.clusters) return launch_cluster<norm_cluster<T, V, ACT>>(p, c, st);
-    launch_dependent(norm_stats<T, V>, grid, threads, c.shared, st, p);
-    launch_dependent(norm_finish, dim3((unsigned)group_ctas), threads, 0, st, p);
-    launch_dependent(norm_apply<T, V, ACT>, grid, threads, 0, st, p);
-    return launched();
+    if (c.clusters) return launch_norm<norm_cluster<T, V, WHOLE, ACT>>(p, ctas, c.shared, c.chunks, st);
+    rc = launch_norm<norm_stats<T, V, WHOLE>>(p, ctas, c.shared, 1, st);
+    return rc != MVR_OK ? rc : launch_norm<norm_apply<T, V, WHOLE, ACT>>(p, ctas, groups + joined * sizeof(Moments), 1, st);
   }
   if (c.clusters) {
-    const int rc = launch_cluster<norm_cluster_backward<T, V, ACT>>(p, c, st);
+    rc = launch_norm<norm_cluster_backward<T, V, WHOLE, ACT>>(p, ctas, c.shared, c.chunks, st);
     if (rc != MVR_OK || channel_ctas == 0) return rc;
-    NormParams sums = p;
-    sums.chunks = 1;
-    launch_dependent(norm_sums_finish, dim3((unsigned)channel_ctas), threads, 0, st, sums, 0);
+    p.chunks = 1;
+    launch_dependent(norm_parameters, dim3((unsigned)channel_ctas), dim3(kNormThreads), 0, st, p);
     return launched();
   }
-  launch_dependent(norm_sums<T, V, ACT>, grid, threads, c.shared, st, p);
-  launch_dependent(norm_sums_finish, dim3((unsigned)(group_ctas + channel_ctas)), threads, 0, st, p, group_ctas);
-  launch_dependent(norm_dx<T, V, ACT>, grid, threads, 0, st, p);
-  return launched();
+  rc = launch_norm<norm_sums<T, V, WHOLE, ACT>>(p, ctas, c.shared, 1, st);
+  p.channel_ctas = channel_ctas;
+  return rc != MVR_OK ? rc : launch_norm<norm_dx<T, V, WHOLE, ACT>>(p, ctas + channel_ctas, groups + joined * sizeof(float2), 1, st);
+}
+template <typename T, int V, int ACT>
+int norm_as(NormParams& p, const NormCut& c, bool backward, cudaStream_t st) {
+  if constexpr (V > 1)
+    if (!c.whole) return norm_as<T, V, false, ACT>(p, c, backward, st);
+  return norm_as<T, V, true, ACT>(p, c, backward, st);
 }
 template <typename T, int V>
-int norm_with(const NormParams& p, const NormCut& c, int activation, bool backward, cudaStream_t st) {
+int norm_with(NormParams& p, const NormCut& c, int activation, bool backward, cudaStream_t st) {
   switch (activation) {
     case MVR_ACT_NONE: return norm_as<T, V, kNoActivation>(p, c, backward, st);
     case MVR_ACT_RELU: return norm_as<T, V, kRelu>(p, c, backward, st);
@@ -221,8 +237,8 @@ int group_norm(const mvr_group_norm* a, bool backward, void* workspace, int64_t 
   const int V = vector_of(a, backward);
   const NormCut c = cut_norm(a, backward, V);
   if (bytes < c.bytes || (c.bytes > 0 && !workspace)) return MVR_ERR_WORKSPACE;
-  if ((long long)a->N * c.chunks * c.blocks > INT32_MAX) return MVR_ERR_TOO_LARGE;
-  const NormParams p = norm_params(a, c, (char*)workspace);
+  if ((long long)a->N * c.chunks * c.blocks > INT32_MAX - (1 << 16)) return MVR_ERR_TOO_LARGE;
+  NormParams p = norm_params(a, c, (char*)workspace);
   switch (a->dtype) {
     case MVR_F32: return V == 4 ? norm_with<float, 4>(p, c, a->activation, backward, st) : norm_with<float, 1>(p, c, a->activation, backward, st);
     case MVR_F16:

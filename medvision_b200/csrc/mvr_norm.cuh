@@ -2,13 +2,19 @@
 //   xhat = (x - mean) rstd    z = xhat w + b    y = act(z)            mean, variance of an image's group: S * C / groups values
 //   dz = dy act'(z)    db = sum dz    dw = sum dz xhat    dx = rstd (dz w - m1 - xhat m2)    m1, m2: the group's means of dz w, dz w xhat
 //
-// Every pass walks rows with one vector of channels a thread, so that what belongs to a channel stays in registers.  Forward: per-channel
-// mean and sum of squares of every chunk of rows, their union per group, then the elements.  Backward: per-channel sums of dz and dz xhat
-// of every chunk, their union, then dx.  No atomics: each sum has one place and one order.
+// A CTA takes a block of whole groups and a chunk of an image's rows, a thread one vector of channels of every `depth`th row, so that what
+// belongs to a channel stays in registers.  Two ways:
+//   passes    one kernel for the chunks' sums per group, one that joins an image's chunks and walks the rows again, backwards: what was
+//             read last is the likeliest still in L2.  All CTAs run at once, so that a chunk is as long as the work allows and its sums
+//             are few (296 of an SM's two; some 38 KB that every CTA of the second kernel reads)
+//   clusters  where the rows of a block fit the shared memory of one to eight CTAs: these tell each other their sums and walk the rows a
+//             second time where they lie
+// No atomics: each sum has one place and one order.
 //
 // Statistics.  A thread sums x - k and (x - k)^2 about its own first value k of a channel, over its r rows.  If k lies far from the others,
 // the thread's sum of squares about its mean is itself at least (r - 1) / r of that distance's square, so that cancellation costs no
-// more than some r of its last bits, whatever the data's offset.  Threads, chunks and channels are joined by their means' differences, for
+// more than some r of its last bits, whatever the data's offset; the same holds where a thread joins threads or chunks about the first
+// one's mean.  Channels, threads and chunks are joined by their means' differences, for
 // which a mean is kept as two floats: rounded to one, means near 1e5 of values with a deviation of 2 put an error of 1e-4 into their variance.
 #pragma once
 #include "mvr_types.cuh"
@@ -17,31 +23,56 @@ namespace mvr {
 
 enum { kNoActivation = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
-// Mean, as a float and what its rounding left, and sum of squares about it.
+// Mean, as a float and what its rounding left, sum of squares about it, and of how many values.
 struct alignas(16) Moments {
-  float mean, rest, square, unused;
+  float mean, rest, square, count;
 };
 
 struct NormParams {
   const void *x, *dy, *weight, *bias;  // (N, S, C) twice; (C), or null: 1 and 0
   void *out, *dx, *dweight, *dbias;
   float *mean, *rstd;                  // (N, groups)
-  Moments* moments;                    // (N, chunks, C): forward
-  float2* part;                        // (N, chunks, C): backward, sums of dz and dz xhat
-  float2* means;                       // (N, groups): m1, m2
+  Moments* moments;                    // (N, chunks, groups): forward
+  float2 *sums, *slopes;               // (N, chunks, groups): sums of dz w, dz w xhat; (N, chunks, C): of dz, dz xhat
   long long S, rows;                   // rows of a chunk, or of a CTA of a cluster
   int N, C, groups, width;             // width: channels of a group
   int parameters;                      // type of weight and bias: 0 float, 1 half, 3 bfloat16
   int chunks;                          // of an image; or CTAs of a cluster
-  int columns, lanes, depth;           // vectors of a row; of those a CTA takes `lanes`, `depth` rows at a time
-  int blocks;                          // of lanes in a row
+  int blocks, block_groups, columns;   // of an image; groups and vectors of a block
+  int lanes, depth;                    // a CTA takes `lanes` vectors of `depth` rows at a time (clusters, nearly always: all of a block)
+  Divisor by_width;
+  int channel_ctas;                    // dx: the first CTAs sum the gradients of weights and biases
   float eps;
 };
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 384;
 
 __device__ __forceinline__ float parameter(const NormParams& p, const void* from, int c) {
   return p.parameters == 0 ? ((const float*)from)[c] : p.parameters == 1 ? to_float(((const __half*)from)[c]) : to_float(((const __nv_bfloat16*)from)[c]);
+}
+// V neighbouring ones, all under way together.
+template <typename PT, int V>
+__device__ __forceinline__ void load_parameters(float (&to)[V], const void* from, int c) {
+  PT v[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = ((const PT*)from)[c + k];
+#pragma unroll
+  for (int k = 0; k < V; ++k) to[k] = to_float(v[k]);
+}
+template <int V>
+__device__ __forceinline__ void parameters_of(const NormParams& p, float (&weight)[V], float (&bias)[V], int c) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) weight[k] = 1.0f, bias[k] = 0.0f;
+  if (p.parameters == 0) {
+    if (p.weight) load_parameters<float>(weight, p.weight, c);
+    if (p.bias) load_parameters<float>(bias, p.bias, c);
+  } else if (p.parameters == 1) {
+    if (p.weight) load_parameters<__half>(weight, p.weight, c);
+    if (p.bias) load_parameters<__half>(bias, p.bias, c);
+  } else {
+    if (p.weight) load_parameters<__nv_bfloat16>(weight, p.weight, c);
+    if (p.bias) load_parameters<__nv_bfloat16>(bias, p.bias, c);
+  }
 }
 __device__ __forceinline__ float weight_of(const NormParams& p, int c) { return p.weight ? parameter(p, p.weight, c) : 1.0f; }
 __device__ __forceinline__ void put_parameter(const NormParams& p, void* to, int c, float v) {
@@ -50,483 +81,707 @@ __device__ __forceinline__ void put_parameter(const NormParams& p, void* to, int
   else ((__nv_bfloat16*)to)[c] = from_float<__nv_bfloat16>(v);
 }
 
-// act(z), and act'(z).
-template <typename T, int ACT>
-__device__ __forceinline__ float activate(float z, float& slope) {
-  constexpr bool kExact = sizeof(T) == 4;  // (the fast forms are off by 2^-20 up to |z| = 10, a 2^-9 of half a step of float16)
-  if (ACT == kRelu) {
-    slope = z > 0.0f ? 1.0f : 0.0f;
-    return z > 0.0f || z != z ? z : 0.0f;
+// ---- pairs of values ----------------------------------------------------------------------------------
+// A vector of V elements as pairs of floats (V 1: half a pair).
+template <typename T, int V>
+struct Pairs {
+  static constexpr int kPairs = (V + 1) / 2;
+  float2 v[kPairs];
+  Pairs() = default;
+  __device__ __forceinline__ explicit Pairs(const Vec<T, V>& from) {
+    if constexpr (V == 1) v[0] = make_float2(to_float(from.v[0]), 0.0f);
+    else
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) v[k] = floats(((const Two<T>*)&from)[k]);
   }
-  if (ACT == kSilu) {
-    const float gate = kExact ? 1.0f / (1.0f + expf(-z)) : __fdividef(1.0f, 1.0f + __expf(-z));
-    slope = gate * fmaf(z, 1.0f - gate, 1.0f);
-    return z * gate;
+  __device__ __forceinline__ Vec<T, V> vector() const {
+    Vec<T, V> to;
+    if constexpr (V == 1) to.v[0] = from_float<T>(v[0].x);
+    else
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) ((Two<T>*)&to)[k] = rounded<T>(v[k]);
+    return to;
   }
-  if (ACT == kGelu) {
-    const float gate = normcdff(z);
-    slope = fmaf(z * 0.3989422804014327f, kExact ? expf(-0.5f * z * z) : __expf(-0.5f * z * z), gate);
-    return z * gate;
-  }
-  slope = 1.0f;
-  return z;
+};
+__device__ __forceinline__ float2 two(float f) { return make_float2(f, f); }
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse_of(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// A thread's place: its channels [channel, channel + V) and the rows of its chunk that it walks.
+// act(z), and act'(z).  Half types: exponentials and inverses by the function units (2^-20 of the result up to |z| = 10), the normal
+// distribution by formula 7.1.26 of Abramowitz and Stegun (1.5e-7), which shares its exponential with the slope.
+template <typename T, int ACT>
+__device__ __forceinline__ float2 activate(float2 z, float2& slope) {
+  constexpr bool kExact = sizeof(T) == 4;
+  if constexpr (ACT == kRelu) {
+    slope = make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
+    return make_float2(z.x > 0.0f || z.x != z.x ? z.x : 0.0f, z.y > 0.0f || z.y != z.y ? z.y : 0.0f);
+  } else if constexpr (ACT == kSilu) {
+    float2 gate;
+    if constexpr (kExact) {
+      gate = make_float2(1.0f / (1.0f + expf(-z.x)), 1.0f / (1.0f + expf(-z.y)));
+    } else {
+      const float2 t = mul2(z, two(-1.4426950408889634f)), d = add2(make_float2(exp2_of(t.x), exp2_of(t.y)), two(1.0f));
+      gate = make_float2(inverse_of(d.x), inverse_of(d.y));
+    }
+    const float2 y = mul2(z, gate);
+    slope = fma2(y, fma2(gate, two(-1.0f), two(1.0f)), gate);
+    return y;
+  } else if constexpr (ACT == kGelu) {
+    float2 gate, bell;  // distribution and density times sqrt(2 pi)
+    if constexpr (kExact) {
+      gate = make_float2(normcdff(z.x), normcdff(z.y));
+      bell = make_float2(expf(-0.5f * z.x * z.x), expf(-0.5f * z.y * z.y));
+    } else {
+      const float2 square = mul2(mul2(z, z), two(-0.7213475204444817f)), d = fma2(make_float2(fabsf(z.x), fabsf(z.y)), two(0.3275911f * 0.7071067811865476f), two(1.0f));
+      bell = make_float2(exp2_of(square.x), exp2_of(square.y));
+      const float2 t = make_float2(inverse_of(d.x), inverse_of(d.y));
+      float2 s = fma2(t, two(0.5f * 1.061405429f), two(0.5f * -1.453152027f));
+      s = fma2(s, t, two(0.5f * 1.421413741f));
+      s = fma2(s, t, two(0.5f * -0.284496736f));
+      s = fma2(s, t, two(0.5f * 0.254829592f));
+      s = mul2(mul2(s, t), bell);  // the part beyond |z|
+      gate = make_float2(z.x < 0.0f ? s.x : 1.0f - s.x, z.y < 0.0f ? s.y : 1.0f - s.y);
+    }
+    slope = fma2(mul2(z, two(0.3989422804014327f)), bell, gate);
+    return mul2(z, gate);
+  } else {
+    slope = two(1.0f);
+    return z;
+  }
+}
+
+// load(i) and then use(i, what it gave) for i < count, U loads under way together (a store between them would hold the next one up).
+template <int U, typename L, typename F>
+__device__ __forceinline__ void walk(int count, L&& load, F&& use) {
+  for (int i = 0; i < count; i += U) {
+    decltype(load(0)) v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < count) v[u] = load(i + u);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < count) use(i + u, v[u]);
+  }
+}
+
+// ---- who takes what -----------------------------------------------------------------------------------
 struct NormPlace {
-  int n, chunk, block, lane, depth, channel;
-  long long begin, end, row;  // of the chunk; its first one
-  bool in;
+  int n, chunk, block, lane, depth;
+  int group;                   // first group of the block
+  long long begin, end, row;   // of the chunk; the thread's first row
+  int count;                   // of its rows
 };
-// CTA `cta` of the grid: block of lanes, chunk, image.
-template <int V>
-__device__ __forceinline__ NormPlace norm_place(const NormParams& p, int cta, bool backwards = false) {
+__device__ __forceinline__ NormPlace norm_place(const NormParams& p, int n, int block, int chunk) {
   NormPlace t;
-  const int number = cta / p.blocks, chunk = number % p.chunks;
-  t.block = cta - number * p.blocks;
-  t.n = number / p.chunks;
-  t.chunk = backwards ? p.chunks - 1 - chunk : chunk;
+  t.n = n;
+  t.block = block;
+  t.chunk = chunk;
+  t.group = block * p.block_groups;
   t.depth = threadIdx.x / p.lanes;
   t.lane = threadIdx.x - t.depth * p.lanes;
-  const int column = t.block * p.lanes + t.lane;
-  t.in = t.depth < p.depth && column < p.columns;
-  t.channel = column * V;
-  t.begin = t.chunk * p.rows;
+  t.begin = chunk * p.rows;
   t.end = max(t.begin, min(p.S, t.begin + p.rows));
   t.row = t.begin + t.depth;
+  t.count = t.depth < p.depth && t.row < t.end ? (int)((t.end - t.row + p.depth - 1) / p.depth) : 0;
   return t;
 }
-
-// Per channel, what every depth has; f(values, their distance, place, channel) joins them.
-template <int V, typename E, typename F>
-__device__ __forceinline__ void by_channel(const NormParams& p, const NormPlace& t, E* norm_shared, const E (&mine)[V], F&& f) {
-  const int width = p.lanes * V;  // norm_shared: (depth, width)
-  if (t.depth < p.depth) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) norm_shared[t.depth * width + t.lane * V + k] = mine[k];
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < width; c += kNormThreads)
-    if (t.block * width + c < p.C) f(norm_shared + c, width, c, t.block * width + c);
+__device__ __forceinline__ NormPlace norm_place(const NormParams& p, int cta) {  // (passes)
+  const int image = cta / p.blocks, n = image / p.chunks;
+  return norm_place(p, n, cta - image * p.blocks, image - n * p.chunks);
 }
 
-// ---- forward ------------------------------------------------------------------------------------------
-__device__ __forceinline__ Moments moments_of(float a, float b, float square) {  // mean: a + b
-  const float mean = a + b, of_b = mean - a;
-  return {mean, (a - (mean - of_b)) + (b - of_b), square, 0.0f};
-}
-__device__ __forceinline__ float distance(const Moments& a, const Moments& b) { return (a.mean - b.mean) + (a.rest - b.rest); }
-
-// Sums about a pivot, of V channels.
-template <int V>
-struct NormMoments {
-  float pivot[V] = {}, sum[V] = {}, square[V] = {};
-  int count = 0;
-  template <typename T>
-  __device__ __forceinline__ void start(const Vec<T, V>& v) {
-    count = 1;
-#pragma unroll
-    for (int k = 0; k < V; ++k) pivot[k] = to_float(v.v[k]);
-  }
-  template <typename T>
-  __device__ __forceinline__ void add(const Vec<T, V>& v) {
-    ++count;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float d = to_float(v.v[k]) - pivot[k];
-      sum[k] += d;
-      square[k] = fmaf(d, d, square[k]);
-    }
-  }
-  __device__ __forceinline__ void get(Moments (&to)[V]) const {
-    const float inverse = count > 0 ? 1.0f / count : 0.0f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) to[k] = moments_of(pivot[k], sum[k] * inverse, fmaxf(0.0f, fmaf(-sum[k] * inverse, sum[k], square[k])));
-  }
-};
-// Of `rows` rows that `depth` threads took in turns, together.
-__device__ __forceinline__ Moments join_moments(const Moments* v, int width, int depth, int rows) {
-  const auto rows_of = [&](int i) { return (float)((rows - i + depth - 1) / depth); };
-  const Moments first = v[0];
-  float mean = 0.0f, m2 = 0.0f;  // (mean: from the first one's)
-  const int some = min(depth, rows);
-  for (int i = 0; i < some; ++i) mean = fmaf(rows_of(i), distance(v[i * width], first), mean);
-  mean /= (float)max(1, rows);
-  for (int i = 0; i < some; ++i) {
-    const float d = distance(v[i * width], first) - mean;
-    m2 += fmaf(rows_of(i) * d, d, v[i * width].square);
-  }
-  return moments_of(first.mean, first.rest + mean, m2);
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_stats(const __grid_constant__ NormParams p) {
-  extern __shared__ Moments norm_moments[];
-  grid_dependency();
-  const NormPlace t = norm_place<V>(p, blockIdx.x);
-  typedef Vec<T, V> Vector;
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  NormMoments<V> m;
-  if (t.in) {
-    long long r = t.row;
-    if (r < t.end) m.start(*(const Vector*)(x + r * p.C));
-#pragma unroll 4
-    for (r += p.depth; r < t.end; r += p.depth) m.add(*(const Vector*)(x + r * p.C));
-  }
-  Moments mine[V];
-  m.get(mine);
-  by_channel<V>(p, t, norm_moments, mine, [&](const Moments* v, int width, int, int channel) {
-    p.moments[((long long)t.n * p.chunks + t.chunk) * p.C + channel] = join_moments(v, width, p.depth, (int)(t.end - t.begin));
-  });
-}
-
-__device__ __forceinline__ float norm_sum(float v, float* shared) {  // over the CTA, the same in all threads
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float total = 0.0f;
-  for (int i = 0; i < kNormThreads / 32; ++i) total += shared[i];
-  return total;
-}
-
-// Statistics of a group of an image, from its channels' chunks.
-static __global__ void __launch_bounds__(kNormThreads) norm_finish(const __grid_constant__ NormParams p) {
-  __shared__ float shared[kNormThreads / 32];
-  grid_dependency();
-  const int n = blockIdx.x / p.groups, g = blockIdx.x - n * p.groups, entries = p.chunks * p.width;
-  const Moments* part = p.moments + (long long)n * p.chunks * p.C + g * p.width;
-  const auto at = [&](int e, float& rows) {
-    const int chunk = e / p.width;
-    rows = (float)min(p.rows, p.S - chunk * p.rows);
-    return part[(long long)chunk * p.C + (e - chunk * p.width)];
-  };
-  const Moments first = part[0];
-  const float all = (float)p.S * p.width;
-  float sum = 0.0f, rows;
-  for (int e = threadIdx.x; e < entries; e += kNormThreads) {
-    const Moments v = at(e, rows);
-    sum = fmaf(rows, distance(v, first), sum);
-  }
-  const float mean = norm_sum(sum, shared) / all;
-  float m2 = 0.0f;
-  for (int e = threadIdx.x; e < entries; e += kNormThreads) {
-    const Moments v = at(e, rows);
-    const float d = distance(v, first) - mean;
-    m2 += fmaf(rows * d, d, v.square);
-  }
-  m2 = norm_sum(m2, shared);
-  if (threadIdx.x == 0) {
-    p.mean[n * p.groups + g] = first.mean + (first.rest + mean);
-    p.rstd[n * p.groups + g] = 1.0f / sqrtf(m2 / all + p.eps);
-  }
-}
-
-// What belongs to a thread's channels.  mean, rstd: of the groups from `first` on.
-template <int V>
-struct NormChannels {
-  float mean[V], rstd[V], weight[V], bias[V];
-  __device__ __forceinline__ NormChannels(const NormParams& p, const NormPlace& t, const float* means, const float* rstds, int first) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = t.in ? t.channel + k : first * p.width, g = c / p.width - first;
-      mean[k] = means[g];
-      rstd[k] = rstds[g];
-      weight[k] = weight_of(p, c);
-      bias[k] = p.bias ? parameter(p, p.bias, c) : 0.0f;
-    }
-  }
-};
-
-template <typename T, int ACT, int V>
-__device__ __forceinline__ Vec<T, V> normalised(Vec<T, V> v, const NormChannels<V>& c) {
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    float slope;
-    v.v[k] = from_float<T>(activate<T, ACT>(fmaf((to_float(v.v[k]) - c.mean[k]) * c.rstd[k], c.weight[k], c.bias[k]), slope));
-  }
-  return v;
-}
-
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_apply(const __grid_constant__ NormParams p) {
-  grid_dependency();
-  // (an image's last chunks were read last, and are the likeliest still in L2)
-  const NormPlace t = norm_place<V>(p, blockIdx.x, true);
-  const NormChannels<V> c(p, t, p.mean + (long long)t.n * p.groups, p.rstd + (long long)t.n * p.groups, 0);
-  if (!t.in) return;
-  typedef Vec<T, V> Vector;
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  T* out = (T*)p.out + t.n * p.S * p.C + t.channel;
-#pragma unroll 4
-  for (long long r = t.row; r < t.end; r += p.depth) *(Vector*)(out + r * p.C) = normalised<T, ACT>(*(const Vector*)(x + r * p.C), c);
-}
-
-// ---- clusters -----------------------------------------------------------------------------------------
-// Where an image's block of whole groups fits the shared memory of a cluster's CTAs (or of one CTA), one kernel does it all: each CTA
-// brings its rows into shared memory, the CTAs tell each other their channels' sums, and the rows are read a second time where they lie.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float2 of_cluster(const float2* mine, int rank) {  // the same place in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t at_rank(const void* mine, int rank) {  // the same place in another CTA of the cluster
   uint32_t at;
-  float2 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
+  return at;
 }
 __device__ __forceinline__ Moments of_cluster(const Moments* mine, int rank) {
-  uint32_t at;
-  Moments v = {};
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.mean), "=f"(v.rest), "=f"(v.square), "=f"(v.unused) : "r"(at) : "memory");
+  Moments v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.mean), "=f"(v.rest), "=f"(v.square), "=f"(v.count) : "r"(at_rank(mine, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+__device__ __forceinline__ float2 of_cluster(const float2* mine, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at_rank(mine, rank)) : "memory");
   return v;
 }
-// Shared memory of a CTA: what each depth tells (depth, lanes V), its channels (lanes V), its groups' two numbers, then the rows.
-template <typename E, int V>
-struct NormShared {
-  E *told, *channels;
-  float *first, *second;
-  char* rows;
-  __device__ __forceinline__ NormShared(const NormParams& p, char* base) {
-    const int width = p.lanes * V, groups = width / p.width;
-    told = (E*)base;
-    channels = told + p.depth * width;
-    first = (float*)(channels + width);
-    second = first + groups;
-    rows = base + bytes(p.depth, width, groups);
+
+// A team of neighbouring threads, at most a warp, for every group of a block.
+struct NormTeam {
+  int size, lane, first, teams;
+  __device__ __forceinline__ NormTeam(int groups, int entries) {  // (of a group)
+    size = 32;
+    while (size > 1 && (kNormThreads / size < groups || size >= 2 * entries)) size >>= 1;
+    lane = threadIdx.x & (size - 1);
+    first = threadIdx.x / size;
+    teams = kNormThreads / size;
   }
-  static __host__ __device__ __forceinline__ int bytes(int depth, int width, int groups) { return ((int)sizeof(E) * (depth + 1) * width + groups * 8 + 15) & ~15; }
+  __device__ __forceinline__ float sum(float v) const {  // (all threads of a warp)
+    for (int d = size >> 1; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+    return v;
+  }
+  // f(g, there) for every group; all threads call it alike often
+  template <typename F>
+  __device__ __forceinline__ void each(int groups, F&& f) const {
+    for (int g = first; g - first < groups; g += teams) f(g < groups ? g : groups - 1, g < groups);
+  }
 };
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_cluster(const __grid_constant__ NormParams p) {
-  extern __shared__ __align__(16) char norm_bytes[];
-  typedef Vec<T, V> Vector;
-  const NormShared<Moments, V> sh(p, norm_bytes);
-  // (block, image, CTA of the cluster)
-  NormPlace t = norm_place<V>(p, blockIdx.x / p.chunks % p.blocks + p.blocks * (blockIdx.x % p.chunks + p.chunks * (blockIdx.x / p.chunks / p.blocks)));
-  const int width = p.lanes * V, groups = width / p.width, first = t.block * groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dependency();
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  T* out = (T*)p.out + t.n * p.S * p.C + t.channel;
-  Vector* rows = (Vector*)sh.rows + t.depth * p.lanes + t.lane;  // of this thread
-  NormMoments<V> m;
-  if (t.in) {
-    int i = 0;
-    if (t.row < t.end) m.start(rows[0] = *(const Vector*)(x + t.row * p.C));
-#pragma unroll 4
-    for (long long r = t.row + p.depth; r < t.end; r += p.depth) m.add(rows[++i * p.depth * p.lanes] = *(const Vector*)(x + r * p.C));
+// ---- moments ------------------------------------------------------------------------------------------
+__device__ __forceinline__ Moments moments_of(float a, float b, float square, float count) {  // mean: a + b
+  const float mean = a + b, of_b = mean - a;
+  return {mean, (a - (mean - of_b)) + (b - of_b), square, count};
+}
+__device__ __forceinline__ float distance(const Moments& a, const Moments& b) { return (a.mean - b.mean) + (a.rest - b.rest); }
+
+// (an empty `a` only with an empty `b`: rows are dealt out from the first thread, CTA and chunk on)
+__device__ __forceinline__ Moments joined(const Moments& a, const Moments& b) {
+  const float count = a.count + b.count, d = distance(b, a), shift = d * b.count * inverse_of(fmaxf(count, 1.0f));
+  return moments_of(a.mean, a.rest + shift, fmaf(shift * d, a.count, a.square + b.square), count);
+}
+__device__ __forceinline__ float2 joined(float2 a, float2 b) { return add2(a, b); }
+
+// (rows, columns) of shared memory joined down to the first row, by halves.  All threads, behind a barrier; ends in one.
+template <typename E>
+__device__ __forceinline__ void join_rows(E* at, int rows, int columns) {
+  while (rows > 1) {
+    const int half = (rows + 1) >> 1;
+    for (int i = threadIdx.x; i < (rows - half) * columns; i += kNormThreads) at[i] = joined(at[i], at[half * columns + i]);
+    __syncthreads();
+    rows = half;
   }
-  Moments mine[V];
-  m.get(mine);
-  by_channel<V>(p, t, sh.told, mine, [&](const Moments* v, int w, int c, int) { sh.channels[c] = join_moments(v, w, p.depth, (int)(t.end - t.begin)); });
-  if (p.chunks > 1) cluster_sync();
-  else __syncthreads();
-  // a warp per group: its channels of all CTAs
-  const float all = (float)p.S * p.width;
-  for (int g = warp; g < groups; g += kNormThreads / 32) {
-    const int entries = p.chunks * p.width;
-    const auto at = [&](int e, float& count) {
-      const int rank = e / p.width;
-      count = (float)max(0ll, min(p.rows, p.S - rank * p.rows));
-      const Moments* from = sh.channels + g * p.width + (e - rank * p.width);
-      return p.chunks > 1 ? of_cluster(from, rank) : *from;
-    };
-    float count, sum = 0.0f, m2 = 0.0f;
-    const Moments pivot = at(0, count);
-    for (int e = lane; e < entries; e += 32) {
-      const Moments v = at(e, count);
-      if (count > 0.0f) sum = fmaf(count, distance(v, pivot), sum);
+}
+
+// Entries in a row, n of them, by a team; in its first thread.
+__device__ __forceinline__ Moments team_join(const NormTeam& team, const Moments* from, int n) {
+  Moments m = {};
+  if (team.lane < n) m = from[team.lane];
+  for (int i = team.lane + team.size; i < n; i += team.size) m = joined(m, from[i]);
+  for (int d = 1; d < team.size; d <<= 1) {  // (neighbours first: a thread without an entry is behind those with one)
+    const Moments other = {__shfl_down_sync(~0u, m.mean, d), __shfl_down_sync(~0u, m.rest, d), __shfl_down_sync(~0u, m.square, d), __shfl_down_sync(~0u, m.count, d)};
+    if (team.lane + d < team.size) m = joined(m, other);
+  }
+  return m;
+}
+
+// A thread's sums about a pivot, of a vector of channels.
+template <typename T, int V>
+struct NormMoments {
+  typedef Pairs<T, V> P;
+  P pivot, sum, square;
+  __device__ __forceinline__ void start(const Vec<T, V>& v) {
+    pivot = P(v);
+#pragma unroll
+    for (int k = 0; k < P::kPairs; ++k) sum.v[k] = square.v[k] = two(0.0f);
+  }
+  __device__ __forceinline__ void add(const Vec<T, V>& v) {
+    const P x(v);
+#pragma unroll
+    for (int k = 0; k < P::kPairs; ++k) {
+      const float2 d = fma2(pivot.v[k], two(-1.0f), x.v[k]);
+      sum.v[k] = add2(sum.v[k], d);
+      square.v[k] = fma2(d, d, square.v[k]);
     }
-    const float shift = warp_sum(sum) / all, mean = pivot.mean + (pivot.rest + shift);
-    for (int e = lane; e < entries; e += 32) {
-      const Moments v = at(e, count);
-      const float d = distance(v, pivot) - shift;
-      if (count > 0.0f) m2 += fmaf(count * d, d, v.square);
+  }
+  __device__ __forceinline__ Moments of(int k, float count, float inverse) const {
+    const float s = k & 1 ? sum.v[k >> 1].y : sum.v[k >> 1].x, q = k & 1 ? square.v[k >> 1].y : square.v[k >> 1].x,
+                c = k & 1 ? pivot.v[k >> 1].y : pivot.v[k >> 1].x, mean = s * inverse;
+    return moments_of(c, mean, fmaxf(0.0f, fmaf(-mean, s, q)), count);
+  }
+  // SPAN neighbouring channels from k on, together
+  template <int SPAN>
+  __device__ __forceinline__ Moments of(int k, float count, float inverse) const {
+    const Moments first = of(k, count, inverse);
+    if constexpr (SPAN == 1) return first;
+    float shift = 0.0f, square = first.square;
+#pragma unroll
+    for (int i = 1; i < SPAN; ++i) shift += distance(of(k + i, count, inverse), first);
+    shift *= 1.0f / SPAN;
+    square = fmaf(count * shift, shift, square);
+#pragma unroll
+    for (int i = 1; i < SPAN; ++i) {
+      const Moments v = of(k + i, count, inverse);
+      const float d = distance(v, first) - shift;
+      square += fmaf(count * d, d, v.square);
     }
-    m2 = warp_sum(m2);
-    if (lane == 0) {
-      const float rstd = 1.0f / sqrtf(m2 / all + p.eps);
-      sh.first[g] = mean;
-      sh.second[g] = rstd;
-      if (t.chunk == 0) {
-        p.mean[(long long)t.n * p.groups + first + g] = mean;
-        p.rstd[(long long)t.n * p.groups + first + g] = rstd;
+    return moments_of(first.mean, first.rest + shift, square, count * SPAN);
+  }
+  template <int SPAN>
+  __device__ __forceinline__ void tell(Moments* to, int rows) const {
+    const float inverse = rows > 0 ? 1.0f / rows : 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; k += SPAN) to[k / SPAN] = rows > 0 ? of<SPAN>(k, (float)rows, inverse) : Moments{};
+  }
+};
+
+// What the CTA's threads have summed, per group of the block: put(g, moments), by one thread each.  `told`: shared memory, an entry for
+// every run of a thread's channels that lie in one group.  Ends in a barrier.
+template <typename T, int V, bool WHOLE, typename F>
+__device__ __forceinline__ void group_moments(const NormParams& p, const NormPlace& t, const NormMoments<T, V>& m, Moments* told, int columns, F&& put) {
+  constexpr int kHalf = V % 2 == 0 ? V / 2 : 1;
+  const int each = WHOLE ? 1 : p.width == kHalf ? V / kHalf : V;  // entries of a thread
+  if (t.depth < p.depth && t.lane < columns) {
+    Moments* mine = told + (t.depth * columns + t.lane) * each;
+    if (WHOLE) m.template tell<V>(mine, t.count);
+    else if (p.width == kHalf) m.template tell<kHalf>(mine, t.count);
+    else m.template tell<1>(mine, t.count);
+  }
+  __syncthreads();
+  join_rows(told, p.depth, columns * each);
+  // (a block wider than the CTA is one group, taken part by part)
+  const int groups = columns < p.columns ? 1 : p.block_groups, entries = columns * each / groups;
+  if (entries == 1) {
+    for (int g = threadIdx.x; g < groups; g += kNormThreads) put(g, told[g]);
+  } else {
+    const NormTeam team(groups, entries);
+    team.each(groups, [&](int g, bool there) {
+      const Moments all = team_join(team, told + g * entries, entries);
+      if (there && team.lane == 0) put(g, all);
+    });
+  }
+  __syncthreads();
+}
+
+template <typename T, int V, bool WHOLE>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_stats(const __grid_constant__ NormParams p) {
+  extern __shared__ Moments norm_told[];
+  __shared__ Moments parts;
+  typedef Vec<T, V> Vector;
+  grid_dependency();
+  const NormPlace t = norm_place(p, blockIdx.x);
+  const T* x = (const T*)p.x + (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
+  const long long step = (long long)p.depth * p.C;
+  Moments* to = p.moments + ((long long)t.n * p.chunks + t.chunk) * p.groups + t.group;
+  for (int c0 = 0; c0 < p.columns; c0 += p.lanes) {  // (once, but for groups wider than the CTA)
+    const int columns = min(p.lanes, p.columns - c0);
+    NormMoments<T, V> m;
+    if (t.count > 0 && t.lane < columns) {
+      const T* at = x + (long long)c0 * V;
+      m.start(*(const Vector*)at);
+      walk<4>(t.count - 1, [&](int) { return *(const Vector*)(at += step); }, [&](int, const Vector& v) { m.add(v); });
+    }
+    group_moments<T, V, WHOLE>(p, t, m, norm_told, columns, [&](int g, const Moments& v) {
+      if (columns == p.columns) {
+        to[g] = v;
+      } else {  // the parts of one group, by one thread
+        parts = c0 == 0 ? v : joined(parts, v);
+        if (c0 + columns == p.columns) to[g] = parts;
+      }
+    });
+  }
+}
+
+// ---- normalised rows ----------------------------------------------------------------------------------
+// What belongs to a thread's channels: z = (x - mean) factor + bias.
+template <typename T, int V, bool WHOLE>
+struct NormChannels {
+  typedef Pairs<T, V> P;
+  static constexpr int kOwn = WHOLE ? 1 : P::kPairs;
+  float2 mean[kOwn];  // of the vector's group, or of the channels'
+  P factor, bias;
+  // weights and biases of the vector `column` of the block (asked for before what they have to wait for)
+  __device__ __forceinline__ NormChannels(const NormParams& p, const NormPlace& t, int column) {
+    float w[V], b[V];
+    parameters_of<V>(p, w, b, t.group * p.width + column * V);
+#pragma unroll
+    for (int k = 0; k < P::kPairs; ++k) {
+      factor.v[k] = make_float2(w[2 * k], w[V == 1 ? 0 : 2 * k + 1]);
+      bias.v[k] = make_float2(b[2 * k], b[V == 1 ? 0 : 2 * k + 1]);
+    }
+  }
+  // `means`, `rstds`: of the groups of the block
+  __device__ __forceinline__ void set(const NormParams& p, int column, const float* means, const float* rstds) {
+    if constexpr (WHOLE) {
+      const int g = p.by_width.quotient(column * V);
+      mean[0] = two(means[g]);
+      const float2 r = two(rstds[g]);
+#pragma unroll
+      for (int k = 0; k < P::kPairs; ++k) factor.v[k] = mul2(factor.v[k], r);
+    } else {
+#pragma unroll
+      for (int k = 0; k < P::kPairs; ++k) {
+        const int g = p.by_width.quotient(column * V + 2 * k), h = p.by_width.quotient(column * V + 2 * k + 1);
+        mean[k] = make_float2(means[g], means[h]);
+        factor.v[k] = mul2(factor.v[k], make_float2(rstds[g], rstds[h]));
       }
     }
   }
+  __device__ __forceinline__ float2 centred(int k, float2 x) const { return fma2(mean[WHOLE ? 0 : k], two(-1.0f), x); }
+};
+
+template <typename T, int ACT, int V, bool WHOLE>
+__device__ __forceinline__ Vec<T, V> normalised(const Vec<T, V>& v, const NormChannels<T, V, WHOLE>& c) {
+  Pairs<T, V> x(v);
+#pragma unroll
+  for (int k = 0; k < Pairs<T, V>::kPairs; ++k) {
+    float2 slope;
+    x.v[k] = activate<T, ACT>(fma2(c.centred(k, x.v[k]), c.factor.v[k], c.bias.v[k]), slope);
+  }
+  return x.vector();
+}
+
+// A store of what this kernel does not read again.
+template <typename V>
+__device__ __forceinline__ void put_once(V* to, const V& v) {
+  if constexpr (sizeof(V) == 16) __stcs((uint4*)to, *(const uint4*)&v);
+  else *to = v;
+}
+
+template <typename T, int V, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_apply(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) float norm_groups[];  // the block's means, their inverse deviations, what the threads have joined
+  typedef Vec<T, V> Vector;
+  grid_dependency();
+  const NormPlace t = norm_place(p, blockIdx.x);
+  float *means = norm_groups, *rstds = means + p.block_groups;
+  NormChannels<T, V, WHOLE> c(p, t, t.lane);
+  // an image's chunks: a thread takes every so many of a group's, then the threads are joined
+  Moments* told = (Moments*)(rstds + p.block_groups + (p.block_groups & 1) * 2);
+  const Moments* from = p.moments + (long long)t.n * p.chunks * p.groups + t.group;
+  const int parts = min(p.chunks, max(1, kNormThreads / p.block_groups));
+  for (int i = threadIdx.x; i < parts * p.block_groups; i += kNormThreads) {
+    const int part = i / p.block_groups, g = i - part * p.block_groups;
+    Moments first = {};
+    float count = 0.0f, sum = 0.0f, square = 0.0f;
+    walk<8>((p.chunks - part + parts - 1) / parts, [&](int k) { return from[(long long)(part + k * parts) * p.groups + g]; }, [&](int k, const Moments& v) {
+      if (k == 0) first = v;
+      const float d = distance(v, first);  // (about the first chunk's mean)
+      count += v.count;
+      sum = fmaf(v.count, d, sum);
+      square += fmaf(v.count * d, d, v.square);
+    });
+    const float shift = sum / count;
+    told[i] = moments_of(first.mean, first.rest + shift, fmaxf(0.0f, fmaf(-shift, sum, square)), count);
+  }
   __syncthreads();
-  const NormChannels<V> c(p, t, sh.first, sh.second, first);
-  if (t.in) {
-    int i = 0;
-    for (long long r = t.row; r < t.end; r += p.depth) *(Vector*)(out + r * p.C) = normalised<T, ACT>(rows[i++ * p.depth * p.lanes], c);
+  join_rows(told, parts, p.block_groups);
+  for (int g = threadIdx.x; g < p.block_groups; g += kNormThreads) {
+    const Moments all = told[g];
+    means[g] = all.mean;
+    rstds[g] = 1.0f / sqrtf(all.square / all.count + p.eps);
+    if (t.chunk == 0) {
+      p.mean[(long long)t.n * p.groups + t.group + g] = means[g];
+      p.rstd[(long long)t.n * p.groups + t.group + g] = rstds[g];
+    }
+  }
+  __syncthreads();
+  if (t.count == 0) return;
+  const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width;
+  for (int column = t.lane; column < p.columns; column += p.lanes) {
+    if (column != t.lane) c = NormChannels<T, V, WHOLE>(p, t, column);
+    c.set(p, column, means, rstds);
+    const long long last = first + (t.count - 1) * step + (long long)column * V;
+    const T* x = (const T*)p.x + last + step;
+    T* out = (T*)p.out + last + step;
+    walk<6>(t.count, [&](int) { return *(const Vector*)(x -= step); }, [&](int, const Vector& v) { put_once((Vector*)(out -= step), normalised<T, ACT>(v, c)); });
+  }
+}
+
+// Shared memory of a CTA of a cluster: what its threads have summed, its groups' sums, its groups' two numbers, then the rows.
+struct NormShared {
+  char *told, *groups;
+  float *first, *second;
+  char* rows;
+  __device__ __forceinline__ NormShared(const NormParams& p, char* base, int told_bytes) {
+    told = base;
+    groups = told + told_bytes;
+    first = (float*)(groups + 16 * p.block_groups);
+    second = first + p.block_groups;
+    rows = base + bytes(told_bytes, p.block_groups);
+  }
+  static __host__ __device__ __forceinline__ int bytes(int told, int groups) { return (told + groups * 24 + 15) & ~15; }
+};
+
+template <typename T, int V, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_cluster(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) char norm_bytes[];
+  typedef Vec<T, V> Vector;
+  const NormShared sh(p, norm_bytes, p.depth * p.lanes * (WHOLE ? 1 : V) * (int)sizeof(Moments));
+  const int image = blockIdx.x / p.chunks, n = image / p.blocks;  // (block, image, CTA of the cluster)
+  const NormPlace t = norm_place(p, n, image - n * p.blocks, blockIdx.x - image * p.chunks);
+  grid_dependency();
+  const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
+  Vector* rows = (Vector*)sh.rows + t.depth * p.lanes + t.lane;  // of this thread
+  const int next = p.depth * p.lanes;
+  NormChannels<T, V, WHOLE> c(p, t, t.lane);
+  NormMoments<T, V> m;
+  if (t.count > 0) {
+    const T* x = (const T*)p.x + first;
+    m.start(rows[0] = *(const Vector*)x);
+    walk<4>(t.count - 1, [&](int) { return *(const Vector*)(x += step); }, [&](int i, const Vector& v) { m.add(rows[(i + 1) * next] = v); });
+  }
+  Moments* groups = (Moments*)sh.groups;
+  group_moments<T, V, WHOLE>(p, t, m, (Moments*)sh.told, p.columns, [&](int g, const Moments& v) { groups[g] = v; });
+  if (p.chunks > 1) cluster_sync();
+  for (int g = threadIdx.x; g < p.block_groups; g += kNormThreads) {
+    Moments all = groups[g];
+    if (p.chunks > 1) {
+      walk<8>(p.chunks, [&](int i) { return of_cluster(groups + g, i); }, [&](int i, const Moments& v) { all = i == 0 ? v : joined(all, v); });
+    }
+    sh.first[g] = all.mean;
+    sh.second[g] = 1.0f / sqrtf(all.square / all.count + p.eps);
+    if (t.chunk == 0) {
+      p.mean[(long long)t.n * p.groups + t.group + g] = sh.first[g];
+      p.rstd[(long long)t.n * p.groups + t.group + g] = sh.second[g];
+    }
+  }
+  __syncthreads();
+  if (t.count > 0) {
+    c.set(p, t.lane, sh.first, sh.second);
+    T* out = (T*)p.out + first;
+    walk<4>(t.count, [&](int i) { return rows[i * next]; }, [&](int i, const Vector& v) { *(Vector*)(out + i * step) = normalised<T, ACT>(v, c); });
   }
   if (p.chunks > 1) cluster_sync();  // (no CTA ends while another reads its shared memory)
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-template <typename T, int ACT, int V>
-__device__ __forceinline__ void add_slopes(float2 (&sums)[V], const Vec<T, V>& x, const Vec<T, V>& dy, const NormChannels<V>& c) {
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const float xhat = (to_float(x.v[k]) - c.mean[k]) * c.rstd[k];
-    float slope;
-    activate<T, ACT>(fmaf(xhat, c.weight[k], c.bias[k]), slope);
-    const float dz = to_float(dy.v[k]) * slope;
-    sums[k].x += dz;
-    sums[k].y = fmaf(dz, xhat, sums[k].y);
-  }
-}
-template <typename T, int ACT, int V>
-__device__ __forceinline__ Vec<T, V> input_gradient(const Vec<T, V>& x, const Vec<T, V>& dy, const NormChannels<V>& c, const float2 (&m)[V]) {
-  Vec<T, V> o;
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const float xhat = (to_float(x.v[k]) - c.mean[k]) * c.rstd[k];
-    float slope;
-    activate<T, ACT>(fmaf(xhat, c.weight[k], c.bias[k]), slope);
-    o.v[k] = from_float<T>(c.rstd[k] * (fmaf(to_float(dy.v[k]) * slope, c.weight[k], -m[k].x) - xhat * m[k].y));
-  }
-  return o;
+template <typename Vector>
+struct Both {
+  Vector x, dy;
+};
+template <typename Vector, typename T>
+__device__ __forceinline__ Both<Vector> load_both(const T*& x, const T*& dy, long long step) {
+  const Both<Vector> v = {*(const Vector*)x, *(const Vector*)dy};
+  x += step;
+  dy += step;
+  return v;
 }
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_sums(const __grid_constant__ NormParams p) {
-  extern __shared__ float2 norm_shared[];
-  grid_dependency();
-  const NormPlace t = norm_place<V>(p, blockIdx.x);
-  const NormChannels<V> c(p, t, p.mean + (long long)t.n * p.groups, p.rstd + (long long)t.n * p.groups, 0);
-  typedef Vec<T, V> Vector;
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  const T* dy = (const T*)p.dy + t.n * p.S * p.C + t.channel;
-  float2 mine[V] = {};
-  if (t.in) {
-#pragma unroll 2
-    for (long long r = t.row; r < t.end; r += p.depth) add_slopes<T, ACT>(mine, *(const Vector*)(x + r * p.C), *(const Vector*)(dy + r * p.C), c);
+// Sums of dz and dz (x - mean), of a vector of channels.
+template <typename T, int V>
+struct NormSlopes {
+  typedef Pairs<T, V> P;
+  P dz, product;
+  __device__ __forceinline__ NormSlopes() {
+#pragma unroll
+    for (int k = 0; k < P::kPairs; ++k) dz.v[k] = product.v[k] = two(0.0f);
   }
-  by_channel<V>(p, t, norm_shared, mine, [&](const float2* v, int width, int, int channel) {
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int i = 0; i < p.depth; ++i) s = add2(s, v[i * width]);
-    p.part[((long long)t.n * p.chunks + t.chunk) * p.C + channel] = s;
-  });
-}
-
-// A group's m1 and m2 of an image (the first N * groups CTAs, if `means`), and 32 channels' gradients of weights and biases over all
-// images' chunks (the others).
-static __global__ void __launch_bounds__(kNormThreads) norm_sums_finish(const __grid_constant__ NormParams p, int group_ctas) {
-  __shared__ float shared[kNormThreads / 32];
-  __shared__ float2 totals[kNormThreads];
-  grid_dependency();
-  if ((int)blockIdx.x < group_ctas) {
-    const int n = blockIdx.x / p.groups, g = blockIdx.x - n * p.groups, entries = p.chunks * p.width;
-    const float2* part = p.part + (long long)n * p.chunks * p.C + g * p.width;
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int e = threadIdx.x; e < entries; e += kNormThreads) {
-      const int chunk = e / p.width, c = e - chunk * p.width;
-      const float w = weight_of(p, g * p.width + c);
-      s = fma2(make_float2(w, w), part[(long long)chunk * p.C + c], s);
+  template <int ACT, bool WHOLE>
+  __device__ __forceinline__ void add(const Vec<T, V>& x, const Vec<T, V>& dy, const NormChannels<T, V, WHOLE>& c) {
+    const P a(x), g(dy);
+#pragma unroll
+    for (int k = 0; k < P::kPairs; ++k) {
+      const float2 centred = c.centred(k, a.v[k]);
+      float2 slope;
+      activate<T, ACT>(fma2(centred, c.factor.v[k], c.bias.v[k]), slope);
+      const float2 d = mul2(g.v[k], slope);
+      dz.v[k] = add2(dz.v[k], d);
+      product.v[k] = fma2(d, centred, product.v[k]);
     }
-    const float all = (float)p.S * p.width, m1 = norm_sum(s.x, shared), m2 = norm_sum(s.y, shared);
-    if (threadIdx.x == 0) p.means[blockIdx.x] = make_float2(m1 / all, m2 / all);
-    return;
   }
-  const int channel = (blockIdx.x - group_ctas) * 32 + (threadIdx.x & 31);
+};
+
+// The CTA's sums per channel (dz, dz xhat), over `columns` vectors from vector c0 of the block on: channel(c, sums) by one thread each, with
+// them in `told`[c].  `told`: shared memory, two floats a channel of every thread.  Ends in a barrier.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void channel_sums(const NormParams& p, const NormPlace& t, const NormSlopes<T, V>& mine, float2* told, int columns, int c0,
+                                             const float* rstds, F&& channel) {
+  const int channels = columns * V;
+  if (t.depth < p.depth && t.lane < columns) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      told[t.depth * channels + t.lane * V + k] = k & 1 ? make_float2(mine.dz.v[k >> 1].y, mine.product.v[k >> 1].y) : make_float2(mine.dz.v[k >> 1].x, mine.product.v[k >> 1].x);
+  }
+  __syncthreads();
+  join_rows(told, p.depth, channels);
+  for (int c = threadIdx.x; c < channels; c += kNormThreads) {
+    float2 s = told[c];
+    s.y *= rstds[p.by_width.quotient(c0 * V + c)];
+    told[c] = s;
+    channel(c0 * V + c, s);
+  }
+  __syncthreads();
+}
+
+template <typename T, int V, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_sums(const __grid_constant__ NormParams p) {
+  extern __shared__ float2 norm_slopes[];
+  typedef Vec<T, V> Vector;
+  grid_dependency();
+  const NormPlace t = norm_place(p, blockIdx.x);
+  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
+  const long long number = (long long)t.n * p.chunks + t.chunk;
+  float2 before = two(0.0f);  // (of the parts of one group)
+  for (int c0 = 0; c0 < p.columns; c0 += p.lanes) {
+    const int columns = min(p.lanes, p.columns - c0);
+    NormSlopes<T, V> s;
+    if (t.count > 0 && t.lane < columns) {
+      NormChannels<T, V, WHOLE> c(p, t, c0 + t.lane);
+      c.set(p, c0 + t.lane, means, rstds);
+      const T *x = (const T*)p.x + first + (long long)c0 * V, *dy = (const T*)p.dy + first + (long long)c0 * V;
+      walk<3>(t.count, [&](int) { return load_both<Vector>(x, dy, step); }, [&](int, const Both<Vector>& v) { s.template add<ACT>(v.x, v.dy, c); });
+    }
+    channel_sums<T, V>(p, t, s, norm_slopes, columns, c0, rstds, [&](int c, float2 v) { p.slopes[number * p.C + (long long)t.group * p.width + c] = v; });
+    const int groups = columns < p.columns ? 1 : p.block_groups, width = columns * V / groups;
+    const NormTeam team(groups, width);
+    team.each(groups, [&](int g, bool there) {
+      float2 all = two(0.0f);
+      for (int k = team.lane; k < width; k += team.size) all = fma2(two(weight_of(p, t.group * p.width + c0 * V + g * width + k)), norm_slopes[g * width + k], all);
+      before = make_float2(before.x * (c0 > 0) + team.sum(all.x), before.y * (c0 > 0) + team.sum(all.y));
+      if (there && team.lane == 0 && c0 + columns == p.columns) p.sums[number * p.groups + t.group + g] = before;
+    });
+    __syncthreads();
+  }
+}
+
+// Gradients of weights and biases of 32 channels: sums over all images' chunks.
+__device__ __forceinline__ void parameter_gradients(const NormParams& p, int cta, float2* shared) {
+  const int channel = cta * 32 + (threadIdx.x & 31);
   const long long entries = (long long)p.N * p.chunks;
-  float2 s = make_float2(0.0f, 0.0f);
+  float2 s = two(0.0f);
   if (channel < p.C) {
-#pragma unroll 8
-    for (long long e = threadIdx.x >> 5; e < entries; e += kNormThreads / 32) s = add2(s, p.part[e * p.C + channel]);
+#pragma unroll 4
+    for (long long e = threadIdx.x >> 5; e < entries; e += kNormThreads / 32) s = add2(s, p.slopes[e * p.C + channel]);
   }
-  totals[threadIdx.x] = s;
+  shared[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x >= 32 || channel >= p.C) return;
-  for (int i = 1; i < kNormThreads / 32; ++i) s = add2(s, totals[i * 32 + threadIdx.x]);
+  for (int i = 1; i < kNormThreads / 32; ++i) s = add2(s, shared[i * 32 + threadIdx.x]);
   if (p.dweight) put_parameter(p, p.dweight, channel, s.y);
   if (p.dbias) put_parameter(p, p.dbias, channel, s.x);
 }
-
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_dx(const __grid_constant__ NormParams p) {
+static __global__ void __launch_bounds__(kNormThreads) norm_parameters(const __grid_constant__ NormParams p) {
+  __shared__ float2 shared[kNormThreads];
   grid_dependency();
-  const NormPlace t = norm_place<V>(p, blockIdx.x, true);
-  const NormChannels<V> c(p, t, p.mean + (long long)t.n * p.groups, p.rstd + (long long)t.n * p.groups, 0);
-  if (!t.in) return;
-  float2 m[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) m[k] = p.means[(long long)t.n * p.groups + (t.channel + k) / p.width];
-  typedef Vec<T, V> Vector;
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  const T* dy = (const T*)p.dy + t.n * p.S * p.C + t.channel;
-  T* dx = (T*)p.dx + t.n * p.S * p.C + t.channel;
-#pragma unroll 2
-  for (long long r = t.row; r < t.end; r += p.depth)
-    *(Vector*)(dx + r * p.C) = input_gradient<T, ACT>(*(const Vector*)(x + r * p.C), *(const Vector*)(dy + r * p.C), c, m);
+  parameter_gradients(p, blockIdx.x, shared);
 }
 
-// All of a block of groups: dx, and the block's channels' sums of the image (p.part, a chunk an image).
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_cluster_backward(const __grid_constant__ NormParams p) {
-  extern __shared__ __align__(16) char norm_bytes[];
-  typedef Vec<T, V> Vector;
-  const NormShared<float2, V> sh(p, norm_bytes);
-  NormPlace t = norm_place<V>(p, blockIdx.x / p.chunks % p.blocks + p.blocks * (blockIdx.x % p.chunks + p.chunks * (blockIdx.x / p.chunks / p.blocks)));
-  const int width = p.lanes * V, groups = width / p.width, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dependency();
-  const NormChannels<V> c(p, t, p.mean + (long long)t.n * p.groups, p.rstd + (long long)t.n * p.groups, 0);
-  const T* x = (const T*)p.x + t.n * p.S * p.C + t.channel;
-  const T* dy = (const T*)p.dy + t.n * p.S * p.C + t.channel;
-  T* dx = (T*)p.dx + t.n * p.S * p.C + t.channel;
-  Vector* rows = (Vector*)sh.rows + (t.depth * p.lanes + t.lane) * 2;  // of this thread: x and dy
-  const int step = p.depth * p.lanes * 2;
-  float2 mine[V] = {};
-  if (t.in) {
-    int i = 0;
-#pragma unroll 2
-    for (long long r = t.row; r < t.end; r += p.depth, ++i)
-      add_slopes<T, ACT>(mine, rows[i * step] = *(const Vector*)(x + r * p.C), rows[i * step + 1] = *(const Vector*)(dy + r * p.C), c);
+// dx = dz factor - rstd m1 - (x - mean) rstd^2 m2
+template <typename T, int V, bool WHOLE>
+struct NormReturn {
+  float2 first[NormChannels<T, V, WHOLE>::kOwn], second[NormChannels<T, V, WHOLE>::kOwn];  // negative
+  // m1, m2, rstds: of the groups of the block
+  __device__ __forceinline__ NormReturn(const NormParams& p, int column, const float* m1, const float* m2, const float* rstds) {
+#pragma unroll
+    for (int k = 0; k < 2 * NormChannels<T, V, WHOLE>::kOwn; ++k) {
+      const int g = p.by_width.quotient(column * V + (k < V ? k : 0));
+      const float a = -rstds[g] * m1[g], b = -rstds[g] * rstds[g] * m2[g];
+      if (k & 1) first[k >> 1].y = a, second[k >> 1].y = b;
+      else first[k >> 1].x = a, second[k >> 1].x = b;
+    }
+    if (WHOLE) first[0].y = first[0].x, second[0].y = second[0].x;
   }
-  by_channel<V>(p, t, sh.told, mine, [&](const float2* v, int w, int at, int) {
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int i = 0; i < p.depth; ++i) s = add2(s, v[i * w]);
-    sh.channels[at] = s;
-  });
-  if (p.chunks > 1) cluster_sync();
-  else __syncthreads();
+  template <int ACT>
+  __device__ __forceinline__ Vec<T, V> gradient(const Vec<T, V>& x, const Vec<T, V>& dy, const NormChannels<T, V, WHOLE>& c) const {
+    const Pairs<T, V> a(x);
+    Pairs<T, V> g(dy);
+#pragma unroll
+    for (int k = 0; k < Pairs<T, V>::kPairs; ++k) {
+      const float2 centred = c.centred(k, a.v[k]);
+      float2 slope;
+      activate<T, ACT>(fma2(centred, c.factor.v[k], c.bias.v[k]), slope);
+      g.v[k] = fma2(centred, second[WHOLE ? 0 : k], fma2(mul2(g.v[k], slope), c.factor.v[k], first[WHOLE ? 0 : k]));
+    }
+    return g.vector();
+  }
+};
+
+template <typename T, int V, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_dx(const __grid_constant__ NormParams p) {
+  extern __shared__ float norm_groups[];  // m1, m2 of the block's groups (and what the parameters' CTAs sum)
+  typedef Vec<T, V> Vector;
+  grid_dependency();
+  if ((int)blockIdx.x < p.channel_ctas) {
+    parameter_gradients(p, blockIdx.x, (float2*)norm_groups);
+    return;
+  }
+  const NormPlace t = norm_place(p, blockIdx.x - p.channel_ctas);
+  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  float *m1 = norm_groups, *m2 = m1 + p.block_groups;
+  NormChannels<T, V, WHOLE> c(p, t, t.lane);
   const float all = (float)p.S * p.width;
-  for (int g = warp; g < groups; g += kNormThreads / 32) {
-    float2 sum = make_float2(0.0f, 0.0f);
-    for (int k = lane; k < p.width; k += 32) {
-      const int at = g * p.width + k, channel = t.block * width + at;
-      float2 s = make_float2(0.0f, 0.0f);
-      for (int rank = 0; rank < p.chunks; ++rank) s = add2(s, p.chunks > 1 ? of_cluster(sh.channels + at, rank) : sh.channels[at]);
-      if (t.chunk == 0) p.part[(long long)t.n * p.C + channel] = s;
-      const float w = weight_of(p, channel);
-      sum = fma2(make_float2(w, w), s, sum);
-    }
-    const float m1 = warp_sum(sum.x), m2 = warp_sum(sum.y);
-    if (lane == 0) {
-      sh.first[g] = m1 / all;
-      sh.second[g] = m2 / all;
-    }
+  float2* told = (float2*)(m2 + p.block_groups);
+  const float2* from = p.sums + (long long)t.n * p.chunks * p.groups + t.group;
+  const int parts = min(p.chunks, max(1, kNormThreads / p.block_groups));
+  for (int i = threadIdx.x; i < parts * p.block_groups; i += kNormThreads) {
+    const int part = i / p.block_groups, g = i - part * p.block_groups;
+    float2 sum = two(0.0f);
+    walk<8>((p.chunks - part + parts - 1) / parts, [&](int k) { return from[(long long)(part + k * parts) * p.groups + g]; },
+            [&](int, const float2& v) { sum = add2(sum, v); });
+    told[i] = sum;
   }
   __syncthreads();
-  if (t.in) {
-    float2 m[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int g = (t.channel + k) / p.width - t.block * groups;
-      m[k] = make_float2(sh.first[g], sh.second[g]);
+  join_rows(told, parts, p.block_groups);
+  for (int g = threadIdx.x; g < p.block_groups; g += kNormThreads) m1[g] = told[g].x / all, m2[g] = told[g].y / all;
+  __syncthreads();
+  if (t.count == 0) return;
+  const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width;
+  for (int column = t.lane; column < p.columns; column += p.lanes) {
+    if (column != t.lane) c = NormChannels<T, V, WHOLE>(p, t, column);
+    c.set(p, column, means, rstds);
+    const NormReturn<T, V, WHOLE> back(p, column, m1, m2, rstds);
+    const long long last = first + (t.count - 1) * step + (long long)column * V;
+    const T *x = (const T*)p.x + last, *dy = (const T*)p.dy + last;
+    T* dx = (T*)p.dx + last + step;
+    walk<3>(t.count, [&](int) { return load_both<Vector>(x, dy, -step); },
+            [&](int, const Both<Vector>& v) { put_once((Vector*)(dx -= step), back.template gradient<ACT>(v.x, v.dy, c)); });
+  }
+}
+
+// All of a block of groups: dx, and the block's channels' sums of the image (a chunk an image).
+template <typename T, int V, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_cluster_backward(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) char norm_bytes[];
+  typedef Vec<T, V> Vector;
+  const NormShared sh(p, norm_bytes, p.depth * p.lanes * V * (int)sizeof(float2));
+  const int image = blockIdx.x / p.chunks, n = image / p.blocks;
+  const NormPlace t = norm_place(p, n, image - n * p.blocks, blockIdx.x - image * p.chunks);
+  grid_dependency();
+  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
+  Vector* rows = (Vector*)sh.rows + (t.depth * p.lanes + t.lane) * 2;  // of this thread: x and dy
+  const int next = p.depth * p.lanes * 2;
+  NormChannels<T, V, WHOLE> c(p, t, t.lane);
+  c.set(p, t.lane, means, rstds);
+  NormSlopes<T, V> s;
+  if (t.count > 0) {
+    const T *x = (const T*)p.x + first, *dy = (const T*)p.dy + first;
+    walk<2>(t.count, [&](int) { return load_both<Vector>(x, dy, step); }, [&](int i, const Both<Vector>& v) {
+      rows[i * next] = v.x;
+      rows[i * next + 1] = v.dy;
+      s.template add<ACT>(v.x, v.dy, c);
+    });
+  }
+  float2* told = (float2*)sh.told;
+  channel_sums<T, V>(p, t, s, told, p.columns, 0, rstds, [&](int, float2) {});
+  if (p.chunks > 1) cluster_sync();
+  const float all = (float)p.S * p.width;
+  const NormTeam team(p.block_groups, p.width);
+  team.each(p.block_groups, [&](int g, bool there) {
+    float2 sum = two(0.0f);
+    for (int k = team.lane; k < p.width; k += team.size) {
+      const int at = g * p.width + k;
+      float2 v = told[at];
+      if (p.chunks > 1) {
+        v = of_cluster(told + at, 0);
+        for (int i = 1; i < p.chunks; ++i) v = add2(v, of_cluster(told + at, i));
+      }
+      if (there && t.chunk == 0) p.slopes[(long long)t.n * p.C + t.group * p.width + at] = v;
+      sum = fma2(two(weight_of(p, t.group * p.width + at)), v, sum);
     }
-    int i = 0;
-    for (long long r = t.row; r < t.end; r += p.depth, ++i) *(Vector*)(dx + r * p.C) = input_gradient<T, ACT>(rows[i * step], rows[i * step + 1], c, m);
+    sum = make_float2(team.sum(sum.x), team.sum(sum.y));
+    if (there && team.lane == 0) sh.first[g] = sum.x / all, sh.second[g] = sum.y / all;
+  });
+  __syncthreads();
+  if (t.count > 0) {
+    const NormReturn<T, V, WHOLE> back(p, t.lane, sh.first, sh.second, rstds);
+    T* dx = (T*)p.dx + first;
+    walk<2>(t.count, [&](int i) { return Both<Vector>{rows[i * next], rows[i * next + 1]}; },
+            [&](int i, const Both<Vector>& v) { *(Vector*)(dx + i * step) = back.template gradient<ACT>(v.x, v.dy, c); });
   }
   if (p.chunks > 1) cluster_sync();
 }

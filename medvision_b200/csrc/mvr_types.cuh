@@ -69,6 +69,18 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec {
   T v[N];
 };
 
+// Division of numbers below 2^31 by a constant of the launch: a product and a shift.
+struct Divisor {
+  unsigned d, factor, shift;
+  void set(unsigned divisor) {
+    d = divisor;
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    factor = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)((__umulhi((unsigned)n, factor) + (unsigned)n) >> shift); }
+};
+
 // What precedes the kernel in its stream has ended completely, and its writes are visible; the next kernel may become resident.
 __device__ __forceinline__ void grid_dependency() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
