@@ -343,7 +343,7 @@ typedef struct mvr_rotary {
   int dtype, interleaved, inverse, axes;
   int64_t N, L, D, heads[2];
   int64_t sections[MVR_MAX_AXES];
-  double base;
+  double base;                           /* at least 1 */
   const void* x[2];                      /* (N, L, heads, D); the last dimension is contiguous */
   int64_t strides[2][3];                 /* elements, of the first three dimensions */
   void* out[2];                          /* contiguous */

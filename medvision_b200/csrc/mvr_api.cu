@@ -188,7 +188,7 @@ const char* mvr_strerror(int code) {
     case MVR_ERR_WINDOW: return "a window's reach and number of first states must not be negative";
     case MVR_ERR_GROUPS: return "the number of groups must divide the number of channels";
     case MVR_ERR_ACTIVATION: return "unknown activation";
-    case MVR_ERR_AXES: return "rotary positions take 1 to 4 axes, sections of no more pairs than the head size has, and a positive base";
+    case MVR_ERR_AXES: return "rotary positions take 1 to 4 axes, sections of no more pairs than the head size has, and a base of at least 1";
     case MVR_ERR_TOP: return "the number of alternatives must be between 0 and 16, and at most the number of classes";
     default: return "unknown error";
   }

@@ -264,37 +264,33 @@ int check_rotary(const mvr_rotary* a) {
     if (2 * pairs > a->D) return MVR_ERR_AXES;
   }
   if (pairs > kRotaryPairs) return MVR_ERR_HEAD_SIZE;
-  if (!(a->base > 0.0) || !std::isfinite(a->base)) return MVR_ERR_AXES;
+  if (!(a->base >= 1.0) || !std::isfinite(a->base)) return MVR_ERR_AXES;
   if (a->position_dtype != MVR_INDEX_F32 && a->position_dtype != MVR_INDEX_I32 && a->position_dtype != MVR_INDEX_I64) return MVR_ERR_DTYPE;
-  if (a->D > 1 << 20 || a->heads[0] > 1 << 20 || a->heads[1] > 1 << 20 || a->L > INT32_MAX || a->N > INT32_MAX) return MVR_ERR_TOO_LARGE;
+  if (a->D > 1 << 14 || a->heads[0] > 1 << 16 || a->heads[1] > 1 << 16 || a->L > 1 << 30 || a->N > INT32_MAX) return MVR_ERR_TOO_LARGE;
   if (a->N == 0 || a->L == 0) return MVR_OK;
   if (a->N * a->L > (1LL << 40)) return MVR_ERR_TOO_LARGE;
+  for (int i = 0; i < 2; ++i)
+    for (int k = 1; k < 3; ++k)
+      if (a->heads[i] > 0 && (a->strides[i][k] > INT32_MAX || a->strides[i][k] < INT32_MIN)) return MVR_ERR_TOO_LARGE;
   if (!a->x[0] || !a->out[0] || (a->heads[1] > 0 && (!a->x[1] || !a->out[1])) || !a->positions) return MVR_ERR_NULL;
   return MVR_OK;
 }
 
 template <typename T>
 int rotary_as(RotaryParams& p, const mvr_rotary* a, cudaStream_t st) {
-  // the widest vector that columns, rows and addresses allow
-  int V = 16 / (int)sizeof(T);
-  for (; V > 1; V /= 2) {
-    bool good = a->D % V == 0 && (a->interleaved ? 2 * p.pairs : p.pairs) % V == 0;
-    for (int i = 0; i < 2; ++i) {
-      if (a->heads[i] == 0) continue;
-      good = good && ((uintptr_t)a->x[i] | (uintptr_t)a->out[i]) % (V * sizeof(T)) == 0;
-      const int64_t sizes[3] = {a->N, a->L, a->heads[i]};
-      for (int k = 0; k < 3; ++k) good = good && (sizes[k] == 1 || a->strides[i][k] % V == 0);
-    }
-    if (good) break;
+  // vectors of 16 bytes, where rows and addresses allow them
+  constexpr int V = 16 / (int)sizeof(T);
+  bool vectors = a->D % V == 0;
+  for (int i = 0; i < 2; ++i) {
+    if (a->heads[i] == 0) continue;
+    vectors = vectors && ((uintptr_t)a->x[i] | (uintptr_t)a->out[i]) % 16 == 0;
+    const int64_t sizes[3] = {a->N, a->L, a->heads[i]};
+    for (int k = 0; k < 3; ++k) vectors = vectors && (sizes[k] == 1 || a->strides[i][k] % V == 0);
   }
-  int rc;
-  switch (V) {
-    case 8: if constexpr (sizeof(T) == 2) { rc = launch_rotary<T, 8>(p, a->interleaved, st); break; }
-    case 4: rc = launch_rotary<T, 4>(p, a->interleaved, st); break;
-    case 2: rc = launch_rotary<T, 2>(p, a->interleaved, st); break;
-    default: rc = launch_rotary<T, 1>(p, a->interleaved, st);
-  }
-  return rc ? MVR_ERR_TOO_LARGE : launched();
+  const int N = (int)a->N;
+  const bool good = !vectors ? launch_rotary<T, 1, kScalar>(p, N, a->interleaved, st) : a->interleaved ? launch_rotary<T, V, kNeighbour>(p, N, true, st)
+                    : p.pairs % V == 0 ? launch_rotary<T, V, kApart>(p, N, false, st) : launch_rotary<T, V, kOwn>(p, N, false, st);
+  return good ? MVR_OK : MVR_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -322,18 +318,20 @@ int mvr_rotary_positions(const mvr_rotary* a, void* stream) {
     p.x[i] = a->x[i];
     p.out[i] = a->out[i];
     p.heads[i] = (int)a->heads[i];
-    p.s_n[i] = a->strides[i][0]; p.s_l[i] = a->strides[i][1]; p.s_h[i] = a->strides[i][2];
+    p.s_n[i] = a->strides[i][0]; p.s_l[i] = (int)a->strides[i][1]; p.s_h[i] = (int)a->strides[i][2];
   }
   p.positions = a->positions;
   p.position_type = a->position_dtype == MVR_INDEX_F32 ? 0 : a->position_dtype == MVR_INDEX_I32 ? 1 : 2;
   p.p_n = a->position_strides[0]; p.p_l = a->position_strides[1]; p.p_a = a->position_strides[2];
-  p.tokens = a->N * a->L;
   p.L = (int)a->L;
   p.D = (int)a->D;
   p.sign = a->inverse ? -1.0f : 1.0f;
   for (int i = 0; i < kRotaryAxes; ++i) {
     const int n = i < a->axes ? (int)a->sections[i] : 0;
-    for (int k = 0; k < n; ++k) p.turns[p.pairs + k] = std::pow(a->base, -(double)k / n) * 0.15915494309189533577;  // / 2 pi
+    // (by repeated products: each off by 2^-64, and calls of powl would take longer than the kernel of a few tokens)
+    const long double ratio = n > 1 ? powl(a->base, -1.0L / n) : 1.0L;
+    long double turns = 0.159154943091895335768883763372514362L;  // 1 / 2 pi
+    for (int k = 0; k < n; ++k, turns *= ratio) p.turns[p.pairs + k] = (unsigned long long)ldexpl(turns, 64);
     p.ends[i] = p.pairs += n;
   }
   const cudaStream_t st = (cudaStream_t)stream;

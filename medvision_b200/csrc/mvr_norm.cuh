@@ -82,29 +82,6 @@ __device__ __forceinline__ void put_parameter(const NormParams& p, void* to, int
 }
 
 // ---- pairs of values ----------------------------------------------------------------------------------
-// A vector of V elements as pairs of floats (V 1: half a pair).
-template <typename T, int V>
-struct Pairs {
-  static constexpr int kPairs = (V + 1) / 2;
-  float2 v[kPairs];
-  Pairs() = default;
-  __device__ __forceinline__ explicit Pairs(const Vec<T, V>& from) {
-    if constexpr (V == 1) v[0] = make_float2(to_float(from.v[0]), 0.0f);
-    else
-#pragma unroll
-      for (int k = 0; k < kPairs; ++k) v[k] = floats(((const Two<T>*)&from)[k]);
-  }
-  __device__ __forceinline__ Vec<T, V> vector() const {
-    Vec<T, V> to;
-    if constexpr (V == 1) to.v[0] = from_float<T>(v[0].x);
-    else
-#pragma unroll
-      for (int k = 0; k < kPairs; ++k) ((Two<T>*)&to)[k] = rounded<T>(v[k]);
-    return to;
-  }
-};
-__device__ __forceinline__ float2 two(float f) { return make_float2(f, f); }
-
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -280,7 +257,7 @@ __device__ __forceinline__ Moments team_join(const NormTeam& team, const Moments
 // A thread's sums about a pivot, of a vector of channels.
 template <typename T, int V>
 struct NormMoments {
-  typedef Pairs<T, V> P;
+  typedef FloatPairs<T, V> P;
   P pivot, sum, square;
   __device__ __forceinline__ void start(const Vec<T, V>& v) {
     pivot = P(v);
@@ -388,7 +365,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_stats(const __grid_const
 // What belongs to a thread's channels: z = (x - mean) factor + bias.
 template <typename T, int V, bool WHOLE>
 struct NormChannels {
-  typedef Pairs<T, V> P;
+  typedef FloatPairs<T, V> P;
   static constexpr int kOwn = WHOLE ? 1 : P::kPairs;
   float2 mean[kOwn];  // of the vector's group, or of the channels'
   P factor, bias;
@@ -424,9 +401,9 @@ struct NormChannels {
 
 template <typename T, int ACT, int V, bool WHOLE>
 __device__ __forceinline__ Vec<T, V> normalised(const Vec<T, V>& v, const NormChannels<T, V, WHOLE>& c) {
-  Pairs<T, V> x(v);
+  FloatPairs<T, V> x(v);
 #pragma unroll
-  for (int k = 0; k < Pairs<T, V>::kPairs; ++k) {
+  for (int k = 0; k < FloatPairs<T, V>::kPairs; ++k) {
     float2 slope;
     x.v[k] = activate<T, ACT>(fma2(c.centred(k, x.v[k]), c.factor.v[k], c.bias.v[k]), slope);
   }
@@ -563,7 +540,7 @@ __device__ __forceinline__ Both<Vector> load_both(const T*& x, const T*& dy, lon
 // Sums of dz and dz (x - mean), of a vector of channels.
 template <typename T, int V>
 struct NormSlopes {
-  typedef Pairs<T, V> P;
+  typedef FloatPairs<T, V> P;
   P dz, product;
   __device__ __forceinline__ NormSlopes() {
 #pragma unroll
@@ -677,10 +654,10 @@ struct NormReturn {
   }
   template <int ACT>
   __device__ __forceinline__ Vec<T, V> gradient(const Vec<T, V>& x, const Vec<T, V>& dy, const NormChannels<T, V, WHOLE>& c) const {
-    const Pairs<T, V> a(x);
-    Pairs<T, V> g(dy);
+    const FloatPairs<T, V> a(x);
+    FloatPairs<T, V> g(dy);
 #pragma unroll
-    for (int k = 0; k < Pairs<T, V>::kPairs; ++k) {
+    for (int k = 0; k < FloatPairs<T, V>::kPairs; ++k) {
       const float2 centred = c.centred(k, a.v[k]);
       float2 slope;
       activate<T, ACT>(fma2(centred, c.factor.v[k], c.bias.v[k]), slope);

@@ -158,7 +158,9 @@ void turn(const Rotary& s, const at::Tensor (&x)[2], const at::Tensor& positions
   int to = 0;
   for (int i = 0; i < 2; ++i) {
     if (!x[i].defined()) continue;
-    rows[i] = x[i].size(3) <= 1 || x[i].stride(3) == 1 ? x[i] : x[i].contiguous();
+    // (the kernel's rows are of consecutive elements, and 32-bit strides apart)
+    const bool good = (x[i].size(3) <= 1 || x[i].stride(3) == 1) && x[i].stride(1) <= INT32_MAX && x[i].stride(2) <= INT32_MAX;
+    rows[i] = good ? x[i] : x[i].contiguous();
     out[i] = at::empty(x[i].sizes(), x[i].options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
     a.heads[to] = x[i].size(2);
     a.x[to] = data_or_null(rows[i]);
@@ -228,7 +230,7 @@ void rotary_positions(const at::Tensor& query, const at::Tensor& key, const at::
   }
   TORCH_CHECK(2 * pairs <= D, what, ": sections must be numbers of pairs, together at most half of the head size");
   TORCH_CHECK(pairs <= 256, what, ": at most 256 pairs of columns can be turned");
-  TORCH_CHECK(std::isfinite(s.base) && s.base > 0, what, ": base must be finite and positive");
+  TORCH_CHECK(std::isfinite(s.base) && s.base >= 1, what, ": base must be finite and at least 1");
   check_cuda(what, query);
   check_tangent(what, query);
   if (key.defined()) check_tangent(what, key);

@@ -69,6 +69,29 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec {
   T v[N];
 };
 
+// A vector of V elements as pairs of floats (V 1: half a pair).
+template <typename T, int V>
+struct FloatPairs {
+  static constexpr int kPairs = (V + 1) / 2;
+  float2 v[kPairs];
+  FloatPairs() = default;
+  __device__ __forceinline__ explicit FloatPairs(const Vec<T, V>& from) {
+    if constexpr (V == 1) v[0] = make_float2(to_float(from.v[0]), 0.0f);
+    else
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) v[k] = floats(((const Two<T>*)&from)[k]);
+  }
+  __device__ __forceinline__ Vec<T, V> vector() const {
+    Vec<T, V> to;
+    if constexpr (V == 1) to.v[0] = from_float<T>(v[0].x);
+    else
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) ((Two<T>*)&to)[k] = rounded<T>(v[k]);
+    return to;
+  }
+};
+__device__ __forceinline__ float2 two(float f) { return make_float2(f, f); }
+
 // Division of numbers below 2^31 by a constant of the launch: a product and a shift.
 struct Divisor {
   unsigned d, factor, shift;

@@ -18,11 +18,11 @@ def rotary_positions(query, positions, key=None, sections=None, base=10000.0, in
         key (Tensor): (images, states, key_heads, dim) of the same type: turned in the same pass
         sections (sequence of int): number of pairs of each axis, together at most dim // 2 and 256; None divides dim // 2 evenly, the
             first axes taking what is left over
-        base (float): the slowest pair of a long section turns by about 1 / base
+        base (float): at least 1; the slowest pair of a long section turns by about 1 / base
         interleaved (bool): pairs are columns (2i, 2i + 1); else (i, i + pairs), counted over all axes.  Columns behind the pairs
             are copied
 
-    Angles are formed in 64 bits: far positions turn as exactly as near ones.
+    Angles are formed in 64 bits, and far positions turn as exactly as near ones (up to 2^31; a position that is not finite gives NaN).
     Returns the turned query, or (query, key): contiguous, of the same shapes and types.
     """
     return _C._native.rotary_positions(query, key, positions, sections, base, interleaved)

@@ -238,7 +238,7 @@ def test_refusals():
             rotary_positions(x, at, sections=sections)
     with pytest.raises(RuntimeError, match="at most 256 pairs"):
         rotary_positions(torch.zeros(2, 3, 1, 600), at)
-    for base in (0.0, -1.0, math.inf, math.nan):
+    for base in (0.0, -1.0, 0.99, math.inf, math.nan):
         with pytest.raises(RuntimeError, match="base must be"):
             rotary_positions(x, at, base=base)
     with pytest.raises(TypeError):
