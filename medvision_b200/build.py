@@ -16,7 +16,7 @@ HEADERS = ["mvr_arith.cuh", "mvr_geom.cuh", "mvr_generic.cuh", "mvr_stream3d.cuh
            os.path.join("..", "..", "include", "mvr.h")]
 ATTENTION_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_attn_host.cuh", "mvr_tc.cuh",
                      os.path.join("..", "..", "include", "mvr.h")]
-HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": ATTENTION_HEADERS + ["mvr_dropout.cuh", "mvr_logprob.cuh"], "mvr_window.cu": ATTENTION_HEADERS,
+HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": ATTENTION_HEADERS + ["mvr_dropout.cuh", "mvr_logprob.cuh"], "mvr_window.cu": ATTENTION_HEADERS + ["mvr_attn_rows.cuh"],
               "mvr_encoder.cu": ["mvr_types.cuh", "mvr_norm.cuh", "mvr_rotary.cuh", os.path.join("..", "..", "include", "mvr.h")]}
 LIB_FILES = sorted(set(SOURCES).union(*HEADERS_OF.values()))
 NATIVE_SOURCES = ["mvr_torch.cpp", "mvr_torch_heads.cpp", "mvr_torch_encoder.cpp"]

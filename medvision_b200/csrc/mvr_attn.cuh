@@ -75,18 +75,16 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >
 __device__ __forceinline__ uint32_t span_bits(const Span& s, int j) {
   return (bits_below(s.hi - j) & ~bits_below(s.lo - j)) | bits_below(s.sink - j);
 }
-// The tiles of STEP states that hold some of a span: those of the first states, then those of the window.
+// The tiles of STEP states that hold a span: those of the first states, then those of the window from its own beginning on.
 template <int STEP>
 struct SpanTiles {
   int sinks, from, count;
   __device__ __forceinline__ SpanTiles(const Span& s) {
-    from = s.lo / STEP;
     sinks = (s.sink + STEP - 1) / STEP;
-    const int to = s.lo < s.hi ? (s.hi + STEP - 1) / STEP : from;
-    if (from <= sinks) from = sinks;  // (one run from 0 on)
-    count = sinks + max(0, to - from);
+    from = max(s.lo, sinks * STEP);  // (what lies before is in the first ones' tiles)
+    count = sinks + max(0, s.hi - from + STEP - 1) / STEP;
   }
-  __device__ __forceinline__ int first(int i) const { return (i < sinks ? i : from + i - sinks) * STEP; }
+  __device__ __forceinline__ int first(int i) const { return i < sinks ? i * STEP : from + (i - sinks) * STEP; }
 };
 
 // Rows of a tile: image n (N: none), its regions, and where the tile begins among the rows of one key head.
@@ -179,7 +177,7 @@ __device__ __forceinline__ void rows_of_state(const AttnParams& p, long long pla
   lo = token_at(p, j - p.after - place0) * p.G;
   hi = (j < p.sinks ? p.T : token_at(p, j + p.before + 1 - place0)) * p.G;
 }
-// The part's tiles of `step` rows for the states from j0 on, `size` of them.
+// The part's tiles of `step` rows for the states from j0 on, `size` of them: the first row, and how many tiles.
 struct TileRows {
   int first, count;
 };
@@ -187,9 +185,9 @@ __device__ __forceinline__ TileRows rows_of_states(const AttnParams& p, const St
   int lo, hi, unused;
   rows_of_state(p, place0, j0, lo, hi);
   if (j0 >= p.sinks) rows_of_state(p, place0, min(j0 + size, states_of(p, s.n)) - 1, unused, hi);
-  const int from = lo / step, all = max(0, (hi + step - 1) / step - from);
+  const int all = max(0, hi - lo + step - 1) / step;
   const int per = s.sink ? (all + p.sink_parts - 1) / p.sink_parts : p.row_tiles_per;
-  return {from + s.part * per, max(0, min(per, all - s.part * per))};
+  return {lo + s.part * per * step, max(0, min(per, all - s.part * per))};
 }
 // Where a state's sums of a part go: parts of the first tiles lie before those of the others, each without the other's states.
 struct PartPlace {

@@ -345,8 +345,8 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
   const long long place0 = WINDOW ? first_place(p, n) : 0;
   if (WINDOW) {
     const TileRows r = rows_of_states(p, st, place0, j0, F::BT, F::BT);
-    first = any ? r.first * F::BT : 0;
-    last = any ? min(o.rows, (r.first + r.count) * F::BT) : 0;
+    first = any ? r.first : 0;
+    last = any ? min(o.rows, r.first + r.count * F::BT) : 0;
   }
   int row_lo[F::MT], row_hi[F::MT];
 #pragma unroll

@@ -137,17 +137,22 @@ struct OperandPieces {
 
 // Float operands of a call in pieces, in its workspace; `b` is the call on them.
 int split_operands(const mvr_attention* a, bool backward, const OperandPieces& c, char* ws, mvr_attention& b, AttnParams& p, cudaStream_t st) {
+  SplitCall call = {};
+  int operands = 0;
+  long long most = 0;
   const auto split = [&](const void* from, const int64_t (&s)[3], long long n0, long long n1, long long n2, long long to) {
-    const long long rows = n0 * n1 * n2;
-    if (rows > 0)
-      launch_dependent(split_floats, dim3((unsigned)cdiv(rows * (c.W / 8), 256)), dim3(256), 0, st, (const float*)from, (long long)s[0], (long long)s[1],
-                       (long long)s[2], (int)n1, (int)n2, rows, (int)a->D, c.W, (__nv_bfloat16*)(ws + to));
-    return launched();
+    if (n0 * n1 * n2 == 0) return;
+    call.of[operands++] = {(const float*)from, (long long)s[0], (long long)s[1], (long long)s[2], (int)n1, (int)n2, n0 * n1 * n2, (__nv_bfloat16*)(ws + to)};
+    most = std::max(most, n0 * n1 * n2);
   };
-  int rc = split(a->q, a->q_strides, a->R, a->T, a->Hq, c.q);
-  if (rc == MVR_OK) rc = split(a->k, a->k_strides, a->N, a->L, a->Hk, c.k);
-  if (rc == MVR_OK) rc = split(a->v, a->v_strides, a->N, a->L, a->Hk, c.v);
-  if (rc == MVR_OK && backward) rc = split(a->grad_out, a->g_strides, a->R, a->T, a->Hq, c.g);
+  split(a->q, a->q_strides, a->R, a->T, a->Hq, c.q);
+  split(a->k, a->k_strides, a->N, a->L, a->Hk, c.k);
+  split(a->v, a->v_strides, a->N, a->L, a->Hk, c.v);
+  if (backward) split(a->grad_out, a->g_strides, a->R, a->T, a->Hq, c.g);
+  call.D = (int)a->D;
+  call.W = c.W;
+  if (operands > 0) launch_dependent(split_floats, dim3((unsigned)cdiv(most * (c.W / 8), 256), operands), dim3(256), 0, st, call);
+  const int rc = launched();
   if (rc != MVR_OK) return rc;
   b = *a;
   b.D = c.W;

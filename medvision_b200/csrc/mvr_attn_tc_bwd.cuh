@@ -131,7 +131,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const bool any = __syncthreads_or(in);
   const RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
-  int first = split * per, count = any ? max(0, min(row_tiles, first + per) - first) : 0, row_lo = 0, row_hi = 0;
+  int first = split * per * F::kStep, count = any ? max(0, min(row_tiles, (split + 1) * per) - split * per) : 0, row_lo = 0, row_hi = 0;  // first: row
   if (WINDOW) {
     const long long place0 = first_place(p, n);
     rows_of_state(p, place0, j, row_lo, row_hi);  // (one state a thread)
@@ -239,7 +239,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const auto look_up = [&](int i) {
 #pragma unroll
       for (int k = 0; k < kParts; ++k) {
-        const int at = (first + i) * F::kStep + (warp - kLoader) * 32 + k * F::kLoaders + lane;
+        const int at = first + i * F::kStep + (warp - kLoader) * 32 + k * F::kLoaders + lane;
         q[k] = g[k] = ~0u;
         lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
         if (i < count && at < o.rows) {
@@ -291,7 +291,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           bar_arrive_warp(bar);
         } else if (elect_one()) {
           bar_expect(bar, 2 * F::kStageBytes);
-          const int token = p.by_G.quotient((first + i) * F::kStep);
+          const int token = p.by_G.quotient(first + i * F::kStep);
 #pragma unroll
           for (int part = 0; part < PIECES; ++part)
 #pragma unroll
@@ -330,7 +330,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     if (count > 0 && TcType<T>::code == 0) {
       float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of a tile of rows
       const int before = o.order ? p.tiles[n] : n * ((o.rows + kTcRows - 1) / kTcRows);
-      for (int t = first * F::kStep / kTcRows + threadIdx.x; t * kTcRows < min(o.rows, (first + count) * F::kStep); t += F::kGroups) {
+      for (int t = first / kTcRows + threadIdx.x; t * kTcRows < min(o.rows, first + count * F::kStep); t += F::kGroups) {
         const float2 peak = p.row_peaks[(long long)(before + t) * p.Hk + hk];
         most[1] = fmaxf(most[1], peak.x);
         most[2] = fmaxf(most[2], peak.y);
@@ -383,7 +383,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       }
       const int col = part_of * 32;
       // rows that do not read this state
-      const uint32_t bits = WINDOW ? bits_below(row_hi - (first + i) * F::kStep - col) & ~bits_below(row_lo - (first + i) * F::kStep - col) : ~0u;
+      const uint32_t bits = WINDOW ? bits_below(row_hi - (first + i * F::kStep + col)) & ~bits_below(row_lo - (first + i * F::kStep + col)) : ~0u;
       float2 w[16];
       uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
@@ -681,7 +681,8 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     if (MODE == kWindow && TcType<T>::code == 0 && tiles > 0) {
       const int state_tiles = (p.L + 127) / 128;
       for (int i = lane; i < tiles; i += 32)
-        peak = max(peak, p.peaks[((long long)o.n * state_tiles + first_of(i) / 128) * p.Hk + hk]);
+        for (int t = first_of(i) / 128; t <= min(state_tiles - 1, (first_of(i) + F::kStep - 1) / 128); ++t)
+          peak = max(peak, p.peaks[((long long)o.n * state_tiles + t) * p.Hk + hk]);
       peak = __reduce_max_sync(~0u, peak);
     }
     if (mine) {

@@ -328,10 +328,17 @@ int mvr_rotary_positions(const mvr_rotary* a, void* stream) {
   p.sign = a->inverse ? -1.0f : 1.0f;
   for (int i = 0; i < kRotaryAxes; ++i) {
     const int n = i < a->axes ? (int)a->sections[i] : 0;
-    // (by repeated products: each off by 2^-64, and calls of powl would take longer than the kernel of a few tokens)
+    // 1 / 2 pi times powers of base^(-1 / n), in 2^-64 (and what lies below): by whole-number products, since a call of powl for each, and
+    // conversions from long double, take longer than the kernel of a few tokens
     const long double ratio = n > 1 ? powl(a->base, -1.0L / n) : 1.0L;
-    long double turns = 0.159154943091895335768883763372514362L;  // 1 / 2 pi
-    for (int k = 0; k < n; ++k, turns *= ratio) p.turns[p.pairs + k] = (unsigned long long)ldexpl(turns, 64);
+    const unsigned __int128 factor = ratio < 1.0L ? (unsigned __int128)(unsigned long long)(ratio * 18446744073709551616.0L) : (unsigned __int128)1 << 64;
+    unsigned long long turns = 0x28be60db9391054aull, below = 0x7f09d5f47d4d3770ull;
+    for (int k = 0; k < n; ++k) {
+      p.turns[p.pairs + k] = turns;
+      const unsigned __int128 next = turns * factor + ((below * factor) >> 64);
+      turns = (unsigned long long)(next >> 64);
+      below = (unsigned long long)next;
+    }
     p.ends[i] = p.pairs += n;
   }
   const cudaStream_t st = (cudaStream_t)stream;

@@ -669,7 +669,7 @@ struct NormReturn {
 
 template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_dx(const __grid_constant__ NormParams p) {
-  extern __shared__ float norm_groups[];  // m1, m2 of the block's groups (and what the parameters' CTAs sum)
+  extern __shared__ __align__(16) float norm_groups[];  // m1, m2 of the block's groups (and what the parameters' CTAs sum)
   typedef Vec<T, V> Vector;
   grid_dependency();
   if ((int)blockIdx.x < p.channel_ctas) {

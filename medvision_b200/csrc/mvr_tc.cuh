@@ -299,14 +299,27 @@ __device__ __forceinline__ void pieces_of(float2 f, uint32_t& a, uint32_t& b, ui
 // takes eight columns.  An infinity is the largest bfloat16 of its sign, 0 and the infinity: the third piece meets nothing but the other
 // operand's first, so that no 0 among that one's smaller pieces makes a NaN of an infinite product, and the first piece gives infinity
 // times infinity.  NaN is the third piece alone.
-static __global__ void __launch_bounds__(256) split_floats(const float* from, long long s0, long long s1, long long s2, int n1, int n2, long long rows,
-                                                    int D, int W, __nv_bfloat16* to) {
+struct SplitFloats {
+  const float* from;
+  long long s0, s1, s2;
+  int n1, n2;
+  long long rows;
+  __nv_bfloat16* to;
+};
+struct SplitCall {
+  SplitFloats of[4];  // blockIdx.y: a call's operands in one launch
+  int D, W;
+};
+static __global__ void __launch_bounds__(256) split_floats(const __grid_constant__ SplitCall call) {
   grid_dependency();
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (W / 8);
+  const SplitFloats& t = call.of[blockIdx.y];
+  const int W = call.W, D = call.D;
+  const long long rows = t.rows, id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (W / 8);
   if (row >= rows) return;
   const int col = (int)(id - row * (W / 8)) * 8;
-  const long long i01 = row / n2, i0 = i01 / n1;
-  const float* src = from + i0 * s0 + (i01 - i0 * n1) * s1 + (row - i01 * n2) * s2 + col;
+  const long long i01 = row / t.n2, i0 = i01 / t.n1;
+  const float* src = t.from + i0 * t.s0 + (i01 - i0 * t.n1) * t.s1 + (row - i01 * t.n2) * t.s2 + col;
+  __nv_bfloat16* to = t.to;
   float f[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) f[k] = col + k < D ? src[k] : 0.0f;

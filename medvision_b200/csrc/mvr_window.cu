@@ -1,5 +1,6 @@
 // C ABI of attention in a sliding window (declared in include/mvr.h): argument checks, how a call is cut into CTAs, launches.  The kernels
-// are those of mvr_attn_fma.cuh, mvr_attn_tc.cuh and mvr_attn_tc_bwd.cuh, each walking the tiles that its rows' windows reach.
+// are those of mvr_attn_fma.cuh, mvr_attn_tc.cuh and mvr_attn_tc_bwd.cuh, each walking the tiles that its rows' windows reach, and for the
+// forward of a few rows that of mvr_attn_rows.cuh.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -8,8 +9,11 @@
 
 #include "../../include/mvr.h"
 #include "mvr_attn_host.cuh"
+#include "mvr_attn_rows.cuh"
 
 namespace {
+
+enum Way { kFloats = 0, kTensorCores = 1, kFewRows = 2 };
 
 struct WindowCut : OperandPieces {
   bool tc;
@@ -31,10 +35,10 @@ Window window_of(const mvr_attention* a, const mvr_window* w) {
 // The most states that `tokens` neighbouring tokens read in their windows.
 long long reach(const mvr_attention* a, const Window& w, long long tokens) { return std::min<long long>(a->L, tokens + w.before + w.after); }
 
-WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backward, bool tc) {
+WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backward, Way way) {
   const Window w = window_of(a, given);
   WindowCut c = {};
-  c.tc = tc;
+  const bool tc = c.tc = way == kTensorCores;
   const bool pieces = tc && a->dtype == MVR_F32, wide = a->D > 64;
   c.W = (int)(pieces ? cdiv(a->D, 8) * 8 : a->D);
   const long long G = a->Hq / a->Hk, per = a->T * G, rows = a->R * a->T * a->Hq;
@@ -51,6 +55,11 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
   c.splits = best_parts(std::max<long long>(1, c.row_tiles * a->Hk), tiles_of(c.state_tile), states_step(tc, pieces, backward, wide, c.tile > kTcRows),
                         rows * a->D * 8 / 4e6, false);
   c.tiles_per = (int)cdiv(tiles_of(step), c.splits);
+  if (way == kFewRows) {
+    // four CTAs an SM (eight: up to 15 % slower), with 128 states each at least (64: 9.4 us instead of 6.8 for 8 caches' windows of 500)
+    const long long states = reach(a, w, a->T) + w.sinks, ctas = std::max<long long>(1, a->N * a->Hk);
+    c.splits = (int)std::max<long long>(1, std::min<long long>({64, cdiv(4 * kMultiprocessors, ctas), cdiv(states, 128)}));
+  }
   c.sink_tiles = (int)cdiv(w.sinks, c.state_tile);
   c.row_splits = c.sink_parts = 1;
   const long long others = cdiv(a->L, c.state_tile) - c.sink_tiles, lead = std::min<long long>(a->L, (long long)c.sink_tiles * c.state_tile);
@@ -93,6 +102,19 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
   }
   c.bytes = at;
   return c;
+}
+
+// Whether a forward is of few rows: those of a key head are the lanes' registers, and rows are read in vectors.  Half types up to two rows (32
+// caches, windows of 2051 states, 8 key heads of 128: one row 55 us, two 57, four 73; tensor cores 61), float up to eight (16 caches of
+// 2000 states, 8 heads of 64: 57 us, in float arithmetic by tiles 209).
+bool few_rows(const mvr_attention* a) {
+  return a->T * (a->Hq / a->Hk) <= (a->dtype == MVR_F32 ? 8 : 2) && a->D % 8 == 0 && a->N <= INT32_MAX / 64 && a->Hk <= 65535;
+}
+bool vectors_aligned(const void* base, const int64_t (&strides)[3], const int64_t (&sizes)[3], int element) {
+  if ((uintptr_t)base % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1 && strides[i] * element % 16 != 0) return false;
+  return true;
 }
 
 // Whether type and sizes are the tensor cores'.  Float operands are cut into pieces whole, states that no token reads among them:
@@ -176,6 +198,24 @@ int fma_window(const AttnParams& p, const WindowCut& c, bool backward, cudaStrea
          : p.D <= 128 ? fma_window<T, 128>(p, c, backward, st) : fma_window<T, 256>(p, c, backward, st);
 }
 
+template <typename T, int DP>
+int rows_forward(const AttnParams& p, const WindowCut& c, cudaStream_t st) {
+  const dim3 grid(p.N, p.Hk, c.splits);
+  const int rows = p.T * p.G;
+  constexpr size_t shared = kRowsShared<T>;
+  if (rows <= 1) return launch_shared<attn_rows_fwd<T, DP, 1>>(grid, kRowsThreads, shared, st, p);
+  if constexpr (sizeof(T) == 4) {
+    if (rows > 4) return launch_shared<attn_rows_fwd<T, DP, 8>>(grid, kRowsThreads, shared, st, p);
+    if (rows > 2) return launch_shared<attn_rows_fwd<T, DP, 4>>(grid, kRowsThreads, shared, st, p);
+  }
+  return launch_shared<attn_rows_fwd<T, DP, 2>>(grid, kRowsThreads, shared, st, p);
+}
+template <typename T>
+int rows_forward(const AttnParams& p, const WindowCut& c, cudaStream_t st) {
+  return p.D <= 32 ? rows_forward<T, 32>(p, c, st) : p.D <= 64 ? rows_forward<T, 64>(p, c, st) : p.D <= 128 ? rows_forward<T, 128>(p, c, st)
+                                                                                                  : rows_forward<T, 256>(p, c, st);
+}
+
 template <typename T, int DP, int TILES, int PIECES>
 int tc_window_forward(const AttnParams& p, const WindowCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
   typedef TcForward<DP, TILES, kWindow, PIECES> F;
@@ -193,9 +233,11 @@ int tc_window_backward(const AttnParams& p, const WindowCut& c, const TcMaps& ma
 }
 
 template <typename T>
-int window_forward(const AttnParams& p, const WindowCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
+int window_forward(const AttnParams& p, const WindowCut& c, Way way, const TcMaps& maps, int* status, cudaStream_t st) {
   int rc;
-  if (!c.tc) {
+  if (way == kFewRows) {
+    rc = rows_forward<T>(p, c, st);
+  } else if (!c.tc) {
     rc = fma_window<T>(p, c, false, st);
   } else if constexpr (sizeof(T) == 4) {
     rc = tc_window_forward<__nv_bfloat16, 64, 1, 3>(p, c, maps, status, st);
@@ -284,13 +326,22 @@ template <typename T>
 int window_as(const mvr_attention* a, const mvr_window* w, bool backward, char* workspace, int* status, cudaStream_t st) {
   TcMaps maps = {};
   bool boxes = false, tc = tc_window(a, w);
+  if (!backward && few_rows(a)) {
+    const int64_t rows[3] = {a->R, a->T, a->Hq}, states[3] = {a->N, a->L, a->Hk};
+    if (vectors_aligned(a->q, a->q_strides, rows, sizeof(T)) && vectors_aligned(a->k, a->k_strides, states, sizeof(T)) &&
+        vectors_aligned(a->v, a->v_strides, states, sizeof(T))) {
+      const WindowCut c = cut_window(a, w, false, kFewRows);
+      return window_forward<T>(window_params(a, w, c, workspace), c, kFewRows, maps, status, st);
+    }
+  }
   if constexpr (sizeof(T) == 2) {
     tc = tc && (uintptr_t)a->out % 16 == 0 && rows_aligned(a->q, a->q_strides, a);
     if (backward)
       tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
     tc = tc && tensor_maps<T>(a, backward, 1, maps, boxes);
   }
-  const WindowCut c = cut_window(a, w, backward, tc);
+  const Way way = tc ? kTensorCores : kFloats;
+  const WindowCut c = cut_window(a, w, backward, way);
   if (c.row_tiles > INT32_MAX) return MVR_ERR_TOO_LARGE;
   AttnParams p = window_params(a, w, c, workspace);
   const AttnParams plain = p;
@@ -302,12 +353,15 @@ int window_as(const mvr_attention* a, const mvr_window* w, bool backward, char* 
       if (!tensor_maps<__nv_bfloat16>(&b, backward, 3, maps, boxes)) return MVR_ERR_LAUNCH;
     }
   }
-  return backward ? window_backward<T>(p, plain, c, maps, boxes, status, st) : window_forward<T>(p, c, maps, status, st);
+  return backward ? window_backward<T>(p, plain, c, maps, boxes, status, st) : window_forward<T>(p, c, way, maps, status, st);
 }
 
 long long window_bytes(const mvr_attention* a, const mvr_window* w, bool backward) {
-  const long long fma = cut_window(a, w, backward, false).bytes;
-  return tc_window(a, w) ? std::max(fma, cut_window(a, w, backward, true).bytes) : fma;
+  // (which way it goes is a matter of the call's addresses too)
+  long long bytes = cut_window(a, w, backward, kFloats).bytes;
+  if (tc_window(a, w)) bytes = std::max(bytes, cut_window(a, w, backward, kTensorCores).bytes);
+  if (!backward && few_rows(a)) bytes = std::max(bytes, cut_window(a, w, false, kFewRows).bytes);
+  return bytes;
 }
 
 int window_attention(const mvr_attention* a, const mvr_window* w, bool backward, void* workspace, int64_t bytes, int* status, void* stream) {

@@ -125,6 +125,27 @@ def test_caches_and_padded_sequences(dtype, window, tokens, dim, heads):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("window", [(0, 0, 0), (90, 0, 5), (700, 0, 0), (30, 9, 200)])
+@pytest.mark.parametrize("tokens,dim,heads", [(1, 64, 2), (1, 8, 2), (2, 64, 2), (1, 256, 4), (1, 128, 6), (1, 40, 16), (3, 32, 4), (8, 128, 2), (1, 96, 8), (7, 200, 2)])
+def test_one_to_eight_rows_of_a_key_head(tokens, dim, heads, window, dtype):
+    L = 733
+    lengths, offsets = [L, 0, 1, 400, 90, 600], [L - tokens, 0, 0, 400 - tokens, 88, 650]
+    compare((len(lengths), tokens, heads, 2, dim, L), window, dtype, offsets, lengths, seed=10)
+
+
+@pytest.mark.gpu
+def test_a_few_rows_with_scores_that_are_not_finite():
+    q, k, v, _ = (t.cuda() for t in make(1, 1, 4, 2, 64, 300, torch.float32, seed=11))
+    want = window_attention(q, k, v, 299, offsets=299)
+    for bad, finite in ((math.nan, False), (math.inf, False), (-math.inf, True)):
+        x = k.clone()
+        x[0, 200, 0] = torch.sign(q[0, 0, 0]) * bad if bad == bad else bad  # (the first query's score of this state)
+        out = window_attention(q, x, v, 299, offsets=299)
+        assert torch.equal(out[0, 0, 2:], want[0, 0, 2:]) and bool(out[0, 0, 0].isfinite().all()) == finite
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("dim", [20, 64, 128])
 def test_unread_states_may_hold_anything(dtype, dim):
     N, T, L, window = 4, 70, 400, (30, 0, 5)
@@ -341,16 +362,15 @@ def parts_of(case):
         j0, sink = t * tile, t < sink_tiles
         lo = token(j0 - after - offset) * G
         hi = (T if j0 < sinks else token(min(j0 + tile, length) - 1 + before + 1 - offset)) * G
-        first, count = lo // step, max(0, -(-hi // step) - lo // step)
+        count = -(-max(0, hi - lo) // step)
         each = -(-count // sink_parts) if sink else per
-        walked = [first + p * each + i for p in range(sink_parts if sink else parts) for i in range(max(0, min(each, count - p * each)))]
-        assert len(walked) == len(set(walked)) and (sink or parts * per >= count)
-        assert sorted(walked) == list(range(first, first + count))
-        seen.update((t, r) for r in walked)
+        walked = [p * each + i for p in range(sink_parts if sink else parts) for i in range(max(0, min(each, count - p * each)))]
+        assert walked == list(range(count)) and (sink or parts * per >= count)
+        seen.update((t, row) for i in walked for row in range(lo + i * step, lo + (i + 1) * step))
     ok = allowed_states(T, L, before, after, sinks, offset, length)
     for i, j in ok.nonzero().tolist():
         for g in range(G):
-            assert (j // tile, (i * G + g) // step) in seen
+            assert (j // tile, i * G + g) in seen
     return seen
 
 
