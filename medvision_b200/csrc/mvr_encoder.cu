@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <numeric>
 
 #include "../../include/mvr.h"
 #include "mvr_norm.cuh"
@@ -33,12 +34,17 @@ struct NormCut {
   long long sums, slopes, bytes;
 };
 
+// Whether rows can be taken in vectors of V channels: a block of whole groups and whole vectors is one group, or fits a CTA's threads.
+bool vectors_fit(const mvr_group_norm* a, int V) {
+  const long long width = a->C / a->groups, groups = V / std::gcd(width, (long long)V);
+  return a->C % V == 0 && (groups == 1 || groups * width / V <= kNormThreads);
+}
 int vector_of(const mvr_group_norm* a, bool backward) {
   uintptr_t all = (uintptr_t)a->x | (uintptr_t)(backward ? a->grad_x : a->out);
   if (backward) all |= (uintptr_t)a->grad_out;
   const int whole = 16 / size_of(a->dtype);
-  if (a->C % whole == 0 && all % 16 == 0) return whole;
-  if (whole == 8 && a->C % 4 == 0 && all % 8 == 0) return 4;
+  if (vectors_fit(a, whole) && all % 16 == 0) return whole;
+  if (whole == 8 && vectors_fit(a, 4) && all % 8 == 0) return 4;
   return 1;
 }
 
@@ -217,7 +223,7 @@ long long norm_bytes(const mvr_group_norm* a, bool backward) {
   // (the vector is a matter of the call's addresses)
   long long most = 0;
   for (int V : {1, 4, 8})
-    if (V * size_of(a->dtype) <= 16 && a->C % V == 0) most = std::max(most, cut_norm(a, backward, V).bytes);
+    if (V * size_of(a->dtype) <= 16 && vectors_fit(a, V)) most = std::max(most, cut_norm(a, backward, V).bytes);
   return most;
 }
 

@@ -34,6 +34,8 @@ int64_t padded_size(const Attention& s, const at::Tensor& q, const at::Tensor& k
   const int64_t D = q.size(3), padded = (D + 7) / 8 * 8;
   if (q.scalar_type() == at::kFloat || D == padded || padded > 128) return D;
   double states = (double)k.size(1);
+  // (a few tokens over long sequences: copying all of their states would cost more than the products with those in the window)
+  if (s.in_window && q.size(1) < k.size(1) / 4) return D;
   if (s.in_window) states = std::min(states, (double)s.window.before + (double)s.window.after + 1 + (double)s.window.sinks);
   const double scores = (double)q.size(0) * q.size(1) * q.size(2) * states;
   return scores >= 1 << 22 ? padded : D;

@@ -98,7 +98,11 @@ SHAPES = [  # shape, groups
     ((2, 1000, 64), 8),
     ((1, 5000, 8), 8),            # one channel a group
     ((2, 777, 84), 7),
-    ((1, 3, 2600), 1),            # more vectors than threads
+    ((1, 3, 2600), 1),
+    ((2, 7, 5000), 1),            # a group of more vectors than a CTA has threads
+    ((1, 200, 9000), 3),
+    ((1, 5, 8008), 8),            # vectors over two groups, and more of them than threads
+    ((2, 9, 4100), 4),
     ((1, 40, 2056), 257),
     ((300, 49, 32), 4),           # many small images
     ((2, 4097, 320), 32),
