@@ -20,6 +20,7 @@ struct AttnParams {
   const void *q, *k, *v, *g;                     // g: gradient of the output (backward)
   void *out, *gq, *gk, *gv;                      // out, gq: (R, T, Hq, D); gk, gv: (N, L, Hk, D); all contiguous
   const void* o;                                 // the forward's output (backward)
+  __nv_bfloat16* rest;                           // (R, T, Hq, D) or null: what the rounding of the output to a half type left
   float *lse, *delta;                            // (R, T, Hq); lse in powers of two: log2 of the sum of 2^(s log2 e)
   float* norm;                                   // (R, T, Hq): |g| (float16 gradients)
   int* peaks;                                    // (N, Hk): largest |v| of the states that are read, float bits (float16 gradients)
@@ -329,6 +330,12 @@ __global__ void __launch_bounds__(256) attn_join(const __grid_constant__ AttnPar
 #pragma unroll
   for (int i = 0; i < W; ++i) out.v[i] = from_float<T>(o[i] * inv);
   *(Vec<T, W>*)((T*)p.out + row * p.D + d) = out;
+  if (p.rest) {
+    Vec<__nv_bfloat16, W> rest;
+#pragma unroll
+    for (int i = 0; i < W; ++i) rest.v[i] = from_float<__nv_bfloat16>(o[i] * inv - to_float(out.v[i]));
+    *(Vec<__nv_bfloat16, W>*)(p.rest + row * p.D + d) = rest;
+  }
   if (p.lse && d == 0) p.lse[row] = l == 0.0f ? -INFINITY : ref + log2f(l);
 }
 
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__(256) attn_delta(const __grid_constant__ AttnPa
   const T* g = (const T*)p.g + r * p.g_r + t * p.g_t + h * p.g_h;
   const T* o = (const T*)p.o + row * p.D;
   float v = 0.0f;
-  for (int d = lane; d < p.D; d += 32) v += to_float(g[d]) * to_float(o[d]);
+  for (int d = lane; d < p.D; d += 32) v += to_float(g[d]) * (to_float(o[d]) + (p.rest ? to_float(p.rest[row * p.D + d]) : 0.0f));
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
   if (lane == 0) p.delta[row] = v;

@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_fwd(const __grid_constan
       if (d >= p.D) continue;
       if (p.splits > 1) p.part_o[(split * rows + row) * p.D + d] = acc[i][c];
       else ((T*)p.out)[row * p.D + d] = from_float<T>(acc[i][c] * inv);
+      if (WINDOW && sizeof(T) == 2 && p.rest && p.splits == 1)
+        p.rest[row * p.D + d] = from_float<__nv_bfloat16>(acc[i][c] * inv - to_float(from_float<T>(acc[i][c] * inv)));
     }
     if (tx == 0) {
       if (p.splits > 1) {

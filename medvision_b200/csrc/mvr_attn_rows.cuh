@@ -233,7 +233,9 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_fwd(const __grid_const
     const long long row = ((long long)n * p.T + token) * p.Hq + hk * p.G + (r - token * p.G);
     if (d < p.D) {
       if (p.splits > 1) p.part_o[(split * number + row) * p.D + d] = o;
-      else ((T*)p.out)[row * p.D + d] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+      const float result = l == 0.0f ? 0.0f : o / l;
+      if (p.splits == 1) ((T*)p.out)[row * p.D + d] = from_float<T>(result);
+      if (p.splits == 1 && p.rest) p.rest[row * p.D + d] = from_float<__nv_bfloat16>(result - to_float(from_float<T>(result)));
     }
     if (d == 0) {
       if (p.splits > 1) {

@@ -571,6 +571,14 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
               for (int e = 0; e < 4; ++e)
                 u[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
               *(uint4*)(to + i) = make_uint4(u[0], u[1], u[2], u[3]);
+              if (MODE == kWindow && p.rest) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = floats(*(const Two<T>*)&u[e]);
+                  u[e] = pack2<__nv_bfloat16>(__uint_as_float(v[i + 2 * e]) * inv - f.x, __uint_as_float(v[i + 2 * e + 1]) * inv - f.y);
+                }
+                *(uint4*)(p.rest + row * p.D + q * 32 + i) = make_uint4(u[0], u[1], u[2], u[3]);
+              }
             }
           }
         };

@@ -522,6 +522,9 @@ __global__ void __launch_bounds__(TcRows<DP, MODE, PIECES>::kThreads, TcRows<DP,
 attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcRows<DP, MODE, PIECES> F;
   constexpr bool MASK = MODE != kAll;
+  // A window's slopes in two pieces: those of a row sum to 0, so that with few states dq is the smaller part of what is summed, and one rounding
+  // of each to a half type was up to 1.2 times as far off as the rounding of dq itself.
+  constexpr bool kRest = MODE == kWindow && PIECES == 1;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // Q, G, then the ring
@@ -646,6 +649,11 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
                      (PIECES == 1 && i > 0) || e > 0 || !first);
             }
           });
+          if constexpr (kRest) {
+#pragma unroll
+            for (int e = 0; e < F::kStep / 16; ++e)
+              mma_ts(tmem + F::kSums, tmem + F::kSlopes + (e >> 1) * 32 + 16 + (e & 1) * 8, ring_mn + (((k % F::kSlots) * F::kSlotBytes + e * 2048) >> 4), d_shape, true);
+          }
           mma_commit(smem_at(&c.empty[k % F::kSlots]));
         }
         __syncwarp();
@@ -737,7 +745,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
       bar_pass(smem_at(&c.scores), i & 1, lost);
       tc_fence_after();
       const int col = part_of * 32;
-      uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
+      uint32_t v[32], u[16], u1[PIECES == 1 && !kRest ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
       tc_fence_before();
@@ -762,8 +770,13 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
         if (bits != ~0u) ds = make_float2((bits >> (2 * e)) & 1 ? ds.x : 0.0f, (bits >> (2 * e + 1)) & 1 ? ds.y : 0.0f);
         if constexpr (PIECES == 1) u[e] = pack2<T>(ds.x, ds.y);
         else pieces_of(ds, u[e], u1[e], u2[e]);
+        if constexpr (kRest) {
+          const float2 f = floats(*(const Two<T>*)&u[e]);
+          u1[e] = pack2<T>(ds.x - f.x, ds.y - f.y);
+        }
       }
       tmem_store16(tmem + lanes + F::kSlopes + col, u);
+      if constexpr (kRest) tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
       if constexpr (PIECES == 3) {
         tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
         tmem_store16(tmem + lanes + F::kThird + col / 2, u2);
@@ -844,10 +857,12 @@ __global__ void __launch_bounds__(kDeltaThreads) attn_tc_delta(const __grid_cons
     if (mine && piece < per) {
       const Vec<T, 8> g = *(const Vec<T, 8>*)((const T*)p.g + w.r * p.g_r + w.t * p.g_t + w.h * p.g_h + piece * 8);
       const Vec<T, 8> out = *(const Vec<T, 8>*)((const T*)p.o + row * p.D + piece * 8);
+      Vec<__nv_bfloat16, 8> rest = {};
+      if (p.rest) rest = *(const Vec<__nv_bfloat16, 8>*)(p.rest + row * p.D + piece * 8);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = to_float(g.v[e]);
-        v += a * to_float(out.v[e]);
+        v += a * (to_float(out.v[e]) + to_float(rest.v[e]));
         if (TcType<T>::code == 0) square += a * a;
       }
     }

@@ -12,6 +12,7 @@ struct Attention {
   bool in_window = false;           // ops.window_attention: a window instead of index and mask
   mvr_window window = {};           // without the address of `offsets`
   at::Tensor offsets;               // or undefined
+  at::Tensor rest;                  // what the rounding of the result left, or undefined
   const char* name() const { return in_window ? "window_attention" : "cross_attention"; }
 };
 
@@ -77,6 +78,7 @@ mvr_window window_of(const Attention& s) {
     w.offsets = data_or_null(s.offsets);
     w.offsets_64 = s.offsets.scalar_type() == at::kLong;
   }
+  if (s.rest.defined()) w.rest = data_or_null(s.rest);
   return w;
 }
 
@@ -88,7 +90,7 @@ at::Tensor workspace_of(const Attention& s, const mvr_attention& a, bool backwar
 
 struct AttentionBackward : public torch::autograd::Node {
   Attention s;
-  SavedVariable q, k, v, out, lse, index, lengths, mask, offsets;
+  SavedVariable q, k, v, out, lse, index, lengths, mask, offsets, rest;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -99,6 +101,7 @@ struct AttentionBackward : public torch::autograd::Node {
     args.lengths = lengths.unpack();
     args.mask = mask.unpack();
     args.offsets = offsets.unpack();
+    args.rest = rest.unpack();
     if (!grads[0].defined()) return result;
     {
       at::NoGradGuard no_grad;
@@ -134,7 +137,7 @@ struct AttentionBackward : public torch::autograd::Node {
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* t : {&q, &k, &v, &out, &lse, &index, &lengths, &mask, &offsets}) t->reset_data();
+    for (SavedVariable* t : {&q, &k, &v, &out, &lse, &index, &lengths, &mask, &offsets, &rest}) t->reset_data();
   }
   std::string name() const override { return s.in_window ? "WindowAttentionBackward" : "CrossAttentionBackward"; }
 };
@@ -194,6 +197,9 @@ at::Tensor attention(const at::Tensor& query, const at::Tensor& key, const at::T
     const at::Tensor ws = workspace_of(s, a, false, q);
     out = at::empty(q.sizes(), query.options().requires_grad(false));
     if (graph) lse = at::empty({R, query.size(1), query.size(2)}, out.options().dtype(at::kFloat));
+    // (a token with few states has slopes that are differences of near numbers: with the result as it is rounded they lose up to three times as
+    // much as the rounding of a gradient)
+    if (graph && s.in_window && query.scalar_type() != at::kFloat) s.rest = at::empty(q.sizes(), out.options().dtype(at::kBFloat16));
     a.out = data_or_null(out);
     a.lse = (float*)data_or_null(lse);
     void* workspace = ws.defined() ? ws.data_ptr() : nullptr;
@@ -211,6 +217,7 @@ at::Tensor attention(const at::Tensor& query, const at::Tensor& key, const at::T
     node->s.in_window = s.in_window;
     node->s.window = s.window;
     node->offsets = SavedVariable(s.offsets, false);
+    node->rest = SavedVariable(s.rest, false);
     node->q = SavedVariable(query, false);
     node->k = SavedVariable(key, false);
     node->v = SavedVariable(value, false);

@@ -122,8 +122,10 @@ bool vectors_aligned(const void* base, const int64_t (&strides)[3], const int64_
 bool tc_window(const mvr_attention* a, const mvr_window* w) {
   const double rows = (double)a->R * a->T * a->Hq;
   if (a->L == 0 || a->N == 0 || a->N > INT32_MAX / 4 || rows > 2e9) return false;
-  if (a->dtype != MVR_F32) return a->D % 8 == 0 && a->D <= 128;
   const Window s = window_of(a, w);
+  // (a few tiles of rows against one of states are as fast in float arithmetic, which rounds nothing on its way)
+  if (a->T * (a->Hq / a->Hk) <= 256 && std::min<long long>(a->L, reach(a, s, a->T) + s.sinks) <= 64) return false;
+  if (a->dtype != MVR_F32) return a->D % 8 == 0 && a->D <= 128;
   return a->D <= 64 && a->T >= a->L / 4 && rows * std::min<long long>(a->L, reach(a, s, 1) + s.sinks) >= kPieceScores;
 }
 
@@ -168,6 +170,7 @@ AttnParams window_params(const mvr_attention* a, const mvr_window* given, const 
   const Window w = window_of(a, given);
   p.before = w.before; p.after = w.after; p.sinks = (int)w.sinks;
   p.offsets = given->offsets; p.offsets64 = given->offsets_64;
+  if (a->dtype != MVR_F32) p.rest = (__nv_bfloat16*)given->rest;
   p.offset = std::max<long long>(-(1ll << 40), std::min<long long>(given->offset, 1ll << 40));
   p.splits = c.splits; p.tiles_per = c.tiles_per;
   p.row_splits = c.row_splits; p.row_tiles_per = c.row_tiles_per; p.sink_tiles = c.sink_tiles; p.sink_parts = c.sink_parts;
@@ -247,7 +250,7 @@ int window_forward(const AttnParams& p, const WindowCut& c, Way way, const TcMap
   }
   if (rc != MVR_OK || c.splits == 1) return rc;
   const long long outputs = (long long)p.R * p.T * p.Hq * p.D;
-  if (p.D % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(T)) == 0)
+  if (p.D % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(T)) == 0 && (uintptr_t)p.rest % 8 == 0)
     launch_dependent(attn_join<T, 4>, dim3((unsigned)cdiv(outputs, 1024)), dim3(256), 0, st, p);
   else
     launch_dependent(attn_join<T, 1>, dim3((unsigned)cdiv(outputs, 256)), dim3(256), 0, st, p);
@@ -335,7 +338,7 @@ int window_as(const mvr_attention* a, const mvr_window* w, bool backward, char* 
     }
   }
   if constexpr (sizeof(T) == 2) {
-    tc = tc && (uintptr_t)a->out % 16 == 0 && rows_aligned(a->q, a->q_strides, a);
+    tc = tc && ((uintptr_t)a->out | (uintptr_t)w->rest) % 16 == 0 && rows_aligned(a->q, a->q_strides, a);
     if (backward)
       tc = tc && rows_aligned(a->grad_out, a->g_strides, a) && (((uintptr_t)a->grad_q | (uintptr_t)a->grad_k | (uintptr_t)a->grad_v) & 15) == 0;
     tc = tc && tensor_maps<T>(a, backward, 1, maps, boxes);

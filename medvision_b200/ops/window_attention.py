@@ -23,7 +23,7 @@ def window_attention(query, key, value, before, after=0, sinks=0, offsets=None, 
     A token that reads no state gives zeros, and no gradients.  States that no token of their sequence reads may hold anything; one
     that is not finite and read by some may spoil the tokens near them.
     Returns a contiguous tensor of the query's shape and type.  Sums, weights and statistics are held in float32 and the
-    result is rounded once; for float16 and bfloat16 the weights are rounded to that type before they meet the values, and the
-    gradients are formed with the rounded result.
+    result is rounded once; for float16 and bfloat16 the weights, and in the gradients the scores' slopes, are rounded to that type
+    before they meet the values (keys, queries).
     """
     return _C._native.window_attention(query, key, value, before, after, sinks, offsets, lengths, scale)
