@@ -54,6 +54,12 @@ struct AttnParams {
 };
 
 // ---- sliding window -----------------------------------------------------------------------------------
+// The kernels walk, of a tile of rows, the tiles that hold the union of its rows' states, from the union's own first state on; scores beyond a
+// row's own window are masked where a tile has any (a row's bits are two shifts), states that no row of the tile reads are zeroed as masked
+// ones are.  Bound as without a window, by a step's chain, and by what a tile's rows read together more than each by itself: 128 rows of four
+// heads a token read 32 + 1023 states of a window of 1024, 128 states meet 128 + 1023 tokens.  2 x 8192 tokens, 16 heads of 64 on 4,
+// bfloat16: forward 0.14 ms, dk and dv 0.25, dq 0.22.  All tokens read the first states, so that their rows are cut into parts as long
+// as the other tiles' and summed by a kernel of their own.
 // A token at place p reads the states [p - before, p + after] and, of the first `sinks`, those up to p + after: [lo, hi) and [0, sink).
 struct Span {
   int lo, hi, sink;

@@ -11,6 +11,12 @@
 //             second time where they lie
 // No atomics: each sum has one place and one order.
 //
+// Measured, bfloat16 rows of 32 channels, groups of 4, silu, 2 x 128^3 rows (268 MB): moments 52 us (5.1 TB/s), elements 106 (5.0), slopes' sums
+// 119 (4.5), dx 152 (5.3); of a copy's rate 70 to 80 %, issue slots 40 % busy and the function units 43 to 64: what is left is a thread's
+// chain of loads, exponentials and stores at 24 warps an SM (loads a step ahead do not fit the registers backward).  The second read comes
+// from memory: 63 MB of L2 are near an SM, and all chunks are walked at once.  2 x 48^3 rows of 64 halves: 20 us forward, 38 backward.
+// 2 x 512 rows of 256 halves by clusters 4.8 us, in passes 7.3.
+//
 // Statistics.  A thread sums x - k and (x - k)^2 about its own first value k of a channel, over its r rows.  If k lies far from the others,
 // the thread's sum of squares about its mean is itself at least (r - 1) / r of that distance's square, so that cancellation costs no
 // more than some r of its last bits, whatever the data's offset; the same holds where a thread joins threads or chunks about the first
