@@ -99,6 +99,9 @@ __global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, P
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcStates<DP, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
+  // A window's slopes in two pieces, as in dq: with states read by a few rows one rounding of each was up to 1.57 times as far off as the plain
+  // form, with two 1.05.  The second product costs 6 % of a training step (2 x 8192 tokens, windows of 1024 + 4, bf16: 627 to 665 us).
+  constexpr bool kRest = WINDOW && PIECES == 1;
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of the stages
   typename F::Control& c = *(typename F::Control*)(base + 2 * PIECES * F::kTileBytes + 2 * F::kStages * F::kStageBytes);
@@ -192,6 +195,11 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
               mma_ts(tmem + to, tmem + at, steps_mn + ((right * F::kStageBytes + b * F::kStepBytes + i * 2048) >> 4), d_shape, (PIECES == 1 && add) || i > 0 || !first);
             }
           });
+          if (kRest && from == F::kSlopes) {
+#pragma unroll
+            for (int i = 0; i < F::kStep / 16; ++i)
+              mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + 16 + (i & 1) * 8, steps_mn + ((right * F::kStageBytes + i * 2048) >> 4), d_shape, true);
+          }
         }
         __syncwarp();
       };
@@ -385,7 +393,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       // rows that do not read this state
       const uint32_t bits = WINDOW ? bits_below(row_hi - (first + i * F::kStep + col)) & ~bits_below(row_lo - (first + i * F::kStep + col)) : ~0u;
       float2 w[16];
-      uint32_t v[32], u[16], u1[PIECES == 1 ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
+      uint32_t v[32], u[16], u1[PIECES == 1 && !kRest ? 1 : 16], u2[PIECES == 1 ? 1 : 16];
       tmem_load32(v, tmem + lanes + F::kScores + col);
       tmem_wait_load();
 #pragma unroll
@@ -427,9 +435,14 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           if (WINDOW && bits != ~0u) ds = make_float2((bits >> (e + 2 * k)) & 1 ? ds.x : 0.0f, (bits >> (e + 2 * k + 1)) & 1 ? ds.y : 0.0f);
           if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(ds.x, ds.y);
           else pieces_of(ds, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
+          if constexpr (kRest) {
+            const float2 f = floats(*(const Two<T>*)&u[e / 2 + k]);
+            u1[e / 2 + k] = pack2<T>(ds.x - f.x, ds.y - f.y);
+          }
         }
       }
       tmem_store16(tmem + lanes + F::kSlopes + col, u);
+      if constexpr (kRest) tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
       if constexpr (PIECES == 3) {
         tmem_store16(tmem + lanes + F::kSlopes + col + 16, u1);
         tmem_store16(tmem + lanes + F::kThird + F::kStep / 2 + col / 2, u2);
