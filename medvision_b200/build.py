@@ -14,7 +14,7 @@ NATIVE = os.path.join(HERE, "_native.so")
 SOURCES = ["mvr_api.cu", "mvr_heads.cu", "mvr_window.cu", "mvr_encoder.cu"]  # one object file each
 HEADERS = ["mvr_arith.cuh", "mvr_geom.cuh", "mvr_generic.cuh", "mvr_stream3d.cuh", "mvr_tma3d.cuh", "mvr_brick3d.cuh", "mvr_bwd3d.cuh", "mvr_offset.cuh", "mvr_cubic3d.cuh", "mvr_flat.cuh", "mvr_label.cuh", "mvr_plane2d.cuh", "mvr_elastic.cuh", "mvr_head.cuh",
            os.path.join("..", "..", "include", "mvr.h")]
-ATTENTION_HEADERS = ["mvr_types.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_attn_host.cuh", "mvr_tc.cuh",
+ATTENTION_HEADERS = ["mvr_types.cuh", "mvr_span.cuh", "mvr_attn.cuh", "mvr_attn_fma.cuh", "mvr_attn_tc.cuh", "mvr_attn_tc_bwd.cuh", "mvr_attn_host.cuh", "mvr_tc.cuh",
                      os.path.join("..", "..", "include", "mvr.h")]
 HEADERS_OF = {"mvr_api.cu": HEADERS, "mvr_heads.cu": ATTENTION_HEADERS + ["mvr_dropout.cuh", "mvr_logprob.cuh"], "mvr_window.cu": ATTENTION_HEADERS + ["mvr_attn_rows.cuh"],
               "mvr_encoder.cu": ["mvr_types.cuh", "mvr_norm.cuh", "mvr_rotary.cuh", os.path.join("..", "..", "include", "mvr.h")]}

@@ -12,6 +12,7 @@
 // regions are grouped by image first, in their order (attn_plan): `order` lists them image by image, `starts` says where each
 // image's begin, and a last group holds those whose image is not in [0, N): no states, zero results.
 #pragma once
+#include "mvr_span.cuh"
 #include "mvr_types.cuh"
 
 namespace mvr {
@@ -44,7 +45,7 @@ struct AttnParams {
   float *part_gq, *part_gk, *part_gv;            // splits > 1: (split, row, D), (split, N, L, Hk, D)
   int row_splits;
   // sliding window (ops.window_attention): no index, no mask
-  long long before, after;                       // token t stands at offset + t; see Span
+  long long before, after;                       // token t stands at offset + t; see mvr_span.cuh
   int sinks;
   const void* offsets;                           // (N) int32 or int64, or null: `offset` for all
   int offsets64;
@@ -60,39 +61,10 @@ struct AttnParams {
 // heads a token read 32 + 1023 states of a window of 1024, 128 states meet 128 + 1023 tokens.  2 x 8192 tokens, 16 heads of 64 on 4,
 // bfloat16: forward 0.14 ms, dk and dv 0.25, dq 0.22.  All tokens read the first states, so that their rows are cut into parts as long
 // as the other tiles' and summed by a kernel of their own.
-// A token at place p reads the states [p - before, p + after] and, of the first `sinks`, those up to p + after: [lo, hi) and [0, sink).
-struct Span {
-  int lo, hi, sink;
-};
-__device__ __forceinline__ long long first_place(const AttnParams& p, int n) {
-  if (!p.offsets) return p.offset;
-  const long long v = p.offsets64 ? ((const long long*)p.offsets)[n] : ((const int*)p.offsets)[n];
-  return max(-(1ll << 40), min(v, 1ll << 40));  // (beyond every state either way)
+__device__ __forceinline__ Places places_of(const AttnParams& p, int n) {
+  const long long offset = !p.offsets ? p.offset : p.offsets64 ? ((const long long*)p.offsets)[n] : ((const int*)p.offsets)[n];
+  return places_from(offset, p.before, p.after);
 }
-// Of the tokens at the places `first` to `last`, together: consecutive places leave no gap between their windows.
-__device__ __forceinline__ Span span_of(const AttnParams& p, long long first, long long last, int end) {
-  Span s;
-  s.hi = (int)max(0ll, min(last + p.after + 1, (long long)end));
-  s.lo = (int)max(0ll, min(first - p.before, (long long)s.hi));
-  s.sink = min(p.sinks, s.hi);
-  return s;
-}
-__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-// Which of the states j to j + 31 lie in it.
-__device__ __forceinline__ uint32_t span_bits(const Span& s, int j) {
-  return (bits_below(s.hi - j) & ~bits_below(s.lo - j)) | bits_below(s.sink - j);
-}
-// The tiles of STEP states that hold a span: those of the first states, then those of the window from its own beginning on.
-template <int STEP>
-struct SpanTiles {
-  int sinks, from, count;
-  __device__ __forceinline__ SpanTiles(const Span& s) {
-    sinks = (s.sink + STEP - 1) / STEP;
-    from = max(s.lo, sinks * STEP);  // (what lies before is in the first ones' tiles)
-    count = sinks + max(0, s.hi - from + STEP - 1) / STEP;
-  }
-  __device__ __forceinline__ int first(int i) const { return i < sinks ? i * STEP : from + (i - sinks) * STEP; }
-};
 
 // Rows of a tile: image n (N: none), its regions, and where the tile begins among the rows of one key head.
 struct RowTile {
@@ -158,56 +130,6 @@ __device__ __forceinline__ int states_of(const AttnParams& p, int n) {
   if (!p.lengths) return p.L;
   const long long l = p.lengths64 ? ((const long long*)p.lengths)[n] : ((const int*)p.lengths)[n];
   return l < 0 ? 0 : l < p.L ? (int)l : p.L;
-}
-
-// ---- a window's gradients of keys and values ------------------------------------------------------------
-// A CTA takes a tile of states and a part of the rows whose windows reach it.  All tokens may read the first tiles, so those are cut
-// into more parts, which come first: sink_parts of each of the sink_tiles of an image, then row_splits of each of the others.
-struct StateTile {
-  int n, tile, part;
-  bool sink;
-};
-__device__ __forceinline__ StateTile state_tile(const AttnParams& p, int state_tiles) {
-  const int leading = p.N * p.sink_tiles * p.sink_parts;
-  StateTile s;
-  s.sink = (int)blockIdx.x < leading;
-  const int at = blockIdx.x - (s.sink ? 0 : leading), parts = s.sink ? p.sink_parts : p.row_splits;
-  const int number = at / parts, tiles = s.sink ? p.sink_tiles : state_tiles - p.sink_tiles;
-  s.part = at - number * parts;
-  s.n = number / tiles;
-  s.tile = number - s.n * tiles + (s.sink ? 0 : p.sink_tiles);
-  return s;
-}
-// Rows of a key head that read state j: [lo, hi).
-__device__ __forceinline__ int token_at(const AttnParams& p, long long token) { return (int)max(0ll, min(token, (long long)p.T)); }
-__device__ __forceinline__ void rows_of_state(const AttnParams& p, long long place0, int j, int& lo, int& hi) {
-  lo = token_at(p, j - p.after - place0) * p.G;
-  hi = (j < p.sinks ? p.T : token_at(p, j + p.before + 1 - place0)) * p.G;
-}
-// The part's tiles of `step` rows for the states from j0 on, `size` of them: the first row, and how many tiles.
-struct TileRows {
-  int first, count;
-};
-__device__ __forceinline__ TileRows rows_of_states(const AttnParams& p, const StateTile& s, long long place0, int j0, int size, int step) {
-  int lo, hi, unused;
-  rows_of_state(p, place0, j0, lo, hi);
-  if (j0 >= p.sinks) rows_of_state(p, place0, min(j0 + size, states_of(p, s.n)) - 1, unused, hi);
-  const int all = max(0, hi - lo + step - 1) / step;
-  const int per = s.sink ? (all + p.sink_parts - 1) / p.sink_parts : p.row_tiles_per;
-  return {lo + s.part * per * step, max(0, min(per, all - s.part * per))};
-}
-// Where a state's sums of a part go: parts of the first tiles lie before those of the others, each without the other's states.
-struct PartPlace {
-  bool parts;
-  long long at;
-};
-__device__ __forceinline__ PartPlace part_place(const AttnParams& p, const StateTile& s, int j, int hk, int tile) {
-  const long long lead = min((long long)p.L, (long long)p.sink_tiles * tile), states = s.sink ? lead : p.L - lead, row = (long long)p.Hk * p.D;
-  PartPlace r;
-  r.parts = (s.sink ? p.sink_parts : p.row_splits) > 1;
-  r.at = (((long long)s.part * p.N + s.n) * states + (s.sink ? j : j - lead)) * row + (long long)hk * p.D;
-  if (!s.sink && p.sink_parts > 1) r.at += p.sink_parts * (p.N * lead * row);
-  return r;
 }
 
 // ---- grouping of regions by image ---------------------------------------------------------------------

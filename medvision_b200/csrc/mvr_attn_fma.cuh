@@ -167,12 +167,12 @@ struct FmaWindow {
   Span span, own[F::MT];
   int first, last;  // tiles of the span
   __device__ __forceinline__ FmaWindow(const AttnParams& p, const RowTile& o, int split, int ty) {
-    const long long place0 = first_place(p, o.n);
+    const Places at = places_of(p, o.n);
     const int end = states_of(p, o.n);
-    const auto place = [&](int row) { return place0 + p.by_G.quotient(min(row, o.rows - 1)); };
-    span = span_of(p, place(o.first), place(o.first + F::BT - 1), end);
+    const auto token = [&](int row) { return p.by_G.quotient(min(row, o.rows - 1)); };
+    span = span_of(p, at, token(o.first), token(o.first + F::BT - 1), end);
 #pragma unroll
-    for (int i = 0; i < F::MT; ++i) own[i] = span_of(p, place(o.first + ty * F::MT + i), place(o.first + ty * F::MT + i), end);
+    for (int i = 0; i < F::MT; ++i) own[i] = span_of(p, at, token(o.first + ty * F::MT + i), token(o.first + ty * F::MT + i), end);
     first = split * p.tiles_per;
     last = min(first + p.tiles_per, SpanTiles<F::BT>(span).count);
   }
@@ -337,22 +337,23 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
         *allowed = ws + F::BT * F::LP, *lse = allowed + F::BT, *delta = lse + F::BT;
   grid_dependency();
   const int tiles = (p.L + F::BT - 1) / F::BT, hk = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const StateTile st = WINDOW ? state_tile(p, tiles) : StateTile{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles, (int)blockIdx.z, false};
+  const StateTile st = WINDOW ? state_tile(p, blockIdx.x, tiles) : StateTile{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles, (int)blockIdx.z, false};
   const int n = st.n, j0 = st.tile * F::BT, split = st.part;
   __shared__ FmaRows<F::BT> at;
   const RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::BT - 1) / F::BT, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   const bool any = fma_allowed(allowed, p, n, j0, states_of(p, n), F::BT);
   int first = any ? split * per * F::BT : 0, last = any ? min(o.rows, (split + 1) * per * F::BT) : 0;
-  const long long place0 = WINDOW ? first_place(p, n) : 0;
+  Places places = {};
   if (WINDOW) {
-    const TileRows r = rows_of_states(p, st, place0, j0, F::BT, F::BT);
+    places = places_of(p, n);
+    const TileRows r = rows_of_states(p, st, places, j0, F::BT, states_of(p, n), F::BT);
     first = any ? r.first : 0;
     last = any ? min(o.rows, r.first + r.count * F::BT) : 0;
   }
   int row_lo[F::MT], row_hi[F::MT];
 #pragma unroll
-  for (int i = 0; i < F::MT; ++i) rows_of_state(p, place0, j0 + ty * F::MT + i, row_lo[i], row_hi[i]);
+  for (int i = 0; i < F::MT; ++i) rows_of_state(p, places, j0 + ty * F::MT + i, row_lo[i], row_hi[i]);
   float dk[F::MT][F::CW] = {}, dv[F::MT][F::CW] = {};
   if (first < last) {
     fma_load_states<T, DP>(ks, (const T*)p.k + (long long)n * p.k_n + (long long)hk * p.k_h, p.k_l, j0, allowed, p.D);

@@ -40,12 +40,12 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_fwd(const __grid_const
   grid_dependency();
   const int n = blockIdx.x, hk = blockIdx.y, split = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % kLanes;
   const int rows = p.T * p.G, end = states_of(p, n);
-  const long long place0 = first_place(p, n);
+  const Places places = places_of(p, n);
   if (threadIdx.x < R) {
-    const long long place = place0 + p.by_G.quotient(min((int)threadIdx.x, rows - 1));
-    spans[threadIdx.x] = span_of(p, place, place, end);
+    const int token = p.by_G.quotient(min((int)threadIdx.x, rows - 1));
+    spans[threadIdx.x] = span_of(p, places, token, token, end);
   }
-  const Span all = span_of(p, place0, place0 + p.T - 1, end);
+  const Span all = span_of(p, places, 0, p.T - 1, end);
   // the states that any row reads, in a row: the first ones, then the window
   const int leading = min(all.sink, all.lo), count = leading + all.hi - all.lo;
   const int per = (count + p.splits - 1) / p.splits, begin = min(count, split * per), stop = min(count, begin + per);

@@ -247,11 +247,14 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
   if (MODE == kListed && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
   // a window: the states that any of the tile's rows reads, and this part's tiles of them
-  const long long place0 = MODE == kWindow && some ? first_place(p, o.n) : 0;
-  const int states = MODE == kWindow && some ? states_of(p, o.n) : 0;
+  Places at = {};
+  int states = 0;
   Span span = {};
-  if (MODE == kWindow && some)
-    span = span_of(p, place0 + p.by_G.quotient(o.first), place0 + p.by_G.quotient(min(o.first + TILES * kTcRows, o.rows) - 1), states);
+  if (MODE == kWindow && some) {
+    at = places_of(p, o.n);
+    states = states_of(p, o.n);
+    span = span_of(p, at, p.by_G.quotient(o.first), p.by_G.quotient(min(o.first + TILES * kTcRows, o.rows) - 1), states);
+  }
   const SpanTiles<F::kStep> window(span);
   const int window_first = split * p.tiles_per;
   tc_fence_before();
@@ -386,7 +389,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       const bool mine = j0 < o.rows;
       if (mine) w = row_of(p, o, j0, hk);
       Span own = {};  // of this row
-      if (MODE == kWindow && mine) own = span_of(p, place0 + w.t, place0 + w.t, states);
+      if (MODE == kWindow && mine) own = span_of(p, at, w.t, w.t, states);
       if (tiles > 0) {
         const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
         if (F::kHalves == 1)

@@ -125,7 +125,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == kIssuer) tmem_alloc(smem_at(&c.tmem), F::kColumns);
   const int state_tiles = (p.L + 127) / 128, hk = blockIdx.y;
-  const StateTile st = WINDOW ? state_tile(p, state_tiles) : StateTile{(int)blockIdx.x / state_tiles, (int)blockIdx.x % state_tiles, (int)blockIdx.z, false};
+  const StateTile st = WINDOW ? state_tile(p, blockIdx.x, state_tiles) : StateTile{(int)blockIdx.x / state_tiles, (int)blockIdx.x % state_tiles, (int)blockIdx.z, false};
   const int n = st.n, j0 = st.tile * 128, split = st.part;
   // one row a thread: its state, and whether it is read
   const int r = ((warp & 3) << 5) + lane, part_of = warp >> 2, j = j0 + r;
@@ -136,9 +136,9 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   int first = split * per * F::kStep, count = any ? max(0, min(row_tiles, (split + 1) * per) - split * per) : 0, row_lo = 0, row_hi = 0;  // first: row
   if (WINDOW) {
-    const long long place0 = first_place(p, n);
-    rows_of_state(p, place0, j, row_lo, row_hi);  // (one state a thread)
-    const TileRows r = rows_of_states(p, st, place0, j0, 128, F::kStep);
+    const Places at = places_of(p, n);
+    rows_of_state(p, at, j, row_lo, row_hi);  // (one state a thread)
+    const TileRows r = rows_of_states(p, st, at, j0, 128, states_of(p, n), F::kStep);
     first = r.first;
     count = any ? r.count : 0;
   }
@@ -570,11 +570,14 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
   int end = 0;
   if (some) end = min(states_of(p, o.n), (split + 1) * per * F::kStep);
   if (MODE == kListed && some && begin < end) list_tiles(p, o.n, begin, end, c.list, c.bits, &c.tiles);
-  const long long place0 = MODE == kWindow && some ? first_place(p, o.n) : 0;
-  const int states = MODE == kWindow && some ? states_of(p, o.n) : 0;
+  Places places = {};
+  int states = 0;
   Span span = {};
-  if (MODE == kWindow && some)
-    span = span_of(p, place0 + p.by_G.quotient(o.first), place0 + p.by_G.quotient(min(o.first + kTcRows, o.rows) - 1), states);
+  if (MODE == kWindow && some) {
+    places = places_of(p, o.n);
+    states = states_of(p, o.n);
+    span = span_of(p, places, p.by_G.quotient(o.first), p.by_G.quotient(min(o.first + kTcRows, o.rows) - 1), states);
+  }
   const SpanTiles<F::kStep> window(span);
   const int window_first = split * p.tiles_per;
   tc_fence_before();
@@ -708,7 +711,7 @@ attn_tc_dq(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps 
     }
     if (mine) {
       w = row_of(p, o, j0, hk);
-      if (MODE == kWindow) own = span_of(p, place0 + w.t, place0 + w.t, states);
+      if (MODE == kWindow) own = span_of(p, places, w.t, w.t, states);
       number = row_number(p, w);
       if (tiles > 0) {
         lse = p.lse[number];

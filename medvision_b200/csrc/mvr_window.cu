@@ -25,18 +25,11 @@ struct WindowCut : OperandPieces {
   long long delta, norm, peaks, row_peaks, part_o, part_ml, part_gq, part_gk, part_gv, bytes;
 };
 
-// What a call reads beside its operands' sizes, limited to what matters: places are below 2^41 either way.
-struct Window {
-  long long before, after, sinks;
-};
-Window window_of(const mvr_attention* a, const mvr_window* w) {
-  return {std::min<long long>(w->before, INT32_MAX), std::min<long long>(w->after, INT32_MAX), std::min<long long>(w->sinks, a->L)};
-}
-// The most states that `tokens` neighbouring tokens read in their windows.
-long long reach(const mvr_attention* a, const Window& w, long long tokens) { return std::min<long long>(a->L, tokens + w.before + w.after); }
+// Its sizes.
+WindowSizes sizes_of(const mvr_attention* a, const mvr_window* w) { return window_sizes(a->T, a->L, a->Hq / a->Hk, w->before, w->after, w->sinks); }
 
 WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backward, Way way) {
-  const Window w = window_of(a, given);
+  const WindowSizes w = sizes_of(a, given);
   WindowCut c = {};
   const bool tc = c.tc = way == kTensorCores;
   const bool pieces = tc && a->dtype == MVR_F32, wide = a->D > 64;
@@ -47,17 +40,13 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
   c.state_tile = tc ? 128 : c.tile;
   // the kernels' own steps through the states (the forward, dq) and the rows (dk, dv)
   const int step = !tc ? c.tile : backward ? (wide ? kGradStep<128> : kGradStep<64>) : c.tile > kTcRows ? 128 : 64;
-  const auto tiles_of = [&](long long size) {
-    const long long tokens = std::min<long long>(a->T, cdiv(c.tile, G) + 1);
-    return std::max<long long>(1, std::min(cdiv(a->L, size), cdiv(reach(a, w, tokens), size) + 1 + cdiv(w.sinks, size)));
-  };
   // (a part's sums are written and read at 4 MB/us)
-  c.splits = best_parts(std::max<long long>(1, c.row_tiles * a->Hk), tiles_of(c.state_tile), states_step(tc, pieces, backward, wide, c.tile > kTcRows),
+  c.splits = best_parts(std::max<long long>(1, c.row_tiles * a->Hk), w.span_tiles(c.tile, c.state_tile), states_step(tc, pieces, backward, wide, c.tile > kTcRows),
                         rows * a->D * 8 / 4e6, false);
-  c.tiles_per = (int)cdiv(tiles_of(step), c.splits);
+  c.tiles_per = (int)cdiv(w.span_tiles(c.tile, step), c.splits);
   if (way == kFewRows) {
     // four CTAs an SM (eight: up to 15 % slower), with 128 states each at least (64: 9.4 us instead of 6.8 for 8 caches' windows of 500)
-    const long long states = reach(a, w, a->T) + w.sinks, ctas = std::max<long long>(1, a->N * a->Hk);
+    const long long states = w.reach(a->T) + w.sinks, ctas = std::max<long long>(1, a->N * a->Hk);
     c.splits = (int)std::max<long long>(1, std::min<long long>({64, cdiv(4 * kMultiprocessors, ctas), cdiv(states, 128)}));
   }
   c.sink_tiles = (int)cdiv(w.sinks, c.state_tile);
@@ -65,11 +54,10 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
   const long long others = cdiv(a->L, c.state_tile) - c.sink_tiles, lead = std::min<long long>(a->L, (long long)c.sink_tiles * c.state_tile);
   if (backward) {
     // rows of a tile that the first states do not belong to; the first ones, which meet all rows, are cut into parts as long
-    const long long reached = std::min<long long>(a->T, c.state_tile + w.before + w.after) * G;
-    c.row_splits = best_parts(std::max<long long>(1, a->N * a->Hk * others), std::max<long long>(1, cdiv(reached, c.tile)), rows_step(tc, pieces, wide),
+    c.row_splits = best_parts(std::max<long long>(1, a->N * a->Hk * others), std::max<long long>(1, cdiv(w.rows_reached(c.state_tile), c.tile)), rows_step(tc, pieces, wide),
                               (double)a->N * (a->L - lead) * a->Hk * a->D * 16 / 4e6, false);
-    c.row_tiles_per = (int)std::max<long long>(1, cdiv(std::min(cdiv(per, step), cdiv(reached, step) + 1), c.row_splits));
-    if (c.sink_tiles > 0) c.sink_parts = (int)std::max<long long>(1, std::min<long long>(64, cdiv(cdiv(per, step), c.row_tiles_per)));
+    c.row_tiles_per = w.row_tiles(c.state_tile, step, c.row_splits);
+    if (c.sink_tiles > 0) c.sink_parts = w.sink_parts(step, c.row_tiles_per);
   }
   long long at = 0;
   const auto take = [&at](long long bytes) {
@@ -122,11 +110,11 @@ bool vectors_aligned(const void* base, const int64_t (&strides)[3], const int64_
 bool tc_window(const mvr_attention* a, const mvr_window* w) {
   const double rows = (double)a->R * a->T * a->Hq;
   if (a->L == 0 || a->N == 0 || a->N > INT32_MAX / 4 || rows > 2e9) return false;
-  const Window s = window_of(a, w);
+  const WindowSizes s = sizes_of(a, w);
   // (a few tiles of rows against one of states are as fast in float arithmetic, which rounds nothing on its way)
-  if (a->T * (a->Hq / a->Hk) <= 256 && std::min<long long>(a->L, reach(a, s, a->T) + s.sinks) <= 64) return false;
+  if (a->T * (a->Hq / a->Hk) <= 256 && std::min<long long>(a->L, s.reach(a->T) + s.sinks) <= 64) return false;
   if (a->dtype != MVR_F32) return a->D % 8 == 0 && a->D <= 128;
-  return a->D <= 64 && a->T >= a->L / 4 && rows * std::min<long long>(a->L, reach(a, s, 1) + s.sinks) >= kPieceScores;
+  return a->D <= 64 && a->T >= a->L / 4 && rows * std::min<long long>(a->L, s.reach(1) + s.sinks) >= kPieceScores;
 }
 
 int check_window(const mvr_attention* a, const mvr_window* w, bool backward, bool sizes_only) {
@@ -167,11 +155,10 @@ AttnParams window_params(const mvr_attention* a, const mvr_window* given, const 
   p.by_G.set((unsigned)p.G);
   p.scale = a->scale;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  const Window w = window_of(a, given);
-  p.before = w.before; p.after = w.after; p.sinks = (int)w.sinks;
+  p.before = given->before; p.after = given->after; p.sinks = (int)std::min<long long>(given->sinks, a->L);
   p.offsets = given->offsets; p.offsets64 = given->offsets_64;
   if (a->dtype != MVR_F32) p.rest = (__nv_bfloat16*)given->rest;
-  p.offset = std::max<long long>(-(1ll << 40), std::min<long long>(given->offset, 1ll << 40));
+  p.offset = given->offset;
   p.splits = c.splits; p.tiles_per = c.tiles_per;
   p.row_splits = c.row_splits; p.row_tiles_per = c.row_tiles_per; p.sink_tiles = c.sink_tiles; p.sink_parts = c.sink_parts;
   p.delta = (float*)(ws + c.delta); p.norm = (float*)(ws + c.norm); p.peaks = (int*)(ws + c.peaks); p.row_peaks = (float2*)(ws + c.row_peaks);
