@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
   const StateTile st = WINDOW ? state_tile(p, blockIdx.x, tiles) : StateTile{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles, (int)blockIdx.z, false};
   const int n = st.n, j0 = st.tile * F::BT, split = st.part;
   __shared__ FmaRows<F::BT> at;
-  const RowTile o = image_rows(p, n);
+  RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::BT - 1) / F::BT, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   const bool any = fma_allowed(allowed, p, n, j0, states_of(p, n), F::BT);
   int first = any ? split * per * F::BT : 0, last = any ? min(o.rows, (split + 1) * per * F::BT) : 0;
@@ -348,6 +348,7 @@ __global__ void __launch_bounds__(kFmaThreads) attn_fma_dkv(const __grid_constan
   if (WINDOW) {
     places = places_of(p, n);
     const TileRows r = rows_of_states(p, st, places, j0, F::BT, states_of(p, n), F::BT);
+    o.rows = r.end;  // (rows behind read none of the states, and may hold NaN)
     first = any ? r.first : 0;
     last = any ? min(o.rows, r.first + r.count * F::BT) : 0;
   }

@@ -79,7 +79,7 @@ struct TcStates {
   static constexpr int kColumns = PIECES == 1 ? 2 * kStep + 2 * DP : 512;
   static constexpr int kResident = DP == 64 && PIECES == 1 ? 2 : 1;
   struct Control {
-    unsigned long long states, full[kStages], empty[kStages], scores, slopes, weights, grads, done;
+    unsigned long long states, full[kStages], empty[kStages], landed, scores, slopes, weights, grads, done;
     uint32_t tmem;
     int lost, peak[3];  // peak: largest |v|, |g|, |delta| (float bits)
     alignas(16) float lse[kStages][kStep];    // negative
@@ -113,6 +113,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       bar_init(smem_at(&c.full[i]), F::kLoaders / 32);
       bar_init(smem_at(&c.empty[i]), 1);
     }
+    bar_init(smem_at(&c.landed), 1);
     bar_init(smem_at(&c.scores), 1);
     bar_init(smem_at(&c.slopes), 1);
     bar_init(smem_at(&c.weights), F::kGroups / 32);
@@ -135,11 +136,13 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   const RowTile o = image_rows(p, n);
   const int row_tiles = (o.rows + F::kStep - 1) / F::kStep, per = (row_tiles + p.row_splits - 1) / p.row_splits;
   int first = split * per * F::kStep, count = any ? max(0, min(row_tiles, (split + 1) * per) - split * per) : 0, row_lo = 0, row_hi = 0;  // first: row
+  int end = o.rows;  // (a window: rows behind read none of the states, and may hold NaN)
   if (WINDOW) {
     const Places at = places_of(p, n);
     rows_of_state(p, at, j, row_lo, row_hi);  // (one state a thread)
     const TileRows r = rows_of_states(p, st, at, j0, 128, states_of(p, n), F::kStep);
     first = r.first;
+    end = r.end;
     count = any ? r.count : 0;
   }
   // what lies behind D in the rows' tiles stays 0
@@ -250,7 +253,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
         const int at = first + i * F::kStep + (warp - kLoader) * 32 + k * F::kLoaders + lane;
         q[k] = g[k] = ~0u;
         lse[k] = INFINITY, delta[k] = 0.0f;  // no row: P = 0
-        if (i < count && at < o.rows) {
+        if (i < count && at < end) {
           const Row row = row_of(p, o, at, hk);
           if (!BOXES) q[k] = (unsigned)((row.r * p.q_r + row.t * p.q_t + row.h * p.q_h) >> 3);
           if (!BOXES) g[k] = (unsigned)((row.r * p.g_r + row.t * p.g_t + row.h * p.g_h) >> 3);
@@ -267,7 +270,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const char *q_piece = (const char*)p.q + (there ? piece * 16 : 0), *g_piece = (const char*)p.g + (there ? piece * 16 : 0);
     const uint32_t to_block = smem_at(base + 2 * PIECES * F::kTileBytes) + (piece >> 3) * (F::kStep * 128);
     look_up(0);
-    bool pending = false;
+    bool pending = false, cleared = false;
     int i = 0;
     for (; i < count; ++i) {
       const int stage = i % F::kStages;
@@ -295,21 +298,35 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       if (BOXES) {
         const uint32_t bar = smem_at(&c.full[stage]), to = smem_at(base + 2 * PIECES * F::kTileBytes) + 2 * stage * F::kStageBytes;
         __syncwarp();
+        // Rows of the box behind the last that reads a state (of the last tile): zero before the products see them.  (They are 0 times 0 there, but
+        // 0 times NaN otherwise.)  Such a box lands at a barrier of its own.
+        cleared = WINDOW && end < o.rows && first + (i + 1) * F::kStep > end;
         if (warp != kLoader) {
           bar_arrive_warp(bar);
         } else if (elect_one()) {
-          bar_expect(bar, 2 * F::kStageBytes);
+          const uint32_t on = cleared ? smem_at(&c.landed) : bar;
+          bar_expect(on, 2 * F::kStageBytes);
           const int token = p.by_G.quotient(first + i * F::kStep);
 #pragma unroll
           for (int part = 0; part < PIECES; ++part)
 #pragma unroll
             for (int b = 0; b < F::kBlocks; ++b) {
               const uint32_t at = to + part * F::kStepBytes + b * F::kStep * 128;
-              tma_load_4d(at, &maps.q, bar, b * 64, hk * p.G, token, n + part * p.R);
-              tma_load_4d(at + F::kStageBytes, &maps.g, bar, b * 64, hk * p.G, token, n + part * p.R);
+              tma_load_4d(at, &maps.q, on, b * 64, hk * p.G, token, n + part * p.R);
+              tma_load_4d(at + F::kStageBytes, &maps.g, on, b * 64, hk * p.G, token, n + part * p.R);
             }
         }
         __syncwarp();
+        if (WINDOW && cleared && warp == kLoader) {
+          bar_pass(smem_at(&c.landed), 0, lost);
+          char* rows = base + 2 * PIECES * F::kTileBytes + 2 * stage * F::kStageBytes;  // blocks of kStep rows, of Q and then of G
+          for (int row = end - (first + i * F::kStep) + lane; row < F::kStep; row += 32)
+#pragma unroll
+            for (int b = 0; b < 2 * PIECES * F::kBlocks; ++b)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) *(uint4*)(rows + (b * F::kStep + row) * 128 + (((k + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          arrived(stage);
+        }
         look_up(i + 1);
         continue;
       }
@@ -329,6 +346,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (BOXES && *lost && warp == kLoader) {  // given up: the copies under way end, or the limit passes, before the CTA does
       const unsigned long long t = nanoseconds();
+      while (cleared && !bar_try(smem_at(&c.landed), 0) && nanoseconds() - t < kWaitLimit) {}
       for (int k = max(0, i - F::kStages); k < i; ++k)
         while (!bar_try(smem_at(&c.full[k % F::kStages]), (k / F::kStages) & 1) && nanoseconds() - t < kWaitLimit) {}
     }
@@ -338,7 +356,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     if (count > 0 && TcType<T>::code == 0) {
       float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of a tile of rows
       const int before = o.order ? p.tiles[n] : n * ((o.rows + kTcRows - 1) / kTcRows);
-      for (int t = first / kTcRows + threadIdx.x; t * kTcRows < min(o.rows, first + count * F::kStep); t += F::kGroups) {
+      for (int t = first / kTcRows + threadIdx.x; t * kTcRows < min(end, first + count * F::kStep); t += F::kGroups) {
         const float2 peak = p.row_peaks[(long long)(before + t) * p.Hk + hk];
         most[1] = fmaxf(most[1], peak.x);
         most[2] = fmaxf(most[2], peak.y);

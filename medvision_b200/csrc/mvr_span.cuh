@@ -88,9 +88,10 @@ MVR_EVERYWHERE void rows_of_state(const P& p, const Places& at, int j, int& lo, 
   lo = (int)larger(0, smaller(j + 1 - at.hi, p.T)) * p.G;
   hi = (j < p.sinks ? p.T : (int)larger(0, smaller(j + 1 - at.lo, p.T))) * p.G;
 }
-// The part's tiles of `step` rows for the states from j0 on, `size` of them, among `end`: the first row, and how many tiles.
+// The part's tiles of `step` rows for the states from j0 on, `size` of them, among `end`: the first row, how many tiles, and behind which row
+// none reads any of the states: what such a row holds may not come near their sums.
 struct TileRows {
-  int first, count;
+  int first, count, end;
 };
 template <typename P>
 MVR_EVERYWHERE TileRows rows_of_states(const P& p, const StateTile& s, const Places& at, int j0, int size, int end, int step) {
@@ -100,7 +101,7 @@ MVR_EVERYWHERE TileRows rows_of_states(const P& p, const StateTile& s, const Pla
   const int all = (hi > lo ? hi - lo + step - 1 : 0) / step;
   const int per = s.sink ? (all + p.sink_parts - 1) / p.sink_parts : p.row_tiles_per;
   const int left = all - s.part * per;
-  return {lo + s.part * per * step, left < 0 ? 0 : left < per ? left : per};
+  return {lo + s.part * per * step, left < 0 ? 0 : left < per ? left : per, hi};
 }
 // Where a state's sums of a part go: parts of the first tiles lie before those of the others, each without the other's states.
 struct PartPlace {

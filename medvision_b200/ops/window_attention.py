@@ -20,8 +20,9 @@ def window_attention(query, key, value, before, after=0, sinks=0, offsets=None, 
         lengths (Tensor): int32 or int64 (sequences,): only the first ``lengths[n]`` states of a sequence are read
         scale (float): None stands for dim ** -0.5
 
-    A token that reads no state gives zeros, and no gradients.  States that no token of their sequence reads may hold anything; one
-    that is not finite and read by some may spoil the tokens near them.
+    A token that reads no state gives zeros, and no gradients, whatever it and its gradient hold.  States that no token of their sequence
+    reads may hold anything; one that is not finite and read by some may spoil the tokens near them, and a query or gradient that is not finite
+    the gradients of states near those that its token reads.
     Returns a contiguous tensor of the query's shape and type.  Sums, weights and statistics are held in float32 and the
     result is rounded once; for float16 and bfloat16 the weights, and in the gradients the scores' slopes, are rounded to that type
     before they meet the values (keys, queries).

@@ -1,11 +1,14 @@
-"""ops.window_attention at the ends of what its arguments may be: places and reaches beyond 32 bits."""
+"""ops.window_attention at the ends of what its arguments may be: places and reaches beyond 32 bits, and tokens
+that read nothing, whatever they hold."""
+import math
+
 import pytest
 import torch
 
 from medvision_b200.ops import window_attention
 
 from test_cross_attention import HALF, NAMES, check
-from test_window_attention import compare, make, reference, run
+from test_window_attention import allowed_states, compare, make, reference, run
 
 
 @pytest.mark.gpu
@@ -32,3 +35,25 @@ def test_one_far_place_for_all_sequences():
             check(a, b, c, name)
     none = window_attention(q.cuda(), k.cuda(), v.cuda(), 10 ** 9, 10 ** 9, offsets=3 * 10 ** 9)
     assert not bool(none.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("heads,dim", [((4, 2), 64), ((2, 2), 128), ((6, 2), 64), ((3, 1), 128), ((8, 1), 32), ((2, 1), 20), ((2, 2), 200), ((1, 1), 96)])
+def test_tokens_that_read_nothing_may_hold_anything(heads, dim, dtype):
+    """Padded tokens behind short sequences, tokens before all states, sequences without states: their queries and incoming gradients come
+    near no sum of another token's or state's, in no bit."""
+    N, T, L, window = 5, 400, 400, (30, 0)
+    offsets, lengths = [0, 0, -150, 37, 0], [150, 277, 400, 100, 0]
+    q, k, v, g = make(N, T, *heads, dim, L, dtype, seed=22)
+    kw = dict(offsets=torch.tensor(offsets, device="cuda"), lengths=torch.tensor(lengths, device="cuda"))
+    clean = run(q, k, v, g, *window, **kw)
+    nothing = torch.stack([~allowed_states(T, L, *window, 0, o, n).any(1) for o, n in zip(offsets, lengths)])
+    assert bool(nothing.any(1).all()) and not bool(nothing[:4].all(1).any())
+    for bad_q, bad_g in ((math.nan, math.nan), (math.inf, -math.inf), (0.5, math.nan), (math.nan, 0.5)):
+        x, y = q.clone(), g.clone()
+        x[nothing], y[nothing] = bad_q, bad_g
+        got = run(x, k, v, y, *window, **kw)
+        for a, b in zip(got, clean):
+            assert torch.equal(a, b)
+        assert not bool(got[0][nothing].any()) and not bool(got[1][nothing].any())

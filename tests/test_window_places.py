@@ -68,7 +68,7 @@ int walk_rows(const int64_t* a, const int64_t* offsets, const int64_t* ends, int
     const int j0 = s.tile * tile;
     const TileRows r = rows_of_states(p, s, at, j0, tile, (int)ends[s.n], step);
     if (j0 < ends[s.n])  // (else the kernel walks nothing)
-      for (int row = r.first; row < r.first + r.count * step && row < rows; ++row) ++seen[((int64_t)s.n * state_tiles + s.tile) * rows + row];
+      for (int row = r.first; row < r.first + r.count * step && row < r.end; ++row) ++seen[((int64_t)s.n * state_tiles + s.tile) * rows + row];
     for (int j = j0; j < j0 + tile && j < p.L; ++j) {
       const PartPlace to = part_place(p, s, j, 0, tile);
       if (to.parts) place[((int64_t)s.n * parts + s.part) * p.L + j] = to.at;
@@ -170,7 +170,7 @@ def test_the_parts_of_a_state_tile_walk_every_row_that_reads_it_once(lib):
             walked = np.array(seen).reshape(N, tiles, T, G)
             for n in range(N):
                 for i in range(tiles):
-                    assert (walked[n, i][read[n][:, i * tile:(i + 1) * tile].any(1)] == 1).all()
+                    assert (walked[n, i] == read[n][:, i * tile:(i + 1) * tile].any(1)[:, None]).all()  # (others may hold anything)
             # a place of its own for every part's sums of every state, one behind another
             lead = min(L, -(-min(sinks, L) // tile) * tile)
             want = N * ((sink_parts * lead if sink_parts > 1 else 0) + (splits * (L - lead) if splits > 1 else 0))
