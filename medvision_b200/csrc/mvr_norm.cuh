@@ -260,6 +260,9 @@ __device__ __forceinline__ Moments team_join(const NormTeam& team, const Moments
   return m;
 }
 
+// A sum of squares about a mean, whose rounding may have left it below 0; NaN (of values that are not finite) stays.
+__device__ __forceinline__ float not_negative(float square) { return square < 0.0f ? 0.0f : square; }
+
 // A thread's sums about a pivot, of a vector of channels.
 template <typename T, int V>
 struct NormMoments {
@@ -282,7 +285,7 @@ struct NormMoments {
   __device__ __forceinline__ Moments of(int k, float count, float inverse) const {
     const float s = k & 1 ? sum.v[k >> 1].y : sum.v[k >> 1].x, q = k & 1 ? square.v[k >> 1].y : square.v[k >> 1].x,
                 c = k & 1 ? pivot.v[k >> 1].y : pivot.v[k >> 1].x, mean = s * inverse;
-    return moments_of(c, mean, fmaxf(0.0f, fmaf(-mean, s, q)), count);
+    return moments_of(c, mean, not_negative(fmaf(-mean, s, q)), count);
   }
   // SPAN neighbouring channels from k on, together
   template <int SPAN>
@@ -447,7 +450,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_apply(const __grid_const
       square += fmaf(v.count * d, d, v.square);
     });
     const float shift = sum / count;
-    told[i] = moments_of(first.mean, first.rest + shift, fmaxf(0.0f, fmaf(-shift, sum, square)), count);
+    told[i] = moments_of(first.mean, first.rest + shift, not_negative(fmaf(-shift, sum, square)), count);
   }
   __syncthreads();
   join_rows(told, parts, p.block_groups);
