@@ -20,9 +20,10 @@
 //
 // float16 has few small numbers: P is scaled by 2^10 on its way to dV, and dS by a power of two that brings a bound of |dS| <= |g.v| +
 // |delta| to 2^14.  Where rows are kept every row has its own, from |g| of the row (2-norms, by attn_tc_delta) and the largest |v| of the
-// states of its image and key head (by the first kernel).  Where states are kept it is one power a CTA, from the largest |v| of its 128 states
+// states of its image and key head (by the first kernel; in a window, of the tiles of 128 states that it walks).  Where states are kept it is one power a CTA, from the largest |v| of its 128 states
 // and the largest |g| and |delta| of the rows that it walks: delta averages the values of all states and has to be counted by itself.  So
-// no gradient depends, in its bits or its range, on rows that have nothing to do with it.  Both are taken out of the sums again, exactly.
+// no gradient depends, in its bits or its range, on rows that have nothing to do with it (in a window: on states that no token reads, tokens that
+// read none, and rows that read none of the CTA's states).  Both are taken out of the sums again, exactly.
 #pragma once
 #include <type_traits>
 
@@ -354,15 +355,25 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float factor = 1.0f;  // of dS
     if (count > 0 && TcType<T>::code == 0) {
-      float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of a tile of rows
-      const int before = o.order ? p.tiles[n] : n * ((o.rows + kTcRows - 1) / kTcRows);
-      for (int t = first / kTcRows + threadIdx.x; t * kTcRows < min(end, first + count * F::kStep); t += F::kGroups) {
+      float most[3] = {};  // |v| of this thread's state, if it is read; |g|, |delta| of rows, whole tiles of them together
+      const int before = o.order ? p.tiles[n] : n * ((o.rows + kTcRows - 1) / kTcRows), stop = min(end, first + count * F::kStep);
+      // (a window's walk begins and ends within tiles: their rows one by one)
+      const int tile0 = WINDOW ? (first + kTcRows - 1) / kTcRows : first / kTcRows, tile1 = WINDOW && stop < o.rows ? stop / kTcRows : (stop + kTcRows - 1) / kTcRows;
+      for (int t = tile0 + threadIdx.x; t < tile1; t += F::kGroups) {
         const float2 peak = p.row_peaks[(long long)(before + t) * p.Hk + hk];
         most[1] = fmaxf(most[1], peak.x);
         most[2] = fmaxf(most[2], peak.y);
       }
+      if (WINDOW) {
+        const int head = min(stop, tile0 * kTcRows), tail = max(head, tile1 * kTcRows), alone = head - first + max(0, stop - tail);
+        for (int i = threadIdx.x; i < alone; i += F::kGroups) {
+          const long long number = row_number(p, row_of(p, o, first + i < head ? first + i : tail + (first + i - head), hk));
+          most[1] = fmaxf(most[1], finite_or_0(p.norm[number]));
+          most[2] = fmaxf(most[2], finite_or_0(fabsf(p.delta[number])));
+        }
+      }
       bar_pass(smem_at(&c.states), 0, lost);
-      if (in && part_of == 0) {
+      if (in && part_of == 0 && (!WINDOW || row_lo < row_hi)) {
         const char* row = base + F::kTileBytes + r * 128;
 #pragma unroll
         for (int piece = 0; piece < DP / 8; ++piece) {
@@ -908,8 +919,10 @@ __global__ void __launch_bounds__(kDeltaThreads) attn_tc_delta(const __grid_cons
       p.delta[row] = v;
       if (TcType<T>::code == 0) {
         p.norm[row] = sqrtf(square);
-        most = fmaxf(most, finite_or_0(sqrtf(square)));
-        most_delta = fmaxf(most_delta, finite_or_0(fabsf(v)));
+        if (p.lse[row] != -INFINITY) {  // (it reads a state)
+          most = fmaxf(most, finite_or_0(sqrtf(square)));
+          most_delta = fmaxf(most_delta, finite_or_0(fabsf(v)));
+        }
       }
     }
   }

@@ -57,3 +57,30 @@ def test_tokens_that_read_nothing_may_hold_anything(heads, dim, dtype):
         for a, b in zip(got, clean):
             assert torch.equal(a, b)
         assert not bool(got[0][nothing].any()) and not bool(got[1][nothing].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("heads", [(2, 2), (6, 2)])
+@pytest.mark.parametrize("loud", ["query", "key"])
+def test_float16_ranges_go_by_what_is_read(loud, heads, dim):
+    """Slopes of weights are brought to float16's range by bounds of the values and of the incoming gradients: not by those of states and
+    tokens that have no part in them, however large.  Here the slopes are as small as the largest factor leaves them; queries (or keys) of
+    2^12 bring their gradients' products back to float16's normal numbers."""
+    N, T, L, window = 3, 128, 400, (63, 0)
+    offsets, lengths = [100, 0, 270], [400, 60, 330]
+    q, k, v, g = make(N, T, *heads, dim, L, torch.float32, seed=23)
+    up, down = (q, k) if loud == "query" else (k, q)
+    up *= 2.0 ** 12
+    down *= 2.0 ** -12
+    q, k, v, g = q.half(), k.half(), (v / 64).half(), (g * 2.0 ** -14).half()
+    read = torch.stack([allowed_states(T, L, *window, 0, o, n) for o, n in zip(offsets, lengths)])
+    v[~read.any(1)], g[~read.any(2)] = 0.0, 0.0
+    kw = dict(offsets=torch.tensor(offsets, device="cuda"), lengths=torch.tensor(lengths, device="cuda"))
+    clean = run(q, k, v, g, *window, **kw)
+    assert bool(clean[1 + (loud == "query")].any())
+    for in_v, in_g in ((6e4, 0.0), (0.0, -6e4), (-6e4, 6e4)):
+        x, y = v.clone(), g.clone()
+        x[~read.any(1)], y[~read.any(2)] = in_v, in_g
+        for a, b in zip(run(q, k, x, y, *window, **kw), clean):
+            assert torch.equal(a, b)
