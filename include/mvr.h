@@ -326,6 +326,8 @@ typedef struct mvr_group_norm {
   const void *x, *weight, *bias;
   void* out;
   float *mean, *rstd;                    /* (N, groups): written by the forward, read by the backward */
+  float *mean_rest;                      /* the same: what the mean's rounding to a float left; or null (0): far from 0 the
+                                            gradients then lose the mean's rounding against the deviation */
   const void* grad_out;                  /* backward only, from here on */
   void *grad_x, *grad_weight, *grad_bias;
 } mvr_group_norm;

@@ -37,7 +37,7 @@ class Window(ctypes.Structure):
 class GroupNorm(ctypes.Structure):
     """struct mvr_group_norm of include/mvr.h."""
     _fields_ = [("dtype", _i32), ("parameter_dtype", _i32), ("activation", _i32), ("eps", _f32)] + [(n, _i64) for n in ("N", "S", "C", "groups")] + \
-        [(n, _vp) for n in ("x", "weight", "bias", "out", "mean", "rstd", "grad_out", "grad_x", "grad_weight", "grad_bias")]
+        [(n, _vp) for n in ("x", "weight", "bias", "out", "mean", "rstd", "mean_rest", "grad_out", "grad_x", "grad_weight", "grad_bias")]
 
 
 class Rotary(ctypes.Structure):

@@ -138,7 +138,7 @@ NormParams norm_params(const mvr_group_norm* a, const NormCut& c, char* ws) {
   NormParams p = {};
   p.x = a->x; p.dy = a->grad_out; p.weight = a->weight; p.bias = a->bias;
   p.out = a->out; p.dx = a->grad_x; p.dweight = a->grad_weight; p.dbias = a->grad_bias;
-  p.mean = a->mean; p.rstd = a->rstd;
+  p.mean = a->mean; p.rstd = a->rstd; p.rest = a->mean_rest;
   p.moments = (Moments*)(ws + c.sums); p.sums = (float2*)(ws + c.sums); p.slopes = (float2*)(ws + c.slopes);
   p.S = a->S; p.rows = c.rows;
   p.N = (int)a->N; p.C = (int)a->C; p.groups = (int)a->groups; p.width = (int)(a->C / a->groups);
@@ -184,8 +184,8 @@ template <typename T, int V, bool WHOLE, int ACT>
 int norm_as(NormParams& p, const NormCut& c, bool backward, cudaStream_t st) {
   const long long ctas = (long long)p.N * c.chunks * c.blocks;
   const int channel_ctas = p.dweight || p.dbias ? (int)cdiv(p.C, 32) : 0;
-  // (the second passes: two numbers a group, and what the threads have joined)
-  const size_t joined = std::max<size_t>(kNormThreads, c.block_groups), groups = (size_t)c.block_groups * 8 + 16;
+  // (the second passes: three numbers a group, or two, and what the threads have joined)
+  const size_t joined = std::max<size_t>(kNormThreads, c.block_groups), groups = (size_t)c.block_groups * 12 + 16;
   int rc;
   if (!backward) {
     if (c.clusters) return launch_norm<norm_cluster<T, V, WHOLE, ACT>>(p, ctas, c.shared, c.chunks, st);

@@ -21,7 +21,9 @@
 // the thread's sum of squares about its mean is itself at least (r - 1) / r of that distance's square, so that cancellation costs no
 // more than some r of its last bits, whatever the data's offset; the same holds where a thread joins threads or chunks about the first
 // one's mean.  Channels, threads and chunks are joined by their means' differences, for
-// which a mean is kept as two floats: rounded to one, means near 1e5 of values with a deviation of 2 put an error of 1e-4 into their variance.
+// which a mean is kept as two floats: rounded to one, means near 1e5 of values with a deviation of 2 put an error of 1e-4 into their variance,
+// and 2e-3 into every xhat of a group.  What a mean's rounding left is taken out of a channel's bias, of its sum of dz xhat and of dx's constant
+// part, so that it costs no value an operation.
 #pragma once
 #include "mvr_types.cuh"
 
@@ -37,7 +39,7 @@ struct alignas(16) Moments {
 struct NormParams {
   const void *x, *dy, *weight, *bias;  // (N, S, C) twice; (C), or null: 1 and 0
   void *out, *dx, *dweight, *dbias;
-  float *mean, *rstd;                  // (N, groups)
+  float *mean, *rstd, *rest;           // (N, groups); rest: what the mean's rounding left, or null
   Moments* moments;                    // (N, chunks, groups): forward
   float2 *sums, *slopes;               // (N, chunks, groups): sums of dz w, dz w xhat; (N, chunks, C): of dz, dz xhat
   long long S, rows;                   // rows of a chunk, or of a CTA of a cluster
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_stats(const __grid_const
 }
 
 // ---- normalised rows ----------------------------------------------------------------------------------
-// What belongs to a thread's channels: z = (x - mean) factor + bias.
+// What belongs to a thread's channels: z = (x - mean) factor + bias (less the mean's rest times factor).
 template <typename T, int V, bool WHOLE>
 struct NormChannels {
   typedef FloatPairs<T, V> P;
@@ -388,20 +390,24 @@ struct NormChannels {
       bias.v[k] = make_float2(b[2 * k], b[V == 1 ? 0 : 2 * k + 1]);
     }
   }
-  // `means`, `rstds`: of the groups of the block
-  __device__ __forceinline__ void set(const NormParams& p, int column, const float* means, const float* rstds) {
+  // `means`, `rstds`, `rests` (or null: 0): of the groups of the block
+  __device__ __forceinline__ void set(const NormParams& p, int column, const float* means, const float* rstds, const float* rests) {
     if constexpr (WHOLE) {
       const int g = p.by_width.quotient(column * V);
       mean[0] = two(means[g]);
-      const float2 r = two(rstds[g]);
+      const float2 r = two(rstds[g]), less = two(rests ? -rests[g] : 0.0f);
 #pragma unroll
-      for (int k = 0; k < P::kPairs; ++k) factor.v[k] = mul2(factor.v[k], r);
+      for (int k = 0; k < P::kPairs; ++k) {
+        factor.v[k] = mul2(factor.v[k], r);
+        bias.v[k] = fma2(factor.v[k], less, bias.v[k]);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < P::kPairs; ++k) {
         const int g = p.by_width.quotient(column * V + 2 * k), h = p.by_width.quotient(column * V + 2 * k + 1);
         mean[k] = make_float2(means[g], means[h]);
         factor.v[k] = mul2(factor.v[k], make_float2(rstds[g], rstds[h]));
+        if (rests) bias.v[k] = fma2(factor.v[k], make_float2(-rests[g], -rests[h]), bias.v[k]);
       }
     }
   }
@@ -426,16 +432,33 @@ __device__ __forceinline__ void put_once(V* to, const V& v) {
   else *to = v;
 }
 
+__device__ __forceinline__ void keep_statistics(const NormParams& p, const NormPlace& t, int g, float mean, float rstd, float rest) {
+  const long long at = (long long)t.n * p.groups + t.group + g;
+  p.mean[at] = mean;
+  p.rstd[at] = rstd;
+  if (p.rest) p.rest[at] = rest;
+}
+// Of the groups of a block, as the forward has left them.
+struct NormStatistics {
+  const float *means, *rstds, *rests;
+  __device__ __forceinline__ NormStatistics(const NormParams& p, const NormPlace& t) {
+    const long long at = (long long)t.n * p.groups + t.group;
+    means = p.mean + at;
+    rstds = p.rstd + at;
+    rests = p.rest ? p.rest + at : nullptr;
+  }
+};
+
 template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_apply(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) float norm_groups[];  // the block's means, their inverse deviations, what the threads have joined
   typedef Vec<T, V> Vector;
   grid_dependency();
   const NormPlace t = norm_place(p, blockIdx.x);
-  float *means = norm_groups, *rstds = means + p.block_groups;
+  float *means = norm_groups, *rstds = means + p.block_groups, *rests = rstds + p.block_groups;
   NormChannels<T, V, WHOLE> c(p, t, t.lane);
   // an image's chunks: a thread takes every so many of a group's, then the threads are joined
-  Moments* told = (Moments*)(rstds + p.block_groups + (p.block_groups & 1) * 2);
+  Moments* told = (Moments*)(norm_groups + ((3 * p.block_groups + 3) & ~3));
   const Moments* from = p.moments + (long long)t.n * p.chunks * p.groups + t.group;
   const int parts = min(p.chunks, max(1, kNormThreads / p.block_groups));
   for (int i = threadIdx.x; i < parts * p.block_groups; i += kNormThreads) {
@@ -457,18 +480,16 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_apply(const __grid_const
   for (int g = threadIdx.x; g < p.block_groups; g += kNormThreads) {
     const Moments all = told[g];
     means[g] = all.mean;
+    rests[g] = all.rest;
     rstds[g] = 1.0f / sqrtf(all.square / all.count + p.eps);
-    if (t.chunk == 0) {
-      p.mean[(long long)t.n * p.groups + t.group + g] = means[g];
-      p.rstd[(long long)t.n * p.groups + t.group + g] = rstds[g];
-    }
+    if (t.chunk == 0) keep_statistics(p, t, g, means[g], rstds[g], rests[g]);
   }
   __syncthreads();
   if (t.count == 0) return;
   const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width;
   for (int column = t.lane; column < p.columns; column += p.lanes) {
     if (column != t.lane) c = NormChannels<T, V, WHOLE>(p, t, column);
-    c.set(p, column, means, rstds);
+    c.set(p, column, means, rstds, rests);
     const long long last = first + (t.count - 1) * step + (long long)column * V;
     const T* x = (const T*)p.x + last + step;
     T* out = (T*)p.out + last + step;
@@ -476,19 +497,20 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_apply(const __grid_const
   }
 }
 
-// Shared memory of a CTA of a cluster: what its threads have summed, its groups' sums, its groups' two numbers, then the rows.
+// Shared memory of a CTA of a cluster: what its threads have summed, its groups' sums, its groups' two or three numbers, then the rows.
 struct NormShared {
   char *told, *groups;
-  float *first, *second;
+  float *first, *second, *third;
   char* rows;
   __device__ __forceinline__ NormShared(const NormParams& p, char* base, int told_bytes) {
     told = base;
     groups = told + told_bytes;
     first = (float*)(groups + 16 * p.block_groups);
     second = first + p.block_groups;
+    third = second + p.block_groups;
     rows = base + bytes(told_bytes, p.block_groups);
   }
-  static __host__ __device__ __forceinline__ int bytes(int told, int groups) { return (told + groups * 24 + 15) & ~15; }
+  static __host__ __device__ __forceinline__ int bytes(int told, int groups) { return (told + groups * 28 + 15) & ~15; }
 };
 
 template <typename T, int V, bool WHOLE, int ACT>
@@ -519,14 +541,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_cluster(const __grid_con
     }
     sh.first[g] = all.mean;
     sh.second[g] = 1.0f / sqrtf(all.square / all.count + p.eps);
-    if (t.chunk == 0) {
-      p.mean[(long long)t.n * p.groups + t.group + g] = sh.first[g];
-      p.rstd[(long long)t.n * p.groups + t.group + g] = sh.second[g];
-    }
+    sh.third[g] = all.rest;
+    if (t.chunk == 0) keep_statistics(p, t, g, sh.first[g], sh.second[g], sh.third[g]);
   }
   __syncthreads();
   if (t.count > 0) {
-    c.set(p, t.lane, sh.first, sh.second);
+    c.set(p, t.lane, sh.first, sh.second, sh.third);
     T* out = (T*)p.out + first;
     walk<4>(t.count, [&](int i) { return rows[i * next]; }, [&](int i, const Vector& v) { *(Vector*)(out + i * step) = normalised<T, ACT>(v, c); });
   }
@@ -574,7 +594,7 @@ struct NormSlopes {
 // them in `told`[c].  `told`: shared memory, two floats a channel of every thread.  Ends in a barrier.
 template <typename T, int V, typename F>
 __device__ __forceinline__ void channel_sums(const NormParams& p, const NormPlace& t, const NormSlopes<T, V>& mine, float2* told, int columns, int c0,
-                                             const float* rstds, F&& channel) {
+                                             const NormStatistics& of, F&& channel) {
   const int channels = columns * V;
   if (t.depth < p.depth && t.lane < columns) {
 #pragma unroll
@@ -585,7 +605,8 @@ __device__ __forceinline__ void channel_sums(const NormParams& p, const NormPlac
   join_rows(told, p.depth, channels);
   for (int c = threadIdx.x; c < channels; c += kNormThreads) {
     float2 s = told[c];
-    s.y *= rstds[p.by_width.quotient(c0 * V + c)];
+    const int g = p.by_width.quotient(c0 * V + c);
+    s.y = (of.rests ? fmaf(-of.rests[g], s.x, s.y) : s.y) * of.rstds[g];
     told[c] = s;
     channel(c0 * V + c, s);
   }
@@ -598,7 +619,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums(const __grid_consta
   typedef Vec<T, V> Vector;
   grid_dependency();
   const NormPlace t = norm_place(p, blockIdx.x);
-  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  const NormStatistics of(p, t);
   const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
   const long long number = (long long)t.n * p.chunks + t.chunk;
   float2 before = two(0.0f);  // (of the parts of one group)
@@ -607,11 +628,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums(const __grid_consta
     NormSlopes<T, V> s;
     if (t.count > 0 && t.lane < columns) {
       NormChannels<T, V, WHOLE> c(p, t, c0 + t.lane);
-      c.set(p, c0 + t.lane, means, rstds);
+      c.set(p, c0 + t.lane, of.means, of.rstds, of.rests);
       const T *x = (const T*)p.x + first + (long long)c0 * V, *dy = (const T*)p.dy + first + (long long)c0 * V;
       walk<3>(t.count, [&](int) { return load_both<Vector>(x, dy, step); }, [&](int, const Both<Vector>& v) { s.template add<ACT>(v.x, v.dy, c); });
     }
-    channel_sums<T, V>(p, t, s, norm_slopes, columns, c0, rstds, [&](int c, float2 v) { p.slopes[number * p.C + (long long)t.group * p.width + c] = v; });
+    channel_sums<T, V>(p, t, s, norm_slopes, columns, c0, of, [&](int c, float2 v) { p.slopes[number * p.C + (long long)t.group * p.width + c] = v; });
     const int groups = columns < p.columns ? 1 : p.block_groups, width = columns * V / groups;
     const NormTeam team(groups, width);
     team.each(groups, [&](int g, bool there) {
@@ -646,16 +667,16 @@ static __global__ void __launch_bounds__(kNormThreads) norm_parameters(const __g
   parameter_gradients(p, blockIdx.x, shared);
 }
 
-// dx = dz factor - rstd m1 - (x - mean) rstd^2 m2
+// dx = dz factor - rstd m1 - (x - mean) rstd^2 m2, with the mean's rest in the part that is the same for all rows
 template <typename T, int V, bool WHOLE>
 struct NormReturn {
   float2 first[NormChannels<T, V, WHOLE>::kOwn], second[NormChannels<T, V, WHOLE>::kOwn];  // negative
-  // m1, m2, rstds: of the groups of the block
-  __device__ __forceinline__ NormReturn(const NormParams& p, int column, const float* m1, const float* m2, const float* rstds) {
+  // m1, m2: of the groups of the block
+  __device__ __forceinline__ NormReturn(const NormParams& p, int column, const float* m1, const float* m2, const NormStatistics& of) {
 #pragma unroll
     for (int k = 0; k < 2 * NormChannels<T, V, WHOLE>::kOwn; ++k) {
       const int g = p.by_width.quotient(column * V + (k < V ? k : 0));
-      const float a = -rstds[g] * m1[g], b = -rstds[g] * rstds[g] * m2[g];
+      const float rstd = of.rstds[g], b = -rstd * rstd * m2[g], a = fmaf(-rstd, m1[g], of.rests ? -of.rests[g] * b : 0.0f);
       if (k & 1) first[k >> 1].y = a, second[k >> 1].y = b;
       else first[k >> 1].x = a, second[k >> 1].x = b;
     }
@@ -686,7 +707,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_dx(const __grid_constant
     return;
   }
   const NormPlace t = norm_place(p, blockIdx.x - p.channel_ctas);
-  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  const NormStatistics of(p, t);
   float *m1 = norm_groups, *m2 = m1 + p.block_groups;
   NormChannels<T, V, WHOLE> c(p, t, t.lane);
   const float all = (float)p.S * p.width;
@@ -708,8 +729,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_dx(const __grid_constant
   const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width;
   for (int column = t.lane; column < p.columns; column += p.lanes) {
     if (column != t.lane) c = NormChannels<T, V, WHOLE>(p, t, column);
-    c.set(p, column, means, rstds);
-    const NormReturn<T, V, WHOLE> back(p, column, m1, m2, rstds);
+    c.set(p, column, of.means, of.rstds, of.rests);
+    const NormReturn<T, V, WHOLE> back(p, column, m1, m2, of);
     const long long last = first + (t.count - 1) * step + (long long)column * V;
     const T *x = (const T*)p.x + last, *dy = (const T*)p.dy + last;
     T* dx = (T*)p.dx + last + step;
@@ -727,12 +748,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_cluster_backward(const _
   const int image = blockIdx.x / p.chunks, n = image / p.blocks;
   const NormPlace t = norm_place(p, n, image - n * p.blocks, blockIdx.x - image * p.chunks);
   grid_dependency();
-  const float *means = p.mean + (long long)t.n * p.groups + t.group, *rstds = p.rstd + (long long)t.n * p.groups + t.group;
+  const NormStatistics of(p, t);
   const long long step = (long long)p.depth * p.C, first = (t.n * p.S + t.row) * p.C + (long long)t.group * p.width + t.lane * V;
   Vector* rows = (Vector*)sh.rows + (t.depth * p.lanes + t.lane) * 2;  // of this thread: x and dy
   const int next = p.depth * p.lanes * 2;
   NormChannels<T, V, WHOLE> c(p, t, t.lane);
-  c.set(p, t.lane, means, rstds);
+  c.set(p, t.lane, of.means, of.rstds, of.rests);
   NormSlopes<T, V> s;
   if (t.count > 0) {
     const T *x = (const T*)p.x + first, *dy = (const T*)p.dy + first;
@@ -743,7 +764,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_cluster_backward(const _
     });
   }
   float2* told = (float2*)sh.told;
-  channel_sums<T, V>(p, t, s, told, p.columns, 0, rstds, [&](int, float2) {});
+  channel_sums<T, V>(p, t, s, told, p.columns, 0, of, [&](int, float2) {});
   if (p.chunks > 1) cluster_sync();
   const float all = (float)p.S * p.width;
   const NormTeam team(p.block_groups, p.width);
@@ -764,7 +785,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_cluster_backward(const _
   });
   __syncthreads();
   if (t.count > 0) {
-    const NormReturn<T, V, WHOLE> back(p, t.lane, sh.first, sh.second, rstds);
+    const NormReturn<T, V, WHOLE> back(p, t.lane, sh.first, sh.second, of);
     T* dx = (T*)p.dx + first;
     walk<2>(t.count, [&](int i) { return Both<Vector>{rows[i * next], rows[i * next + 1]}; },
             [&](int i, const Both<Vector>& v) { *(Vector*)(dx + i * step) = back.template gradient<ACT>(v.x, v.dy, c); });

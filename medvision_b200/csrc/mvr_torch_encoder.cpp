@@ -55,6 +55,7 @@ struct GroupNormBackward : public torch::autograd::Node {
       a.grad_x = data_or_null(gx);
       a.mean = (float*)data_or_null(st);
       a.rstd = a.mean ? a.mean + a.N * a.groups : nullptr;
+      a.mean_rest = a.mean ? a.rstd + a.N * a.groups : nullptr;
       result[0] = gx;
       if (w0.defined() && task_should_compute_output(1)) {
         result[1] = at::empty(w0.sizes(), w0.options().requires_grad(false));
@@ -105,10 +106,11 @@ at::Tensor group_norm(const at::Tensor& x, const at::Tensor& weight, const at::T
     const at::Tensor xc = x.contiguous(), w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
     mvr_group_norm a = describe(s, xc, w, b);
     out = at::empty(xc.sizes(), xc.options().requires_grad(false));
-    statistics = at::empty({2, a.N, s.groups}, out.options().dtype(at::kFloat));
+    statistics = at::empty({3, a.N, s.groups}, out.options().dtype(at::kFloat));
     a.out = data_or_null(out);
     a.mean = (float*)data_or_null(statistics);
     a.rstd = a.mean ? a.mean + a.N * s.groups : nullptr;
+    a.mean_rest = a.mean ? a.rstd + a.N * s.groups : nullptr;
     const at::Tensor ws = norm_workspace(a, false, out);
     check(mvr_group_norm_forward(&a, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, stream_of(out)));
   }
