@@ -4,8 +4,9 @@
 // gradient is the same turn backwards.
 //
 // Angles.  A far position times a frequency has more turns than 24 bits leave room for, so the product is formed in whole numbers:
-// frequencies come as 64-bit fractions of a turn, their product with a position wraps at whole turns by itself, and its upper 32 bits are
-// the angle, off by 2^-33 of a turn for positions up to 2^31.  A floating position is a number of 24 bits, whose product is shifted.  (In
+// frequencies come as 64-bit fractions of a turn, their product with a position wraps at whole turns by itself, and its upper 32 bits,
+// rounded, are the angle: off by 2^-33 of a turn, and by the frequency's own error, up to 2^-64 (of pair i of slow bases about i 2^-66) times the
+// position, which is 2^-33 at 2^31.  A floating position is a number of 24 bits, whose product is shifted.  (In
 // 64-bit floating arithmetic the conversions and products took longer than memory: 80 000 tokens of 128 columns 37 us.)  Half types: sine
 // and cosine by the function units (2^-21); float: the library's, and what the angle's rounding to a float left by their derivatives.
 //
@@ -61,15 +62,15 @@ __device__ __forceinline__ Place place_at(const RotaryParams& p, long long at) {
   }
   return v;
 }
-// The angle in 2^-32 turns.
+// The angle in 2^-32 turns, rounded.
 __device__ __forceinline__ int angle_of(const Place& v, unsigned long long turns) {
-  const unsigned long long low = v.number * turns;
-  if (!v.floating) return (int)(low >> 32);
+  const unsigned long long low = v.number * turns, half = 1ull << 31;
+  if (!v.floating) return (int)((low + half) >> 32);
   const unsigned long long high = __umul64hi(v.number, turns);
   const int s = v.shift;
   unsigned long long a = s >= 0 ? (s < 64 ? low << s : 0) : s > -64 ? (low >> -s) | (high << (64 + s)) : s > -128 ? high >> (-64 - s) : 0;
   if (v.negative) a = 0 - a;
-  return (int)(a >> 32);
+  return (int)((a + half) >> 32);
 }
 template <typename T>
 __device__ __forceinline__ void turn_of(int angle, float& c, float& s) {
