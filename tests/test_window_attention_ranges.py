@@ -84,3 +84,16 @@ def test_float16_ranges_go_by_what_is_read(loud, heads, dim):
         x[~read.any(1)], y[~read.any(2)] = in_v, in_g
         for a, b in zip(run(q, k, x, y, *window, **kw), clean):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape,window", [((1, 1500, 8, 1, 64, 1500), (400, 0, 5)), ((2, 900, 8, 1, 128, 900), (300, 10, 130)), ((1, 700, 6, 1, 64, 700), (200, 200, 130)),
+                                          ((2, 500, 8, 1, 96, 500), (300, 0, 40)), ((1, 600, 4, 1, 200, 600), (250, 0, 40))])
+def test_rows_and_first_states_in_parts_together(shape, window, dtype):
+    """Few sequences and key heads: the rows of the first states' tiles and those of the others are both cut into parts, on the tensor cores and in
+    float arithmetic, and the states of the queries' gradients too."""
+    N, T, L = shape[0], shape[1], shape[5]
+    compare(shape, window, dtype, seed=24)
+    if N > 1:
+        compare(shape, window, dtype, offsets=[-T // 3, 40], lengths=[L, L // 2 + 3], seed=25)
