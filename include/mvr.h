@@ -404,6 +404,8 @@ typedef struct mvr_window {
   int offsets_64;               /* offsets are int64 (else int32) */
   void* rest;                   /* half types: (R, T, Hq, D) bfloat16 or null; what the rounding of out left, written by the
                                    forward and read by the backward, whose gradients are formed with out alone without it */
+  int rounded_weights;          /* half types: not 0: weights are rounded to the type before they meet values (forward) or grad_out
+                                   (grad_v); 0: they keep 16 bits or more */
 } mvr_window;
 int mvr_window_attention_workspace(const mvr_attention* a, const mvr_window* w, int backward, int64_t* bytes);
 int mvr_window_attention_forward(const mvr_attention* a, const mvr_window* w, void* workspace, int64_t bytes, int* status, void* stream);

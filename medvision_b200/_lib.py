@@ -31,7 +31,8 @@ class Attention(ctypes.Structure):
 
 class Window(ctypes.Structure):
     """struct mvr_window of include/mvr.h."""
-    _fields_ = [("before", _i64), ("after", _i64), ("sinks", _i64), ("offset", _i64), ("offsets", _vp), ("offsets_64", _i32), ("rest", _vp)]
+    _fields_ = [("before", _i64), ("after", _i64), ("sinks", _i64), ("offset", _i64), ("offsets", _vp), ("offsets_64", _i32), ("rest", _vp),
+                ("rounded_weights", _i32)]
 
 
 class GroupNorm(ctypes.Structure):

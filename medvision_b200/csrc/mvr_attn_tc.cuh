@@ -22,6 +22,11 @@
 // 2100 to 2500 cycles of a CTA, and tensor memory holds no more CTAs.  Of eight pairs of exponentials two as polynomials were best
 // (none: 3 % slower, four: 6 %).
 //
+// A window's weights are not rounded to T alone: what the rounding left is a second piece, of T as well, for which P V is formed again (a relative
+// error of 2^-16 in bfloat16, 2^-22 in float16, and of the polynomials 2.65e-6).  With one piece a result was 1.2 to 1.4 times as far from
+// float64 as its own rounding puts it, a value's gradient 1.4 to 1.5 times; with two 1.00 (48 random training calls).  The price is a product in three: 32 caches' windows of 2052 states 61 to 70 us, 2 x 8192 tokens of windows of 1028, forward and
+// backward, 657 to 744, 2 x 32768 tokens of windows of 4112, whose tensor pipe is then full, 2419 to 3138; the caller may do without.
+//
 // States that are left out (lengths, mask) are compacted to a list of tiles, with a bit a state, before the walk; tiles without a state
 // are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its
 // own before the product reads them.
@@ -58,8 +63,9 @@ struct StateBits {
   }
 };
 
-// Which states a row reads: all of its image, those on a list (lengths, mask), or those of a sliding window.
-enum { kAll = 0, kListed = 1, kWindow = 2 };
+// Which states a row reads: all of its image, those on a list (lengths, mask), or those of a sliding window, there with weights in two pieces
+// or rounded once.
+enum { kAll = 0, kListed = 1, kWindow = 2, kWindowRounded = 3 };
 
 template <int DP, int TILES, int MODE, int PIECES>
 struct TcForward {
@@ -190,6 +196,8 @@ __global__ void __launch_bounds__(TcForward<DP, TILES, MODE, PIECES>::kThreads, 
 attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcForward<DP, TILES, MODE, PIECES> F;
   constexpr bool MASK = MODE != kAll;
+  constexpr bool kIn = MODE >= kWindow;
+  constexpr bool kRest = MODE == kWindow && PIECES == 1;  // weights in two pieces, the second beside the first
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);
   char* ring = base + TILES * F::kRowsBytes;
@@ -219,7 +227,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   RowTile o;
   const int hk = blockIdx.y, split = blockIdx.z;
   bool some;
-  if (MODE != kWindow && TILES == 1 && p.index) {
+  if (!kIn && TILES == 1 && p.index) {
     // few regions: the CTA looks for those of its image itself, which is faster than a kernel that groups them
     const int n = blockIdx.x;
     if (warp == 0) {
@@ -250,7 +258,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   Places at = {};
   int states = 0;
   Span span = {};
-  if (MODE == kWindow && some) {
+  if (kIn && some) {
     at = places_of(p, o.n);
     states = states_of(p, o.n);
     span = span_of(p, at, p.by_G.quotient(o.first), p.by_G.quotient(min(o.first + TILES * kTcRows, o.rows) - 1), states);
@@ -261,18 +269,18 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tiles = MODE == kWindow ? max(0, min(p.tiles_per, window.count - window_first))
+  const int tiles = kIn ? max(0, min(p.tiles_per, window.count - window_first))
                     : !some || begin >= end ? 0 : MODE == kListed ? c.tiles : (end - begin + F::kStep - 1) / F::kStep;
   const int used = !some ? 0 : TILES == 2 && o.first + kTcRows < o.rows ? 2 : 1;  // row tiles that have rows
   const uint32_t tmem = c.tmem;
   volatile int* lost = &c.lost;
   const auto first_of = [&](int i) {
-    return MODE == kWindow ? window.first(window_first + i) : begin + (MODE == kListed ? (int)c.list[i] : i) * F::kStep;
+    return kIn ? window.first(window_first + i) : begin + (MODE == kListed ? (int)c.list[i] : i) * F::kStep;
   };
 
   const auto clean = [&](int tile, int slot) {
     StateBits<F::kStep> bits;
-    if constexpr (MODE == kWindow) bits = bits_of_span<F::kStep>(span, first_of(tile));
+    if constexpr (kIn) bits = bits_of_span<F::kStep>(span, first_of(tile));
     else bits = c.bits[MASK ? tile : 0];
     for (int piece = 0; piece < PIECES; ++piece)
       clear_rows<F::kStep, F::kBlocks>(ring + slot * F::kSlotBytes + piece * F::kStepBytes, bits, lane);
@@ -355,12 +363,17 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             for_pairs<PIECES>([&](int a, int b, bool first) {
 #pragma unroll
               for (int i = 0; i < F::kStep / 16; ++i) {  // O_t += P_t V
-                const int at = PIECES == 1 ? t * F::kStep + (i >> 2) * 64 + (i & 3) * 8
-                                           : a == 2 ? F::kThird + i * 8 : (i >> 1) * 32 + a * 16 + (i & 1) * 8;
+                const int at = PIECES == 1 && !kRest ? t * F::kStep + (i >> 2) * 64 + (i & 3) * 8
+                                           : kRest ? t * F::kStep + (i >> 1) * 32 + (i & 1) * 8 : a == 2 ? F::kThird + i * 8 : (i >> 1) * 32 + a * 16 + (i & 1) * 8;
                 mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + at, values + ((vs * F::kSlotBytes + b * F::kStepBytes + i * 2048) >> 4), o_shape,
                        (PIECES == 1 && j > 0) || i > 0 || !first);
               }
             });
+            if constexpr (kRest) {
+#pragma unroll
+              for (int i = 0; i < F::kStep / 16; ++i)
+                mma_ts(tmem + F::kOut + t * DP, tmem + F::kScores + t * F::kStep + (i >> 1) * 32 + 16 + (i & 1) * 8, values + ((vs * F::kSlotBytes + i * 2048) >> 4), o_shape, true);
+            }
             if (j + 1 < tiles) {
               multiply(t, ks);
               mma_commit(smem_at(&c.scores[t]));
@@ -389,7 +402,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       const bool mine = j0 < o.rows;
       if (mine) w = row_of(p, o, j0, hk);
       Span own = {};  // of this row
-      if (MODE == kWindow && mine) own = span_of(p, at, w.t, w.t, states);
+      if (kIn && mine) own = span_of(p, at, w.t, w.t, states);
       if (tiles > 0) {
         const char* q = mine ? (const char*)p.q + (w.r * p.q_r + w.t * p.q_t + w.h * p.q_h) * 2 : nullptr;
         if (F::kHalves == 1)
@@ -425,7 +438,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
       } else {
       for (int j = 0; j < tiles; ++j) {
         uint32_t bits[2] = {~0u, ~0u};
-        if (MODE == kWindow) {
+        if (kIn) {
           const int at = first_of(j) + half * 64;
           if (at < own.lo || at + 64 > own.hi) {
             bits[0] = span_bits(own, at);
@@ -508,7 +521,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           tmem_load32(x, s_at + q * 32);
           tmem_wait_load();
           settle(x, q);
-          uint32_t v[16], v1[PIECES == 1 ? 1 : 16], v2[PIECES == 1 ? 1 : 16];
+          uint32_t v[16], v1[PIECES == 1 && !kRest ? 1 : 16], v2[PIECES == 1 ? 1 : 16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 a = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, minus);
@@ -516,9 +529,16 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
             sums[i & 1] = add2(sums[i & 1], e);
             if constexpr (PIECES == 1) v[i] = pack2<T>(e.x, e.y);
             else pieces_of(e, v[i], v1[i], v2[i]);
+            if constexpr (kRest) {
+              const float2 f = floats(*(const Two<T>*)&v[i]);
+              v1[i] = pack2<T>(e.x - f.x, e.y - f.y);
+            }
           }
           // (over this half's own scores; with pieces, over the 32 that have just been read)
-          if constexpr (PIECES == 1) {
+          if constexpr (kRest) {
+            tmem_store16(s_at + q * 32, v);
+            tmem_store16(s_at + q * 32 + 16, v1);
+          } else if constexpr (PIECES == 1) {
             tmem_store16(s_at + q * 16, v);
           } else {
             tmem_store16(s_at + q * 32, v);
@@ -574,7 +594,7 @@ attn_tc_fwd(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
               for (int e = 0; e < 4; ++e)
                 u[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
               *(uint4*)(to + i) = make_uint4(u[0], u[1], u[2], u[3]);
-              if (MODE == kWindow && p.rest) {
+              if (kIn && p.rest) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float2 f = floats(*(const Two<T>*)&u[e]);

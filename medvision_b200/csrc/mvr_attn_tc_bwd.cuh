@@ -94,15 +94,17 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 }
 
 // BOXES: tiles of rows are boxes of the tensors (maps.q, maps.g).
-// WINDOW: a tile of states meets the rows whose windows reach it; the first tiles, which all tokens may read, are cut into more parts.
-template <typename T, int DP, bool BOXES, int PIECES, bool WINDOW = false>
+// MODE: a window (kWindow, kWindowRounded) or not.  There a tile of states meets the rows whose windows reach it; the first tiles, which all tokens
+// may read, are cut into more parts.
+template <typename T, int DP, bool BOXES, int PIECES, int MODE = kAll>
 __global__ void __launch_bounds__(TcStates<DP, PIECES>::kThreads, TcStates<DP, PIECES>::kResident)
 attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps maps, int* status) {
   typedef TcStates<DP, PIECES> F;
   typedef std::conditional_t<PIECES == 1, T, float> Out;
   // A window's slopes in two pieces, as in dq: with states read by a few rows one rounding of each was up to 1.57 times as far off as the plain
   // form, with two 1.05.  The second product costs 6 % of a training step (2 x 8192 tokens, windows of 1024 + 4, bf16: 627 to 665 us).
-  constexpr bool kRest = WINDOW && PIECES == 1;
+  constexpr bool WINDOW = MODE >= kWindow, kRest = WINDOW && PIECES == 1;
+  constexpr bool kRestWeights = MODE == kWindow && PIECES == 1;  // P too: see the forward
   extern __shared__ char tc_smem[];
   char* base = tc_smem + ((1024 - (smem_at(tc_smem) & 1023)) & 1023);  // K, V, then Q and G of the stages
   typename F::Control& c = *(typename F::Control*)(base + 2 * PIECES * F::kTileBytes + 2 * F::kStages * F::kStageBytes);
@@ -199,7 +201,7 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
               mma_ts(tmem + to, tmem + at, steps_mn + ((right * F::kStageBytes + b * F::kStepBytes + i * 2048) >> 4), d_shape, (PIECES == 1 && add) || i > 0 || !first);
             }
           });
-          if (kRest && from == F::kSlopes) {
+          if (from == F::kSlopes ? kRest : kRestWeights) {
 #pragma unroll
             for (int i = 0; i < F::kStep / 16; ++i)
               mma_ts(tmem + to, tmem + from + (i >> 1) * 32 + 16 + (i & 1) * 8, steps_mn + ((right * F::kStageBytes + i * 2048) >> 4), d_shape, true);
@@ -437,9 +439,14 @@ attn_tc_dkv(const __grid_constant__ AttnParams p, const __grid_constant__ TcMaps
           w[e / 2 + k] = TcType<T>::code == 0 ? mul2(y, slope2) : y;
           if constexpr (PIECES == 1) u[e / 2 + k] = pack2<T>(y.x, y.y);
           else pieces_of(y, u[e / 2 + k], u1[e / 2 + k], u2[e / 2 + k]);
+          if constexpr (kRestWeights) {
+            const float2 f = floats(*(const Two<T>*)&u[e / 2 + k]);
+            u1[e / 2 + k] = pack2<T>(y.x - f.x, y.y - f.y);
+          }
         }
       }
       tmem_store16(tmem + lanes + F::kScores + col, u);  // (over this warpgroup's own scores)
+      if constexpr (kRestWeights) tmem_store16(tmem + lanes + F::kScores + col + 16, u1);
       if constexpr (PIECES == 3) {
         tmem_store16(tmem + lanes + F::kScores + col + 16, u1);
         tmem_store16(tmem + lanes + F::kThird + col / 2, u2);

@@ -517,10 +517,10 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// window_attention(query, key, value, before, after, sinks, offsets, lengths, scale)
+// window_attention(query, key, value, before, after, sinks, offsets, lengths, scale, rounded_weights)
 PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  expect(n, 9);
+  expect(n, 10);
   const at::Tensor &q = tensor_arg(a[0], "query"), &k = tensor_arg(a[1], "key"), &v = tensor_arg(a[2], "value");
   Attention s;
   s.in_window = true;
@@ -531,6 +531,9 @@ PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   else if (a[6] != Py_None) s.window.offset = whole_arg(a[6], "offsets");
   s.lengths = optional_tensor(a[7], "lengths");
   s.scale = a[8] == Py_None ? 0.0 : number_arg(a[8]);
+  const int rounded = PyObject_IsTrue(a[9]);
+  if (rounded < 0) throw python_error();
+  s.window.rounded_weights = rounded;
   at::Tensor out;
   {
     pybind11::gil_scoped_release nogil;

@@ -16,7 +16,7 @@ namespace {
 enum Way { kFloats = 0, kTensorCores = 1, kFewRows = 2 };
 
 struct WindowCut : OperandPieces {
-  bool tc;
+  bool tc, rounded;               // rounded: half types' weights, once
   int tile;                       // rows of a CTA's tile
   long long row_tiles;            // of all sequences, per key head
   int splits, tiles_per;          // parts of the states that a row tile walks (forward, dq), and the kernel's tiles of one
@@ -32,6 +32,7 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
   const WindowSizes w = sizes_of(a, given);
   WindowCut c = {};
   const bool tc = c.tc = way == kTensorCores;
+  c.rounded = given->rounded_weights != 0;
   const bool pieces = tc && a->dtype == MVR_F32, wide = a->D > 64;
   c.W = (int)(pieces ? cdiv(a->D, 8) * 8 : a->D);
   const long long G = a->Hq / a->Hk, per = a->T * G, rows = a->R * a->T * a->Hq;
@@ -206,17 +207,29 @@ int rows_forward(const AttnParams& p, const WindowCut& c, cudaStream_t st) {
                                                                                                   : rows_forward<T, 256>(p, c, st);
 }
 
+// MODE: kWindow, or kWindowRounded where the caller wants half types' weights rounded once.
+template <typename T, int DP, int TILES, int PIECES, int MODE>
+int tc_window_forward_as(const AttnParams& p, const WindowCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
+  typedef TcForward<DP, TILES, MODE, PIECES> F;
+  return launch_shared<attn_tc_fwd<T, DP, TILES, MODE, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);
+}
 template <typename T, int DP, int TILES, int PIECES>
 int tc_window_forward(const AttnParams& p, const WindowCut& c, const TcMaps& maps, int* status, cudaStream_t st) {
-  typedef TcForward<DP, TILES, kWindow, PIECES> F;
-  return launch_shared<attn_tc_fwd<T, DP, TILES, kWindow, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);
+  if constexpr (PIECES == 1)
+    if (c.rounded) return tc_window_forward_as<T, DP, TILES, PIECES, kWindowRounded>(p, c, maps, status, st);
+  return tc_window_forward_as<T, DP, TILES, PIECES, kWindow>(p, c, maps, status, st);
+}
+template <typename T, int DP, int PIECES, int MODE>
+int tc_window_states(const AttnParams& p, const WindowCut& c, const TcMaps& maps, bool boxes, int* status, cudaStream_t st) {
+  typedef TcStates<DP, PIECES> S;
+  const dim3 states(state_ctas(p, c), p.Hk);
+  return boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES, MODE>>(states, S::kThreads, S::kShared, st, p, maps, status)
+               : launch_shared<attn_tc_dkv<T, DP, false, PIECES, MODE>>(states, S::kThreads, S::kShared, st, p, maps, status);
 }
 template <typename T, int DP, int PIECES>
 int tc_window_backward(const AttnParams& p, const WindowCut& c, const TcMaps& maps, bool boxes, int* status, cudaStream_t st) {
-  typedef TcStates<DP, PIECES> S;
-  const dim3 states(state_ctas(p, c), p.Hk);
-  const int rc = boxes ? launch_shared<attn_tc_dkv<T, DP, true, PIECES, true>>(states, S::kThreads, S::kShared, st, p, maps, status)
-                       : launch_shared<attn_tc_dkv<T, DP, false, PIECES, true>>(states, S::kThreads, S::kShared, st, p, maps, status);
+  const int rc = PIECES == 1 && c.rounded ? tc_window_states<T, DP, PIECES, PIECES == 1 ? kWindowRounded : kWindow>(p, c, maps, boxes, status, st)
+                                          : tc_window_states<T, DP, PIECES, kWindow>(p, c, maps, boxes, status, st);
   if (rc != MVR_OK || p.R == 0 || p.T == 0) return rc;
   typedef TcRows<DP, kWindow, PIECES> F;
   return launch_shared<attn_tc_dq<T, DP, kWindow, PIECES>>(dim3((unsigned)c.row_tiles, p.Hk, c.splits), F::kThreads, F::kShared, st, p, maps, status);

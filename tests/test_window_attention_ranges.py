@@ -97,3 +97,59 @@ def test_rows_and_first_states_in_parts_together(shape, window, dtype):
     compare(shape, window, dtype, seed=24)
     if N > 1:
         compare(shape, window, dtype, offsets=[-T // 3, 40], lengths=[L, L // 2 + 3], seed=25)
+
+
+PRECISE = [((2, 257, 4, 2, 64, 257), (90, 0, 3)), ((1, 600, 2, 2, 128, 600), (40, 40, 0)), ((3, 1, 16, 4, 128, 700), (500, 0, 4)), ((2, 130, 3, 1, 32, 130), (2, 0, 0)),
+           ((1, 1100, 2, 2, 40, 1100), (10 ** 9, 0, 0)), ((2, 300, 8, 1, 96, 300), (33, 7, 130)), ((1, 70, 2, 2, 33, 70), (9, 0, 1))]
+
+
+def fine(q, k, v, g, window, offsets, lengths, scale, dtype):
+    """What test_window_attention.reference gives for out and dv, with bounds in which a weight is a number of two pieces: off by the square of
+    half a step, 3e-6 where its exponential is a polynomial, and in float16 2^-35 (the second piece's smallest step, weights being scaled by
+    2^10 at least)."""
+    u, few = HALF[dtype], 2.0 ** -35 if dtype == torch.float16 else 0.0
+    rest, tiny = u * u + 3e-6, 2.0 ** -25 if dtype == torch.float16 else 0.0
+    at = (offsets, lengths, scale, torch.float32)
+    res, bound = reference(q, k, v, g, *window, *at)
+    size = reference(q, k, v.abs(), g.abs(), *window, *at)[0]
+    read = torch.stack([allowed_states(q.shape[1], k.shape[1], *window, o, n).double() for o, n in zip(offsets, lengths)])
+    group = q.shape[2] // k.shape[2]
+    every = {0: torch.einsum("ntj,njhd->nthd", read, v.abs().double()).repeat_interleave(group, 2),
+             3: torch.einsum("ntj,nthd->njhd", read, g.abs().double()).unflatten(2, (-1, group)).sum(3)}
+    for i in (0, 3):
+        bound[i] += u * res[i].abs() + 2 * rest * size[i] + few * every[i] + tiny
+    return [(res[i], bound[i]) for i in (0, 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape,window", PRECISE)
+def test_weights_keep_their_bits(shape, window, dtype):
+    """Results and values' gradients are as far off as their own rounding, and the sums in float, put them: no weight is rounded to the type."""
+    N, T, H, Hk, D, L = shape
+    q, k, v, g = make(*shape, dtype, seed=26)
+    offsets = [L - T - 3 * n for n in range(N)]
+    lengths = [max(0, L - 5 * n) for n in range(N)]
+    for alike in (False, True):  # (True: all weights of a row are 1 / n)
+        if alike:
+            q = torch.zeros_like(q)
+        out, dv = fine(q, k, v, g, window, offsets, lengths, D ** -0.5, dtype)
+        got = run(q, k, v, g, *window, offsets=torch.tensor(offsets, device="cuda"), lengths=torch.tensor(lengths, device="cuda"))
+        check(got[0], *out, "out")
+        check(got[3], *dv, "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape,window", PRECISE)
+def test_rounded_weights(shape, window, dtype):
+    """The caller's choice: the bounds of attention whose weights are rounded once.  Without half types, or without tensor cores, it changes nothing."""
+    q, k, v, g = make(*shape, dtype, seed=27)
+    N, T, H, Hk, D, L = shape
+    res, bound = reference(q, k, v, g, *window, [L - T] * N, [L] * N, D ** -0.5, dtype)
+    got = run(q, k, v, g, *window, offsets=L - T, rounded_weights=True)
+    for name, a, b, c in zip(NAMES, got, res, bound):
+        check(a, b, c, name)
+    if dtype == torch.float32:
+        for a, b in zip(got, run(q, k, v, g, *window, offsets=L - T)):
+            assert torch.equal(a, b)
