@@ -22,10 +22,12 @@
 // 2100 to 2500 cycles of a CTA, and tensor memory holds no more CTAs.  Of eight pairs of exponentials two as polynomials were best
 // (none: 3 % slower, four: 6 %).
 //
-// A window's weights are not rounded to T alone: what the rounding left is a second piece, of T as well, for which P V is formed again (a relative
-// error of 2^-16 in bfloat16, 2^-22 in float16, and of the polynomials 2.65e-6).  With one piece a result was 1.2 to 1.4 times as far from
-// float64 as its own rounding puts it, a value's gradient 1.4 to 1.5 times; with two 1.00 (48 random training calls).  The price is a product in three: 32 caches' windows of 2052 states 61 to 70 us, 2 x 8192 tokens of windows of 1028, forward and
-// backward, 657 to 744, 2 x 32768 tokens of windows of 4112, whose tensor pipe is then full, 2419 to 3138; the caller may do without.
+// A window's weights are not rounded to T alone: what the rounding left is a second piece, of T as well, for which P V is formed again (a
+// relative error of 2^-16 in bfloat16, 2^-22 in float16, and of the polynomials 2.65e-6).  With one piece a result was 1.2 to 1.4 times as
+// far from float64 as its own rounding puts it, a value's gradient 1.4 to 1.5 times; with two 1.00 (48 random training calls).  The
+// price is a product in three: 32 caches' windows of 2052 states 70 us instead of 61, 2 x 8192 tokens of windows of 1028, forward and
+// backward, 744 instead of 657, 2 x 32768 tokens of windows of 4112, whose tensor pipe is then full, 3138 instead of 2419.  The caller
+// may do without.
 //
 // States that are left out (lengths, mask) are compacted to a list of tiles, with a bit a state, before the walk; tiles without a state
 // are not read.  Their scores are replaced, and their rows of V, which may hold NaN, are zeroed in shared memory by a warp of its

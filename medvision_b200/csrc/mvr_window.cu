@@ -46,7 +46,8 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
                         rows * a->D * 8 / 4e6, false);
   c.tiles_per = (int)cdiv(w.span_tiles(c.tile, step), c.splits);
   if (way == kFewRows) {
-    // four CTAs an SM (eight: up to 15 % slower), with 128 states each at least (64: 9.4 us instead of 6.8 for 8 caches' windows of 500)
+    // 592 CTAs, four an SM (eight: up to 15 % slower), with 128 states each at least (64: 9.4 us instead of 6.8 for 8 caches' windows of 500).
+    // Their rings let an SM hold three at a time in half types and one in float, so that they run in two waves and in four.
     const long long states = w.reach(a->T) + w.sinks, ctas = std::max<long long>(1, a->N * a->Hk);
     c.splits = (int)std::max<long long>(1, std::min<long long>({64, cdiv(4 * kMultiprocessors, ctas), cdiv(states, 128)}));
   }
@@ -94,7 +95,7 @@ WindowCut cut_window(const mvr_attention* a, const mvr_window* given, bool backw
 }
 
 // Whether a forward is of few rows: those of a key head are the lanes' registers, and rows are read in vectors.  Half types up to two rows (32
-// caches, windows of 2051 states, 8 key heads of 128: one row 55 us, two 57, four 73; tensor cores 61), float up to eight (16 caches of
+// caches, windows of 2051 states, 8 key heads of 128: one row 55 us, two 57, four 73; tensor cores 70), float up to eight (16 caches of
 // 2000 states, 8 heads of 64: 57 us, in float arithmetic by tiles 209).
 bool few_rows(const mvr_attention* a) {
   return a->T * (a->Hq / a->Hk) <= (a->dtype == MVR_F32 ? 8 : 2) && a->D % 8 == 0 && a->N <= INT32_MAX / 64 && a->Hk <= 65535;
